@@ -1,0 +1,211 @@
+// Group norm of rows with a gate (sm_100a): each of `groups` consecutive parts of a row is divided by its root mean
+// square or, centred, freed of its mean first, times a weight, plus a bias.  The gate's activation
+// multiplies the row in front of the norm or the result behind it; without a gate the activation may be
+// that of the result.
+//
+// A part of a row is a problem of its own: rows * groups of them.  A team of threads (one warp up to 1024
+// elements, a CTA above) holds its part in registers, NI vectors of V elements per thread, so that mean and
+// variance are two passes over registers and memory is read once; wider parts are read again.  Bytes bound it.
+#include "common.cuh"
+
+namespace b200 {
+namespace gated_norm {
+
+enum Act : int { kNone = 0, kSilu = 1, kSigmoid = 2 };
+
+struct Args {
+  const void *x, *z;         // [T, C]; z may be null
+  void* out;                 // [T, C]
+  const float *w, *bias;     // [C]; bias may be null
+  long long ldx, ldz, ldo;
+  float eps;
+  int T, C, groups, width;   // width: C / groups
+  int act, center, after;
+};
+
+// fp32 forms for 16-bit rows: the fast exponential and division, relative errors near 1e-6
+template <typename T>
+__device__ __forceinline__ float activate(float v, int act) {
+  if (act == kNone) return v;
+  float s;
+  if constexpr (sizeof(T) == 2) s = __fdividef(1.0f, 1.0f + __expf(-v));
+  else s = 1.0f / (1.0f + expf(-v));
+  return act == kSilu ? v * s : s;
+}
+
+template <typename T, int V>
+struct Raw {
+  T e[V];
+};
+template <>
+struct __align__(16) Raw<__nv_bfloat16, 8> {
+  __nv_bfloat16 e[8];
+};
+template <>
+struct __align__(16) Raw<__half, 8> {
+  __half e[8];
+};
+template <>
+struct __align__(16) Raw<float, 4> {
+  float e[4];
+};
+
+// Sum over the team of a thread: a warp or the whole CTA.
+template <int TEAM>
+__device__ __forceinline__ float team_sum(float v, float* red) {
+  if constexpr (TEAM == 32) return warp_sum(v);
+  else return block_sum(v, red);
+}
+
+template <typename T, int V, int NI, int TEAM>
+__global__ void __launch_bounds__(TEAM == 32 ? 128 : TEAM) group_norm_gate_kernel(const Args a) {
+  __shared__ float red[32];
+  using R = Raw<T, V>;
+  grid_release_small();
+  grid_wait();
+  const int lane = TEAM == 32 ? threadIdx.x & 31 : threadIdx.x;
+  const long long part = TEAM == 32 ? static_cast<long long>(blockIdx.x) * 4 + (threadIdx.x >> 5) : blockIdx.x;
+  if (part >= static_cast<long long>(a.T) * a.groups) return;     // (a whole team)
+  const long long t = part / a.groups;
+  const int c0 = static_cast<int>(part % a.groups) * a.width;
+  const T* x = static_cast<const T*>(a.x) + t * a.ldx + c0;
+  const T* z = a.z != nullptr ? static_cast<const T*>(a.z) + t * a.ldz + c0 : nullptr;
+  T* out = static_cast<T*>(a.out) + t * a.ldo + c0;
+  const float* w = a.w + c0;
+  const float* bias = a.bias != nullptr ? a.bias + c0 : nullptr;
+  const bool before = z != nullptr && !a.after, after = z != nullptr && a.after;
+  const float n = static_cast<float>(a.width);
+
+  R rx[NI], rz[NI];
+  float f[NI][V];
+#pragma unroll
+  for (int i = 0; i < NI; ++i) {
+    const int c = (i * TEAM + lane) * V;
+    if (c < a.width) rx[i] = *reinterpret_cast<const R*>(x + c);
+    if (c < a.width && z != nullptr) rz[i] = *reinterpret_cast<const R*>(z + c);
+  }
+  float sum = 0.0f;
+#pragma unroll
+  for (int i = 0; i < NI; ++i) {
+    const bool in = (i * TEAM + lane) * V < a.width;
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      f[i][v] = 0.0f;
+      if (in) {
+        f[i][v] = to_f32<T>(rx[i].e[v]);
+        if (before) f[i][v] *= activate<T>(to_f32<T>(rz[i].e[v]), a.act);
+      }
+      sum += f[i][v];
+    }
+  }
+  const float mean = a.center ? team_sum<TEAM>(sum, red) / n : 0.0f;
+  float ss = 0.0f;
+#pragma unroll
+  for (int i = 0; i < NI; ++i) {
+    const bool in = (i * TEAM + lane) * V < a.width;
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      f[i][v] -= mean;
+      if (in) ss = fmaf(f[i][v], f[i][v], ss);
+    }
+  }
+  const float inv = 1.0f / sqrtf(team_sum<TEAM>(ss, red) / n + a.eps);
+#pragma unroll
+  for (int i = 0; i < NI; ++i) {
+    const int c = (i * TEAM + lane) * V;
+    if (c >= a.width) continue;
+    R y;
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      float q = f[i][v] * inv * w[c + v];
+      if (bias != nullptr) q += bias[c + v];
+      if (after) q *= activate<T>(to_f32<T>(rz[i].e[v]), a.act);
+      else if (z == nullptr) q = activate<T>(q, a.act);
+      y.e[v] = from_f32<T>(q);
+    }
+    *reinterpret_cast<R*>(out + c) = y;
+  }
+}
+
+// Parts that do not fit a CTA's registers: read once for the mean, once for the variance, once for the result.
+template <typename T>
+__global__ void __launch_bounds__(1024) group_norm_gate_wide_kernel(const Args a) {
+  __shared__ float red[32];
+  grid_release_small();
+  grid_wait();
+  const long long part = blockIdx.x;
+  const long long t = part / a.groups;
+  const int c0 = static_cast<int>(part % a.groups) * a.width;
+  const T* x = static_cast<const T*>(a.x) + t * a.ldx + c0;
+  const T* z = a.z != nullptr ? static_cast<const T*>(a.z) + t * a.ldz + c0 : nullptr;
+  T* out = static_cast<T*>(a.out) + t * a.ldo + c0;
+  const float n = static_cast<float>(a.width);
+  auto value = [&](int c) {
+    float f = to_f32<T>(x[c]);
+    if (z != nullptr && !a.after) f *= activate<T>(to_f32<T>(z[c]), a.act);
+    return f;
+  };
+  float mean = 0.0f;
+  if (a.center) {
+    float sum = 0.0f;
+    for (int c = threadIdx.x; c < a.width; c += blockDim.x) sum += value(c);
+    mean = block_sum(sum, red) / n;
+  }
+  float ss = 0.0f;
+  for (int c = threadIdx.x; c < a.width; c += blockDim.x) {
+    const float f = value(c) - mean;
+    ss = fmaf(f, f, ss);
+  }
+  const float inv = 1.0f / sqrtf(block_sum(ss, red) / n + a.eps);
+  for (int c = threadIdx.x; c < a.width; c += blockDim.x) {
+    float q = (value(c) - mean) * inv * a.w[c0 + c];
+    if (a.bias != nullptr) q += a.bias[c0 + c];
+    if (z != nullptr && a.after) q *= activate<T>(to_f32<T>(z[c]), a.act);
+    else if (z == nullptr) q = activate<T>(q, a.act);
+    out[c] = from_f32<T>(q);
+  }
+}
+
+template <typename T, int V>
+int launch(const Args& a, cudaStream_t s) {
+  const long long parts = static_cast<long long>(a.T) * a.groups;
+  const int vecs = (a.width + V - 1) / V;
+  if (parts > 0x7fffffffll) return -8;
+#define WARP(NI) launch_overlapped(group_norm_gate_kernel<T, V, NI, 32>, dim3((parts + 3) / 4), dim3(128), 0, s, a)
+#define CTA(NI, TEAM) launch_overlapped(group_norm_gate_kernel<T, V, NI, TEAM>, dim3(parts), dim3(TEAM), 0, s, a)
+  if (vecs <= 32) return WARP(1);
+  if (vecs <= 64) return WARP(2);
+  if (vecs <= 128) return WARP(4);
+  if (vecs <= 256) return CTA(2, 128);
+  if (vecs <= 512) return CTA(2, 256);
+  if (vecs <= 1024) return CTA(4, 256);
+  if (vecs <= 2048) return CTA(4, 512);
+  return launch_overlapped(group_norm_gate_wide_kernel<T>, dim3(parts), dim3(1024), 0, s, a);
+#undef WARP
+#undef CTA
+}
+template <typename T>
+int launch_any(const Args& a, bool wide, cudaStream_t s) {
+  return wide ? launch<T, 16 / sizeof(T)>(a, s) : launch<T, 1>(a, s);
+}
+
+}  // namespace gated_norm
+}  // namespace b200
+
+// dtype: 0 bf16, 1 fp16, 2 fp32 rows; act: 0 none, 1 SiLU, 2 sigmoid; wide: parts of rows may be read 16 bytes
+// at a time.
+B200_API int b200_group_norm_gate(const void* x, long long ldx, const void* z, long long ldz, const float* w,
+                                  const float* bias, void* out, long long ldo, float eps, int T, int C, int groups,
+                                  int act, int center, int after, int wide, int dtype, void* stream) {
+  using namespace b200::gated_norm;
+  if (T <= 0 || C <= 0) return 0;
+  if (groups <= 0 || C % groups != 0) return -8;
+  Args a{x, z, out, w, bias, ldx, ldz, ldo, eps, T, C, groups, C / groups, act, center, after};
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  switch (dtype) {
+    case 0: return launch_any<__nv_bfloat16>(a, wide, s);
+    case 1: return launch_any<__half>(a, wide, s);
+    case 2: return launch_any<float>(a, wide, s);
+  }
+  return -8;
+}

@@ -1570,6 +1570,235 @@ def memory_step(h: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Tens
     return out
 
 
+# ---------------------------------------------------------------------------
+# state-space mixers (csrc/selective.cu, csrc/group_norm_gate.cu)
+# ---------------------------------------------------------------------------
+def _rows_of(name: str, t: torch.Tensor, rows: int, cols: int, dtypes, device) -> torch.Tensor:
+    """A row-strided view [rows, cols] of one of ``dtypes``, as the state-space kernels take it."""
+    if t.dim() != 2 or tuple(t.shape) != (rows, cols):
+        raise ValueError(f"{name} has shape {tuple(t.shape)}, not {(rows, cols)}")
+    if t.dtype not in dtypes:
+        raise ValueError(f"{name} is {t.dtype}, not {' or '.join(map(str, dtypes))}")
+    if t.device != device:
+        raise ValueError(f"{name} is on {t.device}, not on {device}")
+    if cols > 1 and t.stride(1) != 1:
+        raise ValueError(f"{name}: neighbouring columns are {t.stride(1)} elements apart")
+    return t
+
+
+def _target(t: torch.Tensor, rows: int, cols: int, dtype, device) -> torch.Tensor:
+    """Rows that a kernel writes: as :func:`_rows_of`, and no two of them share elements."""
+    _rows_of("out", t, rows, cols, (dtype,), device)
+    if rows > 1 and t.stride(0) < cols:
+        raise ValueError(f"out: rows of {cols} columns are {t.stride(0)} elements apart")
+    return t
+
+
+def _whole(name: str, t: Optional[torch.Tensor], shape, dtype, device) -> Optional[torch.Tensor]:
+    """A contiguous tensor of a known shape, or None."""
+    if t is None:
+        return None
+    if tuple(t.shape) != tuple(shape) or t.dtype != dtype or not t.is_contiguous() or t.device != device:
+        raise ValueError(f"{name}: a contiguous {dtype} tensor of shape {tuple(shape)} on {device} is wanted, got "
+                         f"{t.dtype}, {tuple(t.shape)}, strides {tuple(t.stride())} on {t.device}")
+    return t
+
+
+def _overlap(a: torch.Tensor, b: Optional[torch.Tensor]) -> bool:
+    """Whether two row-strided views share elements.  Views of equal pitch are told apart by their columns."""
+    if b is None or not a.numel() or not b.numel():
+        return False
+    reach = lambda t: t.data_ptr() + t.element_size() * (  # noqa: E731
+        1 + sum((n - 1) * st for n, st in zip(t.shape, t.stride())))
+    if a.data_ptr() >= reach(b) or b.data_ptr() >= reach(a):
+        return False
+    if a.dim() == b.dim() == 2 and a.element_size() == b.element_size() and a.stride(0) == b.stride(0):
+        off, ld = (b.data_ptr() - a.data_ptr()) // a.element_size(), a.stride(0)
+        if ld >= a.shape[1] and ld >= b.shape[1]:
+            return off % ld < a.shape[1] or off % ld + b.shape[1] > ld
+    return True
+
+
+def _step_place(md, T: int, slots_wanted: bool, num_slots: int, write_slots, device):
+    """(single tokens, portions, cu_q, positions, read slots, write slots) of a step, checked."""
+    nd, npf, cu = _scan_place(md)
+    if not 0 <= nd <= T:
+        raise ValueError(f"{nd} single tokens in a step of {T} rows")
+    if cu is not None:
+        _whole("md.cu_q_prefill", cu, (npf + 1,), torch.int32, device)
+    if not slots_wanted:
+        return nd, npf, cu, None, None, None
+    pos, slots = md.positions, md.state_slots
+    if slots is None:
+        raise ValueError("a state needs md.state_slots")
+    if pos.dim() != 1 or pos.shape[0] < T or pos.dtype != torch.int64 or pos.device != device \
+            or not pos.is_contiguous():
+        raise ValueError(f"md.positions: {T} int64 positions on {device} are wanted")
+    write_slots = slots if write_slots is None else write_slots
+    for name, t in (("md.state_slots", slots), ("write_slots", write_slots)):
+        if t.dim() != 1 or t.shape[0] < nd + npf or t.dtype != torch.int32 or t.device != device \
+                or not t.is_contiguous():
+            raise ValueError(f"{name}: {nd + npf} int32 slots on {device} are wanted")
+    return nd, npf, cu, pos, slots, write_slots
+
+
+def _on_device(t: torch.Tensor):
+    """Makes the tensor's device the current one for a launch."""
+    if not t.is_cuda:
+        raise ValueError(f"a tensor on a GPU is wanted, not on {t.device}")
+    return torch.cuda.device(t.device)
+
+
+def _wide_rows(*ts: Optional[torch.Tensor]) -> bool:
+    """Whether every row of the views starts on a 16-byte boundary."""
+    return all(t is None or (t.data_ptr() % 16 == 0 and (t.shape[0] <= 1 or t.stride(0) * t.element_size() % 16 == 0))
+               for t in ts)
+
+
+def causal_conv(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor], md,
+                ring: Optional[torch.Tensor], out: Optional[torch.Tensor] = None, act: Optional[str] = "silu",
+                write_slots: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``act(bias + sum_j weight[j] * (x of taps - 1 - j tokens ago))`` per channel over the portions of a
+    step: ``x [T, C]`` (bf16, fp16 or fp32; row-strided views are fine), ``weight [taps, C]`` (up to 8 taps)
+    and ``bias [C]`` fp32, ``act`` "silu" or None.  ``ring [slots, taps - 1, C]`` of x's type holds a request's
+    last rows by position (position p in row ``p % (taps - 1)``), read in slot ``md.state_slots`` and left in
+    ``write_slots`` (default: the same; another one forks a request, and must not be a slot that another request
+    of the step reads); None: zeros in front of the portions.  ``md`` also gives ``positions``,
+    ``num_decode_tokens`` and ``cu_q_prefill``.  A request whose slot lies outside the ring gives zeros, one whose
+    write slot does leaves its ring nowhere; rows behind the last portion are not written."""
+    if x.dim() != 2 or x.dtype not in DTYPE_CODE:
+        raise ValueError(f"x: rows of bf16, fp16 or fp32 are wanted, got {x.dtype} of shape {tuple(x.shape)}")
+    T, Ch = x.shape
+    dev = x.device
+    taps = weight.shape[0]
+    if not 1 <= taps <= 8:
+        raise ValueError(f"a convolution of {taps} taps, 1 to 8 are built")
+    if act not in ("silu", None):
+        raise ValueError(f"activation {act!r}: silu or None")
+    _rows_of("x", x, T, Ch, (x.dtype,), dev)
+    _whole("weight", weight, (taps, Ch), torch.float32, dev)
+    _whole("bias", bias, (Ch,), torch.float32, dev)
+    if ring is not None:
+        _whole("ring", ring, (ring.shape[0], taps - 1, Ch), x.dtype, dev)
+    use = ring is not None and taps > 1
+    nd, npf, cu, pos, slots, wslots = _step_place(md, T, use, ring.shape[0] if use else 0, write_slots, dev)
+    if out is None:
+        out = torch.empty((T, Ch), dtype=x.dtype, device=dev)
+    _target(out, T, Ch, x.dtype, dev)
+    if _overlap(out, x):
+        raise ValueError("out shares memory with x: rows are read by those behind them")
+    ring = ring if use else None
+    wide = Ch % (16 // x.element_size()) == 0 and _wide_rows(x, out, ring) and weight.data_ptr() % 16 == 0
+    with _on_device(x):
+        call("b200_causal_conv", ptr(x), x.stride(0), ptr(weight), taps, ptr(bias), ptr(ring),
+             ring.shape[0] if use else 0, ptr(pos), ptr(slots), ptr(wslots), ptr(cu), ptr(out), out.stride(0), T, Ch,
+             nd, npf, int(act == "silu"), int(wide), DTYPE_CODE[x.dtype], stream_ptr())
+    return out
+
+
+def selective_scan(x: torch.Tensor, dt: torch.Tensor, b: torch.Tensor, c: torch.Tensor, a_log: torch.Tensor,
+                   groups: int, md, state: Optional[torch.Tensor], d: Optional[torch.Tensor] = None,
+                   dt_bias: Optional[torch.Tensor] = None, z: Optional[torch.Tensor] = None, softplus: bool = True,
+                   dt_limits: tuple = (0.0, float("inf")), out: Optional[torch.Tensor] = None,
+                   write_slots: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Selective state space scan over the portions of a step, per column of x
+    ``h = exp(dt A) h + dt x B``, ``y = C . h + d x`` (times ``silu(z)``), ``A = -exp(a_log)`` and
+    ``dt = clamp(softplus(dt + dt_bias), *dt_limits)`` (without ``softplus``: the sum itself, clamped).
+
+    ``a_log [H]``: a rate per head; ``x [T, H * P]``, ``dt [T, H]``, ``d`` and ``dt_bias [H]``, ``state [slots, H,
+    P, N]``.  ``a_log [D, N]``: rates per channel; ``x`` and ``dt [T, D]``, ``d`` and ``dt_bias [D]``, ``state [slots,
+    D, N]``.  ``b`` and ``c [T, groups * N]``, N up to 256, shared by the heads (channels) of a group.  x, b, c, z
+    and out are bf16, fp16 or fp32 alike, dt of that type or fp32, the rest fp32; rows may be strided views.
+    State, slots, ``write_slots`` and ``md`` as in :func:`causal_conv`; ``state`` None: zeros in front of the
+    portions, nothing is kept.  Returns ``[T, H * P]`` (``[T, D]``) in x's type."""
+    if x.dim() != 2 or x.dtype not in DTYPE_CODE:
+        raise ValueError(f"x: rows of bf16, fp16 or fp32 are wanted, got {x.dtype} of shape {tuple(x.shape)}")
+    T, cols = x.shape
+    dev = x.device
+    channels = a_log.dim() == 2
+    if a_log.dim() not in (1, 2) or a_log.shape[0] < 1 or groups < 1:
+        raise ValueError(f"a_log of shape {tuple(a_log.shape)}, {groups} groups")
+    rates = a_log.shape[0]
+    if cols % rates or channels and cols != rates:
+        raise ValueError(f"{cols} columns of x for {rates} rates")
+    if b.dim() != 2 or b.shape[1] % groups or rates % groups:
+        raise ValueError(f"b of shape {tuple(b.shape)} and {rates} rates in {groups} groups")
+    N = b.shape[1] // groups
+    if not 1 <= N <= 256:
+        raise ValueError(f"a state of {N} numbers per column, 1 to 256 are built")
+    _whole("a_log", a_log, (rates, N) if channels else (rates,), torch.float32, dev)
+    lo, hi = (float(v) for v in dt_limits)
+    if not lo <= hi:
+        raise ValueError(f"dt_limits {dt_limits}")
+    own = (x.dtype,)
+    _rows_of("x", x, T, cols, own, dev)
+    _rows_of("dt", dt, T, rates, (x.dtype, torch.float32), dev)
+    for name, t in (("b", b), ("c", c)):
+        _rows_of(name, t, T, groups * N, own, dev)
+    if z is not None:
+        _rows_of("z", z, T, cols, own, dev)
+    _whole("d", d, (rates,), torch.float32, dev)
+    _whole("dt_bias", dt_bias, (rates,), torch.float32, dev)
+    heads, width = (groups, cols // groups) if channels else (rates, cols // rates)
+    use = state is not None
+    if use:
+        _whole("state", state, (state.shape[0], cols, N) if channels else (state.shape[0], rates, width, N),
+               torch.float32, dev)
+        if state.data_ptr() % 16:
+            raise ValueError("state: it does not start on a 16-byte boundary")
+    nd, npf, cu, pos, slots, wslots = _step_place(md, T, use, state.shape[0] if use else 0, write_slots, dev)
+    if out is None:
+        out = torch.empty((T, cols), dtype=x.dtype, device=dev)
+    _target(out, T, cols, x.dtype, dev)
+    for name, t in (("x", x), ("dt", dt), ("b", b), ("c", c), ("z", z)):
+        if _overlap(out, t):
+            raise ValueError(f"out shares memory with {name}")
+    with _on_device(x):
+        call("b200_selective_scan", ptr(x), x.stride(0), ptr(dt), dt.stride(0), int(dt.dtype == torch.float32),
+             ptr(b), b.stride(0), ptr(c), c.stride(0), ptr(z), z.stride(0) if z is not None else 0, ptr(a_log),
+             int(channels), ptr(d), ptr(dt_bias), int(softplus), lo, hi, ptr(state), state.shape[0] if use else 0,
+             ptr(pos), ptr(slots), ptr(wslots), ptr(cu), ptr(out), out.stride(0), T, heads, width, N, groups, nd,
+             npf, DTYPE_CODE[x.dtype], stream_ptr())
+    return out
+
+
+def group_norm_gate(x: torch.Tensor, z: Optional[torch.Tensor], weight: torch.Tensor, groups: int, eps: float,
+                    out: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None, center: bool = False,
+                    gate_after: bool = False, act: Optional[str] = "silu") -> torch.Tensor:
+    """Norm of each of ``groups`` consecutive parts of the rows of ``x [T, C]``: divided by the root mean square,
+    with ``center`` by the deviation from the part's mean, times ``weight [C]``, plus ``bias [C]`` (both fp32).
+    The gate ``act(z)`` ("silu", "sigmoid" or None: z itself) multiplies x in front of the norm or, with
+    ``gate_after``, the result.  Without z the activation is the result's.  x, z and out are bf16, fp16 or fp32
+    alike (row-strided views are fine); out may be x or z."""
+    if x.dim() != 2 or x.dtype not in DTYPE_CODE:
+        raise ValueError(f"x: rows of bf16, fp16 or fp32 are wanted, got {x.dtype} of shape {tuple(x.shape)}")
+    T, Ch = x.shape
+    dev = x.device
+    if groups < 1 or Ch % groups:
+        raise ValueError(f"{Ch} channels in {groups} groups")
+    if act not in (None, "silu", "sigmoid"):
+        raise ValueError(f"activation {act!r}: silu, sigmoid or None")
+    own = (x.dtype,)
+    _rows_of("x", x, T, Ch, own, dev)
+    if z is not None:
+        _rows_of("z", z, T, Ch, own, dev)
+    _whole("weight", weight, (Ch,), torch.float32, dev)
+    _whole("bias", bias, (Ch,), torch.float32, dev)
+    if out is None:
+        out = torch.empty((T, Ch), dtype=x.dtype, device=dev)
+    _target(out, T, Ch, x.dtype, dev)
+    for name, t in (("x", x), ("z", z)):
+        same = t is not None and t.data_ptr() == out.data_ptr() and t.stride(0) == out.stride(0)
+        if not same and _overlap(out, t):
+            raise ValueError(f"out shares memory with {name} and is not {name}")
+    wide = Ch // groups % (16 // x.element_size()) == 0 and _wide_rows(x, z, out, weight[None])
+    with _on_device(x):
+        call("b200_group_norm_gate", ptr(x), x.stride(0), ptr(z), z.stride(0) if z is not None else 0, ptr(weight),
+             ptr(bias), ptr(out), out.stride(0), float(eps), T, Ch, groups, {None: 0, "silu": 1, "sigmoid": 2}[act],
+             int(center), int(gate_after), int(wide), DTYPE_CODE[x.dtype], stream_ptr())
+    return out
+
+
 def merge_attn_states(p_out, p_lse, s_out, s_lse, want_lse: bool = True):
     T, H, Dv = p_out.shape
     out = torch.empty_like(p_out)

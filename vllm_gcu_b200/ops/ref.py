@@ -1007,6 +1007,89 @@ def head_norm_gate(o, weight, z, eps, scale, out, nq=None, low=None, act="sigmoi
     return out
 
 
+def _step_portions(T, md, num_slots, write_slots):
+    """(first, end, read slot, write slot, position of the first row) of every request of a step; slots outside
+    the state are None, and without a state both are."""
+    for r, (lo, hi) in enumerate(_portions(T, md.num_decode_tokens, md.cu_q_prefill)):
+        hi = min(hi, T)
+        if hi <= lo:
+            continue
+        if num_slots is None:
+            yield lo, hi, None, None, 0
+            continue
+        slot = int(md.state_slots[r])
+        to = int((md.state_slots if write_slots is None else write_slots)[r])
+        inside = lambda i: i if 0 <= i < num_slots else None  # noqa: E731
+        yield lo, hi, inside(slot), inside(to), int(md.positions[lo])
+
+
+def causal_conv(x, weight, bias, md, ring, out=None, act="silu", write_slots=None) -> torch.Tensor:
+    """See ``ops.cuda.causal_conv``."""
+    T, back = x.shape[0], weight.shape[0] - 1
+    out = torch.zeros_like(x, memory_format=torch.contiguous_format) if out is None else out
+    ring = ring if back else None
+    kept = None if ring is None else ring.clone()          # every request reads before any one writes
+    for lo, hi, slot, to, p0 in _step_portions(T, md, None if ring is None else ring.shape[0], write_slots):
+        if ring is not None and slot is None:
+            out[lo:hi] = 0
+            continue
+        past = [kept[slot, p % back] if ring is not None and p >= 0 else torch.zeros_like(x[0])
+                for p in range(p0 - back, p0)]
+        seq = torch.cat([torch.stack(past), x[lo:hi]]).float() if back else x[lo:hi].float()
+        y = sum(seq[j:j + hi - lo] * weight[j] for j in range(back + 1))
+        y = y if bias is None else y + bias
+        out[lo:hi] = (torch.nn.functional.silu(y) if act == "silu" else y).to(out.dtype)
+        if ring is None or to is None:
+            continue
+        for p in range(max(0, p0 + hi - lo - back), p0 + hi - lo):
+            ring[to, p % back] = x[lo + p - p0] if p >= p0 else kept[slot, p % back]
+    return out
+
+
+def selective_scan(x, dt, b, c, a_log, groups, md, state, d=None, dt_bias=None, z=None, softplus=True,
+                   dt_limits=(0.0, float("inf")), out=None, write_slots=None) -> torch.Tensor:
+    """See ``ops.cuda.selective_scan``."""
+    T, rates = x.shape[0], a_log.shape[0]
+    P, N = x.shape[1] // rates, b.shape[1] // groups
+    out = torch.zeros_like(x, memory_format=torch.contiguous_format) if out is None else out
+    step = dt.float() if dt_bias is None else dt.float() + dt_bias
+    step = (torch.nn.functional.softplus(step, threshold=1e9) if softplus else step).clamp(*dt_limits)
+    A = -torch.exp(a_log.float()).view(rates, -1)
+    xf = x.float().view(T, rates, P) if x.is_contiguous() else x.float().reshape(T, rates, P)
+    kept = None if state is None else state.clone().view(-1, rates, P, N)
+    share = lambda t: t.float().reshape(groups, 1, N).expand(groups, rates // groups, N).reshape(  # noqa: E731
+        rates, 1, N)
+    for lo, hi, slot, to, p0 in _step_portions(T, md, None if state is None else state.shape[0], write_slots):
+        if state is not None and slot is None:
+            out[lo:hi] = 0
+            continue
+        S = kept[slot] if state is not None and p0 else torch.zeros(rates, P, N, device=x.device)
+        for t in range(lo, hi):
+            S = torch.exp(step[t][:, None] * A)[:, None] * S + (step[t][:, None] * xf[t])[..., None] * share(b[t])
+            y = (S * share(c[t])).sum(-1)
+            y = (y if d is None else y + d[:, None] * xf[t]).flatten()
+            out[t] = (y if z is None else y * torch.nn.functional.silu(z[t].float())).to(out.dtype)
+        if to is not None:
+            state[to] = S.view(state.shape[1:])
+    return out
+
+
+def group_norm_gate(x, z, weight, groups, eps, out=None, bias=None, center=False, gate_after=False, act="silu"
+                    ) -> torch.Tensor:
+    """See ``ops.cuda.group_norm_gate``."""
+    f = {None: lambda t: t, "silu": torch.nn.functional.silu, "sigmoid": torch.sigmoid}[act]
+    g = None if z is None else f(z.float())
+    v = x.float() * g if z is not None and not gate_after else x.float()
+    v = v.unflatten(-1, (groups, -1))
+    v = v - v.mean(-1, keepdim=True) if center else v
+    v = (v * torch.rsqrt(v.pow(2).mean(-1, keepdim=True) + eps)).flatten(-2) * weight
+    v = v if bias is None else v + bias
+    v = f(v) if z is None else v * g if gate_after else v
+    if out is None:
+        return v.to(x.dtype)
+    return out.copy_(v)
+
+
 def input_weighted_experts(x, w13, w2, topk_w, topk_ids) -> tuple[torch.Tensor, torch.Tensor]:
     """See ``ops.cuda.input_weighted_experts`` (gate rows first in ``w13``); one output row per
     (token, slot) pair, so ``pos_of`` is the identity."""
