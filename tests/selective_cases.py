@@ -166,7 +166,8 @@ def scan_case(form, H, P, N, G, md, dtype, seed=0, slots=None, dt32=False):
     g = torch.Generator().manual_seed(seed)
     rnd = lambda *s: torch.randn(*s, generator=g)  # noqa: E731
     T, S = md.positions.shape[0], slots or 2 * len(md.lens) + 1
-    row = rnd(T, H * P + 2 * G * N + 3).to(dtype)              # x, B and C are views of one row
+    # x, B and C are views of one row; where their widths allow it, all of them lie on 16-byte boundaries
+    row = rnd(T, H * P + 2 * G * N + (8 if H * P % 8 == 0 and G * N % 8 == 0 else 3)).to(dtype)
     parts = row[:, :H * P], row[:, H * P:H * P + G * N], row[:, H * P + G * N:H * P + 2 * G * N]
     dt = rnd(T, H) if dt32 else rnd(T, H).to(dtype)
     a_log = torch.log(1 + 7 * torch.rand(H, N, generator=g)) if form == "channels" else \

@@ -16,28 +16,10 @@
 // [heads]): one step size and one decay per head and token.  Rates per channel (a_log [columns, N]): a
 // step size per column, a decay per column and number; the heads are then the groups that share B
 // and C.
-#include "common.cuh"
+#include "selective.cuh"
 
 namespace b200 {
 namespace selective {
-
-constexpr float kLog2e = 1.4426950408889634f;
-
-__device__ __forceinline__ float exp2_fast(float x) {
-  float r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-  return r;
-}
-// SiLU and softplus: with 16-bit rows through the fast exponential, division and logarithm (relative errors
-// near 1e-6; the logarithm of 1 + e switches to its series where e would be rounded away)
-template <typename T>
-__device__ __forceinline__ float silu(float x) {
-  if constexpr (sizeof(T) == 2) return __fdividef(x, 1.0f + __expf(-x));
-  else return x / (1.0f + expf(-x));
-}
-__device__ __forceinline__ float softplus(float z) {
-  return fmaxf(z, 0.0f) + log1pf(expf(-fabsf(z)));
-}
 
 // V neighbouring elements: 16 bytes where V > 1
 template <typename T, int V>
@@ -58,15 +40,6 @@ struct __align__(16) Raw<float, 4> {
 };
 template <typename T>
 constexpr int kWide = 16 / sizeof(T);
-
-// Rows of the step that belong to a request.
-struct Portion {
-  int first, end;
-};
-__device__ __forceinline__ Portion portion_of(int r, int nd, const int* cu_q, int T) {
-  if (r < nd) return {r, r + 1};
-  return {nd + cu_q[r - nd], min(nd + cu_q[r - nd + 1], T)};
-}
 
 // ---------------------------------------------------------------------------
 // short causal convolution
@@ -203,33 +176,6 @@ __global__ void __launch_bounds__(128) causal_conv_kernel(const ConvArgs a) {
 // ---------------------------------------------------------------------------
 // selective scan
 // ---------------------------------------------------------------------------
-struct ScanArgs {
-  const void* x;             // [T, heads * width]
-  const void* dt;            // [T, heads] or [T, heads * width], the rows' type or fp32
-  const void *b, *c;         // [T, groups * N]
-  const void* z;             // [T, heads * width] or null
-  void* out;                 // [T, heads * width]
-  const float* a_log;        // [heads] or [heads * width, N]
-  const float* d;            // like the step sizes' row, or null
-  const float* dt_bias;      // likewise
-  float* state;              // [slots, heads * width, N] or null
-  const long long* positions;
-  const int *slots, *wslots;
-  const int* cu_q;
-  long long ldx, lddt, ldb, ldc, ldz, ldo;
-  float dt_min, dt_max;
-  int T, heads, width, N, groups, num_slots, nd, np, dt_f32, softplus;
-};
-
-template <typename T>
-__device__ __forceinline__ float step_size(const ScanArgs& a, long long row, int i) {
-  const long long at = row * a.lddt + i;
-  float z = a.dt_f32 ? static_cast<const float*>(a.dt)[at] : to_f32<T>(static_cast<const T*>(a.dt)[at]);
-  if (a.dt_bias != nullptr) z += a.dt_bias[i];
-  if (a.softplus) z = softplus(z);
-  return fminf(fmaxf(z, a.dt_min), a.dt_max);
-}
-
 // One token per request.  A row of N numbers of state is spread over LPR lanes, four numbers (one
 // where V is 1) at a time; a warp takes kRows rows per lane group at once, so that their loads are under
 // way together.  The state's bytes bound it: read once, written once.
@@ -501,7 +447,10 @@ int scan_any(const ScanArgs& a, cudaStream_t s) {
     const int rc = launch_step<T, CH>(a, s);
     if (rc != 0) return rc;
   }
-  return a.np > 0 ? launch_scan<T, CH>(a, s) : 0;
+  if (a.np == 0) return 0;
+  if constexpr (!CH && std::is_same<T, __nv_bfloat16>::value)
+    if (heads_by_tiles(a)) return launch_heads_by_tiles(a, s);
+  return launch_scan<T, CH>(a, s);
 }
 
 }  // namespace selective
@@ -536,7 +485,7 @@ B200_API int b200_selective_scan(const void* x, long long ldx, const void* dt, l
                                  const float* dt_bias, int softplus, float dt_min, float dt_max, float* state,
                                  int num_slots, const long long* positions, const int* slots, const int* wslots,
                                  const int* cu_q, void* out, long long ldo, int T, int heads, int width, int N,
-                                 int groups, int nd, int np, int dtype, void* stream) {
+                                 int groups, int nd, int np, int wide, int dtype, void* stream) {
   using namespace b200::selective;
   if (T <= 0 || heads <= 0 || width <= 0 || nd + np <= 0) return 0;
   if (N < 1 || N > 256) return -8;
@@ -546,6 +495,7 @@ B200_API int b200_selective_scan(const void* x, long long ldx, const void* dt, l
   a.ldx = ldx; a.lddt = lddt; a.ldb = ldb; a.ldc = ldc; a.ldz = ldz; a.ldo = ldo;
   a.dt_min = dt_min; a.dt_max = dt_max; a.T = T; a.heads = heads; a.width = width; a.N = N; a.groups = groups;
   a.num_slots = num_slots; a.nd = nd; a.np = np; a.dt_f32 = dt_f32; a.softplus = softplus;
+  a.wide = wide;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   switch (dtype) {
     case 0: return per_channel ? scan_any<__nv_bfloat16, true>(a, s) : scan_any<__nv_bfloat16, false>(a, s);

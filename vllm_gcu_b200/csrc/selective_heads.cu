@@ -1,0 +1,505 @@
+// Selective scan of prompts with rates per head, by products of tiles (sm_100a, tcgen05).
+//
+// A chunk of 128 tokens of a head, with L_i the sum of dt A (base 2) up to and with token i and H the state in
+// front of it, is
+//   y_i  = sum_{j <= i} 2^(L_i - L_j) dt_j (C_i . B_j) x_j  +  2^(L_i) C_i . H
+//   H'   = 2^(L_end) H + sum_j 2^(L_end - L_j) dt_j x_j B_j
+// Four products per chunk, operands bf16, sums fp32 in tensor memory:
+//   G  [i x j]      = C B^T                            both tiles as they are in memory
+//   Y2 [i x (p, 2)] = C (H_hi | H_lo)                  the state in two parts of bf16
+//   S  [n x (p, 3)] = B^T (W_hi | W_mid | W_lo)        W_j = 2^(L_end - L_j) dt_j x_j in three parts: all 24 bits,
+//                                                      since the state is kept in 32
+//   Y1 [i x p]      = (M_hi + M_lo) X                  M_ij = G_ij 2^(L_i - L_j) dt_j in place of G, two parts
+// H lives in registers (lane n, 32 columns p per warp) and goes on as fp32.  Two parts leave 2^-17 of a
+// factor, an eighth of what the rows' own rounding to bf16 is off.
+//
+// Decays: a difference L_i - L_j is taken of 64-bit sums or, in the 32 x 32 blocks on the diagonal, of 32-bit numbers
+// whose rounding the two sides' factors make good, so that a strong decay in front does not cost those
+// behind it their bits.  Outside the diagonal 2^(L_i - L_j) is a product of two factors below 1, with L at the row
+// block's start between them: 32 exponentials a row instead of 128.
+//
+// A CTA walks the chunks of 64 columns of one head of one request; 8 warps do the arithmetic between the
+// products, one warp loads tiles (TMA), one issues the products, one computes step sizes and decays of the
+// chunk after next.  W and M of a chunk are made while the tensor cores do Y2 and S, its state and result while
+// they do the next chunk's G.
+#include "selective.cuh"
+
+namespace b200 {
+namespace selective {
+namespace tiles {
+
+constexpr unsigned int kKernelId = 75;
+constexpr int kRows = 128, kP = 64;                    // tokens of a chunk, columns of a CTA
+constexpr int kSub = kRows * 128;                      // bytes of 128 rows of 64 bf16
+constexpr int kOffC = 0, kOffB = 2 * kSub, kOffX = 4 * kSub, kOffW = 6 * kSub, kOffH = 9 * kSub;
+constexpr int kOffScal = 11 * kSub;
+
+// Per chunk, by token: written by one warp, read by all.
+struct Scalars {
+  float row[kRows];       // 2^(L_i - L at the start of i's block of 32)
+  float diag[kRows];      // that exponent, rounded
+  float row_low[kRows];   // 2^(what the rounding left off)
+  float col_low[kRows];   // dt_j / 2^(the same)
+  float off[192];         // dt_j 2^(L at the start of block I - L_j): I = 1 (32), 2 (64), 3 (96 of them)
+  float w[kRows];         // dt_j 2^(L_end - L_j)
+  float e[kRows];         // 2^(L_i)
+  float end[4];           // 2^(L_end)
+};
+constexpr int kOffBars = kOffScal + 2 * static_cast<int>(sizeof(Scalars));
+constexpr int kSmem = kOffBars + 256 + 1024;
+static_assert(kSmem <= 232448, "shared memory of a CTA");
+
+enum Bar {
+  kCFull, kBFull, kCFree, kBFree, kXFull0, kXFull1, kXFree0, kXFree1, kSFull0, kSFull1, kSFree0, kSFree1, kGDone,
+  kMReady, kWReady, kSDone, kHReady, kYDone, kYFree, kBars
+};
+// columns of tensor memory
+constexpr uint32_t kColG = 0, kColY2 = 128, kColY1 = 256, kColS = 320, kTmem = 512;
+constexpr uint32_t kIdescAMajorMN = 1u << 15;
+constexpr int kThreads = 11 * 32;
+
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) { return __fmul2_rn(a, b); }
+// a pair of fp32 in bf16, and what that left off
+__device__ __forceinline__ uint32_t split(float& a, float& b) {
+  const uint32_t hi = pack_bf16x2(a, b);
+  const float2 f = unpack_bf16x2(hi);
+  a -= f.x;
+  b -= f.y;
+  return hi;
+}
+// 16 bytes of column chunk u (of 8) of row r in a tile of 128-byte rows, 128-byte swizzle
+__device__ __forceinline__ uint32_t tile_at(int r, int u) { return r * 128 + ((u ^ (r & 7)) << 4); }
+
+__device__ __forceinline__ double shfl_d(double v, int from) { return __shfl_sync(0xffffffffu, v, from); }
+
+// Step sizes and decays of tokens [t0, t0 + n) of a head, four per lane.
+__device__ __forceinline__ void chunk_scalars(const ScanArgs& a, int hd, long long t0, int n, double rate, Scalars* s) {
+  const int lane = threadIdx.x & 31;
+  float dt[4];
+  double L[4];
+  double run = 0.0;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const bool in = 4 * lane + k < n;
+    dt[k] = in ? step_size<__nv_bfloat16>(a, t0 + 4 * lane + k, hd) : 0.0f;
+    double la = static_cast<double>(dt[k]) * rate;
+    if (la < -160.0) la = -160.0;                       // 2^-160 is 0 in fp32; sums stay exact to 2^-40
+    run += la;
+    L[k] = run;
+  }
+  double before = run;                                  // inclusive over lanes, then what lies in front of the lane
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const double v = __shfl_up_sync(0xffffffffu, before, o);
+    if (lane >= o) before += v;
+  }
+  before = __shfl_up_sync(0xffffffffu, before, 1);
+  if (lane == 0) before = 0.0;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) L[k] += before;
+  const double ref1 = shfl_d(L[3], 7), ref2 = shfl_d(L[3], 15), ref3 = shfl_d(L[3], 23), end = shfl_d(L[3], 31);
+  const int block = lane >> 3;
+  const double ref = block == 0 ? 0.0 : block == 1 ? ref1 : block == 2 ? ref2 : ref3;
+  float row[4], diag[4], rl[4], cl[4], w[4], e[4], o1[4], o2[4], o3[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const double l = L[k] - ref;
+    diag[k] = static_cast<float>(l);
+    const float low = static_cast<float>(l - static_cast<double>(diag[k]));
+    row[k] = exp2f(diag[k]);
+    rl[k] = exp2f(low);
+    cl[k] = dt[k] * exp2f(-low);
+    w[k] = dt[k] * exp2f(static_cast<float>(end - L[k]));
+    e[k] = exp2f(static_cast<float>(L[k]));
+    o1[k] = dt[k] * exp2f(static_cast<float>(fmin(ref1 - L[k], 0.0)));
+    o2[k] = dt[k] * exp2f(static_cast<float>(fmin(ref2 - L[k], 0.0)));
+    o3[k] = dt[k] * exp2f(static_cast<float>(fmin(ref3 - L[k], 0.0)));
+  }
+  auto put = [&](float* to, const float (&v)[4]) {
+    *reinterpret_cast<float4*>(to + 4 * lane) = make_float4(v[0], v[1], v[2], v[3]);
+  };
+  put(s->row, row);
+  put(s->diag, diag);
+  put(s->row_low, rl);
+  put(s->col_low, cl);
+  put(s->w, w);
+  put(s->e, e);
+  if (lane < 8) put(s->off, o1);
+  if (lane < 16) put(s->off + 32, o2);
+  if (lane < 24) put(s->off + 96, o3);
+  if (lane == 0) s->end[0] = exp2f(static_cast<float>(end));
+}
+
+template <int N>
+__global__ void __launch_bounds__(kThreads, 1)
+heads_kernel(const ScanArgs a, const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_b,
+             const __grid_constant__ CUtensorMap tm_c, unsigned int* status) {
+  constexpr int kU = N / 64;                            // sub-tiles of B and C
+  extern __shared__ unsigned char raw[];
+  unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
+  Scalars* scal = reinterpret_cast<Scalars*>(smem + kOffScal);
+  uint64_t* bar = reinterpret_cast<uint64_t*>(smem + kOffBars);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bar + kBars);
+  volatile uint32_t* abort_flag = tmem_slot + 1;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kBars; ++i) {
+      const bool by_warps = i == kXFree0 || i == kXFree1 || i == kSFree0 || i == kSFree1 || i == kMReady || i == kWReady ||
+                            i == kHReady || i == kYFree;
+      mbar_init(&bar[i], by_warps ? 8 : 1);
+    }
+    *abort_flag = 0u;
+    mbar_fence_init();
+    tma_prefetch_desc(&tm_x);
+    tma_prefetch_desc(&tm_b);
+    tma_prefetch_desc(&tm_c);
+  }
+  if (warp == 9) {
+    tmem_alloc(tmem_slot, kTmem);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  grid_release();
+  grid_wait();
+
+  const int r = a.nd + blockIdx.y, p_blocks = a.width / kP;
+  const int hd = blockIdx.x / p_blocks, p0 = blockIdx.x % p_blocks * kP;
+  const int col0 = hd * a.width + p0, group = hd / (a.heads / a.groups);
+  const Portion po = portion_of(r, a.nd, a.cu_q, a.T);
+  const int chunks = max(0, po.end - po.first + kRows - 1) / kRows;
+  const int slot = a.state != nullptr ? a.slots[r] : 0;
+  const bool padding = a.state != nullptr && (slot < 0 || slot >= a.num_slots);
+  __nv_bfloat16* out = static_cast<__nv_bfloat16*>(a.out) + col0;
+
+  if (padding) {
+    for (int e = threadIdx.x; e < (po.end - po.first) * 8; e += kThreads)
+      *reinterpret_cast<uint4*>(out + (po.first + (e >> 3)) * a.ldo + (e & 7) * 8) = make_uint4(0, 0, 0, 0);
+  } else if (warp < 8) {
+    // ---------------- arithmetic between the products ----------------
+    const int q = warp & 3, half = warp >> 2;
+    const int i = q * 32 + lane;                        // lane of tensor memory: token, or number of the state
+    const uint32_t mine = tmem + (static_cast<uint32_t>(q * 32) << 16);
+    const bool old = a.state != nullptr && chunks > 0 && a.positions[po.first] != 0;
+    const int ws = a.state != nullptr ? a.wslots[r] : -1;
+    const long long head_at = (static_cast<long long>(a.heads) * a.width * N);
+    const long long at = (static_cast<long long>(col0) + half * 32) * N + i;
+    float h[32];
+#pragma unroll
+    for (int k = 0; k < 32; ++k) h[k] = old && i < N ? a.state[slot * head_at + at + k * N] : 0.0f;
+    auto put_state = [&]() {
+      if (i < N) {
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          uint32_t hi[4], lo[4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            float f = h[u * 8 + 2 * k], g = h[u * 8 + 2 * k + 1];
+            hi[k] = split(f, g);
+            lo[k] = pack_bf16x2(f, g);
+          }
+          unsigned char* to = smem + kOffH + tile_at(i, half * 4 + u);
+          *reinterpret_cast<uint4*>(to) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+          *reinterpret_cast<uint4*>(to + kSub) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+        }
+      }
+      fence_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bar[kHReady]);
+    };
+    put_state();
+    const float skip = a.d != nullptr ? a.d[hd] : 0.0f;
+    bool ok = true;
+    for (int c = 0; c < chunks; ++c) {
+      const int stage = c & 1, ph = (c >> 1) & 1, n = min(kRows, po.end - po.first - c * kRows);
+      const Scalars* s = scal + stage;
+      unsigned char* x = smem + kOffX + stage * kSub;
+      ok = mbar_wait_warp(&bar[kSFull0 + stage], ph, status, kKernelId, 0x100u, abort_flag) &&
+           mbar_wait_warp(&bar[kXFull0 + stage], ph, status, kKernelId, 0x101u, abort_flag);
+      if (!ok) break;
+      if (n < kRows) {              // rows of other requests: zeros, they may hold anything
+        ok = mbar_wait_warp(&bar[kBFull], c & 1, status, kKernelId, 0x102u, abort_flag);
+        if (!ok) break;
+      }
+      // W = x times its weight, in three parts
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int row = (threadIdx.x >> 3) + 32 * k, u = threadIdx.x & 7;
+        const uint32_t to = tile_at(row, u);
+        uint4 v = *reinterpret_cast<const uint4*>(x + to);
+        if (row >= n) {
+          v = make_uint4(0, 0, 0, 0);
+          *reinterpret_cast<uint4*>(x + to) = v;
+#pragma unroll
+          for (int b = 0; b < kU; ++b) *reinterpret_cast<uint4*>(smem + kOffB + b * kSub + to) = v;
+        }
+        const float w = s->w[row];
+        const uint32_t in[4] = {v.x, v.y, v.z, v.w};
+        uint32_t part[3][4];
+#pragma unroll
+        for (int m = 0; m < 4; ++m) {
+          const float2 f = unpack_bf16x2(in[m]);
+          float f0 = w * f.x, f1 = w * f.y;
+          part[0][m] = split(f0, f1);
+          part[1][m] = split(f0, f1);
+          part[2][m] = pack_bf16x2(f0, f1);
+        }
+#pragma unroll
+        for (int m = 0; m < 3; ++m)
+          *reinterpret_cast<uint4*>(smem + kOffW + m * kSub + to) =
+              make_uint4(part[m][0], part[m][1], part[m][2], part[m][3]);
+      }
+      fence_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bar[kWReady]);
+
+      // M in place of G: this warp's 16 of every 32 columns
+      ok = mbar_wait_warp(&bar[kGDone], c & 1, status, kKernelId, 0x103u, abort_flag);
+      if (!ok) break;
+      tc_fence_after();
+      uint32_t g[4][16];
+#pragma unroll
+      for (int J = 0; J < 4; ++J)
+        if (J <= q) tmem_ld_32x16(mine + kColG + 32 * J + 16 * half, g[J]);
+      tmem_ld_wait();
+      {
+        const float row = s->row[i], di = s->diag[i], low = s->row_low[i];
+        const float* off = s->off + (q == 2 ? 32 : q == 3 ? 96 : 0);
+#pragma unroll
+        for (int J = 0; J < 4; ++J) {
+          uint32_t m[16];
+          if (J > q) {
+#pragma unroll
+            for (int k = 0; k < 16; ++k) m[k] = 0u;
+          } else {
+#pragma unroll
+            for (int k = 0; k < 16; k += 4) {
+              float v[4];
+              if (J < q) {
+                const float4 f = *reinterpret_cast<const float4*>(off + 32 * J + 16 * half + k);
+                const float fc[4] = {f.x, f.y, f.z, f.w};
+#pragma unroll
+                for (int m4 = 0; m4 < 4; ++m4) v[m4] = __uint_as_float(g[J][k + m4]) * (fc[m4] * row);
+              } else {
+                const float4 d = *reinterpret_cast<const float4*>(s->diag + 32 * q + 16 * half + k);
+                const float4 f = *reinterpret_cast<const float4*>(s->col_low + 32 * q + 16 * half + k);
+                const float dj[4] = {d.x, d.y, d.z, d.w}, fc[4] = {f.x, f.y, f.z, f.w};
+#pragma unroll
+                for (int m4 = 0; m4 < 4; ++m4) {
+                  const float w = exp2_fast(di - dj[m4]) * (fc[m4] * low);
+                  v[m4] = 16 * half + k + m4 <= lane ? __uint_as_float(g[J][k + m4]) * w : 0.0f;
+                }
+              }
+              m[k / 2] = split(v[0], v[1]);
+              m[k / 2 + 1] = split(v[2], v[3]);
+              m[8 + k / 2] = pack_bf16x2(v[0], v[1]);
+              m[8 + k / 2 + 1] = pack_bf16x2(v[2], v[3]);
+            }
+          }
+          tmem_st_32x16(mine + kColG + 32 * J + 16 * half, m);
+        }
+      }
+      tmem_st_wait();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bar[kMReady]);
+
+      // the state behind the chunk
+      ok = mbar_wait_warp(&bar[kSDone], c & 1, status, kKernelId, 0x104u, abort_flag);
+      if (!ok) break;
+      tc_fence_after();
+      {
+        const float keep = s->end[0];
+        uint32_t v[3][32];
+#pragma unroll
+        for (int m = 0; m < 3; ++m) tmem_ld_32x32(mine + kColS + m * 64 + half * 32, v[m]);
+        tmem_ld_wait();
+#pragma unroll
+        for (int k = 0; k < 32; ++k)
+          h[k] = fmaf(keep, h[k], __uint_as_float(v[0][k]) + (__uint_as_float(v[1][k]) + __uint_as_float(v[2][k])));
+      }
+      tc_fence_before();
+      put_state();
+
+      // the result's rows
+      ok = mbar_wait_warp(&bar[kYDone], c & 1, status, kKernelId, 0x105u, abort_flag);
+      if (!ok) break;
+      tc_fence_after();
+      {
+        uint32_t y1[32], y2[32], y3[32];
+        tmem_ld_32x32(mine + kColY1 + half * 32, y1);
+        tmem_ld_32x32(mine + kColY2 + half * 32, y2);
+        tmem_ld_32x32(mine + kColY2 + 64 + half * 32, y3);
+        tmem_ld_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bar[kYFree]);
+        const float e = s->e[i];
+        const long long t = po.first + c * kRows + i;
+        if (i < n) {
+#pragma unroll
+          for (int u = 0; u < 4; ++u) {
+            const uint4 xv = *reinterpret_cast<const uint4*>(x + tile_at(i, half * 4 + u));
+            const uint32_t xi[4] = {xv.x, xv.y, xv.z, xv.w};
+            float f[8];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const float2 xf = unpack_bf16x2(xi[k]);
+              const int at2 = u * 8 + 2 * k;
+              f[2 * k] = fmaf(e, __uint_as_float(y2[at2]) + __uint_as_float(y3[at2]),
+                              fmaf(skip, xf.x, __uint_as_float(y1[at2])));
+              f[2 * k + 1] = fmaf(e, __uint_as_float(y2[at2 + 1]) + __uint_as_float(y3[at2 + 1]),
+                                  fmaf(skip, xf.y, __uint_as_float(y1[at2 + 1])));
+            }
+            if (a.z != nullptr) {
+              float z[8];
+              vec8_load(static_cast<const __nv_bfloat16*>(a.z) + t * a.ldz + col0 + half * 32 + u * 8, z);
+#pragma unroll
+              for (int k = 0; k < 8; ++k) f[k] *= silu<__nv_bfloat16>(z[k]);
+            }
+            vec8_store(out + t * a.ldo + half * 32 + u * 8, f);
+          }
+        }
+      }
+      __syncwarp();
+      if (lane == 0) {
+        mbar_arrive(&bar[kXFree0 + stage]);
+        mbar_arrive(&bar[kSFree0 + stage]);
+      }
+    }
+    if (ok && chunks > 0 && ws >= 0 && ws < a.num_slots && i < N) {
+#pragma unroll
+      for (int k = 0; k < 32; ++k) a.state[ws * head_at + at + k * N] = h[k];
+    }
+  } else if (warp == 8) {
+    // ---------------- tiles ----------------
+    if (elect_one()) {
+      int issued = 0;
+      for (int c = 0; c < chunks; ++c) {
+        const int y = po.first + c * kRows, stage = c & 1;
+        if (c >= 2 && !mbar_wait(&bar[kXFree0 + stage], ((c >> 1) & 1) ^ 1, status, kKernelId, 0x200u, abort_flag)) break;
+        mbar_expect_tx(&bar[kXFull0 + stage], kSub);
+        tma_load_2d(smem + kOffX + stage * kSub, &tm_x, &bar[kXFull0 + stage], col0, y);
+        issued = 4 * c + 1;
+        if (c >= 1 && !mbar_wait(&bar[kCFree], (c - 1) & 1, status, kKernelId, 0x201u, abort_flag)) break;
+        mbar_expect_tx(&bar[kCFull], kU * kSub);
+        for (int u = 0; u < kU; ++u) tma_load_2d(smem + kOffC + u * kSub, &tm_c, &bar[kCFull], group * N + u * 64, y);
+        issued = 4 * c + 2;
+        if (c >= 1 && !mbar_wait(&bar[kBFree], (c - 1) & 1, status, kKernelId, 0x202u, abort_flag)) break;
+        mbar_expect_tx(&bar[kBFull], kU * kSub);
+        for (int u = 0; u < kU; ++u) tma_load_2d(smem + kOffB + u * kSub, &tm_b, &bar[kBFull], group * N + u * 64, y);
+        issued = 4 * c + 3;
+      }
+      // copies in flight end before the CTA does, also when a wait ran out
+      if (*abort_flag != 0u && issued > 0) {
+        const int c = issued >> 2, what = issued & 3;
+        mbar_wait(&bar[kXFull0 + (c & 1)], (c >> 1) & 1, status, kKernelId, 0x210u);
+        if (c >= 1) mbar_wait(&bar[kXFull0 + ((c - 1) & 1)], ((c - 1) >> 1) & 1, status, kKernelId, 0x211u);
+        if (what >= 2 || c >= 1) mbar_wait(&bar[kCFull], (what >= 2 ? c : c - 1) & 1, status, kKernelId, 0x212u);
+        if (what >= 3 || c >= 1) mbar_wait(&bar[kBFull], (what >= 3 ? c : c - 1) & 1, status, kKernelId, 0x213u);
+      }
+    }
+  } else if (warp == 9) {
+    // ---------------- products ----------------
+    if (elect_one()) {
+      constexpr uint32_t kIdG = make_idesc(kRows, 128, 1, 1);
+      constexpr uint32_t kIdY2 = make_idesc(kRows, 128, 1, 1) | kIdescBMajorMN;
+      constexpr uint32_t kIdS = make_idesc(kRows, 192, 1, 1) | kIdescAMajorMN | kIdescBMajorMN;
+      constexpr uint32_t kIdY1 = make_idesc(kRows, kP, 1, 1) | kIdescBMajorMN;
+      constexpr uint32_t kStep = 2048 >> 4;              // 16 rows of a tile
+      const uint32_t base = smem_u32(smem);
+      const uint64_t c_k = make_desc_k_sw128(base + kOffC), b_k = make_desc_k_sw128(base + kOffB);
+      // (64 numbers of state: lanes 64 and up of S come from memory that holds nothing, and nobody reads them)
+      const uint64_t b_mn = make_desc_mn_sw128(base + kOffB, kSub);
+      const uint64_t w_mn = make_desc_mn_sw128(base + kOffW, kSub), h_mn = make_desc_mn_sw128(base + kOffH, kSub);
+      const uint64_t x_mn = make_desc_mn_sw128(base + kOffX, kSub);
+      auto wait = [&](int b, int parity, uint32_t what) {
+        const bool there = mbar_wait(&bar[b], parity, status, kKernelId, 0x300u + what, abort_flag);
+        tc_fence_after();
+        return there;
+      };
+      for (int c = 0; c < chunks; ++c) {
+        const int ph = c & 1;
+        if (!wait(kCFull, ph, 0) || !wait(kBFull, ph, 1)) break;
+#pragma unroll
+        for (int k = 0; k < N / 16; ++k) {
+          const uint32_t step = (k >> 2) * (kSub >> 4) + (k & 3) * 2;
+          umma_f16(tmem + kColG, c_k + step, b_k + step, kIdG, k > 0);
+        }
+        umma_commit(&bar[kGDone]);
+        if (!wait(kHReady, ph, 2) || (c > 0 && !wait(kYFree, ph ^ 1, 3))) break;
+#pragma unroll
+        for (int k = 0; k < N / 16; ++k)
+          umma_f16(tmem + kColY2, c_k + (k >> 2) * (kSub >> 4) + (k & 3) * 2, h_mn + k * kStep, kIdY2, k > 0);
+        umma_commit(&bar[kCFree]);
+        if (!wait(kWReady, ph, 4)) break;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) umma_f16(tmem + kColS, b_mn + k * kStep, w_mn + k * kStep, kIdS, k > 0);
+        umma_commit(&bar[kBFree]);
+        umma_commit(&bar[kSDone]);
+        if (!wait(kMReady, ph, 5)) break;
+        const uint64_t x = x_mn + (c & 1) * (kSub >> 4);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          umma_f16_ts(tmem + kColY1, tmem + kColG + 16 * k, x + k * kStep, kIdY1, k > 0);
+          umma_f16_ts(tmem + kColY1, tmem + kColG + 16 * k + 8, x + k * kStep, kIdY1, 1);
+        }
+        umma_commit(&bar[kYDone]);
+      }
+    }
+  } else {
+    // ---------------- step sizes and decays ----------------
+    const double rate = -exp(static_cast<double>(a.a_log[hd])) * 1.4426950408889634;
+    for (int c = 0; c < chunks; ++c) {
+      if (c >= 2 && !mbar_wait_warp(&bar[kSFree0 + (c & 1)], ((c >> 1) & 1) ^ 1, status, kKernelId, 0x400u, abort_flag))
+        break;
+      chunk_scalars(a, hd, po.first + c * kRows, min(kRows, po.end - po.first - c * kRows), rate, scal + (c & 1));
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bar[kSFull0 + (c & 1)]);
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 9) tmem_dealloc(tmem, kTmem);
+}
+
+template <int N>
+int launch(const ScanArgs& a, cudaStream_t s) {
+  CUtensorMap x, b, c;
+  const CUtensorMapDataType bf = CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  const CUtensorMapSwizzle sw = CU_TENSOR_MAP_SWIZZLE_128B;
+  const uint64_t gn = static_cast<uint64_t>(a.groups) * N;
+  const uint64_t cols = static_cast<uint64_t>(a.heads) * a.width;
+  auto pitch = [&](long long ld, uint64_t width) { return a.T > 1 ? 2 * static_cast<uint64_t>(ld) : 2 * width; };
+  int rc = encode_tmap_2d(&x, bf, 2, a.x, a.T, cols, pitch(a.ldx, cols), kRows, 64, sw);
+  if (rc == 0) rc = encode_tmap_2d(&b, bf, 2, a.b, a.T, gn, pitch(a.ldb, gn), kRows, 64, sw);
+  if (rc == 0) rc = encode_tmap_2d(&c, bf, 2, a.c, a.T, gn, pitch(a.ldc, gn), kRows, 64, sw);
+  if (rc != 0) return rc;
+  unsigned int* status = status_ptr();
+  if (status == nullptr) return -9;
+  static bool ready[64] = {};                            // per device
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return -9;
+  if (dev >= 64 || !ready[dev]) {
+    const int e = launch_code(cudaFuncSetAttribute(heads_kernel<N>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem));
+    if (e != 0) return e;
+    if (dev < 64) ready[dev] = true;
+  }
+  return launch_overlapped(heads_kernel<N>, dim3(a.heads * (a.width / kP), a.np), dim3(kThreads), kSmem, s, a, x, b, c,
+                           status);
+}
+
+}  // namespace tiles
+
+bool heads_by_tiles(const ScanArgs& a) {
+  return a.wide && a.width % tiles::kP == 0 && (a.N == 64 || a.N == 128);
+}
+int launch_heads_by_tiles(const ScanArgs& a, cudaStream_t s) {
+  return a.N == 128 ? tiles::launch<128>(a, s) : tiles::launch<64>(a, s);
+}
+
+}  // namespace selective
+}  // namespace b200

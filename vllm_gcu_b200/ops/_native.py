@@ -173,7 +173,7 @@ class _Sigs:
                         I, I, I, I, I, I, P]
     b200_causal_conv = [P, L, P, I, P, P, I, P, P, P, P, P, L, I, I, I, I, I, I, I, P]
     b200_selective_scan = [P, L, P, L, I, P, L, P, L, P, L, P, I, P, P, I, F, F, P, I, P, P, P, P, P, L,
-                           I, I, I, I, I, I, I, I, P]
+                           I, I, I, I, I, I, I, I, I, P]
     b200_group_norm_gate = [P, L, P, L, P, P, P, L, F, I, I, I, I, I, I, I, I, P]
     b200_gemm_wna16 = [P, L, P, P, P, P, P, L, I, I, I, I, I, P]
     b200_gemm_wna16_grouped = [P, L, P, P, P, P, L, I, I, I, I, I, I, P, P, P, P]

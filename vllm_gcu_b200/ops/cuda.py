@@ -1758,7 +1758,7 @@ def selective_scan(x: torch.Tensor, dt: torch.Tensor, b: torch.Tensor, c: torch.
              ptr(b), b.stride(0), ptr(c), c.stride(0), ptr(z), z.stride(0) if z is not None else 0, ptr(a_log),
              int(channels), ptr(d), ptr(dt_bias), int(softplus), lo, hi, ptr(state), state.shape[0] if use else 0,
              ptr(pos), ptr(slots), ptr(wslots), ptr(cu), ptr(out), out.stride(0), T, heads, width, N, groups, nd,
-             npf, DTYPE_CODE[x.dtype], stream_ptr())
+             npf, int(_wide_rows(x, b, c, z, out)), DTYPE_CODE[x.dtype], stream_ptr())
     return out
 
 
