@@ -128,8 +128,10 @@ def test_refusals():
                 scan(**k)
         # columns of one buffer that do not meet are no overlap
         wide = torch.zeros(5, row.shape[1] + 4 * P, dtype=BF16)
-        assert not C._overlap(wide[:, :4 * P], wide[:, 4 * P:])
-        assert C._overlap(wide[:, :4 * P + 1], wide[:, 4 * P:]) and C._overlap(wide[:, 4 * P:], wide[:, 1:4 * P + 1])
+        meet = lambda u, v: C._overlap(*((t.data_ptr(), t.stride(0), *t.shape, 2) for t in (u, v)))  # noqa: E731
+        assert not meet(wide[:, :4 * P], wide[:, 4 * P:]) and not meet(wide[:, 4 * P:], wide[:, :4 * P])
+        assert meet(wide[:, :4 * P + 1], wide[:, 4 * P:]) and meet(wide[:, 4 * P:], wide[:, 1:4 * P + 1])
+        assert not meet(wide[:2], wide[2:]) and meet(wide[:3], wide[2:]) and not meet(wide[:0], wide)
     z, w8 = torch.randn_like(x), torch.ones(8)
     norm = lambda **k: C.group_norm_gate(**{**dict(x=x, z=z, weight=w8, groups=2, eps=1e-5), **k})  # noqa: E731
     for k, says in [(dict(groups=3), "groups"), (dict(groups=0), "groups"), (dict(act="gelu"), "gelu"),

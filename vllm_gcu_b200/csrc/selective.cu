@@ -285,24 +285,53 @@ __global__ void __launch_bounds__(128) selective_step_kernel(const ScanArgs a) {
   }
 }
 
-// Portions of prompts, token after token.  A CTA holds kCols columns of one head of one request; LPC
-// lanes share a column, RPL numbers of its state each, in registers.  Inputs are staged through shared memory
-// kChunk tokens at a time.
-constexpr int kChunk = 16;
+// Portions of prompts, token after token.  A CTA holds the columns of one request that kThreads / LPC lane groups
+// make: a column's numbers of state lie in the registers of LPC lanes, NPL each, and a token costs a number one
+// decay (rates per channel: a power of two, which the special function unit does 16 of per clock and SM: it bounds
+// them), two multiply-adds and a product.  Inputs pass through shared memory kTok tokens at a time: while a
+// tile is worked on, the next one is on its way to registers, eight neighbouring elements per thread, and a
+// thread finishes the elements that it brought (skip, gate, store).  Each token's sum over the lanes of a column
+// is left for kSum tokens, then lanes trade partial sums so that each ends up with the sums of its own
+// tokens: 3 exchanges for 4 tokens of 4 lanes instead of 8.
+template <int LPC>
+constexpr int kScanThreads = LPC == 16 ? 256 : 128;
 
-template <typename T, bool CH, int LPC, int RPL>
-__global__ void __launch_bounds__(128) selective_scan_kernel(const ScanArgs a) {
-  constexpr int NP = LPC * RPL, kCols = 128 / LPC;
-  __shared__ __align__(16) float sb[kChunk][NP], sc[kChunk][NP];
-  __shared__ float sdt[kChunk][kCols], sx[kChunk][kCols], sy[kChunk][kCols];
-  __shared__ float sdecay[kChunk];
+template <typename T>
+struct __align__(16) Eight {
+  T e[8];
+};
+// eight neighbours of a row; `n` of them are there
+template <typename T, bool WIDE>
+__device__ __forceinline__ Eight<T> load_eight(const T* p, int n) {
+  Eight<T> v;
+  if (WIDE) {
+    if (n > 0) v = *reinterpret_cast<const Eight<T>*>(p);
+    else
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v.e[i] = from_f32<T>(0.0f);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v.e[i] = i < n ? p[i] : from_f32<T>(0.0f);
+  }
+  return v;
+}
+
+template <typename T, bool CH, int LPC, int NPL, bool WIDE>
+__global__ void __launch_bounds__(kScanThreads<LPC>) selective_scan_kernel(const ScanArgs a) {
+  constexpr int kThreads = kScanThreads<LPC>, NP = LPC * NPL, kCols = kThreads / LPC, kTok = LPC == 2 || NP > 128 ? 16 : 32;
+  constexpr int kSum = LPC < 8 ? LPC : 8;
+  constexpr int kVecs = kTok * kCols / 8;                    // threads that bring and finish elements
+  constexpr int kParts = (2 * kTok * NP / 8 + kThreads - 1) / kThreads;
+  static_assert(kVecs <= kThreads, "one vector of eight per thread");
+  __shared__ __align__(16) float sbc[2][kTok][NP];           // B, C
+  __shared__ __align__(16) float2 sd[kTok][kCols];           // step size (rates per head: decay), step size times x
+  __shared__ __align__(16) float sy[kTok][kCols + 4];
   grid_release_small();
   grid_wait();
-  const int r = a.nd + blockIdx.x, hd = blockIdx.y, p0 = blockIdx.z * kCols;
+  const int r = a.nd + blockIdx.x, g = blockIdx.y, per = a.heads / a.groups * a.width;
   const int l = threadIdx.x & (LPC - 1), col = threadIdx.x / LPC;
-  const int cols = min(kCols, a.width - p0);
-  const int c0 = hd * a.width + p0;                          // first column of the CTA
-  const int g = hd / (a.heads / a.groups);
+  const int p0 = blockIdx.z * kCols, cols = min(kCols, per - p0);
+  const int c0 = g * per + p0;                               // first column of the CTA
   const Portion po = portion_of(r, a.nd, a.cu_q, a.T);
   if (po.first >= po.end) return;
   const int slot = a.state != nullptr ? a.slots[r] : 0;
@@ -317,73 +346,156 @@ __global__ void __launch_bounds__(128) selective_scan_kernel(const ScanArgs a) {
   const bool keep = ws >= 0 && ws < a.num_slots;
   const long long pitch = static_cast<long long>(a.heads) * a.width * a.N;
   const long long at = static_cast<long long>(c0 + col) * a.N;
-  float h[RPL], rate[RPL];
+  float2 h[NPL / 2], rate[NPL / 2];
+  auto number = [&](int i) { return (i / 4 * LPC + l) * 4 + i % 4; };
 #pragma unroll
-  for (int i = 0; i < RPL; ++i) {
-    const int n = (i / 4 * LPC + l) * 4 + i % 4;
+  for (int i = 0; i < NPL; ++i) {
+    const int n = number(i);
     const bool in = n < a.N && col < cols;
-    h[i] = old && in ? a.state[slot * pitch + at + n] : 0.0f;
-    rate[i] = CH && in ? -expf(a.a_log[at + n]) * kLog2e : 0.0f;
+    const float v = old && in ? a.state[slot * pitch + at + n] : 0.0f;
+    const float q = CH && in ? -expf(a.a_log[at + n]) * kLog2e : 0.0f;
+    (i & 1 ? h[i / 2].y : h[i / 2].x) = v;
+    (i & 1 ? rate[i / 2].y : rate[i / 2].x) = q;
   }
-  const float head_rate = CH ? 0.0f : -expf(a.a_log[hd]);
 
-  for (int t0 = po.first; t0 < po.end; t0 += kChunk) {
-    const int n = min(kChunk, po.end - t0);
-    for (int e = threadIdx.x; e < n * NP; e += 128) {
-      const int i = e / NP, k = e % NP;
-      const long long t = t0 + i;
-      sb[i][k] = k < a.N ? to_f32<T>(static_cast<const T*>(a.b)[t * a.ldb + g * a.N + k]) : 0.0f;
-      sc[i][k] = k < a.N ? to_f32<T>(static_cast<const T*>(a.c)[t * a.ldc + g * a.N + k]) : 0.0f;
+  // this thread's eight elements of a tile: token vt, columns vc and on; what belongs to a column stays
+  const int vt = threadIdx.x / (kCols / 8), vc = threadIdx.x % (kCols / 8) * 8;
+  const int vn = threadIdx.x < kVecs ? max(0, min(8, cols - vc)) : 0;
+  const bool one_head = !CH && a.width % 8 == 0;             // eight columns share a step size
+  float bias[8], skip[8], hrate[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int which = CH ? c0 + vc + i : (c0 + vc + i) / a.width;
+    const bool in = i < vn;
+    bias[i] = in && a.dt_bias != nullptr ? a.dt_bias[which] : 0.0f;
+    skip[i] = in && a.d != nullptr ? a.d[which] : 0.0f;
+    hrate[i] = !CH && in ? -expf(a.a_log[which]) : 0.0f;
+  }
+  Eight<T> x, z, dth, bc[kParts];
+  Eight<float> dtf;
+  auto bring = [&](int t0) {
+    const int n = po.end - t0;
+    const int here = vt < n ? vn : 0;
+    const long long t = t0 + vt;
+    const int which = CH ? c0 + vc : (c0 + vc) / a.width;
+    x = load_eight<T, WIDE>(static_cast<const T*>(a.x) + t * a.ldx + c0 + vc, here);
+    if (a.z != nullptr) z = load_eight<T, WIDE>(static_cast<const T*>(a.z) + t * a.ldz + c0 + vc, here);
+    if (CH) {
+      if (a.dt_f32) dtf = load_eight<float, false>(static_cast<const float*>(a.dt) + t * a.lddt + which, here);
+      else dth = load_eight<T, WIDE>(static_cast<const T*>(a.dt) + t * a.lddt + which, here);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        if (i > 0 && one_head) break;
+        if (i >= here) break;
+        const long long k = t * a.lddt + (c0 + vc + i) / a.width;
+        if (a.dt_f32) dtf.e[i] = static_cast<const float*>(a.dt)[k];
+        else dth.e[i] = static_cast<const T*>(a.dt)[k];
+      }
     }
-    for (int e = threadIdx.x; e < n * cols; e += 128) {
-      const int i = e / cols, k = e % cols;
-      const long long t = t0 + i;
-      sx[i][k] = to_f32<T>(static_cast<const T*>(a.x)[t * a.ldx + c0 + k]);
-      if (CH) sdt[i][k] = step_size<T>(a, t, c0 + k);
+#pragma unroll
+    for (int i = 0; i < kParts; ++i) {
+      const int e = threadIdx.x + i * kThreads;
+      const int m = e / (kTok * NP / 8), k = e / (NP / 8) % kTok, c = e % (NP / 8) * 8;
+      const T* row = m == 0 ? static_cast<const T*>(a.b) + (t0 + k) * a.ldb : static_cast<const T*>(a.c) + (t0 + k) * a.ldc;
+      bc[i] = load_eight<T, WIDE>(row + g * a.N + c, m < 2 && k < n ? max(0, min(8, a.N - c)) : 0);
     }
-    if (!CH && threadIdx.x < n) {
-      const float dt = step_size<T>(a, t0 + threadIdx.x, hd);
-      sdt[threadIdx.x][0] = dt;
-      sdecay[threadIdx.x] = expf(dt * head_rate);
+  };
+  bring(po.first);
+
+  for (int t0 = po.first; t0 < po.end; t0 += kTok) {
+    // registers -> shared memory; a token behind the portion has a step of 0, which leaves a state as it is
+    const bool here = vt < po.end - t0 && threadIdx.x < kVecs;
+    if (threadIdx.x < kVecs) {
+      float dt = 0.0f, decay = 1.0f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        if (here && i < vn && (i == 0 || !one_head)) {
+          dt = step_from<T>(a, a.dt_f32 ? dtf.e[i] : to_f32<T>(dth.e[i]), bias[i]);
+          if (!CH) decay = expf(dt * hrate[i]);
+        }
+        const bool in = here && i < vn;
+        sd[vt][vc + i] = in ? make_float2(CH ? dt : decay, dt * to_f32<T>(x.e[i])) : make_float2(CH ? 0.0f : 1.0f, 0.0f);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < kParts; ++i) {
+      const int e = threadIdx.x + i * kThreads;
+      if (e < 2 * kTok * NP / 8) {
+        float* to = &sbc[0][0][0] + e * 8;
+#pragma unroll
+        for (int k = 0; k < 8; k += 4)
+          *reinterpret_cast<float4*>(to + k) = make_float4(to_f32<T>(bc[i].e[k]), to_f32<T>(bc[i].e[k + 1]),
+                                                           to_f32<T>(bc[i].e[k + 2]), to_f32<T>(bc[i].e[k + 3]));
+      }
     }
     __syncthreads();
-    for (int i = 0; i < n; ++i) {
-      const float dt = CH ? sdt[i][col < cols ? col : 0] : sdt[i][0];
-      const float dx = dt * sx[i][col < cols ? col : 0];
-      float s = 0.0f;
+    const Eight<T> xs = x, zs = z;
+    if (t0 + kTok < po.end) bring(t0 + kTok);
+#pragma unroll 1
+    for (int i = 0; i < kTok; i += kSum) {
+      float part[kSum];
 #pragma unroll
-      for (int k = 0; k < RPL; k += 4) {
-        const float4 bq = *reinterpret_cast<const float4*>(&sb[i][(k / 4 * LPC + l) * 4]);
-        const float4 cq = *reinterpret_cast<const float4*>(&sc[i][(k / 4 * LPC + l) * 4]);
-        const float be[4] = {bq.x, bq.y, bq.z, bq.w}, ce[4] = {cq.x, cq.y, cq.z, cq.w};
+      for (int u = 0; u < kSum; ++u) {
+        const float2 dd = sd[i + u][col];
+        const float2 dx = make_float2(dd.y, dd.y);
+        float2 s = make_float2(0.0f, 0.0f);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float e = CH ? exp2f(dt * rate[k + j]) : sdecay[i];
-          h[k + j] = fmaf(e, h[k + j], dx * be[j]);
-          s = fmaf(h[k + j], ce[j], s);
+        for (int k = 0; k < NPL / 4; ++k) {
+          const float4 bq = *reinterpret_cast<const float4*>(&sbc[0][i + u][(k * LPC + l) * 4]);
+          const float4 cq = *reinterpret_cast<const float4*>(&sbc[1][i + u][(k * LPC + l) * 4]);
+          const float2 be[2] = {make_float2(bq.x, bq.y), make_float2(bq.z, bq.w)};
+          const float2 ce[2] = {make_float2(cq.x, cq.y), make_float2(cq.z, cq.w)};
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            float2 e = make_float2(dd.x, dd.x);
+            if (CH) {
+              e = __fmul2_rn(e, rate[2 * k + j]);
+              e = make_float2(exp2_fast(e.x), exp2_fast(e.y));
+            }
+            h[2 * k + j] = __ffma2_rn(e, h[2 * k + j], __fmul2_rn(dx, be[j]));
+            s = __ffma2_rn(h[2 * k + j], ce[j], s);
+          }
+        }
+        part[u] = s.x + s.y;
+      }
+      // lane l of a column gets the sums of token i + l % kSum
+#pragma unroll
+      for (int o = kSum / 2; o > 0; o >>= 1) {
+        const bool up = l & o;
+#pragma unroll
+        for (int u = 0; u < o; ++u) {
+          const float mine = up ? part[u + o] : part[u], theirs = up ? part[u] : part[u + o];
+          part[u] = mine + __shfl_xor_sync(0xffffffffu, theirs, o);
         }
       }
 #pragma unroll
-      for (int o = 1; o < LPC; o <<= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-      if (l == 0) sy[i][col] = s;
+      for (int o = kSum; o < LPC; o <<= 1) part[0] += __shfl_xor_sync(0xffffffffu, part[0], o);
+      if (l < kSum) sy[i + l][col] = part[0];
     }
     __syncthreads();
-    for (int e = threadIdx.x; e < n * cols; e += 128) {
-      const int i = e / cols, k = e % cols;
-      const long long t = t0 + i;
-      float y = sy[i][k];
-      if (a.d != nullptr) y = fmaf(a.d[CH ? c0 + k : hd], sx[i][k], y);
-      if (a.z != nullptr) y *= silu<T>(to_f32<T>(static_cast<const T*>(a.z)[t * a.ldz + c0 + k]));
-      out[t * a.ldo + k] = from_f32<T>(y);
+    if (here && vn > 0) {
+      Eight<T> y;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        float f = fmaf(skip[i], to_f32<T>(xs.e[i]), sy[vt][vc + i]);
+        if (a.z != nullptr) f *= silu<T>(to_f32<T>(zs.e[i]));
+        y.e[i] = from_f32<T>(f);
+      }
+      T* to = out + static_cast<long long>(t0 + vt) * a.ldo + vc;
+      if (WIDE) {
+        *reinterpret_cast<Eight<T>*>(to) = y;
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (i < vn) to[i] = y.e[i];
+      }
     }
-    __syncthreads();
   }
   if (keep && col < cols) {
 #pragma unroll
-    for (int i = 0; i < RPL; ++i) {
-      const int n = (i / 4 * LPC + l) * 4 + i % 4;
-      if (n < a.N) a.state[ws * pitch + at + n] = h[i];
-    }
+    for (int i = 0; i < NPL; ++i)
+      if (number(i) < a.N) a.state[ws * pitch + at + number(i)] = i & 1 ? h[i / 2].y : h[i / 2].x;
   }
 }
 
@@ -428,15 +540,18 @@ int launch_step(const ScanArgs& a, cudaStream_t s) {
 #undef STEP
 }
 
-template <typename T, bool CH>
+template <typename T, bool CH, bool WIDE>
 int launch_scan(const ScanArgs& a, cudaStream_t s) {
-#define SCAN(LPC, RPL)                                                                                        \
-  launch_overlapped(selective_scan_kernel<T, CH, LPC, RPL>,                                                   \
-                    dim3(a.np, a.heads, (a.width + 128 / LPC - 1) / (128 / LPC)), dim3(128), 0, s, a)
+  const int per = a.heads / a.groups * a.width;
+#define SCAN(LPC, NPL)                                                                                     \
+  launch_overlapped(selective_scan_kernel<T, CH, LPC, NPL, WIDE>,                                          \
+                    dim3(a.np, a.groups, (per + kScanThreads<LPC> / LPC - 1) / (kScanThreads<LPC> / LPC)), \
+                    dim3(kScanThreads<LPC>), 0, s, a)
+  if (a.N <= 8) return SCAN(2, 4);
   if (a.N <= 16) return SCAN(4, 4);
-  if (a.N <= 32) return SCAN(4, 8);
-  if (a.N <= 64) return SCAN(8, 8);
-  if (a.N <= 128) return SCAN(8, 16);
+  if (a.N <= 32) return SCAN(8, 4);
+  if (a.N <= 64) return SCAN(16, 4);
+  if (a.N <= 128) return SCAN(16, 8);
   return SCAN(16, 16);
 #undef SCAN
 }
@@ -450,7 +565,10 @@ int scan_any(const ScanArgs& a, cudaStream_t s) {
   if (a.np == 0) return 0;
   if constexpr (!CH && std::is_same<T, __nv_bfloat16>::value)
     if (heads_by_tiles(a)) return launch_heads_by_tiles(a, s);
-  return launch_scan<T, CH>(a, s);
+  // eight elements at a time: rows on 16-byte boundaries, and no group or row of B and C ends inside one
+  const bool wide = a.wide && a.N % 8 == 0 && a.heads / a.groups * a.width % 8 == 0 &&
+                    (!CH || a.dt_f32 || (a.lddt % 8 == 0 && reinterpret_cast<uintptr_t>(a.dt) % 16 == 0));
+  return wide ? launch_scan<T, CH, true>(a, s) : launch_scan<T, CH, false>(a, s);
 }
 
 }  // namespace selective

@@ -13,15 +13,35 @@ __device__ __forceinline__ float exp2_fast(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
   return r;
 }
-// SiLU and softplus: with 16-bit rows through the fast exponential, division and logarithm (relative errors
-// near 1e-6; the logarithm of 1 + e switches to its series where e would be rounded away)
+// SiLU; with 16-bit rows through the fast exponential and division (relative errors near 1e-6)
 template <typename T>
 __device__ __forceinline__ float silu(float x) {
   if constexpr (sizeof(T) == 2) return __fdividef(x, 1.0f + __expf(-x));
   else return x / (1.0f + expf(-x));
 }
+// log(1 + e^z) = max(z, 0) + log(1 + e), e = e^-|z|.  With 16-bit rows log(1 + e) = 2 artanh(s), s = e / (2 + e) <=
+// 1/3, by seven terms of its series (the next one is below 2^-26), and e by the fast power of two of a
+// product in two parts: a step size enters every later state, so it keeps 2^-21 where logarithms of
+// sums near 1 would leave 2^-15 of small ones.
+template <typename T>
 __device__ __forceinline__ float softplus(float z) {
-  return fmaxf(z, 0.0f) + log1pf(expf(-fabsf(z)));
+  const float over = z < 0.0f ? 0.0f : z;
+  if constexpr (sizeof(T) == 2) {
+    const float q = fmaxf(-fabsf(z), -120.0f), p = q * kLog2e;
+    const float low = fmaf(q, 1.925963033e-8f, fmaf(q, kLog2e, -p));
+    float e = exp2_fast(p);
+    e = fmaf(e, 0.69314718f * low, e);
+    const float s = __fdividef(e, 2.0f + e), t = s * s;
+    float f = fmaf(t, 1.0f / 13.0f, 1.0f / 11.0f);
+    f = fmaf(t, f, 1.0f / 9.0f);
+    f = fmaf(t, f, 1.0f / 7.0f);
+    f = fmaf(t, f, 1.0f / 5.0f);
+    f = fmaf(t, f, 1.0f / 3.0f);
+    f = fmaf(t, f, 1.0f);
+    return fmaf(2.0f * s, f, over);
+  } else {
+    return over + log1pf(expf(-fabsf(z)));
+  }
 }
 
 // Rows of the step that belong to a request.
@@ -51,13 +71,18 @@ struct ScanArgs {
   int T, heads, width, N, groups, num_slots, nd, np, dt_f32, softplus, wide;
 };
 
+// The step size that comes of a row's number (NaN stays NaN).
+template <typename T>
+__device__ __forceinline__ float step_from(const ScanArgs& a, float z, float bias) {
+  z += bias;
+  if (a.softplus) z = softplus<T>(z);
+  return z < a.dt_min ? a.dt_min : z > a.dt_max ? a.dt_max : z;
+}
 template <typename T>
 __device__ __forceinline__ float step_size(const ScanArgs& a, long long row, int i) {
   const long long at = row * a.lddt + i;
-  float z = a.dt_f32 ? static_cast<const float*>(a.dt)[at] : to_f32<T>(static_cast<const T*>(a.dt)[at]);
-  if (a.dt_bias != nullptr) z += a.dt_bias[i];
-  if (a.softplus) z = softplus(z);
-  return fminf(fmaxf(z, a.dt_min), a.dt_max);
+  const float z = a.dt_f32 ? static_cast<const float*>(a.dt)[at] : to_f32<T>(static_cast<const T*>(a.dt)[at]);
+  return step_from<T>(a, z, a.dt_bias != nullptr ? a.dt_bias[i] : 0.0f);
 }
 
 // Portions of prompts by products of tiles (selective_heads.cu): rates per head, bf16 rows on 16-byte boundaries.

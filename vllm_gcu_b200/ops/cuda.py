@@ -1573,86 +1573,94 @@ def memory_step(h: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Tens
 # ---------------------------------------------------------------------------
 # state-space mixers (csrc/selective.cu, csrc/group_norm_gate.cu)
 # ---------------------------------------------------------------------------
-def _rows_of(name: str, t: torch.Tensor, rows: int, cols: int, dtypes, device) -> torch.Tensor:
-    """A row-strided view [rows, cols] of one of ``dtypes``, as the state-space kernels take it."""
-    if t.dim() != 2 or tuple(t.shape) != (rows, cols):
+def _row_view(name: str, t: torch.Tensor, rows: int, cols: int, dtypes, dev: int) -> int:
+    """Checks a row-strided view [rows, cols] of one of ``dtypes`` as the state-space kernels take it; its row pitch.
+    (One expression where all is well: a call has up to a dozen tensors, and single tokens take microseconds.)"""
+    ld, step = t.stride() if t.dim() == 2 else (0, 0)
+    if t.shape == (rows, cols) and t.dtype in dtypes and t.get_device() == dev and (step == 1 or cols == 1):
+        return ld
+    if t.shape != (rows, cols):
         raise ValueError(f"{name} has shape {tuple(t.shape)}, not {(rows, cols)}")
     if t.dtype not in dtypes:
         raise ValueError(f"{name} is {t.dtype}, not {' or '.join(map(str, dtypes))}")
-    if t.device != device:
-        raise ValueError(f"{name} is on {t.device}, not on {device}")
-    if cols > 1 and t.stride(1) != 1:
-        raise ValueError(f"{name}: neighbouring columns are {t.stride(1)} elements apart")
-    return t
+    if t.get_device() != dev:
+        raise ValueError(f"{name} is on {t.device}, x is not")
+    raise ValueError(f"{name}: neighbouring columns are {step} elements apart")
 
 
-def _target(t: torch.Tensor, rows: int, cols: int, dtype, device) -> torch.Tensor:
-    """Rows that a kernel writes: as :func:`_rows_of`, and no two of them share elements."""
-    _rows_of("out", t, rows, cols, (dtype,), device)
-    if rows > 1 and t.stride(0) < cols:
-        raise ValueError(f"out: rows of {cols} columns are {t.stride(0)} elements apart")
-    return t
-
-
-def _whole(name: str, t: Optional[torch.Tensor], shape, dtype, device) -> Optional[torch.Tensor]:
-    """A contiguous tensor of a known shape, or None."""
-    if t is None:
-        return None
-    if tuple(t.shape) != tuple(shape) or t.dtype != dtype or not t.is_contiguous() or t.device != device:
-        raise ValueError(f"{name}: a contiguous {dtype} tensor of shape {tuple(shape)} on {device} is wanted, got "
+def _whole(name: str, t: torch.Tensor, shape, dtype, dev: int) -> None:
+    """Checks a contiguous tensor of a known shape."""
+    if t.shape != shape or t.dtype is not dtype or not t.is_contiguous() or t.get_device() != dev:
+        raise ValueError(f"{name}: a contiguous {dtype} tensor of shape {tuple(shape)} beside x is wanted, got "
                          f"{t.dtype}, {tuple(t.shape)}, strides {tuple(t.stride())} on {t.device}")
-    return t
 
 
-def _overlap(a: torch.Tensor, b: Optional[torch.Tensor]) -> bool:
-    """Whether two row-strided views share elements.  Views of equal pitch are told apart by their columns."""
-    if b is None or not a.numel() or not b.numel():
+def _overlap(a: tuple, b: tuple) -> bool:
+    """Whether two row-strided views share elements; a view as (address, row pitch, rows, columns, element size).
+    Views of equal pitch are told apart by their columns."""
+    (pa, la, na, ca, ea), (pb, lb, nb, cb, eb) = a, b
+    if not (na and ca and nb and cb) or pa >= pb + ((nb - 1) * lb + cb) * eb or pb >= pa + ((na - 1) * la + ca) * ea:
         return False
-    reach = lambda t: t.data_ptr() + t.element_size() * (  # noqa: E731
-        1 + sum((n - 1) * st for n, st in zip(t.shape, t.stride())))
-    if a.data_ptr() >= reach(b) or b.data_ptr() >= reach(a):
-        return False
-    if a.dim() == b.dim() == 2 and a.element_size() == b.element_size() and a.stride(0) == b.stride(0):
-        off, ld = (b.data_ptr() - a.data_ptr()) // a.element_size(), a.stride(0)
-        if ld >= a.shape[1] and ld >= b.shape[1]:
-            return off % ld < a.shape[1] or off % ld + b.shape[1] > ld
+    if la == lb and ea == eb and la >= ca and la >= cb:
+        off = (pb - pa) // ea % la
+        return off < ca or off + cb > la
     return True
 
 
-def _step_place(md, T: int, slots_wanted: bool, num_slots: int, write_slots, device):
-    """(single tokens, portions, cu_q, positions, read slots, write slots) of a step, checked."""
-    nd, npf, cu = _scan_place(md)
+def _target(out: torch.Tensor, rows: int, cols: int, dtype, dev: int, inputs, same_is_fine: bool = False
+            ) -> tuple[int, int]:
+    """Checks the rows that a kernel writes: no two of them share elements, and none of them meets an input
+    (``inputs``: name, address or None, row pitch, columns, element size); their address and pitch."""
+    ld, at, es = _row_view("out", out, rows, cols, (dtype,), dev), out.data_ptr(), dtype.itemsize
+    if rows > 1 and ld < cols:
+        raise ValueError(f"out: rows of {cols} columns are {ld} elements apart")
+    end = at + ((rows - 1) * ld + cols) * es
+    for name, p, pitch, width, size in inputs:
+        if p is None or p >= end or p + ((rows - 1) * pitch + width) * size <= at \
+                or same_is_fine and p == at and (pitch == ld or rows == 1):
+            continue
+        if _overlap((at, ld, rows, cols, es), (p, pitch, rows, width, size)):
+            raise ValueError(f"out shares memory with {name}" + (f" and is not {name}" if same_is_fine else ""))
+    return at, ld
+
+
+def _step_place(md, T: int, kept: bool, write_slots: Optional[torch.Tensor], dev: int):
+    """(single tokens, portions, cu_q, positions, read slots, write slots) of a step, checked; addresses."""
+    nd, cu = md.num_decode_tokens, md.cu_q_prefill
+    n = nd
     if not 0 <= nd <= T:
         raise ValueError(f"{nd} single tokens in a step of {T} rows")
     if cu is not None:
-        _whole("md.cu_q_prefill", cu, (npf + 1,), torch.int32, device)
-    if not slots_wanted:
-        return nd, npf, cu, None, None, None
+        if cu.dim() != 1 or cu.shape[0] < 1 or cu.dtype is not torch.int32 or cu.get_device() != dev \
+                or not cu.is_contiguous():
+            raise ValueError("md.cu_q_prefill: int32 offsets beside x are wanted")
+        n += cu.shape[0] - 1
+        cu = cu.data_ptr()
+    if not kept:
+        return nd, n - nd, cu, None, None, None
     pos, slots = md.positions, md.state_slots
     if slots is None:
         raise ValueError("a state needs md.state_slots")
-    if pos.dim() != 1 or pos.shape[0] < T or pos.dtype != torch.int64 or pos.device != device \
+    if pos.dim() != 1 or pos.shape[0] < T or pos.dtype is not torch.int64 or pos.get_device() != dev \
             or not pos.is_contiguous():
-        raise ValueError(f"md.positions: {T} int64 positions on {device} are wanted")
-    write_slots = slots if write_slots is None else write_slots
+        raise ValueError(f"md.positions: {T} int64 positions beside x are wanted")
     for name, t in (("md.state_slots", slots), ("write_slots", write_slots)):
-        if t.dim() != 1 or t.shape[0] < nd + npf or t.dtype != torch.int32 or t.device != device \
-                or not t.is_contiguous():
-            raise ValueError(f"{name}: {nd + npf} int32 slots on {device} are wanted")
-    return nd, npf, cu, pos, slots, write_slots
+        if t is not None and (t.dim() != 1 or t.shape[0] < n or t.dtype is not torch.int32 or t.get_device() != dev
+                              or not t.is_contiguous()):
+            raise ValueError(f"{name}: {n} int32 slots beside x are wanted")
+    slots = slots.data_ptr()
+    return nd, n - nd, cu, pos.data_ptr(), slots, slots if write_slots is None else write_slots.data_ptr()
 
 
-def _on_device(t: torch.Tensor):
-    """Makes the tensor's device the current one for a launch."""
-    if not t.is_cuda:
-        raise ValueError(f"a tensor on a GPU is wanted, not on {t.device}")
-    return torch.cuda.device(t.device)
-
-
-def _wide_rows(*ts: Optional[torch.Tensor]) -> bool:
-    """Whether every row of the views starts on a 16-byte boundary."""
-    return all(t is None or (t.data_ptr() % 16 == 0 and (t.shape[0] <= 1 or t.stride(0) * t.element_size() % 16 == 0))
-               for t in ts)
+def _call_on(dev: int, name: str, *args) -> None:
+    """A launch on the current stream of the tensors' device."""
+    if dev < 0:
+        raise ValueError("tensors on a GPU are wanted")
+    if dev == torch._C._cuda_getDevice():
+        call(name, *args, stream_ptr())
+        return
+    with torch.cuda.device(dev):
+        call(name, *args, stream_ptr())
 
 
 def causal_conv(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor], md,
@@ -1669,30 +1677,32 @@ def causal_conv(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tens
     if x.dim() != 2 or x.dtype not in DTYPE_CODE:
         raise ValueError(f"x: rows of bf16, fp16 or fp32 are wanted, got {x.dtype} of shape {tuple(x.shape)}")
     T, Ch = x.shape
-    dev = x.device
-    taps = weight.shape[0]
+    taps, dtype, dev = weight.shape[0], x.dtype, x.get_device()
     if not 1 <= taps <= 8:
         raise ValueError(f"a convolution of {taps} taps, 1 to 8 are built")
-    if act not in ("silu", None):
+    if act != "silu" and act is not None:
         raise ValueError(f"activation {act!r}: silu or None")
-    _rows_of("x", x, T, Ch, (x.dtype,), dev)
+    ldx = _row_view("x", x, T, Ch, (dtype,), dev)
     _whole("weight", weight, (taps, Ch), torch.float32, dev)
-    _whole("bias", bias, (Ch,), torch.float32, dev)
+    if bias is not None:
+        _whole("bias", bias, (Ch,), torch.float32, dev)
+    slots = 0
     if ring is not None:
-        _whole("ring", ring, (ring.shape[0], taps - 1, Ch), x.dtype, dev)
-    use = ring is not None and taps > 1
-    nd, npf, cu, pos, slots, wslots = _step_place(md, T, use, ring.shape[0] if use else 0, write_slots, dev)
+        slots = ring.shape[0]
+        _whole("ring", ring, (slots, taps - 1, Ch), dtype, dev)
+        if taps == 1:
+            ring = None
+    nd, npf, cu, pos, read, write = _step_place(md, T, ring is not None, write_slots, dev)
+    px, pw, pr, es = x.data_ptr(), weight.data_ptr(), None if ring is None else ring.data_ptr(), dtype.itemsize
     if out is None:
-        out = torch.empty((T, Ch), dtype=x.dtype, device=dev)
-    _target(out, T, Ch, x.dtype, dev)
-    if _overlap(out, x):
-        raise ValueError("out shares memory with x: rows are read by those behind them")
-    ring = ring if use else None
-    wide = Ch % (16 // x.element_size()) == 0 and _wide_rows(x, out, ring) and weight.data_ptr() % 16 == 0
-    with _on_device(x):
-        call("b200_causal_conv", ptr(x), x.stride(0), ptr(weight), taps, ptr(bias), ptr(ring),
-             ring.shape[0] if use else 0, ptr(pos), ptr(slots), ptr(wslots), ptr(cu), ptr(out), out.stride(0), T, Ch,
-             nd, npf, int(act == "silu"), int(wide), DTYPE_CODE[x.dtype], stream_ptr())
+        out = torch.empty((T, Ch), dtype=dtype, device=x.device)
+        po, ldo = out.data_ptr(), Ch
+    else:
+        po, ldo = _target(out, T, Ch, dtype, dev, (("x", px, ldx, Ch, es),))
+    vec = 16 // es
+    wide = Ch % vec == 0 and (px | pw | (pr or 0) | po) % 16 == 0 and (T == 1 or ldx % vec == 0 and ldo % vec == 0)
+    _call_on(dev, "b200_causal_conv", px, ldx, pw, taps, None if bias is None else bias.data_ptr(), pr, slots, pos, read,
+             write, cu, po, ldo, T, Ch, nd, npf, act is not None, wide, DTYPE_CODE[dtype])
     return out
 
 
@@ -1714,11 +1724,11 @@ def selective_scan(x: torch.Tensor, dt: torch.Tensor, b: torch.Tensor, c: torch.
     if x.dim() != 2 or x.dtype not in DTYPE_CODE:
         raise ValueError(f"x: rows of bf16, fp16 or fp32 are wanted, got {x.dtype} of shape {tuple(x.shape)}")
     T, cols = x.shape
-    dev = x.device
+    dtype, dev, f32 = x.dtype, x.get_device(), torch.float32
     channels = a_log.dim() == 2
-    if a_log.dim() not in (1, 2) or a_log.shape[0] < 1 or groups < 1:
+    rates = a_log.shape[0] if channels or a_log.dim() == 1 else 0
+    if rates < 1 or groups < 1:
         raise ValueError(f"a_log of shape {tuple(a_log.shape)}, {groups} groups")
-    rates = a_log.shape[0]
     if cols % rates or channels and cols != rates:
         raise ValueError(f"{cols} columns of x for {rates} rates")
     if b.dim() != 2 or b.shape[1] % groups or rates % groups:
@@ -1726,40 +1736,47 @@ def selective_scan(x: torch.Tensor, dt: torch.Tensor, b: torch.Tensor, c: torch.
     N = b.shape[1] // groups
     if not 1 <= N <= 256:
         raise ValueError(f"a state of {N} numbers per column, 1 to 256 are built")
-    _whole("a_log", a_log, (rates, N) if channels else (rates,), torch.float32, dev)
-    lo, hi = (float(v) for v in dt_limits)
+    lo, hi = dt_limits
     if not lo <= hi:
         raise ValueError(f"dt_limits {dt_limits}")
-    own = (x.dtype,)
-    _rows_of("x", x, T, cols, own, dev)
-    _rows_of("dt", dt, T, rates, (x.dtype, torch.float32), dev)
-    for name, t in (("b", b), ("c", c)):
-        _rows_of(name, t, T, groups * N, own, dev)
-    if z is not None:
-        _rows_of("z", z, T, cols, own, dev)
-    _whole("d", d, (rates,), torch.float32, dev)
-    _whole("dt_bias", dt_bias, (rates,), torch.float32, dev)
+    _whole("a_log", a_log, (rates, N) if channels else (rates,), f32, dev)
+    own = (dtype,)
+    ldx = _row_view("x", x, T, cols, own, dev)
+    lddt = _row_view("dt", dt, T, rates, (dtype, f32), dev)
+    ldb = _row_view("b", b, T, groups * N, own, dev)
+    ldc = _row_view("c", c, T, groups * N, own, dev)
+    ldz = 0 if z is None else _row_view("z", z, T, cols, own, dev)
+    if d is not None:
+        _whole("d", d, (rates,), f32, dev)
+    if dt_bias is not None:
+        _whole("dt_bias", dt_bias, (rates,), f32, dev)
     heads, width = (groups, cols // groups) if channels else (rates, cols // rates)
-    use = state is not None
-    if use:
-        _whole("state", state, (state.shape[0], cols, N) if channels else (state.shape[0], rates, width, N),
-               torch.float32, dev)
-        if state.data_ptr() % 16:
+    slots, ps = 0, None
+    if state is not None:
+        slots, ps = state.shape[0], state.data_ptr()
+        _whole("state", state, (slots, cols, N) if channels else (slots, rates, width, N), f32, dev)
+        if ps % 16:
             raise ValueError("state: it does not start on a 16-byte boundary")
-    nd, npf, cu, pos, slots, wslots = _step_place(md, T, use, state.shape[0] if use else 0, write_slots, dev)
+    nd, npf, cu, pos, read, write = _step_place(md, T, state is not None, write_slots, dev)
+    px, pdt, pb, pc = x.data_ptr(), dt.data_ptr(), b.data_ptr(), c.data_ptr()
+    pz, dt32, es, gn = None if z is None else z.data_ptr(), dt.dtype is f32, dtype.itemsize, groups * N
     if out is None:
-        out = torch.empty((T, cols), dtype=x.dtype, device=dev)
-    _target(out, T, cols, x.dtype, dev)
-    for name, t in (("x", x), ("dt", dt), ("b", b), ("c", c), ("z", z)):
-        if _overlap(out, t):
-            raise ValueError(f"out shares memory with {name}")
-    with _on_device(x):
-        call("b200_selective_scan", ptr(x), x.stride(0), ptr(dt), dt.stride(0), int(dt.dtype == torch.float32),
-             ptr(b), b.stride(0), ptr(c), c.stride(0), ptr(z), z.stride(0) if z is not None else 0, ptr(a_log),
-             int(channels), ptr(d), ptr(dt_bias), int(softplus), lo, hi, ptr(state), state.shape[0] if use else 0,
-             ptr(pos), ptr(slots), ptr(wslots), ptr(cu), ptr(out), out.stride(0), T, heads, width, N, groups, nd,
-             npf, int(_wide_rows(x, b, c, z, out)), DTYPE_CODE[x.dtype], stream_ptr())
+        out = torch.empty((T, cols), dtype=dtype, device=x.device)
+        po, ldo = out.data_ptr(), cols
+    else:
+        po, ldo = _target(out, T, cols, dtype, dev,
+                          (("x", px, ldx, cols, es), ("dt", pdt, lddt, rates, 4 if dt32 else es),
+                           ("b", pb, ldb, gn, es), ("c", pc, ldc, gn, es), ("z", pz, ldz, cols, es)))
+    wide = (px | pb | pc | po | (pz or 0)) % 16 == 0 and (T == 1 or (ldx | ldb | ldc | ldz | ldo) * es % 16 == 0)
+    _call_on(dev, "b200_selective_scan", px, ldx, pdt, lddt, dt32, pb, ldb, pc, ldc, pz, ldz,
+             a_log.data_ptr(), channels, None if d is None else d.data_ptr(),
+             None if dt_bias is None else dt_bias.data_ptr(), softplus, lo, hi, ps, slots, pos, read, write, cu, po, ldo,
+             T, heads, width, N, groups, nd, npf, wide, DTYPE_CODE[dtype])
     return out
+
+
+#: activations of a gate, as the native library numbers them
+GATE_ACT = {None: 0, "silu": 1, "sigmoid": 2}
 
 
 def group_norm_gate(x: torch.Tensor, z: Optional[torch.Tensor], weight: torch.Tensor, groups: int, eps: float,
@@ -1773,29 +1790,28 @@ def group_norm_gate(x: torch.Tensor, z: Optional[torch.Tensor], weight: torch.Te
     if x.dim() != 2 or x.dtype not in DTYPE_CODE:
         raise ValueError(f"x: rows of bf16, fp16 or fp32 are wanted, got {x.dtype} of shape {tuple(x.shape)}")
     T, Ch = x.shape
-    dev = x.device
+    dtype, dev = x.dtype, x.get_device()
     if groups < 1 or Ch % groups:
         raise ValueError(f"{Ch} channels in {groups} groups")
-    if act not in (None, "silu", "sigmoid"):
+    if act not in GATE_ACT:
         raise ValueError(f"activation {act!r}: silu, sigmoid or None")
-    own = (x.dtype,)
-    _rows_of("x", x, T, Ch, own, dev)
-    if z is not None:
-        _rows_of("z", z, T, Ch, own, dev)
+    own = (dtype,)
+    ldx = _row_view("x", x, T, Ch, own, dev)
+    ldz = 0 if z is None else _row_view("z", z, T, Ch, own, dev)
     _whole("weight", weight, (Ch,), torch.float32, dev)
-    _whole("bias", bias, (Ch,), torch.float32, dev)
+    if bias is not None:
+        _whole("bias", bias, (Ch,), torch.float32, dev)
+    px, pz, pw, es = x.data_ptr(), None if z is None else z.data_ptr(), weight.data_ptr(), dtype.itemsize
+    pb = None if bias is None else bias.data_ptr()
     if out is None:
-        out = torch.empty((T, Ch), dtype=x.dtype, device=dev)
-    _target(out, T, Ch, x.dtype, dev)
-    for name, t in (("x", x), ("z", z)):
-        same = t is not None and t.data_ptr() == out.data_ptr() and t.stride(0) == out.stride(0)
-        if not same and _overlap(out, t):
-            raise ValueError(f"out shares memory with {name} and is not {name}")
-    wide = Ch // groups % (16 // x.element_size()) == 0 and _wide_rows(x, z, out, weight[None])
-    with _on_device(x):
-        call("b200_group_norm_gate", ptr(x), x.stride(0), ptr(z), z.stride(0) if z is not None else 0, ptr(weight),
-             ptr(bias), ptr(out), out.stride(0), float(eps), T, Ch, groups, {None: 0, "silu": 1, "sigmoid": 2}[act],
-             int(center), int(gate_after), int(wide), DTYPE_CODE[x.dtype], stream_ptr())
+        out = torch.empty((T, Ch), dtype=dtype, device=x.device)
+        po, ldo = out.data_ptr(), Ch
+    else:
+        po, ldo = _target(out, T, Ch, dtype, dev, (("x", px, ldx, Ch, es), ("z", pz, ldz, Ch, es)), same_is_fine=True)
+    wide = Ch // groups * es % 16 == 0 and (px | (pz or 0) | pw | (pb or 0) | po) % 16 == 0 and \
+        (T == 1 or (ldx | ldz | ldo) * es % 16 == 0)
+    _call_on(dev, "b200_group_norm_gate", px, ldx, pz, ldz, pw, pb, po, ldo, eps, T, Ch, groups, GATE_ACT[act], center,
+             gate_after, wide, DTYPE_CODE[dtype])
     return out
 
 
