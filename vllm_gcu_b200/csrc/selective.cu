@@ -285,55 +285,71 @@ __global__ void __launch_bounds__(128) selective_step_kernel(const ScanArgs a) {
   }
 }
 
-// Portions of prompts, token after token.  A CTA holds the columns of one request that kThreads / LPC lane groups
+// Portions of prompts, token after token.  A CTA holds the columns of one request that kCore / LPC lane groups
 // make: a column's numbers of state lie in the registers of LPC lanes, NPL each, and a token costs a number one
 // decay (rates per channel: a power of two, which the special function unit does 16 of per clock and SM: it bounds
-// them), two multiply-adds and a product.  Inputs pass through shared memory kTok tokens at a time: while a
-// tile is worked on, the next one is on its way to registers, eight neighbouring elements per thread, and a
-// thread finishes the elements that it brought (skip, gate, store).  Each token's sum over the lanes of a column
-// is left for kSum tokens, then lanes trade partial sums so that each ends up with the sums of its own
-// tokens: 3 exchanges for 4 tokens of 4 lanes instead of 8.
+// them), two multiply-adds and a product.  Inputs pass through shared memory kTok tokens at a time.  While the core
+// warps walk tile i, four warps of helpers turn tile i + 1 into step sizes and factors, finish tile i - 1 (skip,
+// gate, store) and copy tile i + 3, each helper the eight neighbouring elements that it copied itself; one
+// barrier per tile.  (Without helpers, all warps doing both in turn, 235 us for 2048 tokens of 8192 channels: what is
+// done per element is half of the instructions, and the chain along the tokens leaves the scheduler idle.)
+// The sums over the lanes of a column are left for kSum tokens, then lanes trade partial sums so that each ends up
+// with the sums of its own tokens: 3 exchanges for 4 tokens of 4 lanes instead of 8.  With few numbers per
+// lane, decays and inputs of the next kSum tokens are made while the chain of the present ones runs.
 template <int LPC>
-constexpr int kScanThreads = LPC == 16 ? 256 : 128;
+constexpr int kCore = LPC == 16 ? 256 : 128;
+constexpr int kHelp = 128;
+template <int LPC, int NPL>
+constexpr int kTok = LPC == 2 || LPC * NPL >= 128 ? 16 : 32;
 
 template <typename T>
 struct __align__(16) Eight {
   T e[8];
 };
-// eight neighbours of a row; `n` of them are there
+// Eight neighbours of a row, `n` of them there, into shared memory, zeros behind them.
 template <typename T, bool WIDE>
-__device__ __forceinline__ Eight<T> load_eight(const T* p, int n) {
-  Eight<T> v;
+__device__ __forceinline__ void copy_eight(Eight<T>* to, const T* from, int n) {
   if (WIDE) {
-    if (n > 0) v = *reinterpret_cast<const Eight<T>*>(p);
-    else
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v.e[i] = from_f32<T>(0.0f);
+    for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i)
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(to) + 16 * i),
+                   "l"(reinterpret_cast<const char*>(from) + 16 * i), "r"(n > 0 ? 16 : 0)
+                   : "memory");
   } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v.e[i] = i < n ? p[i] : from_f32<T>(0.0f);
+    for (int i = 0; i < 8; ++i) to->e[i] = i < n ? from[i] : from_f32<T>(0.0f);
   }
-  return v;
 }
 
+template <typename T, bool CH, int LPC, int NPL>
+struct ScanTile {
+  static constexpr int kTokens = kTok<LPC, NPL>, kCols = kCore<LPC> / LPC, kVecs = kTokens * kCols / 8;
+  // as they are in memory, by the helper that copied them: rows for four tiles, the rest for two
+  Eight<T> x[4][kVecs], z[4][kVecs], bc_raw[2][2 * kTokens * LPC * NPL / 8];
+  Eight<float> dt[2][CH ? kVecs : 1];                        // (rows of 16 bits: the first half)
+  // by tile parity
+  float bc[2][2][kTokens][LPC * NPL];                        // B, C
+  float2 d[2][kTokens][kCols];                               // step size (rates per head: decay), step size times x
+  float y[2][kTokens][kCols + 4];
+};
+
 template <typename T, bool CH, int LPC, int NPL, bool WIDE>
-__global__ void __launch_bounds__(kScanThreads<LPC>) selective_scan_kernel(const ScanArgs a) {
-  constexpr int kThreads = kScanThreads<LPC>, NP = LPC * NPL, kCols = kThreads / LPC, kTok = LPC == 2 || NP > 128 ? 16 : 32;
-  constexpr int kSum = LPC < 8 ? LPC : 8;
-  constexpr int kVecs = kTok * kCols / 8;                    // threads that bring and finish elements
-  constexpr int kParts = (2 * kTok * NP / 8 + kThreads - 1) / kThreads;
-  static_assert(kVecs <= kThreads, "one vector of eight per thread");
-  __shared__ __align__(16) float sbc[2][kTok][NP];           // B, C
-  __shared__ __align__(16) float2 sd[kTok][kCols];           // step size (rates per head: decay), step size times x
-  __shared__ __align__(16) float sy[kTok][kCols + 4];
-  grid_release_small();
+__global__ void __launch_bounds__(kCore<LPC> + kHelp) selective_scan_kernel(const ScanArgs a) {
+  using Tile = ScanTile<T, CH, LPC, NPL>;
+  constexpr int NP = LPC * NPL, kCols = Tile::kCols, TOK = Tile::kTokens;
+  constexpr int kSum = LPC < 8 ? LPC : 8, kHalf = NPL / 2;
+  static_assert(Tile::kVecs <= kHelp, "one vector of eight per helper");
+  extern __shared__ float4 raw[];
+  Tile& sm = *reinterpret_cast<Tile*>(raw);
+  // The next kernel is let go by the ends of the CTAs: CTAs of a next scan that came early would be placed
+  // beside the running ones, several on an SM and none on others (two such passes 427 us each, so 253).
   grid_wait();
   const int r = a.nd + blockIdx.x, g = blockIdx.y, per = a.heads / a.groups * a.width;
-  const int l = threadIdx.x & (LPC - 1), col = threadIdx.x / LPC;
   const int p0 = blockIdx.z * kCols, cols = min(kCols, per - p0);
   const int c0 = g * per + p0;                               // first column of the CTA
   const Portion po = portion_of(r, a.nd, a.cu_q, a.T);
   if (po.first >= po.end) return;
+  const int tiles = (po.end - po.first + TOK - 1) / TOK;
   const int slot = a.state != nullptr ? a.slots[r] : 0;
   T* out = static_cast<T*>(a.out) + c0;
   if (a.state != nullptr && (slot < 0 || slot >= a.num_slots)) {
@@ -341,12 +357,150 @@ __global__ void __launch_bounds__(kScanThreads<LPC>) selective_scan_kernel(const
       if (threadIdx.x < cols) out[t * a.ldo + threadIdx.x] = from_f32<T>(0.0f);
     return;
   }
+
+  if (threadIdx.x >= kCore<LPC>) {
+    // ---------------- helpers ----------------
+    const int me = threadIdx.x - kCore<LPC>;
+    // eight elements of a tile: token vt, columns vc and on; what belongs to a column stays
+    const int vt = me / (kCols / 8), vc = me % (kCols / 8) * 8;
+    const int vn = me < Tile::kVecs ? max(0, min(8, cols - vc)) : 0;
+    const bool one_head = !CH && a.width % 8 == 0;           // eight columns share a step size
+    const T* bsrc = static_cast<const T*>(a.b) + g * a.N;
+    const T* csrc = static_cast<const T*>(a.c) + g * a.N;
+    auto bring = [&](int tile) {
+      if (tile < tiles) {
+        const int t0 = po.first + tile * TOK, n = po.end - t0;
+        if (me < Tile::kVecs) {
+          const int here = vt < n ? vn : 0;
+          const long long t = t0 + (here > 0 ? vt : 0);
+          const int c = c0 + (here > 0 ? vc : 0);
+          copy_eight<T, WIDE>(&sm.x[tile & 3][me], static_cast<const T*>(a.x) + t * a.ldx + c, here);
+          if (a.z != nullptr) copy_eight<T, WIDE>(&sm.z[tile & 3][me], static_cast<const T*>(a.z) + t * a.ldz + c, here);
+          if (CH) {
+            Eight<float>* to = &sm.dt[tile & 1][me];
+            if (a.dt_f32) copy_eight<float, WIDE>(to, static_cast<const float*>(a.dt) + t * a.lddt + c, here);
+            else copy_eight<T, WIDE>(reinterpret_cast<Eight<T>*>(to), static_cast<const T*>(a.dt) + t * a.lddt + c, here);
+          }
+        }
+        for (int e = me; e < 2 * TOK * NP / 8; e += kHelp) {
+          const int m = e / (TOK * NP / 8), k = e / (NP / 8) % TOK, c = e % (NP / 8) * 8;
+          const int here = k < n ? max(0, min(8, a.N - c)) : 0;
+          copy_eight<T, WIDE>(&sm.bc_raw[tile & 1][e], (m == 0 ? bsrc : csrc) + (t0 + (here > 0 ? k : 0)) *
+                              (m == 0 ? a.ldb : a.ldc) + (here > 0 ? c : 0), here);
+        }
+      }
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    bring(0);
+    bring(1);
+    float2 bias[4], skip[4];
+    float hrate[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int which = CH ? c0 + vc + i : (c0 + vc + i) / a.width;
+      const bool in = i < vn;
+      (i & 1 ? bias[i / 2].y : bias[i / 2].x) = in && a.dt_bias != nullptr ? a.dt_bias[which] : 0.0f;
+      (i & 1 ? skip[i / 2].y : skip[i / 2].x) = in && a.d != nullptr ? a.d[which] : 0.0f;
+      hrate[i] = !CH && in ? -expf(a.a_log[which]) : 0.0f;
+    }
+    // step sizes and factors; a token behind the portion has a step of 0, which leaves a state as it is
+    auto convert = [&](int tile) {
+      const int t0 = po.first + tile * TOK, here = vt < po.end - t0 ? vn : 0;
+      if (me < Tile::kVecs) {
+        const Eight<T> x = sm.x[tile & 3][me];
+        float2 dt[4], decay[4];
+        if (CH) {
+          const Eight<float>* from = &sm.dt[tile & 1][me];
+          float f[8];
+          if (a.dt_f32) {
+            const Eight<float> v = *from;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) f[i] = v.e[i];
+          } else {
+            const Eight<T> v = *reinterpret_cast<const Eight<T>*>(from);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) f[i] = to_f32<T>(v.e[i]);
+          }
+#pragma unroll
+          for (int i = 0; i < 4; ++i) decay[i] = dt[i] = step_from<T>(a, make_float2(f[2 * i], f[2 * i + 1]), bias[i]);
+        } else {
+          float step = 0.0f, e = 1.0f;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            if (i < here && (i == 0 || !one_head)) {
+              step = step_size<T>(a, t0 + vt, (c0 + vc + i) / a.width);
+              e = expf(step * hrate[i]);
+            }
+            (i & 1 ? dt[i / 2].y : dt[i / 2].x) = step;
+            (i & 1 ? decay[i / 2].y : decay[i / 2].x) = e;
+          }
+        }
+        float2* to = &sm.d[tile & 1][vt][vc];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float none = CH ? 0.0f : 1.0f;
+          const float2 dx = __fmul2_rn(dt[i], make_float2(to_f32<T>(x.e[2 * i]), to_f32<T>(x.e[2 * i + 1])));
+          *reinterpret_cast<float4*>(to + 2 * i) =
+              make_float4(2 * i < here ? decay[i].x : none, 2 * i < here ? dx.x : 0.0f,
+                          2 * i + 1 < here ? decay[i].y : none, 2 * i + 1 < here ? dx.y : 0.0f);
+        }
+      }
+      for (int e = me; e < 2 * TOK * NP / 8; e += kHelp) {
+        const Eight<T> v = sm.bc_raw[tile & 1][e];
+        float* to = &sm.bc[tile & 1][0][0][0] + e * 8;
+#pragma unroll
+        for (int k = 0; k < 8; k += 4)
+          *reinterpret_cast<float4*>(to + k) =
+              make_float4(to_f32<T>(v.e[k]), to_f32<T>(v.e[k + 1]), to_f32<T>(v.e[k + 2]), to_f32<T>(v.e[k + 3]));
+      }
+    };
+    auto finish = [&](int tile) {
+      const int t0 = po.first + tile * TOK, here = vt < po.end - t0 ? vn : 0;
+      if (here <= 0) return;
+      const Eight<T> x = sm.x[tile & 3][me];
+      Eight<T> z, y;
+      if (a.z != nullptr) z = sm.z[tile & 3][me];
+      const float4* from = reinterpret_cast<const float4*>(&sm.y[tile & 1][vt][vc]);
+      const float4 q0 = from[0], q1 = from[1];
+      const float q[8] = {q0.x, q0.y, q0.z, q0.w, q1.x, q1.y, q1.z, q1.w};
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        float f = fmaf(i & 1 ? skip[i / 2].y : skip[i / 2].x, to_f32<T>(x.e[i]), q[i]);
+        if (a.z != nullptr) f *= silu<T>(to_f32<T>(z.e[i]));
+        y.e[i] = from_f32<T>(f);
+      }
+      T* to = out + static_cast<long long>(t0 + vt) * a.ldo + vc;
+      if (WIDE) {
+        *reinterpret_cast<Eight<T>*>(to) = y;
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (i < here) to[i] = y.e[i];
+      }
+    };
+    asm volatile("cp.async.wait_group 1;" ::: "memory");
+    convert(0);
+    bring(2);
+    __syncthreads();
+    for (int i = 0; i < tiles; ++i) {
+      asm volatile("cp.async.wait_group 1;" ::: "memory");
+      if (i + 1 < tiles) convert(i + 1);
+      if (i > 0) finish(i - 1);
+      bring(i + 3);
+      __syncthreads();
+    }
+    finish(tiles - 1);
+    return;
+  }
+
+  // ---------------- core ----------------
+  const int l = threadIdx.x & (LPC - 1), col = threadIdx.x / LPC;
   const bool old = a.state != nullptr && a.positions[po.first] != 0;
   const int ws = a.state != nullptr ? a.wslots[r] : -1;
   const bool keep = ws >= 0 && ws < a.num_slots;
   const long long pitch = static_cast<long long>(a.heads) * a.width * a.N;
   const long long at = static_cast<long long>(c0 + col) * a.N;
-  float2 h[NPL / 2], rate[NPL / 2];
+  float2 h[kHalf], rate[kHalf];
   auto number = [&](int i) { return (i / 4 * LPC + l) * 4 + i % 4; };
 #pragma unroll
   for (int i = 0; i < NPL; ++i) {
@@ -357,108 +511,46 @@ __global__ void __launch_bounds__(kScanThreads<LPC>) selective_scan_kernel(const
     (i & 1 ? h[i / 2].y : h[i / 2].x) = v;
     (i & 1 ? rate[i / 2].y : rate[i / 2].x) = q;
   }
-
-  // this thread's eight elements of a tile: token vt, columns vc and on; what belongs to a column stays
-  const int vt = threadIdx.x / (kCols / 8), vc = threadIdx.x % (kCols / 8) * 8;
-  const int vn = threadIdx.x < kVecs ? max(0, min(8, cols - vc)) : 0;
-  const bool one_head = !CH && a.width % 8 == 0;             // eight columns share a step size
-  float bias[8], skip[8], hrate[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int which = CH ? c0 + vc + i : (c0 + vc + i) / a.width;
-    const bool in = i < vn;
-    bias[i] = in && a.dt_bias != nullptr ? a.dt_bias[which] : 0.0f;
-    skip[i] = in && a.d != nullptr ? a.d[which] : 0.0f;
-    hrate[i] = !CH && in ? -expf(a.a_log[which]) : 0.0f;
-  }
-  Eight<T> x, z, dth, bc[kParts];
-  Eight<float> dtf;
-  auto bring = [&](int t0) {
-    const int n = po.end - t0;
-    const int here = vt < n ? vn : 0;
-    const long long t = t0 + vt;
-    const int which = CH ? c0 + vc : (c0 + vc) / a.width;
-    x = load_eight<T, WIDE>(static_cast<const T*>(a.x) + t * a.ldx + c0 + vc, here);
-    if (a.z != nullptr) z = load_eight<T, WIDE>(static_cast<const T*>(a.z) + t * a.ldz + c0 + vc, here);
-    if (CH) {
-      if (a.dt_f32) dtf = load_eight<float, false>(static_cast<const float*>(a.dt) + t * a.lddt + which, here);
-      else dth = load_eight<T, WIDE>(static_cast<const T*>(a.dt) + t * a.lddt + which, here);
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        if (i > 0 && one_head) break;
-        if (i >= here) break;
-        const long long k = t * a.lddt + (c0 + vc + i) / a.width;
-        if (a.dt_f32) dtf.e[i] = static_cast<const float*>(a.dt)[k];
-        else dth.e[i] = static_cast<const T*>(a.dt)[k];
-      }
-    }
-#pragma unroll
-    for (int i = 0; i < kParts; ++i) {
-      const int e = threadIdx.x + i * kThreads;
-      const int m = e / (kTok * NP / 8), k = e / (NP / 8) % kTok, c = e % (NP / 8) * 8;
-      const T* row = m == 0 ? static_cast<const T*>(a.b) + (t0 + k) * a.ldb : static_cast<const T*>(a.c) + (t0 + k) * a.ldc;
-      bc[i] = load_eight<T, WIDE>(row + g * a.N + c, m < 2 && k < n ? max(0, min(8, a.N - c)) : 0);
-    }
+  constexpr int kE = CH ? kHalf : 1;
+  struct Ahead {                                             // decays and inputs of kSum tokens
+    float2 e[kSum][kE], u[kSum][kHalf];
   };
-  bring(po.first);
-
-  for (int t0 = po.first; t0 < po.end; t0 += kTok) {
-    // registers -> shared memory; a token behind the portion has a step of 0, which leaves a state as it is
-    const bool here = vt < po.end - t0 && threadIdx.x < kVecs;
-    if (threadIdx.x < kVecs) {
-      float dt = 0.0f, decay = 1.0f;
+  __syncthreads();
+  for (int tile = 0; tile < tiles; ++tile) {
+    const float2* sd = &sm.d[tile & 1][0][col];
+    const float* sb = &sm.bc[tile & 1][0][0][4 * l];
+    const float* sc = &sm.bc[tile & 1][1][0][4 * l];
+    auto token_ahead = [&](int t, float2 (&e)[kE], float2 (&u)[kHalf]) {
+      const float2 dd = sd[t * kCols];
+      const float2 dx = make_float2(dd.y, dd.y), step = make_float2(dd.x, dd.x);
+      if (!CH) e[0] = step;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        if (here && i < vn && (i == 0 || !one_head)) {
-          dt = step_from<T>(a, a.dt_f32 ? dtf.e[i] : to_f32<T>(dth.e[i]), bias[i]);
-          if (!CH) decay = expf(dt * hrate[i]);
-        }
-        const bool in = here && i < vn;
-        sd[vt][vc + i] = in ? make_float2(CH ? dt : decay, dt * to_f32<T>(x.e[i])) : make_float2(CH ? 0.0f : 1.0f, 0.0f);
-      }
-    }
+      for (int k = 0; k < kHalf; k += 2) {
+        const float4 b = *reinterpret_cast<const float4*>(sb + t * NP + k / 2 * LPC * 4);
+        u[k] = __fmul2_rn(dx, make_float2(b.x, b.y));
+        u[k + 1] = __fmul2_rn(dx, make_float2(b.z, b.w));
+        if (CH) {
 #pragma unroll
-    for (int i = 0; i < kParts; ++i) {
-      const int e = threadIdx.x + i * kThreads;
-      if (e < 2 * kTok * NP / 8) {
-        float* to = &sbc[0][0][0] + e * 8;
-#pragma unroll
-        for (int k = 0; k < 8; k += 4)
-          *reinterpret_cast<float4*>(to + k) = make_float4(to_f32<T>(bc[i].e[k]), to_f32<T>(bc[i].e[k + 1]),
-                                                           to_f32<T>(bc[i].e[k + 2]), to_f32<T>(bc[i].e[k + 3]));
-      }
-    }
-    __syncthreads();
-    const Eight<T> xs = x, zs = z;
-    if (t0 + kTok < po.end) bring(t0 + kTok);
-#pragma unroll 1
-    for (int i = 0; i < kTok; i += kSum) {
-      float part[kSum];
-#pragma unroll
-      for (int u = 0; u < kSum; ++u) {
-        const float2 dd = sd[i + u][col];
-        const float2 dx = make_float2(dd.y, dd.y);
-        float2 s = make_float2(0.0f, 0.0f);
-#pragma unroll
-        for (int k = 0; k < NPL / 4; ++k) {
-          const float4 bq = *reinterpret_cast<const float4*>(&sbc[0][i + u][(k * LPC + l) * 4]);
-          const float4 cq = *reinterpret_cast<const float4*>(&sbc[1][i + u][(k * LPC + l) * 4]);
-          const float2 be[2] = {make_float2(bq.x, bq.y), make_float2(bq.z, bq.w)};
-          const float2 ce[2] = {make_float2(cq.x, cq.y), make_float2(cq.z, cq.w)};
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            float2 e = make_float2(dd.x, dd.x);
-            if (CH) {
-              e = __fmul2_rn(e, rate[2 * k + j]);
-              e = make_float2(exp2_fast(e.x), exp2_fast(e.y));
-            }
-            h[2 * k + j] = __ffma2_rn(e, h[2 * k + j], __fmul2_rn(dx, be[j]));
-            s = __ffma2_rn(h[2 * k + j], ce[j], s);
+          for (int j = k; j < k + 2; ++j) {
+            const float2 p = __fmul2_rn(step, rate[j]);
+            e[CH ? j : 0] = make_float2(exp2_fast(p.x), exp2_fast(p.y));
           }
         }
-        part[u] = s.x + s.y;
       }
+    };
+    auto token = [&](int t, const float2 (&e)[kE], const float2 (&u)[kHalf]) {
+      float2 s = make_float2(0.0f, 0.0f);
+#pragma unroll
+      for (int k = 0; k < kHalf; k += 2) {
+        const float4 c = *reinterpret_cast<const float4*>(sc + t * NP + k / 2 * LPC * 4);
+        h[k] = __ffma2_rn(e[CH ? k : 0], h[k], u[k]);
+        h[k + 1] = __ffma2_rn(e[CH ? k + 1 : 0], h[k + 1], u[k + 1]);
+        s = __ffma2_rn(h[k], make_float2(c.x, c.y), s);
+        s = __ffma2_rn(h[k + 1], make_float2(c.z, c.w), s);
+      }
+      return s.x + s.y;
+    };
+    auto sums = [&](int i, float (&part)[kSum]) {
       // lane l of a column gets the sums of token i + l % kSum
 #pragma unroll
       for (int o = kSum / 2; o > 0; o >>= 1) {
@@ -471,26 +563,42 @@ __global__ void __launch_bounds__(kScanThreads<LPC>) selective_scan_kernel(const
       }
 #pragma unroll
       for (int o = kSum; o < LPC; o <<= 1) part[0] += __shfl_xor_sync(0xffffffffu, part[0], o);
-      if (l < kSum) sy[i + l][col] = part[0];
+      if (l < kSum) sm.y[tile & 1][i + l][col] = part[0];
+    };
+    if constexpr (NPL * kSum <= 16) {
+      Ahead even, odd;
+      auto make = [&](int i, Ahead& to) {
+#pragma unroll
+        for (int u = 0; u < kSum; ++u) token_ahead(i + u, to.e[u], to.u[u]);
+      };
+      auto walk = [&](int i, const Ahead& from) {
+        float part[kSum];
+#pragma unroll
+        for (int u = 0; u < kSum; ++u) part[u] = token(i + u, from.e[u], from.u[u]);
+        sums(i, part);
+      };
+      make(0, even);
+#pragma unroll 1
+      for (int i = 0; i < TOK; i += 2 * kSum) {
+        make(i + kSum, odd);
+        walk(i, even);
+        make(i + 2 * kSum < TOK ? i + 2 * kSum : 0, even);   // (behind the last one: not used)
+        walk(i + kSum, odd);
+      }
+    } else {
+#pragma unroll 1
+      for (int i = 0; i < TOK; i += kSum) {
+        float part[kSum];
+#pragma unroll
+        for (int u = 0; u < kSum; ++u) {
+          float2 e[kE], v[kHalf];
+          token_ahead(i + u, e, v);
+          part[u] = token(i + u, e, v);
+        }
+        sums(i, part);
+      }
     }
     __syncthreads();
-    if (here && vn > 0) {
-      Eight<T> y;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        float f = fmaf(skip[i], to_f32<T>(xs.e[i]), sy[vt][vc + i]);
-        if (a.z != nullptr) f *= silu<T>(to_f32<T>(zs.e[i]));
-        y.e[i] = from_f32<T>(f);
-      }
-      T* to = out + static_cast<long long>(t0 + vt) * a.ldo + vc;
-      if (WIDE) {
-        *reinterpret_cast<Eight<T>*>(to) = y;
-      } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-          if (i < vn) to[i] = y.e[i];
-      }
-    }
   }
   if (keep && col < cols) {
 #pragma unroll
@@ -540,20 +648,26 @@ int launch_step(const ScanArgs& a, cudaStream_t s) {
 #undef STEP
 }
 
+template <typename T, bool CH, int LPC, int NPL, bool WIDE>
+int launch_scan(const ScanArgs& a, cudaStream_t s) {
+  constexpr int kCols = kCore<LPC> / LPC, kSmem = sizeof(ScanTile<T, CH, LPC, NPL>);
+  const auto kernel = selective_scan_kernel<T, CH, LPC, NPL, WIDE>;
+  if (kSmem > 48 * 1024) {
+    const int rc = launch_code(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem));
+    if (rc != 0) return rc;
+  }
+  const int per = a.heads / a.groups * a.width;
+  return launch_overlapped(kernel, dim3(a.np, a.groups, (per + kCols - 1) / kCols), dim3(kCore<LPC> + kHelp), kSmem,
+                           s, a);
+}
 template <typename T, bool CH, bool WIDE>
 int launch_scan(const ScanArgs& a, cudaStream_t s) {
-  const int per = a.heads / a.groups * a.width;
-#define SCAN(LPC, NPL)                                                                                     \
-  launch_overlapped(selective_scan_kernel<T, CH, LPC, NPL, WIDE>,                                          \
-                    dim3(a.np, a.groups, (per + kScanThreads<LPC> / LPC - 1) / (kScanThreads<LPC> / LPC)), \
-                    dim3(kScanThreads<LPC>), 0, s, a)
-  if (a.N <= 8) return SCAN(2, 4);
-  if (a.N <= 16) return SCAN(4, 4);
-  if (a.N <= 32) return SCAN(8, 4);
-  if (a.N <= 64) return SCAN(16, 4);
-  if (a.N <= 128) return SCAN(16, 8);
-  return SCAN(16, 16);
-#undef SCAN
+  if (a.N <= 8) return launch_scan<T, CH, 2, 4, WIDE>(a, s);
+  if (a.N <= 16) return launch_scan<T, CH, 4, 4, WIDE>(a, s);
+  if (a.N <= 32) return launch_scan<T, CH, 8, 4, WIDE>(a, s);
+  if (a.N <= 64) return launch_scan<T, CH, 16, 4, WIDE>(a, s);
+  if (a.N <= 128) return launch_scan<T, CH, 16, 8, WIDE>(a, s);
+  return launch_scan<T, CH, 16, 16, WIDE>(a, s);
 }
 
 template <typename T, bool CH>
@@ -567,7 +681,7 @@ int scan_any(const ScanArgs& a, cudaStream_t s) {
     if (heads_by_tiles(a)) return launch_heads_by_tiles(a, s);
   // eight elements at a time: rows on 16-byte boundaries, and no group or row of B and C ends inside one
   const bool wide = a.wide && a.N % 8 == 0 && a.heads / a.groups * a.width % 8 == 0 &&
-                    (!CH || a.dt_f32 || (a.lddt % 8 == 0 && reinterpret_cast<uintptr_t>(a.dt) % 16 == 0));
+                    (!CH || (a.lddt % 8 == 0 && reinterpret_cast<uintptr_t>(a.dt) % 16 == 0));
   return wide ? launch_scan<T, CH, true>(a, s) : launch_scan<T, CH, false>(a, s);
 }
 
