@@ -293,9 +293,9 @@ __global__ void __launch_bounds__(128) selective_step_kernel(const ScanArgs a) {
 // gate, store) and copy tile i + 3, each helper the eight neighbouring elements that it copied itself; one
 // barrier per tile.  (Without helpers, all warps doing both in turn, 235 us for 2048 tokens of 8192 channels: what is
 // done per element is half of the instructions, and the chain along the tokens leaves the scheduler idle.)
-// The sums over the lanes of a column are left for kSum tokens, then lanes trade partial sums so that each ends up
-// with the sums of its own tokens: 3 exchanges for 4 tokens of 4 lanes instead of 8.  With few numbers per
-// lane, decays and inputs of the next kSum tokens are made while the chain of the present ones runs.
+// The sum over the lanes of a column is the helpers': up to four lanes leave a part of it each; where there are
+// more, pairs of lanes trade the parts of two tokens first, so that each ends up with those of its own token.  With
+// few numbers per lane, decays and inputs of the next four tokens are made while the chain of these runs.
 template <int LPC>
 constexpr int kCore = LPC == 16 ? 256 : 128;
 constexpr int kHelp = 128;
@@ -330,14 +330,18 @@ struct ScanTile {
   // by tile parity
   float bc[2][2][kTokens][LPC * NPL];                        // B, C
   float2 d[2][kTokens][kCols];                               // step size (rates per head: decay), step size times x
-  float y[2][kTokens][kCols + 4];
+  static constexpr int kParts = LPC < 4 ? LPC : 4;
+  // Parts of C . h.  A helper reads the parts of eight columns in a row, 128 bytes, and its neighbours those of the next
+  // ones: column c of token t lies in place c ^ key, so that they start in different banks.
+  float y[2][kTokens][kCols][kParts];
+  static __device__ __forceinline__ int key(int t, int c) { return (t * (kCols / 8) + c / 8) & 7; }
 };
 
 template <typename T, bool CH, int LPC, int NPL, bool WIDE>
 __global__ void __launch_bounds__(kCore<LPC> + kHelp) selective_scan_kernel(const ScanArgs a) {
   using Tile = ScanTile<T, CH, LPC, NPL>;
   constexpr int NP = LPC * NPL, kCols = Tile::kCols, TOK = Tile::kTokens;
-  constexpr int kSum = LPC < 8 ? LPC : 8, kHalf = NPL / 2;
+  constexpr int kHalf = NPL / 2;
   static_assert(Tile::kVecs <= kHelp, "one vector of eight per helper");
   extern __shared__ float4 raw[];
   Tile& sm = *reinterpret_cast<Tile*>(raw);
@@ -436,14 +440,22 @@ __global__ void __launch_bounds__(kCore<LPC> + kHelp) selective_scan_kernel(cons
           }
         }
         float2* to = &sm.d[tile & 1][vt][vc];
+        float2 dx[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
+        for (int i = 0; i < 4; ++i)
+          dx[i] = __fmul2_rn(dt[i], make_float2(to_f32<T>(x.e[2 * i]), to_f32<T>(x.e[2 * i + 1])));
+        if (here < 8) {
           const float none = CH ? 0.0f : 1.0f;
-          const float2 dx = __fmul2_rn(dt[i], make_float2(to_f32<T>(x.e[2 * i]), to_f32<T>(x.e[2 * i + 1])));
-          *reinterpret_cast<float4*>(to + 2 * i) =
-              make_float4(2 * i < here ? decay[i].x : none, 2 * i < here ? dx.x : 0.0f,
-                          2 * i + 1 < here ? decay[i].y : none, 2 * i + 1 < here ? dx.y : 0.0f);
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            if (i >= here) {
+              (i & 1 ? decay[i / 2].y : decay[i / 2].x) = none;
+              (i & 1 ? dx[i / 2].y : dx[i / 2].x) = 0.0f;
+            }
         }
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          *reinterpret_cast<float4*>(to + 2 * i) = make_float4(decay[i].x, dx[i].x, decay[i].y, dx[i].y);
       }
       for (int e = me; e < 2 * TOK * NP / 8; e += kHelp) {
         const Eight<T> v = sm.bc_raw[tile & 1][e];
@@ -460,9 +472,18 @@ __global__ void __launch_bounds__(kCore<LPC> + kHelp) selective_scan_kernel(cons
       const Eight<T> x = sm.x[tile & 3][me];
       Eight<T> z, y;
       if (a.z != nullptr) z = sm.z[tile & 3][me];
-      const float4* from = reinterpret_cast<const float4*>(&sm.y[tile & 1][vt][vc]);
-      const float4 q0 = from[0], q1 = from[1];
-      const float q[8] = {q0.x, q0.y, q0.z, q0.w, q1.x, q1.y, q1.z, q1.w};
+      const float* from = sm.y[tile & 1][vt][vc];
+      float q[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        if constexpr (Tile::kParts == 4) {
+          const float4 v = *reinterpret_cast<const float4*>(from + 4 * (i ^ (me & 7)));
+          q[i] = (v.x + v.y) + (v.z + v.w);
+        } else {
+          const float2 v = *reinterpret_cast<const float2*>(from + 2 * (i ^ (me & 7)));
+          q[i] = v.x + v.y;
+        }
+      }
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         float f = fmaf(i & 1 ? skip[i / 2].y : skip[i / 2].x, to_f32<T>(x.e[i]), q[i]);
@@ -512,8 +533,8 @@ __global__ void __launch_bounds__(kCore<LPC> + kHelp) selective_scan_kernel(cons
     (i & 1 ? rate[i / 2].y : rate[i / 2].x) = q;
   }
   constexpr int kE = CH ? kHalf : 1;
-  struct Ahead {                                             // decays and inputs of kSum tokens
-    float2 e[kSum][kE], u[kSum][kHalf];
+  struct Ahead {                                             // decays and inputs of four tokens
+    float2 e[4][kE], u[4][kHalf];
   };
   __syncthreads();
   for (int tile = 0; tile < tiles; ++tile) {
@@ -550,52 +571,62 @@ __global__ void __launch_bounds__(kCore<LPC> + kHelp) selective_scan_kernel(cons
       }
       return s.x + s.y;
     };
-    auto sums = [&](int i, float (&part)[kSum]) {
-      // lane l of a column gets the sums of token i + l % kSum
+    auto leave = [&](int i, float (&part)[4]) {              // (i is a multiple of 4: no part of a key)
+      float(*sy)[kCols][Tile::kParts] = sm.y[tile & 1] + i;
+      if constexpr (LPC <= 4) {
 #pragma unroll
-      for (int o = kSum / 2; o > 0; o >>= 1) {
-        const bool up = l & o;
+        for (int u = 0; u < 4; ++u) sy[u][col ^ Tile::key(u, col)][l] = part[u];
+      } else {
+        // round by round, the lanes of a column part by one bit of l, and the tokens with them
 #pragma unroll
-        for (int u = 0; u < o; ++u) {
-          const float mine = up ? part[u + o] : part[u], theirs = up ? part[u] : part[u + o];
-          part[u] = mine + __shfl_xor_sync(0xffffffffu, theirs, o);
+        for (int o = LPC / 2; o >= 4; o >>= 1) {
+          const bool up = l & o;
+#pragma unroll
+          for (int u = 0; u < 16 / LPC * (o / 4); ++u) {
+            const int half = 16 / LPC * (o / 4);
+            const float mine = up ? part[u + half] : part[u], theirs = up ? part[u] : part[u + half];
+            part[u] = mine + __shfl_xor_sync(0xffffffffu, theirs, o);
+          }
+        }
+        // 16 lanes: token l / 4; 8 lanes: tokens 2 (l / 4) and the next
+#pragma unroll
+        for (int u = 0; u < 16 / LPC; ++u) {
+          const int t = l / 4 * (16 / LPC) + u;
+          sy[t][col ^ Tile::key(t, col)][l & 3] = part[u];
         }
       }
-#pragma unroll
-      for (int o = kSum; o < LPC; o <<= 1) part[0] += __shfl_xor_sync(0xffffffffu, part[0], o);
-      if (l < kSum) sm.y[tile & 1][i + l][col] = part[0];
     };
-    if constexpr (NPL * kSum <= 16) {
+    auto make = [&](int i, Ahead& to) {
+#pragma unroll
+      for (int u = 0; u < 4; ++u) token_ahead(i + u, to.e[u], to.u[u]);
+    };
+    auto walk = [&](int i, const Ahead& from) {
+      float part[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) part[u] = token(i + u, from.e[u], from.u[u]);
+      leave(i, part);
+    };
+    if constexpr (NPL == 4) {
       Ahead even, odd;
-      auto make = [&](int i, Ahead& to) {
-#pragma unroll
-        for (int u = 0; u < kSum; ++u) token_ahead(i + u, to.e[u], to.u[u]);
-      };
-      auto walk = [&](int i, const Ahead& from) {
-        float part[kSum];
-#pragma unroll
-        for (int u = 0; u < kSum; ++u) part[u] = token(i + u, from.e[u], from.u[u]);
-        sums(i, part);
-      };
       make(0, even);
 #pragma unroll 1
-      for (int i = 0; i < TOK; i += 2 * kSum) {
-        make(i + kSum, odd);
+      for (int i = 0; i < TOK; i += 8) {
+        make(i + 4, odd);
         walk(i, even);
-        make(i + 2 * kSum < TOK ? i + 2 * kSum : 0, even);   // (behind the last one: not used)
-        walk(i + kSum, odd);
+        make(i + 8 < TOK ? i + 8 : 0, even);                 // (behind the last one: not used)
+        walk(i + 4, odd);
       }
     } else {
 #pragma unroll 1
-      for (int i = 0; i < TOK; i += kSum) {
-        float part[kSum];
+      for (int i = 0; i < TOK; i += 4) {
+        float part[4];
 #pragma unroll
-        for (int u = 0; u < kSum; ++u) {
+        for (int u = 0; u < 4; ++u) {
           float2 e[kE], v[kHalf];
           token_ahead(i + u, e, v);
           part[u] = token(i + u, e, v);
         }
-        sums(i, part);
+        leave(i, part);
       }
     }
     __syncthreads();
@@ -728,6 +759,7 @@ B200_API int b200_selective_scan(const void* x, long long ldx, const void* dt, l
   a.dt_min = dt_min; a.dt_max = dt_max; a.T = T; a.heads = heads; a.width = width; a.N = N; a.groups = groups;
   a.num_slots = num_slots; a.nd = nd; a.np = np; a.dt_f32 = dt_f32; a.softplus = softplus;
   a.wide = wide;
+  a.limits = dt_max < INFINITY || dt_min > 0.0f || !softplus;    // (a softplus is not below 0)
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   switch (dtype) {
     case 0: return per_channel ? scan_any<__nv_bfloat16, true>(a, s) : scan_any<__nv_bfloat16, false>(a, s);

@@ -13,10 +13,15 @@ __device__ __forceinline__ float exp2_fast(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
   return r;
 }
+__device__ __forceinline__ float rcp_fast(float x) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
 // SiLU; with 16-bit rows through the fast exponential and division (relative errors near 1e-6)
 template <typename T>
 __device__ __forceinline__ float silu(float x) {
-  if constexpr (sizeof(T) == 2) return __fdividef(x, 1.0f + __expf(-x));
+  if constexpr (sizeof(T) == 2) return x * rcp_fast(1.0f + exp2_fast(-kLog2e * x));
   else return x / (1.0f + expf(-x));
 }
 // log(1 + e^z) = max(z, 0) + log(1 + e), e = e^-|z|.  With 16-bit rows log(1 + e) = e P(e), P of degree 9
@@ -68,11 +73,12 @@ struct ScanArgs {
   const int* cu_q;
   long long ldx, lddt, ldb, ldc, ldz, ldo;
   float dt_min, dt_max;
-  int T, heads, width, N, groups, num_slots, nd, np, dt_f32, softplus, wide;
+  int T, heads, width, N, groups, num_slots, nd, np, dt_f32, softplus, limits, wide;
 };
 
 // Step sizes that come of rows' numbers (NaN stays NaN).
 __device__ __forceinline__ float limited(const ScanArgs& a, float z) {
+  if (!a.limits) return z;
   return z < a.dt_min ? a.dt_min : z > a.dt_max ? a.dt_max : z;
 }
 template <typename T>
