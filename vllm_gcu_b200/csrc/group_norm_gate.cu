@@ -5,7 +5,9 @@
 //
 // A part of a row is a problem of its own: rows * groups of them.  A team of threads (one warp up to 1024
 // elements, a CTA above) holds its part in registers, NI vectors of V elements per thread, so that mean and
-// variance are two passes over registers and memory is read once; wider parts are read again.  Bytes bound it.
+// variance are two passes over registers and memory is read once; wider parts are read again.  Bytes bound it:
+// weights come from L1 in 16 bytes, and nothing branches per element (teams that walked rows of one group, to keep its
+// weights and have a row under way, had registers for too few of them: 8192 rows of 8 x 1024 in 297 us).
 #include "common.cuh"
 
 namespace b200 {
@@ -21,16 +23,35 @@ struct Args {
   float eps;
   int T, C, groups, width;   // width: C / groups
   int act, center, after;
+  int parts;                 // T * groups
 };
 
-// fp32 forms for 16-bit rows: the fast exponential and division, relative errors near 1e-6
+// fp32 forms for 16-bit rows: the fast exponential and division, relative errors near 1e-6.  (Selects, no
+// branches: `act` is the same for all.)
 template <typename T>
 __device__ __forceinline__ float activate(float v, int act) {
-  if (act == kNone) return v;
   float s;
-  if constexpr (sizeof(T) == 2) s = __fdividef(1.0f, 1.0f + __expf(-v));
-  else s = 1.0f / (1.0f + expf(-v));
-  return act == kSilu ? v * s : s;
+  if constexpr (sizeof(T) == 2) {
+    float e;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(-1.4426950408889634f * v));
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(s) : "f"(1.0f + e));
+  } else s = 1.0f / (1.0f + expf(-v));
+  return (act == kSigmoid ? 1.0f : v) * (act == kNone ? 1.0f : s);
+}
+enum Gate : int { kNoGate = 0, kBefore = 1, kAfter = 2 };
+
+// V floats of a weight or bias
+template <int V>
+__device__ __forceinline__ void floats(const float* from, float (&to)[V]) {
+  if constexpr (V == 1) {
+    to[0] = from[0];
+  } else {
+#pragma unroll
+    for (int v = 0; v < V; v += 4) {
+      const float4 f = *reinterpret_cast<const float4*>(from + v);
+      to[v] = f.x; to[v + 1] = f.y; to[v + 2] = f.z; to[v + 3] = f.w;
+    }
+  }
 }
 
 template <typename T, int V>
@@ -57,73 +78,79 @@ __device__ __forceinline__ float team_sum(float v, float* red) {
   else return block_sum(v, red);
 }
 
-template <typename T, int V, int NI, int TEAM>
+template <typename T, int V, int NI, int TEAM, int GATE>
 __global__ void __launch_bounds__(TEAM == 32 ? 128 : TEAM) group_norm_gate_kernel(const Args a) {
   __shared__ float red[32];
   using R = Raw<T, V>;
   grid_release_small();
   grid_wait();
   const int lane = TEAM == 32 ? threadIdx.x & 31 : threadIdx.x;
-  const long long part = TEAM == 32 ? static_cast<long long>(blockIdx.x) * 4 + (threadIdx.x >> 5) : blockIdx.x;
-  if (part >= static_cast<long long>(a.T) * a.groups) return;     // (a whole team)
+  const int part = TEAM == 32 ? static_cast<int>(blockIdx.x) * 4 + (threadIdx.x >> 5) : blockIdx.x;
+  if (part >= a.parts) return;                   // (a whole team)
   const long long t = part / a.groups;
-  const int c0 = static_cast<int>(part % a.groups) * a.width;
+  const int c0 = part % a.groups * a.width;
   const T* x = static_cast<const T*>(a.x) + t * a.ldx + c0;
-  const T* z = a.z != nullptr ? static_cast<const T*>(a.z) + t * a.ldz + c0 : nullptr;
+  const T* z = static_cast<const T*>(a.z) + t * a.ldz + c0;
   T* out = static_cast<T*>(a.out) + t * a.ldo + c0;
-  const float* w = a.w + c0;
-  const float* bias = a.bias != nullptr ? a.bias + c0 : nullptr;
-  const bool before = z != nullptr && !a.after, after = z != nullptr && a.after;
-  const float n = static_cast<float>(a.width);
+  const float inv_n = 1.0f / static_cast<float>(a.width);
 
   R rx[NI], rz[NI];
-  float f[NI][V];
 #pragma unroll
   for (int i = 0; i < NI; ++i) {
     const int c = (i * TEAM + lane) * V;
-    if (c < a.width) rx[i] = *reinterpret_cast<const R*>(x + c);
-    if (c < a.width && z != nullptr) rz[i] = *reinterpret_cast<const R*>(z + c);
+    if (c < a.width) {
+      rx[i] = *reinterpret_cast<const R*>(x + c);
+      if (GATE != kNoGate) rz[i] = *reinterpret_cast<const R*>(z + c);
+    }
   }
+  float f[NI][V];
   float sum = 0.0f;
 #pragma unroll
   for (int i = 0; i < NI; ++i) {
-    const bool in = (i * TEAM + lane) * V < a.width;
+    if ((i * TEAM + lane) * V < a.width) {
 #pragma unroll
-    for (int v = 0; v < V; ++v) {
-      f[i][v] = 0.0f;
-      if (in) {
+      for (int v = 0; v < V; ++v) {
         f[i][v] = to_f32<T>(rx[i].e[v]);
-        if (before) f[i][v] *= activate<T>(to_f32<T>(rz[i].e[v]), a.act);
+        if (GATE == kBefore) f[i][v] *= activate<T>(to_f32<T>(rz[i].e[v]), a.act);
+        sum += f[i][v];
       }
-      sum += f[i][v];
     }
   }
-  const float mean = a.center ? team_sum<TEAM>(sum, red) / n : 0.0f;
+  const float mean = a.center ? team_sum<TEAM>(sum, red) * inv_n : 0.0f;
   float ss = 0.0f;
 #pragma unroll
   for (int i = 0; i < NI; ++i) {
-    const bool in = (i * TEAM + lane) * V < a.width;
+    if ((i * TEAM + lane) * V < a.width) {
 #pragma unroll
-    for (int v = 0; v < V; ++v) {
-      f[i][v] -= mean;
-      if (in) ss = fmaf(f[i][v], f[i][v], ss);
+      for (int v = 0; v < V; ++v) {
+        f[i][v] -= mean;
+        ss = fmaf(f[i][v], f[i][v], ss);
+      }
     }
   }
-  const float inv = 1.0f / sqrtf(team_sum<TEAM>(ss, red) / n + a.eps);
+  const float inv = 1.0f / sqrtf(team_sum<TEAM>(ss, red) * inv_n + a.eps);
 #pragma unroll
   for (int i = 0; i < NI; ++i) {
     const int c = (i * TEAM + lane) * V;
-    if (c >= a.width) continue;
-    R y;
+    if (c < a.width) {
+      float w[V], b[V];
+      floats<V>(a.w + c0 + c, w);
+      if (a.bias != nullptr) {
+        floats<V>(a.bias + c0 + c, b);
+      } else {
 #pragma unroll
-    for (int v = 0; v < V; ++v) {
-      float q = f[i][v] * inv * w[c + v];
-      if (bias != nullptr) q += bias[c + v];
-      if (after) q *= activate<T>(to_f32<T>(rz[i].e[v]), a.act);
-      else if (z == nullptr) q = activate<T>(q, a.act);
-      y.e[v] = from_f32<T>(q);
+        for (int v = 0; v < V; ++v) b[v] = 0.0f;
+      }
+      R y;
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        float q = fmaf(f[i][v] * inv, w[v], b[v]);
+        if (GATE == kAfter) q *= activate<T>(to_f32<T>(rz[i].e[v]), a.act);
+        else if (GATE == kNoGate) q = activate<T>(q, a.act);
+        y.e[v] = from_f32<T>(q);
+      }
+      *reinterpret_cast<R*>(out + c) = y;
     }
-    *reinterpret_cast<R*>(out + c) = y;
   }
 }
 
@@ -166,23 +193,25 @@ __global__ void __launch_bounds__(1024) group_norm_gate_wide_kernel(const Args a
   }
 }
 
+template <typename T, int V, int NI, int TEAM>
+int launch(const Args& a, cudaStream_t s) {
+  constexpr int kPer = TEAM == 32 ? 4 : 1;
+  const dim3 grid((a.parts + kPer - 1) / kPer), cta(TEAM * kPer);
+  if (a.z == nullptr) return launch_overlapped(group_norm_gate_kernel<T, V, NI, TEAM, kNoGate>, grid, cta, 0, s, a);
+  if (a.after) return launch_overlapped(group_norm_gate_kernel<T, V, NI, TEAM, kAfter>, grid, cta, 0, s, a);
+  return launch_overlapped(group_norm_gate_kernel<T, V, NI, TEAM, kBefore>, grid, cta, 0, s, a);
+}
 template <typename T, int V>
 int launch(const Args& a, cudaStream_t s) {
-  const long long parts = static_cast<long long>(a.T) * a.groups;
   const int vecs = (a.width + V - 1) / V;
-  if (parts > 0x7fffffffll) return -8;
-#define WARP(NI) launch_overlapped(group_norm_gate_kernel<T, V, NI, 32>, dim3((parts + 3) / 4), dim3(128), 0, s, a)
-#define CTA(NI, TEAM) launch_overlapped(group_norm_gate_kernel<T, V, NI, TEAM>, dim3(parts), dim3(TEAM), 0, s, a)
-  if (vecs <= 32) return WARP(1);
-  if (vecs <= 64) return WARP(2);
-  if (vecs <= 128) return WARP(4);
-  if (vecs <= 256) return CTA(2, 128);
-  if (vecs <= 512) return CTA(2, 256);
-  if (vecs <= 1024) return CTA(4, 256);
-  if (vecs <= 2048) return CTA(4, 512);
-  return launch_overlapped(group_norm_gate_wide_kernel<T>, dim3(parts), dim3(1024), 0, s, a);
-#undef WARP
-#undef CTA
+  if (vecs <= 32) return launch<T, V, 1, 32>(a, s);
+  if (vecs <= 64) return launch<T, V, 2, 32>(a, s);
+  if (vecs <= 128) return launch<T, V, 4, 32>(a, s);
+  if (vecs <= 256) return launch<T, V, 2, 128>(a, s);
+  if (vecs <= 512) return launch<T, V, 2, 256>(a, s);
+  if (vecs <= 1024) return launch<T, V, 2, 512>(a, s);
+  if (vecs <= 2048) return launch<T, V, 4, 512>(a, s);
+  return launch_overlapped(group_norm_gate_wide_kernel<T>, dim3(a.parts), dim3(1024), 0, s, a);
 }
 template <typename T>
 int launch_any(const Args& a, bool wide, cudaStream_t s) {
@@ -199,8 +228,10 @@ B200_API int b200_group_norm_gate(const void* x, long long ldx, const void* z, l
                                   int act, int center, int after, int wide, int dtype, void* stream) {
   using namespace b200::gated_norm;
   if (T <= 0 || C <= 0) return 0;
-  if (groups <= 0 || C % groups != 0) return -8;
-  Args a{x, z, out, w, bias, ldx, ldz, ldo, eps, T, C, groups, C / groups, act, center, after};
+  const long long parts = static_cast<long long>(T) * groups;
+  if (groups <= 0 || C % groups != 0 || parts > 0x7fffffffll) return -8;
+  const Args a{x, z, out, w, bias, ldx, ldz, ldo, eps, T, C, groups, C / groups, act, center, after,
+               static_cast<int>(parts)};
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   switch (dtype) {
     case 0: return launch_any<__nv_bfloat16>(a, wide, s);

@@ -97,18 +97,30 @@ __global__ void __launch_bounds__(128) causal_conv_kernel(const ConvArgs a) {
   if (c >= a.C) return;
   const T* x = static_cast<const T*>(a.x) + c;
   T* out = static_cast<T*>(a.out) + c;
-  const R* ring = nullptr;
   auto ring_row = [&](int slot, long long pos) {
     return reinterpret_cast<R*>(static_cast<T*>(a.ring) +
                                 (static_cast<long long>(slot) * kBack + pos % kBack) * a.C + c);
   };
   float w[NT][V], b[V];
+  auto floats = [&](const float* from, float (&to)[V]) {
+    if constexpr (V == 1) {
+      to[0] = from[0];
+    } else {
 #pragma unroll
-  for (int j = 0; j < NT; ++j)
+      for (int v = 0; v < V; v += 4) {
+        const float4 f = *reinterpret_cast<const float4*>(from + v);
+        to[v] = f.x; to[v + 1] = f.y; to[v + 2] = f.z; to[v + 3] = f.w;
+      }
+    }
+  };
 #pragma unroll
-    for (int v = 0; v < V; ++v) w[j][v] = a.w[static_cast<long long>(j) * a.C + c + v];
+  for (int j = 0; j < NT; ++j) floats(a.w + static_cast<long long>(j) * a.C + c, w[j]);
+  if (a.bias != nullptr) {
+    floats(a.bias + c, b);
+  } else {
 #pragma unroll
-  for (int v = 0; v < V; ++v) b[v] = a.bias ? a.bias[c + v] : 0.0f;
+    for (int v = 0; v < V; ++v) b[v] = 0.0f;
+  }
 
   int t = lo;
   while (t < hi) {
@@ -153,23 +165,43 @@ __global__ void __launch_bounds__(128) causal_conv_kernel(const ConvArgs a) {
         }
       }
     }
-    for (; t < end; ++t) {
-      const R now = *reinterpret_cast<const R*>(x + t * a.ldx);
+    if (padding) {
+      R none;
+#pragma unroll
+      for (int v = 0; v < V; ++v) none.e[v] = from_f32<T>(0.0f);
+      for (; t < end; ++t) *reinterpret_cast<R*>(out + t * a.ldo) = none;
+      continue;
+    }
+    float f[NT][V];                              // rows of the window, the last one is the token's
+#pragma unroll
+    for (int j = 0; j < kBack; ++j)
+#pragma unroll
+      for (int v = 0; v < V; ++v) f[j][v] = to_f32<T>(old[j].e[v]);
+    auto row = [&](const R& now) {
       R y;
 #pragma unroll
       for (int v = 0; v < V; ++v) {
+        f[kBack][v] = to_f32<T>(now.e[v]);
         float s = b[v];
 #pragma unroll
-        for (int j = 0; j < kBack; ++j) s = fmaf(w[j][v], to_f32<T>(old[j].e[v]), s);
-        s = fmaf(w[kBack][v], to_f32<T>(now.e[v]), s);
+        for (int j = 0; j < NT; ++j) s = fmaf(w[j][v], f[j][v], s);
         if (a.silu) s = silu<T>(s);
-        y.e[v] = from_f32<T>(padding ? 0.0f : s);
+        y.e[v] = from_f32<T>(s);
+#pragma unroll
+        for (int j = 0; j < kBack; ++j) f[j][v] = f[j + 1][v];
       }
       *reinterpret_cast<R*>(out + t * a.ldo) = y;
+    };
+    // kBatch rows under way at a time
+    constexpr int kBatch = 8;
+    for (; t + kBatch <= end; ) {
+      R now[kBatch];
 #pragma unroll
-      for (int j = 0; j + 1 < kBack; ++j) old[j] = old[j + 1];
-      if (kBack > 0) old[kBack > 0 ? kBack - 1 : 0] = now;
+      for (int i = 0; i < kBatch; ++i) now[i] = *reinterpret_cast<const R*>(x + (t + i) * a.ldx);
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i, ++t) row(now[i]);
     }
+    for (; t < end; ++t) row(*reinterpret_cast<const R*>(x + t * a.ldx));
   }
 }
 
@@ -297,7 +329,7 @@ __global__ void __launch_bounds__(128) selective_step_kernel(const ScanArgs a) {
 // more, pairs of lanes trade the parts of two tokens first, so that each ends up with those of its own token.  With
 // few numbers per lane, decays and inputs of the next four tokens are made while the chain of these runs.
 template <int LPC>
-constexpr int kCore = LPC == 16 ? 256 : 128;
+constexpr int kCore = LPC >= 8 ? 256 : 128;
 constexpr int kHelp = 128;
 template <int LPC, int NPL>
 constexpr int kTok = LPC == 2 || LPC * NPL >= 128 ? 16 : 32;
@@ -522,7 +554,8 @@ __global__ void __launch_bounds__(kCore<LPC> + kHelp) selective_scan_kernel(cons
   const long long pitch = static_cast<long long>(a.heads) * a.width * a.N;
   const long long at = static_cast<long long>(c0 + col) * a.N;
   float2 h[kHalf], rate[kHalf];
-  auto number = [&](int i) { return (i / 4 * LPC + l) * 4 + i % 4; };
+  constexpr int kVec = NPL < 4 ? NPL : 4;                    // neighbouring numbers of a lane
+  auto number = [&](int i) { return (i / kVec * LPC + l) * kVec + i % kVec; };
 #pragma unroll
   for (int i = 0; i < NPL; ++i) {
     const int n = number(i);
@@ -539,20 +572,31 @@ __global__ void __launch_bounds__(kCore<LPC> + kHelp) selective_scan_kernel(cons
   __syncthreads();
   for (int tile = 0; tile < tiles; ++tile) {
     const float2* sd = &sm.d[tile & 1][0][col];
-    const float* sb = &sm.bc[tile & 1][0][0][4 * l];
-    const float* sc = &sm.bc[tile & 1][1][0][4 * l];
+    const float* sb = &sm.bc[tile & 1][0][0][kVec * l];
+    const float* sc = &sm.bc[tile & 1][1][0][kVec * l];
+    // numbers 2 k and 2 k + 1 of this lane and, where it has four neighbours, the next two
+    auto load = [&](const float* from, int t, int k, float2& p, float2& q) {
+      from += t * NP + k / 2 * LPC * 4;
+      if constexpr (kVec == 4) {
+        const float4 v = *reinterpret_cast<const float4*>(from);
+        p = make_float2(v.x, v.y);
+        q = make_float2(v.z, v.w);
+      } else {
+        p = *reinterpret_cast<const float2*>(from);
+      }
+    };
     auto token_ahead = [&](int t, float2 (&e)[kE], float2 (&u)[kHalf]) {
       const float2 dd = sd[t * kCols];
       const float2 dx = make_float2(dd.y, dd.y), step = make_float2(dd.x, dd.x);
       if (!CH) e[0] = step;
 #pragma unroll
       for (int k = 0; k < kHalf; k += 2) {
-        const float4 b = *reinterpret_cast<const float4*>(sb + t * NP + k / 2 * LPC * 4);
-        u[k] = __fmul2_rn(dx, make_float2(b.x, b.y));
-        u[k + 1] = __fmul2_rn(dx, make_float2(b.z, b.w));
-        if (CH) {
+        float2 b[2];
+        load(sb, t, k, b[0], b[1]);
 #pragma unroll
-          for (int j = k; j < k + 2; ++j) {
+        for (int j = k; j < k + kVec / 2; ++j) {
+          u[j] = __fmul2_rn(dx, b[j - k]);
+          if (CH) {
             const float2 p = __fmul2_rn(step, rate[j]);
             e[CH ? j : 0] = make_float2(exp2_fast(p.x), exp2_fast(p.y));
           }
@@ -563,11 +607,13 @@ __global__ void __launch_bounds__(kCore<LPC> + kHelp) selective_scan_kernel(cons
       float2 s = make_float2(0.0f, 0.0f);
 #pragma unroll
       for (int k = 0; k < kHalf; k += 2) {
-        const float4 c = *reinterpret_cast<const float4*>(sc + t * NP + k / 2 * LPC * 4);
-        h[k] = __ffma2_rn(e[CH ? k : 0], h[k], u[k]);
-        h[k + 1] = __ffma2_rn(e[CH ? k + 1 : 0], h[k + 1], u[k + 1]);
-        s = __ffma2_rn(h[k], make_float2(c.x, c.y), s);
-        s = __ffma2_rn(h[k + 1], make_float2(c.z, c.w), s);
+        float2 c[2];
+        load(sc, t, k, c[0], c[1]);
+#pragma unroll
+        for (int j = k; j < k + kVec / 2; ++j) {
+          h[j] = __ffma2_rn(e[CH ? j : 0], h[j], u[j]);
+          s = j == 0 ? __fmul2_rn(h[j], c[0]) : __ffma2_rn(h[j], c[j - k], s);
+        }
       }
       return s.x + s.y;
     };
@@ -606,7 +652,7 @@ __global__ void __launch_bounds__(kCore<LPC> + kHelp) selective_scan_kernel(cons
       for (int u = 0; u < 4; ++u) part[u] = token(i + u, from.e[u], from.u[u]);
       leave(i, part);
     };
-    if constexpr (NPL == 4) {
+    if constexpr (NPL <= 4) {
       Ahead even, odd;
       make(0, even);
 #pragma unroll 1
@@ -693,7 +739,7 @@ int launch_scan(const ScanArgs& a, cudaStream_t s) {
 }
 template <typename T, bool CH, bool WIDE>
 int launch_scan(const ScanArgs& a, cudaStream_t s) {
-  if (a.N <= 8) return launch_scan<T, CH, 2, 4, WIDE>(a, s);
+  if (a.N <= 8) return launch_scan<T, CH, 4, 2, WIDE>(a, s);
   if (a.N <= 16) return launch_scan<T, CH, 4, 4, WIDE>(a, s);
   if (a.N <= 32) return launch_scan<T, CH, 8, 4, WIDE>(a, s);
   if (a.N <= 64) return launch_scan<T, CH, 16, 4, WIDE>(a, s);
