@@ -21,25 +21,23 @@
 namespace b200 {
 namespace selective {
 
-// V neighbouring elements: 16 bytes where V > 1
+// V neighbouring elements, in one access where V is 4
 template <typename T, int V>
 struct Raw {
   T e[V];
 };
 template <>
-struct __align__(16) Raw<__nv_bfloat16, 8> {
-  __nv_bfloat16 e[8];
+struct __align__(8) Raw<__nv_bfloat16, 4> {
+  __nv_bfloat16 e[4];
 };
 template <>
-struct __align__(16) Raw<__half, 8> {
-  __half e[8];
+struct __align__(8) Raw<__half, 4> {
+  __half e[4];
 };
 template <>
 struct __align__(16) Raw<float, 4> {
   float e[4];
 };
-template <typename T>
-constexpr int kWide = 16 / sizeof(T);
 
 // ---------------------------------------------------------------------------
 // short causal convolution
@@ -54,18 +52,21 @@ struct ConvArgs {
   const int *slots, *wslots; // [requests], may be null without a ring
   const int* cu_q;
   long long ldx, ldo;
-  int T, C, num_slots, nd, np, silu;
+  int T, C, num_slots, nd, np, silu, strip;
 };
 
 constexpr int kMaxTaps = 8;
-constexpr int kStrip = 16;                       // rows of prompts that a CTA walks
+constexpr int kStrip = 16;                       // rows of prompts that a CTA walks, at least
 static_assert(kStrip >= kMaxTaps, "a row that reads the ring lies in the strip of its portion's first row");
 
 // A CTA: a strip of rows, V channels per thread.  A single token is a strip of its own; strips of
-// prompts are kStrip rows long, but that the first taps - 1 rows of a portion stay in one strip: they
+// prompts are a.strip rows long, but that the first taps - 1 rows of a portion stay in one strip: they
 // are the only ones that read the ring, and the threads that read a channel of it then write it, so
 // reading and writing need no second launch.
-// Bytes bound it: rows are read once (those in front of a strip a second time, from L2) and written once.
+// Bytes bound it: rows are read once (those in front of a strip a second time, from L2) and written once.  Four
+// channels per thread and kBatch rows under way: with eight channels the registers of the window leave 12 warps an
+// SM (8192 rows of 10240 channels 107 us, so 87); strips of 64 rows make the search for a row's request and
+// the window in front of the strip seldom (16 rows: 8 us more).
 template <typename T, int NT, int V>
 __global__ void __launch_bounds__(128) causal_conv_kernel(const ConvArgs a) {
   constexpr int kBack = NT - 1;
@@ -79,8 +80,8 @@ __global__ void __launch_bounds__(128) causal_conv_kernel(const ConvArgs a) {
     lo = req = strip;
     hi = lo + 1;
   } else {
-    lo = a.nd + (strip - a.nd) * kStrip;
-    hi = min(lo + kStrip, a.T);
+    lo = a.nd + (strip - a.nd) * a.strip;
+    hi = min(lo + a.strip, a.T);
     TokenPlace pl = token_place(lo, a.nd, a.np, a.cu_q);
     if (pl.req < 0) return;                      // behind the last portion
     req = pl.req;
@@ -99,7 +100,7 @@ __global__ void __launch_bounds__(128) causal_conv_kernel(const ConvArgs a) {
   T* out = static_cast<T*>(a.out) + c;
   auto ring_row = [&](int slot, long long pos) {
     return reinterpret_cast<R*>(static_cast<T*>(a.ring) +
-                                (static_cast<long long>(slot) * kBack + pos % kBack) * a.C + c);
+                                (static_cast<long long>(slot) * kBack + pos % (kBack > 0 ? kBack : 1)) * a.C + c);
   };
   float w[NT][V], b[V];
   auto floats = [&](const float* from, float (&to)[V]) {
@@ -185,16 +186,14 @@ __global__ void __launch_bounds__(128) causal_conv_kernel(const ConvArgs a) {
         float s = b[v];
 #pragma unroll
         for (int j = 0; j < NT; ++j) s = fmaf(w[j][v], f[j][v], s);
-        if (a.silu) s = silu<T>(s);
-        y.e[v] = from_f32<T>(s);
+        y.e[v] = from_f32<T>(a.silu ? silu<T>(s) : s);
 #pragma unroll
         for (int j = 0; j < kBack; ++j) f[j][v] = f[j + 1][v];
       }
       *reinterpret_cast<R*>(out + t * a.ldo) = y;
     };
-    // kBatch rows under way at a time
     constexpr int kBatch = 8;
-    for (; t + kBatch <= end; ) {
+    while (t + kBatch <= end) {
       R now[kBatch];
 #pragma unroll
       for (int i = 0; i < kBatch; ++i) now[i] = *reinterpret_cast<const R*>(x + (t + i) * a.ldx);
@@ -458,7 +457,20 @@ __global__ void __launch_bounds__(kCore<LPC> + kHelp) selective_scan_kernel(cons
             for (int i = 0; i < 8; ++i) f[i] = to_f32<T>(v.e[i]);
           }
 #pragma unroll
-          for (int i = 0; i < 4; ++i) decay[i] = dt[i] = step_from<T>(a, make_float2(f[2 * i], f[2 * i + 1]), bias[i]);
+          for (int i = 0; i < 4; ++i) dt[i] = make_float2(f[2 * i] + bias[i].x, f[2 * i + 1] + bias[i].y);
+          if (a.softplus) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              if constexpr (sizeof(T) == 2) dt[i] = softplus_pair(dt[i]);
+              else dt[i] = make_float2(softplus<T>(dt[i].x), softplus<T>(dt[i].y));
+            }
+          }
+          if (a.limits) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) dt[i] = make_float2(limited(a, dt[i].x), limited(a, dt[i].y));
+          }
+#pragma unroll
+          for (int i = 0; i < 4; ++i) decay[i] = dt[i];
         } else {
           float step = 0.0f, e = 1.0f;
 #pragma unroll
@@ -517,11 +529,13 @@ __global__ void __launch_bounds__(kCore<LPC> + kHelp) selective_scan_kernel(cons
         }
       }
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        float f = fmaf(i & 1 ? skip[i / 2].y : skip[i / 2].x, to_f32<T>(x.e[i]), q[i]);
-        if (a.z != nullptr) f *= silu<T>(to_f32<T>(z.e[i]));
-        y.e[i] = from_f32<T>(f);
+      for (int i = 0; i < 8; ++i) q[i] = fmaf(i & 1 ? skip[i / 2].y : skip[i / 2].x, to_f32<T>(x.e[i]), q[i]);
+      if (a.z != nullptr) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) q[i] *= silu<T>(to_f32<T>(z.e[i]));
       }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) y.e[i] = from_f32<T>(q[i]);
       T* to = out + static_cast<long long>(t0 + vt) * a.ldo + vc;
       if (WIDE) {
         *reinterpret_cast<Eight<T>*>(to) = y;
@@ -688,9 +702,12 @@ __global__ void __launch_bounds__(kCore<LPC> + kHelp) selective_scan_kernel(cons
 // host side
 // ---------------------------------------------------------------------------
 template <typename T, int V>
-int launch_conv(const ConvArgs& a, int taps, cudaStream_t s) {
-  const int prompt = a.np > 0 ? (a.T - a.nd + kStrip - 1) / kStrip : 0;
-  const dim3 grid(a.nd + prompt, (a.C + 128 * V - 1) / (128 * V));
+int launch_conv(ConvArgs a, int taps, cudaStream_t s) {
+  const int blocks = (a.C + 128 * V - 1) / (128 * V), rows = a.np > 0 ? a.T - a.nd : 0;
+  // longer strips while there are four of them per SM
+  a.strip = kStrip;
+  while (a.strip < 64 && static_cast<long long>(rows) * blocks >= 8ll * a.strip * sm_count()) a.strip *= 2;
+  const dim3 grid(a.nd + (rows + a.strip - 1) / a.strip, blocks);
   if (grid.x == 0) return 0;
   switch (taps) {
 #define CONV(n) case n: return launch_overlapped(causal_conv_kernel<T, n, V>, grid, dim3(128), 0, s, a)
@@ -701,7 +718,7 @@ int launch_conv(const ConvArgs& a, int taps, cudaStream_t s) {
 }
 template <typename T>
 int conv_any(const ConvArgs& a, int taps, bool wide, cudaStream_t s) {
-  return wide ? launch_conv<T, kWide<T>>(a, taps, s) : launch_conv<T, 1>(a, taps, s);
+  return wide ? launch_conv<T, 4>(a, taps, s) : launch_conv<T, 1>(a, taps, s);
 }
 
 template <typename T, bool CH>
@@ -765,8 +782,8 @@ int scan_any(const ScanArgs& a, cudaStream_t s) {
 }  // namespace selective
 }  // namespace b200
 
-// Short causal convolution of a step's rows.  dtype: 0 bf16, 1 fp16, 2 fp32; taps 1 .. 8; wide: rows, ring and
-// out may be read 16 bytes at a time.  ring may be null (every portion starts from zeros).
+// Short causal convolution of a step's rows.  dtype: 0 bf16, 1 fp16, 2 fp32; taps 1 .. 8; wide: rows, ring,
+// weights, bias and out may be read four elements at a time.  ring may be null (every portion starts from zeros).
 B200_API int b200_causal_conv(const void* x, long long ldx, const float* w, int taps, const float* bias, void* ring,
                               int num_slots, const long long* positions, const int* slots, const int* wslots,
                               const int* cu_q, void* out, long long ldo, int T, int C, int nd, int np, int silu,

@@ -78,23 +78,13 @@ struct ScanArgs {
 
 // Step sizes that come of rows' numbers (NaN stays NaN).
 __device__ __forceinline__ float limited(const ScanArgs& a, float z) {
-  if (!a.limits) return z;
   return z < a.dt_min ? a.dt_min : z > a.dt_max ? a.dt_max : z;
 }
 template <typename T>
 __device__ __forceinline__ float step_from(const ScanArgs& a, float z, float bias) {
   z += bias;
-  return limited(a, a.softplus ? softplus<T>(z) : z);
-}
-template <typename T>
-__device__ __forceinline__ float2 step_from(const ScanArgs& a, float2 z, float2 bias) {
-  if constexpr (sizeof(T) == 2) {
-    z = make_float2(z.x + bias.x, z.y + bias.y);
-    if (a.softplus) z = softplus_pair(z);
-    return make_float2(limited(a, z.x), limited(a, z.y));
-  } else {
-    return make_float2(step_from<T>(a, z.x, bias.x), step_from<T>(a, z.y, bias.y));
-  }
+  if (a.softplus) z = softplus<T>(z);
+  return a.limits ? limited(a, z) : z;
 }
 template <typename T>
 __device__ __forceinline__ float step_size(const ScanArgs& a, long long row, int i) {

@@ -1699,8 +1699,8 @@ def causal_conv(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tens
         po, ldo = out.data_ptr(), Ch
     else:
         po, ldo = _target(out, T, Ch, dtype, dev, (("x", px, ldx, Ch, es),))
-    pb, vec = None if bias is None else bias.data_ptr(), 16 // es
-    wide = Ch % vec == 0 and (px | pw | (pb or 0) | (pr or 0) | po) % 16 == 0 and (T == 1 or ldx % vec == 0 and ldo % vec == 0)
+    pb = None if bias is None else bias.data_ptr()
+    wide = Ch % 4 == 0 and (px | pw | (pb or 0) | (pr or 0) | po) % 16 == 0 and (T == 1 or (ldx | ldo) % 4 == 0)
     _call_on(dev, "b200_causal_conv", px, ldx, pw, taps, pb, pr, slots, pos, read,
              write, cu, po, ldo, T, Ch, nd, npf, act is not None, wide, DTYPE_CODE[dtype])
     return out
