@@ -18,10 +18,12 @@
 // behind it their bits.  Outside the diagonal 2^(L_i - L_j) is a product of two factors below 1, with L at the row
 // block's start between them: 32 exponentials a row instead of 128.
 //
-// A CTA walks the chunks of 64 columns of one head of one request; 8 warps do the arithmetic between the
+// A CTA walks the chunks of 64 columns of one head of one request; 16 warps do the arithmetic between the
 // products, one warp loads tiles (TMA), one issues the products, one computes step sizes and decays of the
 // chunk after next.  W and M of a chunk are made while the tensor cores do Y2 and S, its state and result while
-// they do the next chunk's G.
+// they do the next chunk's G.  The arithmetic bounds it, by latency: with 8 warps 4096 tokens of 128 heads took
+// 213 us.  Lanes 96 and up have four blocks of M that are not zero where lanes below 32 have one, so their
+// warps make less of W.
 #include "selective.cuh"
 
 namespace b200 {
@@ -56,7 +58,8 @@ enum Bar {
 // columns of tensor memory
 constexpr uint32_t kColG = 0, kColY2 = 128, kColY1 = 256, kColS = 320, kTmem = 512;
 constexpr uint32_t kIdescAMajorMN = 1u << 15;
-constexpr int kThreads = 11 * 32;
+constexpr int kWarps = 16;                             // of arithmetic: four per 32 lanes of tensor memory
+constexpr int kThreads = (kWarps + 3) * 32;
 
 __device__ __forceinline__ float2 mul2(float2 a, float2 b) { return __fmul2_rn(a, b); }
 // a pair of fp32 in bf16, and what that left off
@@ -146,7 +149,7 @@ heads_kernel(const ScanArgs a, const __grid_constant__ CUtensorMap tm_x, const _
     for (int i = 0; i < kBars; ++i) {
       const bool by_warps = i == kXFree0 || i == kXFree1 || i == kSFree0 || i == kSFree1 || i == kMReady || i == kWReady ||
                             i == kHReady || i == kYFree;
-      mbar_init(&bar[i], by_warps ? 8 : 1);
+      mbar_init(&bar[i], by_warps ? kWarps : 1);
     }
     *abort_flag = 0u;
     mbar_fence_init();
@@ -154,7 +157,7 @@ heads_kernel(const ScanArgs a, const __grid_constant__ CUtensorMap tm_x, const _
     tma_prefetch_desc(&tm_b);
     tma_prefetch_desc(&tm_c);
   }
-  if (warp == 9) {
+  if (warp == kWarps + 1) {
     tmem_alloc(tmem_slot, kTmem);
     tmem_relinquish();
   }
@@ -177,22 +180,22 @@ heads_kernel(const ScanArgs a, const __grid_constant__ CUtensorMap tm_x, const _
   if (padding) {
     for (int e = threadIdx.x; e < (po.end - po.first) * 8; e += kThreads)
       *reinterpret_cast<uint4*>(out + (po.first + (e >> 3)) * a.ldo + (e & 7) * 8) = make_uint4(0, 0, 0, 0);
-  } else if (warp < 8) {
+  } else if (warp < kWarps) {
     // ---------------- arithmetic between the products ----------------
-    const int q = warp & 3, half = warp >> 2;
+    const int q = warp & 3, part = warp >> 2;           // lanes of tensor memory; 16 of 64 columns
     const int i = q * 32 + lane;                        // lane of tensor memory: token, or number of the state
     const uint32_t mine = tmem + (static_cast<uint32_t>(q * 32) << 16);
     const bool old = a.state != nullptr && chunks > 0 && a.positions[po.first] != 0;
     const int ws = a.state != nullptr ? a.wslots[r] : -1;
     const long long head_at = (static_cast<long long>(a.heads) * a.width * N);
-    const long long at = (static_cast<long long>(col0) + half * 32) * N + i;
-    float h[32];
+    const long long at = (static_cast<long long>(col0) + part * 16) * N + i;
+    float h[16];
 #pragma unroll
-    for (int k = 0; k < 32; ++k) h[k] = old && i < N ? a.state[slot * head_at + at + k * N] : 0.0f;
+    for (int k = 0; k < 16; ++k) h[k] = old && i < N ? a.state[slot * head_at + at + k * N] : 0.0f;
     auto put_state = [&]() {
       if (i < N) {
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
+        for (int u = 0; u < 2; ++u) {
           uint32_t hi[4], lo[4];
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
@@ -200,7 +203,7 @@ heads_kernel(const ScanArgs a, const __grid_constant__ CUtensorMap tm_x, const _
             hi[k] = split(f, g);
             lo[k] = pack_bf16x2(f, g);
           }
-          unsigned char* to = smem + kOffH + tile_at(i, half * 4 + u);
+          unsigned char* to = smem + kOffH + tile_at(i, part * 2 + u);
           *reinterpret_cast<uint4*>(to) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
           *reinterpret_cast<uint4*>(to + kSub) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
         }
@@ -211,6 +214,9 @@ heads_kernel(const ScanArgs a, const __grid_constant__ CUtensorMap tm_x, const _
     };
     put_state();
     const float skip = a.d != nullptr ? a.d[hd] : 0.0f;
+    // 4 rows of W at a time, in groups of 12, 8, 8 and 4 rows for the warps of the four quarters
+    const int w_rows = q == 0 ? 12 : q == 3 ? 4 : 8;
+    const int w_first = part * 32 + (q == 0 ? 0 : q == 1 ? 12 : q == 2 ? 20 : 28);
     bool ok = true;
     for (int c = 0; c < chunks; ++c) {
       const int stage = c & 1, ph = (c >> 1) & 1, n = min(kRows, po.end - po.first - c * kRows);
@@ -224,10 +230,10 @@ heads_kernel(const ScanArgs a, const __grid_constant__ CUtensorMap tm_x, const _
         if (!ok) break;
       }
       // W = x times its weight, in three parts
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const int row = (threadIdx.x >> 3) + 32 * k, u = threadIdx.x & 7;
-        const uint32_t to = tile_at(row, u);
+#pragma unroll 1
+      for (int k = 0; k < w_rows; k += 4) {
+        const int row = w_first + k + (lane >> 3);
+        const uint32_t to = tile_at(row, lane & 7);
         uint4 v = *reinterpret_cast<const uint4*>(x + to);
         if (row >= n) {
           v = make_uint4(0, 0, 0, 0);
@@ -237,68 +243,70 @@ heads_kernel(const ScanArgs a, const __grid_constant__ CUtensorMap tm_x, const _
         }
         const float w = s->w[row];
         const uint32_t in[4] = {v.x, v.y, v.z, v.w};
-        uint32_t part[3][4];
+        uint32_t p[3][4];
 #pragma unroll
         for (int m = 0; m < 4; ++m) {
           const float2 f = unpack_bf16x2(in[m]);
           float f0 = w * f.x, f1 = w * f.y;
-          part[0][m] = split(f0, f1);
-          part[1][m] = split(f0, f1);
-          part[2][m] = pack_bf16x2(f0, f1);
+          p[0][m] = split(f0, f1);
+          p[1][m] = split(f0, f1);
+          p[2][m] = pack_bf16x2(f0, f1);
         }
 #pragma unroll
         for (int m = 0; m < 3; ++m)
-          *reinterpret_cast<uint4*>(smem + kOffW + m * kSub + to) =
-              make_uint4(part[m][0], part[m][1], part[m][2], part[m][3]);
+          *reinterpret_cast<uint4*>(smem + kOffW + m * kSub + to) = make_uint4(p[m][0], p[m][1], p[m][2], p[m][3]);
       }
       fence_async_smem();
       __syncwarp();
       if (lane == 0) mbar_arrive(&bar[kWReady]);
 
-      // M in place of G: this warp's 16 of every 32 columns
+      // M in place of G, every fourth group of 16 columns
       ok = mbar_wait_warp(&bar[kGDone], c & 1, status, kKernelId, 0x103u, abort_flag);
       if (!ok) break;
       tc_fence_after();
-      uint32_t g[4][16];
-#pragma unroll
-      for (int J = 0; J < 4; ++J)
-        if (J <= q) tmem_ld_32x16(mine + kColG + 32 * J + 16 * half, g[J]);
-      tmem_ld_wait();
       {
         const float row = s->row[i], di = s->diag[i], low = s->row_low[i];
         const float* off = s->off + (q == 2 ? 32 : q == 3 ? 96 : 0);
-#pragma unroll
-        for (int J = 0; J < 4; ++J) {
+#pragma unroll 1
+        for (int j = part; j < 8; j += 4) {
           uint32_t m[16];
-          if (J > q) {
+          if (j > 2 * q + 1) {
 #pragma unroll
             for (int k = 0; k < 16; ++k) m[k] = 0u;
           } else {
+            uint32_t g[16];
+            tmem_ld_32x16(mine + kColG + 16 * j, g);
+            float f[16];                                // what G is multiplied by
+            if (j < 2 * q) {
 #pragma unroll
-            for (int k = 0; k < 16; k += 4) {
-              float v[4];
-              if (J < q) {
-                const float4 f = *reinterpret_cast<const float4*>(off + 32 * J + 16 * half + k);
-                const float fc[4] = {f.x, f.y, f.z, f.w};
-#pragma unroll
-                for (int m4 = 0; m4 < 4; ++m4) v[m4] = __uint_as_float(g[J][k + m4]) * (fc[m4] * row);
-              } else {
-                const float4 d = *reinterpret_cast<const float4*>(s->diag + 32 * q + 16 * half + k);
-                const float4 f = *reinterpret_cast<const float4*>(s->col_low + 32 * q + 16 * half + k);
-                const float dj[4] = {d.x, d.y, d.z, d.w}, fc[4] = {f.x, f.y, f.z, f.w};
-#pragma unroll
-                for (int m4 = 0; m4 < 4; ++m4) {
-                  const float w = exp2_fast(di - dj[m4]) * (fc[m4] * low);
-                  v[m4] = 16 * half + k + m4 <= lane ? __uint_as_float(g[J][k + m4]) * w : 0.0f;
-                }
+              for (int k = 0; k < 16; k += 4) {
+                const float4 o = *reinterpret_cast<const float4*>(off + 16 * j + k);
+                f[k] = o.x * row; f[k + 1] = o.y * row; f[k + 2] = o.z * row; f[k + 3] = o.w * row;
               }
-              m[k / 2] = split(v[0], v[1]);
-              m[k / 2 + 1] = split(v[2], v[3]);
-              m[8 + k / 2] = pack_bf16x2(v[0], v[1]);
-              m[8 + k / 2 + 1] = pack_bf16x2(v[2], v[3]);
+              tmem_ld_wait();
+#pragma unroll
+              for (int k = 0; k < 16; ++k) f[k] *= __uint_as_float(g[k]);
+            } else {
+#pragma unroll
+              for (int k = 0; k < 16; k += 4) {
+                const float4 d = *reinterpret_cast<const float4*>(s->diag + 16 * j + k);
+                const float4 o = *reinterpret_cast<const float4*>(s->col_low + 16 * j + k);
+                f[k] = exp2_fast(di - d.x) * (o.x * low);
+                f[k + 1] = exp2_fast(di - d.y) * (o.y * low);
+                f[k + 2] = exp2_fast(di - d.z) * (o.z * low);
+                f[k + 3] = exp2_fast(di - d.w) * (o.w * low);
+              }
+              tmem_ld_wait();
+#pragma unroll
+              for (int k = 0; k < 16; ++k) f[k] = 16 * j + k <= i ? f[k] * __uint_as_float(g[k]) : 0.0f;
+            }
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+              m[k] = split(f[2 * k], f[2 * k + 1]);
+              m[8 + k] = pack_bf16x2(f[2 * k], f[2 * k + 1]);
             }
           }
-          tmem_st_32x16(mine + kColG + 32 * J + 16 * half, m);
+          tmem_st_32x16(mine + kColG + 16 * j, m);
         }
       }
       tmem_st_wait();
@@ -312,12 +320,12 @@ heads_kernel(const ScanArgs a, const __grid_constant__ CUtensorMap tm_x, const _
       tc_fence_after();
       {
         const float keep = s->end[0];
-        uint32_t v[3][32];
+        uint32_t v[3][16];
 #pragma unroll
-        for (int m = 0; m < 3; ++m) tmem_ld_32x32(mine + kColS + m * 64 + half * 32, v[m]);
+        for (int m = 0; m < 3; ++m) tmem_ld_32x16(mine + kColS + m * 64 + part * 16, v[m]);
         tmem_ld_wait();
 #pragma unroll
-        for (int k = 0; k < 32; ++k)
+        for (int k = 0; k < 16; ++k)
           h[k] = fmaf(keep, h[k], __uint_as_float(v[0][k]) + (__uint_as_float(v[1][k]) + __uint_as_float(v[2][k])));
       }
       tc_fence_before();
@@ -328,10 +336,10 @@ heads_kernel(const ScanArgs a, const __grid_constant__ CUtensorMap tm_x, const _
       if (!ok) break;
       tc_fence_after();
       {
-        uint32_t y1[32], y2[32], y3[32];
-        tmem_ld_32x32(mine + kColY1 + half * 32, y1);
-        tmem_ld_32x32(mine + kColY2 + half * 32, y2);
-        tmem_ld_32x32(mine + kColY2 + 64 + half * 32, y3);
+        uint32_t y1[16], y2[16], y3[16];
+        tmem_ld_32x16(mine + kColY1 + part * 16, y1);
+        tmem_ld_32x16(mine + kColY2 + part * 16, y2);
+        tmem_ld_32x16(mine + kColY2 + 64 + part * 16, y3);
         tmem_ld_wait();
         tc_fence_before();
         __syncwarp();
@@ -340,26 +348,26 @@ heads_kernel(const ScanArgs a, const __grid_constant__ CUtensorMap tm_x, const _
         const long long t = po.first + c * kRows + i;
         if (i < n) {
 #pragma unroll
-          for (int u = 0; u < 4; ++u) {
-            const uint4 xv = *reinterpret_cast<const uint4*>(x + tile_at(i, half * 4 + u));
+          for (int u = 0; u < 2; ++u) {
+            const uint4 xv = *reinterpret_cast<const uint4*>(x + tile_at(i, part * 2 + u));
             const uint32_t xi[4] = {xv.x, xv.y, xv.z, xv.w};
             float f[8];
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
               const float2 xf = unpack_bf16x2(xi[k]);
-              const int at2 = u * 8 + 2 * k;
-              f[2 * k] = fmaf(e, __uint_as_float(y2[at2]) + __uint_as_float(y3[at2]),
-                              fmaf(skip, xf.x, __uint_as_float(y1[at2])));
-              f[2 * k + 1] = fmaf(e, __uint_as_float(y2[at2 + 1]) + __uint_as_float(y3[at2 + 1]),
-                                  fmaf(skip, xf.y, __uint_as_float(y1[at2 + 1])));
+              const int k2 = u * 8 + 2 * k;
+              f[2 * k] = fmaf(e, __uint_as_float(y2[k2]) + __uint_as_float(y3[k2]),
+                              fmaf(skip, xf.x, __uint_as_float(y1[k2])));
+              f[2 * k + 1] = fmaf(e, __uint_as_float(y2[k2 + 1]) + __uint_as_float(y3[k2 + 1]),
+                                  fmaf(skip, xf.y, __uint_as_float(y1[k2 + 1])));
             }
             if (a.z != nullptr) {
               float z[8];
-              vec8_load(static_cast<const __nv_bfloat16*>(a.z) + t * a.ldz + col0 + half * 32 + u * 8, z);
+              vec8_load(static_cast<const __nv_bfloat16*>(a.z) + t * a.ldz + col0 + part * 16 + u * 8, z);
 #pragma unroll
               for (int k = 0; k < 8; ++k) f[k] *= silu<__nv_bfloat16>(z[k]);
             }
-            vec8_store(out + t * a.ldo + half * 32 + u * 8, f);
+            vec8_store(out + t * a.ldo + part * 16 + u * 8, f);
           }
         }
       }
@@ -371,9 +379,9 @@ heads_kernel(const ScanArgs a, const __grid_constant__ CUtensorMap tm_x, const _
     }
     if (ok && chunks > 0 && ws >= 0 && ws < a.num_slots && i < N) {
 #pragma unroll
-      for (int k = 0; k < 32; ++k) a.state[ws * head_at + at + k * N] = h[k];
+      for (int k = 0; k < 16; ++k) a.state[ws * head_at + at + k * N] = h[k];
     }
-  } else if (warp == 8) {
+  } else if (warp == kWarps) {
     // ---------------- tiles ----------------
     if (elect_one()) {
       int issued = 0;
@@ -401,7 +409,7 @@ heads_kernel(const ScanArgs a, const __grid_constant__ CUtensorMap tm_x, const _
         if (what >= 3 || c >= 1) mbar_wait(&bar[kBFull], (what >= 3 ? c : c - 1) & 1, status, kKernelId, 0x213u);
       }
     }
-  } else if (warp == 9) {
+  } else if (warp == kWarps + 1) {
     // ---------------- products ----------------
     if (elect_one()) {
       constexpr uint32_t kIdG = make_idesc(kRows, 128, 1, 1);
@@ -463,7 +471,7 @@ heads_kernel(const ScanArgs a, const __grid_constant__ CUtensorMap tm_x, const _
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (warp == 9) tmem_dealloc(tmem, kTmem);
+  if (warp == kWarps + 1) tmem_dealloc(tmem, kTmem);
 }
 
 template <int N>
