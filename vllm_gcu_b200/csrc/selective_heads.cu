@@ -19,8 +19,8 @@
 // block's start between them: 32 exponentials a row instead of 128.
 //
 // A CTA walks the chunks of 64 columns of one head of one request; 16 warps do the arithmetic between the
-// products, one warp loads tiles (TMA), one issues the products, one computes step sizes and decays of the
-// chunk after next.  W and M of a chunk are made while the tensor cores do Y2 and S, its state and result while
+// products, one warp moves tiles (TMA), one issues the products, two compute step sizes and decays, a chunk
+// each, ahead of the rest (one chunk takes a warp 9000 cycles, in which the others do two).  W and M of a chunk are made while the tensor cores do Y2 and S, its state and result while
 // they do the next chunk's G.  The arithmetic bounds it, by latency: with 8 warps 4096 tokens of 128 heads took
 // 213 us.  Lanes 96 and up have four blocks of M that are not zero where lanes below 32 have one, so their
 // warps make less of W.
@@ -47,27 +47,34 @@ struct Scalars {
   float e[kRows];         // 2^(L_i)
   float end[4];           // 2^(L_end)
 };
-constexpr int kOffBars = kOffScal + 2 * static_cast<int>(sizeof(Scalars));
+constexpr int kOffBars = kOffScal + 4 * static_cast<int>(sizeof(Scalars));
 constexpr int kSmem = kOffBars + 256 + 1024;
 static_assert(kSmem <= 232448, "shared memory of a CTA");
 
 enum Bar {
-  kCFull, kBFull, kCFree, kBFree, kXFull0, kXFull1, kXFree0, kXFree1, kSFull0, kSFull1, kSFree0, kSFree1, kGDone,
-  kMReady, kWReady, kSDone, kHReady, kYDone, kYFree, kBars
+  kCFull, kBFull, kCFree, kBFree, kXFull0, kXFull1, kYReady0, kYReady1, kSFull0, kSFull1, kSFull2, kSFull3, kSFree0,
+  kSFree1, kSFree2, kSFree3, kGDone, kMReady, kWReady, kSDone, kHReady, kYDone, kYFree, kBars
 };
 // columns of tensor memory
 constexpr uint32_t kColG = 0, kColY2 = 128, kColY1 = 256, kColS = 320, kTmem = 512;
 constexpr uint32_t kIdescAMajorMN = 1u << 15;
 constexpr int kWarps = 16;                             // of arithmetic: four per 32 lanes of tensor memory
-constexpr int kThreads = (kWarps + 3) * 32;
+constexpr int kScal = 2;                               // of step sizes and decays, a chunk each in turn
+constexpr int kThreads = (kWarps + 2 + kScal) * 32;
 
+// fp32 pairs: two operations per instruction
 __device__ __forceinline__ float2 mul2(float2 a, float2 b) { return __fmul2_rn(a, b); }
-// a pair of fp32 in bf16, and what that left off
-__device__ __forceinline__ uint32_t split(float& a, float& b) {
-  const uint32_t hi = pack_bf16x2(a, b);
-  const float2 f = unpack_bf16x2(hi);
-  a -= f.x;
-  b -= f.y;
+__device__ __forceinline__ float2 add2(float2 a, float2 b) { return __fadd2_rn(a, b); }
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) { return __ffma2_rn(a, b, c); }
+__device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
+__device__ __forceinline__ float2 bits2(uint32_t x, uint32_t y) {
+  return make_float2(__uint_as_float(x), __uint_as_float(y));
+}
+__device__ __forceinline__ uint32_t pack(float2 v) { return pack_bf16x2(v.x, v.y); }
+// a pair in bf16, and what that left off (times -1 twice: a subtraction of pairs is a multiply-add)
+__device__ __forceinline__ uint32_t split(float2& v) {
+  const uint32_t hi = pack(v);
+  v = fma2(unpack_bf16x2(hi), both(-1.0f), v);
   return hi;
 }
 // 16 bytes of column chunk u (of 8) of row r in a tile of 128-byte rows, 128-byte swizzle
@@ -136,7 +143,7 @@ __device__ __forceinline__ void chunk_scalars(const ScanArgs& a, int hd, long lo
 template <int N>
 __global__ void __launch_bounds__(kThreads, 1)
 heads_kernel(const ScanArgs a, const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_b,
-             const __grid_constant__ CUtensorMap tm_c, unsigned int* status) {
+             const __grid_constant__ CUtensorMap tm_c, const __grid_constant__ CUtensorMap tm_y, unsigned int* status) {
   constexpr int kU = N / 64;                            // sub-tiles of B and C
   extern __shared__ unsigned char raw[];
   unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
@@ -147,8 +154,8 @@ heads_kernel(const ScanArgs a, const __grid_constant__ CUtensorMap tm_x, const _
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     for (int i = 0; i < kBars; ++i) {
-      const bool by_warps = i == kXFree0 || i == kXFree1 || i == kSFree0 || i == kSFree1 || i == kMReady || i == kWReady ||
-                            i == kHReady || i == kYFree;
+      const bool by_warps = i == kYReady0 || i == kYReady1 || (i >= kSFree0 && i <= kSFree3) || i == kMReady ||
+                            i == kWReady || i == kHReady || i == kYFree;
       mbar_init(&bar[i], by_warps ? kWarps : 1);
     }
     *abort_flag = 0u;
@@ -189,9 +196,12 @@ heads_kernel(const ScanArgs a, const __grid_constant__ CUtensorMap tm_x, const _
     const int ws = a.state != nullptr ? a.wslots[r] : -1;
     const long long head_at = (static_cast<long long>(a.heads) * a.width * N);
     const long long at = (static_cast<long long>(col0) + part * 16) * N + i;
-    float h[16];
+    float2 h[8];
 #pragma unroll
-    for (int k = 0; k < 16; ++k) h[k] = old && i < N ? a.state[slot * head_at + at + k * N] : 0.0f;
+    for (int k = 0; k < 8; ++k) {
+      h[k] = both(0.0f);
+      if (old && i < N) h[k] = make_float2(a.state[slot * head_at + at + 2 * k * N], a.state[slot * head_at + at + (2 * k + 1) * N]);
+    }
     auto put_state = [&]() {
       if (i < N) {
 #pragma unroll
@@ -199,9 +209,9 @@ heads_kernel(const ScanArgs a, const __grid_constant__ CUtensorMap tm_x, const _
           uint32_t hi[4], lo[4];
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
-            float f = h[u * 8 + 2 * k], g = h[u * 8 + 2 * k + 1];
-            hi[k] = split(f, g);
-            lo[k] = pack_bf16x2(f, g);
+            float2 f = h[u * 4 + k];
+            hi[k] = split(f);
+            lo[k] = pack(f);
           }
           unsigned char* to = smem + kOffH + tile_at(i, part * 2 + u);
           *reinterpret_cast<uint4*>(to) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
@@ -219,11 +229,11 @@ heads_kernel(const ScanArgs a, const __grid_constant__ CUtensorMap tm_x, const _
     const int w_first = part * 32 + (q == 0 ? 0 : q == 1 ? 12 : q == 2 ? 20 : 28);
     bool ok = true;
     for (int c = 0; c < chunks; ++c) {
-      const int stage = c & 1, ph = (c >> 1) & 1, n = min(kRows, po.end - po.first - c * kRows);
-      const Scalars* s = scal + stage;
+      const int stage = c & 1, four = c & 3, n = min(kRows, po.end - po.first - c * kRows);
+      const Scalars* s = scal + four;
       unsigned char* x = smem + kOffX + stage * kSub;
-      ok = mbar_wait_warp(&bar[kSFull0 + stage], ph, status, kKernelId, 0x100u, abort_flag) &&
-           mbar_wait_warp(&bar[kXFull0 + stage], ph, status, kKernelId, 0x101u, abort_flag);
+      ok = mbar_wait_warp(&bar[kSFull0 + four], (c >> 2) & 1, status, kKernelId, 0x100u, abort_flag) &&
+           mbar_wait_warp(&bar[kXFull0 + stage], (c >> 1) & 1, status, kKernelId, 0x101u, abort_flag);
       if (!ok) break;
       if (n < kRows) {              // rows of other requests: zeros, they may hold anything
         ok = mbar_wait_warp(&bar[kBFull], c & 1, status, kKernelId, 0x102u, abort_flag);
@@ -241,16 +251,15 @@ heads_kernel(const ScanArgs a, const __grid_constant__ CUtensorMap tm_x, const _
 #pragma unroll
           for (int b = 0; b < kU; ++b) *reinterpret_cast<uint4*>(smem + kOffB + b * kSub + to) = v;
         }
-        const float w = s->w[row];
+        const float2 w = both(s->w[row]);
         const uint32_t in[4] = {v.x, v.y, v.z, v.w};
         uint32_t p[3][4];
 #pragma unroll
         for (int m = 0; m < 4; ++m) {
-          const float2 f = unpack_bf16x2(in[m]);
-          float f0 = w * f.x, f1 = w * f.y;
-          p[0][m] = split(f0, f1);
-          p[1][m] = split(f0, f1);
-          p[2][m] = pack_bf16x2(f0, f1);
+          float2 f = mul2(w, unpack_bf16x2(in[m]));
+          p[0][m] = split(f);
+          p[1][m] = split(f);
+          p[2][m] = pack(f);
         }
 #pragma unroll
         for (int m = 0; m < 3; ++m)
@@ -276,34 +285,38 @@ heads_kernel(const ScanArgs a, const __grid_constant__ CUtensorMap tm_x, const _
           } else {
             uint32_t g[16];
             tmem_ld_32x16(mine + kColG + 16 * j, g);
-            float f[16];                                // what G is multiplied by
+            float2 f[8];                                // what G is multiplied by
             if (j < 2 * q) {
 #pragma unroll
-              for (int k = 0; k < 16; k += 4) {
-                const float4 o = *reinterpret_cast<const float4*>(off + 16 * j + k);
-                f[k] = o.x * row; f[k + 1] = o.y * row; f[k + 2] = o.z * row; f[k + 3] = o.w * row;
+              for (int k = 0; k < 8; k += 2) {
+                const float4 o = *reinterpret_cast<const float4*>(off + 16 * j + 2 * k);
+                f[k] = mul2(make_float2(o.x, o.y), both(row));
+                f[k + 1] = mul2(make_float2(o.z, o.w), both(row));
               }
               tmem_ld_wait();
 #pragma unroll
-              for (int k = 0; k < 16; ++k) f[k] *= __uint_as_float(g[k]);
+              for (int k = 0; k < 8; ++k) f[k] = mul2(f[k], bits2(g[2 * k], g[2 * k + 1]));
             } else {
 #pragma unroll
-              for (int k = 0; k < 16; k += 4) {
-                const float4 d = *reinterpret_cast<const float4*>(s->diag + 16 * j + k);
-                const float4 o = *reinterpret_cast<const float4*>(s->col_low + 16 * j + k);
-                f[k] = exp2_fast(di - d.x) * (o.x * low);
-                f[k + 1] = exp2_fast(di - d.y) * (o.y * low);
-                f[k + 2] = exp2_fast(di - d.z) * (o.z * low);
-                f[k + 3] = exp2_fast(di - d.w) * (o.w * low);
+              for (int k = 0; k < 8; k += 2) {
+                const float4 d = *reinterpret_cast<const float4*>(s->diag + 16 * j + 2 * k);
+                const float4 o = *reinterpret_cast<const float4*>(s->col_low + 16 * j + 2 * k);
+                f[k] = mul2(make_float2(exp2_fast(di - d.x), exp2_fast(di - d.y)), mul2(make_float2(o.x, o.y), both(low)));
+                f[k + 1] = mul2(make_float2(exp2_fast(di - d.z), exp2_fast(di - d.w)),
+                                mul2(make_float2(o.z, o.w), both(low)));
               }
               tmem_ld_wait();
 #pragma unroll
-              for (int k = 0; k < 16; ++k) f[k] = 16 * j + k <= i ? f[k] * __uint_as_float(g[k]) : 0.0f;
+              for (int k = 0; k < 8; ++k) {
+                f[k] = mul2(f[k], bits2(g[2 * k], g[2 * k + 1]));
+                if (16 * j + 2 * k > i) f[k].x = 0.0f;
+                if (16 * j + 2 * k + 1 > i) f[k].y = 0.0f;
+              }
             }
 #pragma unroll
             for (int k = 0; k < 8; ++k) {
-              m[k] = split(f[2 * k], f[2 * k + 1]);
-              m[8 + k] = pack_bf16x2(f[2 * k], f[2 * k + 1]);
+              m[k] = split(f[k]);
+              m[8 + k] = pack(f[k]);
             }
           }
           tmem_st_32x16(mine + kColG + 16 * j, m);
@@ -325,8 +338,9 @@ heads_kernel(const ScanArgs a, const __grid_constant__ CUtensorMap tm_x, const _
         for (int m = 0; m < 3; ++m) tmem_ld_32x16(mine + kColS + m * 64 + part * 16, v[m]);
         tmem_ld_wait();
 #pragma unroll
-        for (int k = 0; k < 16; ++k)
-          h[k] = fmaf(keep, h[k], __uint_as_float(v[0][k]) + (__uint_as_float(v[1][k]) + __uint_as_float(v[2][k])));
+        for (int k = 0; k < 8; ++k)
+          h[k] = fma2(both(keep), h[k], add2(bits2(v[0][2 * k], v[0][2 * k + 1]),
+                                             add2(bits2(v[1][2 * k], v[1][2 * k + 1]), bits2(v[2][2 * k], v[2][2 * k + 1]))));
       }
       tc_fence_before();
       put_state();
@@ -344,62 +358,81 @@ heads_kernel(const ScanArgs a, const __grid_constant__ CUtensorMap tm_x, const _
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&bar[kYFree]);
-        const float e = s->e[i];
+        const float2 e = both(s->e[i]);
         const long long t = po.first + c * kRows + i;
-        if (i < n) {
 #pragma unroll
-          for (int u = 0; u < 2; ++u) {
-            const uint4 xv = *reinterpret_cast<const uint4*>(x + tile_at(i, part * 2 + u));
-            const uint32_t xi[4] = {xv.x, xv.y, xv.z, xv.w};
-            float f[8];
+        for (int u = 0; u < 2; ++u) {
+          unsigned char* at_x = x + tile_at(i, part * 2 + u);
+          const uint4 xv = *reinterpret_cast<const uint4*>(at_x);
+          const uint32_t xi[4] = {xv.x, xv.y, xv.z, xv.w};
+          float2 f[4];
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              const float2 xf = unpack_bf16x2(xi[k]);
-              const int k2 = u * 8 + 2 * k;
-              f[2 * k] = fmaf(e, __uint_as_float(y2[k2]) + __uint_as_float(y3[k2]),
-                              fmaf(skip, xf.x, __uint_as_float(y1[k2])));
-              f[2 * k + 1] = fmaf(e, __uint_as_float(y2[k2 + 1]) + __uint_as_float(y3[k2 + 1]),
-                                  fmaf(skip, xf.y, __uint_as_float(y1[k2 + 1])));
-            }
-            if (a.z != nullptr) {
-              float z[8];
-              vec8_load(static_cast<const __nv_bfloat16*>(a.z) + t * a.ldz + col0 + part * 16 + u * 8, z);
-#pragma unroll
-              for (int k = 0; k < 8; ++k) f[k] *= silu<__nv_bfloat16>(z[k]);
-            }
-            vec8_store(out + t * a.ldo + part * 16 + u * 8, f);
+          for (int k = 0; k < 4; ++k) {
+            const int k2 = u * 8 + 2 * k;
+            f[k] = fma2(e, add2(bits2(y2[k2], y2[k2 + 1]), bits2(y3[k2], y3[k2 + 1])),
+                        fma2(both(skip), unpack_bf16x2(xi[k]), bits2(y1[k2], y1[k2 + 1])));
           }
+          if (a.z != nullptr && i < n) {
+            float z[8];
+            vec8_load(static_cast<const __nv_bfloat16*>(a.z) + t * a.ldz + col0 + part * 16 + u * 8, z);
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              f[k] = mul2(f[k], make_float2(silu<__nv_bfloat16>(z[2 * k]), silu<__nv_bfloat16>(z[2 * k + 1])));
+          }
+          const uint4 y = make_uint4(pack(f[0]), pack(f[1]), pack(f[2]), pack(f[3]));
+          // a whole chunk leaves as a tile, in place of its x; the last rows of a portion one by one
+          if (n == kRows) *reinterpret_cast<uint4*>(at_x) = y;
+          else if (i < n) *reinterpret_cast<uint4*>(out + t * a.ldo + part * 16 + u * 8) = y;
         }
       }
+      fence_async_smem();
       __syncwarp();
       if (lane == 0) {
-        mbar_arrive(&bar[kXFree0 + stage]);
-        mbar_arrive(&bar[kSFree0 + stage]);
+        mbar_arrive(&bar[kYReady0 + stage]);
+        mbar_arrive(&bar[kSFree0 + four]);
       }
     }
     if (ok && chunks > 0 && ws >= 0 && ws < a.num_slots && i < N) {
 #pragma unroll
-      for (int k = 0; k < 16; ++k) a.state[ws * head_at + at + k * N] = h[k];
+      for (int k = 0; k < 16; ++k) a.state[ws * head_at + at + k * N] = k & 1 ? h[k / 2].y : h[k / 2].x;
     }
   } else if (warp == kWarps) {
     // ---------------- tiles ----------------
     if (elect_one()) {
       int issued = 0;
+      // the result of chunk c, which lies in place of its x, to memory
+      auto send = [&](int c) {
+        if (!mbar_wait(&bar[kYReady0 + (c & 1)], (c >> 1) & 1, status, kKernelId, 0x200u, abort_flag)) return false;
+        if (po.end - po.first - c * kRows >= kRows) {
+          tma_store_2d(&tm_y, smem + kOffX + (c & 1) * kSub, col0, po.first + c * kRows);
+          tma_store_commit();
+        }
+        return true;
+      };
+      bool ok = true;
       for (int c = 0; c < chunks; ++c) {
         const int y = po.first + c * kRows, stage = c & 1;
-        if (c >= 2 && !mbar_wait(&bar[kXFree0 + stage], ((c >> 1) & 1) ^ 1, status, kKernelId, 0x200u, abort_flag)) break;
+        if (c >= 2) {
+          ok = send(c - 2);
+          if (!ok) break;
+          tma_store_wait_read<0>();
+        }
         mbar_expect_tx(&bar[kXFull0 + stage], kSub);
         tma_load_2d(smem + kOffX + stage * kSub, &tm_x, &bar[kXFull0 + stage], col0, y);
         issued = 4 * c + 1;
-        if (c >= 1 && !mbar_wait(&bar[kCFree], (c - 1) & 1, status, kKernelId, 0x201u, abort_flag)) break;
+        ok = c < 1 || mbar_wait(&bar[kCFree], (c - 1) & 1, status, kKernelId, 0x201u, abort_flag);
+        if (!ok) break;
         mbar_expect_tx(&bar[kCFull], kU * kSub);
         for (int u = 0; u < kU; ++u) tma_load_2d(smem + kOffC + u * kSub, &tm_c, &bar[kCFull], group * N + u * 64, y);
         issued = 4 * c + 2;
-        if (c >= 1 && !mbar_wait(&bar[kBFree], (c - 1) & 1, status, kKernelId, 0x202u, abort_flag)) break;
+        ok = c < 1 || mbar_wait(&bar[kBFree], (c - 1) & 1, status, kKernelId, 0x202u, abort_flag);
+        if (!ok) break;
         mbar_expect_tx(&bar[kBFull], kU * kSub);
         for (int u = 0; u < kU; ++u) tma_load_2d(smem + kOffB + u * kSub, &tm_b, &bar[kBFull], group * N + u * 64, y);
         issued = 4 * c + 3;
       }
+      for (int c = max(0, chunks - 2); c < chunks && ok; ++c) ok = send(c);
+      tma_store_wait<0>();
       // copies in flight end before the CTA does, also when a wait ran out
       if (*abort_flag != 0u && issued > 0) {
         const int c = issued >> 2, what = issued & 3;
@@ -460,12 +493,12 @@ heads_kernel(const ScanArgs a, const __grid_constant__ CUtensorMap tm_x, const _
   } else {
     // ---------------- step sizes and decays ----------------
     const double rate = -exp(static_cast<double>(a.a_log[hd])) * 1.4426950408889634;
-    for (int c = 0; c < chunks; ++c) {
-      if (c >= 2 && !mbar_wait_warp(&bar[kSFree0 + (c & 1)], ((c >> 1) & 1) ^ 1, status, kKernelId, 0x400u, abort_flag))
+    for (int c = warp - kWarps - 2; c < chunks; c += kScal) {
+      if (c >= 4 && !mbar_wait_warp(&bar[kSFree0 + (c & 3)], ((c >> 2) & 1) ^ 1, status, kKernelId, 0x400u, abort_flag))
         break;
-      chunk_scalars(a, hd, po.first + c * kRows, min(kRows, po.end - po.first - c * kRows), rate, scal + (c & 1));
+      chunk_scalars(a, hd, po.first + c * kRows, min(kRows, po.end - po.first - c * kRows), rate, scal + (c & 3));
       __syncwarp();
-      if (lane == 0) mbar_arrive(&bar[kSFull0 + (c & 1)]);
+      if (lane == 0) mbar_arrive(&bar[kSFull0 + (c & 3)]);
     }
   }
   tc_fence_before();
@@ -476,7 +509,7 @@ heads_kernel(const ScanArgs a, const __grid_constant__ CUtensorMap tm_x, const _
 
 template <int N>
 int launch(const ScanArgs& a, cudaStream_t s) {
-  CUtensorMap x, b, c;
+  CUtensorMap x, b, c, y;
   const CUtensorMapDataType bf = CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
   const CUtensorMapSwizzle sw = CU_TENSOR_MAP_SWIZZLE_128B;
   const uint64_t gn = static_cast<uint64_t>(a.groups) * N;
@@ -485,6 +518,7 @@ int launch(const ScanArgs& a, cudaStream_t s) {
   int rc = encode_tmap_2d(&x, bf, 2, a.x, a.T, cols, pitch(a.ldx, cols), kRows, 64, sw);
   if (rc == 0) rc = encode_tmap_2d(&b, bf, 2, a.b, a.T, gn, pitch(a.ldb, gn), kRows, 64, sw);
   if (rc == 0) rc = encode_tmap_2d(&c, bf, 2, a.c, a.T, gn, pitch(a.ldc, gn), kRows, 64, sw);
+  if (rc == 0) rc = encode_tmap_2d(&y, bf, 2, a.out, a.T, cols, pitch(a.ldo, cols), kRows, 64, sw);
   if (rc != 0) return rc;
   unsigned int* status = status_ptr();
   if (status == nullptr) return -9;
@@ -496,7 +530,7 @@ int launch(const ScanArgs& a, cudaStream_t s) {
     if (e != 0) return e;
     if (dev < 64) ready[dev] = true;
   }
-  return launch_overlapped(heads_kernel<N>, dim3(a.heads * (a.width / kP), a.np), dim3(kThreads), kSmem, s, a, x, b, c,
+  return launch_overlapped(heads_kernel<N>, dim3(a.heads * (a.width / kP), a.np), dim3(kThreads), kSmem, s, a, x, b, c, y,
                            status);
 }
 
