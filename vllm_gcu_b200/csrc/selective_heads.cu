@@ -13,7 +13,7 @@
 // H lives in registers (lane n, 32 columns p per warp) and goes on as fp32.  Two parts leave 2^-17 of a
 // factor, an eighth of what the rows' own rounding to bf16 is off.
 //
-// Decays: a difference L_i - L_j is taken of 64-bit sums or, in the 32 x 32 blocks on the diagonal, of 32-bit numbers
+// Decays (none above 1: step sizes are not below 0): a difference L_i - L_j is taken of sums in two floats or, in the 32 x 32 blocks on the diagonal, of 32-bit numbers
 // whose rounding the two sides' factors make good, so that a strong decay in front does not cost those
 // behind it their bits.  Outside the diagonal 2^(L_i - L_j) is a product of two factors below 1, with L at the row
 // block's start between them: 32 exponentials a row instead of 128.
@@ -80,50 +80,81 @@ __device__ __forceinline__ uint32_t split(float2& v) {
 // 16 bytes of column chunk u (of 8) of row r in a tile of 128-byte rows, 128-byte swizzle
 __device__ __forceinline__ uint32_t tile_at(int r, int u) { return r * 128 + ((u ^ (r & 7)) << 4); }
 
-__device__ __forceinline__ double shfl_d(double v, int from) { return __shfl_sync(0xffffffffu, v, from); }
+// A sum in two floats: 48 bits, by Knuth's exact sum of two numbers.  (In 64 bits it took a chunk's warp twice as
+// long, for the conversions of 28 differences a lane.)
+struct Two {
+  float hi, lo;
+};
+__device__ __forceinline__ Two add(Two a, Two b) {
+  const float s = a.hi + b.hi, v = s - a.hi;
+  const float e = (a.hi - (s - v)) + (b.hi - v) + (a.lo + b.lo);
+  const float hi = s + e;
+  return {hi, e - (hi - s)};
+}
+__device__ __forceinline__ float less(Two a, Two b) { return (a.hi - b.hi) + (a.lo - b.lo); }
+__device__ __forceinline__ Two shfl(Two v, int from) {
+  return {__shfl_sync(0xffffffffu, v.hi, from), __shfl_sync(0xffffffffu, v.lo, from)};
+}
 
-// Step sizes and decays of tokens [t0, t0 + n) of a head, four per lane.
-__device__ __forceinline__ void chunk_scalars(const ScanArgs& a, int hd, long long t0, int n, double rate, Scalars* s) {
+// What a lane needs of the step sizes of tokens 4 lane .. + 3 of a chunk, raw.
+__device__ __forceinline__ void load_steps(const ScanArgs& a, int hd, long long t0, int n, float (&z)[4]) {
   const int lane = threadIdx.x & 31;
-  float dt[4];
-  double L[4];
-  double run = 0.0;
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
-    const bool in = 4 * lane + k < n;
-    dt[k] = in ? step_size<__nv_bfloat16>(a, t0 + 4 * lane + k, hd) : 0.0f;
-    double la = static_cast<double>(dt[k]) * rate;
-    if (la < -160.0) la = -160.0;                       // 2^-160 is 0 in fp32; sums stay exact to 2^-40
-    run += la;
+    z[k] = 0.0f;
+    if (4 * lane + k < n) {
+      const long long at = (t0 + 4 * lane + k) * a.lddt + hd;
+      z[k] = a.dt_f32 ? static_cast<const float*>(a.dt)[at]
+                      : __bfloat162float(static_cast<const __nv_bfloat16*>(a.dt)[at]);
+    }
+  }
+}
+// Step sizes and decays of n tokens, four per lane.  rate: -exp(a_log) log2(e).
+__device__ __forceinline__ void chunk_scalars(const ScanArgs& a, int n, float bias, Two rate, const float (&z)[4],
+                                              Scalars* s) {
+  const int lane = threadIdx.x & 31;
+  float dt[4];
+  Two L[4], run = {0.0f, 0.0f};
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    dt[k] = step_from<__nv_bfloat16>(a, z[k], bias);
+    Two la = {dt[k] * rate.hi, 0.0f};
+    la.lo = fmaf(dt[k], rate.hi, -la.hi) + dt[k] * rate.lo;
+    if (la.hi < -160.0f) la = {-160.0f, 0.0f};          // 2^-160 is 0 in fp32; sums stay exact to 2^-33
+    if (4 * lane + k >= n) {
+      dt[k] = 0.0f;
+      la = {0.0f, 0.0f};
+    }
+    run = add(run, la);
     L[k] = run;
   }
-  double before = run;                                  // inclusive over lanes, then what lies in front of the lane
+  Two before = run;                                     // over the lanes: inclusive, then what lies in front of one
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const double v = __shfl_up_sync(0xffffffffu, before, o);
-    if (lane >= o) before += v;
+    const Two v = {__shfl_up_sync(0xffffffffu, before.hi, o), __shfl_up_sync(0xffffffffu, before.lo, o)};
+    if (lane >= o) before = add(v, before);
   }
-  before = __shfl_up_sync(0xffffffffu, before, 1);
-  if (lane == 0) before = 0.0;
+  before = {__shfl_up_sync(0xffffffffu, before.hi, 1), __shfl_up_sync(0xffffffffu, before.lo, 1)};
+  if (lane == 0) before = {0.0f, 0.0f};
 #pragma unroll
-  for (int k = 0; k < 4; ++k) L[k] += before;
-  const double ref1 = shfl_d(L[3], 7), ref2 = shfl_d(L[3], 15), ref3 = shfl_d(L[3], 23), end = shfl_d(L[3], 31);
+  for (int k = 0; k < 4; ++k) L[k] = add(before, L[k]);
+  const Two ref1 = shfl(L[3], 7), ref2 = shfl(L[3], 15), ref3 = shfl(L[3], 23), end = shfl(L[3], 31);
   const int block = lane >> 3;
-  const double ref = block == 0 ? 0.0 : block == 1 ? ref1 : block == 2 ? ref2 : ref3;
+  const Two none = {0.0f, 0.0f}, ref = block == 0 ? none : block == 1 ? ref1 : block == 2 ? ref2 : ref3;
+  const Two minus = {-ref.hi, -ref.lo};
   float row[4], diag[4], rl[4], cl[4], w[4], e[4], o1[4], o2[4], o3[4];
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
-    const double l = L[k] - ref;
-    diag[k] = static_cast<float>(l);
-    const float low = static_cast<float>(l - static_cast<double>(diag[k]));
-    row[k] = exp2f(diag[k]);
-    rl[k] = exp2f(low);
-    cl[k] = dt[k] * exp2f(-low);
-    w[k] = dt[k] * exp2f(static_cast<float>(end - L[k]));
-    e[k] = exp2f(static_cast<float>(L[k]));
-    o1[k] = dt[k] * exp2f(static_cast<float>(fmin(ref1 - L[k], 0.0)));
-    o2[k] = dt[k] * exp2f(static_cast<float>(fmin(ref2 - L[k], 0.0)));
-    o3[k] = dt[k] * exp2f(static_cast<float>(fmin(ref3 - L[k], 0.0)));
+    const Two l = add(L[k], minus);
+    diag[k] = l.hi;
+    row[k] = exp2_fast(l.hi);
+    rl[k] = exp2_fast(l.lo);
+    cl[k] = dt[k] * exp2_fast(-l.lo);
+    w[k] = dt[k] * exp2_fast(less(end, L[k]));
+    e[k] = exp2_fast(L[k].hi);
+    o1[k] = dt[k] * exp2_fast(less(ref1, L[k]));        // (lanes behind the reference: not kept)
+    o2[k] = dt[k] * exp2_fast(less(ref2, L[k]));
+    o3[k] = dt[k] * exp2_fast(less(ref3, L[k]));
   }
   auto put = [&](float* to, const float (&v)[4]) {
     *reinterpret_cast<float4*>(to + 4 * lane) = make_float4(v[0], v[1], v[2], v[3]);
@@ -137,7 +168,14 @@ __device__ __forceinline__ void chunk_scalars(const ScanArgs& a, int hd, long lo
   if (lane < 8) put(s->off, o1);
   if (lane < 16) put(s->off + 32, o2);
   if (lane < 24) put(s->off + 96, o3);
-  if (lane == 0) s->end[0] = exp2f(static_cast<float>(end));
+  if (lane == 0) s->end[0] = exp2_fast(end.hi);
+}
+
+// A wait by all lanes.  (By the first lane alone, the others behind a shuffle, a barrier that is through took 400 cycles
+// more.)
+__device__ __forceinline__ bool wait_warp(uint64_t* bar, uint32_t parity, unsigned int* st, unsigned int detail,
+                                          volatile uint32_t* abort_flag) {
+  return mbar_wait_warp(bar, parity, st, kKernelId, detail, abort_flag);
 }
 
 template <int N>
@@ -227,19 +265,16 @@ heads_kernel(const ScanArgs a, const __grid_constant__ CUtensorMap tm_x, const _
     // 4 rows of W at a time, in groups of 12, 8, 8 and 4 rows for the warps of the four quarters
     const int w_rows = q == 0 ? 12 : q == 3 ? 4 : 8;
     const int w_first = part * 32 + (q == 0 ? 0 : q == 1 ? 12 : q == 2 ? 20 : 28);
-    bool ok = true;
-    for (int c = 0; c < chunks; ++c) {
-      const int stage = c & 1, four = c & 3, n = min(kRows, po.end - po.first - c * kRows);
-      const Scalars* s = scal + four;
-      unsigned char* x = smem + kOffX + stage * kSub;
-      ok = mbar_wait_warp(&bar[kSFull0 + four], (c >> 2) & 1, status, kKernelId, 0x100u, abort_flag) &&
-           mbar_wait_warp(&bar[kXFull0 + stage], (c >> 1) & 1, status, kKernelId, 0x101u, abort_flag);
-      if (!ok) break;
-      if (n < kRows) {              // rows of other requests: zeros, they may hold anything
-        ok = mbar_wait_warp(&bar[kBFull], c & 1, status, kKernelId, 0x102u, abort_flag);
-        if (!ok) break;
-      }
-      // W = x times its weight, in three parts
+    // W of chunk c = x times its weight, in three parts
+    auto make_w = [&](int c) {
+      const int n = min(kRows, po.end - po.first - c * kRows);
+      const Scalars* s = scal + (c & 3);
+      unsigned char* x = smem + kOffX + (c & 1) * kSub;
+      if (!wait_warp(&bar[kSFull0 + (c & 3)], (c >> 2) & 1, status, 0x100u, abort_flag) ||
+          !wait_warp(&bar[kXFull0 + (c & 1)], (c >> 1) & 1, status, 0x101u, abort_flag))
+        return false;
+      // rows of other requests: zeros, they may hold anything
+      if (n < kRows && !wait_warp(&bar[kBFull], c & 1, status, 0x102u, abort_flag)) return false;
 #pragma unroll 1
       for (int k = 0; k < w_rows; k += 4) {
         const int row = w_first + k + (lane >> 3);
@@ -268,9 +303,16 @@ heads_kernel(const ScanArgs a, const __grid_constant__ CUtensorMap tm_x, const _
       fence_async_smem();
       __syncwarp();
       if (lane == 0) mbar_arrive(&bar[kWReady]);
+      return true;
+    };
 
+    bool ok = chunks == 0 || make_w(0);
+    for (int c = 0; c < chunks && ok; ++c) {
+      const int stage = c & 1, four = c & 3, n = min(kRows, po.end - po.first - c * kRows);
+      const Scalars* s = scal + four;
+      unsigned char* x = smem + kOffX + stage * kSub;
       // M in place of G, every fourth group of 16 columns
-      ok = mbar_wait_warp(&bar[kGDone], c & 1, status, kKernelId, 0x103u, abort_flag);
+      ok = wait_warp(&bar[kGDone], c & 1, status, 0x103u, abort_flag);
       if (!ok) break;
       tc_fence_after();
       {
@@ -328,7 +370,7 @@ heads_kernel(const ScanArgs a, const __grid_constant__ CUtensorMap tm_x, const _
       if (lane == 0) mbar_arrive(&bar[kMReady]);
 
       // the state behind the chunk
-      ok = mbar_wait_warp(&bar[kSDone], c & 1, status, kKernelId, 0x104u, abort_flag);
+      ok = wait_warp(&bar[kSDone], c & 1, status, 0x104u, abort_flag);
       if (!ok) break;
       tc_fence_after();
       {
@@ -343,10 +385,17 @@ heads_kernel(const ScanArgs a, const __grid_constant__ CUtensorMap tm_x, const _
                                              add2(bits2(v[1][2 * k], v[1][2 * k + 1]), bits2(v[2][2 * k], v[2][2 * k + 1]))));
       }
       tc_fence_before();
+      // (the products with the state before are through)
+      ok = wait_warp(&bar[kCFree], c & 1, status, 0x106u, abort_flag);
+      if (!ok) break;
       put_state();
+      if (c + 1 < chunks) {                              // (the products with W of this chunk are through)
+        ok = make_w(c + 1);
+        if (!ok) break;
+      }
 
       // the result's rows
-      ok = mbar_wait_warp(&bar[kYDone], c & 1, status, kKernelId, 0x105u, abort_flag);
+      ok = wait_warp(&bar[kYDone], c & 1, status, 0x105u, abort_flag);
       if (!ok) break;
       tc_fence_after();
       {
@@ -470,16 +519,17 @@ heads_kernel(const ScanArgs a, const __grid_constant__ CUtensorMap tm_x, const _
           umma_f16(tmem + kColG, c_k + step, b_k + step, kIdG, k > 0);
         }
         umma_commit(&bar[kGDone]);
-        if (!wait(kHReady, ph, 2) || (c > 0 && !wait(kYFree, ph ^ 1, 3))) break;
-#pragma unroll
-        for (int k = 0; k < N / 16; ++k)
-          umma_f16(tmem + kColY2, c_k + (k >> 2) * (kSub >> 4) + (k & 3) * 2, h_mn + k * kStep, kIdY2, k > 0);
-        umma_commit(&bar[kCFree]);
-        if (!wait(kWReady, ph, 4)) break;
+        // (the state is there: S of the chunk before has been read)
+        if (!wait(kHReady, ph, 2) || !wait(kWReady, ph, 4)) break;
 #pragma unroll
         for (int k = 0; k < 8; ++k) umma_f16(tmem + kColS, b_mn + k * kStep, w_mn + k * kStep, kIdS, k > 0);
         umma_commit(&bar[kBFree]);
         umma_commit(&bar[kSDone]);
+        if (c > 0 && !wait(kYFree, ph ^ 1, 3)) break;
+#pragma unroll
+        for (int k = 0; k < N / 16; ++k)
+          umma_f16(tmem + kColY2, c_k + (k >> 2) * (kSub >> 4) + (k & 3) * 2, h_mn + k * kStep, kIdY2, k > 0);
+        umma_commit(&bar[kCFree]);
         if (!wait(kMReady, ph, 5)) break;
         const uint64_t x = x_mn + (c & 1) * (kSub >> 4);
 #pragma unroll
@@ -492,13 +542,21 @@ heads_kernel(const ScanArgs a, const __grid_constant__ CUtensorMap tm_x, const _
     }
   } else {
     // ---------------- step sizes and decays ----------------
-    const double rate = -exp(static_cast<double>(a.a_log[hd])) * 1.4426950408889634;
-    for (int c = warp - kWarps - 2; c < chunks; c += kScal) {
-      if (c >= 4 && !mbar_wait_warp(&bar[kSFree0 + (c & 3)], ((c >> 2) & 1) ^ 1, status, kKernelId, 0x400u, abort_flag))
-        break;
-      chunk_scalars(a, hd, po.first + c * kRows, min(kRows, po.end - po.first - c * kRows), rate, scal + (c & 3));
+    const double rate2 = -exp(static_cast<double>(a.a_log[hd])) * 1.4426950408889634;
+    const Two rate = {static_cast<float>(rate2), static_cast<float>(rate2 - static_cast<double>(static_cast<float>(rate2)))};
+    const float bias = a.dt_bias != nullptr ? a.dt_bias[hd] : 0.0f;
+    auto rows = [&](int c) { return min(kRows, po.end - po.first - c * kRows); };
+    float z[4], next[4];
+    const int first = warp - kWarps - 2;
+    if (first < chunks) load_steps(a, hd, po.first + first * kRows, rows(first), z);
+    for (int c = first; c < chunks; c += kScal) {
+      if (c + kScal < chunks) load_steps(a, hd, po.first + (c + kScal) * kRows, rows(c + kScal), next);
+      if (c >= 4 && !wait_warp(&bar[kSFree0 + (c & 3)], ((c >> 2) & 1) ^ 1, status, 0x400u, abort_flag)) break;
+      chunk_scalars(a, rows(c), bias, rate, z, scal + (c & 3));
       __syncwarp();
       if (lane == 0) mbar_arrive(&bar[kSFull0 + (c & 3)]);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) z[k] = next[k];
     }
   }
   tc_fence_before();
@@ -537,7 +595,7 @@ int launch(const ScanArgs& a, cudaStream_t s) {
 }  // namespace tiles
 
 bool heads_by_tiles(const ScanArgs& a) {
-  return a.wide && a.width % tiles::kP == 0 && (a.N == 64 || a.N == 128);
+  return a.wide && a.width % tiles::kP == 0 && (a.N == 64 || a.N == 128) && a.dt_min >= 0.0f;
 }
 int launch_heads_by_tiles(const ScanArgs& a, cudaStream_t s) {
   return a.N == 128 ? tiles::launch<128>(a, s) : tiles::launch<64>(a, s);
