@@ -52,8 +52,8 @@ constexpr int kSmem = kOffBars + 256 + 1024;
 static_assert(kSmem <= 232448, "shared memory of a CTA");
 
 enum Bar {
-  kCFull, kBFull, kCFree, kBFree, kXFull0, kXFull1, kYReady0, kYReady1, kSFull0, kSFull1, kSFull2, kSFull3, kSFree0,
-  kSFree1, kSFree2, kSFree3, kGDone, kMReady, kWReady, kSDone, kHReady, kYDone, kYFree, kBars
+  kCFull, kBFull, kCFree, kBFree, kXFull0, kXFull1, kYReady0, kYReady1, kSFree0, kSFree1, kSFree2, kSFree3, kGDone,
+  kMReady, kWReady, kSDone, kHReady, kYDone, kYFree, kBars
 };
 // columns of tensor memory
 constexpr uint32_t kColG = 0, kColY2 = 128, kColY1 = 256, kColS = 320, kTmem = 512;
@@ -171,11 +171,15 @@ __device__ __forceinline__ void chunk_scalars(const ScanArgs& a, int n, float bi
   if (lane == 0) s->end[0] = exp2_fast(end.hi);
 }
 
-// A wait by all lanes.  (By the first lane alone, the others behind a shuffle, a barrier that is through took 400 cycles
-// more.)
-__device__ __forceinline__ bool wait_warp(uint64_t* bar, uint32_t parity, unsigned int* st, unsigned int detail,
+// A wait of a warp that computes.  No lane leaves: when the budget runs out the warp goes on over numbers without
+// meaning to the end of its chunk; the flag ends it there, and the warps that load and multiply at once.  (All lanes ask:
+// by the first lane alone, and the others behind a barrier of the warp, a chunk took 400 cycles more.)
+__device__ __forceinline__ void pass_warp(uint64_t* bar, uint32_t parity, unsigned int* st, unsigned int detail,
                                           volatile uint32_t* abort_flag) {
-  return mbar_wait_warp(bar, parity, st, kKernelId, detail, abort_flag);
+  mbar_pass_warp(bar, parity, st, kKernelId, detail, abort_flag);
+}
+__device__ __forceinline__ bool given_up(volatile uint32_t* abort_flag) {
+  return __any_sync(0xffffffffu, *abort_flag != 0u) != 0;
 }
 
 template <int N>
@@ -194,7 +198,7 @@ heads_kernel(const ScanArgs a, const __grid_constant__ CUtensorMap tm_x, const _
     for (int i = 0; i < kBars; ++i) {
       const bool by_warps = i == kYReady0 || i == kYReady1 || (i >= kSFree0 && i <= kSFree3) || i == kMReady ||
                             i == kWReady || i == kHReady || i == kYFree;
-      mbar_init(&bar[i], by_warps ? kWarps : 1);
+      mbar_init(&bar[i], by_warps ? kWarps : i == kXFull0 || i == kXFull1 ? 2 : 1);   // x, and its scalars
     }
     *abort_flag = 0u;
     mbar_fence_init();
@@ -270,11 +274,9 @@ heads_kernel(const ScanArgs a, const __grid_constant__ CUtensorMap tm_x, const _
       const int n = min(kRows, po.end - po.first - c * kRows);
       const Scalars* s = scal + (c & 3);
       unsigned char* x = smem + kOffX + (c & 1) * kSub;
-      if (!wait_warp(&bar[kSFull0 + (c & 3)], (c >> 2) & 1, status, 0x100u, abort_flag) ||
-          !wait_warp(&bar[kXFull0 + (c & 1)], (c >> 1) & 1, status, 0x101u, abort_flag))
-        return false;
+      pass_warp(&bar[kXFull0 + (c & 1)], (c >> 1) & 1, status, 0x101u, abort_flag);
       // rows of other requests: zeros, they may hold anything
-      if (n < kRows && !wait_warp(&bar[kBFull], c & 1, status, 0x102u, abort_flag)) return false;
+      if (n < kRows) pass_warp(&bar[kBFull], c & 1, status, 0x102u, abort_flag);
 #pragma unroll 1
       for (int k = 0; k < w_rows; k += 4) {
         const int row = w_first + k + (lane >> 3);
@@ -303,17 +305,18 @@ heads_kernel(const ScanArgs a, const __grid_constant__ CUtensorMap tm_x, const _
       fence_async_smem();
       __syncwarp();
       if (lane == 0) mbar_arrive(&bar[kWReady]);
-      return true;
     };
 
-    bool ok = chunks == 0 || make_w(0);
-    for (int c = 0; c < chunks && ok; ++c) {
+    if (chunks > 0) make_w(0);
+    bool ok = true;
+    for (int c = 0; c < chunks; ++c) {
+      ok = !given_up(abort_flag);
+      if (!ok) break;
       const int stage = c & 1, four = c & 3, n = min(kRows, po.end - po.first - c * kRows);
       const Scalars* s = scal + four;
       unsigned char* x = smem + kOffX + stage * kSub;
       // M in place of G, every fourth group of 16 columns
-      ok = wait_warp(&bar[kGDone], c & 1, status, 0x103u, abort_flag);
-      if (!ok) break;
+      pass_warp(&bar[kGDone], c & 1, status, 0x103u, abort_flag);
       tc_fence_after();
       {
         const float row = s->row[i], di = s->diag[i], low = s->row_low[i];
@@ -370,8 +373,7 @@ heads_kernel(const ScanArgs a, const __grid_constant__ CUtensorMap tm_x, const _
       if (lane == 0) mbar_arrive(&bar[kMReady]);
 
       // the state behind the chunk
-      ok = wait_warp(&bar[kSDone], c & 1, status, 0x104u, abort_flag);
-      if (!ok) break;
+      pass_warp(&bar[kSDone], c & 1, status, 0x104u, abort_flag);
       tc_fence_after();
       {
         const float keep = s->end[0];
@@ -385,18 +387,11 @@ heads_kernel(const ScanArgs a, const __grid_constant__ CUtensorMap tm_x, const _
                                              add2(bits2(v[1][2 * k], v[1][2 * k + 1]), bits2(v[2][2 * k], v[2][2 * k + 1]))));
       }
       tc_fence_before();
-      // (the products with the state before are through)
-      ok = wait_warp(&bar[kCFree], c & 1, status, 0x106u, abort_flag);
-      if (!ok) break;
       put_state();
-      if (c + 1 < chunks) {                              // (the products with W of this chunk are through)
-        ok = make_w(c + 1);
-        if (!ok) break;
-      }
+      if (c + 1 < chunks) make_w(c + 1);                 // (the products with W of this chunk are through)
 
       // the result's rows
-      ok = wait_warp(&bar[kYDone], c & 1, status, 0x105u, abort_flag);
-      if (!ok) break;
+      pass_warp(&bar[kYDone], c & 1, status, 0x105u, abort_flag);
       tc_fence_after();
       {
         uint32_t y1[16], y2[16], y3[16];
@@ -441,7 +436,7 @@ heads_kernel(const ScanArgs a, const __grid_constant__ CUtensorMap tm_x, const _
         mbar_arrive(&bar[kSFree0 + four]);
       }
     }
-    if (ok && chunks > 0 && ws >= 0 && ws < a.num_slots && i < N) {
+    if (ok && !given_up(abort_flag) && chunks > 0 && ws >= 0 && ws < a.num_slots && i < N) {
 #pragma unroll
       for (int k = 0; k < 16; ++k) a.state[ws * head_at + at + k * N] = k & 1 ? h[k / 2].y : h[k / 2].x;
     }
@@ -479,6 +474,12 @@ heads_kernel(const ScanArgs a, const __grid_constant__ CUtensorMap tm_x, const _
         mbar_expect_tx(&bar[kBFull], kU * kSub);
         for (int u = 0; u < kU; ++u) tma_load_2d(smem + kOffB + u * kSub, &tm_b, &bar[kBFull], group * N + u * 64, y);
         issued = 4 * c + 3;
+        // the next chunk's tiles of B and C to L2: their buffers are free only when this chunk's products are through
+        if (c + 1 < chunks)
+          for (int u = 0; u < kU; ++u) {
+            tma_prefetch_2d(&tm_c, group * N + u * 64, y + kRows);
+            tma_prefetch_2d(&tm_b, group * N + u * 64, y + kRows);
+          }
       }
       for (int c = max(0, chunks - 2); c < chunks && ok; ++c) ok = send(c);
       tma_store_wait<0>();
@@ -519,17 +520,16 @@ heads_kernel(const ScanArgs a, const __grid_constant__ CUtensorMap tm_x, const _
           umma_f16(tmem + kColG, c_k + step, b_k + step, kIdG, k > 0);
         }
         umma_commit(&bar[kGDone]);
-        // (the state is there: S of the chunk before has been read)
-        if (!wait(kHReady, ph, 2) || !wait(kWReady, ph, 4)) break;
-#pragma unroll
-        for (int k = 0; k < 8; ++k) umma_f16(tmem + kColS, b_mn + k * kStep, w_mn + k * kStep, kIdS, k > 0);
-        umma_commit(&bar[kBFree]);
-        umma_commit(&bar[kSDone]);
-        if (c > 0 && !wait(kYFree, ph ^ 1, 3)) break;
+        if (!wait(kHReady, ph, 2) || (c > 0 && !wait(kYFree, ph ^ 1, 3))) break;
 #pragma unroll
         for (int k = 0; k < N / 16; ++k)
           umma_f16(tmem + kColY2, c_k + (k >> 2) * (kSub >> 4) + (k & 3) * 2, h_mn + k * kStep, kIdY2, k > 0);
         umma_commit(&bar[kCFree]);
+        if (!wait(kWReady, ph, 4)) break;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) umma_f16(tmem + kColS, b_mn + k * kStep, w_mn + k * kStep, kIdS, k > 0);
+        umma_commit(&bar[kBFree]);
+        umma_commit(&bar[kSDone]);                       // (and Y2: the state may be replaced)
         if (!wait(kMReady, ph, 5)) break;
         const uint64_t x = x_mn + (c & 1) * (kSub >> 4);
 #pragma unroll
@@ -551,10 +551,13 @@ heads_kernel(const ScanArgs a, const __grid_constant__ CUtensorMap tm_x, const _
     if (first < chunks) load_steps(a, hd, po.first + first * kRows, rows(first), z);
     for (int c = first; c < chunks; c += kScal) {
       if (c + kScal < chunks) load_steps(a, hd, po.first + (c + kScal) * kRows, rows(c + kScal), next);
-      if (c >= 4 && !wait_warp(&bar[kSFree0 + (c & 3)], ((c >> 2) & 1) ^ 1, status, 0x400u, abort_flag)) break;
+      if (c >= 4) pass_warp(&bar[kSFree0 + (c & 3)], ((c >> 2) & 1) ^ 1, status, 0x400u, abort_flag);
+      if (given_up(abort_flag)) break;
       chunk_scalars(a, rows(c), bias, rate, z, scal + (c & 3));
       __syncwarp();
-      if (lane == 0) mbar_arrive(&bar[kSFull0 + (c & 3)]);
+      // (the barrier's turn before, two chunks ago, is over)
+      if (c >= 2) pass_warp(&bar[kXFull0 + (c & 1)], ((c >> 1) & 1) ^ 1, status, 0x401u, abort_flag);
+      if (lane == 0) mbar_arrive(&bar[kXFull0 + (c & 1)]);
 #pragma unroll
       for (int k = 0; k < 4; ++k) z[k] = next[k];
     }
