@@ -174,9 +174,14 @@ __device__ __forceinline__ void chunk_scalars(const ScanArgs& a, int n, float bi
 // A wait of a warp that computes.  No lane leaves: when the budget runs out the warp goes on over numbers without
 // meaning to the end of its chunk; the flag ends it there, and the warps that load and multiply at once.  (All lanes ask:
 // by the first lane alone, and the others behind a barrier of the warp, a chunk took 400 cycles more.)
+__device__ __noinline__ bool wait_for(uint64_t* bar, uint32_t parity, unsigned int* st, unsigned int detail,
+                                      volatile uint32_t* abort_flag) {
+  return mbar_wait(bar, parity, st, kKernelId, detail, abort_flag);
+}
 __device__ __forceinline__ void pass_warp(uint64_t* bar, uint32_t parity, unsigned int* st, unsigned int detail,
                                           volatile uint32_t* abort_flag) {
-  mbar_pass_warp(bar, parity, st, kKernelId, detail, abort_flag);
+  if (!mbar_test(bar, parity)) wait_for(bar, parity, st, detail, abort_flag);
+  __syncwarp();
 }
 __device__ __forceinline__ bool given_up(volatile uint32_t* abort_flag) {
   return __any_sync(0xffffffffu, *abort_flag != 0u) != 0;
@@ -431,10 +436,7 @@ heads_kernel(const ScanArgs a, const __grid_constant__ CUtensorMap tm_x, const _
       }
       fence_async_smem();
       __syncwarp();
-      if (lane == 0) {
-        mbar_arrive(&bar[kYReady0 + stage]);
-        mbar_arrive(&bar[kSFree0 + four]);
-      }
+      if (lane < 2) mbar_arrive(&bar[lane == 0 ? kYReady0 + stage : kSFree0 + four]);
     }
     if (ok && !given_up(abort_flag) && chunks > 0 && ws >= 0 && ws < a.num_slots && i < N) {
 #pragma unroll
@@ -446,7 +448,7 @@ heads_kernel(const ScanArgs a, const __grid_constant__ CUtensorMap tm_x, const _
       int issued = 0;
       // the result of chunk c, which lies in place of its x, to memory
       auto send = [&](int c) {
-        if (!mbar_wait(&bar[kYReady0 + (c & 1)], (c >> 1) & 1, status, kKernelId, 0x200u, abort_flag)) return false;
+        if (!wait_for(&bar[kYReady0 + (c & 1)], (c >> 1) & 1, status, 0x200u, abort_flag)) return false;
         if (po.end - po.first - c * kRows >= kRows) {
           tma_store_2d(&tm_y, smem + kOffX + (c & 1) * kSub, col0, po.first + c * kRows);
           tma_store_commit();
@@ -464,12 +466,12 @@ heads_kernel(const ScanArgs a, const __grid_constant__ CUtensorMap tm_x, const _
         mbar_expect_tx(&bar[kXFull0 + stage], kSub);
         tma_load_2d(smem + kOffX + stage * kSub, &tm_x, &bar[kXFull0 + stage], col0, y);
         issued = 4 * c + 1;
-        ok = c < 1 || mbar_wait(&bar[kCFree], (c - 1) & 1, status, kKernelId, 0x201u, abort_flag);
+        ok = c < 1 || wait_for(&bar[kCFree], (c - 1) & 1, status, 0x201u, abort_flag);
         if (!ok) break;
         mbar_expect_tx(&bar[kCFull], kU * kSub);
         for (int u = 0; u < kU; ++u) tma_load_2d(smem + kOffC + u * kSub, &tm_c, &bar[kCFull], group * N + u * 64, y);
         issued = 4 * c + 2;
-        ok = c < 1 || mbar_wait(&bar[kBFree], (c - 1) & 1, status, kKernelId, 0x202u, abort_flag);
+        ok = c < 1 || wait_for(&bar[kBFree], (c - 1) & 1, status, 0x202u, abort_flag);
         if (!ok) break;
         mbar_expect_tx(&bar[kBFull], kU * kSub);
         for (int u = 0; u < kU; ++u) tma_load_2d(smem + kOffB + u * kSub, &tm_b, &bar[kBFull], group * N + u * 64, y);
@@ -486,10 +488,10 @@ heads_kernel(const ScanArgs a, const __grid_constant__ CUtensorMap tm_x, const _
       // copies in flight end before the CTA does, also when a wait ran out
       if (*abort_flag != 0u && issued > 0) {
         const int c = issued >> 2, what = issued & 3;
-        mbar_wait(&bar[kXFull0 + (c & 1)], (c >> 1) & 1, status, kKernelId, 0x210u);
-        if (c >= 1) mbar_wait(&bar[kXFull0 + ((c - 1) & 1)], ((c - 1) >> 1) & 1, status, kKernelId, 0x211u);
-        if (what >= 2 || c >= 1) mbar_wait(&bar[kCFull], (what >= 2 ? c : c - 1) & 1, status, kKernelId, 0x212u);
-        if (what >= 3 || c >= 1) mbar_wait(&bar[kBFull], (what >= 3 ? c : c - 1) & 1, status, kKernelId, 0x213u);
+        wait_for(&bar[kXFull0 + (c & 1)], (c >> 1) & 1, status, 0x210u, nullptr);
+        if (c >= 1) wait_for(&bar[kXFull0 + ((c - 1) & 1)], ((c - 1) >> 1) & 1, status, 0x211u, nullptr);
+        if (what >= 2 || c >= 1) wait_for(&bar[kCFull], (what >= 2 ? c : c - 1) & 1, status, 0x212u, nullptr);
+        if (what >= 3 || c >= 1) wait_for(&bar[kBFull], (what >= 3 ? c : c - 1) & 1, status, 0x213u, nullptr);
       }
     }
   } else if (warp == kWarps + 1) {
@@ -507,7 +509,7 @@ heads_kernel(const ScanArgs a, const __grid_constant__ CUtensorMap tm_x, const _
       const uint64_t w_mn = make_desc_mn_sw128(base + kOffW, kSub), h_mn = make_desc_mn_sw128(base + kOffH, kSub);
       const uint64_t x_mn = make_desc_mn_sw128(base + kOffX, kSub);
       auto wait = [&](int b, int parity, uint32_t what) {
-        const bool there = mbar_wait(&bar[b], parity, status, kKernelId, 0x300u + what, abort_flag);
+        const bool there = wait_for(&bar[b], parity, status, 0x300u + what, abort_flag);
         tc_fence_after();
         return there;
       };
@@ -542,8 +544,8 @@ heads_kernel(const ScanArgs a, const __grid_constant__ CUtensorMap tm_x, const _
     }
   } else {
     // ---------------- step sizes and decays ----------------
-    const double rate2 = -exp(static_cast<double>(a.a_log[hd])) * 1.4426950408889634;
-    const Two rate = {static_cast<float>(rate2), static_cast<float>(rate2 - static_cast<double>(static_cast<float>(rate2)))};
+    const float per = -expf(a.a_log[hd]);
+    const Two rate = {per * kLog2e, fmaf(per, kLog2e, -(per * kLog2e)) + per * 1.925963033e-8f};
     const float bias = a.dt_bias != nullptr ? a.dt_bias[hd] : 0.0f;
     auto rows = [&](int c) { return min(kRows, po.end - po.first - c * kRows); };
     float z[4], next[4];
