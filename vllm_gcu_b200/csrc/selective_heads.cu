@@ -269,7 +269,6 @@ heads_kernel(const ScanArgs a, const __grid_constant__ CUtensorMap tm_x, const _
       __syncwarp();
       if (lane == 0) mbar_arrive(&bar[kHReady]);
     };
-    put_state();
     const float skip = a.d != nullptr ? a.d[hd] : 0.0f;
     // 4 rows of W at a time, in groups of 12, 8, 8 and 4 rows for the warps of the four quarters
     const int w_rows = q == 0 ? 12 : q == 3 ? 4 : 8;
@@ -312,14 +311,15 @@ heads_kernel(const ScanArgs a, const __grid_constant__ CUtensorMap tm_x, const _
       if (lane == 0) mbar_arrive(&bar[kWReady]);
     };
 
-    if (chunks > 0) make_w(0);
-    bool ok = true;
-    for (int c = 0; c < chunks; ++c) {
-      ok = !given_up(abort_flag);
-      if (!ok) break;
+    // (turn -1: the state in front and W of the first chunk; one copy of the code for both: the kernel's instructions
+    // are more than their caches hold, and what does not fit costs every warp)
+#pragma unroll 1
+    for (int c = -1; c < chunks; ++c) {
+      if (given_up(abort_flag)) break;
       const int stage = c & 1, four = c & 3, n = min(kRows, po.end - po.first - c * kRows);
       const Scalars* s = scal + four;
       unsigned char* x = smem + kOffX + stage * kSub;
+      if (c >= 0) {
       // M in place of G, every fourth group of 16 columns
       pass_warp(&bar[kGDone], c & 1, status, 0x103u, abort_flag);
       tc_fence_after();
@@ -392,8 +392,10 @@ heads_kernel(const ScanArgs a, const __grid_constant__ CUtensorMap tm_x, const _
                                              add2(bits2(v[1][2 * k], v[1][2 * k + 1]), bits2(v[2][2 * k], v[2][2 * k + 1]))));
       }
       tc_fence_before();
+      }
       put_state();
       if (c + 1 < chunks) make_w(c + 1);                 // (the products with W of this chunk are through)
+      if (c < 0) continue;
 
       // the result's rows
       pass_warp(&bar[kYDone], c & 1, status, 0x105u, abort_flag);
@@ -438,7 +440,7 @@ heads_kernel(const ScanArgs a, const __grid_constant__ CUtensorMap tm_x, const _
       __syncwarp();
       if (lane < 2) mbar_arrive(&bar[lane == 0 ? kYReady0 + stage : kSFree0 + four]);
     }
-    if (ok && !given_up(abort_flag) && chunks > 0 && ws >= 0 && ws < a.num_slots && i < N) {
+    if (!given_up(abort_flag) && chunks > 0 && ws >= 0 && ws < a.num_slots && i < N) {
 #pragma unroll
       for (int k = 0; k < 16; ++k) a.state[ws * head_at + at + k * N] = k & 1 ? h[k / 2].y : h[k / 2].x;
     }
@@ -476,7 +478,9 @@ heads_kernel(const ScanArgs a, const __grid_constant__ CUtensorMap tm_x, const _
         mbar_expect_tx(&bar[kBFull], kU * kSub);
         for (int u = 0; u < kU; ++u) tma_load_2d(smem + kOffB + u * kSub, &tm_b, &bar[kBFull], group * N + u * 64, y);
         issued = 4 * c + 3;
-        // the next chunk's tiles of B and C to L2: their buffers are free only when this chunk's products are through
+        // the next chunk's tiles of B and C to L2: their buffers are free only when this chunk's products are through;
+        // x of the chunk behind it
+        if (c + 2 < chunks) tma_prefetch_2d(&tm_x, col0, y + 2 * kRows);
         if (c + 1 < chunks)
           for (int u = 0; u < kU; ++u) {
             tma_prefetch_2d(&tm_c, group * N + u * 64, y + kRows);
@@ -516,25 +520,25 @@ heads_kernel(const ScanArgs a, const __grid_constant__ CUtensorMap tm_x, const _
       for (int c = 0; c < chunks; ++c) {
         const int ph = c & 1;
         if (!wait(kCFull, ph, 0) || !wait(kBFull, ph, 1)) break;
-#pragma unroll
+#pragma unroll 1
         for (int k = 0; k < N / 16; ++k) {
           const uint32_t step = (k >> 2) * (kSub >> 4) + (k & 3) * 2;
           umma_f16(tmem + kColG, c_k + step, b_k + step, kIdG, k > 0);
         }
         umma_commit(&bar[kGDone]);
         if (!wait(kHReady, ph, 2) || (c > 0 && !wait(kYFree, ph ^ 1, 3))) break;
-#pragma unroll
+#pragma unroll 1
         for (int k = 0; k < N / 16; ++k)
           umma_f16(tmem + kColY2, c_k + (k >> 2) * (kSub >> 4) + (k & 3) * 2, h_mn + k * kStep, kIdY2, k > 0);
         umma_commit(&bar[kCFree]);
         if (!wait(kWReady, ph, 4)) break;
-#pragma unroll
+#pragma unroll 1
         for (int k = 0; k < 8; ++k) umma_f16(tmem + kColS, b_mn + k * kStep, w_mn + k * kStep, kIdS, k > 0);
         umma_commit(&bar[kBFree]);
         umma_commit(&bar[kSDone]);                       // (and Y2: the state may be replaced)
         if (!wait(kMReady, ph, 5)) break;
         const uint64_t x = x_mn + (c & 1) * (kSub >> 4);
-#pragma unroll
+#pragma unroll 1
         for (int k = 0; k < 8; ++k) {
           umma_f16_ts(tmem + kColY1, tmem + kColG + 16 * k, x + k * kStep, kIdY1, k > 0);
           umma_f16_ts(tmem + kColY1, tmem + kColG + 16 * k + 8, x + k * kStep, kIdY1, 1);
