@@ -221,22 +221,32 @@ int launch_any(const Args& a, bool wide, cudaStream_t s) {
 }  // namespace gated_norm
 }  // namespace b200
 
-// dtype: 0 bf16, 1 fp16, 2 fp32 rows; act: 0 none, 1 SiLU, 2 sigmoid; wide: parts of rows may be read 16 bytes
-// at a time.
-B200_API int b200_group_norm_gate(const void* x, long long ldx, const void* z, long long ldz, const float* w,
-                                  const float* bias, void* out, long long ldo, float eps, int T, int C, int groups,
-                                  int act, int center, int after, int wide, int dtype, void* stream) {
+// The arguments of a call, packed by the launcher (ops/cuda.py).  dtype: 0 bf16, 1 fp16, 2 fp32 rows; act: 0 none,
+// 1 SiLU, 2 sigmoid; wide: parts of rows may be read 16 bytes at a time.
+namespace {
+struct NormCall {
+  const void *x, *z;
+  void* out;
+  const float *w, *bias;
+  long long ldx, ldz, ldo;
+  float eps;
+  int T, C, groups, act, center, after, wide, dtype;
+};
+}  // namespace
+
+B200_API int b200_group_norm_gate(const void* call, void* stream) {
   using namespace b200::gated_norm;
-  if (T <= 0 || C <= 0) return 0;
-  const long long parts = static_cast<long long>(T) * groups;
-  if (groups <= 0 || C % groups != 0 || parts > 0x7fffffffll) return -8;
-  const Args a{x, z, out, w, bias, ldx, ldz, ldo, eps, T, C, groups, C / groups, act, center, after,
-               static_cast<int>(parts)};
+  const NormCall& k = *static_cast<const NormCall*>(call);
+  if (k.T <= 0 || k.C <= 0) return 0;
+  const long long parts = static_cast<long long>(k.T) * k.groups;
+  if (k.groups <= 0 || k.C % k.groups != 0 || parts > 0x7fffffffll) return -8;
+  const Args a{k.x, k.z, k.out, k.w, k.bias, k.ldx, k.ldz, k.ldo, k.eps, k.T, k.C, k.groups, k.C / k.groups, k.act,
+               k.center, k.after, static_cast<int>(parts)};
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  switch (dtype) {
-    case 0: return launch_any<__nv_bfloat16>(a, wide, s);
-    case 1: return launch_any<__half>(a, wide, s);
-    case 2: return launch_any<float>(a, wide, s);
+  switch (k.dtype) {
+    case 0: return launch_any<__nv_bfloat16>(a, k.wide, s);
+    case 1: return launch_any<__half>(a, k.wide, s);
+    case 2: return launch_any<float>(a, k.wide, s);
   }
   return -8;
 }

@@ -359,7 +359,7 @@ __global__ void __launch_bounds__(128) channels_step_kernel(const ScanArgs a) {
   const int r0 = blockIdx.y * RQ;
   const long long pitch = static_cast<long long>(cols) * a.N, at = static_cast<long long>(col) * a.N + n;
   float4 h[RQ], b[RQ], c[RQ];
-  float x[RQ], dt[RQ];
+  float x[RQ], dt[RQ], z[RQ];
   int ws[RQ];
   bool padding[RQ];
 #pragma unroll
@@ -379,6 +379,7 @@ __global__ void __launch_bounds__(128) channels_step_kernel(const ScanArgs a) {
     x[i] = to_f32<T>(static_cast<const T*>(a.x)[r * a.ldx + col]);
     dt[i] = a.dt_f32 ? static_cast<const float*>(a.dt)[r * a.lddt + col]
                      : to_f32<T>(static_cast<const T*>(a.dt)[r * a.lddt + col]);
+    z[i] = a.z != nullptr ? to_f32<T>(static_cast<const T*>(a.z)[r * a.ldz + col]) : 0.0f;
     b[i] = load_four<T, WIDE>(static_cast<const T*>(a.b) + r * a.ldb + g * a.N + n, in);
     c[i] = load_four<T, WIDE>(static_cast<const T*>(a.c) + r * a.ldc + g * a.N + n, in);
   }
@@ -402,16 +403,17 @@ __global__ void __launch_bounds__(128) channels_step_kernel(const ScanArgs a) {
   for (int i = 0; i < sums.kLeft; ++i) {
     const int k = sums.first + i, r = r0 + k;
     if (!mine || !sums.keeps(l) || r >= a.nd) continue;
-    float xv = 0.0f;
+    float xv = 0.0f, zv = 0.0f;
     bool none = false;
 #pragma unroll
     for (int m = 0; m < RQ; ++m)
       if (m == k) {
         xv = x[m];
+        zv = z[m];
         none = padding[m];
       }
     float y = fmaf(skip, xv, sums.v[i]);
-    if (a.z != nullptr) y *= silu<T>(to_f32<T>(static_cast<const T*>(a.z)[r * a.ldz + col]));
+    if (a.z != nullptr) y *= silu<T>(zv);
     static_cast<T*>(a.out)[r * a.ldo + col] = from_f32<T>(none ? 0.0f : y);
   }
 }
@@ -944,12 +946,12 @@ int launch_channels_step(const ScanArgs& a, cudaStream_t s) {
   return a.wide ? launch_overlapped(channels_step_kernel<T, LPR, RQ, true>, grid, dim3(128), 0, s, a)
                 : launch_overlapped(channels_step_kernel<T, LPR, RQ, false>, grid, dim3(128), 0, s, a);
 }
-// Requests that share a warp: as many as leave eight warps to an SM.
+// Requests that share a warp: four where that leaves eight warps to an SM (64 requests of 8192 channels of 16: two and
+// four 24 us, eight, whose registers leave 12 warps an SM, 34).
 template <typename T, int LPR>
 int launch_channels_step(const ScanArgs& a, cudaStream_t s) {
   const long long warps = (static_cast<long long>(a.heads) * a.width + 32 / LPR - 1) / (32 / LPR);
   auto enough = [&](int rq) { return warps * ((a.nd + rq - 1) / rq) >= 8ll * sm_count(); };
-  if (enough(8)) return launch_channels_step<T, LPR, 8>(a, s);
   if (enough(4)) return launch_channels_step<T, LPR, 4>(a, s);
   return launch_channels_step<T, LPR, 1>(a, s);
 }
@@ -1032,52 +1034,72 @@ int scan_any(const ScanArgs& a, cudaStream_t s) {
 }  // namespace selective
 }  // namespace b200
 
-// Short causal convolution of a step's rows.  dtype: 0 bf16, 1 fp16, 2 fp32; taps 1 .. 8; wide: rows, ring,
-// weights, bias and out may be read four elements at a time.  ring may be null (every portion starts from zeros).
-B200_API int b200_causal_conv(const void* x, long long ldx, const float* w, int taps, const float* bias, void* ring,
-                              int num_slots, const long long* positions, const int* slots, const int* wslots,
-                              const int* cu_q, void* out, long long ldo, int T, int C, int nd, int np, int silu,
-                              int wide, int dtype, void* stream) {
+// The arguments of a call come packed, as the launchers pack them (ops/cuda.py): converting each of them one by one took
+// longer than the kernels of small steps.
+namespace {
+struct ConvCall {
+  const void* x;
+  const float *w, *bias;
+  void *ring, *out;
+  const long long* positions;
+  const int *slots, *wslots, *cu_q;
+  long long ldx, ldo;
+  int taps, num_slots, T, C, nd, np, silu, wide, dtype;
+};
+struct ScanCall {
+  const void *x, *dt, *b, *c, *z;
+  void* out;
+  const float *a_log, *d, *dt_bias;
+  float* state;
+  const long long* positions;
+  const int *slots, *wslots, *cu_q;
+  long long ldx, lddt, ldb, ldc, ldz, ldo;
+  float dt_min, dt_max;
+  int dt_f32, per_channel, softplus, num_slots, T, heads, width, N, groups, nd, np, wide, dtype;
+};
+}  // namespace
+
+// Short causal convolution of a step's rows.  dtype: 0 bf16, 1 fp16, 2 fp32; taps 1 .. 8; wide: rows, ring, weights, bias
+// and out may be read four elements at a time.  ring may be null (every portion starts from zeros).
+B200_API int b200_causal_conv(const void* call, void* stream) {
   using namespace b200::selective;
-  if (T <= 0 || C <= 0 || nd + np <= 0) return 0;
+  const ConvCall& k = *static_cast<const ConvCall*>(call);
+  if (k.T <= 0 || k.C <= 0 || k.nd + k.np <= 0) return 0;
   ConvArgs a;
-  a.x = x; a.w = w; a.bias = bias; a.ring = taps > 1 ? ring : nullptr; a.out = out; a.positions = positions;
-  a.slots = slots; a.wslots = wslots; a.cu_q = cu_q; a.ldx = ldx; a.ldo = ldo; a.T = T; a.C = C;
-  a.num_slots = num_slots; a.nd = nd; a.np = np; a.silu = silu;
+  a.x = k.x; a.w = k.w; a.bias = k.bias; a.ring = k.taps > 1 ? k.ring : nullptr; a.out = k.out;
+  a.positions = k.positions; a.slots = k.slots; a.wslots = k.wslots; a.cu_q = k.cu_q; a.ldx = k.ldx; a.ldo = k.ldo;
+  a.T = k.T; a.C = k.C; a.num_slots = k.num_slots; a.nd = k.nd; a.np = k.np; a.silu = k.silu; a.strip = 0;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  switch (dtype) {
-    case 0: return conv_any<__nv_bfloat16>(a, taps, wide, s);
-    case 1: return conv_any<__half>(a, taps, wide, s);
-    case 2: return conv_any<float>(a, taps, wide, s);
+  switch (k.dtype) {
+    case 0: return conv_any<__nv_bfloat16>(a, k.taps, k.wide, s);
+    case 1: return conv_any<__half>(a, k.taps, k.wide, s);
+    case 2: return conv_any<float>(a, k.taps, k.wide, s);
   }
   return -8;
 }
 
 // Selective scan of a step's rows; per_channel: a_log [heads * width, N] and a step size per column, else
-// a_log [heads] and a step size per head.  state may be null (every portion starts from zeros).
-B200_API int b200_selective_scan(const void* x, long long ldx, const void* dt, long long lddt, int dt_f32,
-                                 const void* b, long long ldb, const void* c, long long ldc, const void* z,
-                                 long long ldz, const float* a_log, int per_channel, const float* d,
-                                 const float* dt_bias, int softplus, float dt_min, float dt_max, float* state,
-                                 int num_slots, const long long* positions, const int* slots, const int* wslots,
-                                 const int* cu_q, void* out, long long ldo, int T, int heads, int width, int N,
-                                 int groups, int nd, int np, int wide, int dtype, void* stream) {
+// a_log [heads] and a step size per head.  state may be null (every portion starts from zeros).  wide: rows of x, b,
+// c, z and out start on 16-byte boundaries.
+B200_API int b200_selective_scan(const void* call, void* stream) {
   using namespace b200::selective;
-  if (T <= 0 || heads <= 0 || width <= 0 || nd + np <= 0) return 0;
-  if (N < 1 || N > 256) return -8;
+  const ScanCall& k = *static_cast<const ScanCall*>(call);
+  if (k.T <= 0 || k.heads <= 0 || k.width <= 0 || k.nd + k.np <= 0) return 0;
+  if (k.N < 1 || k.N > 256) return -8;
   ScanArgs a;
-  a.x = x; a.dt = dt; a.b = b; a.c = c; a.z = z; a.out = out; a.a_log = a_log; a.d = d; a.dt_bias = dt_bias;
-  a.state = state; a.positions = positions; a.slots = slots; a.wslots = wslots; a.cu_q = cu_q;
-  a.ldx = ldx; a.lddt = lddt; a.ldb = ldb; a.ldc = ldc; a.ldz = ldz; a.ldo = ldo;
-  a.dt_min = dt_min; a.dt_max = dt_max; a.T = T; a.heads = heads; a.width = width; a.N = N; a.groups = groups;
-  a.num_slots = num_slots; a.nd = nd; a.np = np; a.dt_f32 = dt_f32; a.softplus = softplus;
-  a.wide = wide;
-  a.limits = dt_max < INFINITY || dt_min > 0.0f || !softplus;    // (a softplus is not below 0)
+  a.x = k.x; a.dt = k.dt; a.b = k.b; a.c = k.c; a.z = k.z; a.out = k.out; a.a_log = k.a_log; a.d = k.d;
+  a.dt_bias = k.dt_bias; a.state = k.state; a.positions = k.positions; a.slots = k.slots; a.wslots = k.wslots;
+  a.cu_q = k.cu_q; a.ldx = k.ldx; a.lddt = k.lddt; a.ldb = k.ldb; a.ldc = k.ldc; a.ldz = k.ldz; a.ldo = k.ldo;
+  a.dt_min = k.dt_min; a.dt_max = k.dt_max; a.T = k.T; a.heads = k.heads; a.width = k.width; a.N = k.N;
+  a.groups = k.groups; a.num_slots = k.num_slots; a.nd = k.nd; a.np = k.np; a.dt_f32 = k.dt_f32;
+  a.softplus = k.softplus; a.wide = k.wide;
+  a.limits = k.dt_max < INFINITY || k.dt_min > 0.0f || !k.softplus;    // (a softplus is not below 0)
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  switch (dtype) {
-    case 0: return per_channel ? scan_any<__nv_bfloat16, true>(a, s) : scan_any<__nv_bfloat16, false>(a, s);
-    case 1: return per_channel ? scan_any<__half, true>(a, s) : scan_any<__half, false>(a, s);
-    case 2: return per_channel ? scan_any<float, true>(a, s) : scan_any<float, false>(a, s);
+  const bool channels = k.per_channel != 0;
+  switch (k.dtype) {
+    case 0: return channels ? scan_any<__nv_bfloat16, true>(a, s) : scan_any<__nv_bfloat16, false>(a, s);
+    case 1: return channels ? scan_any<__half, true>(a, s) : scan_any<__half, false>(a, s);
+    case 2: return channels ? scan_any<float, true>(a, s) : scan_any<float, false>(a, s);
   }
   return -8;
 }

@@ -89,6 +89,7 @@ P = ctypes.c_void_p
 I = ctypes.c_int
 L = ctypes.c_longlong
 F = ctypes.c_float
+S = ctypes.c_char_p                   # arguments packed into one structure
 
 
 class _Sigs:
@@ -171,10 +172,9 @@ class _Sigs:
                        F, F, I, I, I, I, I, I, I, P]
     b200_memory_step = [P, L, I, P, P, P, P, L, P, P, P, P, F, F, P, P, P, P, P, P, I, P, L, F, F,
                         I, I, I, I, I, I, P]
-    b200_causal_conv = [P, L, P, I, P, P, I, P, P, P, P, P, L, I, I, I, I, I, I, I, P]
-    b200_selective_scan = [P, L, P, L, I, P, L, P, L, P, L, P, I, P, P, I, F, F, P, I, P, P, P, P, P, L,
-                           I, I, I, I, I, I, I, I, I, P]
-    b200_group_norm_gate = [P, L, P, L, P, P, P, L, F, I, I, I, I, I, I, I, I, P]
+    b200_causal_conv = [S, P]
+    b200_selective_scan = [S, P]
+    b200_group_norm_gate = [S, P]
     b200_gemm_wna16 = [P, L, P, P, P, P, P, L, I, I, I, I, I, P]
     b200_gemm_wna16_grouped = [P, L, P, P, P, P, L, I, I, I, I, I, I, P, P, P, P]
     b200_sample = [P, L, I, I, I, P, P, P, P, P, L, P, P]

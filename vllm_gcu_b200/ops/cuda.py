@@ -8,6 +8,8 @@ from __future__ import annotations
 
 import ctypes
 import functools
+import math
+import struct
 from typing import Optional, Sequence
 
 import torch
@@ -1573,14 +1575,20 @@ def memory_step(h: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Tens
 # ---------------------------------------------------------------------------
 # state-space mixers (csrc/selective.cu, csrc/group_norm_gate.cu)
 # ---------------------------------------------------------------------------
+# Arguments of a call, packed: one after the other, ctypes takes 4 us for the scan's, as long as a small step's kernel runs.
+_CONV_CALL = struct.Struct("9P2q9i")
+_SCAN_CALL = struct.Struct("14P6q2f13i")
+_NORM_CALL = struct.Struct("5P3qf8i")
+
+
 def _row_view(name: str, t: torch.Tensor, rows: int, cols: int, dtypes, dev: int) -> int:
     """Checks a row-strided view [rows, cols] of one of ``dtypes`` as the state-space kernels take it; its row pitch.
     (One expression where all is well: a call has up to a dozen tensors, and single tokens take microseconds.)"""
-    ld, step = t.stride() if t.dim() == 2 else (0, 0)
-    if t.shape == (rows, cols) and t.dtype in dtypes and t.get_device() == dev and (step == 1 or cols == 1):
-        return ld
     if t.shape != (rows, cols):
         raise ValueError(f"{name} has shape {tuple(t.shape)}, not {(rows, cols)}")
+    ld, step = t.stride()
+    if t.dtype in dtypes and t.get_device() == dev and (step == 1 or cols == 1):
+        return ld
     if t.dtype not in dtypes:
         raise ValueError(f"{name} is {t.dtype}, not {' or '.join(map(str, dtypes))}")
     if t.get_device() != dev:
@@ -1610,13 +1618,13 @@ def _overlap(a: tuple, b: tuple) -> bool:
 def _target(out: torch.Tensor, rows: int, cols: int, dtype, dev: int, inputs, same_is_fine: bool = False
             ) -> tuple[int, int]:
     """Checks the rows that a kernel writes: no two of them share elements, and none of them meets an input
-    (``inputs``: name, address or None, row pitch, columns, element size); their address and pitch."""
+    (``inputs``: name, address or 0, row pitch, columns, element size); their address and pitch."""
     ld, at, es = _row_view("out", out, rows, cols, (dtype,), dev), out.data_ptr(), dtype.itemsize
     if rows > 1 and ld < cols:
         raise ValueError(f"out: rows of {cols} columns are {ld} elements apart")
     end = at + ((rows - 1) * ld + cols) * es
     for name, p, pitch, width, size in inputs:
-        if p is None or p >= end or p + ((rows - 1) * pitch + width) * size <= at \
+        if not p or p >= end or p + ((rows - 1) * pitch + width) * size <= at \
                 or same_is_fine and p == at and (pitch == ld or rows == 1):
             continue
         if _overlap((at, ld, rows, cols, es), (p, pitch, rows, width, size)):
@@ -1637,7 +1645,7 @@ def _step_place(md, T: int, kept: bool, write_slots: Optional[torch.Tensor], dev
         n += cu.shape[0] - 1
         cu = cu.data_ptr()
     if not kept:
-        return nd, n - nd, cu, None, None, None
+        return nd, n - nd, cu or 0, 0, 0, 0
     pos, slots = md.positions, md.state_slots
     if slots is None:
         raise ValueError("a state needs md.state_slots")
@@ -1649,18 +1657,18 @@ def _step_place(md, T: int, kept: bool, write_slots: Optional[torch.Tensor], dev
                               or not t.is_contiguous()):
             raise ValueError(f"{name}: {n} int32 slots beside x are wanted")
     slots = slots.data_ptr()
-    return nd, n - nd, cu, pos.data_ptr(), slots, slots if write_slots is None else write_slots.data_ptr()
+    return nd, n - nd, cu or 0, pos.data_ptr(), slots, slots if write_slots is None else write_slots.data_ptr()
 
 
-def _call_on(dev: int, name: str, *args) -> None:
+def _call_on(dev: int, name: str, packed: bytes) -> None:
     """A launch on the current stream of the tensors' device."""
     if dev < 0:
         raise ValueError("tensors on a GPU are wanted")
     if dev == torch._C._cuda_getDevice():
-        call(name, *args, stream_ptr())
+        call(name, packed, torch._C._cuda_getCurrentRawStream(dev))
         return
     with torch.cuda.device(dev):
-        call(name, *args, stream_ptr())
+        call(name, packed, stream_ptr())
 
 
 def causal_conv(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor], md,
@@ -1693,16 +1701,17 @@ def causal_conv(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tens
         if taps == 1:
             ring = None
     nd, npf, cu, pos, read, write = _step_place(md, T, ring is not None, write_slots, dev)
-    px, pw, pr, es = x.data_ptr(), weight.data_ptr(), None if ring is None else ring.data_ptr(), dtype.itemsize
+    px, pw, pr, es = x.data_ptr(), weight.data_ptr(), 0 if ring is None else ring.data_ptr(), dtype.itemsize
     if out is None:
         out = torch.empty((T, Ch), dtype=dtype, device=x.device)
         po, ldo = out.data_ptr(), Ch
     else:
         po, ldo = _target(out, T, Ch, dtype, dev, (("x", px, ldx, Ch, es),))
-    pb = None if bias is None else bias.data_ptr()
-    wide = Ch % 4 == 0 and (px | pw | (pb or 0) | (pr or 0) | po) % 16 == 0 and (T == 1 or (ldx | ldo) % 4 == 0)
-    _call_on(dev, "b200_causal_conv", px, ldx, pw, taps, pb, pr, slots, pos, read,
-             write, cu, po, ldo, T, Ch, nd, npf, act is not None, wide, DTYPE_CODE[dtype])
+    pb = 0 if bias is None else bias.data_ptr()
+    wide = Ch % 4 == 0 and (px | pw | pb | pr | po) % 16 == 0 and (T == 1 or (ldx | ldo) % 4 == 0)
+    _call_on(dev, "b200_causal_conv",
+             _CONV_CALL.pack(px, pw, pb, pr, po, pos, read, write, cu, ldx, ldo, taps, slots, T, Ch, nd, npf,
+                             act is not None, wide, DTYPE_CODE[dtype]))
     return out
 
 
@@ -1737,8 +1746,9 @@ def selective_scan(x: torch.Tensor, dt: torch.Tensor, b: torch.Tensor, c: torch.
     if not 1 <= N <= 256:
         raise ValueError(f"a state of {N} numbers per column, 1 to 256 are built")
     lo, hi = dt_limits
-    if not lo <= hi:
+    if not lo <= hi or abs(lo) > 3e38:
         raise ValueError(f"dt_limits {dt_limits}")
+    hi = hi if hi < 3e38 else math.inf
     _whole("a_log", a_log, (rates, N) if channels else (rates,), f32, dev)
     own = (dtype,)
     ldx = _row_view("x", x, T, cols, own, dev)
@@ -1751,7 +1761,7 @@ def selective_scan(x: torch.Tensor, dt: torch.Tensor, b: torch.Tensor, c: torch.
     if dt_bias is not None:
         _whole("dt_bias", dt_bias, (rates,), f32, dev)
     heads, width = (groups, cols // groups) if channels else (rates, cols // rates)
-    slots, ps = 0, None
+    slots, ps = 0, 0
     if state is not None:
         slots, ps = state.shape[0], state.data_ptr()
         _whole("state", state, (slots, cols, N) if channels else (slots, rates, width, N), f32, dev)
@@ -1759,7 +1769,7 @@ def selective_scan(x: torch.Tensor, dt: torch.Tensor, b: torch.Tensor, c: torch.
             raise ValueError("state: it does not start on a 16-byte boundary")
     nd, npf, cu, pos, read, write = _step_place(md, T, state is not None, write_slots, dev)
     px, pdt, pb, pc = x.data_ptr(), dt.data_ptr(), b.data_ptr(), c.data_ptr()
-    pz, dt32, es, gn = None if z is None else z.data_ptr(), dt.dtype is f32, dtype.itemsize, groups * N
+    pz, dt32, es, gn = 0 if z is None else z.data_ptr(), dt.dtype is f32, dtype.itemsize, groups * N
     if out is None:
         out = torch.empty((T, cols), dtype=dtype, device=x.device)
         po, ldo = out.data_ptr(), cols
@@ -1767,11 +1777,12 @@ def selective_scan(x: torch.Tensor, dt: torch.Tensor, b: torch.Tensor, c: torch.
         po, ldo = _target(out, T, cols, dtype, dev,
                           (("x", px, ldx, cols, es), ("dt", pdt, lddt, rates, 4 if dt32 else es),
                            ("b", pb, ldb, gn, es), ("c", pc, ldc, gn, es), ("z", pz, ldz, cols, es)))
-    wide = (px | pb | pc | po | (pz or 0)) % 16 == 0 and (T == 1 or (ldx | ldb | ldc | ldz | ldo) * es % 16 == 0)
-    _call_on(dev, "b200_selective_scan", px, ldx, pdt, lddt, dt32, pb, ldb, pc, ldc, pz, ldz,
-             a_log.data_ptr(), channels, None if d is None else d.data_ptr(),
-             None if dt_bias is None else dt_bias.data_ptr(), softplus, lo, hi, ps, slots, pos, read, write, cu, po, ldo,
-             T, heads, width, N, groups, nd, npf, wide, DTYPE_CODE[dtype])
+    wide = (px | pb | pc | po | pz) % 16 == 0 and (T == 1 or (ldx | ldb | ldc | ldz | ldo) * es % 16 == 0)
+    _call_on(dev, "b200_selective_scan",
+             _SCAN_CALL.pack(px, pdt, pb, pc, pz, po, a_log.data_ptr(), 0 if d is None else d.data_ptr(),
+                             0 if dt_bias is None else dt_bias.data_ptr(), ps, pos, read, write, cu, ldx, lddt, ldb, ldc,
+                             ldz, ldo, lo, hi, dt32, channels, softplus, slots, T, heads, width, N, groups, nd, npf, wide,
+                             DTYPE_CODE[dtype]))
     return out
 
 
@@ -1801,17 +1812,18 @@ def group_norm_gate(x: torch.Tensor, z: Optional[torch.Tensor], weight: torch.Te
     _whole("weight", weight, (Ch,), torch.float32, dev)
     if bias is not None:
         _whole("bias", bias, (Ch,), torch.float32, dev)
-    px, pz, pw, es = x.data_ptr(), None if z is None else z.data_ptr(), weight.data_ptr(), dtype.itemsize
-    pb = None if bias is None else bias.data_ptr()
+    px, pz, pw, es = x.data_ptr(), 0 if z is None else z.data_ptr(), weight.data_ptr(), dtype.itemsize
+    pb = 0 if bias is None else bias.data_ptr()
     if out is None:
         out = torch.empty((T, Ch), dtype=dtype, device=x.device)
         po, ldo = out.data_ptr(), Ch
     else:
         po, ldo = _target(out, T, Ch, dtype, dev, (("x", px, ldx, Ch, es), ("z", pz, ldz, Ch, es)), same_is_fine=True)
-    wide = Ch // groups * es % 16 == 0 and (px | (pz or 0) | pw | (pb or 0) | po) % 16 == 0 and \
+    wide = Ch // groups * es % 16 == 0 and (px | pz | pw | pb | po) % 16 == 0 and \
         (T == 1 or (ldx | ldz | ldo) * es % 16 == 0)
-    _call_on(dev, "b200_group_norm_gate", px, ldx, pz, ldz, pw, pb, po, ldo, eps, T, Ch, groups, GATE_ACT[act], center,
-             gate_after, wide, DTYPE_CODE[dtype])
+    _call_on(dev, "b200_group_norm_gate",
+             _NORM_CALL.pack(px, pz, po, pw, pb, ldx, ldz, ldo, eps, T, Ch, groups, GATE_ACT[act], center, gate_after,
+                             wide, DTYPE_CODE[dtype]))
     return out
 
 
