@@ -537,7 +537,7 @@ __global__ void __launch_bounds__(128) selective_step_kernel(const ScanArgs a) {
 // done per element is half of the instructions, and the chain along the tokens leaves the scheduler idle.)
 // The sum over the lanes of a column is the helpers': up to four lanes leave a part of it each; where there are
 // more, pairs of lanes trade the parts of two tokens first, so that each ends up with those of its own token.  With
-// few numbers per lane, decays and inputs of the next four tokens are made while the chain of these runs.
+// few numbers per lane, decays and inputs of eight tokens are made before their chain is walked.
 template <int LPC>
 constexpr int kCore = LPC >= 8 ? 256 : 128;
 constexpr int kHelp = 128;
@@ -613,9 +613,18 @@ __global__ void __launch_bounds__(kCore<LPC> + kHelp) selective_scan_kernel(cons
     const bool one_head = !CH && a.width % 8 == 0;           // eight columns share a step size
     const T* bsrc = static_cast<const T*>(a.b) + g * a.N;
     const T* csrc = static_cast<const T*>(a.c) + g * a.N;
+    uint32_t head_dt[2] = {0u, 0u};                          // rates per head: raw step sizes of two tiles under way
     auto bring = [&](int tile) {
       if (tile < tiles) {
         const int t0 = po.first + tile * TOK, n = po.end - t0;
+        if (one_head && vt < n && vn > 0) {
+          const long long k = static_cast<long long>(t0 + vt) * a.lddt + (c0 + vc) / a.width;
+          uint32_t v;
+          if (a.dt_f32 || sizeof(T) == 4) v = static_cast<const uint32_t*>(a.dt)[k];
+          else v = static_cast<const unsigned short*>(a.dt)[k];
+          if (tile & 1) head_dt[1] = v;
+          else head_dt[0] = v;
+        }
         if (me < Tile::kVecs) {
           const int here = vt < n ? vn : 0;
           const long long t = t0 + (here > 0 ? vt : 0);
@@ -687,7 +696,17 @@ __global__ void __launch_bounds__(kCore<LPC> + kHelp) selective_scan_kernel(cons
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
             if (i < here && (i == 0 || !one_head)) {
-              step = step_size<T>(a, t0 + vt, (c0 + vc + i) / a.width);
+              if (one_head) {
+                const uint32_t v = tile & 1 ? head_dt[1] : head_dt[0];
+                float z = __uint_as_float(v);
+                if (sizeof(T) == 2 && !a.dt_f32) {
+                  const unsigned short u = static_cast<unsigned short>(v);
+                  z = to_f32<T>(*reinterpret_cast<const T*>(&u));
+                }
+                step = step_from<T>(a, z, bias[0].x);
+              } else {
+                step = step_size<T>(a, t0 + vt, (c0 + vc + i) / a.width);
+              }
               e = expf(step * hrate[i]);
             }
             (i & 1 ? dt[i / 2].y : dt[i / 2].x) = step;
@@ -879,12 +898,11 @@ __global__ void __launch_bounds__(kCore<LPC> + kHelp) selective_scan_kernel(cons
     };
     if constexpr (NPL <= 4) {
       Ahead even, odd;
-      make(0, even);
 #pragma unroll 1
       for (int i = 0; i < TOK; i += 8) {
+        make(i, even);
         make(i + 4, odd);
         walk(i, even);
-        make(i + 8 < TOK ? i + 8 : 0, even);                 // (behind the last one: not used)
         walk(i + 4, odd);
       }
     } else {
