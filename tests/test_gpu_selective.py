@@ -313,3 +313,137 @@ def test_bits_repeat():
             kept = state.clone()
             runs.append((K.selective_scan(**dev, groups=1, md=md, state=kept), kept))
         assert all(torch.equal(u, v) for r in runs[1:] for u, v in zip(runs[0], r))
+
+
+# -- the far ends of what the launchers allow ---------------------------------------------
+def _far_rows(rows, cols, seed=0):
+    """Rows a megabyte and more apart: the last ones lie behind 2^31 elements."""
+    pitch = 1 << 20
+    wide = torch.empty(rows, pitch, dtype=BF16, device="cuda")
+    view = wide[:, pitch - cols - 8:pitch - 8]
+    view.copy_(torch.randn(rows, cols, generator=torch.Generator().manual_seed(seed)).to(BF16))
+    return view
+
+
+def test_offsets_behind_32_bits():
+    from vllm_gcu_b200.ops import cuda as K
+    R, C = 2100, 72
+    md = S.step(3, [1500, R - 1503], [5, 0, 9, 0, 3])
+    x = _far_rows(R, C)
+    out = _far_rows(R, C, 1)
+    g = torch.Generator().manual_seed(2)
+    w, bias, ring = torch.randn(4, C, generator=g), torch.randn(C, generator=g), torch.randn(5, 3, C, generator=g).to(BF16)
+    K.causal_conv(x, w.cuda(), bias.cuda(), md.to("cuda"), ring.cuda(), out=out)
+    near = K.causal_conv(x.contiguous(), w.cuda(), bias.cuda(), md.to("cuda"), ring.cuda())
+    assert torch.equal(out, near)
+    norm = K.group_norm_gate(x, x, torch.ones(C, device="cuda"), 3, 1e-5, out)
+    assert torch.equal(norm, K.group_norm_gate(x.contiguous(), x.contiguous(), torch.ones(C, device="cuda"), 3, 1e-5))
+    for form, H, P, N in (("heads", 1, 64, 64), ("heads", 2, 32, 8), ("channels", 64, 1, 16)):
+        k = S.scan_case(form, H, P, N, 1, md, BF16)
+        dev = _views(k)
+        state = dev.pop("state")
+        far = dict(dev, **{n: _far_rows(R, v.shape[1]) for n, v in dev.items() if n in ("x", "b", "c", "dt")})
+        for n in ("x", "b", "c", "dt"):
+            far[n].copy_(dev[n])
+        s1, s2 = state.clone(), state.clone()
+        a = K.selective_scan(**far, groups=1, md=md.to("cuda"), state=s1, out=_far_rows(R, H * P))
+        b = K.selective_scan(**dev, groups=1, md=md.to("cuda"), state=s2)
+        del far
+        # (the far rows may go by other kernels than those that 16-byte boundaries allow)
+        assert (a.float() - b.float()).norm() < 2.0 ** -8 * b.float().norm()
+        assert (s1 - s2).norm() < 2e-6 * s2.norm()
+
+
+@pytest.mark.parametrize("taps", [2, 4, 8])
+def test_far_positions(taps):
+    """A ring goes by positions of 64 bits."""
+    from vllm_gcu_b200.ops import cuda as K
+    md = S.step(2, [9, 3], [2 ** 33 + 5, 2 ** 31 - 1, 2 ** 40 + 1, 2 ** 31 + 6])
+    x, w, bias, ring = S.conv_case(24, taps, md, BF16)
+    want, mag, new = S.conv(x, w, bias, md, ring)
+    kept = ring.cuda()
+    got = K.causal_conv(x.cuda(), w.cuda(), bias.cuda(), md.to("cuda"), kept)
+    S.near(got, want, BF16, 2.0 ** -24 * (taps + 44) * (mag + 1))
+    assert torch.equal(kept.cpu(), new)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("form,H,P,N", [("heads", 2, 64, 64), ("channels", 40, 1, 16)])
+def test_growing_states(form, H, P, N, dtype):
+    """Step sizes below 0, where the limits allow them: states that grow."""
+    from vllm_gcu_b200.ops import cuda as K
+    md = S.step(2, [30, 150], [3, 0, 4, 0])
+    k = S.scan_case(form, H, P, N, 1, md, dtype)
+    k["a_log"] = torch.full_like(k["a_log"], -1.0)
+    more = dict(softplus=False, dt_limits=(-0.02, 0.1))
+    state, dev = k["state"], _views(k)
+    want, mag, new, smag = S.scan(**{n: v for n, v in k.items() if n not in ("row", "state")}, groups=1, md=md, state=state,
+                                  **more)
+    kept = dev.pop("state")
+    got = K.selective_scan(**dev, groups=1, md=md.to("cuda"), state=kept, **more)
+    S.near(got, want, dtype, _rounding(md, N, mag, dtype))
+    S.near(kept, new, F32, S.scan_rounding(md, N, smag))
+
+
+@pytest.mark.parametrize("decodes,lens", [(6, ()), (0, (20, 3)), (2, (9,))])
+@pytest.mark.parametrize("form,H,P,N", [("heads", 2, 64, 128), ("heads", 4, 16, 12), ("channels", 64, 1, 16), ("channels", 20, 1, 7)])
+def test_weights_off_16_byte_boundaries(form, H, P, N, decodes, lens):
+    """Rates, skips and biases that are parts of larger tensors, and rows that start anywhere."""
+    from vllm_gcu_b200.ops import cuda as K
+    md = S.step(decodes, lens)
+    k = S.scan_case(form, H, P, N, 1, md, BF16)
+    state = k["state"]
+    want, mag, new, smag = S.scan(**{n: v for n, v in k.items() if n not in ("row", "state")}, groups=1, md=md, state=state)
+
+    def off(t):                                      # one element behind a boundary
+        buf = torch.empty(t.numel() + 1, dtype=t.dtype, device="cuda")
+        buf[1:].copy_(t.flatten())
+        return buf[1:].view(t.shape)
+
+    dev = {n: off(v) for n, v in k.items() if n in ("a_log", "d", "dt_bias")}
+    for n in ("x", "b", "c", "dt", "z"):
+        buf = torch.zeros(md.tokens, k[n].shape[1] + 5, dtype=BF16, device="cuda")
+        buf[:, 3:-2] = k[n].cuda()
+        dev[n] = buf[:, 3:-2]
+    kept = state.cuda()
+    got = K.selective_scan(**dev, groups=1, md=md.to("cuda"), state=kept)
+    S.near(got, want, BF16, _rounding(md, N, mag, BF16))
+    S.near(kept, new, F32, S.scan_rounding(md, N, smag))
+    with pytest.raises(ValueError, match="16-byte boundary"):
+        K.selective_scan(**dev, groups=1, md=md.to("cuda"), state=off(state))
+
+
+@pytest.mark.parametrize("form,H,P,N", [("heads", 2, 64, 128), ("heads", 2, 8, 8), ("channels", 32, 1, 16)])
+def test_not_a_number_stays_one(form, H, P, N):
+    """A step size that is no number leaves a state and results that are none, from its token on."""
+    from vllm_gcu_b200.ops import cuda as K
+    md = S.step(2, [140, 12], [4, 4, 4, 0])
+    k = S.scan_case(form, H, P, N, 1, md, BF16)
+    k["dt"][1], k["dt"][2 + 70] = math.nan, math.nan
+    dev = _views(k)
+    state = dev.pop("state")
+    got = K.selective_scan(**dev, groups=1, md=md.to("cuda"), state=state).float()
+    bad = torch.zeros(md.tokens, dtype=torch.bool)
+    bad[1], bad[72:142] = True, True
+    assert torch.isnan(got[bad.cuda()]).all() and not torch.isnan(got[~bad.cuda()]).any()
+    nan = torch.isnan(state).flatten(1)
+    for r, want in enumerate((False, True, True, False)):
+        at = int(md.state_slots[r])
+        assert bool(nan[at].all()) == want and bool(nan[at].any()) == want
+
+
+def test_calls_on_another_stream_than_the_tensors():
+    """Tensors made on one stream, used on another behind an event, given back to the allocator at once."""
+    from vllm_gcu_b200.ops import cuda as K
+    md = S.step(2, [150], [3, 4, 5]).to("cuda")
+    dev = _views(S.scan_case("heads", 2, 64, 128, 1, md.to("cpu"), BF16))
+    state = dev.pop("state")
+    want_state, side = state.clone(), torch.cuda.Stream()
+    want = K.selective_scan(**dev, groups=1, md=md, state=want_state)
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = K.selective_scan(**dev, groups=1, md=md, state=state)
+        norm = K.group_norm_gate(got, None, torch.ones(128, device="cuda"), 2, 1e-5)
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(got, want) and torch.equal(state, want_state)
+    assert torch.equal(norm, K.group_norm_gate(want, None, torch.ones(128, device="cuda"), 2, 1e-5))

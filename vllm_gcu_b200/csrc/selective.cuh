@@ -1,4 +1,5 @@
-// What the kernels of the selective scan share (selective.cu, selective_heads.cu).
+// What the kernels of the selective scan share (selective.cu,
+// selective_step.cu, selective_heads.cu) and the causal convolution (causal_conv.cu).
 #pragma once
 
 #include "common.cuh"
@@ -55,7 +56,7 @@ struct Portion {
 };
 __device__ __forceinline__ Portion portion_of(int r, int nd, const int* cu_q, int T) {
   if (r < nd) return {r, r + 1};
-  return {nd + cu_q[r - nd], min(nd + cu_q[r - nd + 1], T)};
+  return {nd + max(cu_q[r - nd], 0), min(nd + cu_q[r - nd + 1], T)};
 }
 
 struct ScanArgs {
@@ -93,6 +94,26 @@ __device__ __forceinline__ float step_size(const ScanArgs& a, long long row, int
   return step_from<T>(a, z, a.dt_bias != nullptr ? a.dt_bias[i] : 0.0f);
 }
 
+// V neighbouring elements, in one access where V is 4
+template <typename T, int V>
+struct Raw {
+  T e[V];
+};
+template <>
+struct __align__(8) Raw<__nv_bfloat16, 4> {
+  __nv_bfloat16 e[4];
+};
+template <>
+struct __align__(8) Raw<__half, 4> {
+  __half e[4];
+};
+template <>
+struct __align__(16) Raw<float, 4> {
+  float e[4];
+};
+
+// One token per request (selective_step.cu).  dtype: 0 bf16, 1 fp16, 2 fp32.
+int launch_single_tokens(const ScanArgs& a, bool per_channel, int dtype, cudaStream_t s);
 // Portions of prompts by products of tiles (selective_heads.cu): rates per head, bf16 rows on 16-byte boundaries.
 bool heads_by_tiles(const ScanArgs& a);
 int launch_heads_by_tiles(const ScanArgs& a, cudaStream_t s);

@@ -1,0 +1,399 @@
+// Selective scan of single tokens (sm_100a), one per request: see selective.cu for the formulas and the state's layout.
+#include "selective.cuh"
+
+namespace b200 {
+namespace selective {
+
+// Sums of ROWS values over LPR neighbouring lanes, lane by lane fewer rows: while there are rows to part, two halves of
+// the lanes take a half of the rows each.  Leaves kLeft sums per lane, of rows from `first` on.
+template <int ROWS, int LPR>
+struct RowSums {
+  static constexpr int kParted = ROWS < LPR ? ROWS : LPR, kLeft = ROWS / kParted;
+  float v[kLeft];
+  int first;
+  __device__ __forceinline__ RowSums(float (&s)[ROWS], int l) {
+    first = 0;
+#pragma unroll
+    for (int half = ROWS / 2, o = LPR / 2; half >= kLeft && o > 0; half >>= 1, o >>= 1) {
+      const bool up = l & o;
+      if (up) first += half;
+#pragma unroll
+      for (int i = 0; i < half; ++i) {
+        const float mine = up ? s[i + half] : s[i], theirs = up ? s[i] : s[i + half];
+        s[i] = mine + __shfl_xor_sync(0xffffffffu, theirs, o);
+      }
+    }
+#pragma unroll
+    for (int o = LPR / kParted / 2; o > 0; o >>= 1)
+#pragma unroll
+      for (int i = 0; i < kLeft; ++i) s[i] += __shfl_xor_sync(0xffffffffu, s[i], o);
+#pragma unroll
+    for (int i = 0; i < kLeft; ++i) v[i] = s[i];
+  }
+  __device__ __forceinline__ static bool keeps(int l) { return l % (LPR / kParted) == 0; }
+};
+
+// Four neighbours of a row of B or C.
+template <typename T, bool WIDE>
+__device__ __forceinline__ float4 load_four(const T* p, bool in) {
+  Raw<T, 4> v;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v.e[i] = from_f32<T>(0.0f);
+  if (in) {
+    if (WIDE) {
+      v = *reinterpret_cast<const Raw<T, 4>*>(p);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v.e[i] = p[i];
+    }
+  }
+  return make_float4(to_f32<T>(v.e[0]), to_f32<T>(v.e[1]), to_f32<T>(v.e[2]), to_f32<T>(v.e[3]));
+}
+// a state's four numbers after a token, and their part of the read-out
+__device__ __forceinline__ float update(float4& h, float2 e0, float2 e1, float2 dx, const float4& b, const float4& c) {
+  const float2 h0 = __ffma2_rn(e0, make_float2(h.x, h.y), __fmul2_rn(dx, make_float2(b.x, b.y)));
+  const float2 h1 = __ffma2_rn(e1, make_float2(h.z, h.w), __fmul2_rn(dx, make_float2(b.z, b.w)));
+  const float2 s = __ffma2_rn(h1, make_float2(c.z, c.w), __fmul2_rn(h0, make_float2(c.x, c.y)));
+  h = make_float4(h0.x, h0.y, h1.x, h1.y);
+  return s.x + s.y;
+}
+
+// One token per request, rates per head, where a warp's columns belong to one head (width a multiple of their number)
+// and N is one of 4: a row of N numbers is spread over LPR lanes, NC times four each.  The state's bytes bound it: a warp
+// has 4 KB of it under way at once, and what a head's columns share is worked out once per warp (by row, 70 per cent of the
+// issue slots went into that: 96 requests of 80 heads of 64 x 128 in 113 us, 4.4 TB/s).
+template <typename T, int LPR, int NC, bool WIDE>
+__global__ void __launch_bounds__(128) heads_step_kernel(const ScanArgs a) {
+  constexpr int kRows = NC > 1 ? 4 : 8, kGroups = 32 / LPR, kWarpCols = kRows * kGroups;
+  grid_release_small();
+  grid_wait();
+  const int r = blockIdx.y, lane = threadIdx.x & 31, l = lane & (LPR - 1), grp = lane / LPR;
+  const int cols = a.heads * a.width;
+  const int c0 = (blockIdx.x * 4 + (threadIdx.x >> 5)) * kWarpCols;
+  if (c0 >= cols) return;
+  const int slot = a.state != nullptr ? a.slots[r] : 0;
+  const int ws = a.state != nullptr ? a.wslots[r] : -1;
+  const bool old = a.state != nullptr && a.positions[r] != 0;
+  T* out = static_cast<T*>(a.out) + r * a.ldo + c0;
+  if (a.state != nullptr && (slot < 0 || slot >= a.num_slots)) {
+    for (int i = lane; i < kWarpCols; i += 32) out[i] = from_f32<T>(0.0f);
+    return;
+  }
+  const long long pitch = static_cast<long long>(cols) * a.N;
+  const long long at = static_cast<long long>(c0 + grp) * a.N + l * 4;
+  float4 h[kRows][NC];
+#pragma unroll
+  for (int i = 0; i < kRows; ++i)
+#pragma unroll
+    for (int k = 0; k < NC; ++k) {
+      h[i][k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      if (old && (l + LPR * k) * 4 < a.N)
+        h[i][k] = *reinterpret_cast<const float4*>(a.state + slot * pitch + at + i * kGroups * a.N + LPR * k * 4);
+    }
+  const int hd = c0 / a.width, g = hd / (a.heads / a.groups);
+  // x of the warp's columns: column j in lane j % 32
+  float x[kWarpCols / 32 + 1];
+#pragma unroll
+  for (int j = 0; j <= (kWarpCols - 1) / 32; ++j)
+    x[j] = j * 32 + lane < kWarpCols ? to_f32<T>(static_cast<const T*>(a.x)[r * a.ldx + c0 + j * 32 + lane]) : 0.0f;
+  float4 b[NC], c[NC];
+#pragma unroll
+  for (int k = 0; k < NC; ++k) {
+    const int n = (l + LPR * k) * 4;
+    b[k] = load_four<T, WIDE>(static_cast<const T*>(a.b) + r * a.ldb + g * a.N + n, n < a.N);
+    c[k] = load_four<T, WIDE>(static_cast<const T*>(a.c) + r * a.ldc + g * a.N + n, n < a.N);
+  }
+  const float dt = step_size<T>(a, r, hd);
+  const float decay = expf(-dt * expf(a.a_log[hd]));
+  float s[kRows];
+#pragma unroll
+  for (int i = 0; i < kRows; ++i) {
+    const float dx = dt * __shfl_sync(0xffffffffu, x[i * kGroups / 32], (i * kGroups + grp) & 31);
+    s[i] = 0.0f;
+#pragma unroll
+    for (int k = 0; k < NC; ++k)
+      s[i] += update(h[i][k], make_float2(decay, decay), make_float2(decay, decay), make_float2(dx, dx), b[k], c[k]);
+  }
+  if (ws >= 0 && ws < a.num_slots) {
+#pragma unroll
+    for (int i = 0; i < kRows; ++i)
+#pragma unroll
+      for (int k = 0; k < NC; ++k)
+        if ((l + LPR * k) * 4 < a.N)
+          *reinterpret_cast<float4*>(a.state + ws * pitch + at + i * kGroups * a.N + LPR * k * 4) = h[i][k];
+  }
+  const RowSums<kRows, LPR> sums(s, l);
+  const float skip = a.d != nullptr ? a.d[hd] : 0.0f;
+#pragma unroll
+  for (int i = 0; i < sums.kLeft; ++i) {
+    const int j = (sums.first + i) * kGroups + grp;      // column of the warp
+    float xv = 0.0f;
+#pragma unroll
+    for (int m = 0; m <= (kWarpCols - 1) / 32; ++m) {
+      const float v = __shfl_sync(0xffffffffu, x[m], j & 31);
+      if (j / 32 == m) xv = v;
+    }
+    float y = fmaf(skip, xv, sums.v[i]);
+    if (a.z != nullptr) y *= silu<T>(to_f32<T>(static_cast<const T*>(a.z)[r * a.ldz + c0 + j]));
+    if (sums.keeps(l)) out[j] = from_f32<T>(y);
+  }
+}
+
+// One token per request, rates per channel, N a multiple of 4 up to 128: a warp holds 32 / LPR columns of RQ requests, so
+// that rates and skips are fetched and worked out once for them.
+template <typename T, int LPR, int RQ, bool WIDE>
+__global__ void __launch_bounds__(128) channels_step_kernel(const ScanArgs a) {
+  constexpr int kGroups = 32 / LPR;
+  grid_release_small();
+  grid_wait();
+  const int lane = threadIdx.x & 31, l = lane & (LPR - 1), grp = lane / LPR;
+  const int cols = a.heads * a.width;
+  const int c0 = (blockIdx.x * 4 + (threadIdx.x >> 5)) * kGroups;
+  if (c0 >= cols) return;
+  const bool in = c0 + grp < cols && l * 4 < a.N, mine = c0 + grp < cols;
+  const int col = min(c0 + grp, cols - 1), n = l * 4;
+  const int g = col / (cols / a.groups);
+  const int r0 = blockIdx.y * RQ;
+  const long long pitch = static_cast<long long>(cols) * a.N, at = static_cast<long long>(col) * a.N + n;
+  float4 h[RQ], b[RQ], c[RQ];
+  float x[RQ], dt[RQ], z[RQ];
+  int ws[RQ];
+  bool padding[RQ];
+#pragma unroll
+  for (int i = 0; i < RQ; ++i) {
+    const int r = min(r0 + i, a.nd - 1);
+    const int slot = a.state != nullptr ? a.slots[r] : 0;
+    ws[i] = a.state != nullptr && r0 + i < a.nd ? a.wslots[r] : -1;
+    padding[i] = a.state != nullptr && (slot < 0 || slot >= a.num_slots);
+    if (padding[i]) ws[i] = -1;
+    h[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    if (a.state != nullptr && !padding[i] && in && a.positions[r] != 0)
+      h[i] = *reinterpret_cast<const float4*>(a.state + slot * pitch + at);
+  }
+#pragma unroll
+  for (int i = 0; i < RQ; ++i) {
+    const int r = min(r0 + i, a.nd - 1);
+    x[i] = to_f32<T>(static_cast<const T*>(a.x)[r * a.ldx + col]);
+    dt[i] = a.dt_f32 ? static_cast<const float*>(a.dt)[r * a.lddt + col]
+                     : to_f32<T>(static_cast<const T*>(a.dt)[r * a.lddt + col]);
+    z[i] = a.z != nullptr ? to_f32<T>(static_cast<const T*>(a.z)[r * a.ldz + col]) : 0.0f;
+    b[i] = load_four<T, WIDE>(static_cast<const T*>(a.b) + r * a.ldb + g * a.N + n, in);
+    c[i] = load_four<T, WIDE>(static_cast<const T*>(a.c) + r * a.ldc + g * a.N + n, in);
+  }
+  float4 rate = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  if (in) rate = *reinterpret_cast<const float4*>(a.a_log + at);
+  rate = make_float4(-expf(rate.x) * kLog2e, -expf(rate.y) * kLog2e, -expf(rate.z) * kLog2e, -expf(rate.w) * kLog2e);
+  const float bias = a.dt_bias != nullptr ? a.dt_bias[col] : 0.0f, skip = a.d != nullptr ? a.d[col] : 0.0f;
+  float s[RQ];
+#pragma unroll
+  for (int i = 0; i < RQ; ++i) {
+    const float step = step_from<T>(a, dt[i], bias), dx = step * x[i];
+    const float2 p0 = __fmul2_rn(make_float2(step, step), make_float2(rate.x, rate.y));
+    const float2 p1 = __fmul2_rn(make_float2(step, step), make_float2(rate.z, rate.w));
+    const float2 e0 = make_float2(exp2_fast(p0.x), exp2_fast(p0.y)), e1 = make_float2(exp2_fast(p1.x), exp2_fast(p1.y));
+    s[i] = update(h[i], e0, e1, make_float2(dx, dx), b[i], c[i]);
+    s[i] = in ? s[i] : 0.0f;
+    if (in && ws[i] >= 0 && ws[i] < a.num_slots) *reinterpret_cast<float4*>(a.state + ws[i] * pitch + at) = h[i];
+  }
+  const RowSums<RQ, LPR> sums(s, l);
+#pragma unroll
+  for (int i = 0; i < sums.kLeft; ++i) {
+    const int k = sums.first + i, r = r0 + k;
+    if (!mine || !sums.keeps(l) || r >= a.nd) continue;
+    float xv = 0.0f, zv = 0.0f;
+    bool none = false;
+#pragma unroll
+    for (int m = 0; m < RQ; ++m)
+      if (m == k) {
+        xv = x[m];
+        zv = z[m];
+        none = padding[m];
+      }
+    float y = fmaf(skip, xv, sums.v[i]);
+    if (a.z != nullptr) y *= silu<T>(zv);
+    static_cast<T*>(a.out)[r * a.ldo + col] = from_f32<T>(none ? 0.0f : y);
+  }
+}
+
+// One token per request, in general.  A row of N numbers of state is spread over LPR lanes, four numbers (one
+// where V is 1) at a time; a warp takes kRows rows per lane group at once, so that their loads are under
+// way together.
+template <typename T, bool CH, int LPR, int NC, int V>
+__global__ void __launch_bounds__(128) selective_step_kernel(const ScanArgs a) {
+  constexpr int kRows = NC > 1 ? 4 : 8, kGroups = 32 / LPR;
+  grid_release_small();
+  grid_wait();
+  const int r = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int l = lane & (LPR - 1), grp = lane / LPR;
+  const int cols = a.heads * a.width;
+  const int c0 = (blockIdx.x * 4 + warp) * kRows * kGroups + grp;    // column of row i: c0 + i * kGroups
+  const int slot = a.state != nullptr ? a.slots[r] : 0;
+  const bool padding = a.state != nullptr && (slot < 0 || slot >= a.num_slots);
+  T* out = static_cast<T*>(a.out) + r * a.ldo;
+  if (padding) {
+#pragma unroll
+    for (int i = 0; i < kRows; ++i)
+      if (l == 0 && c0 + i * kGroups < cols) out[c0 + i * kGroups] = from_f32<T>(0.0f);
+    return;
+  }
+  const bool old = a.state != nullptr && a.positions[r] != 0;
+  const int ws = a.state != nullptr ? a.wslots[r] : -1;
+  const bool keep = ws >= 0 && ws < a.num_slots;
+  const long long pitch = static_cast<long long>(cols) * a.N;
+  float h[kRows][NC][V];
+#pragma unroll
+  for (int i = 0; i < kRows; ++i) {
+    const int col = c0 + i * kGroups;
+#pragma unroll
+    for (int k = 0; k < NC; ++k) {
+      const int n = (l + LPR * k) * V;
+#pragma unroll
+      for (int v = 0; v < V; ++v) h[i][k][v] = 0.0f;
+      if (old && col < cols && n < a.N) {
+        const float* src = a.state + slot * pitch + static_cast<long long>(col) * a.N + n;
+        if constexpr (V == 4) {
+          const float4 q = *reinterpret_cast<const float4*>(src);
+          h[i][k][0] = q.x; h[i][k][1] = q.y; h[i][k][2] = q.z; h[i][k][3] = q.w;
+        } else {
+          h[i][k][0] = *src;
+        }
+      }
+    }
+  }
+  float bb[NC][V], cc[NC][V];
+  int group = -1, head = -1;
+  float dt = 0.0f, decay = 0.0f;
+  float y[kRows];
+#pragma unroll
+  for (int i = 0; i < kRows; ++i) {
+    const int col = min(c0 + i * kGroups, cols - 1);
+    const int hd = col / a.width;
+    const int g = hd / (a.heads / a.groups);
+    if (g != group) {
+      group = g;
+#pragma unroll
+      for (int k = 0; k < NC; ++k)
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+          const int n = (l + LPR * k) * V + v;
+          const bool in = n < a.N;
+          bb[k][v] = in ? to_f32<T>(static_cast<const T*>(a.b)[r * a.ldb + g * a.N + n]) : 0.0f;
+          cc[k][v] = in ? to_f32<T>(static_cast<const T*>(a.c)[r * a.ldc + g * a.N + n]) : 0.0f;
+        }
+    }
+    if (CH || hd != head) {
+      head = hd;
+      dt = step_size<T>(a, r, CH ? col : hd);
+      if (!CH) decay = expf(-dt * expf(a.a_log[hd]));
+    }
+    const float x = to_f32<T>(static_cast<const T*>(a.x)[r * a.ldx + col]);
+    const float dx = dt * x;
+    float s = 0.0f;
+#pragma unroll
+    for (int k = 0; k < NC; ++k)
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        const int n = (l + LPR * k) * V + v;
+        float e = decay;
+        if (CH) e = n < a.N ? expf(-dt * expf(a.a_log[static_cast<long long>(col) * a.N + n])) : 0.0f;
+        h[i][k][v] = fmaf(e, h[i][k][v], dx * bb[k][v]);
+        s = fmaf(h[i][k][v], cc[k][v], s);
+      }
+#pragma unroll
+    for (int o = 1; o < LPR; o <<= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    if (a.d != nullptr) s = fmaf(a.d[CH ? col : hd], x, s);
+    if (a.z != nullptr) s *= silu<T>(to_f32<T>(static_cast<const T*>(a.z)[r * a.ldz + col]));
+    y[i] = s;
+  }
+#pragma unroll
+  for (int i = 0; i < kRows; ++i) {
+    const int col = c0 + i * kGroups;
+    if (col >= cols) continue;
+    if (l == 0) out[col] = from_f32<T>(y[i]);
+    if (!keep) continue;
+#pragma unroll
+    for (int k = 0; k < NC; ++k) {
+      const int n = (l + LPR * k) * V;
+      if (n >= a.N) continue;
+      float* dst = a.state + ws * pitch + static_cast<long long>(col) * a.N + n;
+      if constexpr (V == 4)
+        *reinterpret_cast<float4*>(dst) = make_float4(h[i][k][0], h[i][k][1], h[i][k][2], h[i][k][3]);
+      else
+        *dst = h[i][k][0];
+    }
+  }
+}
+
+template <typename T, int LPR, int NC>
+int launch_heads_step(const ScanArgs& a, cudaStream_t s) {
+  constexpr int kCtaCols = 4 * (NC > 1 ? 4 : 8) * (32 / LPR);
+  const dim3 grid((a.heads * a.width + kCtaCols - 1) / kCtaCols, a.nd);
+  return a.wide ? launch_overlapped(heads_step_kernel<T, LPR, NC, true>, grid, dim3(128), 0, s, a)
+                : launch_overlapped(heads_step_kernel<T, LPR, NC, false>, grid, dim3(128), 0, s, a);
+}
+template <typename T, int LPR, int RQ>
+int launch_channels_step(const ScanArgs& a, cudaStream_t s) {
+  constexpr int kCtaCols = 4 * (32 / LPR);
+  const dim3 grid((a.heads * a.width + kCtaCols - 1) / kCtaCols, (a.nd + RQ - 1) / RQ);
+  return a.wide ? launch_overlapped(channels_step_kernel<T, LPR, RQ, true>, grid, dim3(128), 0, s, a)
+                : launch_overlapped(channels_step_kernel<T, LPR, RQ, false>, grid, dim3(128), 0, s, a);
+}
+// Requests that share a warp: four where that leaves eight warps to an SM (64 requests of 8192 channels of 16: two and
+// four 24 us, eight, whose registers leave 12 warps an SM, 34).
+template <typename T, int LPR>
+int launch_channels_step(const ScanArgs& a, cudaStream_t s) {
+  const long long warps = (static_cast<long long>(a.heads) * a.width + 32 / LPR - 1) / (32 / LPR);
+  auto enough = [&](int rq) { return warps * ((a.nd + rq - 1) / rq) >= 8ll * sm_count(); };
+  if (enough(4)) return launch_channels_step<T, LPR, 4>(a, s);
+  return launch_channels_step<T, LPR, 1>(a, s);
+}
+
+template <typename T, bool CH>
+int launch_step(const ScanArgs& a, cudaStream_t s) {
+  const int cols = a.heads * a.width;
+  if (a.N % 4 == 0 && reinterpret_cast<uintptr_t>(a.a_log) % (CH ? 16 : 4) == 0) {
+    if constexpr (CH) {
+      if (a.N <= 8) return launch_channels_step<T, 2>(a, s);
+      if (a.N <= 16) return launch_channels_step<T, 4>(a, s);
+      if (a.N <= 32) return launch_channels_step<T, 8>(a, s);
+      if (a.N <= 64) return launch_channels_step<T, 16>(a, s);
+      if (a.N <= 128) return launch_channels_step<T, 32>(a, s);
+    } else {
+      if (a.N > 64 && a.N <= 128 && a.width % 8 == 0) return launch_heads_step<T, 32, 1>(a, s);
+      if (a.N > 128 && a.width % 4 == 0) return launch_heads_step<T, 32, 2>(a, s);
+      if (a.N > 32 && a.N <= 64 && a.width % 16 == 0) return launch_heads_step<T, 16, 1>(a, s);
+      if (a.N > 16 && a.N <= 32 && a.width % 32 == 0) return launch_heads_step<T, 8, 1>(a, s);
+      if (a.N <= 16 && a.width % 64 == 0) return launch_heads_step<T, 4, 1>(a, s);
+    }
+  }
+#define STEP(LPR, NC, V)                                                              \
+  launch_overlapped(selective_step_kernel<T, CH, LPR, NC, V>,                         \
+                    dim3((cols + 4 * (NC > 1 ? 4 : 8) * (32 / LPR) - 1) /             \
+                             (4 * (NC > 1 ? 4 : 8) * (32 / LPR)), a.nd),              \
+                    dim3(128), 0, s, a)
+  if (a.N % 4 == 0) {
+    if constexpr (!CH) {
+      if (a.N <= 16) return STEP(4, 1, 4);
+      if (a.N <= 32) return STEP(8, 1, 4);
+      if (a.N <= 64) return STEP(16, 1, 4);
+      if (a.N <= 128) return STEP(32, 1, 4);
+    }
+    return STEP(32, 2, 4);
+  }
+  if (a.N <= 32) return STEP(32, 1, 1);
+  if (a.N <= 128) return STEP(32, 4, 1);
+  return STEP(32, 8, 1);
+#undef STEP
+}
+
+int launch_single_tokens(const ScanArgs& a, bool per_channel, int dtype, cudaStream_t s) {
+  switch (dtype) {
+    case 0: return per_channel ? launch_step<__nv_bfloat16, true>(a, s) : launch_step<__nv_bfloat16, false>(a, s);
+    case 1: return per_channel ? launch_step<__half, true>(a, s) : launch_step<__half, false>(a, s);
+    case 2: return per_channel ? launch_step<float, true>(a, s) : launch_step<float, false>(a, s);
+  }
+  return -8;
+}
+
+}  // namespace selective
+}  // namespace b200
