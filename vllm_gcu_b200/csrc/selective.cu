@@ -19,18 +19,18 @@ namespace selective {
 
 // Portions of prompts, token after token.  A CTA holds the columns of one request that kCore / LPC lane groups
 // make: a column's numbers of state lie in the registers of LPC lanes, NPL each, and a token costs a number one
-// decay (rates per channel: a power of two, which the special function unit does 16 of per clock and SM: it bounds
-// them), two multiply-adds and a product.  Inputs pass through shared memory kTok tokens at a time.  While the core
-// warps walk tile i, four warps of helpers turn tile i + 1 into step sizes and factors, finish tile i - 1 (skip,
-// gate, store) and copy tile i + 3, each helper the eight neighbouring elements that it copied itself; one
-// barrier per tile.  (Without helpers, all warps doing both in turn, 235 us for 2048 tokens of 8192 channels: what is
-// done per element is half of the instructions, and the chain along the tokens leaves the scheduler idle.)
+// decay (rates per channel: a power of two, of which the special function unit does 16 per clock and SM), two
+// multiply-adds and a product.  Inputs pass through shared memory kTok tokens at a time.  While the core
+// warps walk tile i, four warps copy tile i + 2 and turn tile i + 1 into step sizes and factors, eight neighbouring
+// elements a thread, and four others finish tile i - 1 (skip, gate, store); one barrier per tile.  What is done per element
+// is half of the instructions and the chain along the tokens leaves the scheduler idle: 2048 tokens of 8192 channels
+// took 235 us with all warps doing both in turn and 145 with four warps for the elements.
 // The sum over the lanes of a column is the helpers': up to four lanes leave a part of it each; where there are
 // more, pairs of lanes trade the parts of two tokens first, so that each ends up with those of its own token.  With
 // few numbers per lane, decays and inputs of eight tokens are made before their chain is walked.
 template <int LPC>
 constexpr int kCore = LPC >= 8 ? 256 : 128;
-constexpr int kHelp = 128;
+constexpr int kHelp = 128;                       // threads that bring elements, and threads that finish them
 template <int LPC, int NPL>
 constexpr int kTok = LPC == 2 || LPC * NPL >= 128 ? 16 : 32;
 
@@ -56,7 +56,7 @@ __device__ __forceinline__ void copy_eight(Eight<T>* to, const T* from, int n) {
 template <typename T, bool CH, int LPC, int NPL>
 struct ScanTile {
   static constexpr int kTokens = kTok<LPC, NPL>, kCols = kCore<LPC> / LPC, kVecs = kTokens * kCols / 8;
-  // as they are in memory, by the helper that copied them: rows for four tiles, the rest for two
+  // as they are in memory: rows for four tiles, the rest for two
   Eight<T> x[4][kVecs], z[4][kVecs], bc_raw[2][2 * kTokens * LPC * NPL / 8];
   Eight<float> dt[2][CH ? kVecs : 1];                        // (rows of 16 bits: the first half)
   // by tile parity
@@ -70,7 +70,7 @@ struct ScanTile {
 };
 
 template <typename T, bool CH, int LPC, int NPL, bool WIDE>
-__global__ void __launch_bounds__(kCore<LPC> + kHelp) selective_scan_kernel(const ScanArgs a) {
+__global__ void __launch_bounds__(kCore<LPC> + 2 * kHelp) selective_scan_kernel(const ScanArgs a) {
   using Tile = ScanTile<T, CH, LPC, NPL>;
   constexpr int NP = LPC * NPL, kCols = Tile::kCols, TOK = Tile::kTokens;
   constexpr int kHalf = NPL / 2;
@@ -96,7 +96,8 @@ __global__ void __launch_bounds__(kCore<LPC> + kHelp) selective_scan_kernel(cons
 
   if (threadIdx.x >= kCore<LPC>) {
     // ---------------- helpers ----------------
-    const int me = threadIdx.x - kCore<LPC>;
+    const bool front = threadIdx.x < kCore<LPC> + kHelp;     // copies and factors; else: finishes
+    const int me = (threadIdx.x - kCore<LPC>) % kHelp;
     // eight elements of a tile: token vt, columns vc and on; what belongs to a column stays
     const int vt = me / (kCols / 8), vc = me % (kCols / 8) * 8;
     const int vn = me < Tile::kVecs ? max(0, min(8, cols - vc)) : 0;
@@ -136,8 +137,7 @@ __global__ void __launch_bounds__(kCore<LPC> + kHelp) selective_scan_kernel(cons
       }
       asm volatile("cp.async.commit_group;" ::: "memory");
     };
-    bring(0);
-    bring(1);
+    if (front) bring(0);
     float2 bias[4], skip[4];
     float hrate[8];
 #pragma unroll
@@ -265,18 +265,23 @@ __global__ void __launch_bounds__(kCore<LPC> + kHelp) selective_scan_kernel(cons
           if (i < here) to[i] = y.e[i];
       }
     };
-    asm volatile("cp.async.wait_group 1;" ::: "memory");
-    convert(0);
-    bring(2);
+    if (front) {
+      bring(1);
+      asm volatile("cp.async.wait_group 1;" ::: "memory");
+      convert(0);
+    }
     __syncthreads();
     for (int i = 0; i < tiles; ++i) {
-      asm volatile("cp.async.wait_group 1;" ::: "memory");
-      if (i + 1 < tiles) convert(i + 1);
-      if (i > 0) finish(i - 1);
-      bring(i + 3);
+      if (front) {
+        bring(i + 2);
+        asm volatile("cp.async.wait_group 1;" ::: "memory");
+        if (i + 1 < tiles) convert(i + 1);
+      } else if (i > 0) {
+        finish(i - 1);
+      }
       __syncthreads();
     }
-    finish(tiles - 1);
+    if (!front) finish(tiles - 1);
     return;
   }
 
@@ -426,7 +431,7 @@ int launch_scan(const ScanArgs& a, cudaStream_t s) {
     if (rc != 0) return rc;
   }
   const int per = a.heads / a.groups * a.width;
-  return launch_overlapped(kernel, dim3(a.np, a.groups, (per + kCols - 1) / kCols), dim3(kCore<LPC> + kHelp), kSmem,
+  return launch_overlapped(kernel, dim3(a.np, a.groups, (per + kCols - 1) / kCols), dim3(kCore<LPC> + 2 * kHelp), kSmem,
                            s, a);
 }
 template <typename T, bool CH, bool WIDE>
