@@ -25,14 +25,17 @@ namespace selective {
 // elements a thread, and four others finish tile i - 1 (skip, gate, store); one barrier per tile.  What is done per element
 // is half of the instructions and the chain along the tokens leaves the scheduler idle: 2048 tokens of 8192 channels
 // took 235 us with all warps doing both in turn and 145 with four warps for the elements.
-// The sum over the lanes of a column is the helpers': up to four lanes leave a part of it each; where there are
+// The sum over the lanes of a column is the helpers': four lanes leave a part of it each; where there are
 // more, pairs of lanes trade the parts of two tokens first, so that each ends up with those of its own token.  With
 // few numbers per lane, decays and inputs of eight tokens are made before their chain is walked.
+// Shared memory's bandwidth bounds rates per channel: 11 turns of 128 bytes a warp and token, about 100 of 120 cycles a token
+// on the SMs that hold two CTAs (two columns per lane group, whose B and C would be read once, leave one core warp a
+// scheduler and are no faster: 143 us, so 132).
 template <int LPC>
 constexpr int kCore = LPC >= 8 ? 256 : 128;
 constexpr int kHelp = 128;                       // threads that bring elements, and threads that finish them
 template <int LPC, int NPL>
-constexpr int kTok = LPC == 2 || LPC * NPL >= 128 ? 16 : 32;
+constexpr int kTok = LPC * NPL >= 128 ? 16 : 32;
 
 template <typename T>
 struct __align__(16) Eight {
@@ -61,8 +64,11 @@ struct ScanTile {
   Eight<float> dt[2][CH ? kVecs : 1];                        // (rows of 16 bits: the first half)
   // by tile parity
   float bc[2][2][kTokens][LPC * NPL];                        // B, C
-  float2 d[2][kTokens][kCols];                               // step size (rates per head: decay), step size times x
-  static constexpr int kParts = LPC < 4 ? LPC : 4;
+  // Step size (rates per head: decay) and step size times x, two columns in a place: column c of token t lies in
+  // place c / 2 ^ pair_key, so that helpers, who write four places in a row each, start in different banks.
+  float4 d[2][kTokens][kCols / 2];
+  static __device__ __forceinline__ int pair_key(int t, int c) { return (t * (kCols / 8) + c / 8) >> 1 & 3; }
+  static constexpr int kParts = 4;
   // Parts of C . h.  A helper reads the parts of eight columns in a row, 128 bytes, and its neighbours those of the next
   // ones: column c of token t lies in place c ^ key, so that they start in different banks.
   float y[2][kTokens][kCols][kParts];
@@ -203,7 +209,7 @@ __global__ void __launch_bounds__(kCore<LPC> + 2 * kHelp) selective_scan_kernel(
             (i & 1 ? decay[i / 2].y : decay[i / 2].x) = e;
           }
         }
-        float2* to = &sm.d[tile & 1][vt][vc];
+        float4* to = &sm.d[tile & 1][vt][vc / 2];
         float2 dx[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i)
@@ -219,7 +225,7 @@ __global__ void __launch_bounds__(kCore<LPC> + 2 * kHelp) selective_scan_kernel(
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-          *reinterpret_cast<float4*>(to + 2 * i) = make_float4(decay[i].x, dx[i].x, decay[i].y, dx[i].y);
+          to[i ^ Tile::pair_key(vt, vc)] = make_float4(decay[i].x, dx[i].x, decay[i].y, dx[i].y);
       }
       for (int e = me; e < 2 * TOK * NP / 8; e += kHelp) {
         const Eight<T> v = sm.bc_raw[tile & 1][e];
@@ -236,17 +242,12 @@ __global__ void __launch_bounds__(kCore<LPC> + 2 * kHelp) selective_scan_kernel(
       const Eight<T> x = sm.x[tile & 3][me];
       Eight<T> z, y;
       if (a.z != nullptr) z = sm.z[tile & 3][me];
-      const float* from = sm.y[tile & 1][vt][vc];
+      const float* from = sm.y[tile & 1][vt][0];
       float q[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        if constexpr (Tile::kParts == 4) {
-          const float4 v = *reinterpret_cast<const float4*>(from + 4 * (i ^ (me & 7)));
-          q[i] = (v.x + v.y) + (v.z + v.w);
-        } else {
-          const float2 v = *reinterpret_cast<const float2*>(from + 2 * (i ^ (me & 7)));
-          q[i] = v.x + v.y;
-        }
+        const float4 v = *reinterpret_cast<const float4*>(from + 4 * ((vc + i) ^ (me & 7)));
+        q[i] = (v.x + v.y) + (v.z + v.w);
       }
 #pragma unroll
       for (int i = 0; i < 8; ++i) q[i] = fmaf(i & 1 ? skip[i / 2].y : skip[i / 2].x, to_f32<T>(x.e[i]), q[i]);
@@ -300,17 +301,16 @@ __global__ void __launch_bounds__(kCore<LPC> + 2 * kHelp) selective_scan_kernel(
     const int n = number(i);
     const bool in = n < a.N && col < cols;
     const float v = old && in ? a.state[slot * pitch + at + n] : 0.0f;
-    const float q = CH && in ? -expf(a.a_log[at + n]) * kLog2e : 0.0f;
+    const float w = CH && in ? -expf(a.a_log[at + n]) * kLog2e : 0.0f;
     (i & 1 ? h[i / 2].y : h[i / 2].x) = v;
-    (i & 1 ? rate[i / 2].y : rate[i / 2].x) = q;
+    (i & 1 ? rate[i / 2].y : rate[i / 2].x) = w;
   }
   constexpr int kE = CH ? kHalf : 1;
-  struct Ahead {                                             // decays and inputs of four tokens
-    float2 e[4][kE], u[4][kHalf];
+  struct Ahead {                                             // decays and inputs of a token
+    float2 e[kE], u[kHalf];
   };
   __syncthreads();
   for (int tile = 0; tile < tiles; ++tile) {
-    const float2* sd = &sm.d[tile & 1][0][col];
     const float* sb = &sm.bc[tile & 1][0][0][kVec * l];
     const float* sc = &sm.bc[tile & 1][1][0][kVec * l];
     // numbers 2 k and 2 k + 1 of this lane and, where it has four neighbours, the next two
@@ -324,33 +324,34 @@ __global__ void __launch_bounds__(kCore<LPC> + 2 * kHelp) selective_scan_kernel(
         p = *reinterpret_cast<const float2*>(from);
       }
     };
-    auto token_ahead = [&](int t, float2 (&e)[kE], float2 (&u)[kHalf]) {
-      const float2 dd = sd[t * kCols];
+    auto token_ahead = [&](int i, int u, Ahead& to) {        // token i + u, i a multiple of 4: no part of a key
+      const float4* place = &sm.d[tile & 1][i + u][col / 2 ^ Tile::pair_key(u, col)];
+      const float2 dd = reinterpret_cast<const float2*>(place)[col & 1];
       const float2 dx = make_float2(dd.y, dd.y), step = make_float2(dd.x, dd.x);
-      if (!CH) e[0] = step;
+      if (!CH) to.e[0] = step;
 #pragma unroll
       for (int k = 0; k < kHalf; k += 2) {
         float2 b[2];
-        load(sb, t, k, b[0], b[1]);
+        load(sb, i + u, k, b[0], b[1]);
 #pragma unroll
         for (int j = k; j < k + kVec / 2; ++j) {
-          u[j] = __fmul2_rn(dx, b[j - k]);
+          to.u[j] = __fmul2_rn(dx, b[j - k]);
           if (CH) {
             const float2 p = __fmul2_rn(step, rate[j]);
-            e[CH ? j : 0] = make_float2(exp2_fast(p.x), exp2_fast(p.y));
+            to.e[CH ? j : 0] = make_float2(exp2_fast(p.x), exp2_fast(p.y));
           }
         }
       }
     };
-    auto token = [&](int t, const float2 (&e)[kE], const float2 (&u)[kHalf]) {
-      float2 s = make_float2(0.0f, 0.0f);
+    auto token = [&](int t, const Ahead& from) {
+      float2 s;
 #pragma unroll
       for (int k = 0; k < kHalf; k += 2) {
         float2 c[2];
         load(sc, t, k, c[0], c[1]);
 #pragma unroll
         for (int j = k; j < k + kVec / 2; ++j) {
-          h[j] = __ffma2_rn(e[CH ? j : 0], h[j], u[j]);
+          h[j] = __ffma2_rn(from.e[CH ? j : 0], h[j], from.u[j]);
           s = j == 0 ? __fmul2_rn(h[j], c[0]) : __ffma2_rn(h[j], c[j - k], s);
         }
       }
@@ -358,7 +359,7 @@ __global__ void __launch_bounds__(kCore<LPC> + 2 * kHelp) selective_scan_kernel(
     };
     auto leave = [&](int i, float (&part)[4]) {              // (i is a multiple of 4: no part of a key)
       float(*sy)[kCols][Tile::kParts] = sm.y[tile & 1] + i;
-      if constexpr (LPC <= 4) {
+      if constexpr (LPC == 4) {
 #pragma unroll
         for (int u = 0; u < 4; ++u) sy[u][col ^ Tile::key(u, col)][l] = part[u];
       } else {
@@ -381,36 +382,23 @@ __global__ void __launch_bounds__(kCore<LPC> + 2 * kHelp) selective_scan_kernel(
         }
       }
     };
-    auto make = [&](int i, Ahead& to) {
-#pragma unroll
-      for (int u = 0; u < 4; ++u) token_ahead(i + u, to.e[u], to.u[u]);
-    };
-    auto walk = [&](int i, const Ahead& from) {
-      float part[4];
-#pragma unroll
-      for (int u = 0; u < 4; ++u) part[u] = token(i + u, from.e[u], from.u[u]);
-      leave(i, part);
-    };
-    if constexpr (NPL <= 4) {
-      Ahead even, odd;
+    constexpr int kAhead = NPL <= 4 ? 8 : 4;
 #pragma unroll 1
-      for (int i = 0; i < TOK; i += 8) {
-        make(i, even);
-        make(i + 4, odd);
-        walk(i, even);
-        walk(i + 4, odd);
+    for (int i = 0; i < TOK; i += kAhead) {
+      Ahead x[kAhead];
+      if constexpr (NPL <= 4) {
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) token_ahead(i + u / 4 * 4, u % 4, x[u]);
       }
-    } else {
-#pragma unroll 1
-      for (int i = 0; i < TOK; i += 4) {
+#pragma unroll
+      for (int g4 = 0; g4 < kAhead; g4 += 4) {
         float part[4];
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
-          float2 e[kE], v[kHalf];
-          token_ahead(i + u, e, v);
-          part[u] = token(i + u, e, v);
+          if constexpr (NPL > 4) token_ahead(i, u, x[u]);
+          part[u] = token(i + g4 + u, x[g4 + u]);
         }
-        leave(i, part);
+        leave(i + g4, part);
       }
     }
     __syncthreads();
@@ -424,7 +412,7 @@ __global__ void __launch_bounds__(kCore<LPC> + 2 * kHelp) selective_scan_kernel(
 
 template <typename T, bool CH, int LPC, int NPL, bool WIDE>
 int launch_scan(const ScanArgs& a, cudaStream_t s) {
-  constexpr int kCols = kCore<LPC> / LPC, kSmem = sizeof(ScanTile<T, CH, LPC, NPL>);
+  constexpr int kCols = ScanTile<T, CH, LPC, NPL>::kCols, kSmem = sizeof(ScanTile<T, CH, LPC, NPL>);
   const auto kernel = selective_scan_kernel<T, CH, LPC, NPL, WIDE>;
   if (kSmem > 48 * 1024) {
     const int rc = launch_code(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem));
