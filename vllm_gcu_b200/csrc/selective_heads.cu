@@ -10,20 +10,26 @@
 //   S  [n x (p, 3)] = B^T (W_hi | W_mid | W_lo)        W_j = 2^(L_end - L_j) dt_j x_j in three parts: all 24 bits,
 //                                                      since the state is kept in 32
 //   Y1 [i x p]      = (M_hi + M_lo) X                  M_ij = G_ij 2^(L_i - L_j) dt_j in place of G, two parts
-// H lives in registers (lane n, 32 columns p per warp) and goes on as fp32.  Two parts leave 2^-17 of a
-// factor, an eighth of what the rows' own rounding to bf16 is off.
+// H lives in registers (lane n, 16 columns p per warp) and goes on as fp32.  Two parts leave 2^-17 of a
+// factor, which does not show beside the rows' own rounding to bf16; one part alone would make a result's error
+// 1.4 times as large.
 //
-// Decays (none above 1: step sizes are not below 0): a difference L_i - L_j is taken of sums in two floats or, in the 32 x 32 blocks on the diagonal, of 32-bit numbers
-// whose rounding the two sides' factors make good, so that a strong decay in front does not cost those
-// behind it their bits.  Outside the diagonal 2^(L_i - L_j) is a product of two factors below 1, with L at the row
-// block's start between them: 32 exponentials a row instead of 128.
+// Decays (none above 1: step sizes are not below 0): a difference L_i - L_j is taken of sums in two floats or, in the
+// 32 x 32 blocks on the diagonal, of 32-bit numbers whose rounding the two sides' factors make good, so that a
+// strong decay in front does not cost those behind it their bits.  Outside the diagonal 2^(L_i - L_j) is a product of two
+// factors below 1, with L at the row block's start between them: 32 exponentials a row instead of 128.
 //
 // A CTA walks the chunks of 64 columns of one head of one request; 16 warps do the arithmetic between the
 // products, one warp moves tiles (TMA), one issues the products, two compute step sizes and decays, a chunk
-// each, ahead of the rest (one chunk takes a warp 9000 cycles, in which the others do two).  W and M of a chunk are made while the tensor cores do Y2 and S, its state and result while
-// they do the next chunk's G.  The arithmetic bounds it, by latency: with 8 warps 4096 tokens of 128 heads took
-// 213 us.  Lanes 96 and up have four blocks of M that are not zero where lanes below 32 have one, so their
-// warps make less of W.
+// each, ahead of the rest.  W of a chunk is made a chunk ahead, M while the tensor cores do Y2 and S, state and result
+// while they do Y1 and the next chunk's G.  Lanes 96 and up have four blocks of M that are not zero where lanes below 32
+// have one, so their warps make less of W.
+//
+// 4096 tokens of 128 heads, 8 groups, N = 128, in one prompt: 115 us, 32 chunks of 3.1 us and 8 us of start (157 MB: 24
+// us at the copy's rate; the products' 78 GFLOP, splits included: 47 us).  The arithmetic between the products
+// bounds it: 60 per cent of the issue slots and half of the integer pipe, most of that for splits into parts of bf16;
+// tensor pipe 36 per cent.  On the way: 8 warps 213 us; decays from sums in 64 bits, by one warp, 131; with
+// more of it unrolled the instruction caches miss (no wait, no loop over products or groups is copied: 137 so, 119).
 #include "selective.cuh"
 
 namespace b200 {

@@ -60,8 +60,8 @@ __device__ __forceinline__ float update(float4& h, float2 e0, float2 e1, float2 
 
 // One token per request, rates per head, where a warp's columns belong to one head (width a multiple of their number)
 // and N is one of 4: a row of N numbers is spread over LPR lanes, NC times four each.  The state's bytes bound it: a warp
-// has 4 KB of it under way at once, and what a head's columns share is worked out once per warp (by row, 70 per cent of the
-// issue slots went into that: 96 requests of 80 heads of 64 x 128 in 113 us, 4.4 TB/s).
+// has 4 KB of it under way at once, and what a head's columns share is worked out once per warp.  96 requests of 80 heads of
+// 64 x 128: 77 us, 6.5 TB/s, the copy's rate (row by row, 70 per cent of the issue slots went into what they share: 113).
 template <typename T, int LPR, int NC, bool WIDE>
 __global__ void __launch_bounds__(128) heads_step_kernel(const ScanArgs a) {
   constexpr int kRows = NC > 1 ? 4 : 8, kGroups = 32 / LPR, kWarpCols = kRows * kGroups;
@@ -140,7 +140,8 @@ __global__ void __launch_bounds__(128) heads_step_kernel(const ScanArgs a) {
 }
 
 // One token per request, rates per channel, N a multiple of 4 up to 128: a warp holds 32 / LPR columns of RQ requests, so
-// that rates and skips are fetched and worked out once for them.
+// that rates and skips are fetched and worked out once for them.  64 requests of 8192 channels of 16, bf16: 24 us, 3.0 TB/s; the
+// chain slot - state - sum - row of a warp that lives for a few microseconds bounds it.
 template <typename T, int LPR, int RQ, bool WIDE>
 __global__ void __launch_bounds__(128) channels_step_kernel(const ScanArgs a) {
   constexpr int kGroups = 32 / LPR;
@@ -165,14 +166,14 @@ __global__ void __launch_bounds__(128) channels_step_kernel(const ScanArgs a) {
     const int slot = a.state != nullptr ? a.slots[r] : 0;
     ws[i] = a.state != nullptr && r0 + i < a.nd ? a.wslots[r] : -1;
     padding[i] = a.state != nullptr && (slot < 0 || slot >= a.num_slots);
-    if (padding[i]) ws[i] = -1;
+    if (padding[i] || ws[i] >= a.num_slots) ws[i] = -1;
     h[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     if (a.state != nullptr && !padding[i] && in && a.positions[r] != 0)
       h[i] = *reinterpret_cast<const float4*>(a.state + slot * pitch + at);
   }
 #pragma unroll
   for (int i = 0; i < RQ; ++i) {
-    const int r = min(r0 + i, a.nd - 1);
+    const int r = min(r0 + i, a.nd - 1);         // (behind the last request: its row again, and nothing is kept)
     x[i] = to_f32<T>(static_cast<const T*>(a.x)[r * a.ldx + col]);
     dt[i] = a.dt_f32 ? static_cast<const float*>(a.dt)[r * a.lddt + col]
                      : to_f32<T>(static_cast<const T*>(a.dt)[r * a.lddt + col]);
@@ -184,16 +185,35 @@ __global__ void __launch_bounds__(128) channels_step_kernel(const ScanArgs a) {
   if (in) rate = *reinterpret_cast<const float4*>(a.a_log + at);
   rate = make_float4(-expf(rate.x) * kLog2e, -expf(rate.y) * kLog2e, -expf(rate.z) * kLog2e, -expf(rate.w) * kLog2e);
   const float bias = a.dt_bias != nullptr ? a.dt_bias[col] : 0.0f, skip = a.d != nullptr ? a.d[col] : 0.0f;
+#pragma unroll
+  for (int i = 0; i < RQ; ++i) dt[i] += bias;
+  if (a.softplus) {
+#pragma unroll
+    for (int i = 0; i < RQ; i += 2) {
+      if constexpr (sizeof(T) == 2) {
+        const float2 p = softplus_pair(make_float2(dt[i], dt[i + 1 < RQ ? i + 1 : i]));
+        dt[i] = p.x;
+        if (i + 1 < RQ) dt[i + 1 < RQ ? i + 1 : i] = p.y;
+      } else {
+        dt[i] = softplus<T>(dt[i]);
+        if (i + 1 < RQ) dt[i + 1 < RQ ? i + 1 : i] = softplus<T>(dt[i + 1 < RQ ? i + 1 : i]);
+      }
+    }
+  }
+  if (a.limits) {
+#pragma unroll
+    for (int i = 0; i < RQ; ++i) dt[i] = limited(a, dt[i]);
+  }
   float s[RQ];
 #pragma unroll
   for (int i = 0; i < RQ; ++i) {
-    const float step = step_from<T>(a, dt[i], bias), dx = step * x[i];
+    const float step = dt[i], dx = step * x[i];
     const float2 p0 = __fmul2_rn(make_float2(step, step), make_float2(rate.x, rate.y));
     const float2 p1 = __fmul2_rn(make_float2(step, step), make_float2(rate.z, rate.w));
     const float2 e0 = make_float2(exp2_fast(p0.x), exp2_fast(p0.y)), e1 = make_float2(exp2_fast(p1.x), exp2_fast(p1.y));
     s[i] = update(h[i], e0, e1, make_float2(dx, dx), b[i], c[i]);
     s[i] = in ? s[i] : 0.0f;
-    if (in && ws[i] >= 0 && ws[i] < a.num_slots) *reinterpret_cast<float4*>(a.state + ws[i] * pitch + at) = h[i];
+    if (in && ws[i] >= 0) *reinterpret_cast<float4*>(a.state + ws[i] * pitch + at) = h[i];
   }
   const RowSums<RQ, LPR> sums(s, l);
 #pragma unroll

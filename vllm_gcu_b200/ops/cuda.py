@@ -1678,8 +1678,8 @@ def causal_conv(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tens
     step: ``x [T, C]`` (bf16, fp16 or fp32; row-strided views are fine), ``weight [taps, C]`` (up to 8 taps)
     and ``bias [C]`` fp32, ``act`` "silu" or None.  ``ring [slots, taps - 1, C]`` of x's type holds a request's
     last rows by position (position p in row ``p % (taps - 1)``), read in slot ``md.state_slots`` and left in
-    ``write_slots`` (default: the same; another one forks a request, and must not be a slot that another request
-    of the step reads); None: zeros in front of the portions.  ``md`` also gives ``positions``,
+    ``write_slots`` (default: the same; another one forks a request); None: zeros in front of the portions.  A slot
+    that one request writes must be neither read nor written by another one of the step.  ``md`` also gives ``positions``,
     ``num_decode_tokens`` and ``cu_q_prefill``.  A request whose slot lies outside the ring gives zeros, one whose
     write slot does leaves its ring nowhere; rows behind the last portion are not written."""
     if x.dim() != 2 or x.dtype not in DTYPE_CODE:
