@@ -447,3 +447,40 @@ def test_calls_on_another_stream_than_the_tensors():
     torch.cuda.current_stream().wait_stream(side)
     assert torch.equal(got, want) and torch.equal(state, want_state)
     assert torch.equal(norm, K.group_norm_gate(want, None, torch.ones(128, device="cuda"), 2, 1e-5))
+
+
+@pytest.mark.parametrize("bad", [math.inf, -math.inf, math.nan])
+@pytest.mark.parametrize("form,H,P,N,G", [("heads", 2, 64, 128, 1), ("heads", 2, 64, 64, 2), ("heads", 2, 8, 8, 1), ("channels", 32, 1, 16, 1)])
+def test_later_tokens_never_show(form, H, P, N, G, bad):
+    """A number of x, B or C that is none shows in its own token's results and, of x and B, in later ones', nowhere
+    else: a token is masked from those in front of it, a column of x from the other ones."""
+    from vllm_gcu_b200.ops import cuda as K
+    md = S.step(1, [200, 40], [3, 4, 0])
+    k = S.scan_case(form, H, P, N, G, md, BF16)
+    k["z"] = None
+    good = _views({n: v for n, v in k.items() if v is not None})
+    state = good.pop("state")
+    kept = state.clone()
+    want = K.selective_scan(**good, groups=G, md=md.to("cuda"), state=kept)
+    first, end, col = 1 + 77, 201, 3                          # token 77 of the first portion
+    for which in ("x", "b", "c"):
+        dev = _views({n: v for n, v in k.items() if v is not None})
+        new = dev.pop("state")
+        dev[which][first, col] = bad
+        got = K.selective_scan(**dev, groups=G, md=md.to("cuda"), state=new)
+        hit = torch.zeros(got.shape, dtype=torch.bool, device="cuda")
+        per = H * P // G                                      # columns of B's and C's first group
+        if which == "x":
+            hit[first:end, col] = True
+        else:
+            hit[first:end if which == "b" else first + 1, :per] = True
+        assert not torch.isfinite(got[hit]).any(), which
+        assert torch.equal(got[~hit], want[~hit]), which
+        slot = int(md.state_slots[1])
+        a, b = new[slot].flatten(0, -2), kept[slot].flatten(0, -2)   # [columns, N]
+        lost = torch.zeros(a.shape, dtype=torch.bool, device="cuda")
+        if which == "x":
+            lost[col] = True
+        elif which == "b":
+            lost[:per, col] = True
+        assert not torch.isfinite(a[lost]).any() and torch.equal(a[~lost], b[~lost]), which

@@ -52,6 +52,8 @@ struct Scalars {
   float w[kRows];         // dt_j 2^(L_end - L_j)
   float e[kRows];         // 2^(L_i)
   float end[4];           // 2^(L_end)
+  int bad[kP];            // by column: the first token whose x is infinite or no number (kRows: none)
+  int any_bad[4];
 };
 constexpr int kOffBars = kOffScal + 4 * static_cast<int>(sizeof(Scalars));
 constexpr int kSmem = kOffBars + 256 + 1024;
@@ -175,6 +177,29 @@ __device__ __forceinline__ void chunk_scalars(const ScanArgs& a, int n, float bi
   if (lane < 16) put(s->off + 32, o2);
   if (lane < 24) put(s->off + 96, o3);
   if (lane == 0) s->end[0] = exp2_fast(end.hi);
+  s->bad[lane] = s->bad[lane + 32] = kRows;
+  if (lane == 0) s->any_bad[0] = 0;
+}
+
+// Numbers of x that are infinite or none, eight at `x` (columns col and on of a token): in the product M X they would
+// show in the tokens in front, whose weights are 0.  Zeros take their place there (W keeps them), and the
+// results of their column from their token on are no numbers.
+__device__ __noinline__ void hide_bad(Scalars* s, unsigned char* x, int token, int col) {
+  unsigned short* v = reinterpret_cast<unsigned short*>(x);
+  for (int i = 0; i < 8; ++i) {
+    if ((v[i] & 0x7f80) != 0x7f80) continue;
+    v[i] = 0;
+    atomicMin(&s->bad[col + i], token);
+    s->any_bad[0] = 1;
+  }
+}
+
+__device__ __noinline__ uint4 show_bad(const Scalars* s, uint4 y, int token, int col) {
+  uint32_t v[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    if (token >= s->bad[col + i]) v[i / 2] |= 0x7fffu << (i % 2 * 16);
+  return make_uint4(v[0], v[1], v[2], v[3]);
 }
 
 // A wait of a warp that computes.  No lane leaves: when the budget runs out the warp goes on over numbers without
@@ -282,7 +307,7 @@ heads_kernel(const ScanArgs a, const __grid_constant__ CUtensorMap tm_x, const _
     // W of chunk c = x times its weight, in three parts
     auto make_w = [&](int c) {
       const int n = min(kRows, po.end - po.first - c * kRows);
-      const Scalars* s = scal + (c & 3);
+      Scalars* s = scal + (c & 3);
       unsigned char* x = smem + kOffX + (c & 1) * kSub;
       pass_warp(&bar[kXFull0 + (c & 1)], (c >> 1) & 1, status, 0x101u, abort_flag);
       // rows of other requests: zeros, they may hold anything
@@ -301,9 +326,12 @@ heads_kernel(const ScanArgs a, const __grid_constant__ CUtensorMap tm_x, const _
         const float2 w = both(s->w[row]);
         const uint32_t in[4] = {v.x, v.y, v.z, v.w};
         uint32_t p[3][4];
+        float2 none = both(0.0f);
 #pragma unroll
         for (int m = 0; m < 4; ++m) {
-          float2 f = mul2(w, unpack_bf16x2(in[m]));
+          float2 f = unpack_bf16x2(in[m]);
+          none = fma2(f, both(0.0f), none);
+          f = mul2(w, f);
           p[0][m] = split(f);
           p[1][m] = split(f);
           p[2][m] = pack(f);
@@ -311,6 +339,7 @@ heads_kernel(const ScanArgs a, const __grid_constant__ CUtensorMap tm_x, const _
 #pragma unroll
         for (int m = 0; m < 3; ++m)
           *reinterpret_cast<uint4*>(smem + kOffW + m * kSub + to) = make_uint4(p[m][0], p[m][1], p[m][2], p[m][3]);
+        if (none.x + none.y != 0.0f) hide_bad(s, x + to, row, (lane & 7) * 8);
       }
       fence_async_smem();
       __syncwarp();
@@ -416,6 +445,7 @@ heads_kernel(const ScanArgs a, const __grid_constant__ CUtensorMap tm_x, const _
         __syncwarp();
         if (lane == 0) mbar_arrive(&bar[kYFree]);
         const float2 e = both(s->e[i]);
+        const bool bad = s->any_bad[0] != 0;
         const long long t = po.first + c * kRows + i;
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
@@ -436,7 +466,8 @@ heads_kernel(const ScanArgs a, const __grid_constant__ CUtensorMap tm_x, const _
             for (int k = 0; k < 4; ++k)
               f[k] = mul2(f[k], make_float2(silu<__nv_bfloat16>(z[2 * k]), silu<__nv_bfloat16>(z[2 * k + 1])));
           }
-          const uint4 y = make_uint4(pack(f[0]), pack(f[1]), pack(f[2]), pack(f[3]));
+          uint4 y = make_uint4(pack(f[0]), pack(f[1]), pack(f[2]), pack(f[3]));
+          if (bad) y = show_bad(s, y, i, part * 16 + u * 8);
           // a whole chunk leaves as a tile, in place of its x; the last rows of a portion one by one
           if (n == kRows) *reinterpret_cast<uint4*>(at_x) = y;
           else if (i < n) *reinterpret_cast<uint4*>(out + t * a.ldo + part * 16 + u * 8) = y;
