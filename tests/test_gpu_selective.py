@@ -484,3 +484,26 @@ def test_later_tokens_never_show(form, H, P, N, G, bad):
         elif which == "b":
             lost[:per, col] = True
         assert not torch.isfinite(a[lost]).any() and torch.equal(a[~lost], b[~lost]), which
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("H,P,N,G", [(16, 64, 128, 2), (16, 64, 64, 1), (4, 16, 64, 1), (2, 64, 16, 1), (4, 32, 32, 2), (4, 12, 160, 1), (3, 7, 12, 1)])
+def test_many_short_portions(H, P, N, G, dtype):
+    """Many portions of a few tokens, some without any, beside single tokens; then two of them long enough for other
+    kernels: states and results of the same formula."""
+    from vllm_gcu_b200.ops import cuda as K
+    for lens in ([1, 3, 0, 2, 5, 1, 1, 9, 4, 2, 0, 1], [2, 1, 140, 1], [31, 90]):
+        md = S.step(3, lens, behind=2)
+        k = S.scan_case("heads", H, P, N, G, md, dtype)
+        state, dev = k["state"], _views(k)
+        R = len(md.lens)
+        write = (md.state_slots + R).int()
+        want, mag, new, smag = S.scan(**{n: v for n, v in k.items() if n not in ("row", "state")}, groups=G, md=md,
+                                      state=state, write=write)
+        kept, got = dev.pop("state"), _fill((md.positions.shape[0], H * P), dtype)
+        before = got.clone()
+        K.selective_scan(**dev, groups=G, md=md.to("cuda"), state=kept, out=got, write_slots=write.cuda())
+        n = md.tokens
+        S.near(got[:n], want[:n], dtype, _rounding(md, N, mag[:n], dtype))
+        assert torch.equal(got[n:], before[n:])
+        S.near(kept, new, F32, S.scan_rounding(md, N, smag))

@@ -480,8 +480,10 @@ B200_API int b200_selective_scan(const void* call, void* stream) {
   a.limits = k.dt_max < INFINITY || k.dt_min > 0.0f || !k.softplus;    // (a softplus is not below 0)
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const bool channels = k.per_channel != 0;
+  int rc = 0;
+  if (!channels && launch_short_portions(a, k.dtype, s, &rc)) return rc;
   if (a.nd > 0) {
-    const int rc = launch_single_tokens(a, channels, k.dtype, s);
+    rc = launch_single_tokens(a, channels, k.dtype, s);
     if (rc != 0) return rc;
   }
   if (a.np == 0) return 0;

@@ -114,6 +114,8 @@ struct __align__(16) Raw<float, 4> {
 
 // One token per request (selective_step.cu).  dtype: 0 bf16, 1 fp16, 2 fp32.
 int launch_single_tokens(const ScanArgs& a, bool per_channel, int dtype, cudaStream_t s);
+// The whole step where its portions are short and rates are per head; false where it does not apply.
+bool launch_short_portions(const ScanArgs& a, int dtype, cudaStream_t s, int* rc);
 // Portions of prompts by products of tiles (selective_heads.cu): rates per head, bf16 rows on 16-byte boundaries.
 bool heads_by_tiles(const ScanArgs& a);
 int launch_heads_by_tiles(const ScanArgs& a, cudaStream_t s);

@@ -58,13 +58,15 @@ __device__ __forceinline__ float update(float4& h, float2 e0, float2 e1, float2 
   return s.x + s.y;
 }
 
-// One token per request, rates per head, where a warp's columns belong to one head (width a multiple of their number)
-// and N is one of 4: a row of N numbers is spread over LPR lanes, NC times four each.  The state's bytes bound it: a warp
-// has 4 KB of it under way at once, and what a head's columns share is worked out once per warp.  96 requests of 80 heads of
-// 64 x 128: 77 us, 6.5 TB/s, the copy's rate (row by row, 70 per cent of the issue slots went into what they share: 113).
-template <typename T, int LPR, int NC, bool WIDE>
+// Single tokens and short portions, rates per head, where a warp's columns belong to one head (width a multiple of their
+// number) and N is one of 4: a row of N numbers is spread over LPR lanes, NC times four each, and stays in registers while the
+// warp walks the request's tokens, the next one under way.  The state's bytes bound it: a warp has 4 KB of it under way
+// at once, and what a head's columns share is worked out once per warp.  96 requests of 80 heads of 64 x 128: 77 us, 6.5
+// TB/s, the copy's rate (row by row, 70 per cent of the issue slots went into what they share: 113; with the next token's
+// registers, which MANY is for, 91).
+template <typename T, int LPR, int NC, bool MANY, bool WIDE>
 __global__ void __launch_bounds__(128) heads_step_kernel(const ScanArgs a) {
-  constexpr int kRows = NC > 1 ? 4 : 8, kGroups = 32 / LPR, kWarpCols = kRows * kGroups;
+  constexpr int kRows = NC > 1 ? 4 : 8, kGroups = 32 / LPR, kWarpCols = kRows * kGroups, kX = (kWarpCols + 31) / 32;
   grid_release_small();
   grid_wait();
   const int r = blockIdx.y, lane = threadIdx.x & 31, l = lane & (LPR - 1), grp = lane / LPR;
@@ -73,10 +75,16 @@ __global__ void __launch_bounds__(128) heads_step_kernel(const ScanArgs a) {
   if (c0 >= cols) return;
   const int slot = a.state != nullptr ? a.slots[r] : 0;
   const int ws = a.state != nullptr ? a.wslots[r] : -1;
-  const bool old = a.state != nullptr && a.positions[r] != 0;
-  T* out = static_cast<T*>(a.out) + r * a.ldo + c0;
+  Portion po = {r, r + 1};
+  if constexpr (MANY) {
+    po = portion_of(r, a.nd, a.cu_q, a.T);
+    if (po.first >= po.end) return;
+  }
+  const bool old = a.state != nullptr && a.positions[po.first] != 0;
+  T* out = static_cast<T*>(a.out) + c0;
   if (a.state != nullptr && (slot < 0 || slot >= a.num_slots)) {
-    for (int i = lane; i < kWarpCols; i += 32) out[i] = from_f32<T>(0.0f);
+    for (int t = po.first; t < po.end; ++t)
+      for (int i = lane; i < kWarpCols; i += 32) out[t * a.ldo + i] = from_f32<T>(0.0f);
     return;
   }
   const long long pitch = static_cast<long long>(cols) * a.N;
@@ -91,52 +99,71 @@ __global__ void __launch_bounds__(128) heads_step_kernel(const ScanArgs a) {
         h[i][k] = *reinterpret_cast<const float4*>(a.state + slot * pitch + at + i * kGroups * a.N + LPR * k * 4);
     }
   const int hd = c0 / a.width, g = hd / (a.heads / a.groups);
-  // x of the warp's columns: column j in lane j % 32
-  float x[kWarpCols / 32 + 1];
+  const T* bsrc = static_cast<const T*>(a.b) + g * a.N + l * 4;
+  const T* csrc = static_cast<const T*>(a.c) + g * a.N + l * 4;
+  const float rate = expf(a.a_log[hd]), skip = a.d != nullptr ? a.d[hd] : 0.0f;
+  const float bias = a.dt_bias != nullptr ? a.dt_bias[hd] : 0.0f;
+  struct Token {
+    float x[kX];                                 // x of the warp's columns: column j in lane j % 32
+    float4 b[NC], c[NC];
+    float dt;
+  };
+  auto bring = [&](long long t, Token& to) {
 #pragma unroll
-  for (int j = 0; j <= (kWarpCols - 1) / 32; ++j)
-    x[j] = j * 32 + lane < kWarpCols ? to_f32<T>(static_cast<const T*>(a.x)[r * a.ldx + c0 + j * 32 + lane]) : 0.0f;
-  float4 b[NC], c[NC];
+    for (int j = 0; j < kX; ++j) {
+      const int c = min(j * 32 + lane, kWarpCols - 1);
+      to.x[j] = to_f32<T>(static_cast<const T*>(a.x)[t * a.ldx + c0 + c]);
+    }
 #pragma unroll
-  for (int k = 0; k < NC; ++k) {
-    const int n = (l + LPR * k) * 4;
-    b[k] = load_four<T, WIDE>(static_cast<const T*>(a.b) + r * a.ldb + g * a.N + n, n < a.N);
-    c[k] = load_four<T, WIDE>(static_cast<const T*>(a.c) + r * a.ldc + g * a.N + n, n < a.N);
-  }
-  const float dt = step_size<T>(a, r, hd);
-  const float decay = expf(-dt * expf(a.a_log[hd]));
-  float s[kRows];
+    for (int k = 0; k < NC; ++k) {
+      to.b[k] = load_four<T, WIDE>(bsrc + t * a.ldb + LPR * k * 4, (l + LPR * k) * 4 < a.N);
+      to.c[k] = load_four<T, WIDE>(csrc + t * a.ldc + LPR * k * 4, (l + LPR * k) * 4 < a.N);
+    }
+    to.dt = a.dt_f32 ? static_cast<const float*>(a.dt)[t * a.lddt + hd]
+                     : to_f32<T>(static_cast<const T*>(a.dt)[t * a.lddt + hd]);
+  };
+  Token now, next;
+  bring(po.first, now);
+  int t = po.first;
+  do {
+    const bool more = MANY && t + 1 < po.end;
+    if (more) bring(t + 1, next);
+    const float dt = step_from<T>(a, now.dt, bias);
+    const float decay = expf(-dt * rate);
+    float s[kRows];
 #pragma unroll
-  for (int i = 0; i < kRows; ++i) {
-    const float dx = dt * __shfl_sync(0xffffffffu, x[i * kGroups / 32], (i * kGroups + grp) & 31);
-    s[i] = 0.0f;
-#pragma unroll
-    for (int k = 0; k < NC; ++k)
-      s[i] += update(h[i][k], make_float2(decay, decay), make_float2(decay, decay), make_float2(dx, dx), b[k], c[k]);
-  }
-  if (ws >= 0 && ws < a.num_slots) {
-#pragma unroll
-    for (int i = 0; i < kRows; ++i)
+    for (int i = 0; i < kRows; ++i) {
+      const float dx = dt * __shfl_sync(0xffffffffu, now.x[i * kGroups / 32], (i * kGroups + grp) & 31);
+      s[i] = 0.0f;
 #pragma unroll
       for (int k = 0; k < NC; ++k)
-        if ((l + LPR * k) * 4 < a.N)
-          *reinterpret_cast<float4*>(a.state + ws * pitch + at + i * kGroups * a.N + LPR * k * 4) = h[i][k];
-  }
-  const RowSums<kRows, LPR> sums(s, l);
-  const float skip = a.d != nullptr ? a.d[hd] : 0.0f;
-#pragma unroll
-  for (int i = 0; i < sums.kLeft; ++i) {
-    const int j = (sums.first + i) * kGroups + grp;      // column of the warp
-    float xv = 0.0f;
-#pragma unroll
-    for (int m = 0; m <= (kWarpCols - 1) / 32; ++m) {
-      const float v = __shfl_sync(0xffffffffu, x[m], j & 31);
-      if (j / 32 == m) xv = v;
+        s[i] += update(h[i][k], make_float2(decay, decay), make_float2(decay, decay), make_float2(dx, dx), now.b[k],
+                       now.c[k]);
     }
-    float y = fmaf(skip, xv, sums.v[i]);
-    if (a.z != nullptr) y *= silu<T>(to_f32<T>(static_cast<const T*>(a.z)[r * a.ldz + c0 + j]));
-    if (sums.keeps(l)) out[j] = from_f32<T>(y);
-  }
+    if (!more && ws >= 0 && ws < a.num_slots) {
+#pragma unroll
+      for (int i = 0; i < kRows; ++i)
+#pragma unroll
+        for (int k = 0; k < NC; ++k)
+          if ((l + LPR * k) * 4 < a.N)
+            *reinterpret_cast<float4*>(a.state + ws * pitch + at + i * kGroups * a.N + LPR * k * 4) = h[i][k];
+    }
+    const RowSums<kRows, LPR> sums(s, l);
+#pragma unroll
+    for (int i = 0; i < sums.kLeft; ++i) {
+      const int j = (sums.first + i) * kGroups + grp;    // column of the warp
+      float xv = 0.0f;
+#pragma unroll
+      for (int m = 0; m < kX; ++m) {
+        const float v = __shfl_sync(0xffffffffu, now.x[m], j & 31);
+        if (j / 32 == m) xv = v;
+      }
+      float y = fmaf(skip, xv, sums.v[i]);
+      if (a.z != nullptr) y *= silu<T>(to_f32<T>(static_cast<const T*>(a.z)[t * a.ldz + c0 + j]));
+      if (sums.keeps(l)) out[t * a.ldo + j] = from_f32<T>(y);
+    }
+    if constexpr (MANY) now = next;
+  } while (MANY && ++t < po.end);
 }
 
 // One token per request, rates per channel, N a multiple of 4 up to 128: a warp holds 32 / LPR columns of RQ requests, so
@@ -344,12 +371,12 @@ __global__ void __launch_bounds__(128) selective_step_kernel(const ScanArgs a) {
   }
 }
 
-template <typename T, int LPR, int NC>
+template <typename T, int LPR, int NC, bool MANY>
 int launch_heads_step(const ScanArgs& a, cudaStream_t s) {
   constexpr int kCtaCols = 4 * (NC > 1 ? 4 : 8) * (32 / LPR);
-  const dim3 grid((a.heads * a.width + kCtaCols - 1) / kCtaCols, a.nd);
-  return a.wide ? launch_overlapped(heads_step_kernel<T, LPR, NC, true>, grid, dim3(128), 0, s, a)
-                : launch_overlapped(heads_step_kernel<T, LPR, NC, false>, grid, dim3(128), 0, s, a);
+  const dim3 grid((a.heads * a.width + kCtaCols - 1) / kCtaCols, MANY ? a.nd + a.np : a.nd);
+  return a.wide ? launch_overlapped(heads_step_kernel<T, LPR, NC, MANY, true>, grid, dim3(128), 0, s, a)
+                : launch_overlapped(heads_step_kernel<T, LPR, NC, MANY, false>, grid, dim3(128), 0, s, a);
 }
 template <typename T, int LPR, int RQ>
 int launch_channels_step(const ScanArgs& a, cudaStream_t s) {
@@ -368,6 +395,19 @@ int launch_channels_step(const ScanArgs& a, cudaStream_t s) {
   return launch_channels_step<T, LPR, 1>(a, s);
 }
 
+constexpr int kNotTaken = -1000;
+// The single tokens of a step (MANY: all of its requests) by heads_step_kernel, where the sizes allow it.
+template <typename T, bool MANY>
+int launch_heads(const ScanArgs& a, cudaStream_t s) {
+  if (a.N % 4 != 0) return kNotTaken;
+  if (a.N > 64 && a.N <= 128 && a.width % 8 == 0) return launch_heads_step<T, 32, 1, MANY>(a, s);
+  if (a.N > 128 && a.width % 4 == 0) return launch_heads_step<T, 32, 2, MANY>(a, s);
+  if (a.N > 32 && a.N <= 64 && a.width % 16 == 0) return launch_heads_step<T, 16, 1, MANY>(a, s);
+  if (a.N > 16 && a.N <= 32 && a.width % 32 == 0) return launch_heads_step<T, 8, 1, MANY>(a, s);
+  if (a.N <= 16 && a.width % 64 == 0) return launch_heads_step<T, 4, 1, MANY>(a, s);
+  return kNotTaken;
+}
+
 template <typename T, bool CH>
 int launch_step(const ScanArgs& a, cudaStream_t s) {
   const int cols = a.heads * a.width;
@@ -379,11 +419,8 @@ int launch_step(const ScanArgs& a, cudaStream_t s) {
       if (a.N <= 64) return launch_channels_step<T, 16>(a, s);
       if (a.N <= 128) return launch_channels_step<T, 32>(a, s);
     } else {
-      if (a.N > 64 && a.N <= 128 && a.width % 8 == 0) return launch_heads_step<T, 32, 1>(a, s);
-      if (a.N > 128 && a.width % 4 == 0) return launch_heads_step<T, 32, 2>(a, s);
-      if (a.N > 32 && a.N <= 64 && a.width % 16 == 0) return launch_heads_step<T, 16, 1>(a, s);
-      if (a.N > 16 && a.N <= 32 && a.width % 32 == 0) return launch_heads_step<T, 8, 1>(a, s);
-      if (a.N <= 16 && a.width % 64 == 0) return launch_heads_step<T, 4, 1>(a, s);
+      const int rc = launch_heads<T, false>(a, s);
+      if (rc != kNotTaken) return rc;
     }
   }
 #define STEP(LPR, NC, V)                                                              \
@@ -404,6 +441,26 @@ int launch_step(const ScanArgs& a, cudaStream_t s) {
   if (a.N <= 128) return STEP(32, 4, 1);
   return STEP(32, 8, 1);
 #undef STEP
+}
+
+// Portions of a dozen tokens on average, whose state's way in and out is most of the work.  us by this kernel and by tiles,
+// 96 requests of 80 heads of 64 x 128: 95 and 404 for 1 token each, 246 and 418 for 8, 440 and 422 for 16; token after
+// token in 16 bits, 12 requests of 16 heads: 18 and 27 for 8, 32 and 39 for 32, 60 and 60 for 64.  Only the mean length is
+// known here.  A token of a portion takes 0.55 us, so the rows of a step are kept to what the tiles would take twice
+// as long for were they all one portion's (8 us for a CTA per SM), or, for other types, to 512.
+bool launch_short_portions(const ScanArgs& a, int dtype, cudaStream_t s, int* rc) {
+  const long long rows = a.T - a.nd;
+  if (a.np == 0) return false;
+  if (dtype == 0 && heads_by_tiles(a)) {
+    const long long ctas = static_cast<long long>(a.np) * a.heads * (a.width / 64), sms = sm_count();
+    if (rows > 12ll * a.np || rows > 28 * ((ctas + sms - 1) / sms)) return false;
+  } else if (rows > 32ll * a.np || rows > 512) {
+    return false;
+  }
+  *rc = dtype == 0   ? launch_heads<__nv_bfloat16, true>(a, s)
+        : dtype == 1 ? launch_heads<__half, true>(a, s)
+                     : launch_heads<float, true>(a, s);
+  return *rc != kNotTaken;
 }
 
 int launch_single_tokens(const ScanArgs& a, bool per_channel, int dtype, cudaStream_t s) {
