@@ -126,7 +126,8 @@ def test_scan_of_longer_portions(lens, form, H, P, N, G):
         k = S.scan_case(form, H, P, N, G, md, BF16, seed=len(lens))
         if strong:
             dt = k["dt"].float()
-            k["dt"] = torch.where(torch.rand(dt.shape, generator=torch.Generator().manual_seed(1)) < 0.1, 300.0, dt - 3).to(BF16)
+            some = torch.rand(dt.shape, generator=torch.Generator().manual_seed(1)) < 0.1
+            k["dt"] = torch.where(some, 300.0, dt - 3).to(BF16)
         state, dev = k["state"], _views(k)
         kw = {n: v for n, v in k.items() if n not in ("row", "state")}
         want, mag, new, smag = S.scan(**kw, groups=G, md=md, state=state)
@@ -239,7 +240,8 @@ class Mixer:
 
     def rows(self, T, dtype, seed=0):
         g = torch.Generator().manual_seed(seed)
-        return torch.randn(T, 2 * self.D + 2 * self.G * self.N + (self.D if self.channels else self.H), generator=g).to(dtype)
+        steps = self.D if self.channels else self.H
+        return torch.randn(T, 2 * self.D + 2 * self.G * self.N + steps, generator=g).to(dtype)
 
     def __call__(self, ops, row, md):
         D, gn = self.D, self.G * self.N
@@ -386,7 +388,8 @@ def test_growing_states(form, H, P, N, dtype):
 
 
 @pytest.mark.parametrize("decodes,lens", [(6, ()), (0, (20, 3)), (2, (9,))])
-@pytest.mark.parametrize("form,H,P,N", [("heads", 2, 64, 128), ("heads", 4, 16, 12), ("channels", 64, 1, 16), ("channels", 20, 1, 7)])
+@pytest.mark.parametrize("form,H,P,N", [("heads", 2, 64, 128), ("heads", 4, 16, 12), ("channels", 64, 1, 16),
+                                        ("channels", 20, 1, 7)])
 def test_weights_off_16_byte_boundaries(form, H, P, N, decodes, lens):
     """Rates, skips and biases that are parts of larger tensors, and rows that start anywhere."""
     from vllm_gcu_b200.ops import cuda as K
@@ -450,7 +453,8 @@ def test_calls_on_another_stream_than_the_tensors():
 
 
 @pytest.mark.parametrize("bad", [math.inf, -math.inf, math.nan])
-@pytest.mark.parametrize("form,H,P,N,G", [("heads", 2, 64, 128, 1), ("heads", 2, 64, 64, 2), ("heads", 2, 8, 8, 1), ("channels", 32, 1, 16, 1)])
+@pytest.mark.parametrize("form,H,P,N,G", [("heads", 2, 64, 128, 1), ("heads", 2, 64, 64, 2), ("heads", 2, 8, 8, 1),
+                                          ("channels", 32, 1, 16, 1)])
 def test_later_tokens_never_show(form, H, P, N, G, bad):
     """A number of x, B or C that is none shows in its own token's results and, of x and B, in later ones', nowhere
     else: a token is masked from those in front of it, a column of x from the other ones."""
@@ -487,7 +491,8 @@ def test_later_tokens_never_show(form, H, P, N, G, bad):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("H,P,N,G", [(16, 64, 128, 2), (16, 64, 64, 1), (4, 16, 64, 1), (2, 64, 16, 1), (4, 32, 32, 2), (4, 12, 160, 1), (3, 7, 12, 1)])
+@pytest.mark.parametrize("H,P,N,G", [(16, 64, 128, 2), (16, 64, 64, 1), (4, 16, 64, 1), (2, 64, 16, 1), (4, 32, 32, 2),
+                                     (4, 12, 160, 1), (3, 7, 12, 1)])
 def test_many_short_portions(H, P, N, G, dtype):
     """Many portions of a few tokens, some without any, beside single tokens; then two of them long enough for other
     kernels: states and results of the same formula."""

@@ -1,8 +1,8 @@
 // Short causal convolution of a state-space mixer (sm_100a), over the rows of a step: nd single tokens, one per
 // request, then the portions of np prompts (offsets behind row nd in cu_q):
 //   c_t = act(bias + sum_j w[j] x of (taps - 1 - j) tokens ago), per channel
-// A request's last inputs lie in ring [slot, taps - 1, channels], position p in row p % (taps - 1), read in one slot and left
-// in another (usually the same).  A portion that starts at position 0 starts from zeros whatever the slot holds.  A
+// A request's last inputs lie in ring [slot, taps - 1, channels], position p in row p % (taps - 1), read in one slot
+// and left in another (usually the same).  A portion that starts at position 0 starts from zeros whatever the slot holds.  A
 // request whose slot is outside the ring (padding of a captured batch) gives rows of zeros; one whose write slot is
 // outside leaves its inputs nowhere.
 #include "selective.cuh"

@@ -20,18 +20,18 @@ namespace selective {
 // Portions of prompts, token after token.  A CTA holds the columns of one request that kCore / LPC lane groups
 // make: a column's numbers of state lie in the registers of LPC lanes, NPL each, and a token costs a number one
 // decay (rates per channel: a power of two, of which the special function unit does 16 per clock and SM), two
-// multiply-adds and a product.  Inputs pass through shared memory kTok tokens at a time.  While the core
-// warps walk tile i, four warps copy tile i + 2 and turn tile i + 1 into step sizes and factors, eight neighbouring
-// elements a thread, and four others finish tile i - 1 (skip, gate, store); one barrier per tile.  What is done per element
-// is half of the instructions and the chain along the tokens leaves the scheduler idle: 2048 tokens of 8192 channels
-// took 235 us with all warps doing both in turn and 145 with four warps for the elements.
-// The sum over the lanes of a column is the helpers': four lanes leave a part of it each; where there are
-// more, pairs of lanes trade the parts of two tokens first, so that each ends up with those of its own token.  With
-// few numbers per lane, decays and inputs of eight tokens are made before their chain is walked.
-// Shared memory's bandwidth bounds rates per channel: 11 turns of 128 bytes a warp and token, about 100 of 120 cycles a token
-// on the SMs that hold two CTAs: 2048 tokens of 8192 channels in 132 us, 73 per cent of all SMs' turns.  (Two columns per
-// lane group, whose B and C would be read once, leave one core warp a scheduler: 143 us.  B and C in 16 bits until a lane
-// has them save 4 of the turns and cost 8 instructions: 139.)
+// multiply-adds and a product.  Inputs pass through shared memory kTok tokens at a time.  While the core warps
+// walk tile i, four warps copy tile i + 2 and turn tile i + 1 into step sizes and factors, eight neighbouring
+// elements a thread, and four others finish tile i - 1 (skip, gate, store); one barrier per tile.  What is done
+// per element is half of the instructions and the chain along the tokens leaves the scheduler idle: 2048 tokens of
+// 8192 channels took 235 us with all warps doing both in turn and 145 with four warps for the elements. The sum
+// over the lanes of a column is the helpers': four lanes leave a part of it each; where there are more, pairs of
+// lanes trade the parts of two tokens first, so that each ends up with those of its own token.  With few numbers
+// per lane, decays and inputs of eight tokens are made before their chain is walked. Shared memory's bandwidth
+// bounds rates per channel: 11 turns of 128 bytes a warp and token, about 100 of 120 cycles a token on the SMs
+// that hold two CTAs: 2048 tokens of 8192 channels in 132 us, 73 per cent of all SMs' turns.  (Two columns per
+// lane group, whose B and C would be read once, leave one core warp a scheduler: 143 us.  B and C in 16 bits until
+// a lane has them save 4 of the turns and cost 8 instructions: 139.)
 template <int LPC>
 constexpr int kCore = LPC >= 8 ? 256 : 128;
 constexpr int kHelp = 128;                       // threads that bring elements, and threads that finish them

@@ -278,7 +278,8 @@ heads_kernel(const ScanArgs a, const __grid_constant__ CUtensorMap tm_x, const _
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
       h[k] = both(0.0f);
-      if (old && i < N) h[k] = make_float2(a.state[slot * head_at + at + 2 * k * N], a.state[slot * head_at + at + (2 * k + 1) * N]);
+      const float* from = a.state + slot * head_at + at + 2 * k * N;
+      if (old && i < N) h[k] = make_float2(from[0], from[N]);
     }
     auto put_state = [&]() {
       if (i < N) {
@@ -423,8 +424,9 @@ heads_kernel(const ScanArgs a, const __grid_constant__ CUtensorMap tm_x, const _
         tmem_ld_wait();
 #pragma unroll
         for (int k = 0; k < 8; ++k)
-          h[k] = fma2(both(keep), h[k], add2(bits2(v[0][2 * k], v[0][2 * k + 1]),
-                                             add2(bits2(v[1][2 * k], v[1][2 * k + 1]), bits2(v[2][2 * k], v[2][2 * k + 1]))));
+          h[k] = fma2(both(keep), h[k],
+                      add2(bits2(v[0][2 * k], v[0][2 * k + 1]),
+                           add2(bits2(v[1][2 * k], v[1][2 * k + 1]), bits2(v[2][2 * k], v[2][2 * k + 1]))));
       }
       tc_fence_before();
       }

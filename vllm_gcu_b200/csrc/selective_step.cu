@@ -58,12 +58,12 @@ __device__ __forceinline__ float update(float4& h, float2 e0, float2 e1, float2 
   return s.x + s.y;
 }
 
-// Single tokens and short portions, rates per head, where a warp's columns belong to one head (width a multiple of their
-// number) and N is one of 4: a row of N numbers is spread over LPR lanes, NC times four each, and stays in registers while the
-// warp walks the request's tokens, the next one under way.  The state's bytes bound it: a warp has 4 KB of it under way
-// at once, and what a head's columns share is worked out once per warp.  96 requests of 80 heads of 64 x 128: 77 us, 6.5
-// TB/s, the copy's rate (row by row, 70 per cent of the issue slots went into what they share: 113; with the next token's
-// registers, which MANY is for, 91).
+// Single tokens and short portions, rates per head, where a warp's columns belong to one head (width a multiple of
+// their number) and N is one of 4: a row of N numbers is spread over LPR lanes, NC times four each, and stays in
+// registers while the warp walks the request's tokens, the next one under way.  The state's bytes bound it: a warp
+// has 4 KB of it under way at once, and what a head's columns share is worked out once per warp.  96 requests of
+// 80 heads of 64 x 128: 77 us, 6.5 TB/s, the copy's rate (row by row, 70 per cent of the issue slots went into
+// what they share: 113; with the next token's registers, which MANY is for, 91).
 template <typename T, int LPR, int NC, bool MANY, bool WIDE>
 __global__ void __launch_bounds__(128) heads_step_kernel(const ScanArgs a) {
   constexpr int kRows = NC > 1 ? 4 : 8, kGroups = 32 / LPR, kWarpCols = kRows * kGroups, kX = (kWarpCols + 31) / 32;
@@ -166,9 +166,9 @@ __global__ void __launch_bounds__(128) heads_step_kernel(const ScanArgs a) {
   } while (MANY && ++t < po.end);
 }
 
-// One token per request, rates per channel, N a multiple of 4 up to 128: a warp holds 32 / LPR columns of RQ requests, so
-// that rates and skips are fetched and worked out once for them.  64 requests of 8192 channels of 16, bf16: 24 us, 3.0 TB/s; the
-// chain slot - state - sum - row of a warp that lives for a few microseconds bounds it.
+// One token per request, rates per channel, N a multiple of 4 up to 128: a warp holds 32 / LPR columns of RQ
+// requests, so that rates and skips are fetched and worked out once for them.  64 requests of 8192 channels of 16,
+// bf16: 24 us, 3.0 TB/s; the chain slot - state - sum - row of a warp that lives for a few microseconds bounds it.
 template <typename T, int LPR, int RQ, bool WIDE>
 __global__ void __launch_bounds__(128) channels_step_kernel(const ScanArgs a) {
   constexpr int kGroups = 32 / LPR;
