@@ -104,28 +104,25 @@ __device__ __forceinline__ Two shfl(Two v, int from) {
   return {__shfl_sync(0xffffffffu, v.hi, from), __shfl_sync(0xffffffffu, v.lo, from)};
 }
 
-// What a lane needs of the step sizes of tokens 4 lane .. + 3 of a chunk, raw.
-__device__ __forceinline__ void load_steps(const ScanArgs& a, int hd, long long t0, int n, float (&z)[4]) {
+// What a lane needs of the step sizes of tokens 4 lane .. + 3 of a chunk, as it lies in memory: nothing waits for it here.
+__device__ __forceinline__ void load_steps(const ScanArgs& a, int hd, long long t0, int n, uint32_t (&z)[4]) {
   const int lane = threadIdx.x & 31;
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
-    z[k] = 0.0f;
-    if (4 * lane + k < n) {
-      const long long at = (t0 + 4 * lane + k) * a.lddt + hd;
-      z[k] = a.dt_f32 ? static_cast<const float*>(a.dt)[at]
-                      : __bfloat162float(static_cast<const __nv_bfloat16*>(a.dt)[at]);
-    }
+    const long long at = (t0 + min(4 * lane + k, n - 1)) * a.lddt + hd;    // (behind the last token: it again)
+    if (a.dt_f32) z[k] = static_cast<const uint32_t*>(a.dt)[at];
+    else z[k] = static_cast<const unsigned short*>(a.dt)[at];
   }
 }
 // Step sizes and decays of n tokens, four per lane.  rate: -exp(a_log) log2(e).
-__device__ __forceinline__ void chunk_scalars(const ScanArgs& a, int n, float bias, Two rate, const float (&z)[4],
+__device__ __forceinline__ void chunk_scalars(const ScanArgs& a, int n, float bias, Two rate, const uint32_t (&z)[4],
                                               Scalars* s) {
   const int lane = threadIdx.x & 31;
   float dt[4];
   Two L[4], run = {0.0f, 0.0f};
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
-    dt[k] = step_from<__nv_bfloat16>(a, z[k], bias);
+    dt[k] = step_from<__nv_bfloat16>(a, __uint_as_float(a.dt_f32 ? z[k] : z[k] << 16), bias);
     Two la = {dt[k] * rate.hi, 0.0f};
     la.lo = fmaf(dt[k], rate.hi, -la.hi) + dt[k] * rate.lo;
     if (la.hi < -160.0f) la = {-160.0f, 0.0f};          // 2^-160 is 0 in fp32; sums stay exact to 2^-33
@@ -587,13 +584,13 @@ heads_kernel(const ScanArgs a, const __grid_constant__ CUtensorMap tm_x, const _
     }
   } else {
     // ---------------- step sizes and decays ----------------
-    const float per = -expf(a.a_log[hd]);
-    const Two rate = {per * kLog2e, fmaf(per, kLog2e, -(per * kLog2e)) + per * 1.925963033e-8f};
-    const float bias = a.dt_bias != nullptr ? a.dt_bias[hd] : 0.0f;
     auto rows = [&](int c) { return min(kRows, po.end - po.first - c * kRows); };
-    float z[4], next[4];
+    uint32_t z[4], next[4];
     const int first = warp - kWarps - 2;
     if (first < chunks) load_steps(a, hd, po.first + first * kRows, rows(first), z);
+    const float bias = a.dt_bias != nullptr ? a.dt_bias[hd] : 0.0f;
+    const float per = -expf(a.a_log[hd]);
+    const Two rate = {per * kLog2e, fmaf(per, kLog2e, -(per * kLog2e)) + per * 1.925963033e-8f};
     for (int c = first; c < chunks; c += kScal) {
       if (c + kScal < chunks) load_steps(a, hd, po.first + (c + kScal) * kRows, rows(c + kScal), next);
       if (c >= 4) pass_warp(&bar[kSFree0 + (c & 3)], ((c >> 2) & 1) ^ 1, status, 0x400u, abort_flag);
