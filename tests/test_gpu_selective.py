@@ -512,3 +512,35 @@ def test_many_short_portions(H, P, N, G, dtype):
         S.near(got[:n], want[:n], dtype, _rounding(md, N, mag[:n], dtype))
         assert torch.equal(got[n:], before[n:])
         S.near(kept, new, F32, S.scan_rounding(md, N, smag))
+
+
+@pytest.mark.parametrize("form,H,P,N", [("heads", 2, 64, 128), ("heads", 2, 8, 16), ("channels", 32, 1, 16)])
+def test_steps_of_zero_keep_the_state(form, H, P, N):
+    """Tokens whose step size is 0 leave a state as it is, bit for bit; so do the places behind a portion's end."""
+    from vllm_gcu_b200.ops import cuda as K
+    md = S.step(3, [40, 131, 1], [2, 5, 7, 1, 9, 4])
+    dev = _views(S.scan_case(form, H, P, N, 1, md, F32 if P == 8 else BF16))
+    state, kept = dev["state"].clone(), dev.pop("state")
+    dev["dt"].zero_()
+    K.selective_scan(**{**dev, "dt_bias": None}, groups=1, md=md.to("cuda"), state=kept, softplus=False)
+    assert torch.equal(kept, state)
+
+
+def test_long_memory():
+    """A state that forgets over thousands of tokens: its decays' mean error would add up over 4000 of them."""
+    from vllm_gcu_b200.ops import cuda as K
+    T, D, N = 4000, 16, 16
+    md = S.step(0, [T], [0])
+    g = torch.Generator().manual_seed(5)
+    x, b, c = (torch.randn(T, n, generator=g).abs().to(BF16) for n in (D, N, N))
+    dt = torch.full((T, D), 1.5e-3)
+    a_log = torch.log(torch.linspace(0.2, 1.0, N)).repeat(D, 1)
+    kept = torch.zeros(1, D, N, device="cuda")
+    K.selective_scan(x.cuda(), dt.cuda(), b.cuda(), c.cuda(), a_log.cuda(), 1, md.to("cuda"), kept, softplus=False)
+    want = torch.zeros(D, N, dtype=S.F64)
+    keep = torch.exp(-dt[0, 0].double() * torch.exp(a_log.double()))
+    for t in range(T):
+        want = keep * want + (dt[t].double() * x[t].double())[:, None] * b[t].double()
+    # terms last 1 / (1 - keep) = 670 to 3300 tokens; a decay is off by half a step and less than that on average
+    err = (kept[0].cpu().double() / want - 1).abs()
+    assert err.max() < 3300 * 2.0 ** -25 + 2.0 ** -20, err.max().item()

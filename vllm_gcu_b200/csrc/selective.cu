@@ -337,10 +337,7 @@ __global__ void __launch_bounds__(kCore<LPC> + 2 * kHelp) selective_scan_kernel(
 #pragma unroll
         for (int j = k; j < k + kVec / 2; ++j) {
           to.u[j] = __fmul2_rn(dx, b[j - k]);
-          if (CH) {
-            const float2 p = __fmul2_rn(step, rate[j]);
-            to.e[CH ? j : 0] = make_float2(exp2_fast(p.x), exp2_fast(p.y));
-          }
+          if (CH) to.e[CH ? j : 0] = decays(step, rate[j]);
         }
       }
     };

@@ -235,9 +235,8 @@ __global__ void __launch_bounds__(128) channels_step_kernel(const ScanArgs a) {
 #pragma unroll
   for (int i = 0; i < RQ; ++i) {
     const float step = dt[i], dx = step * x[i];
-    const float2 p0 = __fmul2_rn(make_float2(step, step), make_float2(rate.x, rate.y));
-    const float2 p1 = __fmul2_rn(make_float2(step, step), make_float2(rate.z, rate.w));
-    const float2 e0 = make_float2(exp2_fast(p0.x), exp2_fast(p0.y)), e1 = make_float2(exp2_fast(p1.x), exp2_fast(p1.y));
+    const float2 e0 = decays(make_float2(step, step), make_float2(rate.x, rate.y));
+    const float2 e1 = decays(make_float2(step, step), make_float2(rate.z, rate.w));
     s[i] = update(h[i], e0, e1, make_float2(dx, dx), b[i], c[i]);
     s[i] = in ? s[i] : 0.0f;
     if (in && ws[i] >= 0) *reinterpret_cast<float4*>(a.state + ws[i] * pitch + at) = h[i];

@@ -1639,23 +1639,23 @@ def _step_place(md, T: int, kept: bool, write_slots: Optional[torch.Tensor], dev
     if not 0 <= nd <= T:
         raise ValueError(f"{nd} single tokens in a step of {T} rows")
     if cu is not None:
-        if cu.dim() != 1 or cu.shape[0] < 1 or cu.dtype is not torch.int32 or cu.get_device() != dev \
+        if cu.dim() != 1 or cu.numel() < 1 or cu.dtype is not torch.int32 or cu.get_device() != dev \
                 or not cu.is_contiguous():
             raise ValueError("md.cu_q_prefill: int32 offsets beside x are wanted")
-        n += cu.shape[0] - 1
+        n += cu.numel() - 1
         cu = cu.data_ptr()
     if not kept:
         return nd, n - nd, cu or 0, 0, 0, 0
     pos, slots = md.positions, md.state_slots
     if slots is None:
         raise ValueError("a state needs md.state_slots")
-    if pos.dim() != 1 or pos.shape[0] < T or pos.dtype is not torch.int64 or pos.get_device() != dev \
+    if pos.dim() != 1 or pos.numel() < T or pos.dtype is not torch.int64 or pos.get_device() != dev \
             or not pos.is_contiguous():
         raise ValueError(f"md.positions: {T} int64 positions beside x are wanted")
-    for name, t in (("md.state_slots", slots), ("write_slots", write_slots)):
-        if t is not None and (t.dim() != 1 or t.shape[0] < n or t.dtype is not torch.int32 or t.get_device() != dev
-                              or not t.is_contiguous()):
-            raise ValueError(f"{name}: {n} int32 slots beside x are wanted")
+    for t in (slots,) if write_slots is None or write_slots is slots else (slots, write_slots):
+        if t.dim() != 1 or t.numel() < n or t.dtype is not torch.int32 or t.get_device() != dev \
+                or not t.is_contiguous():
+            raise ValueError(f"{'md.state_slots' if t is slots else 'write_slots'}: {n} int32 slots beside x are wanted")
     slots = slots.data_ptr()
     return nd, n - nd, cu or 0, pos.data_ptr(), slots, slots if write_slots is None else write_slots.data_ptr()
 
@@ -1749,27 +1749,47 @@ def selective_scan(x: torch.Tensor, dt: torch.Tensor, b: torch.Tensor, c: torch.
     if not lo <= hi or abs(lo) > 3e38:
         raise ValueError(f"dt_limits {dt_limits}")
     hi = hi if hi < 3e38 else math.inf
-    _whole("a_log", a_log, (rates, N) if channels else (rates,), f32, dev)
-    own = (dtype,)
-    ldx = _row_view("x", x, T, cols, own, dev)
-    lddt = _row_view("dt", dt, T, rates, (dtype, f32), dev)
-    ldb = _row_view("b", b, T, groups * N, own, dev)
-    ldc = _row_view("c", c, T, groups * N, own, dev)
-    ldz = 0 if z is None else _row_view("z", z, T, cols, own, dev)
-    if d is not None:
-        _whole("d", d, (rates,), f32, dev)
-    if dt_bias is not None:
-        _whole("dt_bias", dt_bias, (rates,), f32, dev)
+    gn, per, dt32 = groups * N, (rates,), dt.dtype is f32
+    # all of it in one expression, for the calls that are right; the ones that are not are told by the checks below
+    if (dt.shape == (T, rates) and (dt32 or dt.dtype is dtype) and dt.get_device() == dev
+            and b.shape == (T, gn) and b.dtype is dtype and b.get_device() == dev
+            and c.shape == (T, gn) and c.dtype is dtype and c.get_device() == dev
+            and (z is None or z.shape == (T, cols) and z.dtype is dtype and z.get_device() == dev)
+            and a_log.shape == ((rates, N) if channels else per) and a_log.dtype is f32 and a_log.is_contiguous()
+            and a_log.get_device() == dev
+            and (d is None or d.shape == per and d.dtype is f32 and d.is_contiguous() and d.get_device() == dev)
+            and (dt_bias is None or dt_bias.shape == per and dt_bias.dtype is f32 and dt_bias.is_contiguous()
+                 and dt_bias.get_device() == dev)):
+        (ldx, sx), (lddt, sdt), (ldb, sb), (ldc, sc) = x.stride(), dt.stride(), b.stride(), c.stride()
+        ldz, sz = (0, 1) if z is None else z.stride()
+        right = sx == sdt == sb == sc == sz == 1
+    else:
+        right = False
+    if not right:
+        own = (dtype,)
+        _whole("a_log", a_log, (rates, N) if channels else per, f32, dev)
+        ldx = _row_view("x", x, T, cols, own, dev)
+        lddt = _row_view("dt", dt, T, rates, (dtype, f32), dev)
+        ldb = _row_view("b", b, T, gn, own, dev)
+        ldc = _row_view("c", c, T, gn, own, dev)
+        ldz = 0 if z is None else _row_view("z", z, T, cols, own, dev)
+        if d is not None:
+            _whole("d", d, per, f32, dev)
+        if dt_bias is not None:
+            _whole("dt_bias", dt_bias, per, f32, dev)
     heads, width = (groups, cols // groups) if channels else (rates, cols // rates)
     slots, ps = 0, 0
     if state is not None:
-        slots, ps = state.shape[0], state.data_ptr()
-        _whole("state", state, (slots, cols, N) if channels else (slots, rates, width, N), f32, dev)
+        shape, ps = state.shape, state.data_ptr()
+        slots = shape[0] if len(shape) else 0
+        if shape != ((slots, cols, N) if channels else (slots, rates, width, N)) or state.dtype is not f32 \
+                or not state.is_contiguous() or state.get_device() != dev:
+            _whole("state", state, (slots, cols, N) if channels else (slots, rates, width, N), f32, dev)
         if ps % 16:
             raise ValueError("state: it does not start on a 16-byte boundary")
     nd, npf, cu, pos, read, write = _step_place(md, T, state is not None, write_slots, dev)
     px, pdt, pb, pc = x.data_ptr(), dt.data_ptr(), b.data_ptr(), c.data_ptr()
-    pz, dt32, es, gn = 0 if z is None else z.data_ptr(), dt.dtype is f32, dtype.itemsize, groups * N
+    pz, es = 0 if z is None else z.data_ptr(), dtype.itemsize
     if out is None:
         out = torch.empty((T, cols), dtype=dtype, device=x.device)
         po, ldo = out.data_ptr(), cols
