@@ -544,3 +544,25 @@ def test_long_memory():
     # terms last 1 / (1 - keep) = 670 to 3300 tokens; a decay is off by half a step and less than that on average
     err = (kept[0].cpu().double() / want - 1).abs()
     assert err.max() < 3300 * 2.0 ** -25 + 2.0 ** -20, err.max().item()
+
+
+@pytest.mark.parametrize("form,H,P,N", [("heads", 2, 64, 128), ("heads", 2, 32, 8), ("channels", 64, 1, 16)])
+def test_rows_that_are_one(form, H, P, N):
+    """Rows of an expanded tensor are all the same memory."""
+    from vllm_gcu_b200.ops import cuda as K
+    md = S.step(2, [150, 3]).to("cuda")
+    dev = _views(S.scan_case(form, H, P, N, 1, md.to("cpu"), BF16))
+    state, T = dev.pop("state"), md.tokens
+    one = dict(dev, **{n: dev[n][:1].contiguous().expand(T, -1) for n in ("x", "b", "c", "dt", "z")})
+    kept, want_kept = state.clone(), state.clone()
+    got = K.selective_scan(**one, groups=1, md=md, state=kept)
+    want = K.selective_scan(**{n: v.contiguous() if torch.is_tensor(v) else v for n, v in one.items()}, groups=1, md=md,
+                            state=want_kept)
+    # (another kernel may take them: each result is half a step of its type off, and states what 32 bits leave of sums)
+    assert (got.float() - want.float()).norm() <= 2.0 ** -8 * want.float().norm()
+    assert (kept - want_kept).norm() <= 2e-6 * want_kept.norm()
+    x = one["x"]
+    w, ones = torch.randn(4, x.shape[1], device="cuda"), torch.ones(x.shape[1], device="cuda")
+    ring = torch.zeros(state.shape[0], 3, x.shape[1], dtype=BF16, device="cuda")
+    assert torch.equal(K.causal_conv(x, w, None, md, ring), K.causal_conv(x.contiguous(), w, None, md, ring.zero_()))
+    assert torch.equal(K.group_norm_gate(x, x, ones, 2, 1e-5), K.group_norm_gate(x.contiguous(), x.contiguous(), ones, 2, 1e-5))

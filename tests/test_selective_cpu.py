@@ -144,3 +144,11 @@ def test_refusals():
         norm(x=buf[:5], z=None, out=buf[1:])
     with pytest.raises(ValueError, match="on a GPU"):
         norm(out=x)                                          # in place is fine
+
+
+def test_too_many_requests():
+    T = 65536
+    md = S.Step(torch.zeros(T, dtype=torch.int64), torch.zeros(T, dtype=torch.int32), T, None, [1] * T, [0] * T)
+    one = torch.zeros(T, 1, dtype=BF16)
+    with pytest.raises(ValueError, match="65536 requests"):
+        C.selective_scan(one, one, one, one, torch.zeros(1), 1, md, None)

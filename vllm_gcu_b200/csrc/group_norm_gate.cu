@@ -240,7 +240,7 @@ B200_API int b200_group_norm_gate(const void* call, void* stream) {
   const NormCall& k = *static_cast<const NormCall*>(call);
   if (k.T <= 0 || k.C <= 0) return 0;
   const long long parts = static_cast<long long>(k.T) * k.groups;
-  if (k.groups <= 0 || k.C % k.groups != 0 || parts > 0x7fffffffll) return -8;
+  if (k.groups <= 0 || k.C % k.groups != 0 || parts > 0x7ffffff0ll) return -8;
   const Args a{k.x, k.z, k.out, k.w, k.bias, k.ldx, k.ldz, k.ldo, k.eps, k.T, k.C, k.groups, k.C / k.groups, k.act,
                k.center, k.after, static_cast<int>(parts)};
   cudaStream_t s = static_cast<cudaStream_t>(stream);

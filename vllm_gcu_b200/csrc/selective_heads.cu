@@ -640,7 +640,10 @@ int launch(const ScanArgs& a, cudaStream_t s) {
 }  // namespace tiles
 
 bool heads_by_tiles(const ScanArgs& a) {
-  return a.wide && a.width % tiles::kP == 0 && (a.N == 64 || a.N == 128) && a.dt_min >= 0.0f;
+  // (rows that share elements, as those of an expanded tensor, have no tensor map)
+  const long long cols = static_cast<long long>(a.heads) * a.width, gn = static_cast<long long>(a.groups) * a.N;
+  const bool apart = a.T == 1 || (a.ldx >= cols && a.ldb >= gn && a.ldc >= gn);
+  return a.wide && apart && a.width % tiles::kP == 0 && (a.N == 64 || a.N == 128) && a.dt_min >= 0.0f;
 }
 int launch_heads_by_tiles(const ScanArgs& a, cudaStream_t s) {
   return a.N == 128 ? tiles::launch<128>(a, s) : tiles::launch<64>(a, s);

@@ -1729,7 +1729,7 @@ def selective_scan(x: torch.Tensor, dt: torch.Tensor, b: torch.Tensor, c: torch.
     D, N]``.  ``b`` and ``c [T, groups * N]``, N up to 256, shared by the heads (channels) of a group.  x, b, c, z
     and out are bf16, fp16 or fp32 alike, dt of that type or fp32, the rest fp32; rows may be strided views.
     State, slots, ``write_slots`` and ``md`` as in :func:`causal_conv`; ``state`` None: zeros in front of the
-    portions, nothing is kept.  Returns ``[T, H * P]`` (``[T, D]``) in x's type."""
+    portions, nothing is kept.  Up to 65535 requests.  Returns ``[T, H * P]`` (``[T, D]``) in x's type."""
     if x.dim() != 2 or x.dtype not in DTYPE_CODE:
         raise ValueError(f"x: rows of bf16, fp16 or fp32 are wanted, got {x.dtype} of shape {tuple(x.shape)}")
     T, cols = x.shape
@@ -1788,6 +1788,8 @@ def selective_scan(x: torch.Tensor, dt: torch.Tensor, b: torch.Tensor, c: torch.
         if ps % 16:
             raise ValueError("state: it does not start on a 16-byte boundary")
     nd, npf, cu, pos, read, write = _step_place(md, T, state is not None, write_slots, dev)
+    if nd + npf > 65535:
+        raise ValueError(f"{nd + npf} requests in a step, up to 65535 are built")
     px, pdt, pb, pc = x.data_ptr(), dt.data_ptr(), b.data_ptr(), c.data_ptr()
     pz, es = 0 if z is None else z.data_ptr(), dtype.itemsize
     if out is None:
