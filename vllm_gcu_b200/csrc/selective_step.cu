@@ -31,6 +31,12 @@ struct RowSums {
     for (int i = 0; i < kLeft; ++i) v[i] = s[i];
   }
   __device__ __forceinline__ static bool keeps(int l) { return l % (LPR / kParted) == 0; }
+  // row i's number, where each lane has those of the rows whose sums it is left with
+  template <typename V>
+  __device__ __forceinline__ static V of(const V (&own)[kLeft], int i) {
+    if constexpr (kParted == 1) return own[i];
+    else return __shfl_sync(0xffffffffu, own[i % kLeft], i / kLeft * (LPR / kParted), LPR);
+  }
 };
 
 // Four neighbours of a row of B or C.
@@ -167,11 +173,15 @@ __global__ void __launch_bounds__(128) heads_step_kernel(const ScanArgs a) {
 }
 
 // One token per request, rates per channel, N a multiple of 4 up to 128: a warp holds 32 / LPR columns of RQ
-// requests, so that rates and skips are fetched and worked out once for them.  64 requests of 8192 channels of 16,
-// bf16: 24 us, 3.0 TB/s; the chain slot - state - sum - row of a warp that lives for a few microseconds bounds it.
+// requests, so that rates and skips are fetched and worked out once for them; what is one number per column and request
+// (slots, step sizes, x, gates) is one lane's, the one that RowSums leaves that request's sum in, and goes round from there.
+// 64 requests of 8192 channels of 16, bf16: 16.5 us, 4.3 TB/s (23.4 with all of them in every lane: issue slots);
+// the chain slot - state - sum - row of a warp that lives for a few microseconds bounds it.
 template <typename T, int LPR, int RQ, bool WIDE>
 __global__ void __launch_bounds__(128) channels_step_kernel(const ScanArgs a) {
   constexpr int kGroups = 32 / LPR;
+  using Sums = RowSums<RQ, LPR>;
+  constexpr int kOwn = Sums::kLeft, kApart = LPR / Sums::kParted;    // requests of a lane, lanes of the same ones
   grid_release_small();
   grid_wait();
   const int lane = threadIdx.x & 31, l = lane & (LPR - 1), grp = lane / LPR;
@@ -181,30 +191,41 @@ __global__ void __launch_bounds__(128) channels_step_kernel(const ScanArgs a) {
   const bool in = c0 + grp < cols && l * 4 < a.N, mine = c0 + grp < cols;
   const int col = min(c0 + grp, cols - 1), n = l * 4;
   const int g = col / (cols / a.groups);
-  const int r0 = blockIdx.y * RQ;
+  const int r0 = blockIdx.y * RQ, own = r0 + l / kApart * kOwn;
+  constexpr int kPadding = -2, kNone = -1;
   const long long pitch = static_cast<long long>(cols) * a.N, at = static_cast<long long>(col) * a.N + n;
   float4 h[RQ], b[RQ], c[RQ];
-  float x[RQ], dt[RQ], z[RQ];
-  int ws[RQ];
-  bool padding[RQ];
+  int from[kOwn], to[kOwn];                      // slots
 #pragma unroll
-  for (int i = 0; i < RQ; ++i) {
-    const int r = min(r0 + i, a.nd - 1);
-    const int slot = a.state != nullptr ? a.slots[r] : 0;
-    ws[i] = a.state != nullptr && r0 + i < a.nd ? a.wslots[r] : -1;
-    padding[i] = a.state != nullptr && (slot < 0 || slot >= a.num_slots);
-    if (padding[i] || ws[i] >= a.num_slots) ws[i] = -1;
-    h[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    if (a.state != nullptr && !padding[i] && in && a.positions[r] != 0)
-      h[i] = *reinterpret_cast<const float4*>(a.state + slot * pitch + at);
+  for (int m = 0; m < kOwn; ++m) {
+    const int r = min(own + m, a.nd - 1);        // (behind the last request: its row again, and nothing is kept)
+    from[m] = to[m] = kNone;
+    if (a.state != nullptr) {
+      const int slot = a.slots[r], ws = a.wslots[r];
+      const long long pos = a.positions[r];
+      const bool there = slot >= 0 && slot < a.num_slots;
+      from[m] = !there ? kPadding : pos != 0 ? slot : kNone;
+      if (there && ws >= 0 && ws < a.num_slots && own + m < a.nd) to[m] = ws;
+    }
   }
 #pragma unroll
   for (int i = 0; i < RQ; ++i) {
-    const int r = min(r0 + i, a.nd - 1);         // (behind the last request: its row again, and nothing is kept)
-    x[i] = to_f32<T>(static_cast<const T*>(a.x)[r * a.ldx + col]);
-    dt[i] = a.dt_f32 ? static_cast<const float*>(a.dt)[r * a.lddt + col]
+    const int slot = Sums::of(from, i);
+    h[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    if (slot >= 0 && in) h[i] = *reinterpret_cast<const float4*>(a.state + slot * pitch + at);
+  }
+  float x[kOwn], dt[kOwn], z[kOwn], dx[kOwn];
+#pragma unroll
+  for (int m = 0; m < kOwn; ++m) {
+    const int r = min(own + m, a.nd - 1);
+    x[m] = to_f32<T>(static_cast<const T*>(a.x)[r * a.ldx + col]);
+    dt[m] = a.dt_f32 ? static_cast<const float*>(a.dt)[r * a.lddt + col]
                      : to_f32<T>(static_cast<const T*>(a.dt)[r * a.lddt + col]);
-    z[i] = a.z != nullptr ? to_f32<T>(static_cast<const T*>(a.z)[r * a.ldz + col]) : 0.0f;
+    z[m] = a.z != nullptr ? to_f32<T>(static_cast<const T*>(a.z)[r * a.ldz + col]) : 0.0f;
+  }
+#pragma unroll
+  for (int i = 0; i < RQ; ++i) {
+    const int r = min(r0 + i, a.nd - 1);
     b[i] = load_four<T, WIDE>(static_cast<const T*>(a.b) + r * a.ldb + g * a.N + n, in);
     c[i] = load_four<T, WIDE>(static_cast<const T*>(a.c) + r * a.ldc + g * a.N + n, in);
   }
@@ -213,51 +234,29 @@ __global__ void __launch_bounds__(128) channels_step_kernel(const ScanArgs a) {
   rate = make_float4(-expf(rate.x) * kLog2e, -expf(rate.y) * kLog2e, -expf(rate.z) * kLog2e, -expf(rate.w) * kLog2e);
   const float bias = a.dt_bias != nullptr ? a.dt_bias[col] : 0.0f, skip = a.d != nullptr ? a.d[col] : 0.0f;
 #pragma unroll
-  for (int i = 0; i < RQ; ++i) dt[i] += bias;
-  if (a.softplus) {
-#pragma unroll
-    for (int i = 0; i < RQ; i += 2) {
-      if constexpr (sizeof(T) == 2) {
-        const float2 p = softplus_pair(make_float2(dt[i], dt[i + 1 < RQ ? i + 1 : i]));
-        dt[i] = p.x;
-        if (i + 1 < RQ) dt[i + 1 < RQ ? i + 1 : i] = p.y;
-      } else {
-        dt[i] = softplus<T>(dt[i]);
-        if (i + 1 < RQ) dt[i + 1 < RQ ? i + 1 : i] = softplus<T>(dt[i + 1 < RQ ? i + 1 : i]);
-      }
-    }
-  }
-  if (a.limits) {
-#pragma unroll
-    for (int i = 0; i < RQ; ++i) dt[i] = limited(a, dt[i]);
+  for (int m = 0; m < kOwn; ++m) {
+    dt[m] = step_from<T>(a, dt[m], bias);
+    dx[m] = dt[m] * x[m];
   }
   float s[RQ];
 #pragma unroll
   for (int i = 0; i < RQ; ++i) {
-    const float step = dt[i], dx = step * x[i];
+    const float step = Sums::of(dt, i), add = Sums::of(dx, i);
+    const int ws = Sums::of(to, i);
     const float2 e0 = decays(make_float2(step, step), make_float2(rate.x, rate.y));
     const float2 e1 = decays(make_float2(step, step), make_float2(rate.z, rate.w));
-    s[i] = update(h[i], e0, e1, make_float2(dx, dx), b[i], c[i]);
+    s[i] = update(h[i], e0, e1, make_float2(add, add), b[i], c[i]);
     s[i] = in ? s[i] : 0.0f;
-    if (in && ws[i] >= 0) *reinterpret_cast<float4*>(a.state + ws[i] * pitch + at) = h[i];
+    if (in && ws >= 0) *reinterpret_cast<float4*>(a.state + ws * pitch + at) = h[i];
   }
-  const RowSums<RQ, LPR> sums(s, l);
+  const Sums sums(s, l);
 #pragma unroll
-  for (int i = 0; i < sums.kLeft; ++i) {
-    const int k = sums.first + i, r = r0 + k;
+  for (int m = 0; m < kOwn; ++m) {
+    const int r = own + m;
     if (!mine || !sums.keeps(l) || r >= a.nd) continue;
-    float xv = 0.0f, zv = 0.0f;
-    bool none = false;
-#pragma unroll
-    for (int m = 0; m < RQ; ++m)
-      if (m == k) {
-        xv = x[m];
-        zv = z[m];
-        none = padding[m];
-      }
-    float y = fmaf(skip, xv, sums.v[i]);
-    if (a.z != nullptr) y *= silu<T>(zv);
-    static_cast<T*>(a.out)[r * a.ldo + col] = from_f32<T>(none ? 0.0f : y);
+    float y = fmaf(skip, x[m], sums.v[m]);
+    if (a.z != nullptr) y *= silu<T>(z[m]);
+    static_cast<T*>(a.out)[r * a.ldo + col] = from_f32<T>(from[m] == kPadding ? 0.0f : y);
   }
 }
 
