@@ -1053,7 +1053,7 @@ def selective_scan(x, dt, b, c, a_log, groups, md, state, d=None, dt_bias=None, 
     P, N = x.shape[1] // rates, b.shape[1] // groups
     out = torch.zeros_like(x, memory_format=torch.contiguous_format) if out is None else out
     step = dt.float() if dt_bias is None else dt.float() + dt_bias
-    step = (torch.nn.functional.softplus(step, threshold=1e9) if softplus else step).clamp(*dt_limits)
+    step = (torch.logaddexp(step, torch.zeros_like(step)) if softplus else step).clamp(*dt_limits)   # log(1 + e^step)
     A = -torch.exp(a_log.float()).view(rates, -1)
     xf = x.float().view(T, rates, P) if x.is_contiguous() else x.float().reshape(T, rates, P)
     kept = None if state is None else state.clone().view(-1, rates, P, N)
