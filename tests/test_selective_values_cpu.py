@@ -21,3 +21,14 @@ def test_large_and_small_step_sizes(form, H, P, N, G):
     got = ref.selective_scan(**k, groups=G, md=md, state=kept)
     S.near(got, want, F32, S.scan_rounding(md, N, mag))
     S.near(kept, new, F32, S.scan_rounding(md, N, smag))
+
+
+@pytest.mark.parametrize("form,H,P,N", [("heads", 2, 3, 4), ("channels", 6, 1, 3)])
+def test_a_state_without_slots(form, H, P, N):
+    md = S.step(2, [3])
+    k = S.scan_case(form, H, P, N, 1, md, F32)
+    k.pop("row")
+    state = k.pop("state")[:0]
+    assert (ref.selective_scan(**k, groups=1, md=md, state=state) == 0).all()
+    x, w, bias, ring = S.conv_case(6, 4, md, F32)
+    assert (ref.causal_conv(x, w, bias, md, ring[:0]) == 0).all()

@@ -1701,7 +1701,10 @@ def causal_conv(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tens
         if taps == 1:
             ring = None
     nd, npf, cu, pos, read, write = _step_place(md, T, ring is not None, write_slots, dev)
-    px, pw, pr, es = x.data_ptr(), weight.data_ptr(), 0 if ring is None else ring.data_ptr(), dtype.itemsize
+    px, pw, es = x.data_ptr(), weight.data_ptr(), dtype.itemsize
+    # (a ring without slots has no address, which would say that there is no ring: another one stands in, where nothing
+    # is read)
+    pr = 0 if ring is None else ring.data_ptr() if slots else pw
     if out is None:
         out = torch.empty((T, Ch), dtype=dtype, device=x.device)
         po, ldo = out.data_ptr(), Ch
@@ -1787,6 +1790,8 @@ def selective_scan(x: torch.Tensor, dt: torch.Tensor, b: torch.Tensor, c: torch.
             _whole("state", state, (slots, cols, N) if channels else (slots, rates, width, N), f32, dev)
         if ps % 16:
             raise ValueError("state: it does not start on a 16-byte boundary")
+        if not slots:                          # no address either; see causal_conv
+            ps = a_log.data_ptr()
     nd, npf, cu, pos, read, write = _step_place(md, T, state is not None, write_slots, dev)
     if nd + npf > 65535:
         raise ValueError(f"{nd + npf} requests in a step, up to 65535 are built")
