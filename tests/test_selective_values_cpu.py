@@ -3,7 +3,7 @@ import pytest
 import torch
 
 import selective_cases as S
-from vllm_gcu_b200.ops import ref
+from vllm_gcu_b200.ops import cuda as C, ref
 
 F32 = torch.float32
 
@@ -32,3 +32,35 @@ def test_a_state_without_slots(form, H, P, N):
     assert (ref.selective_scan(**k, groups=1, md=md, state=state) == 0).all()
     x, w, bias, ring = S.conv_case(6, 4, md, F32)
     assert (ref.causal_conv(x, w, bias, md, ring[:0]) == 0).all()
+
+
+def test_results_do_not_go_into_what_is_kept():
+    """Rows of results that meet the ring or the state, which other requests read at the same time, are refused; a state
+    between two rows of results is none of theirs."""
+    md = S.step(1, [3])
+    T = md.tokens
+    x, w, bias, _ = S.conv_case(8, 4, md, F32)
+    buf = torch.zeros(64 * 8)
+    ring = buf[:6 * 3 * 8].view(6, 3, 8)
+    conv = lambda out: C.causal_conv(x, w, bias, md, ring, out=out)  # noqa: E731
+    last = buf[17 * 8 + 7:]
+    for out in (buf[:T * 8].view(T, 8), last[:T * 8].view(T, 8), buf.as_strided((T, 8), (17 * 8, 1), 40)):
+        with pytest.raises(ValueError, match="shares memory with ring"):
+            conv(out)
+    k = S.scan_case("heads", 2, 4, 4, 1, md, F32)
+    k.pop("row"), k.pop("state")
+    mem = torch.zeros(4096)
+    state = mem[1000:1000 + 4 * 32].view(4, 2, 4, 4)
+    scan = lambda out: C.selective_scan(**k, groups=1, md=md, state=state, out=out)  # noqa: E731
+    for first, pitch in ((1000, 8), (993, 900), (0, 1000), (1127, 500), (500, 300)):
+        with pytest.raises(ValueError, match="shares memory with state"):
+            scan(mem.as_strided((T, 8), (pitch, 1), first))
+    for first, pitch in ((992, 1128 - 992), (1128, 8), (968, 8), (0, 800)):
+        with pytest.raises(ValueError, match="on a GPU"):
+            scan(mem.as_strided((T, 8), (pitch, 1), first))
+    # every place of four rows beside a block, against the elements themselves
+    for pitch in (8, 11, 30):
+        for lo in range(0, 140, 3):
+            for size in (1, 5, 40):
+                rows = {i * pitch + j + 20 for i in range(4) for j in range(8)}
+                assert C._rows_meet(20, pitch, 4, 8, lo, size) == bool(rows & set(range(lo, lo + size)))

@@ -1615,10 +1615,17 @@ def _overlap(a: tuple, b: tuple) -> bool:
     return True
 
 
-def _target(out: torch.Tensor, rows: int, cols: int, dtype, dev: int, inputs, same_is_fine: bool = False
-            ) -> tuple[int, int]:
+def _rows_meet(at: int, pitch: int, rows: int, width: int, lo: int, size: int) -> bool:
+    """Whether rows of ``width`` bytes, ``pitch`` bytes apart, share any with the ``size`` bytes at ``lo``."""
+    first = 0 if lo < at + width else (lo - at - width) // max(pitch, 1) + 1      # the first row that ends behind lo
+    return first < rows and at + first * pitch < lo + size
+
+
+def _target(out: torch.Tensor, rows: int, cols: int, dtype, dev: int, inputs, same_is_fine: bool = False,
+            kept: Optional[torch.Tensor] = None, kept_name: str = "") -> tuple[int, int]:
     """Checks the rows that a kernel writes: no two of them share elements, and none of them meets an input
-    (``inputs``: name, address or 0, row pitch, columns, element size); their address and pitch."""
+    (``inputs``: name, address or 0, row pitch, columns, element size) or what is kept between calls; their address and
+    pitch."""
     ld, at, es = _row_view("out", out, rows, cols, (dtype,), dev), out.data_ptr(), dtype.itemsize
     if rows > 1 and ld < cols:
         raise ValueError(f"out: rows of {cols} columns are {ld} elements apart")
@@ -1629,6 +1636,8 @@ def _target(out: torch.Tensor, rows: int, cols: int, dtype, dev: int, inputs, sa
             continue
         if _overlap((at, ld, rows, cols, es), (p, pitch, rows, width, size)):
             raise ValueError(f"out shares memory with {name}" + (f" and is not {name}" if same_is_fine else ""))
+    if kept is not None and _rows_meet(at, ld * es, rows, cols * es, kept.data_ptr(), kept.numel() * kept.itemsize):
+        raise ValueError(f"out shares memory with {kept_name}")
     return at, ld
 
 
@@ -1709,7 +1718,7 @@ def causal_conv(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tens
         out = torch.empty((T, Ch), dtype=dtype, device=x.device)
         po, ldo = out.data_ptr(), Ch
     else:
-        po, ldo = _target(out, T, Ch, dtype, dev, (("x", px, ldx, Ch, es),))
+        po, ldo = _target(out, T, Ch, dtype, dev, (("x", px, ldx, Ch, es),), kept=ring, kept_name="ring")
     pb = 0 if bias is None else bias.data_ptr()
     wide = Ch % 4 == 0 and (px | pw | pb | pr | po) % 16 == 0 and (T == 1 or (ldx | ldo) % 4 == 0)
     _call_on(dev, "b200_causal_conv",
@@ -1803,7 +1812,8 @@ def selective_scan(x: torch.Tensor, dt: torch.Tensor, b: torch.Tensor, c: torch.
     else:
         po, ldo = _target(out, T, cols, dtype, dev,
                           (("x", px, ldx, cols, es), ("dt", pdt, lddt, rates, 4 if dt32 else es),
-                           ("b", pb, ldb, gn, es), ("c", pc, ldc, gn, es), ("z", pz, ldz, cols, es)))
+                           ("b", pb, ldb, gn, es), ("c", pc, ldc, gn, es), ("z", pz, ldz, cols, es)), kept=state,
+                          kept_name="state")
     wide = (px | pb | pc | po | pz) % 16 == 0 and (T == 1 or (ldx | ldb | ldc | ldz | ldo) * es % 16 == 0)
     _call_on(dev, "b200_selective_scan",
              _SCAN_CALL.pack(px, pdt, pb, pc, pz, po, a_log.data_ptr(), 0 if d is None else d.data_ptr(),
