@@ -5,7 +5,7 @@ import torch
 import selective_cases as S
 
 pytestmark = pytest.mark.gpu
-F32, BF16 = torch.float32, torch.bfloat16
+F32, BF16, F16 = torch.float32, torch.bfloat16, torch.float16
 
 
 def _on_gpu(k):
@@ -30,3 +30,21 @@ def test_a_state_without_slots(form, H, P, N, decodes, lens, dtype):
     ring = torch.empty(0, 3, H * P, dtype=dtype, device="cuda")
     got = K.causal_conv(dev["x"], torch.randn(4, H * P, device="cuda"), torch.ones(H * P, device="cuda"), md.to("cuda"), ring)
     assert got.shape == (md.tokens, H * P) and (got == 0).all()
+
+
+@pytest.mark.parametrize("dtype,H,P,N", [(F32, 4, 64, 128), (F16, 16, 64, 128), (BF16, 4, 64, 16), (BF16, 8, 32, 64)])
+@pytest.mark.parametrize("many", [3, 9, 15])
+def test_a_long_portion_beside_short_ones(many, dtype, H, P, N):
+    """A portion that is long beside those of one token takes the way that it takes alone, where many tokens are not one
+    slow walk: the same bits.  (The walk for short portions sums in another order.)"""
+    from vllm_gcu_b200.ops import cuda as K
+    long = 30 * many
+    md = S.step(0, [long] + [1] * many, [5] * (many + 1), slots=list(range(many + 1)))
+    k = S.scan_case("heads", H, P, N, 1, md, dtype)
+    dev = _on_gpu(k)
+    state = dev.pop("state")
+    both, alone = state.clone(), state.clone()
+    got = K.selective_scan(**dev, groups=1, md=md.to("cuda"), state=both)
+    cut = {n: v[:long] if n in ("x", "b", "c", "dt", "z") else v for n, v in dev.items()}
+    want = K.selective_scan(**cut, groups=1, md=S.step(0, [long], [5], slots=[0]).to("cuda"), state=alone)
+    assert torch.equal(got[:long], want) and torch.equal(both[0], alone[0])

@@ -1,4 +1,6 @@
 // Selective scan of single tokens (sm_100a), one per request: see selective.cu for the formulas and the state's layout.
+#include <algorithm>
+
 #include "selective.cuh"
 
 namespace b200 {
@@ -441,18 +443,41 @@ int launch_step(const ScanArgs& a, cudaStream_t s) {
 #undef STEP
 }
 
-// Portions of a dozen tokens on average, whose state's way in and out is most of the work.  us by this kernel and by tiles,
-// 96 requests of 80 heads of 64 x 128: 95 and 404 for 1 token each, 246 and 418 for 8, 440 and 422 for 16; token after
-// token in 16 bits, 12 requests of 16 heads: 18 and 27 for 8, 32 and 39 for 32, 60 and 60 for 64.  Only the mean length is
-// known here.  A token of a portion takes 0.55 us, so the rows of a step are kept to what the tiles would take twice
-// as long for were they all one portion's (8 us for a CTA per SM), or, for other types, to 512.
+// Steps whose portions are short, whose state's way in and out is most of the work.  Only the mean length is known here,
+// and one portion may hold nearly all of the rows.
+//
+// Where the others would go by tiles: us by this kernel and by tiles, 96 requests of 80 heads of 64 x 128: 95 and 404 for
+// 1 token each, 246 and 418 for 8, 440 and 422 for 16.  A token of a portion takes 0.55 us, so the rows of a step are kept
+// to what the tiles would take twice as long for were they all one portion's (8 us for a CTA per SM).
+//
+// Where they would go token after token (selective.cu), us by this kernel and by that one, 16 heads of 64 x 128 in 16 bits:
+// even portions, 48 of 8 tokens 25 and 90, 12 of 32 31 and 38, 1 of 16 11 and 5; one long portion beside others of one
+// token, 300 and nine 184 and 57, 30 and one 20 and 7.  Both are estimated, for an even step and for one whose rows are
+// all one portion's, from times of 2 to 80 heads of 32 to 128 columns with 16 to 256 numbers: this kernel 0.55 us a token (32
+// bits: 0.45) and no faster than the states' arithmetic, the other one its start per CTA and SM and then its tokens.
+// An even step (drafted tokens that are verified) counts double.  What the rule costs at the most: 12 portions of 4
+// tokens, 16 heads of 64 x 16, 8 us where a walk takes 4; 300 and nine, 32 heads of 64 x 64, 184 where the other takes 66.
+bool worth_a_walk(const ScanArgs& a, int dtype, long long rows) {
+  const int per = a.heads / a.groups * a.width, cta_cols = a.N <= 32 ? 32 : 16;
+  const double ctas = static_cast<double>(a.groups) * ((per + cta_cols - 1) / cta_cols), sms = sm_count();
+  const double rounds = ctas * a.np / sms;
+  const double start = std::max(rounds, 1.0) * (a.N <= 16 ? 2.1 : a.N <= 128 ? 4.2 : 6.5);
+  const double alone = a.N <= 16 ? 0.05 : 0.12;
+  const double shared = ctas * (a.N <= 64 ? 0.0008 : a.N <= 128 ? 0.0011 : 0.0018);
+  const double arithmetic = 5.2e-7 * rows * a.heads * a.width * a.N;
+  auto walk = [&](double n) { return std::max(2 + (dtype == 2 ? 0.45 : 0.55) * n, arithmetic); };
+  auto other = [&](double n) { return start + std::max(alone, shared) * n; };
+  const double mean = static_cast<double>(rows) / a.np;
+  return walk(mean) * walk(rows) <= 2 * other(mean) * other(rows);
+}
+
 bool launch_short_portions(const ScanArgs& a, int dtype, cudaStream_t s, int* rc) {
   const long long rows = a.T - a.nd;
   if (a.np == 0) return false;
   if (dtype == 0 && heads_by_tiles(a)) {
     const long long ctas = static_cast<long long>(a.np) * a.heads * (a.width / 64), sms = sm_count();
     if (rows > 12ll * a.np || rows > 28 * ((ctas + sms - 1) / sms)) return false;
-  } else if (rows > 32ll * a.np || rows > 512) {
+  } else if (rows > 32ll * a.np || rows > 512 || !worth_a_walk(a, dtype, rows)) {
     return false;
   }
   *rc = dtype == 0   ? launch_heads<__nv_bfloat16, true>(a, s)
