@@ -3,6 +3,7 @@ import pytest
 import torch
 
 import selective_cases as S
+import selective_states as E
 from vllm_gcu_b200.ops import cuda as C, ref
 
 F32 = torch.float32
@@ -64,3 +65,27 @@ def test_results_do_not_go_into_what_is_kept():
             for size in (1, 5, 40):
                 rows = {i * pitch + j + 20 for i in range(4) for j in range(8)}
                 assert C._rows_meet(20, pitch, 4, 8, lo, size) == bool(rows & set(range(lo, lo + size)))
+
+
+@pytest.mark.parametrize("kind", ["signs", "strong"])
+@pytest.mark.parametrize("N", [64, 128])
+@pytest.mark.parametrize("lens", [[128], [129, 127], [400]])
+def test_bounds_of_states_tell_mistakes(lens, N, kind):
+    """What the GPU tests ask of states by products of tiles holds for weighted x in three parts of bf16 and sums in two
+    floats, not for two parts, and behind strong decays not for sums in one float."""
+    k = E.heads_case(N, lens, kind)
+    k.pop("row"), k.pop("c")
+    starts = [5] * len(lens)
+    args = dict(x=k["x"], dt=k["dt"], b=k["b"], a_log=k["a_log"], lens=lens, starts=starts, state=k["state"])
+    want, off = E.states(**args, groups=1)
+    bound = E.chunk_bound(lens)
+    whole = E.by_chunks(**args)
+    assert E.norm_error(whole, want) < bound / 4
+    assert E.norm_error(E.by_chunks(**args, parts=2), want) > 1.5 * bound
+    if kind == "strong":
+        assert E.norm_error(E.by_chunks(**args, two_floats=False), want) > 50 * bound
+    # and the torch formulation holds the bounds of each number
+    md = S.step(0, lens, starts, slots=list(range(len(lens))))
+    kept = k["state"].clone()
+    ref.selective_scan(**{n: k[n] for n in ("x", "dt", "b", "a_log")}, c=k["b"], groups=1, md=md, state=kept, softplus=False)
+    assert ((kept.to(E.F64) - want).abs() <= off).all()
