@@ -1,4 +1,6 @@
 """State-space operators at the ends of what their launchers allow."""
+import math
+
 import pytest
 import torch
 
@@ -48,3 +50,37 @@ def test_a_long_portion_beside_short_ones(many, dtype, H, P, N):
     cut = {n: v[:long] if n in ("x", "b", "c", "dt", "z") else v for n, v in dev.items()}
     want = K.selective_scan(**cut, groups=1, md=S.step(0, [long], [5], slots=[0]).to("cuda"), state=alone)
     assert torch.equal(got[:long], want) and torch.equal(both[0], alone[0])
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("form,H,P,N", [("heads", 2, 64, 64), ("channels", 40, 1, 16)])
+@pytest.mark.parametrize("limits,softplus", [((-math.inf, math.inf), False), ((-1e300, 0.05), False), ((-0.01, 1e300), False),
+                                             ((-math.inf, math.inf), True), ((-3.0, 0.2), True), ((-3.0, -0.01), True)])
+def test_limits_of_step_sizes(limits, softplus, form, H, P, N, dtype):
+    """Limits that limit nothing, on either side, and those below 0, as single tokens and portions take them."""
+    from vllm_gcu_b200.ops import cuda as K
+    md = S.step(2, [30, 150], [3, 0, 4, 0])
+    k = S.scan_case(form, H, P, N, 1, md, dtype)
+    k["a_log"] = torch.full_like(k["a_log"], -1.0)
+    if not softplus:
+        k["dt"], k["dt_bias"] = (0.02 * k["dt"].float()).to(dtype), None
+    state, dev = k["state"], _on_gpu({n: v for n, v in k.items() if v is not None})
+    dev.setdefault("dt_bias", None)
+    more = dict(softplus=softplus, dt_limits=limits)
+    want, mag, new, smag = S.scan(**{n: v for n, v in k.items() if n not in ("row", "state")}, groups=1, md=md, state=state,
+                                  **more)
+    kept = dev.pop("state")
+    got = K.selective_scan(**dev, groups=1, md=md.to("cuda"), state=kept, **more)
+    S.near(got, want, dtype, S.scan_rounding(md, N, mag) + (mag * (2.0 ** -15 + 4e-6) if dtype != F32 else 0))
+    S.near(kept, new, F32, S.scan_rounding(md, N, smag))
+
+
+@pytest.mark.parametrize("N", [64, 128])
+def test_limits_below_zero_leave_softplus_its_way(N):
+    """A softplus is not below 0, so a limit below 0 changes nothing: the same bits."""
+    from vllm_gcu_b200.ops import cuda as K
+    md = S.step(0, [200], [0]).to("cuda")
+    dev = _on_gpu(S.scan_case("heads", 2, 64, N, 1, md, BF16))
+    state = dev.pop("state")
+    a, b = (K.selective_scan(**dev, groups=1, md=md, state=state.clone(), dt_limits=(lo, math.inf)) for lo in (0.0, -1.0))
+    assert torch.equal(a, b)

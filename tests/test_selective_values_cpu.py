@@ -1,4 +1,6 @@
 """State-space operators of the torch formulation at the ends of their inputs' ranges."""
+import math
+
 import pytest
 import torch
 
@@ -89,3 +91,14 @@ def test_bounds_of_states_tell_mistakes(lens, N, kind):
     kept = k["state"].clone()
     ref.selective_scan(**{n: k[n] for n in ("x", "dt", "b", "a_log")}, c=k["b"], groups=1, md=md, state=kept, softplus=False)
     assert ((kept.to(E.F64) - want).abs() <= off).all()
+
+
+def test_limits_of_step_sizes():
+    md = S.step(0, [3])
+    k = S.scan_case("heads", 2, 3, 4, 1, md, F32)
+    k.pop("row")
+    for limits, says in [((-math.inf, math.inf), "on a GPU"), ((-1e300, 0.5), "on a GPU"), ((0.0, 1e300), "on a GPU"),
+                         ((math.inf, math.inf), "dt_limits"), ((-math.inf, -math.inf), "dt_limits"),
+                         ((math.nan, 1.0), "dt_limits"), ((0.0, math.nan), "dt_limits"), ((1.0, 0.0), "dt_limits")]:
+        with pytest.raises(ValueError, match=says):
+            C.selective_scan(**k, groups=1, md=md, softplus=False, dt_limits=limits)

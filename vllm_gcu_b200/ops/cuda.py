@@ -1758,9 +1758,11 @@ def selective_scan(x: torch.Tensor, dt: torch.Tensor, b: torch.Tensor, c: torch.
     if not 1 <= N <= 256:
         raise ValueError(f"a state of {N} numbers per column, 1 to 256 are built")
     lo, hi = dt_limits
-    if not lo <= hi or abs(lo) > 3e38:
+    if not lo <= hi or lo > 3e38 or hi < -3e38:
         raise ValueError(f"dt_limits {dt_limits}")
-    hi = hi if hi < 3e38 else math.inf
+    lo, hi = lo if lo > -3e38 else -math.inf, hi if hi < 3e38 else math.inf
+    if softplus and lo < 0 <= hi:              # a softplus is not below 0
+        lo = 0.0
     gn, per, dt32 = groups * N, (rates,), dt.dtype is f32
     # all of it in one expression, for the calls that are right; the ones that are not are told by the checks below
     if (dt.shape == (T, rates) and (dt32 or dt.dtype is dtype) and dt.get_device() == dev
