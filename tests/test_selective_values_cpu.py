@@ -102,3 +102,24 @@ def test_limits_of_step_sizes():
                          ((math.nan, 1.0), "dt_limits"), ((0.0, math.nan), "dt_limits"), ((1.0, 0.0), "dt_limits")]:
         with pytest.raises(ValueError, match=says):
             C.selective_scan(**k, groups=1, md=md, softplus=False, dt_limits=limits)
+
+
+def test_arguments_without_dimensions_or_positions():
+    md = S.step(1, [3])
+    x, w, bias, ring = S.conv_case(8, 4, md, F32)
+    conv = lambda **k: C.causal_conv(**{**dict(x=x, weight=w, bias=bias, md=md, ring=ring), **k})  # noqa: E731
+    one = torch.tensor(1.0)
+    none = S.dataclasses.replace(md, positions=None)
+    for k, says in [(dict(weight=one), "0 taps"), (dict(ring=one), "ring"), (dict(bias=one), "bias"), (dict(x=one), "x:"),
+                    (dict(md=none), "positions"), (dict(out=one), "out")]:
+        with pytest.raises(ValueError, match=says):
+            conv(**k)
+    k = S.scan_case("heads", 2, 3, 4, 1, md, F32)
+    k.pop("row")
+    for more, says in [({n: one}, n) for n in ("x", "dt", "b", "c", "a_log", "d", "dt_bias", "z", "state")] + \
+            [(dict(md=none), "positions")]:
+        with pytest.raises(ValueError, match=says):
+            C.selective_scan(**{**k, **dict(groups=1, md=md), **more})
+    for more, says in [({n: one}, n) for n in ("x", "z", "weight", "bias")]:
+        with pytest.raises(ValueError, match=says):
+            C.group_norm_gate(**{**dict(x=x, z=x, weight=torch.ones(8), groups=2, eps=1e-5), **more})

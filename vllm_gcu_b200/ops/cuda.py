@@ -1656,8 +1656,8 @@ def _step_place(md, T: int, kept: bool, write_slots: Optional[torch.Tensor], dev
     if not kept:
         return nd, n - nd, cu or 0, 0, 0, 0
     pos, slots = md.positions, md.state_slots
-    if slots is None:
-        raise ValueError("a state needs md.state_slots")
+    if slots is None or pos is None:
+        raise ValueError("a state needs md.state_slots and md.positions")
     if pos.dim() != 1 or pos.numel() < T or pos.dtype is not torch.int64 or pos.get_device() != dev \
             or not pos.is_contiguous():
         raise ValueError(f"md.positions: {T} int64 positions beside x are wanted")
@@ -1694,7 +1694,7 @@ def causal_conv(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tens
     if x.dim() != 2 or x.dtype not in DTYPE_CODE:
         raise ValueError(f"x: rows of bf16, fp16 or fp32 are wanted, got {x.dtype} of shape {tuple(x.shape)}")
     T, Ch = x.shape
-    taps, dtype, dev = weight.shape[0], x.dtype, x.get_device()
+    taps, dtype, dev = weight.shape[0] if weight.dim() else 0, x.dtype, x.get_device()
     if not 1 <= taps <= 8:
         raise ValueError(f"a convolution of {taps} taps, 1 to 8 are built")
     if act != "silu" and act is not None:
@@ -1705,7 +1705,7 @@ def causal_conv(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tens
         _whole("bias", bias, (Ch,), torch.float32, dev)
     slots = 0
     if ring is not None:
-        slots = ring.shape[0]
+        slots = ring.shape[0] if ring.dim() else 0
         _whole("ring", ring, (slots, taps - 1, Ch), dtype, dev)
         if taps == 1:
             ring = None
