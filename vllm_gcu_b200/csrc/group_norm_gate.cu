@@ -6,9 +6,9 @@
 // A part of a row is a problem of its own: rows * groups of them.  A team of threads (one warp up to 1024
 // elements, a CTA above) holds its part in registers, NI vectors of V elements per thread, so that mean and
 // variance are two passes over registers and memory is read once; wider parts are read again.  Bytes bound it
-// (8192 rows of 8 x 1024, bf16: 72 us, 5.6 TB/s): weights come from L1 in 16 bytes, and nothing branches per
-// element (140 us without either; teams that walked rows of one group, to keep its weights and have a row under
-// way, had registers for too few of them: 297 us).
+// (8192 rows of 8 x 1024, bf16: 75 us, 5.3 TB/s, among other calls, 68 in a captured graph): weights come from L1
+// in 16 bytes, and nothing branches per element (140 us without either; teams that walked rows of one group, to keep
+// its weights and have a row under way, had registers for too few of them: 297 us).
 #include "common.cuh"
 
 namespace b200 {

@@ -25,9 +25,9 @@
 // while they do Y1 and the next chunk's G.  Lanes 96 and up have four blocks of M that are not zero where lanes below 32
 // have one, so their warps make less of W.
 //
-// 4096 tokens of 128 heads, 8 groups, N = 128, in one prompt: 115 to 123 us on different boards, 32 chunks of 3.2 us
-// and 5 us of start (157 MB: 24 us at the copy's rate; the products' 78 GFLOP, splits included: 47 us).  The arithmetic between the products
-// bounds it: 60 per cent of the issue slots and half of the integer pipe, most of that for splits into parts of bf16;
+// 4096 tokens of 128 heads, 8 groups, N = 128, in one prompt: 114 us in a captured graph, up to 125 among other calls, 32
+// chunks of 3.35 us and 5 us of start (156 MB: 24 us at the copy's rate; the products' 78 GFLOP, splits included: 47 us); as
+// long with 8 heads, one chain of chunks per 64 columns.  The arithmetic between the products bounds it: 60 per cent of the issue slots and half of the integer pipe, most of that for splits into parts of bf16;
 // tensor pipe 36 per cent.  On the way: 8 warps 213 us; decays from sums in 64 bits, by one warp, 131; with
 // more of it unrolled the instruction caches miss (no wait, no loop over products or groups is copied: 137 so, 119).
 #include "selective.cuh"

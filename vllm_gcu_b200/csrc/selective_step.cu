@@ -446,8 +446,8 @@ int launch_step(const ScanArgs& a, cudaStream_t s) {
 // Steps whose portions are short, whose state's way in and out is most of the work.  Only the mean length is known here,
 // and one portion may hold nearly all of the rows.
 //
-// Where the others would go by tiles: us by this kernel and by tiles, 96 requests of 80 heads of 64 x 128: 95 and 404 for
-// 1 token each, 246 and 418 for 8, 440 and 422 for 16.  A token of a portion takes 0.55 us, so the rows of a step are kept
+// Where the others would go by tiles: us by this kernel and by tiles, 96 requests of 80 heads of 64 x 128: 74 and 392 for
+// 1 token each, 147 and 392 for 4, 247 and 393 for 8, 449 and 395 for 16.  A token of a portion takes 0.55 us, so the rows of a step are kept
 // to what the tiles would take twice as long for were they all one portion's (8 us for a CTA per SM).
 //
 // Where they would go token after token (selective.cu), us by this kernel and by that one, 16 heads of 64 x 128 in 16 bits:

@@ -1690,7 +1690,8 @@ def causal_conv(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tens
     ``write_slots`` (default: the same; another one forks a request); None: zeros in front of the portions.  A slot
     that one request writes must be neither read nor written by another one of the step.  ``md`` also gives ``positions``,
     ``num_decode_tokens`` and ``cu_q_prefill``.  A request whose slot lies outside the ring gives zeros, one whose
-    write slot does leaves its ring nowhere; rows behind the last portion are not written."""
+    write slot does leaves its ring nowhere; rows behind the last portion are not written (without ``out`` they hold
+    anything).  ``out`` may share memory neither with x nor with the ring."""
     if x.dim() != 2 or x.dtype not in DTYPE_CODE:
         raise ValueError(f"x: rows of bf16, fp16 or fp32 are wanted, got {x.dtype} of shape {tuple(x.shape)}")
     T, Ch = x.shape
@@ -1741,7 +1742,9 @@ def selective_scan(x: torch.Tensor, dt: torch.Tensor, b: torch.Tensor, c: torch.
     D, N]``.  ``b`` and ``c [T, groups * N]``, N up to 256, shared by the heads (channels) of a group.  x, b, c, z
     and out are bf16, fp16 or fp32 alike, dt of that type or fp32, the rest fp32; rows may be strided views.
     State, slots, ``write_slots`` and ``md`` as in :func:`causal_conv`; ``state`` None: zeros in front of the
-    portions, nothing is kept.  Up to 65535 requests.  Returns ``[T, H * P]`` (``[T, D]``) in x's type."""
+    portions, nothing is kept.  Either end of ``dt_limits`` may be infinite.  Up to 65535 requests.  Returns ``[T, H *
+    P]`` (``[T, D]``) in x's type; rows behind the last portion are not written (without ``out`` they hold anything).
+    ``out`` may share memory with no other argument."""
     if x.dim() != 2 or x.dtype not in DTYPE_CODE:
         raise ValueError(f"x: rows of bf16, fp16 or fp32 are wanted, got {x.dtype} of shape {tuple(x.shape)}")
     T, cols = x.shape
