@@ -85,3 +85,28 @@ def test_step_sizes(form, decode, dtype):
         got = kept.view(T, D, N)[..., n].cpu().to(E.F64)
         off = (got / want - 1).abs().max().item()
         assert off < (2.0 ** -20.8 if dtype == F32 else 2.0 ** -21), off
+
+
+@pytest.mark.parametrize("step", [1, 8, 4000])
+@pytest.mark.parametrize("dtype,form,H,P,N", [(F32, "heads", 4, 8, 16), (F32, "heads", 4, 64, 64), (F16, "heads", 4, 40, 64),
+                                              (F32, "heads", 3, 7, 5)])
+def test_rates_per_head_over_thousands_of_tokens(dtype, form, H, P, N, step):
+    """A prompt, short portions and single tokens whose states forget a part in 600 to 3000 a token.  Decays and sums
+    are rounded by half a step (2^-25 on average over all roundings' sizes) either way, so that of some 3000 tokens
+    that a state holds, two roundings each, sqrt(2 * 3000) * 2^-25 shows, 2.3e-6; twice that for the largest of a few
+    hundred numbers, which share their decays.  A mean error of 1.5e-8 of a decay would leave 1500 times as much, 2.3e-5."""
+    from vllm_gcu_b200.ops import cuda as K
+    T = 4000
+    g = torch.Generator().manual_seed(7)
+    x, b = (torch.randn(T, n, generator=g).abs().to(dtype) for n in (H * P, N))
+    dt = 1e-3 + 1e-3 * torch.rand(T, H, generator=g)
+    a_log = torch.log(torch.linspace(0.2, 1.0, H))
+    want, _ = E.states(x, dt, b, a_log, 1, [T], [0], torch.zeros(1, H, P, N))
+    kept = torch.zeros(1, H, P, N, device="cuda")
+    dev = [t.cuda() for t in (x, dt, b, b)]
+    rates = a_log.cuda()
+    for t in range(0, T, step):
+        md = S.step(*((1, []) if step == 1 else (0, [step])), [t], slots=[0]).to("cuda")
+        K.selective_scan(*(v[t:t + step] for v in dev), rates, 1, md, kept, softplus=False)
+    worst = (kept.cpu().to(E.F64) / want - 1).abs().max().item()
+    assert worst < 4.6e-6

@@ -204,7 +204,7 @@ __global__ void __launch_bounds__(kCore<LPC> + 2 * kHelp) selective_scan_kernel(
               } else {
                 step = step_size<T>(a, t0 + vt, (c0 + vc + i) / a.width);
               }
-              e = expf(step * hrate[i]);
+              e = decay_of(step * hrate[i]);
             }
             (i & 1 ? dt[i / 2].y : dt[i / 2].x) = step;
             (i & 1 ? decay[i / 2].y : decay[i / 2].x) = e;

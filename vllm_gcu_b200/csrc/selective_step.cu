@@ -137,7 +137,7 @@ __global__ void __launch_bounds__(128) heads_step_kernel(const ScanArgs a) {
     const bool more = MANY && t + 1 < po.end;
     if (more) bring(t + 1, next);
     const float dt = step_from<T>(a, now.dt, bias);
-    const float decay = expf(-dt * rate);
+    const float decay = decay_of(-dt * rate);
     float s[kRows];
 #pragma unroll
     for (int i = 0; i < kRows; ++i) {
@@ -331,7 +331,7 @@ __global__ void __launch_bounds__(128) selective_step_kernel(const ScanArgs a) {
     if (CH || hd != head) {
       head = hd;
       dt = step_size<T>(a, r, CH ? col : hd);
-      if (!CH) decay = expf(-dt * expf(a.a_log[hd]));
+      if (!CH) decay = decay_of(-dt * expf(a.a_log[hd]));
     }
     const float x = to_f32<T>(static_cast<const T*>(a.x)[r * a.ldx + col]);
     const float dx = dt * x;
@@ -342,7 +342,7 @@ __global__ void __launch_bounds__(128) selective_step_kernel(const ScanArgs a) {
       for (int v = 0; v < V; ++v) {
         const int n = (l + LPR * k) * V + v;
         float e = decay;
-        if (CH) e = n < a.N ? expf(-dt * expf(a.a_log[static_cast<long long>(col) * a.N + n])) : 0.0f;
+        if (CH) e = n < a.N ? decay_of(-dt * expf(a.a_log[static_cast<long long>(col) * a.N + n])) : 0.0f;
         h[i][k][v] = fmaf(e, h[i][k][v], dx * bb[k][v]);
         s = fmaf(h[i][k][v], cc[k][v], s);
       }
