@@ -57,8 +57,18 @@ __device__ __forceinline__ float ex2_approx(float x) {
   return y;
 }
 
+template <bool kHalf>
+__device__ __forceinline__ uint32_t pack_pair(float lo, float hi) {
+  if constexpr (kHalf) {
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  } else {
+    return pack_bf16x2(lo, hi);
+  }
+}
+
 struct Args {
-  __nv_bfloat16* out;      // [T, Hq * HD], row pitch ldo
+  __nv_bfloat16* out;      // [T, Hq * HD], row pitch ldo (kHalf kernels: fp16)
   float* lse;              // optional [Hq, T] (without the sink's term)
   const float* sink;       // optional [Hq]: exp(sink) joins the denominator
   const int* cu_q;         // [B + 1]
@@ -73,6 +83,7 @@ struct Args {
   int OD;                  // output columns per head (the first of the HD)
   const float* slopes;     // biased kernels: [Hq], slope * (key - query position) joins the score
   int rope_col;            // latent form: first shared key column in a row of the latent rows
+  int first;               // kFirst kernels: the first keys of a request that stay visible beside the window
   unsigned int* status;
 };
 
@@ -109,7 +120,9 @@ __device__ __forceinline__ void find_tile(const Args& a, int tile, int lane, int
 // MODE 1 (shaped): soft cap, chunk and output columns of Args are in force.  The soft cap is
 // monotonic, so row maxima are taken over uncapped scores.  MODE 2 (biased): slopes and output columns;
 // row maxima are those of the biased scores, in the log2 domain.
-template <int HD, int MODE>
+// kFirst: the first keys of a request (Args::first) stay visible beside the window: their tiles come in front of the
+// window's.  kHalf: fp16 in place of bf16.
+template <int HD, int MODE, bool kFirst = false, bool kHalf = false>
 __global__ void __launch_bounds__(kThreads, 1)
     fmha_prefill_kernel(const __grid_constant__ CUtensorMap tmQ,
                         const __grid_constant__ CUtensorMap tmK,
@@ -188,7 +201,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (a.window > 0) kv_lo = max(0, pos0 - a.window + 1);
   if (kShaped && a.chunk > 0) kv_lo = max(kv_lo, pos0 / a.chunk * a.chunk);
   const int t0 = kv_lo / BKV;
-  const int nt = (kv_hi + BKV - 1) / BKV - t0;          // >= 1
+  const int nf = kFirst && a.window > 0 ? min(t0, (a.first + BKV - 1) / BKV) : 0;
+  const int nt = nf + (kv_hi + BKV - 1) / BKV - t0;     // >= 1
+  auto tile_of = [&](int j) { return kFirst ? (j < nf ? j : t0 + j - nf) : t0 + j; };
   const int kvh = head / (a.Hq / a.Hkv);
 
   if (warp == 0) {
@@ -204,7 +219,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int j = 0; ok && j < nt; ++j) {
         const int st = j & 1;
         const uint32_t par = ((j >> 1) & 1) ^ 1u;
-        const int key0 = (t0 + j) * BKV;
+        const int key0 = tile_of(j) * BKV;
         for (int kv = 0; kv < 2 && ok; ++kv) {
           uint64_t* empty = kv == 0 ? &k_empty[st] : &v_empty[st];
           uint64_t* full = kv == 0 ? &k_full[st] : &v_full[st];
@@ -229,8 +244,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   } else if (warp == 1) {
     // ---------------- MMA issuer ----------------
     if (elect_one()) {
-      constexpr uint32_t kIdescS = make_idesc(BQ, BKV, 1, 1);
-      constexpr uint32_t kIdescO = make_idesc(BQ, HD, 1, 1) | kIdescBMajorMN;
+      constexpr uint32_t kType = kHalf ? 0 : 1;
+      constexpr uint32_t kIdescS = make_idesc(BQ, BKV, kType, kType);
+      constexpr uint32_t kIdescO = make_idesc(BQ, HD, kType, kType) | kIdescBMajorMN;
       const uint32_t q_addr = smem_u32(smem + kOffQ);
       const uint32_t p_addr = smem_u32(smem + kOffP);
       auto issue_s = [&](int j) -> bool {
@@ -316,10 +332,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         ok = false;
       tc_fence_after();
       const uint32_t s_addr = lane_addr + kColS + b * BKV + g * 64;
-      const int key0 = (t0 + j) * BKV + g * 64;
+      const int key0 = tile_of(j) * BKV + g * 64;
       // Only tiles that touch the causal diagonal, the window start or the end of the
       // sequence need per-element masks; the test is uniform over the CTA.
-      const int tile_key0 = (t0 + j) * BKV;
+      const int tile_key0 = tile_of(j) * BKV;
       const bool need_mask =
           (tile_key0 + BKV - 1 > (a.causal ? min(pos0, seq_len - 1) : seq_len - 1)) ||
           (a.window > 0 && tile_key0 < pos0 + BQ - a.window) ||
@@ -341,7 +357,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
             for (int i = 0; i < 32; ++i) {
               const int key = key0 + c * 32 + i;
-              if (key <= hi && key >= lo) mt = fmaxf(mt, __uint_as_float(v[i]));
+              if (key <= hi && (key >= lo || (kFirst && key < a.first))) mt = fmaxf(mt, __uint_as_float(v[i]));
             }
           } else {
             float m0 = mt, m1 = -INFINITY, m2 = -INFINITY, m3 = -INFINITY;
@@ -402,11 +418,11 @@ __global__ void __launch_bounds__(kThreads, 1)
               const int key = key0 + c * 32 + i;
               float p0 = prob(v[i], i, base);
               float p1 = prob(v[i + 1], i + 1, base);
-              if (key > hi || key < lo) p0 = 0.0f;
-              if (key + 1 > hi || key + 1 < lo) p1 = 0.0f;
+              if (key > hi || (key < lo && !(kFirst && key < a.first))) p0 = 0.0f;
+              if (key + 1 > hi || (key + 1 < lo && !(kFirst && key + 1 < a.first))) p1 = 0.0f;
               rs0 += p0;
               rs1 += p1;
-              pk[c * 16 + (i >> 1)] = pack_bf16x2(p0, p1);
+              pk[c * 16 + (i >> 1)] = pack_pair<kHalf>(p0, p1);
             }
           } else {
 #pragma unroll
@@ -415,7 +431,7 @@ __global__ void __launch_bounds__(kThreads, 1)
               const float p1 = prob(v[i + 1], i + 1, base);
               rs0 += p0;
               rs1 += p1;
-              pk[c * 16 + (i >> 1)] = pack_bf16x2(p0, p1);
+              pk[c * 16 + (i >> 1)] = pack_pair<kHalf>(p0, p1);
             }
           }
         }
@@ -478,10 +494,10 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             uint4 u;
-            u.x = pack_bf16x2(__uint_as_float(v[i * 8 + 0]) * inv, __uint_as_float(v[i * 8 + 1]) * inv);
-            u.y = pack_bf16x2(__uint_as_float(v[i * 8 + 2]) * inv, __uint_as_float(v[i * 8 + 3]) * inv);
-            u.z = pack_bf16x2(__uint_as_float(v[i * 8 + 4]) * inv, __uint_as_float(v[i * 8 + 5]) * inv);
-            u.w = pack_bf16x2(__uint_as_float(v[i * 8 + 6]) * inv, __uint_as_float(v[i * 8 + 7]) * inv);
+            u.x = pack_pair<kHalf>(__uint_as_float(v[i * 8 + 0]) * inv, __uint_as_float(v[i * 8 + 1]) * inv);
+            u.y = pack_pair<kHalf>(__uint_as_float(v[i * 8 + 2]) * inv, __uint_as_float(v[i * 8 + 3]) * inv);
+            u.z = pack_pair<kHalf>(__uint_as_float(v[i * 8 + 4]) * inv, __uint_as_float(v[i * 8 + 5]) * inv);
+            u.w = pack_pair<kHalf>(__uint_as_float(v[i * 8 + 6]) * inv, __uint_as_float(v[i * 8 + 7]) * inv);
             if constexpr (MODE != 0) {
               const int col = g * 64 + c * 32 + i * 8;
               if ((OD & 7) != 0) {
@@ -562,25 +578,25 @@ static int get_map(const void* base, unsigned long long rows, unsigned long long
 namespace b200 {
 namespace fmha {
 
-template <int HD, int MODE>
+template <int HD, int MODE, bool kFirst = false, bool kHalf = false>
 static int launch(const CUtensorMap& tmQ, const CUtensorMap& tmK, const CUtensorMap& tmV,
                   const Args& a, int num_q_tiles, cudaStream_t s) {
   static bool configured[64] = {false};
   int dev = 0;
   cudaGetDevice(&dev);
   if (dev >= 0 && dev < 64 && !configured[dev]) {
-    cudaError_t e = cudaFuncSetAttribute(fmha_prefill_kernel<HD, MODE>,
+    cudaError_t e = cudaFuncSetAttribute(fmha_prefill_kernel<HD, MODE, kFirst, kHalf>,
                                          cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
     if (e != cudaSuccess) return static_cast<int>(e);
     configured[dev] = true;
   }
   dim3 grid(num_q_tiles, a.Hq);
-  fmha_prefill_kernel<HD, MODE><<<grid, kThreads, kSmemBytes, s>>>(tmQ, tmK, tmV, a);
+  fmha_prefill_kernel<HD, MODE, kFirst, kHalf><<<grid, kThreads, kSmemBytes, s>>>(tmQ, tmK, tmV, a);
   return static_cast<int>(cudaGetLastError());
 }
 
 // num_tiles pieces of 128 rows (latent: 256) for every pair of heads (latent: head)
-template <bool kLatent>
+template <bool kLatent, bool kFirst = false, bool kHalf = false>
 static int launch_pair(const CUtensorMap& tmQ, const CUtensorMap& tmK, const CUtensorMap& tmV,
                        const Args& a, int num_tiles, cudaStream_t s) {
   static bool configured[64] = {false};
@@ -588,14 +604,14 @@ static int launch_pair(const CUtensorMap& tmQ, const CUtensorMap& tmK, const CUt
   cudaGetDevice(&dev);
   if (dev >= 0 && dev < 64 && !configured[dev]) {
     cudaError_t e = cudaFuncSetAttribute(
-        fmha_pair_kernel<kLatent>, cudaFuncAttributeMaxDynamicSharedMemorySize, kPairSmemBytes);
+        fmha_pair_kernel<kLatent, kFirst, kHalf>, cudaFuncAttributeMaxDynamicSharedMemorySize, kPairSmemBytes);
     if (e != cudaSuccess) return static_cast<int>(e);
     configured[dev] = true;
   }
   const long long total = static_cast<long long>(num_tiles) * (kLatent ? a.Hq : a.Hq / 2);
   if (total > 0x3fffffff) return -2;
   const int grid = static_cast<int>(total < sm_count() ? total : sm_count());
-  return launch_overlapped(fmha_pair_kernel<kLatent>, dim3(grid), dim3(kPairThreads), kPairSmemBytes, s, tmQ,
+  return launch_overlapped(fmha_pair_kernel<kLatent, kFirst, kHalf>, dim3(grid), dim3(kPairThreads), kPairSmemBytes, s, tmQ,
                            tmK, tmV, a, static_cast<int>(total));
 }
 
@@ -688,7 +704,7 @@ B200_API int b200_fmha_prefill_sink(const void* q, long long ldq, void* out, lon
   a.lse = lse; a.sink = sink; a.cu_q = cu_q; a.seq_lens = seq_lens; a.block_tables = block_tables;
   a.ldo = ldo; a.B = B; a.T = T; a.Hq = Hq; a.Hkv = Hkv; a.max_blocks = max_blocks;
   a.block_size = block_size; a.causal = causal; a.window = window; a.scale = scale;
-  a.softcap = softcap; a.chunk = chunk; a.OD = OD; a.slopes = slopes; a.rope_col = 0;
+  a.softcap = softcap; a.chunk = chunk; a.OD = OD; a.slopes = slopes; a.rope_col = 0; a.first = 0;
   a.status = status_ptr();
   cudaStream_t s = static_cast<cudaStream_t>(stream);
 #define B200_FMHA(MODE)                                                        \
@@ -767,4 +783,61 @@ B200_API int b200_latent_prefill(const void* q, long long ldq, void* out, long l
   a.scale = scale; a.rope_col = W - 64;
   a.status = status_ptr();
   return launch_pair<true>(tmQ, tmKV, tmPe, a, num_tiles, static_cast<cudaStream_t>(stream));
+}
+
+namespace {
+struct ExpandedCall {
+  const void* q;
+  void* out;
+  const void *keys, *values;
+  const int *cu_q, *seq_lens, *table;
+  long long ldq, ldo;
+  float scale;
+  int T, B, Hq, Hkv, D, tiles, table_width, num_q_tiles, window, first, dtype;
+};
+}  // namespace
+
+// Causal attention over keys and values that b200_block_scaled_expand laid out in tiles of 128 (`table` says where a
+// request's tiles lie), head dimension 64 or 128, dtype 0 bf16 or 1 fp16: keys of the window (0: all) and the first ones.
+B200_API int b200_fmha_expanded(const void* call, void* stream) {
+  using namespace b200;
+  using namespace b200::fmha;
+  const ExpandedCall& k = *static_cast<const ExpandedCall*>(call);
+  if (k.B <= 0 || k.T <= 0 || k.num_q_tiles <= 0) return 0;
+  if (k.Hkv <= 0 || k.Hq % k.Hkv != 0 || (k.D != 64 && k.D != 128) || k.ldq % 8 != 0 || k.ldo % 8 != 0 ||
+      (reinterpret_cast<uintptr_t>(k.q) | reinterpret_cast<uintptr_t>(k.out) | reinterpret_cast<uintptr_t>(k.keys) |
+       reinterpret_cast<uintptr_t>(k.values)) & 15)
+    return -2;
+  CUtensorMap tmQ, tmK, tmV;
+  const unsigned long long rows = static_cast<unsigned long long>(k.tiles) * BKV,
+                           cols = static_cast<unsigned long long>(k.Hkv) * k.D;
+  int r = get_map(k.q, k.T, static_cast<unsigned long long>(k.Hq) * k.D, static_cast<unsigned long long>(k.ldq) * 2, BQ,
+                  false, &tmQ);
+  if (r == 0) r = get_map(k.keys, rows, cols, cols * 2, kPage, false, &tmK);
+  if (r == 0) r = get_map(k.values, rows, cols, cols * 2, kPage, false, &tmV);
+  if (r != 0) return r < 0 ? -6 : r;
+  Args a = {};
+  a.out = static_cast<__nv_bfloat16*>(k.out);
+  a.cu_q = k.cu_q; a.seq_lens = k.seq_lens; a.block_tables = k.table; a.ldo = k.ldo; a.B = k.B; a.T = k.T;
+  a.Hq = k.Hq; a.Hkv = k.Hkv; a.max_blocks = k.table_width; a.block_size = BKV; a.causal = 1; a.window = k.window;
+  a.first = k.first; a.scale = k.scale; a.OD = k.D;
+  a.status = status_ptr();
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const bool firsts = k.window > 0 && k.first > 0;
+  // heads in pairs where one head a CTA takes more than one round of the SMs, as in b200_fmha_prefill_sink
+  const bool pairs = k.D == 128 && ((k.Hq / k.Hkv) & 1) == 0 && static_cast<long long>(k.num_q_tiles) * k.Hq > sm_count();
+#define B200_EXPANDED(FIRST, HALF)                                                             \
+  do {                                                                                         \
+    if (pairs) return launch_pair<false, FIRST, HALF>(tmQ, tmK, tmV, a, k.num_q_tiles, s);     \
+    if (k.D == 64) return launch<64, 0, FIRST, HALF>(tmQ, tmK, tmV, a, k.num_q_tiles, s);      \
+    return launch<128, 0, FIRST, HALF>(tmQ, tmK, tmV, a, k.num_q_tiles, s);                    \
+  } while (0)
+  if (k.dtype == 0) {
+    if (firsts) B200_EXPANDED(true, false);
+    B200_EXPANDED(false, false);
+  }
+  if (k.dtype != 1) return -8;
+  if (firsts) B200_EXPANDED(true, true);
+  B200_EXPANDED(false, true);
+#undef B200_EXPANDED
 }

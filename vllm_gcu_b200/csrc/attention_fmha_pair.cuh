@@ -136,10 +136,12 @@ struct Work {            // what the TMA warp tells the others about a pair of t
   int head;              // head (kLatent) or first of two heads
   int t0;                // first key tile
   int nt[2];             // key tiles of both slots
-  int pad[3];
+  int nf;                // kFirst: tiles of first keys in front of t0's
+  int pad[2];
 };
 
-template <bool kLatent>
+// kFirst, kHalf: see attention_fmha.cu
+template <bool kLatent, bool kFirst = false, bool kHalf = false>
 __global__ void __launch_bounds__(kPairThreads, 1)
     fmha_pair_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                      const __grid_constant__ CUtensorMap tmV, const Args a, const int total) {
@@ -239,12 +241,13 @@ __global__ void __launch_bounds__(kPairThreads, 1)
           k.pos = k.keys - q_len + qt * RT;
           k.head = kLatent ? w % pairs : 2 * (w % pairs);
           k.t0 = a.window > 0 ? max(0, k.pos - a.window + 1) / BKV : 0;
+          k.nf = kFirst && a.window > 0 ? min(k.t0, (a.first + BKV - 1) / BKV) : 0;
   #pragma unroll
           for (int h = 0; h < 2; ++h) {
             const int off = kLatent ? h * BQ : 0;
             const int rows = min(BQ, k.rows - off);
             const int hi = a.causal ? min(k.keys, k.pos + off + rows) : k.keys;
-            k.nt[h] = rows > 0 ? max(1, (hi + BKV - 1) / BKV - k.t0) : 0;
+            k.nt[h] = rows > 0 ? k.nf + max(1, (hi + BKV - 1) / BKV - k.t0) : 0;
           }
           if constexpr (kLatent) {
             int s = 0;             // the sequences' keys follow each other, each from a whole tile on
@@ -266,6 +269,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
             o->t0 = k.t0;
             o->nt[0] = k.nt[0];
             o->nt[1] = k.nt[1];
+            if constexpr (kFirst) o->nf = k.nf;
           }
           mbar_arrive(&w_full[it & 1]);
         }
@@ -326,7 +330,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
           const int last_tok = k.keys - 1;
           const int page = lane >> 1, half = lane & 1;
           auto row_of = [&](int j) {           // pages past the end: any valid page
-            const int key = (k.t0 + j) * BKV + page * kPage;
+            const int key = (kFirst && j < k.nf ? j : k.t0 + j - k.nf) * BKV + page * kPage;
             return lane < 2 * (BKV / kPage)
                        ? bt[min(key, last_tok) / a.block_size] * a.block_size + key % a.block_size
                        : 0;
@@ -352,9 +356,10 @@ __global__ void __launch_bounds__(kPairThreads, 1)
     } else if (warp <= 2) {
       // ---------------- MMA issuers, one per slot ----------------
       if (elect_one()) {
-        constexpr uint32_t kIdescS = make_idesc(BQ, BKV, 1, 1);
-        constexpr uint32_t kIdescO = make_idesc(BQ, HD, 1, 1) | kIdescBMajorMN;
-        constexpr uint32_t kIdescHalf = make_idesc(BQ, HD / 2, 1, 1) | kIdescBMajorMN;
+        constexpr uint32_t kType = kHalf ? 0 : 1;
+        constexpr uint32_t kIdescS = make_idesc(BQ, BKV, kType, kType);
+        constexpr uint32_t kIdescO = make_idesc(BQ, HD, kType, kType) | kIdescBMajorMN;
+        constexpr uint32_t kIdescHalf = make_idesc(BQ, HD / 2, kType, kType) | kIdescBMajorMN;
         const int h = warp - 1;
         const uint32_t t_s = tmem + h * BKV, t_o = tmem + kPairColO + h * HD;
         const uint64_t q_desc = make_desc_k_sw128(smem_u32(smem) + h * kQU * kSub);
@@ -481,6 +486,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
       if (!mbar_wait_warp(&w_full[it & 1], (it >> 1) & 1, a.status, kKernelId, 0x640u, abort_flag)) break;
       const volatile Work* k = works + (it & 1);
       const int seq = k->seq;
+      const int nf = kFirst ? k->nf : 0;
       const int nt = k->nt[h], nt_both = min(nt, k->nt[h ^ 1]), t0 = k->t0, keys = k->keys, head = kLatent ? k->head : k->head + h;
       const int pos0 = k->pos + (kLatent ? h * BQ : 0), row0 = k->row + (kLatent ? h * BQ : 0);
       const int rows = k->rows - (kLatent ? h * BQ : 0);
@@ -503,7 +509,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
         s_phase ^= 1u;
         tc_fence_after();
         uint32_t v[4][32];
-        const int key0 = (t0 + j) * BKV;
+        const int key0 = (kFirst ? (j < nf ? j : t0 + j - nf) : t0 + j) * BKV;
         const bool need_mask = (key0 + BKV - 1 > edge) || (a.window > 0 && key0 < pos0 + BQ - a.window);
         float mx[4];
         auto masked = [&](int c) {          // chunk of 32 keys, where a row of the warp does not see all of them
@@ -511,7 +517,8 @@ __global__ void __launch_bounds__(kPairThreads, 1)
           if (need_mask && (first + 31 > hi_warp || (a.window > 0 && first < lo_warp))) {
 #pragma unroll
             for (int i = 0; i < 32; ++i)
-              if (i > hi - first || i < lo - first) v[c][i] = 0xff800000u;            // -inf
+              if (i > hi - first || (i < lo - first && !(kFirst && i < a.first - first)))
+                v[c][i] = 0xff800000u;                                                 // -inf
           }
         };
         auto row_max = [&](int c) {
@@ -576,7 +583,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
             p0 = ex2_approx(p0);
             p1 = ex2_approx(p1);
             sum[c] += p0 + p1;
-            pk[i >> 1] = pack_bf16x2(p0, p1);
+            pk[i >> 1] = pack_pair<kHalf>(p0, p1);
           }
           if (c == 3 && lane == 0 && j < nt_both) mbar_arrive(&turn[h]);
           tmem_st_32x16(s_addr + c * 16, pk);
@@ -615,8 +622,8 @@ __global__ void __launch_bounds__(kPairThreads, 1)
           uint32_t w[4];
 #pragma unroll
           for (int e = 0; e < 4; ++e)
-            w[e] = pack_bf16x2(__uint_as_float(o[i + 2 * e]) * inv,
-                               __uint_as_float(o[i + 2 * e + 1]) * inv);
+            w[e] = pack_pair<kHalf>(__uint_as_float(o[i + 2 * e]) * inv,
+                                  __uint_as_float(o[i + 2 * e + 1]) * inv);
           *reinterpret_cast<uint4*>(orow + c * 32 + i) = make_uint4(w[0], w[1], w[2], w[3]);
         }
       }

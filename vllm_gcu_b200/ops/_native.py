@@ -175,6 +175,11 @@ class _Sigs:
     b200_causal_conv = [S, P]
     b200_selective_scan = [S, P]
     b200_group_norm_gate = [S, P]
+    b200_block_scaled_cache = [S, P]
+    b200_block_scaled_expand = [S, P]
+    b200_block_scaled_rows = [S, P]
+    b200_fmha_expanded = [S, P]
+    b200_cache_pages = [S, P]
     b200_gemm_wna16 = [P, L, P, P, P, P, P, L, I, I, I, I, I, P]
     b200_gemm_wna16_grouped = [P, L, P, P, P, P, L, I, I, I, I, I, I, P, P, P, P]
     b200_sample = [P, L, I, I, I, P, P, P, P, P, L, P, P]

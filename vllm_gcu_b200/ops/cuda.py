@@ -1869,6 +1869,311 @@ def group_norm_gate(x: torch.Tensor, z: Optional[torch.Tensor], weight: torch.Te
     return out
 
 
+# ---------------------------------------------------------------------------
+# a cache in 8 bits with a scale for each block and head
+# ---------------------------------------------------------------------------
+_SCALED_WRITE = struct.Struct("7P4q8i")
+_SCALED_EXPAND = struct.Struct("10Pq12i")
+_SCALED_ROWS = struct.Struct("11P3qf15i")
+_EXPANDED_CALL = struct.Struct("7P2qf11i")
+_PAGES_CALL = struct.Struct("7Pq6i")
+_SCALED_WIDTHS = (64, 128, 256)       # head dimensions of these kernels
+# Portions take the kernel for few rows up to this many query rows a key head, else keys are expanded to 16 bits
+SCALED_ROWS = 64
+# Keys that are expanded at once (a longer request alone): 2 x 2 bytes for each of a key's numbers
+SCALED_EXPANDED_KEYS = 1 << 17
+
+
+def _scaled_cache(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor):
+    """Checks a cache of codes and scales: (blocks, block size, heads, head dimension, bytes of a token, int8, device)."""
+    if k_cache.dim() != 4 or v_cache.shape != k_cache.shape:
+        raise ValueError(f"caches [blocks, block size, heads, head dimension] of one shape are wanted, got "
+                         f"{tuple(k_cache.shape)} and {tuple(v_cache.shape)}")
+    nb, bs, H, D = k_cache.shape
+    dtype, dev = k_cache.dtype, k_cache.get_device()
+    if dtype is not FP8 and dtype is not torch.int8 or v_cache.dtype is not dtype:
+        raise ValueError(f"codes of float8_e4m3fn or int8 are wanted, got {k_cache.dtype} and {v_cache.dtype}")
+    if D not in _SCALED_WIDTHS or bs % 16 or not nb:
+        raise ValueError(f"{nb} blocks of {bs} tokens, heads of {D}: blocks of a multiple of 16 tokens and heads of "
+                         f"{_SCALED_WIDTHS} are built")
+    row = k_cache.stride(1)
+    for name, t in (("k_cache", k_cache), ("v_cache", v_cache)):
+        if t.stride() != (bs * row, row, D, 1) or row < H * D or row % 16 or t.data_ptr() % 16 or t.get_device() != dev:
+            raise ValueError(f"{name}: tokens that follow each other at equal distances of a multiple of 16 bytes are "
+                             f"wanted, both caches alike on one device, got strides {tuple(t.stride())} on {t.device}")
+    if nb * bs >= 1 << 31:
+        raise ValueError(f"a cache of {nb * bs} tokens")
+    for name, t in (("k_scale", k_scale), ("v_scale", v_scale)):
+        if t.shape != (nb, H) or t.dtype is not torch.float32 or not t.is_contiguous() or t.get_device() != dev:
+            raise ValueError(f"{name}: contiguous float32 scales of shape {(nb, H)} beside the cache are wanted, got "
+                             f"{t.dtype}, {tuple(t.shape)} on {t.device}")
+    return nb, bs, H, D, row, dtype is torch.int8, dev
+
+
+def _indices(name: str, t: torch.Tensor, shape, dev: int, dtype=torch.int32) -> int:
+    if t.shape != shape or t.dtype is not dtype or t.get_device() != dev or not t.is_contiguous():
+        raise ValueError(f"{name}: contiguous {dtype} of shape {tuple(shape)} beside the cache are wanted, got {t.dtype}, "
+                         f"{tuple(t.shape)}, strides {tuple(t.stride())} on {t.device}")
+    return t.data_ptr()
+
+
+def block_scaled_cache(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                       k_scale: torch.Tensor, v_scale: torch.Tensor, slot_mapping: torch.Tensor) -> None:
+    """Keys and values ``[T, H * D]`` (bf16, fp16 or fp32; row-strided views are fine) of a step into a cache in 8 bits:
+    codes ``[blocks, block size, H, D]`` (float8_e4m3fn or int8; D 64, 128 or 256, blocks of a multiple of 16 tokens) with
+    scales ``[blocks, H]`` fp32.  ``slot_mapping [T]`` int64: block * block size + place, -1 for a row that goes nowhere.
+    The rows of a block follow each other in rising order of places, and no other row of the step goes to it.
+
+    A scale is a power of two.  A block whose first place is written starts anew, with the least scale (2^-100 .. 2^121)
+    that holds the rows' numbers; else the scale stays, or grows where a number does not fit, and the codes in front of the
+    new rows are rounded to it.  Infinities become the largest code and NaN the code 0; neither counts for the scale."""
+    nb, bs, H, D, row, int8, dev = _scaled_cache(k_cache, v_cache, k_scale, v_scale)
+    if k.dtype not in DTYPE_CODE or k.dim() != 2:
+        raise ValueError(f"k: rows of bf16, fp16 or fp32 are wanted, got {k.dtype} of shape {tuple(k.shape)}")
+    T, es = k.shape[0], k.element_size()
+    ldk = _row_view("k", k, T, H * D, (k.dtype,), dev)
+    ldv = _row_view("v", v, T, H * D, (k.dtype,), dev)
+    slots = _indices("slot_mapping", slot_mapping, (T,), dev, torch.int64)
+    if T == 0:
+        return
+    pk, pv = k.data_ptr(), v.data_ptr()
+    wide = (pk | pv) % 16 == 0 and (T == 1 or (ldk | ldv) * es % 16 == 0)
+    _call_on(dev, "b200_block_scaled_cache",
+             _SCALED_WRITE.pack(pk, pv, k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
+                                slots, ldk, ldv, row, nb * bs, T, H, D, bs, wide, int8, DTYPE_CODE[k.dtype], 0))
+
+
+def block_scaled_splits(requests: int, heads: int, max_seq_len: int) -> int:
+    """Splits of the keys that ``block_scaled_decode`` takes for so many requests and key heads."""
+    ctas = requests * heads
+    if ctas <= 0 or max_seq_len <= 256:
+        return 1
+    want = -(-2 * _sms() // ctas)
+    return max(1, min(want, max_seq_len // 128, 8 if max_seq_len < 8 * 2048 else 32))
+
+
+def _scaled_query(q: torch.Tensor, out: Optional[torch.Tensor], H: int, D: int, dev: int, caches):
+    """Checks queries and their output: (query heads, address and pitch of q, out, address and pitch of out)."""
+    if q.dim() != 3 or q.dtype not in (torch.bfloat16, torch.float16):
+        raise ValueError(f"q: [tokens, heads, head dimension] of bf16 or fp16 is wanted, got {q.dtype} of shape "
+                         f"{tuple(q.shape)}")
+    T, Hq, Dq = q.shape
+    if Dq != D or not Hq or Hq % H:
+        raise ValueError(f"q has {Hq} heads of {Dq}, the cache {H} heads of {D}")
+    ld, pq = q.stride(0), q.data_ptr()
+    if q.stride(2) != 1 or (q.stride(1) != D and Hq > 1) or q.get_device() != dev:
+        raise ValueError(f"q: heads that follow each other beside the cache are wanted, got strides {tuple(q.stride())} "
+                         f"on {q.device}")
+    if pq % 16 or (ld % 8 and T > 1):
+        q = q.contiguous()
+        ld, pq = q.stride(0), q.data_ptr()
+    if T == 1:
+        ld = Hq * D
+    if out is None:
+        out = torch.empty((T, Hq, D), dtype=q.dtype, device=q.device)
+        return Hq, q, pq, ld, out, out.data_ptr(), Hq * D
+    ldo, po = out.stride(0), out.data_ptr()
+    if out.shape != (T, Hq, D) or out.dtype is not q.dtype or out.get_device() != dev or out.stride(2) != 1 \
+            or (out.stride(1) != D and Hq > 1):
+        raise ValueError(f"out: {q.dtype} of shape {(T, Hq, D)} with heads that follow each other is wanted, got "
+                         f"{out.dtype}, {tuple(out.shape)}, strides {tuple(out.stride())}")
+    if T == 1:
+        ldo = Hq * D
+    if po % 16 or ldo % 8 or ldo < Hq * D:
+        raise ValueError(f"out: rows of a multiple of 8 elements that start at 16 bytes and share none are wanted, got a "
+                         f"pitch of {ldo}")
+    if T and _overlap((po, ldo, T, Hq * D, 2), (pq, ld, T, Hq * D, 2)):
+        raise ValueError("out shares memory with q")
+    for c in caches:
+        if T and po < c.data_ptr() + ((c.shape[0] * c.shape[1] - 1) * c.stride(1) + H * D) \
+                and c.data_ptr() < po + ((T - 1) * ldo + Hq * D) * 2:
+            raise ValueError("out shares memory with the cache")
+    return Hq, q, pq, ld, out, po, ldo
+
+
+def _visible(window: int, first: int) -> tuple[int, int]:
+    if window < 0 or first < 0 or max(window, first) >= 1 << 31:
+        raise ValueError(f"a window of {window} tokens and {first} first ones")
+    return int(window), int(first)
+
+
+def _scaled_rows(q, pq, ldq, out, po, ldo, k_cache, v_cache, k_scale, v_scale, cu_q, seq_lens, tables, B, max_blocks, max_q,
+                 scale, window, first, splits, workspace, shape) -> None:
+    nb, bs, H, D, row, int8, dev = shape
+    T, Hq = q.shape[0], q.shape[1]
+    tmp_out = tmp_lse = None
+    if splits > 8:
+        if workspace is None:
+            tmp_out = torch.empty(T * Hq * splits * D, device=q.device, dtype=torch.float32)
+            tmp_lse = torch.empty(T * Hq * splits, device=q.device, dtype=torch.float32)
+        else:
+            tmp_out, tmp_lse = workspace
+            for t, n in ((tmp_out, T * Hq * splits * D), (tmp_lse, T * Hq * splits)):
+                if t.numel() < n or t.dtype is not torch.float32 or not t.is_contiguous() or t.get_device() != dev:
+                    raise ValueError(f"workspace: contiguous float32 numbers are wanted, {T * Hq * splits * D} and "
+                                     f"{T * Hq * splits} of them for {splits} splits")
+    _call_on(dev, "b200_block_scaled_rows",
+             _SCALED_ROWS.pack(pq, po, k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), cu_q,
+                               seq_lens, tables, 0 if tmp_out is None else tmp_out.data_ptr(),
+                               0 if tmp_lse is None else tmp_lse.data_ptr(), ldq, ldo, row, scale, T, B, max_q, Hq, H, D,
+                               splits, max_blocks, bs, nb, window, first, int8, DTYPE_CODE[q.dtype], 0))
+
+
+def block_scaled_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor,
+                        v_scale: torch.Tensor, block_tables: torch.Tensor, seq_lens: torch.Tensor, scale: float,
+                        out: Optional[torch.Tensor] = None, num_splits: int = 0,
+                        workspace: Optional[tuple[torch.Tensor, torch.Tensor]] = None, max_seq_len: int = 0,
+                        window: int = 0, first: int = 0) -> torch.Tensor:
+    """Attention of one token of each request over a cache that ``block_scaled_cache`` wrote: ``q [B, Hq, D]`` (bf16 or
+    fp16, row stride free), ``block_tables [B, blocks]`` and ``seq_lens [B]`` int32 (the token itself counts; 0: a row of
+    zeros).  ``window``: only the last so many keys, and the ``first`` ones of the request (0: all keys).  ``num_splits``
+    0 chooses by ``max_seq_len`` (a bound of seq_lens; default: what the tables hold); more than 8 splits, up to 32, use
+    ``workspace`` (fp32, B * Hq * splits * D and B * Hq * splits numbers), by default a new one."""
+    shape = _scaled_cache(k_cache, v_cache, k_scale, v_scale)
+    _, bs, H, D, _, _, dev = shape
+    Hq, q, pq, ldq, out, po, ldo = _scaled_query(q, out, H, D, dev, (k_cache, v_cache))
+    B = q.shape[0]
+    window, first = _visible(window, first)
+    M = block_tables.shape[1] if block_tables.dim() == 2 else 0
+    tables, lens = _indices("block_tables", block_tables, (B, M), dev), _indices("seq_lens", seq_lens, (B,), dev)
+    if B == 0:
+        return out
+    if not M:
+        return out.zero_()
+    seen = min(max_seq_len or M * bs, M * bs)
+    if window:
+        seen = min(seen, window + first)
+    if not 0 <= num_splits <= 32:
+        raise ValueError(f"{num_splits} splits, up to 32 are built")
+    splits = num_splits or block_scaled_splits(B, H * -(-(Hq // H) // 32), seen)
+    if workspace is not None and num_splits == 0:
+        while splits > 8 and (workspace[0].numel() < B * Hq * splits * D or workspace[1].numel() < B * Hq * splits):
+            splits -= 1
+    _scaled_rows(q, pq, ldq, out, po, ldo, k_cache, v_cache, k_scale, v_scale, 0, lens, tables, B, M, 1, scale, window,
+                 first, splits, workspace, shape)
+    return out
+
+
+def _expanded_tiles(q_len: int, kv_len: int, window: int, first: int) -> int:
+    """Tiles of 128 keys that a request's tokens can see."""
+    if q_len <= 0 or kv_len <= 0:
+        return 0
+    lo = max(0, kv_len - q_len - window + 1) // 128 if window else 0
+    return -(-kv_len // 128) - lo + (min(lo, -(-first // 128)) if window else 0)
+
+
+def block_scaled_prefill(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor,
+                         v_scale: torch.Tensor, block_tables: torch.Tensor, cu_q: torch.Tensor, seq_lens: torch.Tensor,
+                         scale: float, q_lens: Sequence[int], kv_lens: Sequence[int], out: Optional[torch.Tensor] = None,
+                         window: int = 0, first: int = 0) -> torch.Tensor:
+    """The same for portions: ``q [T, Hq, D]``, the rows of request b from ``cu_q[b]`` on (``[B + 1]`` int32), its last token
+    at position ``seq_lens[b] - 1``.  ``q_lens`` and ``kv_lens`` hold the same numbers on the host.  Rows of no request are
+    left as they are.  Requests of few tokens read the codes as they are; for longer ones the keys and values that their
+    tokens can see are expanded to 16 bits, at most ``SCALED_EXPANDED_KEYS`` keys (or one request's) at a time."""
+    shape = nb, bs, H, D, row, int8, dev = _scaled_cache(k_cache, v_cache, k_scale, v_scale)
+    Hq, q, pq, ldq, out, po, ldo = _scaled_query(q, out, H, D, dev, (k_cache, v_cache))
+    T, B = q.shape[0], len(q_lens)
+    window, first = _visible(window, first)
+    M = block_tables.shape[1] if block_tables.dim() == 2 else 0
+    tables = _indices("block_tables", block_tables, (B, M), dev)
+    cu, lens = _indices("cu_q", cu_q, (B + 1,), dev), _indices("seq_lens", seq_lens, (B,), dev)
+    if len(kv_lens) != B or any(not 0 <= n <= k <= M * bs for n, k in zip(q_lens, kv_lens)) or sum(q_lens) > T:
+        raise ValueError(f"{B} portions of together {sum(q_lens)} tokens for {T} rows: every one takes the last places of "
+                         f"its keys, of which a table holds {M * bs}")
+    G = Hq // H
+    # requests one behind the other that take the same way; where the ways change often, one for all
+    few = [n * G <= SCALED_ROWS or D == 256 for n in q_lens]
+    runs = [0] + [b for b in range(1, B) if few[b] != few[b - 1]] + [B]
+    if len(runs) > 5:
+        few, runs = [D == 256] * B, [0, B]
+    for lo, hi in zip(runs, runs[1:]):
+        if lo == hi:
+            continue
+        if few[lo]:
+            max_q, seen = max(q_lens[lo:hi]), max(kv_lens[lo:hi])
+            if max_q == 0:
+                continue
+            if window:
+                seen = min(seen, window + max_q + first)
+            splits = block_scaled_splits(hi - lo, H * -(-max_q * G // 32), seen)
+            _scaled_rows(q, pq, ldq, out, po, ldo, k_cache, v_cache, k_scale, v_scale, cu + 4 * lo, lens + 4 * lo,
+                         tables + 4 * lo * M, hi - lo, M, max_q, scale, window, first, min(splits, 8), None, shape)
+            continue
+        tiles = [_expanded_tiles(n, k, window, first) for n, k in zip(q_lens[lo:hi], kv_lens[lo:hi])]
+        while lo < hi:
+            n, count = 1, tiles[0]
+            while lo + n < hi and (count + tiles[n]) * 128 <= SCALED_EXPANDED_KEYS:
+                count += tiles[n]
+                n += 1
+            if count:
+                width = -(-max(kv_lens[lo:lo + n]) // 128)
+                keys, values = torch.empty((2, count * 128, H * D), dtype=q.dtype, device=q.device)
+                table = torch.empty((n, width), dtype=torch.int32, device=q.device)
+                at = cu + 4 * lo, lens + 4 * lo
+                _call_on(dev, "b200_block_scaled_expand", _SCALED_EXPAND.pack(
+                    k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), keys.data_ptr(),
+                    values.data_ptr(), table.data_ptr(), *at, tables + 4 * lo * M, row, n, H, D, bs, M, nb, width, count,
+                    window, first, int8, DTYPE_CODE[q.dtype]))
+                _call_on(dev, "b200_fmha_expanded", _EXPANDED_CALL.pack(
+                    pq, po, keys.data_ptr(), values.data_ptr(), *at, table.data_ptr(), ldq, ldo, scale, T, n, Hq, H, D,
+                    count, width, sum(-(-m // 128) for m in q_lens[lo:lo + n]), window, first, DTYPE_CODE[q.dtype]))
+            tiles = tiles[n:]
+            lo += n
+    return out
+
+
+class CachePages:
+    """Blocks of several tensors that belong together, keys and values of a cache's layers and their scales: copied and
+    forked in one launch.  ``tensors``: contiguous, blocks along the first dimension, tokens of a block along the second where
+    there are three or more (``[blocks, block size, ...]``); entries of ``[blocks, width]`` belong to the block as a whole."""
+
+    def __init__(self, tensors: Sequence[torch.Tensor], block_size: int):
+        if not tensors or block_size <= 0:
+            raise ValueError("tensors of blocks, and the tokens of a block, are wanted")
+        self.tensors, self.block_size = list(tensors), int(block_size)
+        self.num_blocks, self.device = tensors[0].shape[0] if tensors[0].dim() else 0, tensors[0].device
+        planes = []
+        for t in self.tensors:
+            if t.dim() < 1 or t.shape[0] != self.num_blocks or not t.is_contiguous() or t.device != self.device \
+                    or not t.is_cuda:
+                raise ValueError(f"contiguous tensors of {self.num_blocks} blocks on one GPU are wanted, got shape "
+                                 f"{tuple(t.shape)}, strides {tuple(t.stride())} on {t.device}")
+            if t.dim() >= 3 and t.shape[1] != block_size:
+                raise ValueError(f"blocks of {t.shape[1]} tokens, not {block_size}")
+            size = t.numel() // max(1, self.num_blocks) * t.element_size()
+            planes.append((t.data_ptr(), size, size // block_size if t.dim() >= 3 else 0))
+        self._largest = max(size for _, size, _ in planes)
+        self._planes = torch.tensor(planes, dtype=torch.int64, device=self.device)
+
+    def copy(self, mapping: torch.Tensor) -> None:
+        """Blocks ``mapping[:, 0]`` to blocks ``mapping[:, 1]`` (int64 ``[n, 2]``; -1 in either place: none).  No block is
+        written twice, and none is both read and written."""
+        dev = self._planes.get_device()
+        pairs = _indices("mapping", mapping, (mapping.shape[0] if mapping.dim() else 0, 2), dev, torch.int64)
+        if mapping.shape[0] and self.num_blocks:
+            _call_on(dev, "b200_cache_pages", _PAGES_CALL.pack(
+                self._planes.data_ptr(), pairs, 0, 0, 0, 0, 0, self._largest, len(self.tensors), self.num_blocks,
+                mapping.shape[0], 0, 0, self.block_size))
+
+    def fork(self, block_tables: torch.Tensor, seq_lens: torch.Tensor, parents: torch.Tensor, fresh: torch.Tensor
+             ) -> torch.Tensor:
+        """Block tables of requests that go on from others, ``[n, blocks]``: row i is that of request ``parents[i]`` (of
+        ``block_tables [B, blocks]``; -1: zeros), whose blocks are shared.  The one that takes its next token becomes
+        ``fresh[i]``, with copies of the tokens that it holds already (of ``seq_lens [B]``); -1: it stays, for the one
+        request that goes on in its parent's place.  All int32.  Fresh blocks are in no table and differ."""
+        dev = self._planes.get_device()
+        B, M = block_tables.shape if block_tables.dim() == 2 else (0, 0)
+        n = parents.shape[0] if parents.dim() else 0
+        args = (_indices("block_tables", block_tables, (B, M), dev), _indices("seq_lens", seq_lens, (B,), dev),
+                _indices("parents", parents, (n,), dev), _indices("fresh", fresh, (n,), dev))
+        out = torch.empty((n, M), dtype=torch.int32, device=self.device)
+        if n and M:
+            _call_on(dev, "b200_cache_pages", _PAGES_CALL.pack(
+                self._planes.data_ptr(), 0, *args, out.data_ptr(), self._largest, len(self.tensors), self.num_blocks, n, M,
+                B, self.block_size))
+        return out
+
+
 def merge_attn_states(p_out, p_lse, s_out, s_lse, want_lse: bool = True):
     T, H, Dv = p_out.shape
     out = torch.empty_like(p_out)

@@ -343,6 +343,81 @@ def swap_blocks(src: torch.Tensor, dst: torch.Tensor, mapping: torch.Tensor) -> 
 
 
 # ---------------------------------------------------------------------------
+# a cache in 8 bits with a scale for each block and head
+# ---------------------------------------------------------------------------
+def block_scale(top: torch.Tensor, int8: bool) -> torch.Tensor:
+    """The least power of two (2^-100 .. 2^121), fp32, whose largest code reaches ``top``."""
+    m, e = torch.frexp(top.float())                       # top = m 2^e, m in [0.5, 1)
+    e = e - 7 + (m > 127 / 128).int() if int8 else e - 9 + (m > 448 / 512).int()
+    return (torch.where(top > 0, e, -100).clamp(-100, 121) + 127 << 23).to(torch.int32).view(torch.float32)
+
+
+def block_codes(x: torch.Tensor, scale: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
+    """``x / scale`` as codes, ties to even; NaN is the code 0."""
+    top = 127.0 if dtype == torch.int8 else FP8_MAX
+    y = x.float() / scale
+    y = torch.where(torch.isnan(y), 0.0, y).clamp(-top, top)
+    return (torch.round(y) if dtype == torch.int8 else y).to(dtype)
+
+
+def block_scaled_cache(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                       k_scale: torch.Tensor, v_scale: torch.Tensor, slot_mapping: torch.Tensor) -> None:
+    """See ``ops.cuda.block_scaled_cache``."""
+    nb, bs, H, D = k_cache.shape
+    slots = slot_mapping.tolist()
+    t = 0
+    while t < len(slots):
+        n = 1
+        while slots[t] >= 0 and t + n < len(slots) and slots[t + n] >= 0 and slots[t + n] // bs == slots[t] // bs:
+            n += 1
+        if slots[t] >= 0:
+            page, off = divmod(slots[t], bs)
+            at = torch.tensor([s % bs for s in slots[t:t + n]], device=k.device)
+            for x, cache, scale in ((k, k_cache, k_scale), (v, v_cache, v_scale)):
+                rows = x[t:t + n].float().reshape(n, H, D)
+                need = block_scale(torch.where(torch.isfinite(rows), rows.abs(), 0.0).amax((0, 2)),
+                                   cache.dtype == torch.int8)
+                if off:
+                    old = scale[page].clone()
+                    need = torch.where(old > need, old, need)
+                    again = block_codes(cache[page, :off].float() * old[:, None], need[:, None], cache.dtype)
+                    cache[page, :off].view(torch.uint8).copy_(again.view(torch.uint8))
+                cache[page].view(torch.uint8)[at] = block_codes(rows, need[:, None], cache.dtype).view(torch.uint8)
+                scale[page] = need
+        t += n
+
+
+def block_scaled_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor,
+                           v_scale: torch.Tensor, block_tables: torch.Tensor, cu_q: torch.Tensor,
+                           seq_lens: torch.Tensor, scale: float, window: int = 0, first: int = 0) -> torch.Tensor:
+    """See ``ops.cuda.block_scaled_prefill`` (one token per request: ``block_scaled_decode``)."""
+    kv = [(c.float() * s[:, None, :, None]) for c, s in ((k_cache, k_scale), (v_cache, v_scale))]
+    return varlen_prefill_attention(q, *kv, block_tables, cu_q, seq_lens, scale, window=window, first=first)
+
+
+def fork_blocks(caches: Sequence[torch.Tensor], block_size: int, block_tables: torch.Tensor, seq_lens: torch.Tensor,
+                parents: torch.Tensor, fresh: torch.Tensor) -> torch.Tensor:
+    """See ``ops.cuda.CachePages.fork``."""
+    out = torch.zeros(parents.shape[0], block_tables.shape[1], dtype=torch.int32, device=block_tables.device)
+    for i, (p, f) in enumerate(zip(parents.tolist(), fresh.tolist())):
+        if p < 0:
+            continue
+        out[i] = block_tables[p]
+        last, used = divmod(int(seq_lens[p]), block_size)
+        if f < 0 or last >= out.shape[1]:
+            continue
+        src = int(out[i, last])
+        out[i, last] = f
+        if used:
+            for c in caches:
+                if c.dim() >= 3:
+                    c[f, :used].view(torch.uint8).copy_(c[src, :used].view(torch.uint8))
+                else:
+                    c[f] = c[src]
+    return out
+
+
+# ---------------------------------------------------------------------------
 # attention
 # ---------------------------------------------------------------------------
 def _gather_kv(k_cache: torch.Tensor, v_cache: torch.Tensor, block_table_row: torch.Tensor,
@@ -390,10 +465,12 @@ def paged_attention_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torc
 def varlen_prefill_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
                              block_tables: torch.Tensor, cu_q: torch.Tensor,
                              seq_lens: torch.Tensor, scale: float, causal: bool = True,
-                             window: int = 0, return_lse: bool = False, alibi_slopes=None):
+                             window: int = 0, return_lse: bool = False, alibi_slopes=None,
+                             first: int = 0):
     """Attention of the new tokens of each sequence (``cu_q`` offsets into q
     ``[T, Hq, D]``) over all ``seq_lens[b]`` cached tokens, causal with respect to
-    absolute positions (csrc/src/context_attention_forward.cpp:49)."""
+    absolute positions (csrc/src/context_attention_forward.cpp:49).  ``first``: so many first
+    tokens of a sequence stay visible beside the window."""
     T, Hq, D = q.shape
     Hkv = k_cache.shape[2]
     G = Hq // Hkv
@@ -417,7 +494,7 @@ def varlen_prefill_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: to
         if causal:
             mask &= kpos <= qpos
         if window > 0:
-            mask &= kpos > qpos - window
+            mask &= (kpos > qpos - window) | (kpos < first)
         s = s.masked_fill(~mask[None], float("-inf"))
         l = torch.logsumexp(s, dim=-1)
         p = torch.exp(s - l[..., None])
