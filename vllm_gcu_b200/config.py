@@ -145,6 +145,7 @@ class ModelConfig:
     qk_norm: bool = False                  # per-head RMSNorm on q and k (Qwen3)
     sandwich_norm: bool = False            # GLM-4-0414: extra post-attn / post-mlp norms
     sliding_window: int = 0
+    sliding_window_first: int = 0          # first tokens of a request that stay visible beside the window
     dtype: torch.dtype = torch.bfloat16
     # MoE
     num_experts: int = 0
@@ -170,7 +171,7 @@ class ModelConfig:
     # quantisation (HF quantization_config / quantize_config.json, see layers/quant)
     quantization: Optional[str] = None
     quant_config: Optional[dict] = None
-    kv_cache_dtype: str = "auto"
+    kv_cache_dtype: str = "auto"           # fp8, int8; fp8_block, int8_block: a scale for each block and head
     # designs described layer by layer (None: every layer has the sizes above)
     layer_specs: Optional[tuple[LayerSpec, ...]] = None
     residual_alpha: float = 1.0            # norm after the sum: norm(alpha * x + sublayer(x))
@@ -232,7 +233,7 @@ class ModelConfig:
         return (layer_idx + 1) % step == 0
 
     def kv_bytes_per_token(self, tp_size: int = 1) -> int:
-        es = 1 if self.kv_cache_dtype.startswith("fp8") or self.kv_cache_dtype == "int8" else \
+        es = 1 if self.kv_cache_dtype.startswith(("fp8", "int8")) else \
             torch.empty((), dtype=self.dtype).element_size()
         if self.layer_specs is not None:
             return sum(self.layer_specs[i].cached_per_token for i, _ in self.layer_runs) * es

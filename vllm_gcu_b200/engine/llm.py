@@ -294,6 +294,8 @@ class LLMEngine:
         if "layer_shapes" in self.model.kv_cache_spec():
             raise ValueError(f"the caches of {self.cfg.model.architecture} differ from layer to "
                              "layer, which the connector does not ship")
+        if any(not isinstance(c, torch.Tensor) for c in self.runner.kv_caches):
+            raise ValueError("an 8-bit cache with scales for each block, which the connector does not ship")
         self.disagg = DisaggCoordinator(self, connector, recv_timeout_s)
         self.scheduler.on_free = self.disagg.before_free
         return self.disagg

@@ -27,7 +27,7 @@ import numpy as np
 import torch
 
 from ..config import EngineConfig
-from ..layers.attention import AttentionMetadata
+from ..layers.attention import AttentionMetadata, BlockScaledCache
 from ..layers.sampler import RowParallelSampler, Sampler, SamplingTensors
 from ..ops import _native
 from .scheduler import ScheduledRequest, SchedulerOutput
@@ -231,6 +231,8 @@ class ModelRunner:
                 self.cfg.parallel.tensor_parallel_size) * self.block_size
             bytes_per_block = bytes_per_block * self.model.num_local_layers \
                 // max(1, self.cfg.model.num_hidden_layers)
+            if self.is_cuda and self._block_scaled(spec):
+                bytes_per_block += spec["layers"] * 2 * 4 * spec["kv_heads"]
         if not self.is_cuda:
             return max(64, min(4096, (1 << 28) // max(1, bytes_per_block)))
         torch.cuda.synchronize()
@@ -244,6 +246,10 @@ class ModelRunner:
         state_bytes = self.max_seqs * sum(
             math.prod(shape) * torch.empty((), dtype=dt).element_size()
             for layer in spec.get("request_state", ()) for shape, dt in layer.values())
+        if self._block_scaled(spec):       # keys and values of a prompt, expanded to 16 bits
+            from ..ops import cuda as C
+            state_bytes += 4 * spec["kv_heads"] * spec["head_dim"] * max(C.SCALED_EXPANDED_KEYS,
+                                                                         self.cfg.scheduler.max_model_len)
         budget = int(total * cc.gpu_memory_utilization) - weights_and_act - state_bytes
         # the dummy forward is gone but other processes may hold memory too
         budget = min(budget, int(torch.cuda.mem_get_info()[0] * 0.97) - state_bytes)
@@ -263,6 +269,18 @@ class ModelRunner:
             pass
         return n
 
+    def _block_scaled(self, spec: dict) -> bool:
+        """Whether the caches are held in 8 bits with a scale for each block and head."""
+        return self.cfg.model.kv_cache_dtype in ("fp8_block", "int8_block") and spec["type"] == "gqa"
+
+    def _cache_tensors(self) -> list[torch.Tensor]:
+        """Tensors that a block's content lies in: ``[2, blocks, ...]`` with more than three dimensions, else
+        ``[blocks, ...]``."""
+        out: list[torch.Tensor] = []
+        for c in self.kv_caches:
+            out += [c.codes, *c.scales] if isinstance(c, BlockScaledCache) else [c]
+        return out + self.block_state
+
     def init_kv_cache(self, num_blocks: int) -> None:
         spec = self.model.kv_cache_spec()
         mc = self.cfg.model
@@ -273,8 +291,20 @@ class ModelRunner:
             # the way into shared memory.  The CPU path keeps the model dtype.
             if kvd.startswith("fp8"):
                 dt = torch.float8_e4m3fn
-            elif kvd == "int8":
+            elif kvd.startswith("int8"):
                 dt = torch.int8
+        if mc.sliding_window_first and self.is_cuda and not self._block_scaled(spec):
+            raise ValueError("first tokens that stay visible beside a sliding window need "
+                             "kv_cache_dtype fp8_block or int8_block")
+        if kvd.endswith("_block") and self.is_cuda and spec["type"] == "gqa" and not self._block_scaled(spec):
+            raise ValueError(f"kv_cache_dtype {mc.kv_cache_dtype!r}: fp8_block or int8_block")
+        scaled = self.is_cuda and self._block_scaled(spec)
+
+        def kv(blocks: int, heads: int, dim: int):
+            if scaled:
+                return BlockScaledCache.zeros(blocks, self.block_size, heads, dim, dt, self.device)
+            return torch.zeros(2, blocks, self.block_size, heads, dim, dtype=dt, device=self.device)
+
         if spec["type"] == "mla":
             widths = spec.get("widths") or [spec["width"]] * spec["layers"]
             self.kv_caches = [torch.zeros(num_blocks, self.block_size, w, dtype=dt,
@@ -289,8 +319,7 @@ class ModelRunner:
                               new(2, num_blocks if s else 0, self.block_size, *(s or (1, 1)))
                               for s in spec["layer_shapes"]]
         else:
-            self.kv_caches = [torch.zeros(2, num_blocks, self.block_size, spec["kv_heads"],
-                                          spec["head_dim"], dtype=dt, device=self.device)
+            self.kv_caches = [kv(num_blocks, spec["kv_heads"], spec["head_dim"])
                               for _ in range(spec["layers"])]
         # recurrent rows that live with the cache blocks (token shift): one per block and layer
         self.block_state = [torch.zeros(num_blocks, w, dtype=torch.float32, device=self.device)
@@ -307,8 +336,7 @@ class ModelRunner:
                                                    dtype=dt, device=self.device)
                                        for _ in range(ds["layers"])]
             else:
-                self.drafter_caches = [torch.zeros(2, num_blocks, self.block_size, ds["kv_heads"],
-                                                   ds["head_dim"], dtype=dt, device=self.device)
+                self.drafter_caches = [kv(num_blocks, ds["kv_heads"], ds["head_dim"])
                                        for _ in range(ds["layers"])]
         if self.is_cuda and spec["type"] in ("gqa", "layers"):
             Hq = spec.get("q_heads") or \
@@ -387,7 +415,7 @@ class ModelRunner:
         if getattr(self, "cpu_caches", None) is None:
             pin = self.is_cuda
             self.cpu_caches = []
-            for c in self.kv_caches + self.block_state:
+            for c in self._cache_tensors():
                 shape = list(c.shape)
                 shape[0 if c.dim() <= 3 else 1] = n_cpu
                 self.cpu_caches.append(torch.zeros(shape, dtype=c.dtype, device="cpu",
@@ -396,7 +424,7 @@ class ModelRunner:
         swap = C.swap_blocks if self.is_cuda else ref.swap_blocks
         m_in = torch.tensor(so.swap_in, dtype=torch.int64).view(-1, 2)
         m_out = torch.tensor(so.swap_out, dtype=torch.int64).view(-1, 2)
-        for dev_c, cpu_c in zip(self.kv_caches + self.block_state, self.cpu_caches):
+        for dev_c, cpu_c in zip(self._cache_tensors(), self.cpu_caches):
             planes = [(dev_c, cpu_c)] if dev_c.dim() <= 3 else [(dev_c[0], cpu_c[0]),
                                                                 (dev_c[1], cpu_c[1])]
             for d, h in planes:
@@ -636,7 +664,8 @@ class ModelRunner:
         out_ids = self.sampled[cur]
         common_prefix = 0
         if (not use_graph and self.cascade_min_tokens > 0 and B >= 4 and not mm_step
-                and not self.max_spec and self.model.kv_cache_spec()["type"] == "gqa"):
+                and not self.max_spec and self.model.kv_cache_spec()["type"] == "gqa"
+                and not isinstance(self.kv_caches[0], BlockScaledCache)):
             nblk = int(starts.min()) // bs          # only tokens that are already in the cache
             if nblk * bs >= self.cascade_min_tokens:
                 same = (self.bt_host[rows, :nblk] == self.bt_host[rows[0], :nblk][None, :]).all(0)

@@ -676,7 +676,8 @@ def add_engine_arguments(ap: argparse.ArgumentParser) -> None:
     ap.add_argument("--enforce-eager", action="store_true")
     ap.add_argument("--device", default="auto")
     ap.add_argument("--dtype", default=None)
-    ap.add_argument("--kv-cache-dtype", default="auto", choices=["auto", "fp8", "int8"])
+    ap.add_argument("--kv-cache-dtype", default="auto", choices=["auto", "fp8", "int8", "fp8_block", "int8_block"],
+                    help="*_block: a scale for each block of tokens and head")
     ap.add_argument("--quantization", default=None,
                     help="for architecture presets with random weights: fp8, fp8_block, w8a8; "
                          "checkpoints carry their own quantization_config")

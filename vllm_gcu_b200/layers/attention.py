@@ -6,7 +6,8 @@ scheduled token (prefill chunks, speculative verification).  The reference order
 its MLA batches the same way (vllm_gcu/attention/backends/mla_v1_fusion.py:126-138).
 
 KV cache of a layer: one tensor ``[2, num_blocks, block_size, kv_heads, head_dim]``
-(the "flash" layout of csrc/src/reshape_and_cache_flash.cpp:23).
+(the "flash" layout of csrc/src/reshape_and_cache_flash.cpp:23), or a ``BlockScaledCache``: the same
+in 8 bits with a scale for each block and head.
 
 GPU path per layer: one fused RoPE + cache-write kernel, then the split-KV decode
 kernel on the decode rows and the varlen paged-prefill kernel on the rest.  CPU path:
@@ -111,6 +112,27 @@ def allocate_kv_cache(num_layers: int, num_blocks: int, block_size: int, kv_head
             for _ in range(num_layers)]
 
 
+@dataclass
+class BlockScaledCache:
+    """Cache of a layer in 8 bits with a scale for each block and head."""
+    codes: torch.Tensor                  # [2, blocks, block size, kv heads, head dim], fp8 e4m3 or int8
+    scales: torch.Tensor                 # [2, blocks, kv heads] fp32
+
+    @classmethod
+    def zeros(cls, num_blocks: int, block_size: int, kv_heads: int, head_dim: int, dtype: torch.dtype, device
+              ) -> "BlockScaledCache":
+        return cls(torch.zeros(2, num_blocks, block_size, kv_heads, head_dim, dtype=dtype, device=device),
+                   torch.zeros(2, num_blocks, kv_heads, dtype=torch.float32, device=device))
+
+    def planes(self) -> list[torch.Tensor]:
+        """Tensors whose first dimension is the block (``ops.cuda.CachePages``)."""
+        return [*self.codes, *self.scales]
+
+    def parts(self) -> tuple[torch.Tensor, ...]:
+        """Keys, values and their scales, as the operators take them."""
+        return self.codes[0], self.codes[1], self.scales[0], self.scales[1]
+
+
 def alibi_slopes(num_heads: int) -> torch.Tensor:
     """ALiBi slopes of all heads, fp32 ``[num_heads]``: a geometric sequence 2^(-8 i / n) for the
     largest power of two n <= num_heads, then every other term of the sequence for 2n (the
@@ -132,7 +154,7 @@ class PagedAttention(nn.Module):
     def __init__(self, num_heads: int, num_kv_heads: int, head_dim: int, scale: float,
                  rotary: Optional[RotaryEmbedding], q_norm: Optional[RMSNorm] = None,
                  k_norm: Optional[RMSNorm] = None, sliding_window: int = 0,
-                 alibi: Optional[torch.Tensor] = None):
+                 alibi: Optional[torch.Tensor] = None, window_first: int = 0):
         super().__init__()
         # ALiBi slopes of this rank's heads (fp32 [num_heads]); the kernels add
         # slope * (key position - query position) to the scores
@@ -143,6 +165,8 @@ class PagedAttention(nn.Module):
         self.rotary = rotary
         self.q_norm, self.k_norm = q_norm, k_norm
         self.window = sliding_window
+        # first tokens of a request that stay visible beside the window
+        self.window_first = window_first if sliding_window else 0
         self.mrope_section: Optional[list[int]] = None     # set by M-RoPE models (Qwen2.5-VL)
         # per-tensor scales of an fp8 / int8 KV cache (value = stored * scale); checkpoints may
         # provide them (``load_kv_cache_scales`` of the reference's quantised models,
@@ -160,6 +184,8 @@ class PagedAttention(nn.Module):
         if kv_cache is None or md.is_dummy:
             # memory profile / keep-alive step of an idle rank: no cache, no attention
             return torch.zeros((T, Hq * D), dtype=qkv.dtype, device=qkv.device)
+        if isinstance(kv_cache, BlockScaledCache):
+            return self._forward_scaled(q, k, v, kv_cache, md)
         k_cache, v_cache = kv_cache[0], kv_cache[1]
         if ops.use_native(qkv) and qkv.dtype in (torch.bfloat16, torch.float16):
             return self._forward_cuda(q, k, v, k_cache, v_cache, md)
@@ -189,6 +215,50 @@ class PagedAttention(nn.Module):
                 rot.cos_sin_cache.float(), md.mrope_positions[:, :T], self.mrope_section)
             md.mrope_arange = torch.arange(T, device=md.mrope_cos_sin.device)
         return md.mrope_arange, md.mrope_cos_sin
+
+    # -- a cache in 8 bits with scales -----------------------------------------
+    def _forward_scaled(self, q, k, v, cache: BlockScaledCache, md: AttentionMetadata) -> torch.Tensor:
+        T = q.shape[0]
+        D, Hq, nd = self.head_dim, self.num_heads, md.num_decode_tokens
+        parts, lo, B = cache.parts(), md.num_decodes, md.num_decodes + md.num_prefills
+        if self.alibi is not None:
+            raise NotImplementedError("ALiBi attention over an 8-bit KV cache")
+        rope_pos, rope_table = self._rope_inputs(md, T)
+        if not (ops.use_native(q) and q.dtype in (torch.bfloat16, torch.float16)):
+            q, k = self._head_norms(q, k)
+            if self.rotary is not None:
+                q, k = ref.rotary_embedding(rope_pos, q, k, D, rope_table, self.rotary.is_neox)
+            ref.block_scaled_cache(k, v, *parts, md.slot_mapping)
+            q_lens = torch.tensor([0] + [1] * lo + list(md.q_lens_cpu[lo:B]))
+            cu = q_lens.cumsum(0).to(torch.int32)
+            out = torch.zeros((T, Hq * D), dtype=q.dtype, device=q.device)
+            n = int(cu[-1])
+            out[:n] = ref.block_scaled_attention(
+                q[:n].reshape(n, Hq, D), *parts, md.block_tables[:B], cu, md.seq_lens[:B], self.scale,
+                window=self.window, first=self.window_first).reshape(n, Hq * D)
+            return out
+        qn, kn = self.q_norm, self.k_norm
+        rope = (rope_pos, rope_table, self.rotary.is_neox if self.rotary is not None else True, D)
+        fused = (rope_table is not None and qn is not None and type(qn) is RMSNorm and type(kn) is RMSNorm
+                 and qn.eps == kn.eps and qn.weight.dtype == q.dtype and kn.weight.dtype == q.dtype
+                 and C.rope_cache_flash(q, k, None, *rope, norms=(qn.weight, kn.weight, qn.eps)))
+        if not fused:
+            q, k = self._head_norms(q, k)
+            if rope_table is not None:
+                C.rope_cache_flash(q, k, None, *rope)
+        C.block_scaled_cache(k, v, *parts, md.slot_mapping)
+        # (rows of no request, the padding of a step, are zeros)
+        n = nd + sum(md.q_lens_cpu[lo:B])
+        out = q.new_empty((T, Hq * D)) if n == T else q.new_zeros((T, Hq * D))
+        if nd > 0:
+            C.block_scaled_decode(q[:nd].view(nd, Hq, D), *parts, md.block_tables[:nd], md.seq_lens[:nd], self.scale,
+                                  out=out[:nd].view(nd, Hq, D), workspace=md.decode_workspace,
+                                  max_seq_len=md.max_seq_len, window=self.window, first=self.window_first)
+        if md.num_prefills > 0:
+            C.block_scaled_prefill(q[nd:].view(T - nd, Hq, D), *parts, md.block_tables[lo:B], md.cu_q_prefill,
+                                   md.seq_lens[lo:B], self.scale, md.q_lens_cpu[lo:B], md.seq_lens_cpu[lo:B],
+                                   out=out[nd:].view(T - nd, Hq, D), window=self.window, first=self.window_first)
+        return out
 
     # -- GPU -----------------------------------------------------------------
     def _forward_cuda(self, q, k, v, k_cache, v_cache, md: AttentionMetadata) -> torch.Tensor:
@@ -283,6 +353,7 @@ class PagedAttention(nn.Module):
             return out
         o = ref.varlen_prefill_attention(q[:n_real].reshape(n_real, Hq, D), k_cache, v_cache,
                                          md.block_tables[:B], cu, md.seq_lens[:B], self.scale,
-                                         window=self.window, alibi_slopes=self.alibi)
+                                         window=self.window, alibi_slopes=self.alibi,
+                                         first=self.window_first)
         out[:n_real] = o.reshape(n_real, Hq * D)
         return out
