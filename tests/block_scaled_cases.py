@@ -44,12 +44,13 @@ def random_codes(shape, codes, gen):
 
 
 def attention(q, cache, q_lens, scale, window=0, first=0):
-    """Definition in 64 bits: (outputs [T, Hq, D], sums of p |v| over sums of p, largest sums of |q k|) for the rows of the
-    requests, one behind the other."""
+    """Definition in 64 bits: (outputs [T, Hq, D], sums of p |v| over sums of p, largest sums of |q k|, largest share of a
+    key times its values' scale) for the rows of the requests, one behind the other."""
     q = q.double().cpu()
     codes, scales = cache.codes.cpu().float().double(), cache.scales.cpu().double()
     Hq, G = q.shape[1], q.shape[1] // cache.heads
     out, size, reach = torch.zeros_like(q), torch.zeros_like(q), torch.zeros(q.shape[0], Hq, dtype=torch.float64)
+    top = torch.zeros_like(reach)
     at = 0
     for r, n in enumerate(q_lens):
         length = cache.lens[r]
@@ -68,24 +69,31 @@ def attention(q, cache, q_lens, scale, window=0, first=0):
             p = torch.where(seen.any(-1)[:, None], p, 0.0)
             out[at:at + n] = (p @ v).transpose(0, 1)
             size[at:at + n] = (p @ v.abs()).transpose(0, 1)
+            unit = scales[1][pages].repeat_interleave(cache.block, 0)[:length].T.repeat_interleave(G, 0)
+            top[at:at + n] = (p * unit[:, None]).amax(-1).T
             reach[at:at + n] = ((rows.abs() @ k.abs().transpose(1, 2)) * scale).masked_fill(~seen, 0.0).amax(-1).T
         at += n
-    return out, size, reach
+    return out, size, reach, top
 
 
-def allowed(out, size, reach, dtype, p_type, keys, width):
+def allowed(out, size, reach, top, dtype, p_type, keys, width):
     """How far a kernel may be: half a step of the result's type; half a step of the probabilities' type each; scores in 32
     bits whose sum of ``width`` products and scale round by 2^-24 each (an error d of a score is one of 2 d of its
-    probability's share); sums of ``keys`` terms in 32 bits, truncated."""
+    probability's share); sums of ``keys`` terms in 32 bits, truncated.
+
+    Where the codes meet 8-bit parts of a probability times its block's scale, the last part ends at a fixed place behind
+    the largest of them, which is 1 or more: int8 digits of a multiple of 2^-26 are off by 2^-27; e4m3 parts of 64 times
+    the number by half of the smallest step 2^-9 with weight 2^-8, 2^-18, which is 2^-24 of the number.  Each of ``keys``
+    codes of at most 448 takes that part of ``top``.  (It shows where the keys that count have codes of 0.)"""
     p = torch.finfo(p_type).eps / 2 + 2 * (width + 8) * 2.0 ** -23 * reach[..., None] + (keys + 16) * 2.0 ** -22
-    return size * p + out.abs() * torch.finfo(dtype).eps / 2 * 1.01 + 1e-30 + torch.finfo(dtype).tiny
+    return size * p + keys * 448 * 2.0 ** -24 * top[..., None] + out.abs() * torch.finfo(dtype).eps / 2 * 1.01 + 1e-30 + torch.finfo(dtype).tiny
 
 
 def check(got, q, cache, q_lens, scale, window, first, p_type):
-    out, size, reach = attention(q, cache, q_lens, scale, window, first)
+    out, size, reach, top = attention(q, cache, q_lens, scale, window, first)
     n = sum(q_lens)
     far = (got[:n].double().cpu() - out[:n]).abs()
-    may = allowed(out, size, reach, got.dtype, p_type, max(cache.lens, default=0), cache.width)[:n]
+    may = allowed(out, size, reach, top, got.dtype, p_type, max(cache.lens, default=0), cache.width)[:n]
     assert torch.isfinite(got[:n]).all()
     worst = (far / may).max().item() if n else 0.0
     assert worst <= 1.0, worst

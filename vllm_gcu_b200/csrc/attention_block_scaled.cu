@@ -90,10 +90,11 @@ struct Place {
 template <int kRows>
 __device__ __forceinline__ Place place_of(const Args& a) {
   Place p;
-  p.b = blockIdx.x;
-  p.kvh = blockIdx.y / a.row_blocks;
+  // (the key heads of a request, whose rows lie side by side, run at the same time)
+  p.b = blockIdx.y;
+  p.kvh = blockIdx.x / a.row_blocks;
   p.G = a.Hq / a.Hkv;
-  p.row0 = blockIdx.y % a.row_blocks * kRows;
+  p.row0 = blockIdx.x % a.row_blocks * kRows;
   const int q_len = a.cu_q != nullptr ? a.cu_q[p.b + 1] - a.cu_q[p.b] : 1;
   p.q_start = a.cu_q != nullptr ? a.cu_q[p.b] : p.b;
   p.rows = q_len * p.G;
@@ -106,6 +107,69 @@ __device__ __forceinline__ Place place_of(const Args& a) {
   p.firsts = a.window > 0 ? min(p.lo_chunk, (a.first + kChunk - 1) / kChunk) : 0;
   p.chunks = p.row0 < p.rows && p.hi_pos >= 0 ? p.firsts + p.hi_pos / kChunk + 1 - p.lo_chunk : 0;
   return p;
+}
+
+// The splits of a cluster, each with its rows' log2 sums and outputs in shared memory: every CTA adds up a share of the
+// numbers.  All threads of the cluster call it.
+template <typename T, int HD>
+__device__ __forceinline__ void merge_cluster(const Args& a, const Place& p, int live, const float* part_lse,
+                                              const float* part_o) {
+  cluster_sync();
+  uint32_t rank;
+  asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
+  for (int idx = static_cast<int>(rank) * blockDim.x + threadIdx.x; idx < live * HD; idx += a.splits * blockDim.x) {
+    const int r = idx / HD, d = idx % HD;
+    float pl[8], po[8], M = -INFINITY, o = 0.0f, sum = 0.0f;
+#pragma unroll
+    for (int s = 0; s < 8; ++s) {
+      pl[s] = -INFINITY;
+      if (s >= a.splits) continue;
+      pl[s] = ld_peer(part_lse + r, s);
+      po[s] = ld_peer(part_o + idx, s);
+    }
+#pragma unroll
+    for (int s = 0; s < 8; ++s) M = fmaxf(M, pl[s]);
+#pragma unroll
+    for (int s = 0; s < 8; ++s) {
+      if (pl[s] == -INFINITY) continue;
+      const float w = exp2f(pl[s] - M);
+      sum += w;
+      o = fmaf(w, po[s], o);
+    }
+    const int row = p.row0 + r, token = p.q_start + row / p.G, head = p.kvh * p.G + row % p.G;
+    static_cast<T*>(a.out)[static_cast<long long>(token) * a.ldo + head * HD + d] =
+        from_f32<T>(sum == 0.0f ? 0.0f : o / sum);
+  }
+  cluster_sync();                   // nobody leaves while another CTA may still read its numbers
+}
+
+// Launch with the splits of a request and key head as a cluster, or as CTAs on their own.
+// (`done`: per device, whether the kernel has its shared memory)
+using Kernel = void (*)(CUtensorMap, CUtensorMap, Args);
+inline int launch_splits(Kernel kernel, bool (&done)[64], int threads, int smem, bool cluster, const Args& a,
+                         const CUtensorMap& tmK, const CUtensorMap& tmV, cudaStream_t s) {
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev >= 0 && dev < 64 && !done[dev]) {
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return launch_code(e);
+    done[dev] = true;
+  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(a.Hkv * a.row_blocks, a.B, a.splits);
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = 1;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = a.splits;
+  cfg.attrs = attr;
+  cfg.numAttrs = cluster ? 2 : 1;
+  return launch_code(cudaLaunchKernelEx(&cfg, kernel, tmK, tmV, a));
 }
 
 // Columns of a head's row that accumulator `nt` of lane column c (0 .. 7) holds
@@ -200,16 +264,17 @@ __global__ void __launch_bounds__(kGroups * 128 + 32)
     const int part = warp & 3;                       // chunk of a tile
     const int group = kGroups == 1 ? 0 : warp >> 2;  // rows
     // scales of this warp's chunk of 32 tiles, one a lane
+    // (a block that was never written has no scale: its values are zeros, its keys count all the same)
     auto scales_of = [&](int it, float& ks, float& vs) {
       const int c = c0 + (it + lane) * 4 + part;
       ks = 0.0f;
-      vs = 0.0f;
+      vs = power_of_two(kLowExponent);
       if (c < c1) {
         const int block = bt[first_token(c) / a.block_size];
         if (block >= 0 && block < a.num_blocks) {
           const long long at = static_cast<long long>(block) * a.Hkv + p.kvh;
           ks = a.ks[at];
-          vs = a.vs[at];
+          vs = fmaxf(a.vs[at], vs);
         } else {
           report_status(a.status, kStatusBounds, kKernelId, static_cast<unsigned>(p.b));
         }
@@ -269,8 +334,7 @@ __global__ void __launch_bounds__(kGroups * 128 + 32)
         if (it + 32 < ntiles) scales_of(it + 32, ks_next, vs_next);
       }
       const float ks = __shfl_sync(0xffffffffu, ks_now, it & 31);
-      // (a block that was never written has no scale: its values are zeros, its keys count all the same)
-      const float vs = fmaxf(__shfl_sync(0xffffffffu, vs_now, it & 31), power_of_two(kLowExponent));
+      const float vs = __shfl_sync(0xffffffffu, vs_now, it & 31);
       ok = mbar_wait_warp(&full_bar[stage], phase, a.status, kKernelId, 0x200u + stage, abort_flag);
       if (!ok) break;
       const int chunk = c0 + it * 4 + part;
@@ -338,7 +402,7 @@ __global__ void __launch_bounds__(kGroups * 128 + 32)
             }
           }
         }
-        const float unit = 1.0f / vs;
+        const float unit = __fdividef(1.0f, vs);
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
           const float m = m_run[r] == -INFINITY ? 0.0f : m_run[r];
@@ -459,35 +523,7 @@ __global__ void __launch_bounds__(kGroups * 128 + 32)
       }
     }
   }
-  if constexpr (kCluster) {
-    cluster_sync();
-    uint32_t rank;
-    asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
-    for (int idx = static_cast<int>(rank) * blockDim.x + threadIdx.x; idx < live * HD; idx += a.splits * blockDim.x) {
-      const int r = idx / HD, d = idx % HD;
-      float pl[8], po[8], M = -INFINITY, o = 0.0f, sum = 0.0f;
-#pragma unroll
-      for (int s = 0; s < 8; ++s) {
-        pl[s] = -INFINITY;
-        if (s >= a.splits) continue;
-        pl[s] = ld_peer(part_lse + r, s);
-        po[s] = ld_peer(part_o + idx, s);
-      }
-#pragma unroll
-      for (int s = 0; s < 8; ++s) M = fmaxf(M, pl[s]);
-#pragma unroll
-      for (int s = 0; s < 8; ++s) {
-        if (pl[s] == -INFINITY) continue;
-        const float w = exp2f(pl[s] - M);
-        sum += w;
-        o = fmaf(w, po[s], o);
-      }
-      const int row = p.row0 + r, token = p.q_start + row / p.G, head = p.kvh * p.G + row % p.G;
-      static_cast<T*>(a.out)[static_cast<long long>(token) * a.ldo + head * HD + d] =
-          from_f32<T>(sum == 0.0f ? 0.0f : o / sum);
-    }
-    cluster_sync();                 // nobody leaves while another CTA may still read its numbers
-  }
+  if constexpr (kCluster) merge_cluster<T, HD>(a, p, live, part_lse, part_o);
 }
 
 // Splits that are no cluster: a warp a row.
@@ -542,30 +578,8 @@ int launch_rows(const CUtensorMap& tmK, const CUtensorMap& tmV, const Args& a, c
   // (the merge's numbers lie where the stages were; the barriers behind the stages are not used any more by then)
   constexpr int kSmem = (kMerge > kRing ? kMerge : kRing) + 256 + 1024;
   static_assert(kSmem <= 232448, "exceeds the shared memory of one CTA");
-  auto kernel = rows_kernel<T, kInt8, HD, kGroups, kCluster>;
   static bool done[64] = {};
-  int dev = 0;
-  cudaGetDevice(&dev);
-  if (dev >= 0 && dev < 64 && !done[dev]) {
-    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
-    if (e != cudaSuccess) return launch_code(e);
-    done[dev] = true;
-  }
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(a.B, a.Hkv * a.row_blocks, a.splits);
-  cfg.blockDim = dim3(kGroups * 128 + 32);
-  cfg.dynamicSmemBytes = kSmem;
-  cfg.stream = s;
-  cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  attr[1].id = cudaLaunchAttributeClusterDimension;
-  attr[1].val.clusterDim.x = 1;
-  attr[1].val.clusterDim.y = 1;
-  attr[1].val.clusterDim.z = a.splits;
-  cfg.attrs = attr;
-  cfg.numAttrs = kCluster ? 2 : 1;
-  return launch_code(cudaLaunchKernelEx(&cfg, kernel, tmK, tmV, a));
+  return launch_splits(rows_kernel<T, kInt8, HD, kGroups, kCluster>, done, kGroups * 128 + 32, kSmem, kCluster, a, tmK, tmV, s);
 }
 
 template <typename T, bool kInt8, int HD>
@@ -580,12 +594,35 @@ int launch_any(const CUtensorMap& tmK, const CUtensorMap& tmV, const Args& a, in
   return launch_overlapped(merge_rows_kernel<T, HD>, dim3((total + 3) / 4), dim3(128), 0, s, a, total);
 }
 
+}  // namespace rows8
+}  // namespace b200
+
+#include "attention_block_scaled_tc.cuh"
+
+namespace b200 {
+namespace rows8 {
+
+template <typename T, bool kInt8, int kR>
+int launch_tc_any(const CUtensorMap& tmK, const CUtensorMap& tmV, const Args& a, int T_rows, cudaStream_t s) {
+  if (a.splits > 1 && a.splits <= 8) return launch_tc<T, kInt8, kR, true>(tmK, tmV, a, s);
+  const int e = launch_tc<T, kInt8, kR, false>(tmK, tmV, a, s);
+  if (e != 0 || a.splits <= 1) return e;
+  const int total = T_rows * a.Hq;
+  return launch_overlapped(merge_rows_kernel<T, 128>, dim3((total + 3) / 4), dim3(128), 0, s, a, total);
+}
+
 template <typename T, bool kInt8>
-int launch_width(int D, const CUtensorMap& tmK, const CUtensorMap& tmV, const Args& a, int T_rows, bool two, cudaStream_t s) {
+int launch_width(int D, const CUtensorMap& tmK, const CUtensorMap& tmV, const Args& a, int T_rows, int rows, cudaStream_t s) {
   switch (D) {
-    case 64: return launch_any<T, kInt8, 64>(tmK, tmV, a, T_rows, two, s);
-    case 128: return launch_any<T, kInt8, 128>(tmK, tmV, a, T_rows, two, s);
-    case 256: return launch_any<T, kInt8, 256>(tmK, tmV, a, T_rows, two, s);
+    case 64: return launch_any<T, kInt8, 64>(tmK, tmV, a, T_rows, rows > 16, s);
+    case 256: return launch_any<T, kInt8, 256>(tmK, tmV, a, T_rows, false, s);
+    case 128:
+      switch (rows) {
+        case 4: return launch_tc_any<T, kInt8, 4>(tmK, tmV, a, T_rows, s);
+        case 8: return launch_tc_any<T, kInt8, 8>(tmK, tmV, a, T_rows, s);
+        case 16: return launch_tc_any<T, kInt8, 16>(tmK, tmV, a, T_rows, s);
+        case 32: return launch_tc_any<T, kInt8, 32>(tmK, tmV, a, T_rows, s);
+      }
   }
   return -8;
 }
@@ -611,23 +648,23 @@ B200_API int b200_block_scaled_rows(const void* call, void* stream) {
   if (r != 0) return r < 0 ? -6 : r;
   const int group = k.Hq / k.Hkv;
   const long long all = static_cast<long long>(k.max_q) * group;
-  const bool two = all > 16 && k.D != 256;
+  // rows of a CTA
+  const int per = k.D == 128 ? (all <= 4 ? 4 : all <= 8 ? 8 : all <= 16 ? 16 : 32) : k.D == 64 && all > 16 ? 32 : 16;
   Args a;
   a.q = k.q; a.out = k.out; a.tmp_out = k.tmp_out; a.tmp_lse = k.tmp_lse; a.ks = k.ks; a.vs = k.vs; a.cu_q = k.cu_q;
   a.seq_lens = k.seq_lens; a.block_tables = k.block_tables; a.ldq = k.ldq; a.ldo = k.ldo; a.B = k.B; a.Hq = k.Hq;
   a.Hkv = k.Hkv; a.splits = k.splits; a.max_blocks = k.max_blocks; a.block_size = k.block_size;
   a.num_blocks = k.num_blocks; a.window = k.window; a.first = k.first; a.scale = k.scale;
-  const int per = two ? 32 : 16;
   const long long row_blocks = (all + per - 1) / per;
-  if (row_blocks * k.Hkv > 65535) return -2;
+  if (k.B > 65535) return -2;
   a.row_blocks = static_cast<int>(row_blocks);
   a.status = status_ptr();
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (k.dtype == 0)
-    return k.int8 ? launch_width<__nv_bfloat16, true>(k.D, tmK, tmV, a, k.T, two, s)
-                  : launch_width<__nv_bfloat16, false>(k.D, tmK, tmV, a, k.T, two, s);
+    return k.int8 ? launch_width<__nv_bfloat16, true>(k.D, tmK, tmV, a, k.T, per, s)
+                  : launch_width<__nv_bfloat16, false>(k.D, tmK, tmV, a, k.T, per, s);
   if (k.dtype == 1)
-    return k.int8 ? launch_width<__half, true>(k.D, tmK, tmV, a, k.T, two, s)
-                  : launch_width<__half, false>(k.D, tmK, tmV, a, k.T, two, s);
+    return k.int8 ? launch_width<__half, true>(k.D, tmK, tmV, a, k.T, per, s)
+                  : launch_width<__half, false>(k.D, tmK, tmV, a, k.T, per, s);
   return -8;
 }

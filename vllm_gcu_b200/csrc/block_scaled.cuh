@@ -68,10 +68,14 @@ __device__ __forceinline__ void unpack4(uint32_t w, uint32_t& lo, uint32_t& hi) 
     lo = *reinterpret_cast<const uint32_t*>(&a);
     hi = *reinterpret_cast<const uint32_t*>(&b);
   } else {
-    const __half2_raw a = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(w & 0xffffu), __NV_E4M3);
-    const __half2_raw b = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(w >> 16), __NV_E4M3);
-    lo = static_cast<uint32_t>(a.x) | static_cast<uint32_t>(a.y) << 16;
-    hi = static_cast<uint32_t>(b.x) | static_cast<uint32_t>(b.y) << 16;
+    asm("{\n\t"
+        ".reg .b16 l, h;\n\t"
+        "mov.b32 {l, h}, %2;\n\t"
+        "cvt.rn.f16x2.e4m3x2 %0, l;\n\t"
+        "cvt.rn.f16x2.e4m3x2 %1, h;\n\t"
+        "}"
+        : "=r"(lo), "=r"(hi)
+        : "r"(w));
   }
 }
 __device__ __forceinline__ float2 half_pair(uint32_t w) {
