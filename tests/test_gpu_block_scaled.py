@@ -271,18 +271,15 @@ def test_rows_that_are_no_numbers_stay_alone():
     assert torch.isfinite(want).all()
 
 
-def test_workspace_and_its_limits():
-    cache = K.Cache(K.INT8, 2, 128, 16, [5000, 3001]).to("cuda")
-    q = torch.randn(2, 8, 128, device="cuda", dtype=K.F16)
-    args = (q, *cache.parts(), cache.tables, cache.seq_lens, 0.09)
-    ws = torch.empty(2 * 8 * 16 * 128, device="cuda"), torch.empty(2 * 8 * 16, device="cuda")
-    assert torch.equal(C.block_scaled_decode(*args, num_splits=16, workspace=ws), C.block_scaled_decode(*args, num_splits=16))
-    with pytest.raises(ValueError, match="workspace"):
-        C.block_scaled_decode(*args, num_splits=17, workspace=ws)
-    with pytest.raises(ValueError, match="workspace"):
-        C.block_scaled_decode(*args, num_splits=12, workspace=(ws[0].half(), ws[1]))
-    # (a number of splits of its own fits what there is)
-    C.block_scaled_decode(*args, workspace=(ws[0][:100], ws[1]), max_seq_len=1 << 20)
+@pytest.mark.parametrize("codes", CODES)
+@pytest.mark.parametrize("G", [1, 4, 7, 16, 24])
+def test_shares_of_all_sizes(codes, G):
+    """Requests of very different lengths, more of them than CTAs and fewer, shares that start and end anywhere."""
+    for lens in ([1] * 700, [3, 0, 20000, 1, 129] + [40] * 90, [2500], list(range(1, 400, 7))):
+        cache = K.Cache(codes, 2, 128, 16, lens, seed=G).to("cuda")
+        q = torch.randn(len(lens), 2 * G, 128, device="cuda", dtype=K.BF16)
+        got = C.block_scaled_decode(q, *cache.parts(), cache.tables, cache.seq_lens, 0.09)
+        K.check(got, q, cache, [1] * len(lens), 0.09, 0, 0, K.F16)
 
 
 def test_the_same_bits_again_and_on_another_stream():

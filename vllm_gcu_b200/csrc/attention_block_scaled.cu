@@ -36,7 +36,8 @@ constexpr float kLog2e = 1.4426950408889634f;
 struct Args {
   const void* q;               // [T, Hq * D], row pitch ldq
   void* out;                   // [T, Hq * D], row pitch ldo
-  float *tmp_out, *tmp_lse;    // splits without a cluster: [T, Hq, splits, D], [T, Hq, splits]
+  float *tmp_out, *tmp_lse;    // splits without a cluster: [T, Hq, splits, D], [T, Hq, splits]; D 128: parts of the CTAs
+  int4* units;                 // D 128: what the CTA's share starts inside of
   const float *ks, *vs;        // [num_blocks, Hkv]
   const int *cu_q;             // [B + 1], null: one token per request
   const int *seq_lens, *block_tables;
@@ -143,18 +144,22 @@ __device__ __forceinline__ void merge_cluster(const Args& a, const Place& p, int
   cluster_sync();                   // nobody leaves while another CTA may still read its numbers
 }
 
-// Launch with the splits of a request and key head as a cluster, or as CTAs on their own.
 // (`done`: per device, whether the kernel has its shared memory)
 using Kernel = void (*)(CUtensorMap, CUtensorMap, Args);
-inline int launch_splits(Kernel kernel, bool (&done)[64], int threads, int smem, bool cluster, const Args& a,
-                         const CUtensorMap& tmK, const CUtensorMap& tmV, cudaStream_t s) {
+inline int set_shared(Kernel kernel, bool (&done)[64], int smem) {
   int dev = 0;
   cudaGetDevice(&dev);
-  if (dev >= 0 && dev < 64 && !done[dev]) {
-    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-    if (e != cudaSuccess) return launch_code(e);
-    done[dev] = true;
-  }
+  if (dev < 0 || dev >= 64 || done[dev]) return 0;
+  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e != cudaSuccess) return launch_code(e);
+  done[dev] = true;
+  return 0;
+}
+// Launch with the splits of a request and key head as a cluster, or as CTAs on their own.
+inline int launch_splits(Kernel kernel, bool (&done)[64], int threads, int smem, bool cluster, const Args& a,
+                         const CUtensorMap& tmK, const CUtensorMap& tmV, cudaStream_t s) {
+  const int set = set_shared(kernel, done, smem);
+  if (set != 0) return set;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(a.Hkv * a.row_blocks, a.B, a.splits);
   cfg.blockDim = dim3(threads);
@@ -564,6 +569,7 @@ struct Call {
   const float *ks, *vs;
   const int *cu_q, *seq_lens, *block_tables;
   float *tmp_out, *tmp_lse;
+  int* units;
   long long ldq, ldo, slot_bytes;
   float scale;
   int T, B, max_q, Hq, Hkv, D, splits, max_blocks, block_size, num_blocks, window, first, int8, dtype;
@@ -602,13 +608,10 @@ int launch_any(const CUtensorMap& tmK, const CUtensorMap& tmV, const Args& a, in
 namespace b200 {
 namespace rows8 {
 
-template <typename T, bool kInt8, int kR>
-int launch_tc_any(const CUtensorMap& tmK, const CUtensorMap& tmV, const Args& a, int T_rows, cudaStream_t s) {
-  if (a.splits > 1 && a.splits <= 8) return launch_tc<T, kInt8, kR, true>(tmK, tmV, a, s);
-  const int e = launch_tc<T, kInt8, kR, false>(tmK, tmV, a, s);
-  if (e != 0 || a.splits <= 1) return e;
-  const int total = T_rows * a.Hq;
-  return launch_overlapped(merge_rows_kernel<T, 128>, dim3((total + 3) / 4), dim3(128), 0, s, a, total);
+// Rows that a CTA takes, of `all` of a request and key head.
+inline int rows_of_cta(int D, long long all) {
+  if (D == 128) return all <= 4 ? 4 : all <= 8 ? 8 : all <= 16 ? 16 : 32;
+  return D == 64 && all > 16 ? 32 : 16;
 }
 
 template <typename T, bool kInt8>
@@ -618,10 +621,10 @@ int launch_width(int D, const CUtensorMap& tmK, const CUtensorMap& tmV, const Ar
     case 256: return launch_any<T, kInt8, 256>(tmK, tmV, a, T_rows, false, s);
     case 128:
       switch (rows) {
-        case 4: return launch_tc_any<T, kInt8, 4>(tmK, tmV, a, T_rows, s);
-        case 8: return launch_tc_any<T, kInt8, 8>(tmK, tmV, a, T_rows, s);
-        case 16: return launch_tc_any<T, kInt8, 16>(tmK, tmV, a, T_rows, s);
-        case 32: return launch_tc_any<T, kInt8, 32>(tmK, tmV, a, T_rows, s);
+        case 4: return launch_tc<T, kInt8, 4>(tmK, tmV, a, a.splits, s);
+        case 8: return launch_tc<T, kInt8, 8>(tmK, tmV, a, a.splits, s);
+        case 16: return launch_tc<T, kInt8, 16>(tmK, tmV, a, a.splits, s);
+        case 32: return launch_tc<T, kInt8, 32>(tmK, tmV, a, a.splits, s);
       }
   }
   return -8;
@@ -630,15 +633,27 @@ int launch_width(int D, const CUtensorMap& tmK, const CUtensorMap& tmV, const Ar
 }  // namespace rows8
 }  // namespace b200
 
+// Rows of a CTA and CTAs that run at the same time for head dimension 128 and so many query rows a request and key head:
+// rows << 16 | CTAs.
+B200_API int b200_block_scaled_slots(int rows, int int8) {
+  using namespace b200::rows8;
+  const int per = rows_of_cta(128, rows);
+  return per << 16 | (int8 ? tc_slots<true>(per) : tc_slots<false>(per));
+}
+
 // Attention over blocks with scales.  dtype 0 bf16, 1 fp16; D 64, 128 or 256; max_q: most tokens of a request;
-// block_size a multiple of 16; up to 32 splits, more than 8 need tmp_out and tmp_lse.
+// block_size a multiple of 16.  D 64 and 256: up to 32 splits, more than 8 need tmp_out and tmp_lse (fp32 [T, Hq, splits, D]
+// and [T, Hq, splits]).  D 128: `splits` CTAs, tmp_out [2 * splits, rows of a CTA, 128], tmp_lse [2 * splits, rows of a CTA],
+// units int32 [splits, 4]; a multiple of Hkv.
 B200_API int b200_block_scaled_rows(const void* call, void* stream) {
   using namespace b200;
   using namespace b200::rows8;
   const Call& k = *static_cast<const Call*>(call);
   if (k.B <= 0 || k.T <= 0 || k.Hkv <= 0) return 0;
-  if (k.splits < 1 || k.splits > 32 || k.Hq % k.Hkv != 0 || k.block_size % kChunk != 0) return -2;
-  if (k.splits > 8 && (k.tmp_out == nullptr || k.tmp_lse == nullptr)) return -5;
+  if (k.splits < 1 || k.Hq % k.Hkv != 0 || k.block_size % kChunk != 0) return -2;
+  if (k.D == 128 ? k.tmp_out == nullptr || k.tmp_lse == nullptr || k.units == nullptr
+                 : k.splits > 32 || (k.splits > 8 && (k.tmp_out == nullptr || k.tmp_lse == nullptr)))
+    return -5;
   const int cols = k.D < 128 ? k.D : 128;
   const CUtensorMapSwizzle swizzle = k.D == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B;
   CUtensorMap tmK, tmV;
@@ -649,14 +664,15 @@ B200_API int b200_block_scaled_rows(const void* call, void* stream) {
   const int group = k.Hq / k.Hkv;
   const long long all = static_cast<long long>(k.max_q) * group;
   // rows of a CTA
-  const int per = k.D == 128 ? (all <= 4 ? 4 : all <= 8 ? 8 : all <= 16 ? 16 : 32) : k.D == 64 && all > 16 ? 32 : 16;
+  const int per = rows_of_cta(k.D, all);
   Args a;
-  a.q = k.q; a.out = k.out; a.tmp_out = k.tmp_out; a.tmp_lse = k.tmp_lse; a.ks = k.ks; a.vs = k.vs; a.cu_q = k.cu_q;
+  a.q = k.q; a.out = k.out; a.tmp_out = k.tmp_out; a.tmp_lse = k.tmp_lse;
+  a.units = reinterpret_cast<int4*>(k.units); a.ks = k.ks; a.vs = k.vs; a.cu_q = k.cu_q;
   a.seq_lens = k.seq_lens; a.block_tables = k.block_tables; a.ldq = k.ldq; a.ldo = k.ldo; a.B = k.B; a.Hq = k.Hq;
   a.Hkv = k.Hkv; a.splits = k.splits; a.max_blocks = k.max_blocks; a.block_size = k.block_size;
   a.num_blocks = k.num_blocks; a.window = k.window; a.first = k.first; a.scale = k.scale;
   const long long row_blocks = (all + per - 1) / per;
-  if (k.B > 65535) return -2;
+  if (k.B > 65535 || row_blocks * k.Hkv * k.B > 0x7fffffffll) return -2;
   a.row_blocks = static_cast<int>(row_blocks);
   a.status = status_ptr();
   cudaStream_t s = static_cast<cudaStream_t>(stream);

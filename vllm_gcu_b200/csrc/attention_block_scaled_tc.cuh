@@ -13,6 +13,14 @@
 // that feeds 16-bit matrix instructions from 8-bit codes (attention_block_scaled.cu, head dimensions 64 and 256: there a
 // chunk of 16 tokens takes a warp 490 instructions, here 80 of them for four query rows).
 //
+// A CTA stays on its SM and takes an even share of the tiles of all requests for one key head, one behind the other (as
+// many CTAs as run at the same time, or one per tile where there are fewer; those of a share's key heads are neighbours,
+// since the heads' rows of a token lie side by side and memory is read in pieces of two: 613 against 904 MB where a CTA
+// took the key heads one after the other): the shares depend on the lengths that the
+// step holds, not on a bound that a captured graph was made with, no CTA has more than a tile more than another one, and a
+// request's start (block table, queries) overlaps with the end of the one before.  Where a share begins or ends inside a
+// request's keys, its part of the result goes to memory, and merge_units_kernel puts the parts together in their order.
+//
 // Warps: 0..3 (32 rows: 0..7) queries and softmax, lane = token of a tile and at the end column of the output; then one
 // for TMA, block tables and scales and one for tcgen05.mma and tensor memory.  K Q^T of a tile runs while the one before is
 // at its softmax; keys and values have places of their own, given back when their product is done.
@@ -50,9 +58,10 @@ struct Tc {
   static constexpr int kOffP = kOffQ + kNS * 128;
   static constexpr int kOffScale = kOffP + 2 * kN * 128;       // [kGroups][32] scales of keys, log2 and inverse of values', flag
   static constexpr int kOffBar = kOffScale + kGroups * 32 * 16;
-  static constexpr int kOffRow = kOffBar + 256;                // factor and position of every row
-  static constexpr int kOffMax = kOffRow + 2 * kR * 4;         // of four warps and every row; log2 sums of the rows
-  static constexpr int kBytes = kOffMax + 5 * kR * 4 + 1024;
+  static constexpr int kOffWork = kOffBar + 256;               // [2]
+  static constexpr int kOffRow = kOffWork + 128;               // factor and position of every row; [2] token and head
+  static constexpr int kOffMax = kOffRow + 6 * kR * 4;         // of four warps and every row; inverse sum and log2 of them
+  static constexpr int kBytes = kOffMax + 6 * kR * 4 + 1024;
 };
 
 // A pair of fp16 numbers as three pairs of e4m3 parts: x = p0 + p1 / 16 + p2 / 256, each pair in 16 bits.
@@ -145,9 +154,110 @@ __device__ __forceinline__ float warp_top_of(float x) {
   return __int_as_float(i < 0 ? i ^ 0x7fffffff : i);
 }
 
-template <typename T, bool kInt8, int kR, bool kCluster>
+// Waits whose code is small: some thirty of them lie in the kernel, whose first pass is as long as its instructions take
+// to arrive (mbar_wait's loop is unrolled: 150 KB in all, and 6 us until the first tile was done).
+__device__ __noinline__ void wait_failed(unsigned int* status, unsigned int detail, volatile uint32_t* abort_flag) {
+  report_status(status, kStatusMbarTimeout, kKernelId, detail);
+  *abort_flag = 1u;
+}
+__device__ __noinline__ void bad_block(unsigned int* status, unsigned int detail) {
+  report_status(status, kStatusBounds, kKernelId, detail);
+}
+__device__ __forceinline__ bool wait_one(uint64_t* bar, uint32_t parity, unsigned int* status, unsigned int detail,
+                                         volatile uint32_t* abort_flag) {
+#pragma unroll 1
+  for (uint32_t i = 0; i < kMbarSpinLimit; ++i) {
+    if (mbar_test(bar, parity)) return true;
+    if ((i & 1023u) == 1023u && *abort_flag != 0u) return false;
+  }
+  wait_failed(status, detail, abort_flag);
+  return false;
+}
+// By all lanes of a warp: with one answer; or going on whatever it is.
+__device__ __forceinline__ bool wait_warp(uint64_t* bar, uint32_t parity, unsigned int* status, unsigned int detail,
+                                          volatile uint32_t* abort_flag) {
+  return __all_sync(0xffffffffu, wait_one(bar, parity, status, detail, abort_flag)) != 0;
+}
+__device__ __forceinline__ void pass_warp(uint64_t* bar, uint32_t parity, unsigned int* status, unsigned int detail,
+                                          volatile uint32_t* abort_flag) {
+  wait_one(bar, parity, status, detail, abort_flag);
+  __syncwarp();
+}
+
+// An even share of `total` tiles for each of n: where share j starts, and the share that tile x lies in.
+struct Shares {
+  int each, more;            // the first `more` shares have one tile more
+  __device__ __forceinline__ Shares(int total, int n) : each(total / n), more(total - total / n * n) {}
+  __device__ __forceinline__ int start(int j) const { return j * each + min(j, more); }
+  __device__ __forceinline__ int of(int x) const {
+    const int front = more * (each + 1);
+    return x < front ? x / (each + 1) : more + (x - front) / each;
+  }
+};
+
+// Sums of kRW numbers over the lanes of a warp, in kRW - 1 and a few exchanges: this lane has that of row `row`.
+template <int kRW>
+__device__ __forceinline__ float sums_of_rows(float (&v)[kRW], int lane, int& row) {
+  row = 0;
+  int d = 16;
+#pragma unroll
+  for (int n = kRW / 2; n > 0; n >>= 1, d >>= 1) {
+    const bool upper = (lane & d) != 0;
+    row = upper ? row + n : row;
+#pragma unroll
+    for (int i = 0; i < n; ++i) {
+      const float keep = upper ? v[i + n] : v[i], give = upper ? v[i] : v[i + n];
+      v[i] = keep + __shfl_xor_sync(0xffffffffu, give, d);
+    }
+  }
+#pragma unroll
+  for (; d > 0; d >>= 1) v[0] += __shfl_xor_sync(0xffffffffu, v[0], d);
+  return v[0];
+}
+
+// What the TMA warp tells the others about the part of a request's and key head's tiles that the CTA takes.
+struct Work {
+  int q_start;             // -1: no more work
+  int pos0, kvh, row0, rows;
+  int lo_pos, hi_pos;      // positions of the CTA's rows
+  int firsts, lo_chunk;
+  int c0, c1;              // chunks
+  int ntiles;
+  int part;                // -1: all of the tiles; place of the part's numbers
+  int pad[3];
+};
+
+// Tiles of rows kR * block .. of request b (1 where the rows see no key: they give zeros), 0 where there are no such rows.
+template <int kR>
+__device__ __noinline__ Place tc_place(const Args& a, int b, int block, int* tiles) {
+  Place p;
+  p.b = b;
+  p.kvh = 0;
+  p.G = a.Hq / a.Hkv;
+  p.row0 = block * kR;
+  p.q_start = a.cu_q != nullptr ? a.cu_q[b] : b;
+  const int q_len = a.cu_q != nullptr ? a.cu_q[b + 1] - p.q_start : 1;
+  p.rows = q_len * p.G;
+  const int len = min(a.seq_lens[b], a.max_blocks * a.block_size);
+  p.pos0 = len - q_len;
+  p.lo_pos = p.pos0;
+  p.hi_pos = len - 1;
+  if (a.row_blocks > 1) {
+    p.lo_pos += p.row0 / p.G;
+    p.hi_pos = p.pos0 + (min(p.row0 + kR, p.rows) - 1) / p.G;
+  }
+  const int lo = a.window > 0 ? max(0, p.lo_pos - a.window + 1) : 0;
+  p.lo_chunk = lo / kChunk;
+  p.firsts = a.window > 0 ? min(p.lo_chunk, (a.first + kChunk - 1) / kChunk) : 0;
+  p.chunks = p.hi_pos >= 0 ? p.firsts + p.hi_pos / kChunk + 1 - p.lo_chunk : 0;
+  *tiles = p.row0 < p.rows ? max(1, (p.chunks + 7) / 8) : 0;
+  return p;
+}
+
+template <typename T, bool kInt8, int kR>
 __global__ void __launch_bounds__(Tc<kInt8, kR>::kThreads, Tc<kInt8, kR>::kCtas)
-    rows_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const Args a) {
+    rows_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
+                   const __grid_constant__ Args a) {
   using S = Tc<kInt8, kR>;
   constexpr int kN = S::kN, kNS = S::kNS, kStages = S::kStages, kParts = S::kParts, kWarps = S::kWarps, kRW = S::kRW, kScores = S::kScores;
   constexpr int kSoft = kWarps * 32;
@@ -164,29 +274,23 @@ __global__ void __launch_bounds__(Tc<kInt8, kR>::kThreads, Tc<kInt8, kR>::kCtas)
   uint64_t* s_free = s_full + kScores;      // [kScores]
   uint64_t* p_full = s_free + kScores;      // [2]
   uint64_t* o_done = p_full + 2;            // [2]
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(o_done + 2);
+  uint64_t* w_full = o_done + 2;            // [2] a Work is there
+  uint64_t* w_empty = w_full + 2;           // [2]
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(w_empty + 2);
   volatile uint32_t* abort_flag = tmem_slot + 1;
   volatile uint32_t* adds = tmem_slot + 2;  // [2]: whether P V of the buffer's tile adds to what is there
-  static_assert((4 * kStages + 5 + kGroups + 2 * kScores) * 8 + 16 <= 256, "barrier area");
+  static_assert((4 * kStages + 9 + kGroups + 2 * kScores) * 8 + 16 <= 256, "barrier area");
+  static_assert(sizeof(Work) == 64, "place of the works");
   float4* chunk_scale = reinterpret_cast<float4*>(smem + S::kOffScale);
+  Work* works = reinterpret_cast<Work*>(smem + S::kOffWork);
   float* row_factor = reinterpret_cast<float*>(smem + S::kOffRow);
   int* row_pos = reinterpret_cast<int*>(row_factor + kR);
+  int2* row_place = reinterpret_cast<int2*>(row_pos + kR);              // [2][kR]
   float* warp_top = reinterpret_cast<float*>(smem + S::kOffMax);        // [4][kR]
-  float* part_lse = warp_top + 4 * kR;                                  // [kR]
-  float* part_o = reinterpret_cast<float*>(smem);                       // [kR][128], where keys were
+  float* row_inv = warp_top + 4 * kR;                                   // [kR]
+  float* row_lse = row_inv + kR;                                        // [kR]
 
-  grid_wait();
-  const Place p = place_of<kR>(a);
-  if (p.row0 >= p.rows) return;             // surplus rows (of a whole cluster)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int split = blockIdx.z;
-  const int live = min(kR, p.rows - p.row0);
-  const int tiles_all = (p.chunks + 7) / 8;
-  const int per_split = (tiles_all + a.splits - 1) / a.splits * 8;
-  const int c0 = split * per_split, c1 = min(p.chunks, c0 + per_split);
-  const int ntiles = c1 > c0 ? (c1 - c0 + 7) / 8 : 0;
-  auto first_token = [&](int chunk) { return (chunk < p.firsts ? chunk : p.lo_chunk + chunk - p.firsts) * kChunk; };
-
   if (threadIdx.x == 0) {
     for (int s = 0; s < kStages; ++s) {
       mbar_init(&k_full[s], 1);
@@ -203,6 +307,8 @@ __global__ void __launch_bounds__(Tc<kInt8, kR>::kThreads, Tc<kInt8, kR>::kCtas)
     for (int b = 0; b < 2; ++b) {
       mbar_init(&p_full[b], kWarps);
       mbar_init(&o_done[b], 1);
+      mbar_init(&w_full[b], 1);
+      mbar_init(&w_empty[b], kWarps + 1);
     }
     *abort_flag = 0u;
     mbar_fence_init();
@@ -217,85 +323,207 @@ __global__ void __launch_bounds__(Tc<kInt8, kR>::kThreads, Tc<kInt8, kR>::kCtas)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  grid_release();                           // (behind the allocation, see common.cuh)
+  grid_wait();
 
   if (warp == kWarps) {
-    // ---------------- TMA, block tables, scales ----------------
-    // lane = (tile of a group of four, chunk of it); a group's blocks are read two groups ahead, its scales one
-    const int* bt = a.block_tables + static_cast<long long>(p.b) * a.max_blocks;
-    auto chunk_of = [&](int g) { return c0 + g * (8 * kGroup) + lane; };
-    auto block_of = [&](int g) {
-      const int c = chunk_of(g);
-      return c < c1 ? bt[first_token(c) / a.block_size] : 0;
-    };
-    auto row_of = [&](int g, int block) { return block * a.block_size + first_token(chunk_of(g)) % a.block_size; };
-    auto scales_of = [&](int g, int block) {
-      float4 s = make_float4(0.0f, power_of_two(kLowExponent), 0.0f, 0.0f);
-      const int c = chunk_of(g);
-      if (c >= c1) return s;
-      if (block >= 0 && block < a.num_blocks) {
-        const long long at = static_cast<long long>(block) * a.Hkv + p.kvh;
-        s.x = a.ks[at];
-        s.y = a.vs[at];
-      } else {
-        report_status(a.status, kStatusBounds, kKernelId, static_cast<unsigned>(p.b));
+    // ---------------- work, TMA, block tables, scales ----------------
+    // tiles of the requests (those of the first 512 stay where scales will lie)
+    int* kept = reinterpret_cast<int*>(smem + S::kOffScale);
+    static_assert(kGroups * 32 * 16 >= 512 * 4, "room for the requests' tiles");
+    int total = 0;
+#pragma unroll 1
+    for (int b = lane; b < a.B; b += 32) {
+      int n = 0;
+#pragma unroll 1
+      for (int rb = 0; rb < a.row_blocks; ++rb) {
+        int t;
+        tc_place<kR>(a, b, rb, &t);
+        if (t == 0) break;
+        n += t;
       }
-      return s;
-    };
-    auto publish = [&](int g, float4 s) {
-      const int c = chunk_of(g), tok = first_token(c);
-      // (a block that was never written has no scale: its keys count all the same)
-      const float vs = fmaxf(s.y, power_of_two(kLowExponent));
-      s.y = __log2f(vs);
-      s.z = __fdividef(1.0f, vs);
-      // whether all rows see all of the chunk
-      s.w = c < c1 && tok + kChunk - 1 <= p.lo_pos && (a.window <= 0 || tok > p.hi_pos - a.window || tok + kChunk <= a.first)
-                ? 1.0f : 0.0f;
-      chunk_scale[g % kGroups * 32 + lane] = s;
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&c_full[g % kGroups]);
-    };
-    int block = block_of(0), block_next = block_of(1);
-    float4 scales = scales_of(0, block);
-    int row = row_of(0, block), row_next = row_of(1, block_next);
-    bool ok = true;
-    // copies of tile `it`, whose rows lie in `rows`
-    auto copy = [&](int it, int rows, bool values) {
-      const int st = it % kStages, n = min(8, c1 - c0 - it * 8);
-      ok = mbar_wait_warp(values ? &v_empty[st] : &k_empty[st], ((it / kStages) & 1) ^ 1, a.status, kKernelId,
-                          0x300u + st, abort_flag);
-      if (!ok) return;
-      const int y = __shfl_sync(0xffffffffu, rows, it % kGroup * 8 + (lane & 7));
-      uint64_t* bar = values ? &v_full[st] : &k_full[st];
-      if (lane == 0) mbar_expect_tx(bar, static_cast<uint32_t>(n) * kChunk * 128u);
-      __syncwarp();
-      if (lane < n)
-        tma_load_2d(smem + ((values ? kStages : 0) + st) * kTcBytes + lane * (kChunk * 128), values ? &tmV : &tmK, bar,
-                    p.kvh * 128, y);
-    };
-    if (ntiles > 0) copy(0, row, false);
-    for (int it = 0; it < ntiles && ok; ++it) {
-      const int g = it / kGroup;
-      const bool first = it % kGroup == 0;
-      int block_after = 0;
-      float4 scales_next = scales;
-      if (first) {
-        block_after = block_of(g + 2);
-        scales_next = scales_of(g + 1, block_next);
-      }
-      if (it + 1 < ntiles) copy(it + 1, (it + 1) % kGroup == 0 ? row_next : row, false);
-      if (ok) copy(it, row, true);
-      // (behind the copies: nothing in front waits for this tile's softmax)
-      if (first) {
-        publish(g, scales);
-        scales = scales_next;
-        block_next = block_after;
-      }
-      if (it % kGroup == kGroup - 1) {
-        row = row_next;
-        row_next = row_of(g + 2, block_next);
+      if (b < 512) kept[b] = n;
+      total += n;
+    }
+    total = __reduce_add_sync(0xffffffffu, total);
+    // this CTA's key head and tiles; every share has one at least, those behind the last tile have none
+    const int kvh = static_cast<int>(blockIdx.x) % a.Hkv, cta = static_cast<int>(blockIdx.x) / a.Hkv;
+    const int ctas = min(total, static_cast<int>(gridDim.x) / a.Hkv);
+    const Shares shares(total, max(ctas, 1));
+    int at = cta < ctas ? shares.start(cta) : 0;
+    const int end = cta < ctas ? shares.start(cta + 1) : 0;
+    // request of the first one, and the tile in it
+    int b = 0, in_b = 0;
+    if (at < end) {
+      int base = 0;
+#pragma unroll 1
+      for (int b0 = 0; b0 < a.B; b0 += 32) {
+        int n = 0;
+        if (b0 + lane < a.B) {
+          if (b0 + lane < 512) {
+            n = kept[b0 + lane];
+          } else {
+#pragma unroll 1
+            for (int rb = 0; rb < a.row_blocks; ++rb) {
+              int t;
+              tc_place<kR>(a, b0 + lane, rb, &t);
+              n += t;
+            }
+          }
+        }
+        int inc = n;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+          const int x = __shfl_up_sync(0xffffffffu, inc, d);
+          if (lane >= d) inc += x;
+        }
+        const uint32_t vote = __ballot_sync(0xffffffffu, at < base + inc);
+        if (vote != 0u) {
+          const int src = __ffs(vote) - 1;
+          b = b0 + src;
+          in_b = at - base - __shfl_sync(0xffffffffu, inc - n, src);
+          break;
+        }
+        base += __shfl_sync(0xffffffffu, inc, 31);
       }
     }
+    __syncwarp();
+    int rb = 0, tile = 0, tiles = 0;                        // row block, its next tile, its tiles
+    Place p = {};
+    if (at < end) {
+#pragma unroll 1
+      for (;; ++rb) {
+        p = tc_place<kR>(a, b, rb, &tiles);
+        if (in_b < tiles) break;
+        in_b -= tiles;
+      }
+      tile = in_b;
+    }
+    // a share that starts inside a request's tiles tells the shares that they lie in
+    if (lane == 0)
+      a.units[blockIdx.x] = tile == 0 ? make_int4(-1, 0, 0, 0)
+                                      : make_int4(b, rb, shares.of(at - tile), shares.of(at - tile + tiles - 1));
+    bool ok = true;
+    int t = 0, groups = 0;                                  // tiles and groups of tiles so far
+    for (int w = 0; ok; ++w) {
+      Work k = {};
+      k.q_start = -1;
+      if (at < end) {
+        const int n = min(tiles - tile, end - at);
+        k.q_start = p.q_start;
+        k.pos0 = p.pos0; k.kvh = kvh; k.row0 = p.row0; k.rows = p.rows; k.lo_pos = p.lo_pos; k.hi_pos = p.hi_pos;
+        k.firsts = p.firsts; k.lo_chunk = p.lo_chunk;
+        k.c0 = tile * 8;
+        k.c1 = min(p.chunks, (tile + n) * 8);
+        k.ntiles = n;
+        // a part that starts inside a request's tiles is the CTA's first one
+        k.part = n == tiles ? -1 : 2 * static_cast<int>(blockIdx.x) + (tile == 0 ? 1 : 0);
+      }
+      ok = wait_warp(&w_empty[w & 1], ((w >> 1) & 1) ^ 1, a.status, 0x3b0u, abort_flag);
+      if (!ok) break;
+      if (lane == 0) {
+        works[w & 1] = k;
+        mbar_arrive(&w_full[w & 1]);
+      }
+      __syncwarp();
+      if (k.q_start < 0) break;
+
+      // lane = (tile of a group of four, chunk of it); a group's blocks are read two groups ahead, its scales one
+      const int* bt = a.block_tables + static_cast<long long>(p.b) * a.max_blocks;
+      auto first_token = [&](int chunk) { return (chunk < p.firsts ? chunk : p.lo_chunk + chunk - p.firsts) * kChunk; };
+      auto chunk_of = [&](int g) { return k.c0 + g * (8 * kGroup) + lane; };
+      auto block_of = [&](int g) {
+        const int c = chunk_of(g);
+        return c < k.c1 ? bt[first_token(c) / a.block_size] : 0;
+      };
+      auto row_of = [&](int g, int block) { return block * a.block_size + first_token(chunk_of(g)) % a.block_size; };
+      auto scales_of = [&](int g, int block) {
+        float4 s = make_float4(0.0f, power_of_two(kLowExponent), 0.0f, 0.0f);
+        if (chunk_of(g) >= k.c1) return s;
+        if (block >= 0 && block < a.num_blocks) {
+          const long long i = static_cast<long long>(block) * a.Hkv + kvh;
+          s.x = a.ks[i];
+          s.y = a.vs[i];
+        } else {
+          bad_block(a.status, static_cast<unsigned>(p.b));
+        }
+        return s;
+      };
+      auto publish = [&](int g, float4 s) {
+        const int c = chunk_of(g), tok = first_token(c), slot = (groups + g) % kGroups;
+        // (a block that was never written has no scale: its keys count all the same)
+        const float vs = fmaxf(s.y, power_of_two(kLowExponent));
+        s.y = __log2f(vs);
+        s.z = __fdividef(1.0f, vs);
+        // whether all rows see all of the chunk
+        s.w = c < k.c1 && tok + kChunk - 1 <= p.lo_pos &&
+                      (a.window <= 0 || tok > p.hi_pos - a.window || tok + kChunk <= a.first) ? 1.0f : 0.0f;
+        chunk_scale[slot * 32 + lane] = s;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&c_full[slot]);
+      };
+      // rows of groups g and g + 1, block of g + 1, scales of g
+      int row = 0, row_next = 0, block_next = 0;
+      float4 scales = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      // copies of tiles: a tile's keys, then the values of the one before
+#pragma unroll 1
+      for (int it = -1; it < k.ntiles && ok; ++it) {
+        const int g = it >= 0 ? it / kGroup : -1;
+        const bool first = it < 0 || it % kGroup == 0;
+        float4 scales_next = scales;
+        int block_after = 0;
+        if (first) {
+          // (of group 0 before anything, its scales with the first tile)
+          if (it < 0) {
+            block_next = block_of(0);
+            row_next = row_of(0, block_next);
+          }
+          block_after = block_of(g + 2);
+          scales_next = scales_of(g + 1, block_next);
+        }
+#pragma unroll 1
+        for (int values = 0; values < 2; ++values) {
+          const int i = values ? it : it + 1;
+          if (i < 0 || i >= k.ntiles) continue;
+          const int st = (t + i) % kStages, n = max(0, min(8, k.c1 - k.c0 - i * 8));
+          ok = wait_warp((values ? v_empty : k_empty) + st, (((t + i) / kStages) & 1) ^ 1, a.status, 0x300u + st, abort_flag);
+          if (!ok) break;
+          const int y = __shfl_sync(0xffffffffu, !values && i % kGroup == 0 ? row_next : row, i % kGroup * 8 + (lane & 7));
+          uint64_t* bar = (values ? v_full : k_full) + st;
+          if (lane == 0) mbar_expect_tx(bar, static_cast<uint32_t>(n) * kChunk * 128u);
+          __syncwarp();
+          if (lane < n)
+            tma_load_2d(smem + ((values ? kStages : 0) + st) * kTcBytes + lane * (kChunk * 128), values ? &tmV : &tmK, bar,
+                        kvh * 128, y);
+        }
+        // (behind the copies: nothing in front waits for this tile's softmax)
+        if (it >= 0 && first) publish(g, scales);
+        if (first) {
+          scales = scales_next;
+          block_next = block_after;
+        }
+        if (it < 0 || it % kGroup == kGroup - 1) {
+          row = row_next;
+          row_next = row_of(g + 2, block_next);
+        }
+      }
+      t += k.ntiles;
+      groups += (k.ntiles + kGroup - 1) / kGroup;
+      // the next row block or request
+      at += k.ntiles;
+      tile = 0;
+      if (at < end) {
+        ++rb;
+        tiles = 0;
+        if (rb < a.row_blocks) p = tc_place<kR>(a, b, rb, &tiles);
+        while (tiles == 0) {
+          rb = 0;
+          p = tc_place<kR>(a, ++b, 0, &tiles);
+        }
+      }
+    }
+    // The next kernel may start now, not before: its CTAs would take registers of this one's that are still to come, whose
+    // tiles would then wait for a first CTA's end (steps one behind the other 160 us a pass, alone 120).
+    grid_release();
   } else if (warp == kWarps + 1) {
     // ---------------- tcgen05.mma ----------------
     if (elect_one()) {
@@ -308,8 +536,8 @@ __global__ void __launch_bounds__(Tc<kInt8, kR>::kThreads, Tc<kInt8, kR>::kCtas)
       const uint64_t v_desc = make_desc_mn_sw128(smem_u32(smem + kStages * kTcBytes), kTcBytes);
       auto pv = [&](int j) -> bool {
         const int b = j & 1, st = j % kStages;
-        if (!mbar_wait(&v_full[st], (j / kStages) & 1, a.status, kKernelId, 0x310u + st, abort_flag) ||
-            !mbar_wait(&p_full[b], (j >> 1) & 1, a.status, kKernelId, 0x320u + b, abort_flag))
+        if (!wait_one(&v_full[st], (j / kStages) & 1, a.status, 0x310u + st, abort_flag) ||
+            !wait_one(&p_full[b], (j >> 1) & 1, a.status, 0x320u + b, abort_flag))
           return false;
         tc_fence_after();
         const uint32_t add = adds[b];
@@ -321,86 +549,112 @@ __global__ void __launch_bounds__(Tc<kInt8, kR>::kThreads, Tc<kInt8, kR>::kCtas)
         umma_commit(&v_empty[st]);
         return true;
       };
-      bool ok = ntiles == 0 || mbar_wait(q_full, 0, a.status, kKernelId, 0x322u, abort_flag);
-      for (int it = 0; ok && it < ntiles; ++it) {
-        const int b = it % kScores, st = it % kStages;
-        ok = mbar_wait(&k_full[st], (it / kStages) & 1, a.status, kKernelId, 0x330u + st, abort_flag) &&
-             mbar_wait(&s_free[b], ((it / kScores) & 1) ^ 1, a.status, kKernelId, 0x340u + b, abort_flag);
+      bool ok = true;
+      int t = 0;
+      for (int w = 0; ok; ++w) {
+        ok = wait_one(&w_full[w & 1], (w >> 1) & 1, a.status, 0x3c0u, abort_flag);
         if (!ok) break;
-        tc_fence_after();
+        const bool over = static_cast<volatile Work*>(works)[w & 1].q_start < 0;
+        const int ntiles = static_cast<volatile Work*>(works)[w & 1].ntiles;
+        mbar_arrive(&w_empty[w & 1]);
+        if (over) break;
+        ok = wait_one(q_full, w & 1, a.status, 0x322u, abort_flag);
+        for (int it = 0; ok && it < ntiles; ++it, ++t) {
+          const int b = t % kScores, st = t % kStages;
+          ok = wait_one(&k_full[st], (t / kStages) & 1, a.status, 0x330u + st, abort_flag) &&
+               wait_one(&s_free[b], ((t / kScores) & 1) ^ 1, a.status, 0x340u + b, abort_flag);
+          if (!ok) break;
+          tc_fence_after();
 #pragma unroll
-        for (int ks = 0; ks < 4; ++ks)
-          mma8<kInt8>(tmem + b * kNS, k_desc + static_cast<uint32_t>((st * kTcBytes + ks * 32) >> 4),
-                      q_desc + static_cast<uint32_t>(ks * 2), kIdescS, ks > 0 ? 1u : 0u);
-        umma_commit(&s_full[b]);
-        umma_commit(&k_empty[st]);
-        if (it > 0) ok = pv(it - 1);
+          for (int ks = 0; ks < 4; ++ks)
+            mma8<kInt8>(tmem + b * kNS, k_desc + static_cast<uint32_t>((st * kTcBytes + ks * 32) >> 4),
+                        q_desc + static_cast<uint32_t>(ks * 2), kIdescS, ks > 0 ? 1u : 0u);
+          umma_commit(&s_full[b]);
+          umma_commit(&k_empty[st]);
+          if (it > 0) ok = pv(t - 1);
+        }
+        if (ok) ok = pv(t - 1);
       }
-      if (ok && ntiles > 0) pv(ntiles - 1);
     }
     __syncwarp();
   } else {
-    // ---------------- queries ----------------
-    for (int r = warp; r < kR; r += kWarps) {
-      const int row = p.row0 + r;
-      const int token = row / p.G, head = p.kvh * p.G + row % p.G;
-      uint2 raw = make_uint2(0u, 0u);
-      if (r < live)
-        raw = *reinterpret_cast<const uint2*>(static_cast<const T*>(a.q) +
-                                              static_cast<long long>(p.q_start + token) * a.ldq + head * 128 + lane * 4);
-      const T* e = reinterpret_cast<const T*>(&raw);
-      float x[4], top = 0.0f;
-      bool number = true;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        x[i] = to_f32<T>(e[i]);
-        number = number && fabsf(x[i]) < INFINITY;
-        top = fmaxf(top, finite_size(x[i]));
-      }
-      const int e2 = max(-100, min(126, static_cast<int>(__float_as_uint(warp_top_of(top)) >> 23) - 127));
-      const float down = power_of_two(-e2);
-      uint32_t w[3] = {0u, 0u, 0u};
-      float unit;                           // of the parts, times 2^e2
-      if constexpr (kInt8) {
-        // |x| 2^-e2 < 2 as whole numbers of 21 bits, digits -64 .. 63 (the first one up to 64)
-        unit = 1.0f / 524287.0f;
+    const int row0 = kWarps == 4 ? 0 : warp / 4 * kRW;       // first row of the warp
+    static_assert(kWarps == 4 || kRW % 8 == 0, "places of rows in groups of eight");
+    const int i_tok = (warp & 3) * 32 + lane, c16 = i_tok >> 4;
+    const uint32_t lane_addr = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16) + row0;
+    const int G = a.Hq / a.Hkv;
+    const float inv_g = 1.0f / static_cast<float>(G);
+    // ---------------- queries of a part ----------------
+    auto queries = [&](const Work& k, int w) {
+      const int live = min(kR, k.rows - k.row0);
+#pragma unroll 1
+      for (int r = warp; r < kR; r += kWarps) {
+        const int row = k.row0 + r;
+        // row / G: half a G off the next whole number, and 2^-23 of itself wrong
+        const int token = __float2int_rd((static_cast<float>(row) + 0.5f) * inv_g), head = k.kvh * G + row - token * G;
+        uint2 raw = make_uint2(0u, 0u);
+        if (r < live)
+          raw = *reinterpret_cast<const uint2*>(static_cast<const T*>(a.q) +
+                                                static_cast<long long>(k.q_start + token) * a.ldq + head * 128 + lane * 4);
+        const T* e = reinterpret_cast<const T*>(&raw);
+        float x[4], top = 0.0f;
+        bool number = true;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const int f = __float2int_rn(fminf(fmaxf(x[i] * down, -2.0f), 2.0f) * 524287.0f);
-          const int d2 = ((f + 64) & 127) - 64, f1 = (f - d2) >> 7;
-          const int d1 = ((f1 + 64) & 127) - 64, d0 = (f1 - d1) >> 7;
-          w[0] |= static_cast<uint32_t>(d0 & 255) << (8 * i);
-          w[1] |= static_cast<uint32_t>(d1 & 255) << (8 * i);
-          w[2] |= static_cast<uint32_t>(d2 & 255) << (8 * i);
+          x[i] = to_f32<T>(e[i]);
+          number = number && fabsf(x[i]) < INFINITY;
+          top = fmaxf(top, finite_size(x[i]));
         }
-      } else {
-        // the largest in [128, 256), in 32 bits: a bf16 number's 8 bits are two parts, an fp16 number's 11 are three
-        unit = 1.0f / 128.0f;
+        const int e2 = max(-100, min(126, static_cast<int>(__float_as_uint(warp_top_of(top)) >> 23) - 127));
+        const float down = power_of_two(-e2);
+        uint32_t part[3] = {0u, 0u, 0u};
+        float unit;                         // of the parts, times 2^e2
+        if constexpr (kInt8) {
+          // |x| 2^-e2 < 2 as whole numbers of 21 bits, digits -64 .. 63 (the first one up to 64)
+          unit = 1.0f / 524287.0f;
 #pragma unroll
-        for (int i = 0; i < 4; i += 2) {
-          float y0 = x[i] * down * 128.0f, y1 = x[i + 1] * down * 128.0f;
+          for (int i = 0; i < 4; ++i) {
+            const int f = __float2int_rn(fminf(fmaxf(x[i] * down, -2.0f), 2.0f) * 524287.0f);
+            const int d2 = ((f + 64) & 127) - 64, f1 = (f - d2) >> 7;
+            const int d1 = ((f1 + 64) & 127) - 64, d0 = (f1 - d1) >> 7;
+            part[0] |= static_cast<uint32_t>(d0 & 255) << (8 * i);
+            part[1] |= static_cast<uint32_t>(d1 & 255) << (8 * i);
+            part[2] |= static_cast<uint32_t>(d2 & 255) << (8 * i);
+          }
+        } else {
+          // the largest in [128, 256), in 32 bits: a bf16 number's 8 bits are two parts, an fp16 number's 11 are three
+          unit = 1.0f / 128.0f;
 #pragma unroll
-          for (int k = 0; k < 3; ++k) {
-            const uint32_t c = __nv_cvt_float2_to_fp8x2(make_float2(y0, y1), __NV_SATFINITE, __NV_E4M3);
-            w[k] |= c << (8 * i);
-            y0 = (y0 - e4m3_to_f32(static_cast<uint8_t>(c & 255u))) * 16.0f;
-            y1 = (y1 - e4m3_to_f32(static_cast<uint8_t>(c >> 8))) * 16.0f;
+          for (int i = 0; i < 4; i += 2) {
+            float y0 = x[i] * down * 128.0f, y1 = x[i + 1] * down * 128.0f;
+#pragma unroll
+            for (int j = 0; j < 3; ++j) {
+              const uint32_t c = __nv_cvt_float2_to_fp8x2(make_float2(y0, y1), __NV_SATFINITE, __NV_E4M3);
+              part[j] |= c << (8 * i);
+              y0 = (y0 - e4m3_to_f32(static_cast<uint8_t>(c & 255u))) * 16.0f;
+              y1 = (y1 - e4m3_to_f32(static_cast<uint8_t>(c >> 8))) * 16.0f;
+            }
           }
         }
-      }
-      number = __all_sync(0xffffffffu, number);
+        number = __all_sync(0xffffffffu, number);
 #pragma unroll
-      for (int k = 0; k < 3; ++k) {
-        const int n = k * kR + r;
-        *reinterpret_cast<uint32_t*>(smem + S::kOffQ + (n >> 3) * 1024 + (n & 7) * 128 + (((lane >> 2) ^ (n & 7)) << 4) +
-                                     (lane & 3) * 4) = w[k];
+        for (int j = 0; j < 3; ++j) {
+          const int n = j * kR + r;
+          *reinterpret_cast<uint32_t*>(smem + S::kOffQ + (n >> 3) * 1024 + (n & 7) * 128 +
+                                       (((lane >> 2) ^ (n & 7)) << 4) + (lane & 3) * 4) = part[j];
+        }
+        if (lane == 0) {
+          // (a row that holds infinities or NaN gives NaN, as its products do)
+          row_factor[r] = number ? power_of_two(e2) * unit * a.scale * kLog2e : __int_as_float(0x7fffffff);
+          // (rows of no query see what the last one sees)
+          row_pos[r] = min(k.pos0 + token, k.hi_pos);
+          row_place[(w & 1) * kR + r] = make_int2(k.q_start + token, head);
+        }
       }
-      if (lane == 0) {
-        // (a row that holds infinities or NaN gives NaN, as its products do)
-        row_factor[r] = number ? power_of_two(e2) * unit * a.scale * kLog2e : __int_as_float(0x7fffffff);
-        row_pos[r] = p.pos0 + min(token, (p.rows - 1) / p.G);
-      }
-    }
+      fence_async_smem();
+      sync_softmax<kSoft>();                // (factors and positions)
+      if (lane == 0) mbar_arrive(q_full);
+    };
     // columns of no row, of queries and of both buffers of probabilities
     auto clear = [&](int from, int to, int off) {
       for (int i = threadIdx.x; i < (to - from) * 32; i += kSoft) {
@@ -411,21 +665,14 @@ __global__ void __launch_bounds__(Tc<kInt8, kR>::kThreads, Tc<kInt8, kR>::kCtas)
     clear(3 * kR, kNS, S::kOffQ);
     clear(kParts * kR, kN, S::kOffP);
     clear(kParts * kR, kN, S::kOffP + kN * 128);
-    fence_async_smem();
-    sync_softmax<kSoft>();                  // (factors and positions)
-    if (lane == 0) mbar_arrive(q_full);
 
     // ---------------- softmax: lane = token of the tile ----------------
-    const int row0 = warp / 4 * kRW;        // first row of the warp
-    const int i_tok = (warp & 3) * 32 + lane, c16 = i_tok >> 4;
-    const uint32_t lane_addr = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16) + row0;
+    constexpr float kUnit = kInt8 ? 16777216.0f : 16.0f;       // of a probability: 16 of them fill the parts
+    int t = 0, groups = 0;
+    Work k = {};
     float m[kRW], l[kRW], o[kRW];
 #pragma unroll
-    for (int r = 0; r < kRW; ++r) {
-      m[r] = -INFINITY;
-      l[r] = o[r] = 0.0f;
-    }
-    constexpr float kUnit = kInt8 ? 16777216.0f : 16.0f;       // of a probability: 16 of them fill the parts
+    for (int r = 0; r < kRW; ++r) m[r] = l[r] = o[r] = 0.0f;
     // what P V of earlier tiles left in tensor memory
     auto drain = [&]() {
       float v[kRW];
@@ -433,165 +680,240 @@ __global__ void __launch_bounds__(Tc<kInt8, kR>::kThreads, Tc<kInt8, kR>::kCtas)
 #pragma unroll
       for (int r = 0; r < kRW; ++r) o[r] = fmaf(v[r], 1.0f / kUnit, o[r]);
     };
-    bool drained = true;                    // nothing of these maxima in tensor memory
-    for (int it = 0; it < ntiles; ++it) {
-      const int g = it / kGroup;
-      if (it % kGroup == 0)
-        mbar_pass_warp(&c_full[g % kGroups], (g / kGroups) & 1, a.status, kKernelId, 0x390u, abort_flag);
-      const float4 scale = chunk_scale[g % kGroups * 32 + it % kGroup * 8 + c16];
-      const bool all_whole = __all_sync(0xffffffffu, scale.w != 0.0f);
-      // (the scores of a tile are there when P V two tiles ago is done, which was issued before: its probabilities may
-      // be overwritten)
-      mbar_pass_warp(&s_full[it % kScores], (it / kScores) & 1, a.status, kKernelId, 0x350u, abort_flag);
-      tc_fence_after();
-      float x[kRW];
-      sum_parts<kInt8, kRW, kR, 3>(lane_addr + it % kScores * kNS, x);
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&s_free[it % kScores]);
+#pragma unroll 1
+    for (int w = 0;; ++w) {
+      // the next part's queries first: its scores are computed while the results of the one before are written
+      pass_warp(&w_full[w & 1], (w >> 1) & 1, a.status, 0x3d0u, abort_flag);
+      Work next = works[w & 1];
+      // (a wait that ran out ends all warps at the same place: what they would read is not there; and all warps are done
+      // with the rows' factors)
+      if (any_of<kSoft>(*abort_flag != 0u)) next.q_start = -1;
+      if (next.q_start >= 0) queries(next, w);
+      if (w > 0) {
+        pass_warp(&o_done[(t - 1) & 1], ((t - 1) >> 1) & 1, a.status, 0x380u, abort_flag);
+        tc_fence_after();
+        drain();
+        tc_fence_before();
+        // sums over the tokens
+        int mine;
+        const float sum = sums_of_rows<kRW>(l, lane, mine);
+        warp_top[(warp & 3) * kR + row0 + mine] = *abort_flag != 0u ? 0.0f : sum;
+        if (k.part >= 0 && (warp & 3) == 0 && lane == 0) {
 #pragma unroll
-      for (int r = 0; r < kRW; ++r) x[r] *= row_factor[row0 + r] * scale.x;
-      int tok = 0;
-      bool lost = false;                    // no row sees the token
-      if (!all_whole) {
-        const int c = c0 + it * 8 + c16;
-        const bool there = c < c1;
-        tok = first_token(c) + (i_tok & 15);
-        lost = !there || tok > p.hi_pos || (a.window > 0 && tok <= p.lo_pos - a.window && tok >= a.first);
-#pragma unroll
-        for (int r = 0; r < kRW; ++r) {
-          const int pos = row_pos[row0 + r];
-          if (!there || tok > pos || (a.window > 0 && tok <= pos - a.window && tok >= a.first)) x[r] = -INFINITY;
-        }
-      }
-      // exponents, relative to the running maximum (in place: a new maximum moves them on)
-      float top = -INFINITY;
-#pragma unroll
-      for (int r = 0; r < kRW; ++r) {
-        x[r] += scale.y - (m[r] == -INFINITY ? 0.0f : m[r]);
-        top = fmaxf(top, m[r] == -INFINITY && x[r] > -INFINITY ? INFINITY : x[r]);
-      }
-      if (any_of<kSoft>(top > kRaise || (kInt8 && it % kMostTiles == kMostTiles - 1))) {
-        // new maxima of all rows; the sums in tensor memory belong to the old ones
-#pragma unroll
-        for (int r = 0; r < kRW; ++r) {
-          const float t = warp_top_of(x[r]);
-          if (lane == 0) warp_top[(warp & 3) * kR + row0 + r] = t;
+          for (int r = 0; r < kRW; ++r) row_lse[row0 + r] = m[r];
         }
         sync_softmax<kSoft>();
-        if (!drained) {
-          mbar_pass_warp(&o_done[(it - 1) & 1], ((it - 1) >> 1) & 1, a.status, kKernelId, 0x360u, abort_flag);
-          tc_fence_after();
-          drain();
-          tc_fence_before();
+        const int i = threadIdx.x;
+        if (i < kR) {
+          const float L = (warp_top[i] + warp_top[kR + i]) + (warp_top[2 * kR + i] + warp_top[3 * kR + i]);
+          row_inv[i] = L == 0.0f ? 0.0f : __fdividef(1.0f, L);
+          if (k.part >= 0 && k.row0 + i < k.rows)
+            a.tmp_lse[static_cast<long long>(k.part) * kR + i] = L == 0.0f ? -INFINITY : row_lse[i] + log2f(L);
         }
+        sync_softmax<kSoft>();
+        const int live = min(kR, k.rows - k.row0), d = i_tok;
+        const int2* place = row_place + ((w - 1) & 1) * kR + row0;
 #pragma unroll
         for (int r = 0; r < kRW; ++r) {
-          const float* t = warp_top + row0 + r;
-          const float over = fmaxf(fmaxf(t[0], t[kR]), fmaxf(t[2 * kR], t[3 * kR]));       // the old maximum
-          if (over > 0.0f || m[r] == -INFINITY) {
-            const float up = over == -INFINITY ? 0.0f : over;
-            const float corr = m[r] == -INFINITY ? 0.0f : ex2(-up);
-            m[r] = over == -INFINITY ? m[r] : m[r] == -INFINITY ? over : m[r] + over;
-            l[r] *= corr;
-            o[r] *= corr;
-            x[r] -= up;
+          const float inv = row_inv[row0 + r];
+          const float val = inv == 0.0f ? 0.0f : o[r] * inv;
+          if (row0 + r >= live) {
+          } else if (k.part >= 0) {
+            a.tmp_out[(static_cast<long long>(k.part) * kR + row0 + r) * 128 + d] = val;
+          } else {
+            static_cast<T*>(a.out)[place[r].x * a.ldo + place[r].y * 128 + d] = from_f32<T>(val);
+          }
+          m[r] = l[r] = o[r] = 0.0f;
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&w_empty[(w - 1) & 1]);
+      }
+      if (next.q_start < 0) break;
+      k = next;
+      uint32_t unseen = (1u << kRW) - 1u;   // rows of which no key was seen (the same in all warps): their maximum is 0
+      bool drained = true;                  // nothing of these maxima in tensor memory
+#pragma unroll 1
+      for (int it = 0; it < k.ntiles; ++it, ++t) {
+        const int g = groups + it / kGroup;
+        if (it % kGroup == 0)
+          pass_warp(&c_full[g % kGroups], (g / kGroups) & 1, a.status, 0x390u, abort_flag);
+        const float4 scale = chunk_scale[g % kGroups * 32 + it % kGroup * 8 + c16];
+        const bool all_whole = __all_sync(0xffffffffu, scale.w != 0.0f);
+        // (the scores of a tile are there when P V two tiles ago is done, which was issued before: its probabilities may
+        // be overwritten)
+        pass_warp(&s_full[t % kScores], (t / kScores) & 1, a.status, 0x350u, abort_flag);
+        tc_fence_after();
+        float x[kRW];
+        sum_parts<kInt8, kRW, kR, 3>(lane_addr + t % kScores * kNS, x);
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&s_free[t % kScores]);
+        // exponents, relative to the running maximum
+        float top = -INFINITY;
+#pragma unroll
+        for (int r = 0; r < kRW; ++r) x[r] = fmaf(x[r], row_factor[row0 + r] * scale.x, scale.y - m[r]);
+        bool lost = false;                  // no row sees the token
+        if (!all_whole) {
+          const int c = k.c0 + it * 8 + c16;
+          const bool there = c < k.c1;
+          const int tok = (c < k.firsts ? c : k.lo_chunk + c - k.firsts) * kChunk + (i_tok & 15);
+          lost = !there || tok > k.hi_pos || (a.window > 0 && tok <= k.lo_pos - a.window && tok >= a.first);
+#pragma unroll
+          for (int r = 0; r < kRW; ++r) {
+            const int pos = row_pos[row0 + r];
+            if (!there || tok > pos || (a.window > 0 && tok <= pos - a.window && tok >= a.first)) x[r] = -INFINITY;
           }
         }
-        sync_softmax<kSoft>();              // (warp_top is free again)
-        drained = true;
-      }
-      if (threadIdx.x == 0) adds[it & 1] = drained ? 0u : 1u;
-      drained = false;
-      uint8_t* sp = smem + S::kOffP + (it & 1) * kN * 128 + (i_tok & 15);
-      auto put = [&](int n, uint32_t byte) {
-        sp[(n >> 3) * 1024 + (n & 7) * 128 + ((c16 ^ (n & 7)) << 4)] = static_cast<uint8_t>(byte);
-      };
 #pragma unroll
-      for (int r = 0; r < kRW; r += 2) {
-        float v[2];
+        for (int r = 0; r < kRW; ++r) top = fmaxf(top, x[r]);
+        if (unseen != 0u) {
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          v[e] = ex2(x[r + e]);             // up to 16
-          l[r + e] = fmaf(v[e], scale.z, l[r + e]);
+          for (int r = 0; r < kRW; ++r)
+            if ((unseen >> r & 1u) != 0u && x[r] > -INFINITY) top = INFINITY;
         }
-        if constexpr (kInt8) {
+        if (any_of<kSoft>(top > kRaise || (kInt8 && it % kMostTiles == kMostTiles - 1))) {
+          // new maxima of all rows; the sums in tensor memory belong to the old ones
+#pragma unroll
+          for (int r = 0; r < kRW; ++r) {
+            const float up = warp_top_of(x[r]);
+            if (lane == 0) warp_top[(warp & 3) * kR + row0 + r] = up;
+          }
+          sync_softmax<kSoft>();
+          if (!drained) {
+            pass_warp(&o_done[(t - 1) & 1], ((t - 1) >> 1) & 1, a.status, 0x360u, abort_flag);
+            tc_fence_after();
+            drain();
+            tc_fence_before();
+          }
+#pragma unroll
+          for (int r = 0; r < kRW; ++r) {
+            const float* w4 = warp_top + row0 + r;
+            const float up = fmaxf(fmaxf(w4[0], w4[kR]), fmaxf(w4[2 * kR], w4[3 * kR]));   // over the old maximum
+            const bool seen = (unseen >> r & 1u) == 0u;
+            if (seen ? up > 0.0f : up > -INFINITY) {
+              const float corr = seen ? ex2(-up) : 0.0f;
+              m[r] += up;
+              l[r] *= corr;
+              o[r] *= corr;
+              x[r] -= up;
+              unseen &= ~(1u << r);
+            }
+          }
+          sync_softmax<kSoft>();            // (warp_top is free again)
+          drained = true;
+        }
+        if (threadIdx.x == 0) adds[t & 1] = drained ? 0u : 1u;
+        drained = false;
+        // (rows of a warp start at a multiple of 8 columns: their places in a group of eight are constants)
+        uint8_t* sp = smem + S::kOffP + (t & 1) * kN * 128 + row0 * 128 + (i_tok & 15);
+        auto put = [&](int n, uint32_t byte) {
+          sp[(n >> 3) * 1024 + (n & 7) * 128 + ((c16 ^ (n & 7)) << 4)] = static_cast<uint8_t>(byte);
+        };
+#pragma unroll
+        for (int r = 0; r < kRW; r += 2) {
+          float v[2];
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            const uint32_t f = min(__float2uint_rn(v[e] * kUnit), (1u << 28) - 1u);
-#pragma unroll
-            for (int k = 0; k < kParts; ++k) put(k * kR + row0 + r + e, f >> 7 * (kParts - 1 - k) & 127u);
+            v[e] = ex2(x[r + e]);           // up to 16
+            l[r + e] = fmaf(v[e], scale.z, l[r + e]);
           }
-        } else {
-          uint32_t q[3];
-          parts_e4m3(pack_half(v[0] * kUnit, v[1] * kUnit), q);
+          if constexpr (kInt8) {
 #pragma unroll
-          for (int k = 0; k < 3; ++k) {
-            put(k * kR + row0 + r, q[k]);
-            put(k * kR + row0 + r + 1, q[k] >> 8);
+            for (int e = 0; e < 2; ++e) {
+              const uint32_t f = min(__float2uint_rn(v[e] * kUnit), (1u << 28) - 1u);
+#pragma unroll
+              for (int j = 0; j < kParts; ++j) put(j * kR + r + e, f >> 7 * (kParts - 1 - j) & 127u);
+            }
+          } else {
+            uint32_t q[3];
+            parts_e4m3(pack_half(v[0] * kUnit, v[1] * kUnit), q);
+#pragma unroll
+            for (int j = 0; j < 3; ++j) {
+              put(j * kR + r, q[j]);
+              put(j * kR + r + 1, q[j] >> 8);
+            }
           }
         }
-      }
-      if (lost && warp < 4) {
-        // what lies behind the last key, in a gap that no row sees, or was not loaded may be anything
-        mbar_wait(&v_full[it % kStages], (it / kStages) & 1, a.status, kKernelId, 0x3a0u, abort_flag);
-        uint4* v = reinterpret_cast<uint4*>(smem + (kStages + it % kStages) * kTcBytes + i_tok * 128);
+        if (lost && warp < 4) {
+          // what lies behind the last key, in a gap that no row sees, or was not loaded may be anything
+          wait_one(&v_full[t % kStages], (t / kStages) & 1, a.status, 0x3a0u, abort_flag);
+          uint4* v = reinterpret_cast<uint4*>(smem + (kStages + t % kStages) * kTcBytes + i_tok * 128);
 #pragma unroll
-        for (int k = 0; k < 8; ++k) v[k ^ (lane & 7)] = make_uint4(0u, 0u, 0u, 0u);
+          for (int j = 0; j < 8; ++j) v[j ^ (lane & 7)] = make_uint4(0u, 0u, 0u, 0u);
+        }
+        fence_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_full[t & 1]);
       }
-      fence_async_smem();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&p_full[it & 1]);
-    }
-    if (ntiles > 0) {
-      mbar_pass_warp(&o_done[(ntiles - 1) & 1], ((ntiles - 1) >> 1) & 1, a.status, kKernelId, 0x380u, abort_flag);
-      tc_fence_after();
-      drain();
-      tc_fence_before();
-    }
-    // sums over the tokens
-#pragma unroll
-    for (int r = 0; r < kRW; ++r) {
-      const float sum = warp_sum(l[r]);
-      if (lane == 0) warp_top[(warp & 3) * kR + row0 + r] = *abort_flag != 0u ? 0.0f : sum;
-    }
-    sync_softmax<kSoft>();
-#pragma unroll
-    for (int r = 0; r < kRW; ++r) {
-      if (row0 + r >= live) break;
-      const float* t = warp_top + row0 + r;
-      const float L = (t[0] + t[kR]) + (t[2 * kR] + t[3 * kR]);
-      const float val = L == 0.0f ? 0.0f : o[r] / L;
-      const float lse = L == 0.0f ? -INFINITY : (m[r] == -INFINITY ? 0.0f : m[r]) + log2f(L);
-      const int d = i_tok;
-      if constexpr (kCluster) {
-        part_o[(row0 + r) * 128 + d] = val;
-        if (d == 0) part_lse[row0 + r] = lse;
-        continue;
-      }
-      const int row = p.row0 + row0 + r, token = p.q_start + row / p.G, head = p.kvh * p.G + row % p.G;
-      if (a.splits > 1) {
-        const long long base = (static_cast<long long>(token) * a.Hq + head) * a.splits + split;
-        a.tmp_out[base * 128 + d] = val;
-        if (d == 0) a.tmp_lse[base] = lse;
-      } else {
-        static_cast<T*>(a.out)[static_cast<long long>(token) * a.ldo + head * 128 + d] = from_f32<T>(val);
-      }
+      groups += (k.ntiles + kGroup - 1) / kGroup;
     }
   }
   tc_fence_before();
   __syncthreads();
   if (warp == kWarps + 1) tmem_dealloc(tmem, S::kAlloc);
-  if constexpr (kCluster) merge_cluster<T, 128>(a, p, live, part_lse, part_o);
 }
 
-template <typename T, bool kInt8, int kR, bool kCluster>
-int launch_tc(const CUtensorMap& tmK, const CUtensorMap& tmV, const Args& a, cudaStream_t s) {
+// Parts of a request's rows that several CTAs computed, a warp a row: by the CTA whose number is that of the second of
+// them.
+template <typename T>
+__global__ void __launch_bounds__(128) merge_units_kernel(const Args a, int kR) {
+  grid_release_small();
+  grid_wait();
+  const int4 unit = a.units[blockIdx.x];           // request, row block, first and last share
+  const int kvh = static_cast<int>(blockIdx.x) % a.Hkv, share = static_cast<int>(blockIdx.x) / a.Hkv;
+  if (unit.x < 0 || unit.z != share - 1) return;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int q_start = a.cu_q != nullptr ? a.cu_q[unit.x] : unit.x;
+  const int G = a.Hq / a.Hkv, rows = (a.cu_q != nullptr ? a.cu_q[unit.x + 1] - q_start : 1) * G;
+  const int parts = unit.w - unit.z + 1;
+  // the first share's part is its last one, the others' is their first
+  auto place = [&](int i) { return static_cast<long long>(2 * ((unit.z + i) * a.Hkv + kvh) + (i == 0 ? 1 : 0)) * kR; };
+  for (int r = warp; r < min(kR, rows - unit.y * kR); r += 4) {
+    float M = -INFINITY;
+    for (int i = lane; i < parts; i += 32) M = fmaxf(M, a.tmp_lse[place(i) + r]);
+    M = warp_max(M);
+    float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    float sum = 0.0f;
+    for (int i0 = 0; i0 < parts; i0 += 32) {
+      const float lse = i0 + lane < parts ? a.tmp_lse[place(i0 + lane) + r] : -INFINITY;
+      const float mine = lse == -INFINITY ? 0.0f : exp2f(lse - M);
+#pragma unroll 4
+      for (int i = i0; i < min(parts, i0 + 32); ++i) {
+        const float w = __shfl_sync(0xffffffffu, mine, i - i0);
+        const float4 x = reinterpret_cast<const float4*>(a.tmp_out + (place(i) + r) * 128)[lane];
+        sum += w;
+        o.x = fmaf(w, x.x, o.x);
+        o.y = fmaf(w, x.y, o.y);
+        o.z = fmaf(w, x.z, o.z);
+        o.w = fmaf(w, x.w, o.w);
+      }
+    }
+    const int row = unit.y * kR + r, token = q_start + row / G, head = kvh * G + row % G;
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+    T* out = static_cast<T*>(a.out) + static_cast<long long>(token) * a.ldo + head * 128 + lane * 4;
+    T v[4] = {from_f32<T>(o.x * inv), from_f32<T>(o.y * inv), from_f32<T>(o.z * inv), from_f32<T>(o.w * inv)};
+    *reinterpret_cast<uint2*>(out) = *reinterpret_cast<const uint2*>(v);
+  }
+}
+
+// CTAs that run at the same time.
+template <bool kInt8>
+int tc_slots(int rows) {
+  const int ctas = rows == 4 ? Tc<kInt8, 4>::kCtas : rows == 8 ? Tc<kInt8, 8>::kCtas
+                   : rows == 16 ? Tc<kInt8, 16>::kCtas : Tc<kInt8, 32>::kCtas;
+  return ctas * sm_count();
+}
+
+template <typename T, bool kInt8, int kR>
+int launch_tc(const CUtensorMap& tmK, const CUtensorMap& tmV, const Args& a, int ctas, cudaStream_t s) {
   using S = Tc<kInt8, kR>;
   static_assert(S::kBytes * S::kCtas + 1024 * S::kCtas <= 233472, "shared memory of the CTAs of an SM");
-  static_assert(kR * 128 * 4 <= S::kOffQ, "merge buffers must fit");
   static bool done[64] = {};
-  return launch_splits(rows_tc_kernel<T, kInt8, kR, kCluster>, done, S::kThreads, S::kBytes, kCluster, a, tmK, tmV, s);
+  const int e = set_shared(rows_tc_kernel<T, kInt8, kR>, done, S::kBytes);
+  if (e != 0) return e;
+  const int r = launch_overlapped(rows_tc_kernel<T, kInt8, kR>, dim3(ctas), dim3(S::kThreads), S::kBytes, s, tmK, tmV, a);
+  if (r != 0) return r;
+  return launch_overlapped(merge_units_kernel<T>, dim3(ctas), dim3(128), 0, s, a, kR);
 }
 
 }  // namespace rows8

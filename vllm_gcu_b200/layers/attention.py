@@ -252,7 +252,7 @@ class PagedAttention(nn.Module):
         out = q.new_empty((T, Hq * D)) if n == T else q.new_zeros((T, Hq * D))
         if nd > 0:
             C.block_scaled_decode(q[:nd].view(nd, Hq, D), *parts, md.block_tables[:nd], md.seq_lens[:nd], self.scale,
-                                  out=out[:nd].view(nd, Hq, D), workspace=md.decode_workspace,
+                                  out=out[:nd].view(nd, Hq, D),
                                   max_seq_len=md.max_seq_len, window=self.window, first=self.window_first)
         if md.num_prefills > 0:
             C.block_scaled_prefill(q[nd:].view(T - nd, Hq, D), *parts, md.block_tables[lo:B], md.cu_q_prefill,

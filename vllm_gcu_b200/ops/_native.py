@@ -178,6 +178,7 @@ class _Sigs:
     b200_block_scaled_cache = [S, P]
     b200_block_scaled_expand = [S, P]
     b200_block_scaled_rows = [S, P]
+    b200_block_scaled_slots = [I, I]
     b200_fmha_expanded = [S, P]
     b200_cache_pages = [S, P]
     b200_gemm_wna16 = [P, L, P, P, P, P, P, L, I, I, I, I, I, P]

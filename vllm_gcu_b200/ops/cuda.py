@@ -1874,7 +1874,7 @@ def group_norm_gate(x: torch.Tensor, z: Optional[torch.Tensor], weight: torch.Te
 # ---------------------------------------------------------------------------
 _SCALED_WRITE = struct.Struct("7P4q8i")
 _SCALED_EXPAND = struct.Struct("10Pq12i")
-_SCALED_ROWS = struct.Struct("11P3qf15i")
+_SCALED_ROWS = struct.Struct("12P3qf15i")
 _EXPANDED_CALL = struct.Struct("7P2qf11i")
 _PAGES_CALL = struct.Struct("7Pq6i")
 _SCALED_WIDTHS = (64, 128, 256)       # head dimensions of these kernels
@@ -1944,7 +1944,7 @@ def block_scaled_cache(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, 
 
 
 def block_scaled_splits(requests: int, heads: int, max_seq_len: int) -> int:
-    """Splits of the keys that ``block_scaled_decode`` takes for so many requests and key heads."""
+    """Splits of the keys that ``block_scaled_decode`` takes for so many requests and key heads of 64 or 256."""
     ctas = requests * heads
     if ctas <= 0 or max_seq_len <= 256:
         return 1
@@ -1997,38 +1997,54 @@ def _visible(window: int, first: int) -> tuple[int, int]:
     return int(window), int(first)
 
 
+@functools.lru_cache(maxsize=None)
+def _scaled_slots(rows: int, int8: bool, dev: int) -> tuple[int, int]:
+    """Rows of a CTA of the kernel for head dimension 128, and CTAs that run at the same time."""
+    with torch.cuda.device(dev):
+        got = N.lib().b200_block_scaled_slots(rows, int(int8))
+    return got >> 16, got & 0xffff
+
+
 def _scaled_rows(q, pq, ldq, out, po, ldo, k_cache, v_cache, k_scale, v_scale, cu_q, seq_lens, tables, B, max_blocks, max_q,
-                 scale, window, first, splits, workspace, shape) -> None:
+                 scale, window, first, splits, seen, shape) -> None:
     nb, bs, H, D, row, int8, dev = shape
     T, Hq = q.shape[0], q.shape[1]
-    tmp_out = tmp_lse = None
-    if splits > 8:
-        if workspace is None:
-            tmp_out = torch.empty(T * Hq * splits * D, device=q.device, dtype=torch.float32)
-            tmp_lse = torch.empty(T * Hq * splits, device=q.device, dtype=torch.float32)
-        else:
-            tmp_out, tmp_lse = workspace
-            for t, n in ((tmp_out, T * Hq * splits * D), (tmp_lse, T * Hq * splits)):
-                if t.numel() < n or t.dtype is not torch.float32 or not t.is_contiguous() or t.get_device() != dev:
-                    raise ValueError(f"workspace: contiguous float32 numbers are wanted, {T * Hq * splits * D} and "
-                                     f"{T * Hq * splits} of them for {splits} splits")
+    if dev < 0:
+        raise ValueError("tensors on a GPU are wanted")
+    G, units = Hq // H, 0
+    if D == 128:
+        # an even share of a key head's tiles for each CTA: as many as run at once, or (splits) so many a request
+        per, slots = _scaled_slots(min(33, max_q * G), int8, dev)
+        units = B * H * -(-max_q * G // per)
+        splits = max(1, min(units * splits, 1 << 16) if splits else min(slots, units * -(-seen // 128)))
+        splits = max(splits // H, 1) * H
+        need = 2 * splits * per * 128, 2 * splits * per
+    else:
+        splits = splits or block_scaled_splits(B, H * -(-max_q * G // 32), seen)
+        if cu_q:
+            splits = min(splits, 8)         # (the rest of the rows are another launch's)
+        need = (T * Hq * splits * D, T * Hq * splits) if splits > 8 else (0, 0)
+    tmp_out = tmp_lse = 0
+    if need[0]:
+        room = torch.empty(need[0] + need[1] + (4 * splits if units else 0), device=q.device, dtype=torch.float32)
+        tmp_out = room.data_ptr()
+        tmp_lse = tmp_out + 4 * need[0]
     _call_on(dev, "b200_block_scaled_rows",
              _SCALED_ROWS.pack(pq, po, k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), cu_q,
-                               seq_lens, tables, 0 if tmp_out is None else tmp_out.data_ptr(),
-                               0 if tmp_lse is None else tmp_lse.data_ptr(), ldq, ldo, row, scale, T, B, max_q, Hq, H, D,
-                               splits, max_blocks, bs, nb, window, first, int8, DTYPE_CODE[q.dtype], 0))
+                               seq_lens, tables, tmp_out, tmp_lse, tmp_lse + 4 * need[1] if units else 0, ldq, ldo, row,
+                               scale, T, B, max_q, Hq, H, D, splits, max_blocks, bs, nb, window, first, int8,
+                               DTYPE_CODE[q.dtype], 0))
 
 
 def block_scaled_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor,
                         v_scale: torch.Tensor, block_tables: torch.Tensor, seq_lens: torch.Tensor, scale: float,
-                        out: Optional[torch.Tensor] = None, num_splits: int = 0,
-                        workspace: Optional[tuple[torch.Tensor, torch.Tensor]] = None, max_seq_len: int = 0,
+                        out: Optional[torch.Tensor] = None, num_splits: int = 0, max_seq_len: int = 0,
                         window: int = 0, first: int = 0) -> torch.Tensor:
     """Attention of one token of each request over a cache that ``block_scaled_cache`` wrote: ``q [B, Hq, D]`` (bf16 or
     fp16, row stride free), ``block_tables [B, blocks]`` and ``seq_lens [B]`` int32 (the token itself counts; 0: a row of
-    zeros).  ``window``: only the last so many keys, and the ``first`` ones of the request (0: all keys).  ``num_splits``
-    0 chooses by ``max_seq_len`` (a bound of seq_lens; default: what the tables hold); more than 8 splits, up to 32, use
-    ``workspace`` (fp32, B * Hq * splits * D and B * Hq * splits numbers), by default a new one."""
+    zeros).  ``window``: only the last so many keys, and the ``first`` ones of the request (0: all keys).  ``num_splits``:
+    parts (up to 32) that the keys of a request and key head are taken in, on the mean where heads have 128 columns; 0
+    chooses by ``max_seq_len``, a bound of seq_lens (default: what the tables hold)."""
     shape = _scaled_cache(k_cache, v_cache, k_scale, v_scale)
     _, bs, H, D, _, _, dev = shape
     Hq, q, pq, ldq, out, po, ldo = _scaled_query(q, out, H, D, dev, (k_cache, v_cache))
@@ -2045,12 +2061,8 @@ def block_scaled_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.T
         seen = min(seen, window + first)
     if not 0 <= num_splits <= 32:
         raise ValueError(f"{num_splits} splits, up to 32 are built")
-    splits = num_splits or block_scaled_splits(B, H * -(-(Hq // H) // 32), seen)
-    if workspace is not None and num_splits == 0:
-        while splits > 8 and (workspace[0].numel() < B * Hq * splits * D or workspace[1].numel() < B * Hq * splits):
-            splits -= 1
     _scaled_rows(q, pq, ldq, out, po, ldo, k_cache, v_cache, k_scale, v_scale, 0, lens, tables, B, M, 1, scale, window,
-                 first, splits, workspace, shape)
+                 first, num_splits, seen, shape)
     return out
 
 
@@ -2095,9 +2107,8 @@ def block_scaled_prefill(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
                 continue
             if window:
                 seen = min(seen, window + max_q + first)
-            splits = block_scaled_splits(hi - lo, H * -(-max_q * G // 32), seen)
             _scaled_rows(q, pq, ldq, out, po, ldo, k_cache, v_cache, k_scale, v_scale, cu + 4 * lo, lens + 4 * lo,
-                         tables + 4 * lo * M, hi - lo, M, max_q, scale, window, first, min(splits, 8), None, shape)
+                         tables + 4 * lo * M, hi - lo, M, max_q, scale, window, first, 0, seen, shape)
             continue
         tiles = [_expanded_tiles(n, k, window, first) for n, k in zip(q_lens[lo:hi], kv_lens[lo:hi])]
         while lo < hi:
