@@ -51,7 +51,7 @@ struct Eight {
 // maximum and their codes.  A run that does not start its block raises the block's scale where a number does not fit, and
 // rounds the codes in front of it anew.
 template <typename T, bool kInt8, bool kWide, int D>
-__global__ void __launch_bounds__(256) write_kernel(const WriteArgs a) {
+__global__ void __launch_bounds__(256, sizeof(T) == 4 || D == 256 ? 2 : 4) write_kernel(const WriteArgs a) {
   grid_release_small();
   grid_wait();
   constexpr int kLanes = D / 8, kRows = 32 / kLanes;      // lanes of a row, rows of a pass
@@ -84,17 +84,22 @@ __global__ void __launch_bounds__(256) write_kernel(const WriteArgs a) {
     starts &= starts - 1u;
     const int page = __shfl_sync(0xffffffffu, mine, first - row0);
     const long long slot0 = static_cast<long long>(page) * a.block_size;
-    const int off = static_cast<int>(a.slots[first] - slot0);
     const long long at = static_cast<long long>(page) * a.H + h;
-    const float old = off > 0 ? scales[at] : 0.0f;
-    int n = 0;                                            // rows of the run
+    float old = scales[at];
+    // places of the run's first 32 rows, a lane each, and its rows
+    int place = -1, n = 0;
+#pragma unroll 1
     for (int base = 0; base < a.block_size; base += 32) {
       const int t = first + base + lane;
-      const bool in = base + lane < a.block_size && t < a.T && a.slots[t] >= slot0 && a.slots[t] < slot0 + a.block_size;
-      const uint32_t out = __ballot_sync(0xffffffffu, !in);
+      const long long in = t < a.T && base + lane < a.block_size ? a.slots[t] - slot0 : -1;
+      const bool ours = in >= 0 && in < a.block_size;
+      if (base == 0) place = static_cast<int>(in);
+      const uint32_t out = __ballot_sync(0xffffffffu, !ours);
       n = base + (out != 0u ? __ffs(out) - 1 : 32);
       if (out != 0u) break;
     }
+    const int off = __shfl_sync(0xffffffffu, place, 0);
+    if (off == 0) old = 0.0f;
     Eight<T, kWide> held[kHold];
     float top = 0.0f;
 #pragma unroll
@@ -105,6 +110,7 @@ __global__ void __launch_bounds__(256) write_kernel(const WriteArgs a) {
 #pragma unroll
     for (int i = 0; i < kHold; ++i)
       if (i * kRows + lane / kLanes < n) top = fmaxf(top, held[i].top());
+#pragma unroll 1
     for (int r = kHold * kRows + lane / kLanes; r < n; r += kRows) {
       Eight<T, kWide> e;
       e.load(src + (first + r) * ld);
@@ -129,8 +135,8 @@ __global__ void __launch_bounds__(256) write_kernel(const WriteArgs a) {
         *p = w;
       }
     }
-    auto store = [&](const Eight<T, kWide>& e, int r) {
-      const long long slot = a.slots[first + r];
+    auto store = [&](const Eight<T, kWide>& e, int r, int in) {
+      const long long slot = in >= 0 ? slot0 + in : a.slots[first + r];
       uint2 w;
       w.x = codes4<kInt8>(e.at(0) * unit, e.at(1) * unit, e.at(2) * unit, e.at(3) * unit);
       w.y = codes4<kInt8>(e.at(4) * unit, e.at(5) * unit, e.at(6) * unit, e.at(7) * unit);
@@ -139,14 +145,16 @@ __global__ void __launch_bounds__(256) write_kernel(const WriteArgs a) {
 #pragma unroll
     for (int i = 0; i < kHold; ++i) {
       const int r = i * kRows + lane / kLanes;
-      if (r < n) store(held[i], r);
+      const int in = __shfl_sync(0xffffffffu, place, r);
+      if (r < n) store(held[i], r, in);
     }
+#pragma unroll 1
     for (int r = kHold * kRows + lane / kLanes; r < n; r += kRows) {
       Eight<T, kWide> e;
       e.load(src + (first + r) * ld);
-      store(e, r);
+      store(e, r, -1);
     }
-    if (lane == 0 && scale != old) scales[at] = scale;
+    if (lane == 0 && (scale != old || off == 0)) scales[at] = scale;
   }
 }
 

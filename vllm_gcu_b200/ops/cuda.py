@@ -1885,29 +1885,40 @@ SCALED_EXPANDED_KEYS = 1 << 17
 
 
 def _scaled_cache(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor):
-    """Checks a cache of codes and scales: (blocks, block size, heads, head dimension, bytes of a token, int8, device)."""
+    """Checks a cache of codes and scales: (blocks, block size, heads, head dimension, bytes of a token, int8, device,
+    the four addresses).  (One expression where all is well: single tokens take microseconds.)"""
+    shape, stride, dtype, dev = k_cache.shape, k_cache.stride(), k_cache.dtype, k_cache.get_device()
+    if len(shape) == 4:
+        nb, bs, H, D = shape
+        row, pk, pv = stride[1], k_cache.data_ptr(), v_cache.data_ptr()
+        if ((dtype is FP8 or dtype is torch.int8) and v_cache.dtype is dtype and v_cache.shape == shape
+                and v_cache.stride() == stride and stride[0] == bs * row and stride[2] == D and stride[3] == 1
+                and row >= H * D and (pk | pv | row | bs) % 16 == 0 and D in _SCALED_WIDTHS and 0 < nb * bs < 1 << 31
+                and v_cache.get_device() == dev and k_scale.shape == (nb, H) and v_scale.shape == (nb, H)
+                and k_scale.dtype is torch.float32 and v_scale.dtype is torch.float32 and k_scale.is_contiguous()
+                and v_scale.is_contiguous() and k_scale.get_device() == dev and v_scale.get_device() == dev):
+            return nb, bs, H, D, row, dtype is torch.int8, dev, pk, pv, k_scale.data_ptr(), v_scale.data_ptr()
+    _refuse_scaled_cache(k_cache, v_cache, k_scale, v_scale)
+
+
+def _refuse_scaled_cache(k_cache, v_cache, k_scale, v_scale) -> None:
+    """What is wrong with a cache of codes and scales."""
     if k_cache.dim() != 4 or v_cache.shape != k_cache.shape:
         raise ValueError(f"caches [blocks, block size, heads, head dimension] of one shape are wanted, got "
                          f"{tuple(k_cache.shape)} and {tuple(v_cache.shape)}")
     nb, bs, H, D = k_cache.shape
-    dtype, dev = k_cache.dtype, k_cache.get_device()
-    if dtype is not FP8 and dtype is not torch.int8 or v_cache.dtype is not dtype:
+    if k_cache.dtype not in (FP8, torch.int8) or v_cache.dtype is not k_cache.dtype:
         raise ValueError(f"codes of float8_e4m3fn or int8 are wanted, got {k_cache.dtype} and {v_cache.dtype}")
-    if D not in _SCALED_WIDTHS or bs % 16 or not nb:
+    if D not in _SCALED_WIDTHS or bs % 16 or not 0 < nb * bs < 1 << 31:
         raise ValueError(f"{nb} blocks of {bs} tokens, heads of {D}: blocks of a multiple of 16 tokens and heads of "
                          f"{_SCALED_WIDTHS} are built")
-    row = k_cache.stride(1)
-    for name, t in (("k_cache", k_cache), ("v_cache", v_cache)):
-        if t.stride() != (bs * row, row, D, 1) or row < H * D or row % 16 or t.data_ptr() % 16 or t.get_device() != dev:
-            raise ValueError(f"{name}: tokens that follow each other at equal distances of a multiple of 16 bytes are "
-                             f"wanted, both caches alike on one device, got strides {tuple(t.stride())} on {t.device}")
-    if nb * bs >= 1 << 31:
-        raise ValueError(f"a cache of {nb * bs} tokens")
     for name, t in (("k_scale", k_scale), ("v_scale", v_scale)):
-        if t.shape != (nb, H) or t.dtype is not torch.float32 or not t.is_contiguous() or t.get_device() != dev:
+        if t.shape != (nb, H) or t.dtype is not torch.float32 or not t.is_contiguous() or t.device != k_cache.device:
             raise ValueError(f"{name}: contiguous float32 scales of shape {(nb, H)} beside the cache are wanted, got "
                              f"{t.dtype}, {tuple(t.shape)} on {t.device}")
-    return nb, bs, H, D, row, dtype is torch.int8, dev
+    raise ValueError(f"k_cache and v_cache: tokens that follow each other at equal distances of a multiple of 16 bytes are "
+                     f"wanted, both caches alike on one device, got strides {tuple(k_cache.stride())} on {k_cache.device} "
+                     f"and {tuple(v_cache.stride())} on {v_cache.device}")
 
 
 def _indices(name: str, t: torch.Tensor, shape, dev: int, dtype=torch.int32) -> int:
@@ -1927,20 +1938,21 @@ def block_scaled_cache(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, 
     A scale is a power of two.  A block whose first place is written starts anew, with the least scale (2^-100 .. 2^121)
     that holds the rows' numbers; else the scale stays, or grows where a number does not fit, and the codes in front of the
     new rows are rounded to it.  Infinities become the largest code and NaN the code 0; neither counts for the scale."""
-    nb, bs, H, D, row, int8, dev = _scaled_cache(k_cache, v_cache, k_scale, v_scale)
-    if k.dtype not in DTYPE_CODE or k.dim() != 2:
-        raise ValueError(f"k: rows of bf16, fp16 or fp32 are wanted, got {k.dtype} of shape {tuple(k.shape)}")
-    T, es = k.shape[0], k.element_size()
-    ldk = _row_view("k", k, T, H * D, (k.dtype,), dev)
-    ldv = _row_view("v", v, T, H * D, (k.dtype,), dev)
+    nb, bs, H, D, row, int8, dev, pkc, pvc, pks, pvs = _scaled_cache(k_cache, v_cache, k_scale, v_scale)
+    dtype = k.dtype
+    if dtype not in DTYPE_CODE or k.dim() != 2:
+        raise ValueError(f"k: rows of bf16, fp16 or fp32 are wanted, got {dtype} of shape {tuple(k.shape)}")
+    T = k.shape[0]
+    ldk = _row_view("k", k, T, H * D, (dtype,), dev)
+    ldv = _row_view("v", v, T, H * D, (dtype,), dev)
     slots = _indices("slot_mapping", slot_mapping, (T,), dev, torch.int64)
     if T == 0:
         return
     pk, pv = k.data_ptr(), v.data_ptr()
-    wide = (pk | pv) % 16 == 0 and (T == 1 or (ldk | ldv) * es % 16 == 0)
+    wide = (pk | pv) % 16 == 0 and (T == 1 or (ldk | ldv) * dtype.itemsize % 16 == 0)
     _call_on(dev, "b200_block_scaled_cache",
-             _SCALED_WRITE.pack(pk, pv, k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
-                                slots, ldk, ldv, row, nb * bs, T, H, D, bs, wide, int8, DTYPE_CODE[k.dtype], 0))
+             _SCALED_WRITE.pack(pk, pv, pkc, pvc, pks, pvs, slots, ldk, ldv, row, nb * bs, T, H, D, bs, wide, int8,
+                                DTYPE_CODE[dtype], 0))
 
 
 def block_scaled_splits(requests: int, heads: int, max_seq_len: int) -> int:
@@ -1952,43 +1964,43 @@ def block_scaled_splits(requests: int, heads: int, max_seq_len: int) -> int:
     return max(1, min(want, max_seq_len // 128, 8 if max_seq_len < 8 * 2048 else 32))
 
 
-def _scaled_query(q: torch.Tensor, out: Optional[torch.Tensor], H: int, D: int, dev: int, caches):
-    """Checks queries and their output: (query heads, address and pitch of q, out, address and pitch of out)."""
-    if q.dim() != 3 or q.dtype not in (torch.bfloat16, torch.float16):
-        raise ValueError(f"q: [tokens, heads, head dimension] of bf16 or fp16 is wanted, got {q.dtype} of shape "
-                         f"{tuple(q.shape)}")
-    T, Hq, Dq = q.shape
+def _scaled_query(q: torch.Tensor, out: Optional[torch.Tensor], shape):
+    """Checks queries and their output: (tokens, query heads, q, its address and pitch, out, its address and pitch)."""
+    nb, bs, H, D, row, _, dev, pk, pv, _, _ = shape
+    size, stride, dtype = q.shape, q.stride(), q.dtype
+    if len(size) != 3 or dtype is not torch.bfloat16 and dtype is not torch.float16:
+        raise ValueError(f"q: [tokens, heads, head dimension] of bf16 or fp16 is wanted, got {dtype} of shape {tuple(size)}")
+    T, Hq, Dq = size
     if Dq != D or not Hq or Hq % H:
         raise ValueError(f"q has {Hq} heads of {Dq}, the cache {H} heads of {D}")
-    ld, pq = q.stride(0), q.data_ptr()
-    if q.stride(2) != 1 or (q.stride(1) != D and Hq > 1) or q.get_device() != dev:
-        raise ValueError(f"q: heads that follow each other beside the cache are wanted, got strides {tuple(q.stride())} "
+    if stride[2] != 1 or stride[1] != D and Hq > 1 or q.get_device() != dev:
+        raise ValueError(f"q: heads that follow each other beside the cache are wanted, got strides {tuple(stride)} "
                          f"on {q.device}")
-    if pq % 16 or (ld % 8 and T > 1):
+    width, pq, ld = Hq * D, q.data_ptr(), stride[0]
+    if T == 1:
+        ld = width
+    if pq % 16 or ld % 8:
         q = q.contiguous()
-        ld, pq = q.stride(0), q.data_ptr()
-    if T == 1:
-        ld = Hq * D
+        ld, pq = width, q.data_ptr()
     if out is None:
-        out = torch.empty((T, Hq, D), dtype=q.dtype, device=q.device)
-        return Hq, q, pq, ld, out, out.data_ptr(), Hq * D
-    ldo, po = out.stride(0), out.data_ptr()
-    if out.shape != (T, Hq, D) or out.dtype is not q.dtype or out.get_device() != dev or out.stride(2) != 1 \
-            or (out.stride(1) != D and Hq > 1):
-        raise ValueError(f"out: {q.dtype} of shape {(T, Hq, D)} with heads that follow each other is wanted, got "
-                         f"{out.dtype}, {tuple(out.shape)}, strides {tuple(out.stride())}")
-    if T == 1:
-        ldo = Hq * D
-    if po % 16 or ldo % 8 or ldo < Hq * D:
+        out = torch.empty(size, dtype=dtype, device=q.device)
+        return T, Hq, q, pq, ld, out, out.data_ptr(), width
+    stride, po = out.stride(), out.data_ptr()
+    if out.shape != size or out.dtype is not dtype or out.get_device() != dev or stride[2] != 1 or stride[1] != D and Hq > 1:
+        raise ValueError(f"out: {dtype} of shape {tuple(size)} with heads that follow each other is wanted, got "
+                         f"{out.dtype}, {tuple(out.shape)}, strides {tuple(stride)}")
+    ldo = stride[0] if T != 1 else width
+    if po % 16 or ldo % 8 or ldo < width:
         raise ValueError(f"out: rows of a multiple of 8 elements that start at 16 bytes and share none are wanted, got a "
                          f"pitch of {ldo}")
-    if T and _overlap((po, ldo, T, Hq * D, 2), (pq, ld, T, Hq * D, 2)):
-        raise ValueError("out shares memory with q")
-    for c in caches:
-        if T and po < c.data_ptr() + ((c.shape[0] * c.shape[1] - 1) * c.stride(1) + H * D) \
-                and c.data_ptr() < po + ((T - 1) * ldo + Hq * D) * 2:
+    if T:
+        end = po + ((T - 1) * ldo + width) * 2
+        if not (pq >= end or pq + ((T - 1) * ld + width) * 2 <= po) and _overlap((po, ldo, T, width, 2), (pq, ld, T, width, 2)):
+            raise ValueError("out shares memory with q")
+        held = (nb * bs - 1) * row + H * D
+        if po < pk + held and pk < end or po < pv + held and pv < end:
             raise ValueError("out shares memory with the cache")
-    return Hq, q, pq, ld, out, po, ldo
+    return T, Hq, q, pq, ld, out, po, ldo
 
 
 def _visible(window: int, first: int) -> tuple[int, int]:
@@ -2005,35 +2017,33 @@ def _scaled_slots(rows: int, int8: bool, dev: int) -> tuple[int, int]:
     return got >> 16, got & 0xffff
 
 
-def _scaled_rows(q, pq, ldq, out, po, ldo, k_cache, v_cache, k_scale, v_scale, cu_q, seq_lens, tables, B, max_blocks, max_q,
-                 scale, window, first, splits, seen, shape) -> None:
-    nb, bs, H, D, row, int8, dev = shape
-    T, Hq = q.shape[0], q.shape[1]
+def _scaled_rows(shape, T, Hq, dtype, pq, ldq, po, ldo, cu_q, seq_lens, tables, B, max_blocks, max_q, scale, window, first,
+                 splits, seen) -> None:
+    nb, bs, H, D, row, int8, dev, pk, pv, pks, pvs = shape
     if dev < 0:
         raise ValueError("tensors on a GPU are wanted")
-    G, units = Hq // H, 0
+    G = Hq // H
     if D == 128:
         # an even share of a key head's tiles for each CTA: as many as run at once, or (splits) so many a request
         per, slots = _scaled_slots(min(33, max_q * G), int8, dev)
         units = B * H * -(-max_q * G // per)
         splits = max(1, min(units * splits, 1 << 16) if splits else min(slots, units * -(-seen // 128)))
         splits = max(splits // H, 1) * H
-        need = 2 * splits * per * 128, 2 * splits * per
+        out, lse = 2 * splits * per * 128, 2 * splits * per
+        room = torch.empty(out + lse + 4 * splits, device=torch.device("cuda", dev), dtype=torch.float32).data_ptr()
+        lse, units = room + 4 * out, room + 4 * (out + lse)
     else:
         splits = splits or block_scaled_splits(B, H * -(-max_q * G // 32), seen)
         if cu_q:
             splits = min(splits, 8)         # (the rest of the rows are another launch's)
-        need = (T * Hq * splits * D, T * Hq * splits) if splits > 8 else (0, 0)
-    tmp_out = tmp_lse = 0
-    if need[0]:
-        room = torch.empty(need[0] + need[1] + (4 * splits if units else 0), device=q.device, dtype=torch.float32)
-        tmp_out = room.data_ptr()
-        tmp_lse = tmp_out + 4 * need[0]
+        room = lse = units = 0
+        if splits > 8:
+            out = T * Hq * splits * D
+            room = torch.empty(out + T * Hq * splits, device=torch.device("cuda", dev), dtype=torch.float32).data_ptr()
+            lse = room + 4 * out
     _call_on(dev, "b200_block_scaled_rows",
-             _SCALED_ROWS.pack(pq, po, k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), cu_q,
-                               seq_lens, tables, tmp_out, tmp_lse, tmp_lse + 4 * need[1] if units else 0, ldq, ldo, row,
-                               scale, T, B, max_q, Hq, H, D, splits, max_blocks, bs, nb, window, first, int8,
-                               DTYPE_CODE[q.dtype], 0))
+             _SCALED_ROWS.pack(pq, po, pk, pv, pks, pvs, cu_q, seq_lens, tables, room, lse, units, ldq, ldo, row, scale, T, B,
+                               max_q, Hq, H, D, splits, max_blocks, bs, nb, window, first, int8, DTYPE_CODE[dtype], 0))
 
 
 def block_scaled_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor,
@@ -2046,10 +2056,10 @@ def block_scaled_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.T
     parts (up to 32) that the keys of a request and key head are taken in, on the mean where heads have 128 columns; 0
     chooses by ``max_seq_len``, a bound of seq_lens (default: what the tables hold)."""
     shape = _scaled_cache(k_cache, v_cache, k_scale, v_scale)
-    _, bs, H, D, _, _, dev = shape
-    Hq, q, pq, ldq, out, po, ldo = _scaled_query(q, out, H, D, dev, (k_cache, v_cache))
-    B = q.shape[0]
-    window, first = _visible(window, first)
+    bs, dev = shape[1], shape[6]
+    B, Hq, q, pq, ldq, out, po, ldo = _scaled_query(q, out, shape)
+    if window or first:
+        window, first = _visible(window, first)
     M = block_tables.shape[1] if block_tables.dim() == 2 else 0
     tables, lens = _indices("block_tables", block_tables, (B, M), dev), _indices("seq_lens", seq_lens, (B,), dev)
     if B == 0:
@@ -2061,8 +2071,7 @@ def block_scaled_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.T
         seen = min(seen, window + first)
     if not 0 <= num_splits <= 32:
         raise ValueError(f"{num_splits} splits, up to 32 are built")
-    _scaled_rows(q, pq, ldq, out, po, ldo, k_cache, v_cache, k_scale, v_scale, 0, lens, tables, B, M, 1, scale, window,
-                 first, num_splits, seen, shape)
+    _scaled_rows(shape, B, Hq, q.dtype, pq, ldq, po, ldo, 0, lens, tables, B, M, 1, scale, window, first, num_splits, seen)
     return out
 
 
@@ -2082,9 +2091,9 @@ def block_scaled_prefill(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
     at position ``seq_lens[b] - 1``.  ``q_lens`` and ``kv_lens`` hold the same numbers on the host.  Rows of no request are
     left as they are.  Requests of few tokens read the codes as they are; for longer ones the keys and values that their
     tokens can see are expanded to 16 bits, at most ``SCALED_EXPANDED_KEYS`` keys (or one request's) at a time."""
-    shape = nb, bs, H, D, row, int8, dev = _scaled_cache(k_cache, v_cache, k_scale, v_scale)
-    Hq, q, pq, ldq, out, po, ldo = _scaled_query(q, out, H, D, dev, (k_cache, v_cache))
-    T, B = q.shape[0], len(q_lens)
+    shape = nb, bs, H, D, row, int8, dev, *caches = _scaled_cache(k_cache, v_cache, k_scale, v_scale)
+    T, Hq, q, pq, ldq, out, po, ldo = _scaled_query(q, out, shape)
+    B = len(q_lens)
     window, first = _visible(window, first)
     M = block_tables.shape[1] if block_tables.dim() == 2 else 0
     tables = _indices("block_tables", block_tables, (B, M), dev)
@@ -2107,8 +2116,8 @@ def block_scaled_prefill(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
                 continue
             if window:
                 seen = min(seen, window + max_q + first)
-            _scaled_rows(q, pq, ldq, out, po, ldo, k_cache, v_cache, k_scale, v_scale, cu + 4 * lo, lens + 4 * lo,
-                         tables + 4 * lo * M, hi - lo, M, max_q, scale, window, first, 0, seen, shape)
+            _scaled_rows(shape, T, Hq, q.dtype, pq, ldq, po, ldo, cu + 4 * lo, lens + 4 * lo, tables + 4 * lo * M, hi - lo, M,
+                         max_q, scale, window, first, 0, seen)
             continue
         tiles = [_expanded_tiles(n, k, window, first) for n, k in zip(q_lens[lo:hi], kv_lens[lo:hi])]
         while lo < hi:
@@ -2118,15 +2127,14 @@ def block_scaled_prefill(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
                 n += 1
             if count:
                 width = -(-max(kv_lens[lo:lo + n]) // 128)
-                keys, values = torch.empty((2, count * 128, H * D), dtype=q.dtype, device=q.device)
-                table = torch.empty((n, width), dtype=torch.int32, device=q.device)
+                size = count * 256 * H * D              # bytes of the keys, or values
+                room = torch.empty(2 * size + 4 * n * width, dtype=torch.uint8, device=q.device).data_ptr()
                 at = cu + 4 * lo, lens + 4 * lo
                 _call_on(dev, "b200_block_scaled_expand", _SCALED_EXPAND.pack(
-                    k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), keys.data_ptr(),
-                    values.data_ptr(), table.data_ptr(), *at, tables + 4 * lo * M, row, n, H, D, bs, M, nb, width, count,
-                    window, first, int8, DTYPE_CODE[q.dtype]))
+                    *caches, room, room + size, room + 2 * size, *at, tables + 4 * lo * M, row, n, H, D, bs, M, nb, width,
+                    count, window, first, int8, DTYPE_CODE[q.dtype]))
                 _call_on(dev, "b200_fmha_expanded", _EXPANDED_CALL.pack(
-                    pq, po, keys.data_ptr(), values.data_ptr(), *at, table.data_ptr(), ldq, ldo, scale, T, n, Hq, H, D,
+                    pq, po, room, room + size, *at, room + 2 * size, ldq, ldo, scale, T, n, Hq, H, D,
                     count, width, sum(-(-m // 128) for m in q_lens[lo:lo + n]), window, first, DTYPE_CODE[q.dtype]))
             tiles = tiles[n:]
             lo += n
