@@ -587,16 +587,23 @@ __global__ void __launch_bounds__(Tc<kInt8, kR>::kThreads, Tc<kInt8, kR>::kCtas)
     // ---------------- queries of a part ----------------
     auto queries = [&](const Work& k, int w) {
       const int live = min(kR, k.rows - k.row0);
-#pragma unroll 1
-      for (int r = warp; r < kR; r += kWarps) {
-        const int row = k.row0 + r;
-        // row / G: half a G off the next whole number, and 2^-23 of itself wrong
-        const int token = __float2int_rd((static_cast<float>(row) + 0.5f) * inv_g), head = k.kvh * G + row - token * G;
-        uint2 raw = make_uint2(0u, 0u);
+      constexpr int kMine = kR / kWarps;
+      uint2 raws[kMine];
+      // row / G: half a G off the next whole number, and 2^-23 of itself wrong
+      auto token_of = [&](int r) { return __float2int_rd((static_cast<float>(k.row0 + r) + 0.5f) * inv_g); };
+#pragma unroll
+      for (int i = 0; i < kMine; ++i) {
+        const int r = warp + i * kWarps, token = token_of(r), head = k.kvh * G + k.row0 + r - token * G;
+        raws[i] = make_uint2(0u, 0u);
         if (r < live)
-          raw = *reinterpret_cast<const uint2*>(static_cast<const T*>(a.q) +
-                                                static_cast<long long>(k.q_start + token) * a.ldq + head * 128 + lane * 4);
-        const T* e = reinterpret_cast<const T*>(&raw);
+          raws[i] = *reinterpret_cast<const uint2*>(static_cast<const T*>(a.q) +
+                                                    static_cast<long long>(k.q_start + token) * a.ldq + head * 128 + lane * 4);
+      }
+#pragma unroll
+      for (int mine = 0; mine < kMine; ++mine) {
+        const int r = warp + mine * kWarps;
+        const int token = token_of(r), head = k.kvh * G + k.row0 + r - token * G;
+        const T* e = reinterpret_cast<const T*>(&raws[mine]);
         float x[4], top = 0.0f;
         bool number = true;
 #pragma unroll

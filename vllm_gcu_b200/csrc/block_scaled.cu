@@ -36,11 +36,29 @@ struct Eight {
       for (int i = 0; i < 8; ++i) e[i] = p[i];
     }
   }
-  __device__ __forceinline__ float at(int i) const { return to_f32<T>(reinterpret_cast<const T*>(raw)[i]); }
+  __device__ __forceinline__ float at(int i) const {
+    if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+      const uint32_t w = reinterpret_cast<const uint32_t*>(raw)[i >> 1];
+      return __uint_as_float((i & 1) != 0 ? w & 0xffff0000u : w << 16);
+    } else {
+      return to_f32<T>(reinterpret_cast<const T*>(raw)[i]);
+    }
+  }
+  // largest magnitude of the finite ones
   __device__ __forceinline__ float top() const {
     float m = 0.0f;
 #pragma unroll
     for (int i = 0; i < 8; ++i) m = fmaxf(m, finite_size(at(i)));
+    return m;
+  }
+  // largest bits behind the sign, of 16-bit types in pairs: the order of magnitudes, infinities and NaN above all others
+  __device__ __forceinline__ uint32_t top_bits(uint32_t m) const {
+    const uint32_t* w = reinterpret_cast<const uint32_t*>(raw);
+#pragma unroll
+    for (int i = 0; i < static_cast<int>(sizeof(raw) / 4); ++i) {
+      if constexpr (sizeof(T) == 4) m = max(m, w[i] & 0x7fffffffu);
+      else m = __vmaxu2(m, w[i] & 0x7fff7fffu);
+    }
     return m;
   }
 };
@@ -101,22 +119,45 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 || D == 256 ? 2 : 4) write
     const int off = __shfl_sync(0xffffffffu, place, 0);
     if (off == 0) old = 0.0f;
     Eight<T, kWide> held[kHold];
-    float top = 0.0f;
+    uint32_t bits = 0u;
 #pragma unroll
     for (int i = 0; i < kHold; ++i) {
       const int r = i * kRows + lane / kLanes;
+#pragma unroll
+      for (int j = 0; j < static_cast<int>(sizeof(held[0].raw) / 16); ++j) held[i].raw[j] = make_uint4(0u, 0u, 0u, 0u);
       if (r < n) held[i].load(src + (first + r) * ld);
     }
 #pragma unroll
-    for (int i = 0; i < kHold; ++i)
-      if (i * kRows + lane / kLanes < n) top = fmaxf(top, held[i].top());
+    for (int i = 0; i < kHold; ++i) bits = held[i].top_bits(bits);
 #pragma unroll 1
     for (int r = kHold * kRows + lane / kLanes; r < n; r += kRows) {
       Eight<T, kWide> e;
       e.load(src + (first + r) * ld);
-      top = fmaxf(top, e.top());
+      bits = e.top_bits(bits);
     }
-    const float need = power_of_two(scale_exponent<kInt8>(warp_max(top)));
+    if constexpr (sizeof(T) == 2) bits = max(bits & 0xffffu, bits >> 16);
+    bits = __reduce_max_sync(0xffffffffu, bits);
+    // (rare: numbers that are none, which do not count, and sizes above what the largest scale holds)
+    constexpr uint32_t kInfinity = sizeof(T) == 4 ? 0x7f800000u : std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
+    float top;
+    if (bits < kInfinity) {
+      if constexpr (sizeof(T) == 4) {
+        top = __uint_as_float(bits);
+      } else {
+        const uint16_t half = static_cast<uint16_t>(bits);
+        top = to_f32<T>(*reinterpret_cast<const T*>(&half));
+      }
+    } else {
+      top = 0.0f;
+      for (int r = lane / kLanes; r < n; r += kRows) {
+        Eight<T, kWide> e;
+        e.load(src + (first + r) * ld);
+        top = fmaxf(top, e.top());
+      }
+      top = warp_max(top);
+    }
+    const float need = power_of_two(scale_exponent<kInt8>(top));
+    const bool plain = bits < kInfinity && need < power_of_two(kHighExponent);
     const float scale = old > need ? old : need;          // (old may be anything where nothing was written yet)
     const float unit = 1.0f / scale;
     if (off > 0 && scale != old) {
@@ -135,12 +176,20 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 || D == 256 ? 2 : 4) write
         *p = w;
       }
     }
+    uint8_t* block = cache + slot0 * a.slot_bytes;
+    const int pitch = static_cast<int>(a.slot_bytes);
     auto store = [&](const Eight<T, kWide>& e, int r, int in) {
-      const long long slot = in >= 0 ? slot0 + in : a.slots[first + r];
+      if (in < 0) in = static_cast<int>(a.slots[first + r] - slot0);
       uint2 w;
-      w.x = codes4<kInt8>(e.at(0) * unit, e.at(1) * unit, e.at(2) * unit, e.at(3) * unit);
-      w.y = codes4<kInt8>(e.at(4) * unit, e.at(5) * unit, e.at(6) * unit, e.at(7) * unit);
-      *reinterpret_cast<uint2*>(cache + slot * a.slot_bytes) = w;
+      if (plain) {
+        const float lo[4] = {e.at(0), e.at(1), e.at(2), e.at(3)}, hi[4] = {e.at(4), e.at(5), e.at(6), e.at(7)};
+        w.x = codes4_of<kInt8>(lo, unit);
+        w.y = codes4_of<kInt8>(hi, unit);
+      } else {
+        w.x = codes4<kInt8>(e.at(0) * unit, e.at(1) * unit, e.at(2) * unit, e.at(3) * unit);
+        w.y = codes4<kInt8>(e.at(4) * unit, e.at(5) * unit, e.at(6) * unit, e.at(7) * unit);
+      }
+      *reinterpret_cast<uint2*>(block + static_cast<long long>(in) * pitch) = w;
     };
 #pragma unroll
     for (int i = 0; i < kHold; ++i) {
@@ -247,17 +296,24 @@ __global__ void __launch_bounds__(256) expand_kernel(const ExpandArgs a) {
                          (static_cast<long long>(block) * a.block_size + key0 % a.block_size) * a.slot_bytes;
   const float* scales = (blockIdx.y == 0 ? a.ks : a.vs) + static_cast<long long>(block) * a.H;
   constexpr int kAtOnce = 4;
+  const int rows_on = 256 / vecs, on = 256 - rows_on * vecs, head_shift = a.D == 64 ? 2 : a.D == 128 ? 3 : 4;
+  int r = static_cast<int>(threadIdx.x) / vecs, c = static_cast<int>(threadIdx.x) - r * vecs;
   for (int i0 = threadIdx.x; i0 < 16 * vecs; i0 += 256 * kAtOnce) {
     uint4 w[kAtOnce];
     float scale[kAtOnce];
 #pragma unroll
     for (int u = 0; u < kAtOnce; ++u) {
-      const int i = i0 + u * 256, r = i / vecs, c = i - r * vecs;
       w[u] = make_uint4(0, 0, 0, 0);
       scale[u] = 0.0f;                                    // what no token sees is zeros
-      if (i < 16 * vecs && key0 + r < keys && (key0 + r >= gap || key0 + r < a.first)) {
+      if (r < 16 && key0 + r < keys && (key0 + r >= gap || key0 + r < a.first)) {
         w[u] = *reinterpret_cast<const uint4*>(cache + r * a.slot_bytes + c * 16);
-        scale[u] = scales[c * 16 / a.D];
+        scale[u] = scales[c >> head_shift];
+      }
+      r += rows_on;
+      c += on;
+      if (c >= vecs) {
+        c -= vecs;
+        ++r;
       }
     }
 #pragma unroll
@@ -304,10 +360,9 @@ struct CopyArgs {
   unsigned int* status;
 };
 
-// A CTA copies one block's piece of one tensor.  blockIdx.x: pair or answer, .y: tensors (strided), .z: piece.
-// (16 bytes a thread at a time, eight under way; entries of scales by words, others by bytes.)
-__device__ __forceinline__ void copy_bytes(const uint8_t* src, uint8_t* dst, long long bytes, int piece, int pieces) {
-  const int t = piece * static_cast<int>(blockDim.x) + threadIdx.x, step = pieces * static_cast<int>(blockDim.x);
+// blockIdx.x: pair or answer, .y: tensors (strided), .z: piece of a block.  16 bytes a thread at a time, four under way;
+// entries of scales by words, others by bytes.
+__device__ __forceinline__ void copy_bytes(const uint8_t* src, uint8_t* dst, long long bytes, int t, int step) {
   const unsigned long long low = reinterpret_cast<unsigned long long>(src) | reinterpret_cast<unsigned long long>(dst) |
                                  static_cast<unsigned long long>(bytes);
   if ((low & 15u) == 0u) {
@@ -332,7 +387,8 @@ __device__ __forceinline__ void copy_bytes(const uint8_t* src, uint8_t* dst, lon
   }
 }
 
-template <bool kFork>
+// kWarp: a warp a tensor (blocks of up to 16 KB: 64 forks in 128 tensors 10.0 us with a CTA for each, 5.9 so).
+template <bool kFork, bool kWarp>
 __global__ void __launch_bounds__(128) copy_kernel(const CopyArgs a) {
   grid_release_small();
   grid_wait();
@@ -363,11 +419,13 @@ __global__ void __launch_bounds__(128) copy_kernel(const CopyArgs a) {
     return;
   }
   if (src == dst) return;
-  for (int p = blockIdx.y; p < a.num_planes; p += gridDim.y) {
+  const int first = kWarp ? blockIdx.y * 4 + (threadIdx.x >> 5) : blockIdx.y, on = kWarp ? 4 * gridDim.y : gridDim.y;
+  const int t = kWarp ? threadIdx.x & 31 : blockIdx.z * 128 + threadIdx.x, step = kWarp ? 32 : a.pieces * 128;
+  for (int p = first; p < a.num_planes; p += on) {
     const Plane plane = a.planes[p];
     const long long bytes = kFork && plane.token_bytes > 0 ? used * plane.token_bytes : plane.block_bytes;
     uint8_t* base = reinterpret_cast<uint8_t*>(plane.base);
-    copy_bytes(base + src * plane.block_bytes, base + dst * plane.block_bytes, bytes, blockIdx.z, a.pieces);
+    copy_bytes(base + src * plane.block_bytes, base + dst * plane.block_bytes, bytes, t, step);
   }
 }
 
@@ -466,11 +524,18 @@ B200_API int b200_cache_pages(const void* call, void* stream) {
   a.seq_lens = k.seq_lens; a.parents = k.parents; a.fresh = k.fresh; a.out = k.out; a.n = k.n; a.width = k.width;
   a.num_requests = k.num_requests; a.block_size = k.block_size;
   a.status = status_ptr();
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  a.pieces = 1;
+  if (k.largest <= 16384) {
+    const int rows = (k.num_planes + 3) / 4;
+    const dim3 grid(k.n, rows < 1 ? 1 : rows < 65535 ? rows : 65535);
+    if (k.pairs != nullptr) return launch_overlapped(copy_kernel<false, true>, grid, dim3(128), 0, s, a);
+    return launch_overlapped(copy_kernel<true, true>, grid, dim3(128), 0, s, a);
+  }
   // 8 KB a CTA: four 16-byte pieces of a thread
   const long long pieces = (k.largest + 8191) / 8192;
-  a.pieces = static_cast<int>(pieces < 1 ? 1 : pieces > 64 ? 64 : pieces);
+  a.pieces = static_cast<int>(pieces > 64 ? 64 : pieces);
   const dim3 grid(k.n, k.num_planes < 1 ? 1 : k.num_planes < 65535 ? k.num_planes : 65535, a.pieces);
-  cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (k.pairs != nullptr) return launch_overlapped(copy_kernel<false>, grid, dim3(128), 0, s, a);
-  return launch_overlapped(copy_kernel<true>, grid, dim3(128), 0, s, a);
+  if (k.pairs != nullptr) return launch_overlapped(copy_kernel<false, false>, grid, dim3(128), 0, s, a);
+  return launch_overlapped(copy_kernel<true, false>, grid, dim3(128), 0, s, a);
 }

@@ -55,6 +55,30 @@ __device__ __forceinline__ uint32_t codes4(float a, float b, float c, float d) {
   }
 }
 
+// The same for numbers that are finite and reach no further than the largest code, without a look at each of them.  int8: in
+// 1.5 * 2^23 + x the last bits are x rounded to a whole number (one instruction with the product in front, where a
+// conversion has a quarter of the rate).
+template <bool kInt8>
+__device__ __forceinline__ uint32_t codes4_of(const float (&x)[4], float unit) {
+  if constexpr (kInt8) {
+    uint32_t b[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) b[i] = __float_as_uint(fmaf(x[i], unit, 12582912.0f));
+    return __byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410);
+  } else {
+    uint32_t r;
+    asm("{\n\t"
+        ".reg .b16 l, h;\n\t"
+        "cvt.rn.satfinite.e4m3x2.f32 l, %2, %1;\n\t"
+        "cvt.rn.satfinite.e4m3x2.f32 h, %4, %3;\n\t"
+        "mov.b32 %0, {l, h};\n\t"
+        "}"
+        : "=r"(r)
+        : "f"(x[0] * unit), "f"(x[1] * unit), "f"(x[2] * unit), "f"(x[3] * unit));
+    return r;
+  }
+}
+
 // Four codes of a word -> two pairs of fp16, exact: `lo` holds bytes 0 and 1, `hi` bytes 2 and 3.  int8: with the sign
 // bit turned a byte u is the last part of the fp16 number 1024 + u, less 1152 the code.
 template <bool kInt8>
