@@ -672,7 +672,7 @@ B200_API int b200_block_scaled_rows(const void* call, void* stream) {
   a.Hkv = k.Hkv; a.splits = k.splits; a.max_blocks = k.max_blocks; a.block_size = k.block_size;
   a.num_blocks = k.num_blocks; a.window = k.window; a.first = k.first; a.scale = k.scale;
   const long long row_blocks = (all + per - 1) / per;
-  if (k.B > 65535 || row_blocks * k.Hkv * k.B > 0x7fffffffll) return -2;
+  if (k.D != 128 && k.B > 65535) return -2;          // (a dimension of the grid)
   a.row_blocks = static_cast<int>(row_blocks);
   a.status = status_ptr();
   cudaStream_t s = static_cast<cudaStream_t>(stream);

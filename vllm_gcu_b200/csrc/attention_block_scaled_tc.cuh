@@ -195,9 +195,11 @@ struct Shares {
   }
 };
 
-// Sums of kRW numbers over the lanes of a warp, in kRW - 1 and a few exchanges: this lane has that of row `row`.
-template <int kRW>
-__device__ __forceinline__ float sums_of_rows(float (&v)[kRW], int lane, int& row) {
+// Sums, or largest, of kRW numbers over the lanes of a warp, in kRW - 1 and a few exchanges: this lane has that of row
+// `row`.  (NaN is passed over by the largest.)
+template <int kRW, bool kMax>
+__device__ __forceinline__ float over_lanes(float (&v)[kRW], int lane, int& row) {
+  auto join = [](float x, float y) { return kMax ? fmaxf(x, y) : x + y; };
   row = 0;
   int d = 16;
 #pragma unroll
@@ -207,11 +209,11 @@ __device__ __forceinline__ float sums_of_rows(float (&v)[kRW], int lane, int& ro
 #pragma unroll
     for (int i = 0; i < n; ++i) {
       const float keep = upper ? v[i + n] : v[i], give = upper ? v[i] : v[i + n];
-      v[i] = keep + __shfl_xor_sync(0xffffffffu, give, d);
+      v[i] = join(keep, __shfl_xor_sync(0xffffffffu, give, d));
     }
   }
 #pragma unroll
-  for (; d > 0; d >>= 1) v[0] += __shfl_xor_sync(0xffffffffu, v[0], d);
+  for (; d > 0; d >>= 1) v[0] = join(v[0], __shfl_xor_sync(0xffffffffu, v[0], d));
   return v[0];
 }
 
@@ -703,7 +705,7 @@ __global__ void __launch_bounds__(Tc<kInt8, kR>::kThreads, Tc<kInt8, kR>::kCtas)
         tc_fence_before();
         // sums over the tokens
         int mine;
-        const float sum = sums_of_rows<kRW>(l, lane, mine);
+        const float sum = over_lanes<kRW, false>(l, lane, mine);
         warp_top[(warp & 3) * kR + row0 + mine] = *abort_flag != 0u ? 0.0f : sum;
         if (k.part >= 0 && (warp & 3) == 0 && lane == 0) {
 #pragma unroll
@@ -780,11 +782,12 @@ __global__ void __launch_bounds__(Tc<kInt8, kR>::kThreads, Tc<kInt8, kR>::kCtas)
         }
         if (any_of<kSoft>(top > kRaise || (kInt8 && it % kMostTiles == kMostTiles - 1))) {
           // new maxima of all rows; the sums in tensor memory belong to the old ones
+          float tops[kRW];
 #pragma unroll
-          for (int r = 0; r < kRW; ++r) {
-            const float up = warp_top_of(x[r]);
-            if (lane == 0) warp_top[(warp & 3) * kR + row0 + r] = up;
-          }
+          for (int r = 0; r < kRW; ++r) tops[r] = x[r];
+          int mine;
+          const float largest = over_lanes<kRW, true>(tops, lane, mine);
+          warp_top[(warp & 3) * kR + row0 + mine] = largest == largest ? largest : -INFINITY;
           sync_softmax<kSoft>();
           if (!drained) {
             pass_warp(&o_done[(t - 1) & 1], ((t - 1) >> 1) & 1, a.status, 0x360u, abort_flag);
@@ -792,19 +795,21 @@ __global__ void __launch_bounds__(Tc<kInt8, kR>::kThreads, Tc<kInt8, kR>::kCtas)
             drain();
             tc_fence_before();
           }
+          // lane r has row r's
+          const float* w4 = warp_top + row0 + lane % kRW;
+          float up = fmaxf(fmaxf(w4[0], w4[kR]), fmaxf(w4[2 * kR], w4[3 * kR]));         // over the old maximum
+          const bool seen = (unseen >> lane % kRW & 1u) == 0u;
+          const bool moves = seen ? up > 0.0f : up > -INFINITY;
+          if (!moves) up = 0.0f;
+          const float corr = moves ? (seen ? ex2(-up) : 0.0f) : 1.0f;
+          unseen &= ~__ballot_sync(0xffffffffu, moves && lane < kRW);
 #pragma unroll
           for (int r = 0; r < kRW; ++r) {
-            const float* w4 = warp_top + row0 + r;
-            const float up = fmaxf(fmaxf(w4[0], w4[kR]), fmaxf(w4[2 * kR], w4[3 * kR]));   // over the old maximum
-            const bool seen = (unseen >> r & 1u) == 0u;
-            if (seen ? up > 0.0f : up > -INFINITY) {
-              const float corr = seen ? ex2(-up) : 0.0f;
-              m[r] += up;
-              l[r] *= corr;
-              o[r] *= corr;
-              x[r] -= up;
-              unseen &= ~(1u << r);
-            }
+            const float d = __shfl_sync(0xffffffffu, up, r), c = __shfl_sync(0xffffffffu, corr, r);
+            m[r] += d;
+            l[r] *= c;
+            o[r] *= c;
+            x[r] -= d;
           }
           sync_softmax<kSoft>();            // (warp_top is free again)
           drained = true;

@@ -2027,7 +2027,7 @@ def _scaled_rows(shape, T, Hq, dtype, pq, ldq, po, ldo, cu_q, seq_lens, tables, 
         # an even share of a key head's tiles for each CTA: as many as run at once, or (splits) so many a request
         per, slots = _scaled_slots(min(33, max_q * G), int8, dev)
         units = B * H * -(-max_q * G // per)
-        splits = max(1, min(units * splits, 1 << 16) if splits else min(slots, units * -(-seen // 128)))
+        splits = max(1, min(units * splits, 1 << 13) if splits else min(slots, units * -(-seen // 128)))
         splits = max(splits // H, 1) * H
         out, lse = 2 * splits * per * 128, 2 * splits * per
         room = torch.empty(out + lse + 4 * splits, device=torch.device("cuda", dev), dtype=torch.float32).data_ptr()
