@@ -67,6 +67,12 @@ __device__ __forceinline__ uint32_t pack_pair(float lo, float hi) {
   }
 }
 
+// Which of the 32 keys from `key0` on a row sees: those up to `hi`, of them those from `lo` on and those in front of `first`.
+__device__ __forceinline__ uint32_t seen_keys(int hi, int lo, int first, int key0) {
+  auto below = [](int n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u; };
+  return below(hi + 1 - key0) & (~below(lo - key0) | below(first - key0));
+}
+
 struct Args {
   __nv_bfloat16* out;      // [T, Hq * HD], row pitch ldo (kHalf kernels: fp16)
   float* lse;              // optional [Hq, T] (without the sink's term)
@@ -354,10 +360,11 @@ __global__ void __launch_bounds__(kThreads, 1)
             for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(biased(v[i], i, base));
           }
           if (need_mask) {
+            const uint32_t seen = kFirst ? seen_keys(hi, lo, a.first, key0 + c * 32) : 0u;
 #pragma unroll
             for (int i = 0; i < 32; ++i) {
               const int key = key0 + c * 32 + i;
-              if (key <= hi && (key >= lo || (kFirst && key < a.first))) mt = fmaxf(mt, __uint_as_float(v[i]));
+              if (kFirst ? (seen >> i & 1u) != 0u : key <= hi && key >= lo) mt = fmaxf(mt, __uint_as_float(v[i]));
             }
           } else {
             float m0 = mt, m1 = -INFINITY, m2 = -INFINITY, m3 = -INFINITY;
@@ -413,13 +420,14 @@ __global__ void __launch_bounds__(kThreads, 1)
           const float base =
               kBiased ? fmaf(slope2, static_cast<float>(key0 + c * 32 - pos), -mb) : 0.0f;
           if (need_mask) {
+            const uint32_t seen = kFirst ? seen_keys(hi, lo, a.first, key0 + c * 32) : 0u;
 #pragma unroll
             for (int i = 0; i < 32; i += 2) {
               const int key = key0 + c * 32 + i;
               float p0 = prob(v[i], i, base);
               float p1 = prob(v[i + 1], i + 1, base);
-              if (key > hi || (key < lo && !(kFirst && key < a.first))) p0 = 0.0f;
-              if (key + 1 > hi || (key + 1 < lo && !(kFirst && key + 1 < a.first))) p1 = 0.0f;
+              if (kFirst ? (seen >> i & 1u) == 0u : key > hi || key < lo) p0 = 0.0f;
+              if (kFirst ? (seen >> (i + 1) & 1u) == 0u : key + 1 > hi || key + 1 < lo) p1 = 0.0f;
               rs0 += p0;
               rs1 += p1;
               pk[c * 16 + (i >> 1)] = pack_pair<kHalf>(p0, p1);
