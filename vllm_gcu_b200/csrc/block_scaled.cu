@@ -236,8 +236,9 @@ struct ExpandArgs {
 
 constexpr int kTileKeys = 128;
 
-// 16 keys of a tile by a CTA, of keys (blockIdx.y 0) or values (1): a thread 16 codes at a time.  Bound by memory: one
-// byte read and two written, and most of what is written stays in L2 for the attention behind it.
+// 16 keys of a tile and their values by a CTA: a thread 8 codes at a time (one store of 16 bytes beside its neighbours'),
+// four of the keys and four of the values under way.  Bound by memory: one byte read and two written, and most of what is written stays in L2 for the attention behind
+// it.
 template <typename T, bool kInt8>
 __global__ void __launch_bounds__(256) expand_kernel(const ExpandArgs a) {
   grid_release_small();
@@ -280,10 +281,10 @@ __global__ void __launch_bounds__(256) expand_kernel(const ExpandArgs a) {
     base += __shfl_sync(0xffffffffu, inc, 31);
   }
   if (seq < 0) return;
-  if (threadIdx.x == 0 && part == 0 && blockIdx.y == 0) a.table[static_cast<long long>(seq) * a.table_width + key_tile] = tile;
+  if (threadIdx.x == 0 && part == 0) a.table[static_cast<long long>(seq) * a.table_width + key_tile] = tile;
   const int key0 = key_tile * kTileKeys + part * 16;
-  const int vecs = a.H * a.D / 16;                        // of a key
-  T* out = static_cast<T*>(blockIdx.y == 0 ? a.ko : a.vo) + (static_cast<long long>(tile) * kTileKeys + part * 16) * a.H * a.D;
+  const int vecs = a.H * a.D / 8;                         // of a key
+  const long long to = (static_cast<long long>(tile) * kTileKeys + part * 16) * a.H * a.D;
   int block = 0;
   if (key0 < keys) {
     block = a.block_tables[static_cast<long long>(seq) * a.max_blocks + key0 / a.block_size];
@@ -292,22 +293,28 @@ __global__ void __launch_bounds__(256) expand_kernel(const ExpandArgs a) {
       keys = 0;
     }
   }
-  const uint8_t* cache = (blockIdx.y == 0 ? a.kc : a.vc) +
-                         (static_cast<long long>(block) * a.block_size + key0 % a.block_size) * a.slot_bytes;
-  const float* scales = (blockIdx.y == 0 ? a.ks : a.vs) + static_cast<long long>(block) * a.H;
+  const long long from = (static_cast<long long>(block) * a.block_size + key0 % a.block_size) * a.slot_bytes;
+  const uint8_t* cache[2] = {a.kc + from, a.vc + from};
+  const float* scales[2] = {a.ks + static_cast<long long>(block) * a.H, a.vs + static_cast<long long>(block) * a.H};
+  T* out[2] = {static_cast<T*>(a.ko) + to, static_cast<T*>(a.vo) + to};
   constexpr int kAtOnce = 4;
-  const int rows_on = 256 / vecs, on = 256 - rows_on * vecs, head_shift = a.D == 64 ? 2 : a.D == 128 ? 3 : 4;
+  const int rows_on = 256 / vecs, on = 256 - rows_on * vecs, head_shift = a.D == 64 ? 3 : a.D == 128 ? 4 : 5;
   int r = static_cast<int>(threadIdx.x) / vecs, c = static_cast<int>(threadIdx.x) - r * vecs;
   for (int i0 = threadIdx.x; i0 < 16 * vecs; i0 += 256 * kAtOnce) {
-    uint4 w[kAtOnce];
-    float scale[kAtOnce];
+    uint2 w[2][kAtOnce];
+    float scale[2][kAtOnce];
 #pragma unroll
     for (int u = 0; u < kAtOnce; ++u) {
-      w[u] = make_uint4(0, 0, 0, 0);
-      scale[u] = 0.0f;                                    // what no token sees is zeros
-      if (r < 16 && key0 + r < keys && (key0 + r >= gap || key0 + r < a.first)) {
-        w[u] = *reinterpret_cast<const uint4*>(cache + r * a.slot_bytes + c * 16);
-        scale[u] = scales[c >> head_shift];
+      // what no token sees is zeros
+      const bool seen = r < 16 && key0 + r < keys && (key0 + r >= gap || key0 + r < a.first);
+#pragma unroll
+      for (int kv = 0; kv < 2; ++kv) {
+        w[kv][u] = make_uint2(0u, 0u);
+        scale[kv][u] = 0.0f;
+        if (seen) {
+          w[kv][u] = *reinterpret_cast<const uint2*>(cache[kv] + r * a.slot_bytes + c * 8);
+          scale[kv][u] = scales[kv][c >> head_shift];
+        }
       }
       r += rows_on;
       c += on;
@@ -320,20 +327,20 @@ __global__ void __launch_bounds__(256) expand_kernel(const ExpandArgs a) {
     for (int u = 0; u < kAtOnce; ++u) {
       const int i = i0 + u * 256;
       if (i >= 16 * vecs) break;
-      const uint32_t in[4] = {w[u].x, w[u].y, w[u].z, w[u].w};
-      float f[2][8];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        uint32_t lo, hi;
-        unpack4<kInt8>(in[j], lo, hi);
-        const float2 x = half_pair(lo), y = half_pair(hi);
-        float* o = &f[j >> 1][(j & 1) * 4];
-        // (a row of zeros is zeros whatever its codes would be: they were not loaded)
-        o[0] = x.x * scale[u]; o[1] = x.y * scale[u]; o[2] = y.x * scale[u]; o[3] = y.y * scale[u];
+      for (int kv = 0; kv < 2; ++kv) {
+        const uint32_t in[2] = {w[kv][u].x, w[kv][u].y};
+        float f[8];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          uint32_t lo, hi;
+          unpack4<kInt8>(in[j], lo, hi);
+          const float2 x = half_pair(lo), y = half_pair(hi);
+          f[4 * j] = x.x * scale[kv][u]; f[4 * j + 1] = x.y * scale[kv][u];
+          f[4 * j + 2] = y.x * scale[kv][u]; f[4 * j + 3] = y.y * scale[kv][u];
+        }
+        vec8_store<T>(out[kv] + static_cast<long long>(i) * 8, f);
       }
-      T* p = out + static_cast<long long>(i) * 16;
-      vec8_store<T>(p, f[0]);
-      vec8_store<T>(p + 8, f[1]);
     }
   }
 }
@@ -501,7 +508,7 @@ B200_API int b200_block_scaled_expand(const void* call, void* stream) {
   a.block_size = k.block_size; a.max_blocks = k.max_blocks; a.num_blocks = k.num_blocks;
   a.table_width = k.table_width; a.tiles = k.tiles; a.window = k.window; a.first = k.first;
   a.status = status_ptr();
-  const dim3 grid(k.tiles * (kTileKeys / 16), 2);
+  const dim3 grid(k.tiles * (kTileKeys / 16));
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (k.dtype == 0)
     return k.int8 ? launch_overlapped(expand_kernel<__nv_bfloat16, true>, grid, dim3(256), 0, s, a)
