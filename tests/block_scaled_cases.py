@@ -82,7 +82,7 @@ def allowed(out, size, reach, top, dtype, p_type, keys, width):
     probability's share); sums of ``keys`` terms in 32 bits, truncated.
 
     Where the codes meet 8-bit parts of a probability times its block's scale, the last part ends at a fixed place behind
-    the largest of them, which is 1 or more: int8 digits of a multiple of 2^-24 are off by 2^-25; e4m3 parts of 16 times
+    the largest of them, which is 1 or more: int8 digits of a multiple of 2^-26 are off by 2^-27; e4m3 parts of 16 times
     the number by half of the smallest step 2^-9 with weight 2^-8, 2^-18, which is 2^-22 of the number.  Each of ``keys``
     codes of at most 448 takes that part of ``top``.  (It shows where the keys that count have codes of 0.)"""
     p = torch.finfo(p_type).eps / 2 + 2 * (width + 8) * 2.0 ** -23 * reach[..., None] + (keys + 16) * 2.0 ** -22

@@ -7,8 +7,8 @@
 //   S^T = K Q^T    M = 128 tokens (K-major rows of 128 bytes), N = 3 kR columns: part x query row
 //   O^T = V^T P^T  M = 128 columns of the values (MN-major, as they lie), N = 3 or 4 kR columns, K = 128 tokens
 // e4m3: parts of 4 bits each, every one 16 times the rest of the one before, 12 bits together (probabilities are rounded
-// to fp16 before); int8: digits to the base 128 of a number of 21 bits, 28 for probabilities, whose small ones lose
-// bits where numbers of one size for all do not; the products' sums are exact.  A lane of the softmax warps owns a token: block scales are
+// to fp16 before); int8: digits to the base 128 of a number of 21 bits, of a probability to the base 256 of one of 30,
+// since those of many keys may be small beside the largest; the products' sums are exact.  A lane of the softmax warps owns a token: block scales are
 // factors of its scores and of its probabilities, and there is no conversion of codes at all, which is what bounds a kernel
 // that feeds 16-bit matrix instructions from 8-bit codes (attention_block_scaled.cu, head dimensions 64 and 256: there a
 // chunk of 16 tokens takes a warp 490 instructions, here 80 of them for four query rows).
@@ -21,7 +21,7 @@
 // request's start (block table, queries) overlaps with the end of the one before.  Where a share begins or ends inside a
 // request's keys, its part of the result goes to memory, and merge_units_kernel puts the parts together in their order.
 //
-// Warps: 0..3 (32 rows: 0..7) queries and softmax, lane = token of a tile and at the end column of the output; then one
+// Warps: four for every eight rows queries and softmax, lane = token of a tile and at the end column of the output; then one
 // for TMA, block tables and scales and one for tcgen05.mma and tensor memory.  K Q^T of a tile runs while the one before is
 // at its softmax; keys and values have places of their own, given back when their product is done.
 // The running maximum is raised when a score exceeds it by 4 (log2), which all softmax warps vote on; then the sums in
@@ -37,29 +37,29 @@ constexpr int kTcBytes = kTcTile * 128;      // of its keys, or values
 constexpr int kGroup = 4;                    // tiles whose block-table entries and scales a lane each of the TMA warp reads
 constexpr int kGroups = 4;                   // places for their scales
 constexpr float kRaise = 4.0f;               // log2, by which a score may exceed the running maximum
-constexpr int kMostTiles = 512;              // int8: whose sums of whole numbers one accumulator takes, 2^16 * 127 * 128 < 2^31
+constexpr int kMostTiles = 512;              // int8: whose sums of whole numbers one accumulator takes, 2^16 * 128 * 128 < 2^31
 
 template <bool kInt8, int kR>
 struct Tc {
   static constexpr int kParts = kInt8 ? 4 : 3;                 // of a probability
   static constexpr int kNS = (3 * kR + 15) / 16 * 16;          // columns of scores
   static constexpr int kN = (kParts * kR + 15) / 16 * 16;      // and of outputs
-  static constexpr int kWarps = kR == 32 ? 8 : 4;              // of the softmax
-  static constexpr int kRW = kR * 4 / kWarps;                  // rows of one of them
+  static constexpr int kRW = kR < 8 ? kR : 8;                  // rows of a softmax warp
+  static constexpr int kWarps = 4 * kR / kRW;
   static constexpr int kThreads = kWarps * 32 + 64;
   // CTAs of an SM, which hide each other's starts and ends, and places for keys and values of each
-  static constexpr int kCtas = kR == 4 ? 3 : 2;
-  static constexpr int kStages = kR == 8 ? 3 : 2;
-  static constexpr int kScores = kR == 32 ? 1 : 2;             // score buffers (32 rows: else one CTA had all of tensor memory)
+  static constexpr int kCtas = kR == 4 ? 3 : kR == 32 ? 1 : 2;
+  static constexpr int kStages = kR == 32 ? 5 : kR == 8 ? 3 : 2;
+  static constexpr int kScores = 2;                            // score buffers
   static constexpr int kColumns = kScores * kNS + kN;
-  static constexpr int kAlloc = kColumns <= 64 ? 64 : kColumns <= 128 ? 128 : 256;
-  static_assert(kColumns <= 256, "tensor memory of two CTAs");
+  static constexpr int kAlloc = kColumns <= 64 ? 64 : kColumns <= 128 ? 128 : kColumns <= 256 ? 256 : 512;
+  static_assert(kAlloc * kCtas <= 512, "tensor memory of an SM");
   static constexpr int kOffQ = 2 * kStages * kTcBytes;         // (keys, then values in front)
   static constexpr int kOffP = kOffQ + kNS * 128;
   static constexpr int kOffScale = kOffP + 2 * kN * 128;       // [kGroups][32] scales of keys, log2 and inverse of values', flag
   static constexpr int kOffBar = kOffScale + kGroups * 32 * 16;
-  static constexpr int kOffWork = kOffBar + 256;               // [2]
-  static constexpr int kOffRow = kOffWork + 128;               // factor and position of every row; [2] token and head
+  static constexpr int kOffWork = kOffBar + 384;               // [2]
+  static constexpr int kOffRow = kOffWork + 128;               // (16-byte places) factor and position of every row; [2] token and head
   static constexpr int kOffMax = kOffRow + 6 * kR * 4;         // of four warps and every row; inverse sum and log2 of them
   static constexpr int kBytes = kOffMax + 6 * kR * 4 + 1024;
 };
@@ -87,12 +87,19 @@ __device__ __forceinline__ void mma8(uint32_t d, uint64_t a, uint64_t b, uint32_
   else umma_f8(d, a, b, idesc, accumulate);
 }
 
+__device__ __forceinline__ void tmem_ld_32x8(uint32_t taddr, uint32_t (&r)[8]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+               : "r"(taddr)
+               : "memory");
+}
+
 // Numbers of a lane's columns, parts put together: column part * kStride + row -> [row].
-template <bool kInt8, int kRW, int kStride, int kParts>
+template <bool kInt8, int kRW, int kStride, int kParts, int kBits>
 __device__ __forceinline__ void sum_parts(uint32_t tmem, float (&s)[kRW]) {
-  // weights of the parts: 128^-p (the last digit's is 1) or 16^-p
+  // weights of the parts: of digits to the base 2^kBits (the last one's is 1), or 16^-p
   auto weight = [](int p) {
-    return kInt8 ? static_cast<float>(1 << 7 * (kParts - 1 - p)) : 1.0f / static_cast<float>(1 << 4 * p);
+    return kInt8 ? static_cast<float>(1 << kBits * (kParts - 1 - p)) : 1.0f / static_cast<float>(1 << 4 * p);
   };
   const float last = weight(kParts - 1);
   auto number = [](uint32_t u) { return kInt8 ? static_cast<float>(static_cast<int>(u)) : __uint_as_float(u); };
@@ -111,15 +118,18 @@ __device__ __forceinline__ void sum_parts(uint32_t tmem, float (&s)[kRW]) {
       }
     }
   } else {
-    static_assert(kStride <= 8 || kRW == 16, "one load a part");
-    // (part after part: registers)
+    uint32_t v[kParts][kRW];
+    static_assert(kRW == 8, "loads of eight columns");
 #pragma unroll
-    for (int p = kParts - 1; p >= 0; --p) {
-      uint32_t v[16];
-      tmem_ld_32x16(tmem + p * kStride, v);
-      tmem_ld_wait();
+    for (int p = 0; p < kParts; ++p) tmem_ld_32x8(tmem + p * kStride, v[p]);
+    tmem_ld_wait();
 #pragma unroll
-      for (int r = 0; r < kRW; ++r) s[r] = p == kParts - 1 ? number(v[r]) * last : fmaf(number(v[r]), weight(p), s[r]);
+    for (int r = 0; r < kRW; ++r) {
+#pragma unroll
+      for (int p = kParts - 1; p >= 0; --p) {
+        const float x = number(v[p][r]);
+        s[r] = p == kParts - 1 ? x * last : fmaf(x, weight(p), s[r]);
+      }
     }
   }
 }
@@ -281,7 +291,7 @@ __global__ void __launch_bounds__(Tc<kInt8, kR>::kThreads, Tc<kInt8, kR>::kCtas)
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(w_empty + 2);
   volatile uint32_t* abort_flag = tmem_slot + 1;
   volatile uint32_t* adds = tmem_slot + 2;  // [2]: whether P V of the buffer's tile adds to what is there
-  static_assert((4 * kStages + 9 + kGroups + 2 * kScores) * 8 + 16 <= 256, "barrier area");
+  static_assert((4 * kStages + 9 + kGroups + 2 * kScores) * 8 + 16 <= 384, "barrier area");
   static_assert(sizeof(Work) == 64, "place of the works");
   float4* chunk_scale = reinterpret_cast<float4*>(smem + S::kOffScale);
   Work* works = reinterpret_cast<Work*>(smem + S::kOffWork);
@@ -676,7 +686,7 @@ __global__ void __launch_bounds__(Tc<kInt8, kR>::kThreads, Tc<kInt8, kR>::kCtas)
     clear(kParts * kR, kN, S::kOffP + kN * 128);
 
     // ---------------- softmax: lane = token of the tile ----------------
-    constexpr float kUnit = kInt8 ? 16777216.0f : 16.0f;       // of a probability: 16 of them fill the parts
+    constexpr float kUnit = kInt8 ? 67108864.0f : 16.0f;       // of a probability: 16 of them (nearly) fill the parts
     int t = 0, groups = 0;
     Work k = {};
     float m[kRW], l[kRW], o[kRW];
@@ -685,7 +695,7 @@ __global__ void __launch_bounds__(Tc<kInt8, kR>::kThreads, Tc<kInt8, kR>::kCtas)
     // what P V of earlier tiles left in tensor memory
     auto drain = [&]() {
       float v[kRW];
-      sum_parts<kInt8, kRW, kR, kParts>(lane_addr + kScores * kNS, v);
+      sum_parts<kInt8, kRW, kR, kParts, 8>(lane_addr + kScores * kNS, v);
 #pragma unroll
       for (int r = 0; r < kRW; ++r) o[r] = fmaf(v[r], 1.0f / kUnit, o[r]);
     };
@@ -753,14 +763,20 @@ __global__ void __launch_bounds__(Tc<kInt8, kR>::kThreads, Tc<kInt8, kR>::kCtas)
         pass_warp(&s_full[t % kScores], (t / kScores) & 1, a.status, 0x350u, abort_flag);
         tc_fence_after();
         float x[kRW];
-        sum_parts<kInt8, kRW, kR, 3>(lane_addr + t % kScores * kNS, x);
+        sum_parts<kInt8, kRW, kR, 3, 7>(lane_addr + t % kScores * kNS, x);
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&s_free[t % kScores]);
         // exponents, relative to the running maximum
         float top = -INFINITY;
 #pragma unroll
-        for (int r = 0; r < kRW; ++r) x[r] = fmaf(x[r], row_factor[row0 + r] * scale.x, scale.y - m[r]);
+        for (int r = 0; r < kRW; r += 4) {
+          const float4 f = *reinterpret_cast<const float4*>(row_factor + row0 + r);
+          x[r] = fmaf(x[r], f.x * scale.x, scale.y - m[r]);
+          x[r + 1] = fmaf(x[r + 1], f.y * scale.x, scale.y - m[r + 1]);
+          x[r + 2] = fmaf(x[r + 2], f.z * scale.x, scale.y - m[r + 2]);
+          x[r + 3] = fmaf(x[r + 3], f.w * scale.x, scale.y - m[r + 3]);
+        }
         bool lost = false;                  // no row sees the token
         if (!all_whole) {
           const int c = k.c0 + it * 8 + c16;
@@ -832,9 +848,10 @@ __global__ void __launch_bounds__(Tc<kInt8, kR>::kThreads, Tc<kInt8, kR>::kCtas)
           if constexpr (kInt8) {
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-              const uint32_t f = min(__float2uint_rn(v[e] * kUnit), (1u << 28) - 1u);
+              // digits -128 .. 127: with 128 added to each but the first one they are the number's bytes
+              const uint32_t f = (__float2uint_rn(v[e] * kUnit) + 0x00808080u) ^ 0x00808080u;
 #pragma unroll
-              for (int j = 0; j < kParts; ++j) put(j * kR + r + e, f >> 7 * (kParts - 1 - j) & 127u);
+              for (int j = 0; j < kParts; ++j) put(j * kR + r + e, f >> 8 * (kParts - 1 - j));
             }
           } else {
             uint32_t q[3];
