@@ -201,3 +201,11 @@ def test_engine_config_knows_the_types():
     from vllm_gcu_b200.config import preset
     wide, small = (preset("llama-3-8b", kv_cache_dtype=t) for t in ("auto", "int8_block"))
     assert small.kv_bytes_per_token() * 2 == wide.kv_bytes_per_token()
+
+
+def test_long_documents_leave_the_wide_kernel_idle(monkeypatch):
+    """A few dozen rows behind one long document go by the kernel for few rows, a prompt does not."""
+    monkeypatch.setattr(C, "_sms", lambda: 148)
+    assert C._rows_pay([64], [250], 4, 8) and C._rows_pay([16] * 32, [16] * 32, 4, 8)
+    assert not C._rows_pay([32] * 64, [8] * 64, 4, 4) and not C._rows_pay([2048], [16], 8, 4)
+    assert not C._rows_pay([2048], [128], 8, 4)

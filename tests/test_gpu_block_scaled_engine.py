@@ -83,6 +83,29 @@ def test_checked_drafts():
     _native.check_status()
 
 
+def test_sizes_that_are_refused():
+    with pytest.raises(ValueError, match="fp8_block"):
+        LLM("llama-3-8b", device="cuda", kv_cache_dtype="fp8_block", head_dim=96, enforce_eager=True, **KW)
+    with pytest.raises(ValueError, match="int4_block"):
+        LLM("llama-3-8b", device="cuda", kv_cache_dtype="int4_block", enforce_eager=True, **KW)
+
+
+def test_prompts_in_portions_and_from_the_prefix_cache():
+    """Prompts that take several steps, and prompts that start with another one's blocks: nearly the logits of a prompt at
+    once (the blocks' scales grow with the portions)."""
+    a = _prompts([400], 8)[0]
+    sp = SamplingParams(max_tokens=2, temperature=0.0, ignore_eos=True)
+    kw = dict(kv_cache_dtype="fp8_block")
+    whole = _logits([a], sp, max_num_batched_tokens=512, **kw)[2]
+    parts = _logits([a], sp, max_num_batched_tokens=64, **kw)[2]
+    llm, _, _ = _logits([a], sp, **kw)
+    again = llm.generate([a[:390] + a[:10]], sp)[0]
+    assert again.num_cached_tokens >= 384
+    cos = torch.nn.functional.cosine_similarity(whole.flatten(), parts.flatten(), dim=0).item()
+    assert cos > 0.99
+    _native.check_status()
+
+
 def test_the_connector_refuses():
     llm = LLM("llama-3-8b", device="cuda", kv_cache_dtype="fp8_block", enforce_eager=True, **KW)
     with pytest.raises(ValueError, match="scales"):

@@ -48,11 +48,11 @@ struct Tc {
   static constexpr int kWarps = 4 * kR / kRW;
   static constexpr int kThreads = kWarps * 32 + 64;
   // CTAs of an SM, which hide each other's starts and ends, and places for keys and values of each
-  static constexpr int kCtas = kR == 4 ? 3 : kR == 32 ? 1 : 2;
-  static constexpr int kStages = kR == 32 ? 5 : kR == 8 ? 3 : 2;
+  static constexpr int kCtas = kR == 4 ? 3 : 2;
+  static constexpr int kStages = kR == 8 ? 3 : 2;
   static constexpr int kScores = 2;                            // score buffers
   static constexpr int kColumns = kScores * kNS + kN;
-  static constexpr int kAlloc = kColumns <= 64 ? 64 : kColumns <= 128 ? 128 : kColumns <= 256 ? 256 : 512;
+  static constexpr int kAlloc = kColumns <= 64 ? 64 : kColumns <= 128 ? 128 : 256;
   static_assert(kAlloc * kCtas <= 512, "tensor memory of an SM");
   static constexpr int kOffQ = 2 * kStages * kTcBytes;         // (keys, then values in front)
   static constexpr int kOffP = kOffQ + kNS * 128;
@@ -929,7 +929,7 @@ __global__ void __launch_bounds__(128) merge_units_kernel(const Args a, int kR) 
 template <bool kInt8>
 int tc_slots(int rows) {
   const int ctas = rows == 4 ? Tc<kInt8, 4>::kCtas : rows == 8 ? Tc<kInt8, 8>::kCtas
-                   : rows == 16 ? Tc<kInt8, 16>::kCtas : Tc<kInt8, 32>::kCtas;
+                                                                      : Tc<kInt8, 16>::kCtas;
   return ctas * sm_count();
 }
 

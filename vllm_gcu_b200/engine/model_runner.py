@@ -299,6 +299,9 @@ class ModelRunner:
         if kvd.endswith("_block") and self.is_cuda and spec["type"] == "gqa" and not self._block_scaled(spec):
             raise ValueError(f"kv_cache_dtype {mc.kv_cache_dtype!r}: fp8_block or int8_block")
         scaled = self.is_cuda and self._block_scaled(spec)
+        if scaled and (spec["head_dim"] not in (64, 128, 256) or self.block_size % 16):
+            raise ValueError(f"kv_cache_dtype {mc.kv_cache_dtype!r}: heads of 64, 128 or 256 and blocks of a multiple of 16 "
+                             f"tokens, not {spec['head_dim']} and {self.block_size}")
 
         def kv(blocks: int, heads: int, dim: int):
             if scaled:

@@ -1878,7 +1878,8 @@ _SCALED_ROWS = struct.Struct("12P3qf15i")
 _EXPANDED_CALL = struct.Struct("7P2qf11i")
 _PAGES_CALL = struct.Struct("7Pq6i")
 _SCALED_WIDTHS = (64, 128, 256)       # head dimensions of these kernels
-# Portions take the kernel for few rows up to this many query rows a key head, else keys are expanded to 16 bits
+# Portions of up to this many query rows a key head take the kernel for few rows; longer ones do where it is estimated to take
+# less time than keys that are expanded to 16 bits (0: keys are always expanded)
 SCALED_ROWS = 64
 # Keys that are expanded at once (a longer request alone): 2 x 2 bytes for each of a key's numbers
 SCALED_EXPANDED_KEYS = 1 << 17
@@ -2025,7 +2026,7 @@ def _scaled_rows(shape, T, Hq, dtype, pq, ldq, po, ldo, cu_q, seq_lens, tables, 
     G = Hq // H
     if D == 128:
         # an even share of a key head's tiles for each CTA: as many as run at once, or (splits) so many a request
-        per, slots = _scaled_slots(min(33, max_q * G), int8, dev)
+        per, slots = _scaled_slots(min(17, max_q * G), int8, dev)
         units = B * H * -(-max_q * G // per)
         splits = max(1, min(units * splits, 1 << 13) if splits else min(slots, units * -(-seen // 128)))
         splits = max(splits // H, 1) * H
@@ -2083,6 +2084,17 @@ def _expanded_tiles(q_len: int, kv_len: int, window: int, first: int) -> int:
     return -(-kv_len // 128) - lo + (min(lo, -(-first // 128)) if window else 0)
 
 
+def _rows_pay(q_lens, tiles, heads: int, G: int) -> bool:
+    """Whether portions (head dimension 128) over so many tiles of 128 keys each take less time in the kernel for few rows,
+    16 of a key head at a time, than with keys expanded and two heads of 128 rows at a time.  us of both, 4 key heads: 64
+    requests of 1000 keys, 4 query heads each and 16 rows 79 : 119, 32 rows 140 : 119; 32 of 2000 and 16 rows of 8 heads
+    125 : 183, 32 rows 232 : 184; one of 32000 and 64 rows of 8 heads, whose expanded form leaves most SMs idle, 215 : 421."""
+    rows = 15.0 + 0.007 * heads * sum(-(-n * G // 16) * t for n, t in zip(q_lens, tiles))
+    pieces = sum(-(-n // 128) * t for n, t in zip(q_lens, tiles)) * heads * G / 2
+    wide = 9.0 + 1.65 * max(max(tiles), pieces / _sms()) + sum(tiles) * 128 * heads * 128 * 6 / 6.5e6
+    return rows < wide
+
+
 def block_scaled_prefill(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor,
                          v_scale: torch.Tensor, block_tables: torch.Tensor, cu_q: torch.Tensor, seq_lens: torch.Tensor,
                          scale: float, q_lens: Sequence[int], kv_lens: Sequence[int], out: Optional[torch.Tensor] = None,
@@ -2110,7 +2122,8 @@ def block_scaled_prefill(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
     for lo, hi in zip(runs, runs[1:]):
         if lo == hi:
             continue
-        if few[lo]:
+        tiles = [_expanded_tiles(n, k, window, first) for n, k in zip(q_lens[lo:hi], kv_lens[lo:hi])]
+        if few[lo] or SCALED_ROWS and D == 128 and _rows_pay(q_lens[lo:hi], tiles, H, G):
             max_q, seen = max(q_lens[lo:hi]), max(kv_lens[lo:hi])
             if max_q == 0:
                 continue
@@ -2119,7 +2132,6 @@ def block_scaled_prefill(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
             _scaled_rows(shape, T, Hq, q.dtype, pq, ldq, po, ldo, cu + 4 * lo, lens + 4 * lo, tables + 4 * lo * M, hi - lo, M,
                          max_q, scale, window, first, 0, seen)
             continue
-        tiles = [_expanded_tiles(n, k, window, first) for n, k in zip(q_lens[lo:hi], kv_lens[lo:hi])]
         while lo < hi:
             n, count = 1, tiles[0]
             while lo + n < hi and (count + tiles[n]) * 128 <= SCALED_EXPANDED_KEYS:
