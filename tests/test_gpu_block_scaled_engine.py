@@ -110,3 +110,12 @@ def test_the_connector_refuses():
     llm = LLM("llama-3-8b", device="cuda", kv_cache_dtype="fp8_block", enforce_eager=True, **KW)
     with pytest.raises(ValueError, match="scales"):
         llm.engine.attach_kv_connector(object())
+
+
+def test_models_that_are_refused():
+    """Caches of another layout, and attention with distances among the scores, have no form with block scales."""
+    with pytest.raises(ValueError, match="alike"):
+        LLM("tiny-deepseek", device="cuda", kv_cache_dtype="fp8_block", enforce_eager=True, num_gpu_blocks=64)
+    with pytest.raises(ValueError, match="ALiBi"):
+        LLM("llama-3-8b", device="cuda", kv_cache_dtype="fp8_block", extra={"position_embedding": "ALIBI"},
+            enforce_eager=True, **KW)

@@ -1,6 +1,6 @@
 // Attention of few query rows per request over a key / value cache held in 8 bits with a scale for each block of tokens
 // and head (block_scaled.cuh): single tokens of running requests, drafts that are checked, short portions; bf16 and fp16
-// queries, head dimensions 64, 128 and 256.
+// queries, head dimensions 64 and 256 (128: attention_block_scaled_tc.cuh).
 //
 //   o = sum_j p_j v_j / sum_j p_j,  p_j = exp(scale * q.k_j - m)
 //
@@ -36,7 +36,7 @@ constexpr float kLog2e = 1.4426950408889634f;
 struct Args {
   const void* q;               // [T, Hq * D], row pitch ldq
   void* out;                   // [T, Hq * D], row pitch ldo
-  float *tmp_out, *tmp_lse;    // splits without a cluster: [T, Hq, splits, D], [T, Hq, splits]; D 128: parts of the CTAs
+  float *tmp_out, *tmp_lse;    // splits without a cluster: [T, Hq, splits, D], [T, Hq, splits]; D 128: two parts a CTA
   int4* units;                 // D 128: what the CTA's share starts inside of
   const float *ks, *vs;        // [num_blocks, Hkv]
   const int *cu_q;             // [B + 1], null: one token per request
@@ -192,7 +192,7 @@ __global__ void __launch_bounds__(kGroups * 128 + 32)
   constexpr int kRows = 16 * kGroups, kConsumers = 128 * kGroups;
   constexpr int kCols = HD < 128 ? HD : 128, kBoxes = HD / kCols, kBoxBytes = kChunk * kCols;
   constexpr int kStageBytes = 2 * kTile * HD;
-  constexpr int kStages = HD == 256 ? 3 : HD == 128 ? 5 : 8;
+  constexpr int kStages = HD == 256 ? 3 : 8;
   constexpr int kNT = HD / 8;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem =
@@ -578,7 +578,7 @@ struct Call {
 
 template <typename T, bool kInt8, int HD, int kGroups, bool kCluster>
 int launch_rows(const CUtensorMap& tmK, const CUtensorMap& tmV, const Args& a, cudaStream_t s) {
-  constexpr int kStages = HD == 256 ? 3 : HD == 128 ? 5 : 8;
+  constexpr int kStages = HD == 256 ? 3 : 8;
   constexpr int kMerge = (8 * 16 * kGroups + 4 * 16 * kGroups * HD + (kCluster ? 16 * kGroups * (HD + 1) : 0)) * 4;
   constexpr int kRing = kStages * 2 * kTile * HD;
   // (the merge's numbers lie where the stages were; the barriers behind the stages are not used any more by then)

@@ -8,18 +8,23 @@
 //   O^T = V^T P^T  M = 128 columns of the values (MN-major, as they lie), N = 3 or 4 kR columns, K = 128 tokens
 // e4m3: parts of 4 bits each, every one 16 times the rest of the one before, 12 bits together (probabilities are rounded
 // to fp16 before); int8: digits to the base 128 of a number of 21 bits, of a probability to the base 256 of one of 30,
-// since those of many keys may be small beside the largest; the products' sums are exact.  A lane of the softmax warps owns a token: block scales are
-// factors of its scores and of its probabilities, and there is no conversion of codes at all, which is what bounds a kernel
-// that feeds 16-bit matrix instructions from 8-bit codes (attention_block_scaled.cu, head dimensions 64 and 256: there a
-// chunk of 16 tokens takes a warp 490 instructions, here 80 of them for four query rows).
+// since those of many keys may be small beside the largest; the products' sums are exact.  A lane of the softmax warps owns
+// a token: block scales are factors of its scores and of its probabilities, and there is no conversion of codes at all,
+// which is what bounds a kernel that feeds 16-bit matrix instructions from 8-bit codes (attention_block_scaled.cu, head
+// dimensions 64 and 256).
+//
+// Bound by memory: 256 requests of 1024 to 1279 keys, 8 key heads, 4 query rows each: 114 us and 621 MB, 83 per cent of the
+// measured copy rate, tensor pipe 4.5 per cent, issue slots 35 per cent; 4 requests of 31007 to 120001 keys, 4 key heads, 7
+// query rows: 60 us and 324 MB, 82 per cent.  What the rate does not explain is some 5 us of start (lengths, block table,
+// first tile).
 //
 // A CTA stays on its SM and takes an even share of the tiles of all requests for one key head, one behind the other (as
 // many CTAs as run at the same time, or one per tile where there are fewer; those of a share's key heads are neighbours,
 // since the heads' rows of a token lie side by side and memory is read in pieces of two: 613 against 904 MB where a CTA
-// took the key heads one after the other): the shares depend on the lengths that the
-// step holds, not on a bound that a captured graph was made with, no CTA has more than a tile more than another one, and a
-// request's start (block table, queries) overlaps with the end of the one before.  Where a share begins or ends inside a
-// request's keys, its part of the result goes to memory, and merge_units_kernel puts the parts together in their order.
+// took the key heads one after the other): the shares depend on the lengths that the step holds, not on a bound that a
+// captured graph was made with, no CTA has more than a tile more than another one, and a request's start (block table,
+// queries) overlaps with the end of the one before.  Where a share begins or ends inside a request's keys, its part of the
+// result goes to memory, and merge_units_kernel puts the parts together in their order.
 //
 // Warps: four for every eight rows queries and softmax, lane = token of a tile and at the end column of the output; then one
 // for TMA, block tables and scales and one for tcgen05.mma and tensor memory.  K Q^T of a tile runs while the one before is
@@ -883,7 +888,7 @@ __global__ void __launch_bounds__(Tc<kInt8, kR>::kThreads, Tc<kInt8, kR>::kCtas)
 }
 
 // Parts of a request's rows that several CTAs computed, a warp a row: by the CTA whose number is that of the second of
-// them.
+// them.  Bound by latency (unit, sums, outputs one behind the other): 3 to 6 us behind the kernel in front.
 template <typename T>
 __global__ void __launch_bounds__(128) merge_units_kernel(const Args a, int kR) {
   grid_release_small();
@@ -928,8 +933,7 @@ __global__ void __launch_bounds__(128) merge_units_kernel(const Args a, int kR) 
 // CTAs that run at the same time.
 template <bool kInt8>
 int tc_slots(int rows) {
-  const int ctas = rows == 4 ? Tc<kInt8, 4>::kCtas : rows == 8 ? Tc<kInt8, 8>::kCtas
-                                                                      : Tc<kInt8, 16>::kCtas;
+  const int ctas = rows == 4 ? Tc<kInt8, 4>::kCtas : rows == 8 ? Tc<kInt8, 8>::kCtas : Tc<kInt8, 16>::kCtas;
   return ctas * sm_count();
 }
 

@@ -63,6 +63,8 @@ struct Eight {
   }
 };
 
+// Bound by issue slots (56 per cent) and the chain slot - row - maximum - code: 8192 rows of 8 heads of 128, 50 MB, 14.5 us,
+// 53 per cent of the measured copy rate.
 // A warp takes one head of the keys or the values for every run of rows that starts in its window of `window` rows: a run
 // is the rows of one block, which follow each other in rising order of slots, and lies in no other warp.  The rows of a run
 // stay in registers (the first kHold pieces of a lane; blocks of 32 tokens and more are read again from L1) between their
@@ -237,8 +239,9 @@ struct ExpandArgs {
 constexpr int kTileKeys = 128;
 
 // 16 keys of a tile and their values by a CTA: a thread 8 codes at a time (one store of 16 bytes beside its neighbours'),
-// four of the keys and four of the values under way.  Bound by memory: one byte read and two written, and most of what is written stays in L2 for the attention behind
-// it.
+// four of the keys and four of the values under way.  Bound by memory: one byte read and two written, and most of what is
+// written stays in L2 for the attention behind it (12.3 us for 7048 keys of 8 heads of 128, 43 MB: 53 per cent of
+// the measured copy rate, with the latency of lengths, table entry, code and store one behind the other).
 template <typename T, bool kInt8>
 __global__ void __launch_bounds__(256) expand_kernel(const ExpandArgs a) {
   grid_release_small();
@@ -250,7 +253,7 @@ __global__ void __launch_bounds__(256) expand_kernel(const ExpandArgs a) {
     const int b = b0 + lane;
     int count = 0, lo = 0, firsts = 0, len = 0, hidden = 0;
     if (b < a.B) {
-      len = min(a.seq_lens[b], a.max_blocks * a.block_size);
+      len = min(min(a.seq_lens[b], a.max_blocks * a.block_size), a.table_width * kTileKeys);
       const int q = a.cu_q[b + 1] - a.cu_q[b];
       if (q > 0 && len > 0) {
         if (a.window > 0) {
@@ -394,7 +397,9 @@ __device__ __forceinline__ void copy_bytes(const uint8_t* src, uint8_t* dst, lon
   }
 }
 
-// kWarp: a warp a tensor (blocks of up to 16 KB: 64 forks in 128 tensors 10.0 us with a CTA for each, 5.9 so).
+// Bound by latency (table or pair, then plane, then bytes): 64 forks of 32 layers, 24 MB read and written, 8.8 us in a
+// captured graph, 2.4 times the bytes' time.  kWarp: a warp a tensor (blocks of up to 16 KB; with a CTA for each piece 12.3
+// us).
 template <bool kFork, bool kWarp>
 __global__ void __launch_bounds__(128) copy_kernel(const CopyArgs a) {
   grid_release_small();

@@ -296,9 +296,12 @@ class ModelRunner:
         if mc.sliding_window_first and self.is_cuda and not self._block_scaled(spec):
             raise ValueError("first tokens that stay visible beside a sliding window need "
                              "kv_cache_dtype fp8_block or int8_block")
-        if kvd.endswith("_block") and self.is_cuda and spec["type"] == "gqa" and not self._block_scaled(spec):
-            raise ValueError(f"kv_cache_dtype {mc.kv_cache_dtype!r}: fp8_block or int8_block")
         scaled = self.is_cuda and self._block_scaled(spec)
+        if kvd.endswith("_block") and self.is_cuda and not scaled:
+            raise ValueError(f"kv_cache_dtype {mc.kv_cache_dtype!r}: fp8_block or int8_block, of models whose layers all "
+                             f"cache keys and values alike")
+        if scaled and any(getattr(m, "alibi", None) is not None for m in self.model.modules()):
+            raise ValueError(f"kv_cache_dtype {mc.kv_cache_dtype!r}: not with ALiBi")
         if scaled and (spec["head_dim"] not in (64, 128, 256) or self.block_size % 16):
             raise ValueError(f"kv_cache_dtype {mc.kv_cache_dtype!r}: heads of 64, 128 or 256 and blocks of a multiple of 16 "
                              f"tokens, not {spec['head_dim']} and {self.block_size}")

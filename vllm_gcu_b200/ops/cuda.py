@@ -1934,7 +1934,8 @@ def block_scaled_cache(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, 
     """Keys and values ``[T, H * D]`` (bf16, fp16 or fp32; row-strided views are fine) of a step into a cache in 8 bits:
     codes ``[blocks, block size, H, D]`` (float8_e4m3fn or int8; D 64, 128 or 256, blocks of a multiple of 16 tokens) with
     scales ``[blocks, H]`` fp32.  ``slot_mapping [T]`` int64: block * block size + place, -1 for a row that goes nowhere.
-    The rows of a block follow each other in rising order of places, and no other row of the step goes to it.
+    The rows of a block follow each other in rising order of places, none of them twice, and no other row of the step goes
+    to it.
 
     A scale is a power of two.  A block whose first place is written starts anew, with the least scale (2^-100 .. 2^121)
     that holds the rows' numbers; else the scale stays, or grows where a number does not fit, and the codes in front of the
@@ -2089,8 +2090,12 @@ def _rows_pay(q_lens, tiles, heads: int, G: int) -> bool:
     16 of a key head at a time, than with keys expanded and two heads of 128 rows at a time.  us of both, 4 key heads: 64
     requests of 1000 keys, 4 query heads each and 16 rows 79 : 119, 32 rows 140 : 119; 32 of 2000 and 16 rows of 8 heads
     125 : 183, 32 rows 232 : 184; one of 32000 and 64 rows of 8 heads, whose expanded form leaves most SMs idle, 215 : 421."""
-    rows = 15.0 + 0.007 * heads * sum(-(-n * G // 16) * t for n, t in zip(q_lens, tiles))
-    pieces = sum(-(-n // 128) * t for n, t in zip(q_lens, tiles)) * heads * G / 2
+    rows, pieces = 0, 0
+    for n, t in zip(q_lens, tiles):
+        rows += -(-n * G // 16) * t
+        pieces += -(-n // 128) * t
+    rows = 15.0 + 0.007 * heads * rows
+    pieces *= heads * G / 2
     wide = 9.0 + 1.65 * max(max(tiles), pieces / _sms()) + sum(tiles) * 128 * heads * 128 * 6 / 6.5e6
     return rows < wide
 
@@ -2110,19 +2115,28 @@ def block_scaled_prefill(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
     M = block_tables.shape[1] if block_tables.dim() == 2 else 0
     tables = _indices("block_tables", block_tables, (B, M), dev)
     cu, lens = _indices("cu_q", cu_q, (B + 1,), dev), _indices("seq_lens", seq_lens, (B,), dev)
-    if len(kv_lens) != B or any(not 0 <= n <= k <= M * bs for n, k in zip(q_lens, kv_lens)) or sum(q_lens) > T:
+    G, room, all_tiles, few, total = Hq // H, M * bs, [], [], 0
+    for n, k in zip(q_lens, kv_lens):
+        if not 0 <= n <= k <= room:
+            total = T + 1
+            break
+        total += n
+        few.append(n * G <= SCALED_ROWS or D == 256)
+        all_tiles.append(_expanded_tiles(n, k, window, first))
+    if total > T or len(kv_lens) != B:
         raise ValueError(f"{B} portions of together {sum(q_lens)} tokens for {T} rows: every one takes the last places of "
-                         f"its keys, of which a table holds {M * bs}")
-    G = Hq // H
+                         f"its keys, of which a table holds {room}")
+    if not total:
+        return out
     # requests one behind the other that take the same way; where the ways change often, one for all
-    few = [n * G <= SCALED_ROWS or D == 256 for n in q_lens]
-    runs = [0] + [b for b in range(1, B) if few[b] != few[b - 1]] + [B]
-    if len(runs) > 5:
-        few, runs = [D == 256] * B, [0, B]
+    if few.count(few[0]) == B:
+        runs = [0, B]
+    else:
+        runs = [0] + [b for b in range(1, B) if few[b] != few[b - 1]] + [B]
+        if len(runs) > 5:
+            few, runs = [D == 256] * B, [0, B]
     for lo, hi in zip(runs, runs[1:]):
-        if lo == hi:
-            continue
-        tiles = [_expanded_tiles(n, k, window, first) for n, k in zip(q_lens[lo:hi], kv_lens[lo:hi])]
+        tiles = all_tiles[lo:hi]
         if few[lo] or SCALED_ROWS and D == 128 and _rows_pay(q_lens[lo:hi], tiles, H, G):
             max_q, seen = max(q_lens[lo:hi]), max(kv_lens[lo:hi])
             if max_q == 0:
