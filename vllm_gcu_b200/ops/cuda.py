@@ -1957,13 +1957,19 @@ def block_scaled_cache(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, 
                                 DTYPE_CODE[dtype], 0))
 
 
-def block_scaled_splits(requests: int, heads: int, max_seq_len: int) -> int:
-    """Splits of the keys that ``block_scaled_decode`` takes for so many requests and key heads of 64 or 256."""
-    ctas = requests * heads
+def block_scaled_splits(requests: int, heads: int, max_seq_len: int, width: int = 64) -> int:
+    """Splits of the keys that ``block_scaled_decode`` takes for so many requests and key heads of 64 or 256.  Up to 8 are a
+    cluster; more are merged by a second launch, which pays for long keys: a request of 8 key heads, 16384 keys of 64, 26 us
+    in 8 splits and 16 in 32 (4096 keys: 10 and 11), four such requests 34 and, in 10, 31."""
+    ctas, sms = requests * heads, _sms()
     if ctas <= 0 or max_seq_len <= 256:
         return 1
-    want = -(-2 * _sms() // ctas)
-    return max(1, min(want, max_seq_len // 128, 8 if max_seq_len < 8 * 2048 else 32))
+    # of 256 columns an SM holds one CTA: one more round of them takes longer than fewer splits
+    want = sms // ctas if width == 256 else -(-2 * sms // ctas)
+    most = 32 if max_seq_len >= 6144 else 8
+    if width == 256 and 4 < min(want, most) <= 8 and 8 * ctas > sms * 3 // 4:
+        most = 4                            # (clusters of 8 leave SMs idle)
+    return max(1, min(want, max_seq_len // 128, most))
 
 
 def _scaled_query(q: torch.Tensor, out: Optional[torch.Tensor], shape):
@@ -2035,7 +2041,7 @@ def _scaled_rows(shape, T, Hq, dtype, pq, ldq, po, ldo, cu_q, seq_lens, tables, 
         room = torch.empty(out + lse + 4 * splits, device=torch.device("cuda", dev), dtype=torch.float32).data_ptr()
         lse, units = room + 4 * out, room + 4 * (out + lse)
     else:
-        splits = splits or block_scaled_splits(B, H * -(-max_q * G // 32), seen)
+        splits = splits or block_scaled_splits(B, H * -(-max_q * G // (32 if D == 64 else 16)), seen, D)
         if cu_q:
             splits = min(splits, 8)         # (the rest of the rows are another launch's)
         room = lse = units = 0
