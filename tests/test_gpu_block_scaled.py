@@ -282,6 +282,24 @@ def test_shares_of_all_sizes(codes, G):
         K.check(got, q, cache, [1] * len(lens), 0.09, 0, 0, K.F16)
 
 
+@pytest.mark.parametrize("codes,H,G,D", [(K.FP8, 1, 7, 128), (K.INT8, 1, 20, 128), (K.INT8, 3, 1, 128), (K.FP8, 2, 4, 64),
+                                         (K.INT8, 2, 4, 256), (K.FP8, 9, 2, 256)])
+def test_few_requests_of_many_keys(codes, H, G, D):
+    """Keys of a request that many CTAs share, whose parts many CTAs merge; single tokens, and portions in several blocks of
+    rows."""
+    lens = [9000, 6200, 1]
+    cache = K.Cache(codes, H, D, 16, lens, seed=G).to("cuda")
+    q = torch.randn(3, H * G, D, device="cuda", dtype=K.BF16)
+    got = C.block_scaled_decode(q, *cache.parts(), cache.tables, cache.seq_lens, D ** -0.5)
+    K.check(got, q, cache, [1] * 3, D ** -0.5, 0, 0, K.F16)
+    q_lens = [4, 2, 1]
+    q = torch.randn(7, H * G, D, device="cuda", dtype=K.F16)
+    cu = torch.tensor([0] + q_lens).cumsum(0).int().cuda()
+    got = C.block_scaled_prefill(q, *cache.parts(), cache.tables, cu, cache.seq_lens, D ** -0.5, q_lens, lens, window=7000,
+                                 first=9)
+    K.check(got, q, cache, q_lens, D ** -0.5, 7000, 9, K.F16)
+
+
 def test_the_same_bits_again_and_on_another_stream():
     cache = K.Cache(K.FP8, 2, 128, 16, [5000, 3001, 77]).to("cuda")
     q = torch.randn(3, 8, 128, device="cuda", dtype=K.BF16)

@@ -119,3 +119,13 @@ def test_models_that_are_refused():
     with pytest.raises(ValueError, match="ALiBi"):
         LLM("llama-3-8b", device="cuda", kv_cache_dtype="fp8_block", extra={"position_embedding": "ALIBI"},
             enforce_eager=True, **KW)
+
+
+def test_a_drafter_with_its_own_cache():
+    prompts, sp = _prompts([60, 33], 9), SamplingParams(max_tokens=12, temperature=0.0, ignore_eos=True)
+    llm = LLM("llama-3-8b", device="cuda", kv_cache_dtype="fp8_block", speculative_method="eagle", num_speculative_tokens=1,
+              enforce_eager=True, **KW)
+    got = llm.generate(prompts, sp)
+    assert all(len(o.outputs[0].token_ids) == 12 for o in got)
+    assert all(type(c) is type(llm.engine.runner.kv_caches[0]) for c in llm.engine.runner.drafter_caches)
+    _native.check_status()

@@ -195,8 +195,8 @@ __global__ void __launch_bounds__(kGroups * 128 + 32)
   constexpr int kStages = HD == 256 ? 3 : 8;
   constexpr int kNT = HD / 8;
   extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem =
-      reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  // (an offset, so that the compiler knows the accesses to be of shared memory)
+  uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   uint64_t* full_bar = reinterpret_cast<uint64_t*>(smem + kStages * kStageBytes);
   uint64_t* empty_bar = full_bar + kStages;
   volatile uint32_t* abort_flag = reinterpret_cast<uint32_t*>(empty_bar + kStages);

@@ -279,8 +279,8 @@ __global__ void __launch_bounds__(Tc<kInt8, kR>::kThreads, Tc<kInt8, kR>::kCtas)
   constexpr int kN = S::kN, kNS = S::kNS, kStages = S::kStages, kParts = S::kParts, kWarps = S::kWarps, kRW = S::kRW, kScores = S::kScores;
   constexpr int kSoft = kWarps * 32;
   extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem =
-      reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  // (an offset, so that the compiler knows the accesses to be of shared memory)
+  uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   uint64_t* k_full = reinterpret_cast<uint64_t*>(smem + S::kOffBar);    // [kStages]
   uint64_t* k_empty = k_full + kStages;
   uint64_t* v_full = k_empty + kStages;
