@@ -837,10 +837,12 @@ __global__ void __launch_bounds__(Tc<kInt8, kR>::kThreads, Tc<kInt8, kR>::kCtas)
         }
         if (threadIdx.x == 0) adds[t & 1] = drained ? 0u : 1u;
         drained = false;
-        // (rows of a warp start at a multiple of 8 columns: their places in a group of eight are constants)
-        uint8_t* sp = smem + S::kOffP + (t & 1) * kN * 128 + row0 * 128 + (i_tok & 15);
+        // (rows of a warp start at a multiple of 8 columns: their places in a group of eight are constants; bits 4 .. 6 of an
+        // address are those of c16 alone)
+        const uint32_t sp = smem_u32(smem) + S::kOffP + (t & 1) * kN * 128 + row0 * 128 + (i_tok & 15) + (c16 << 4);
         auto put = [&](int n, uint32_t byte) {
-          sp[(n >> 3) * 1024 + (n & 7) * 128 + ((c16 ^ (n & 7)) << 4)] = static_cast<uint8_t>(byte);
+          asm volatile("st.shared.u8 [%0], %1;" ::"r"((sp ^ ((n & 7) << 4)) + (n >> 3) * 1024 + (n & 7) * 128), "r"(byte)
+                       : "memory");
         };
 #pragma unroll
         for (int r = 0; r < kRW; r += 2) {
