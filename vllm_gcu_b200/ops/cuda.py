@@ -1991,7 +1991,7 @@ def _scaled_query(q: torch.Tensor, out: Optional[torch.Tensor], shape):
         q = q.contiguous()
         ld, pq = width, q.data_ptr()
     if out is None:
-        out = torch.empty(size, dtype=dtype, device=q.device)
+        out = q.new_empty(size)
         return T, Hq, q, pq, ld, out, out.data_ptr(), width
     stride, po = out.stride(), out.data_ptr()
     if out.shape != size or out.dtype is not dtype or out.get_device() != dev or stride[2] != 1 or stride[1] != D and Hq > 1:
@@ -2025,7 +2025,7 @@ def _scaled_slots(rows: int, int8: bool, dev: int) -> tuple[int, int]:
     return got >> 16, got & 0xffff
 
 
-def _scaled_rows(shape, T, Hq, dtype, pq, ldq, po, ldo, cu_q, seq_lens, tables, B, max_blocks, max_q, scale, window, first,
+def _scaled_rows(shape, T, Hq, q, pq, ldq, po, ldo, cu_q, seq_lens, tables, B, max_blocks, max_q, scale, window, first,
                  splits, seen) -> None:
     nb, bs, H, D, row, int8, dev, pk, pv, pks, pvs = shape
     if dev < 0:
@@ -2038,7 +2038,7 @@ def _scaled_rows(shape, T, Hq, dtype, pq, ldq, po, ldo, cu_q, seq_lens, tables, 
         splits = max(1, min(units * splits, 1 << 13) if splits else min(slots, units * -(-seen // 128)))
         splits = max(splits // H, 1) * H
         out, lse = 2 * splits * per * 128, 2 * splits * per
-        room = torch.empty(out + lse + 4 * splits, device=torch.device("cuda", dev), dtype=torch.float32).data_ptr()
+        room = q.new_empty(2 * (out + lse + 4 * splits)).data_ptr()           # (of 32 bits, in elements of 16)
         lse, units = room + 4 * out, room + 4 * (out + lse)
     else:
         splits = splits or block_scaled_splits(B, H * -(-max_q * G // (32 if D == 64 else 16)), seen, D)
@@ -2047,11 +2047,11 @@ def _scaled_rows(shape, T, Hq, dtype, pq, ldq, po, ldo, cu_q, seq_lens, tables, 
         room = lse = units = 0
         if splits > 8:
             out = T * Hq * splits * D
-            room = torch.empty(out + T * Hq * splits, device=torch.device("cuda", dev), dtype=torch.float32).data_ptr()
+            room = q.new_empty(2 * (out + T * Hq * splits)).data_ptr()
             lse = room + 4 * out
     _call_on(dev, "b200_block_scaled_rows",
              _SCALED_ROWS.pack(pq, po, pk, pv, pks, pvs, cu_q, seq_lens, tables, room, lse, units, ldq, ldo, row, scale, T, B,
-                               max_q, Hq, H, D, splits, max_blocks, bs, nb, window, first, int8, DTYPE_CODE[dtype], 0))
+                               max_q, Hq, H, D, splits, max_blocks, bs, nb, window, first, int8, DTYPE_CODE[q.dtype], 0))
 
 
 def block_scaled_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor,
@@ -2079,7 +2079,7 @@ def block_scaled_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.T
         seen = min(seen, window + first)
     if not 0 <= num_splits <= 32:
         raise ValueError(f"{num_splits} splits, up to 32 are built")
-    _scaled_rows(shape, B, Hq, q.dtype, pq, ldq, po, ldo, 0, lens, tables, B, M, 1, scale, window, first, num_splits, seen)
+    _scaled_rows(shape, B, Hq, q, pq, ldq, po, ldo, 0, lens, tables, B, M, 1, scale, window, first, num_splits, seen)
     return out
 
 
@@ -2149,7 +2149,7 @@ def block_scaled_prefill(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
                 continue
             if window:
                 seen = min(seen, window + max_q + first)
-            _scaled_rows(shape, T, Hq, q.dtype, pq, ldq, po, ldo, cu + 4 * lo, lens + 4 * lo, tables + 4 * lo * M, hi - lo, M,
+            _scaled_rows(shape, T, Hq, q, pq, ldq, po, ldo, cu + 4 * lo, lens + 4 * lo, tables + 4 * lo * M, hi - lo, M,
                          max_q, scale, window, first, 0, seen)
             continue
         while lo < hi:
