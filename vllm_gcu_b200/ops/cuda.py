@@ -2094,8 +2094,8 @@ def _expanded_tiles(q_len: int, kv_len: int, window: int, first: int) -> int:
 def _rows_pay(q_lens, tiles, heads: int, G: int) -> bool:
     """Whether portions (head dimension 128) over so many tiles of 128 keys each take less time in the kernel for few rows,
     16 of a key head at a time, than with keys expanded and two heads of 128 rows at a time.  us of both, 4 key heads: 64
-    requests of 1000 keys, 4 query heads each and 16 rows 79 : 119, 32 rows 140 : 119; 32 of 2000 and 16 rows of 8 heads
-    125 : 183, 32 rows 232 : 184; one of 32000 and 64 rows of 8 heads, whose expanded form leaves most SMs idle, 215 : 421."""
+    requests of 1000 keys and 16 tokens of 4 query heads 74 : 118, 32 tokens 131 : 118; 32 of 2000 and 16 tokens of 8 heads
+    118 : 182, 32 tokens 218 : 183; one of 32000 and 64 tokens of 8 heads, whose expanded form leaves most SMs idle, 201 : 422."""
     rows, pieces = 0, 0
     for n, t in zip(q_lens, tiles):
         rows += -(-n * G // 16) * t
