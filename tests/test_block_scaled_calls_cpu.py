@@ -1,0 +1,74 @@
+"""Calls of the operators of a cache in 8 bits with block scales, up to their launches: workspaces, addresses, bounds."""
+import weakref
+
+import pytest
+import torch
+
+import block_scaled_cases as K
+from vllm_gcu_b200.ops import cuda as C
+
+
+class Launches:
+    """Stands in for the launches of ``ops.cuda`` on tensors of the host: their names and arguments, and whether the
+    workspaces that were made for them are still held."""
+
+    def __init__(self, monkeypatch):
+        self.calls, self.made = [], []
+        empty, new_empty = torch.empty, torch.Tensor.new_empty
+
+        def recorded(make):
+            def made(*args, **kw):
+                t = make(*args, **kw)
+                self.made.append(weakref.ref(t))
+                return t
+            return made
+
+        def launch(dev, name, packed):
+            self.calls.append((name, packed))
+            assert all(t() is not None for t in self.made), f"{name}: a workspace was given back before the launch"
+
+        monkeypatch.setattr(C, "_call_on", launch)
+        monkeypatch.setattr(C, "_scaled_slots", lambda rows, int8, dev: (4 if rows <= 4 else 8 if rows <= 8 else 16, 296))
+        monkeypatch.setattr(C, "_sms", lambda: 148)
+        monkeypatch.setattr(torch, "empty", recorded(empty))
+        monkeypatch.setattr(torch.Tensor, "new_empty", recorded(new_empty))
+
+    def packed(self, name, fields):
+        return [fields.unpack(p) for n, p in self.calls if n == name]
+
+
+def _few_rows(cache, q, splits, window=0, first=0):
+    """A launch of the kernel for few rows, as if the tensors lay on a GPU."""
+    shape = list(C._scaled_cache(*cache.parts()))
+    shape[6] = 0
+    B, Hq, q, pq, ld, out, po, ldo = C._scaled_query(q, q.clone(), C._scaled_cache(*cache.parts()))
+    C._scaled_rows(tuple(shape), B, Hq, q, pq, ld, po, ldo, 0, cache.seq_lens.data_ptr(), cache.tables.data_ptr(), B,
+                   cache.tables.shape[1], 1, 0.1, window, first, splits, max(cache.lens))
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_workspaces_are_held_until_the_launches_of_few_rows(D, monkeypatch):
+    cache = K.Cache(K.FP8, 2, D, 16, [900, 40])
+    q = torch.zeros(2, 8, D, dtype=K.BF16)
+    launches = Launches(monkeypatch)
+    _few_rows(cache, q, 12)
+    assert [n for n, _ in launches.calls] == ["b200_block_scaled_rows"] and launches.made
+
+
+def test_workspaces_are_held_between_expansion_and_attention(monkeypatch):
+    q_lens, lens = [130, 200, 90], [130, 700, 333]
+    cache = K.Cache(K.FP8, 2, 128, 16, lens)
+    q = torch.zeros(sum(q_lens), 8, 128, dtype=K.BF16)
+    cu = torch.tensor([0] + q_lens).cumsum(0).int()
+    monkeypatch.setattr(C, "SCALED_ROWS", 0)
+    monkeypatch.setattr(C, "SCALED_EXPANDED_KEYS", 900)
+    out = torch.zeros_like(q)
+    launches = Launches(monkeypatch)
+    launch = C._call_on
+
+    def one_workspace(dev, name, packed):                 # (the one of an earlier group of requests may go)
+        launches.made = launches.made[-1:]
+        launch(dev, name, packed)
+    monkeypatch.setattr(C, "_call_on", one_workspace)
+    C.block_scaled_prefill(q, *cache.parts(), cache.tables, cu, cache.seq_lens, 0.1, q_lens, lens, out=out)
+    assert [n for n, _ in launches.calls] == ["b200_block_scaled_expand", "b200_fmha_expanded"] * 3 and launches.made

@@ -1,0 +1,54 @@
+"""Calls of the operators of a cache in 8 bits with block scales that meet each other or the ends of their ranges."""
+import threading
+
+import pytest
+import torch
+
+import block_scaled_cases as K
+from vllm_gcu_b200.ops import cuda as C
+
+pytestmark = pytest.mark.gpu
+CODES = [K.FP8, K.INT8]
+
+
+@pytest.fixture(autouse=True)
+def _clean_status():
+    from vllm_gcu_b200.ops import _native
+    yield
+    assert _native.take_status()[0] == 0
+
+
+@pytest.mark.parametrize("few", [64, 0])
+@pytest.mark.parametrize("D", [64, 128])
+def test_two_threads_on_one_stream(D, few, monkeypatch):
+    """Portions and single tokens from two threads that launch on the same stream: each gets what it gets alone."""
+    monkeypatch.setattr(C, "SCALED_ROWS", few)
+    jobs, wants, faults = [], [], []
+    for seed in (1, 2):
+        q_lens, lens = [70 + seed, 130, 33], [200, 700 + 9 * seed, 333]
+        cache = K.Cache(K.FP8, 2, D, 16, lens, seed=seed).to("cuda")
+        q = torch.randn(sum(q_lens), 8, D, device="cuda", dtype=K.BF16)
+        cu = torch.tensor([0] + q_lens).cumsum(0).int().cuda()
+        single = torch.randn(3, 8, D, device="cuda", dtype=K.BF16)
+
+        def job(q=q, cache=cache, cu=cu, q_lens=q_lens, lens=lens, single=single):
+            return (C.block_scaled_prefill(q, *cache.parts(), cache.tables, cu, cache.seq_lens, 0.09, q_lens, lens),
+                    C.block_scaled_decode(single, *cache.parts(), cache.tables, cache.seq_lens, 0.09, num_splits=12))
+        jobs.append(job)
+        wants.append(job())
+    torch.cuda.synchronize()
+
+    def work(n):
+        try:
+            got = [jobs[n]() for _ in range(60)]
+            torch.cuda.synchronize()
+            assert all(torch.equal(g, w) for pair in got for g, w in zip(pair, wants[n]))
+        except Exception as e:                            # (an assertion of a thread alone would be lost)
+            faults.append(e)
+
+    threads = [threading.Thread(target=work, args=(n,)) for n in (0, 1)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not faults, faults[0]

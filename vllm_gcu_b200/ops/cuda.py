@@ -2031,6 +2031,8 @@ def _scaled_rows(shape, T, Hq, q, pq, ldq, po, ldo, cu_q, seq_lens, tables, B, m
     if dev < 0:
         raise ValueError("tensors on a GPU are wanted")
     G = Hq // H
+    # (`held` keeps the workspace until its last launch is on the stream: given back earlier, another thread that launches on
+    # this stream could be given it in between)
     if D == 128:
         # an even share of a key head's tiles for each CTA: as many as run at once, or (splits) so many a request
         per, slots = _scaled_slots(min(17, max_q * G), int8, dev)
@@ -2038,7 +2040,8 @@ def _scaled_rows(shape, T, Hq, q, pq, ldq, po, ldo, cu_q, seq_lens, tables, B, m
         splits = max(1, min(units * splits, 1 << 13) if splits else min(slots, units * -(-seen // 128)))
         splits = max(splits // H, 1) * H
         out, lse = 2 * splits * per * 128, 2 * splits * per
-        room = q.new_empty(2 * (out + lse + 4 * splits)).data_ptr()           # (of 32 bits, in elements of 16)
+        held = q.new_empty(2 * (out + lse + 4 * splits))                      # (of 32 bits, in elements of 16)
+        room = held.data_ptr()
         lse, units = room + 4 * out, room + 4 * (out + lse)
     else:
         splits = splits or block_scaled_splits(B, H * -(-max_q * G // (32 if D == 64 else 16)), seen, D)
@@ -2047,7 +2050,8 @@ def _scaled_rows(shape, T, Hq, q, pq, ldq, po, ldo, cu_q, seq_lens, tables, B, m
         room = lse = units = 0
         if splits > 8:
             out = T * Hq * splits * D
-            room = q.new_empty(2 * (out + T * Hq * splits)).data_ptr()
+            held = q.new_empty(2 * (out + T * Hq * splits))
+            room = held.data_ptr()
             lse = room + 4 * out
     _call_on(dev, "b200_block_scaled_rows",
              _SCALED_ROWS.pack(pq, po, pk, pv, pks, pvs, cu_q, seq_lens, tables, room, lse, units, ldq, ldo, row, scale, T, B,
@@ -2160,7 +2164,8 @@ def block_scaled_prefill(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
             if count:
                 width = -(-max(kv_lens[lo:lo + n]) // 128)
                 size = count * 256 * H * D              # bytes of the keys, or values
-                room = torch.empty(2 * size + 4 * n * width, dtype=torch.uint8, device=q.device).data_ptr()
+                held = torch.empty(2 * size + 4 * n * width, dtype=torch.uint8, device=q.device)     # (see _scaled_rows)
+                room = held.data_ptr()
                 at = cu + 4 * lo, lens + 4 * lo
                 _call_on(dev, "b200_block_scaled_expand", _SCALED_EXPAND.pack(
                     *caches, room, room + size, room + 2 * size, *at, tables + 4 * lo * M, row, n, H, D, bs, M, nb, width,
