@@ -72,3 +72,24 @@ def test_workspaces_are_held_between_expansion_and_attention(monkeypatch):
     monkeypatch.setattr(C, "_call_on", one_workspace)
     C.block_scaled_prefill(q, *cache.parts(), cache.tables, cu, cache.seq_lens, 0.1, q_lens, lens, out=out)
     assert [n for n, _ in launches.calls] == ["b200_block_scaled_expand", "b200_fmha_expanded"] * 3 and launches.made
+
+
+@pytest.mark.parametrize("D", [64, 128])
+def test_queries_that_start_anywhere_are_copied(D, monkeypatch):
+    """The kernels read rows 16 bytes at a time: contiguous rows behind an odd number of elements, rows at an odd pitch, one
+    row for all tokens."""
+    lens = [40, 33]
+    cache, width = K.Cache(K.FP8, 2, D, 16, lens), 4 * D
+    shape = C._scaled_cache(*cache.parts())
+    wide = torch.randn(2 * width + 12).to(K.BF16)
+    rows = [wide[o:o + 2 * width].view(2, 4, D) for o in (0, 1, 4, 7)]
+    rows += [torch.as_strided(wide, (2, 4, D), (width + 4, D, 1)), wide[:width].view(1, 4, D).expand(2, 4, D)]
+    rows.append(wide[3:3 + width].view(1, 4, D))
+    for q in rows:
+        T, Hq, held, pq, ld, _, _, _ = C._scaled_query(q, None, shape)
+        assert pq == held.data_ptr() and pq % 16 == 0 and ld % 8 == 0 and ld >= width and torch.equal(held, q)
+    monkeypatch.setattr(C, "SCALED_ROWS", 0)
+    launches = Launches(monkeypatch)
+    C.block_scaled_prefill(rows[1], *cache.parts(), cache.tables, torch.tensor([0, 1, 2], dtype=torch.int32), cache.seq_lens,
+                           0.1, [1, 1], lens)
+    assert all(p[0] % 16 == 0 for p in launches.packed("b200_fmha_expanded", C._EXPANDED_CALL))

@@ -52,3 +52,24 @@ def test_two_threads_on_one_stream(D, few, monkeypatch):
     for t in threads:
         t.join()
     assert not faults, faults[0]
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_queries_that_start_anywhere(D):
+    """Contiguous rows behind one element, rows at an odd pitch, one row for all tokens: as the same numbers at 16 bytes."""
+    lens = [300, 40, 129]
+    cache = K.Cache(K.INT8, 2, D, 16, lens, seed=D).to("cuda")
+    wide = torch.randn(3 * 8 * D + 40, device="cuda").to(K.BF16)
+    rows = [wide[1:1 + 3 * 8 * D].view(3, 8, D), torch.as_strided(wide, (3, 8, D), (8 * D + 12, D, 1)),
+            wide[:8 * D].view(1, 8, D).expand(3, 8, D)]
+    cu = torch.arange(4, dtype=torch.int32, device="cuda")
+    for q in rows:
+        K.check(C.block_scaled_decode(q, *cache.parts(), cache.tables, cache.seq_lens, D ** -0.5), q, cache, [1] * 3,
+                D ** -0.5, 0, 0, K.F16)
+        for few in (64, 0):
+            before, C.SCALED_ROWS = C.SCALED_ROWS, few
+            try:
+                got = C.block_scaled_prefill(q, *cache.parts(), cache.tables, cu, cache.seq_lens, D ** -0.5, [1] * 3, lens)
+            finally:
+                C.SCALED_ROWS = before
+            K.check(got, q, cache, [1] * 3, D ** -0.5, 0, 0, K.F16 if few or D == 256 else K.BF16)

@@ -1987,8 +1987,9 @@ def _scaled_query(q: torch.Tensor, out: Optional[torch.Tensor], shape):
     width, pq, ld = Hq * D, q.data_ptr(), stride[0]
     if T == 1:
         ld = width
-    if pq % 16 or ld % 8:
-        q = q.contiguous()
+    if pq % 16 or ld % 8 or ld < width:
+        # (a copy always: a contiguous part of a larger tensor may start anywhere)
+        q = q.clone(memory_format=torch.contiguous_format)
         ld, pq = width, q.data_ptr()
     if out is None:
         out = q.new_empty(size)
