@@ -93,3 +93,22 @@ def test_queries_that_start_anywhere_are_copied(D, monkeypatch):
     C.block_scaled_prefill(rows[1], *cache.parts(), cache.tables, torch.tensor([0, 1, 2], dtype=torch.int32), cache.seq_lens,
                            0.1, [1, 1], lens)
     assert all(p[0] % 16 == 0 for p in launches.packed("b200_fmha_expanded", C._EXPANDED_CALL))
+
+
+@pytest.mark.parametrize("first", [2 ** 31 - 1, 2 ** 31 - 20, 2 ** 31 - 130, 5000])
+def test_first_tokens_reach_no_further_than_the_tables(first, monkeypatch):
+    """Kernels add up to 127 to the number of first tokens in 32 bits."""
+    lens = [40, 333]
+    cache = K.Cache(K.FP8, 2, 128, 16, lens)
+    room = cache.tables.shape[1] * 16
+    q, cu = torch.zeros(140, 8, 128, dtype=K.BF16), torch.tensor([0, 10, 140], dtype=torch.int32)
+    monkeypatch.setattr(C, "SCALED_ROWS", 0)
+    launches = Launches(monkeypatch)
+    C.block_scaled_prefill(q, *cache.parts(), cache.tables, cu, cache.seq_lens, 0.1, [10, 130], lens, window=40, first=first)
+    for name, fields in (("b200_block_scaled_expand", C._SCALED_EXPAND), ("b200_fmha_expanded", C._EXPANDED_CALL)):
+        got, = launches.packed(name, fields)
+        assert room in got and first not in got
+    monkeypatch.setattr(C, "_scaled_rows", lambda *args: launches.calls.append(("rows", args)))
+    C.block_scaled_decode(q[:2], *cache.parts(), cache.tables, cache.seq_lens, 0.1, window=40, first=first)
+    assert launches.calls[-1][1][-4:-2] == (40, room)
+    assert C._visible(40, 7, room) == (40, 7)

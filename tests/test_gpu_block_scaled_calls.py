@@ -73,3 +73,23 @@ def test_queries_that_start_anywhere(D):
             finally:
                 C.SCALED_ROWS = before
             K.check(got, q, cache, [1] * 3, D ** -0.5, 0, 0, K.F16 if few or D == 256 else K.BF16)
+
+
+@pytest.mark.parametrize("first", [2 ** 31 - 1, 2 ** 31 - 100])
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_all_tokens_as_first_ones(D, first):
+    """A window beside first tokens without end hides nothing."""
+    q_lens, lens = [3, 140, 20], [300, 700, 129]
+    cache = K.Cache(K.FP8, 2, D, 16, lens, seed=D).to("cuda")
+    q = torch.randn(sum(q_lens), 8, D, device="cuda", dtype=K.BF16)
+    cu = torch.tensor([0] + q_lens).cumsum(0).int().cuda()
+    got = C.block_scaled_decode(q[:3], *cache.parts(), cache.tables, cache.seq_lens, D ** -0.5, window=40, first=first)
+    K.check(got, q[:3], cache, [1] * 3, D ** -0.5, 0, 0, K.F16)
+    for few in (64, 0):
+        before, C.SCALED_ROWS = C.SCALED_ROWS, few
+        try:
+            got = C.block_scaled_prefill(q, *cache.parts(), cache.tables, cu, cache.seq_lens, D ** -0.5, q_lens, lens,
+                                         window=40, first=first)
+        finally:
+            C.SCALED_ROWS = before
+        K.check(got, q, cache, q_lens, D ** -0.5, 0, 0, K.BF16)

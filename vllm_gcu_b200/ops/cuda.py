@@ -2012,10 +2012,12 @@ def _scaled_query(q: torch.Tensor, out: Optional[torch.Tensor], shape):
     return T, Hq, q, pq, ld, out, po, ldo
 
 
-def _visible(window: int, first: int) -> tuple[int, int]:
+def _visible(window: int, first: int, room: int) -> tuple[int, int]:
+    """Window and first tokens as the kernels take them: of first tokens no more than a table's ``room``, since what they add
+    to it are sums of 32 bits."""
     if window < 0 or first < 0 or max(window, first) >= 1 << 31:
         raise ValueError(f"a window of {window} tokens and {first} first ones")
-    return int(window), int(first)
+    return int(window), min(int(first), room)
 
 
 @functools.lru_cache(maxsize=None)
@@ -2071,9 +2073,9 @@ def block_scaled_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.T
     shape = _scaled_cache(k_cache, v_cache, k_scale, v_scale)
     bs, dev = shape[1], shape[6]
     B, Hq, q, pq, ldq, out, po, ldo = _scaled_query(q, out, shape)
-    if window or first:
-        window, first = _visible(window, first)
     M = block_tables.shape[1] if block_tables.dim() == 2 else 0
+    if window or first:
+        window, first = _visible(window, first, M * bs)
     tables, lens = _indices("block_tables", block_tables, (B, M), dev), _indices("seq_lens", seq_lens, (B,), dev)
     if B == 0:
         return out
@@ -2122,8 +2124,8 @@ def block_scaled_prefill(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
     shape = nb, bs, H, D, row, int8, dev, *caches = _scaled_cache(k_cache, v_cache, k_scale, v_scale)
     T, Hq, q, pq, ldq, out, po, ldo = _scaled_query(q, out, shape)
     B = len(q_lens)
-    window, first = _visible(window, first)
     M = block_tables.shape[1] if block_tables.dim() == 2 else 0
+    window, first = _visible(window, first, M * bs)
     tables = _indices("block_tables", block_tables, (B, M), dev)
     cu, lens = _indices("cu_q", cu_q, (B + 1,), dev), _indices("seq_lens", seq_lens, (B,), dev)
     G, room, all_tiles, few, total = Hq // H, M * bs, [], [], 0
