@@ -112,3 +112,13 @@ def test_first_tokens_reach_no_further_than_the_tables(first, monkeypatch):
     C.block_scaled_decode(q[:2], *cache.parts(), cache.tables, cache.seq_lens, 0.1, window=40, first=first)
     assert launches.calls[-1][1][-4:-2] == (40, room)
     assert C._visible(40, 7, room) == (40, 7)
+
+
+def test_tables_of_more_tokens_than_32_bits_hold_are_refused():
+    cache = K.Cache(K.FP8, 2, 128, 16, [40])
+    tables = torch.zeros(1, 1, dtype=torch.int32).expand(1, 1 << 27)
+    q, cu = torch.zeros(1, 8, 128, dtype=K.BF16), torch.tensor([0, 1], dtype=torch.int32)
+    with pytest.raises(ValueError, match="2.31 tokens"):
+        C.block_scaled_decode(q, *cache.parts(), tables, cache.seq_lens, 0.1)
+    with pytest.raises(ValueError, match="2.31 tokens"):
+        C.block_scaled_prefill(q, *cache.parts(), tables, cu, cache.seq_lens, 0.1, [1], [40])

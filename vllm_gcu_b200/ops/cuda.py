@@ -2020,6 +2020,14 @@ def _visible(window: int, first: int, room: int) -> tuple[int, int]:
     return int(window), min(int(first), room)
 
 
+def _table_room(block_tables: torch.Tensor, bs: int) -> tuple[int, int]:
+    """Columns of the tables, and the tokens that a row of them holds (a number of 32 bits in the kernels)."""
+    M = block_tables.shape[1] if block_tables.dim() == 2 else 0
+    if M * bs > (1 << 31) - 256:
+        raise ValueError(f"block_tables: {M} columns of {bs} tokens, requests of fewer than 2^31 tokens are wanted")
+    return M, M * bs
+
+
 @functools.lru_cache(maxsize=None)
 def _scaled_slots(rows: int, int8: bool, dev: int) -> tuple[int, int]:
     """Rows of a CTA of the kernel for head dimension 128, and CTAs that run at the same time."""
@@ -2073,15 +2081,15 @@ def block_scaled_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.T
     shape = _scaled_cache(k_cache, v_cache, k_scale, v_scale)
     bs, dev = shape[1], shape[6]
     B, Hq, q, pq, ldq, out, po, ldo = _scaled_query(q, out, shape)
-    M = block_tables.shape[1] if block_tables.dim() == 2 else 0
+    M, room = _table_room(block_tables, bs)
     if window or first:
-        window, first = _visible(window, first, M * bs)
+        window, first = _visible(window, first, room)
     tables, lens = _indices("block_tables", block_tables, (B, M), dev), _indices("seq_lens", seq_lens, (B,), dev)
     if B == 0:
         return out
     if not M:
         return out.zero_()
-    seen = min(max_seq_len or M * bs, M * bs)
+    seen = min(max_seq_len or room, room)
     if window:
         seen = min(seen, window + first)
     if not 0 <= num_splits <= 32:
@@ -2124,11 +2132,11 @@ def block_scaled_prefill(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
     shape = nb, bs, H, D, row, int8, dev, *caches = _scaled_cache(k_cache, v_cache, k_scale, v_scale)
     T, Hq, q, pq, ldq, out, po, ldo = _scaled_query(q, out, shape)
     B = len(q_lens)
-    M = block_tables.shape[1] if block_tables.dim() == 2 else 0
-    window, first = _visible(window, first, M * bs)
+    M, room = _table_room(block_tables, bs)
+    window, first = _visible(window, first, room)
     tables = _indices("block_tables", block_tables, (B, M), dev)
     cu, lens = _indices("cu_q", cu_q, (B + 1,), dev), _indices("seq_lens", seq_lens, (B,), dev)
-    G, room, all_tiles, few, total = Hq // H, M * bs, [], [], 0
+    G, all_tiles, few, total = Hq // H, [], [], 0
     for n, k in zip(q_lens, kv_lens):
         if not 0 <= n <= k <= room:
             total = T + 1
