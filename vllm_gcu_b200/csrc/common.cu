@@ -42,6 +42,17 @@ static EncodeTiledFn get_encode_fn() {
   return fn;
 }
 
+// The driver's answer to an encoding.  It wants a context, which a thread has from its first call of the runtime on that needs
+// one: a thread whose first launch is encoded here, its memory being torch's, may have none yet.
+template <typename F>
+static int in_context(F encode) {
+  CUresult r = encode();
+  int dev = 0;
+  if (r == CUDA_ERROR_INVALID_CONTEXT && cudaGetDevice(&dev) == cudaSuccess && cudaSetDevice(dev) == cudaSuccess)
+    r = encode();
+  return r == CUDA_SUCCESS ? 0 : static_cast<int>(r);
+}
+
 int encode_tmap_2d(CUtensorMap* out, CUtensorMapDataType dt, int elt_bytes, const void* base,
                    uint64_t rows, uint64_t cols, uint64_t ld_bytes, uint32_t box_rows,
                    uint32_t box_cols, CUtensorMapSwizzle swz) {
@@ -52,10 +63,10 @@ int encode_tmap_2d(CUtensorMap* out, CUtensorMapDataType dt, int elt_bytes, cons
   cuuint32_t box[2] = {box_cols, box_rows};
   cuuint32_t estr[2] = {1, 1};
   (void)elt_bytes;
-  CUresult r = fn(out, dt, 2, const_cast<void*>(base), dims, strides, box, estr,
-                  CU_TENSOR_MAP_INTERLEAVE_NONE, swz, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  return r == CUDA_SUCCESS ? 0 : static_cast<int>(r);
+  return in_context([&] {
+    return fn(out, dt, 2, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, swz,
+              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  });
 }
 
 int encode_tmap_3d(CUtensorMap* out, CUtensorMapDataType dt, int elt_bytes, const void* base,
@@ -69,10 +80,10 @@ int encode_tmap_3d(CUtensorMap* out, CUtensorMapDataType dt, int elt_bytes, cons
   cuuint32_t box[3] = {box0, box1, box2};
   cuuint32_t estr[3] = {1, 1, 1};
   (void)elt_bytes;
-  CUresult r = fn(out, dt, 3, const_cast<void*>(base), dims, strides, box, estr,
-                  CU_TENSOR_MAP_INTERLEAVE_NONE, swz, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  return r == CUDA_SUCCESS ? 0 : static_cast<int>(r);
+  return in_context([&] {
+    return fn(out, dt, 3, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, swz,
+              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  });
 }
 
 int sm_count() {
