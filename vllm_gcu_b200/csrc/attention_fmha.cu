@@ -57,6 +57,14 @@ __device__ __forceinline__ float ex2_approx(float x) {
   return y;
 }
 
+// Probabilities, log2 domain: what a score may exceed the running maximum by, and the power of two that they are held with.
+// fp16 ends at 2^-24: 2^11 times a probability of up to 2^4 leaves the sums of keys that lie far below the largest as they
+// are (11 bits down to 2^-25 of it, steps of 2^-35 below), beside a key that takes nearly all of a row.
+template <bool kHalf>
+struct Span {
+  static constexpr float kRaise = kHalf ? 4.0f : 8.0f, kUp = kHalf ? 11.0f : 0.0f;
+};
+
 template <bool kHalf>
 __device__ __forceinline__ uint32_t pack_pair(float lo, float hi) {
   if constexpr (kHalf) {
@@ -127,7 +135,7 @@ __device__ __forceinline__ void find_tile(const Args& a, int tile, int lane, int
 // monotonic, so row maxima are taken over uncapped scores.  MODE 2 (biased): slopes and output columns;
 // row maxima are those of the biased scores, in the log2 domain.
 // kFirst: the first keys of a request (Args::first) stay visible beside the window: their tiles come in front of the
-// window's.  kHalf: fp16 in place of bf16.
+// window's.  kHalf: fp16 in place of bf16 (without sinks and log sums).
 template <int HD, int MODE, bool kFirst = false, bool kHalf = false>
 __global__ void __launch_bounds__(kThreads, 1)
     fmha_prefill_kernel(const __grid_constant__ CUtensorMap tmQ,
@@ -393,11 +401,12 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         mb = m_new == -INFINITY ? 0.0f : l2(m_new);
       } else {
-        if (mt > m_used && (m_used == -INFINITY || (mt - m_used) * sl2 > 8.0f)) {
+        if (mt > m_used && (m_used == -INFINITY || (mt - m_used) * sl2 > Span<kHalf>::kRaise)) {
           m_new = mt;
           alpha = m_used == -INFINITY ? 0.0f : ex2_approx((m_used - m_new) * sl2);
         }
         mb = (m_new == -INFINITY ? 0.0f : m_new) * sl2;
+        if constexpr (kHalf) mb -= Span<kHalf>::kUp;
       }
       // exponential of a score relative to the running maximum
       auto prob = [&](uint32_t raw, int i, float base) {

@@ -553,11 +553,12 @@ __global__ void __launch_bounds__(kPairThreads, 1)
         row_max(3);
         const float mt = fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]);
         float alpha = 1.0f;
-        if (mt > m_used && (m_used == -INFINITY || (mt - m_used) * sl2 > 8.0f)) {
+        if (mt > m_used && (m_used == -INFINITY || (mt - m_used) * sl2 > Span<kHalf>::kRaise)) {
           alpha = m_used == -INFINITY ? 0.0f : ex2_approx((m_used - mt) * sl2);
           m_used = mt;
         }
-        const float mb = (m_used == -INFINITY ? 0.0f : m_used) * sl2;
+        float mb = (m_used == -INFINITY ? 0.0f : m_used) * sl2;
+        if constexpr (kHalf) mb -= Span<kHalf>::kUp;
         if (j > 0 && __any_sync(0xffffffffu, alpha != 1.0f)) {
           // (rare behind the first tiles; the scores stay in registers meanwhile)
 #pragma unroll 1
