@@ -1,4 +1,5 @@
 """Calls of the operators of a cache in 8 bits with block scales that meet each other or the ends of their ranges."""
+import math
 import threading
 
 import pytest
@@ -93,3 +94,33 @@ def test_all_tokens_as_first_ones(D, first):
         finally:
             C.SCALED_ROWS = before
         K.check(got, q, cache, q_lens, D ** -0.5, 0, 0, K.BF16)
+
+
+@pytest.mark.parametrize("codes", CODES)
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("late", [65504.0, -65504.0, math.inf])
+def test_the_largest_numbers_of_fp16_in_expanded_values(codes, D, late, monkeypatch):
+    """A code that stands for more than fp16 holds: rows in front of it keep their bits, rows that see it are finite and off
+    by 2^-11 of its share (65504 in place of 65536) beside what they are allowed anyway; so are those that see an
+    infinity, whose code is the largest."""
+    monkeypatch.setattr(C, "SCALED_ROWS", 0)
+    H, G, n, at = 2, 4, 200, 181
+    gen = torch.Generator().manual_seed(D)
+    cache = K.Cache(codes, H, D, 16, [n], seed=1).to("cuda")
+    q = torch.randn(n, H * G, D, generator=gen).to(K.F16).cuda()
+    cu, slots = torch.tensor([0, n], dtype=torch.int32).cuda(), torch.arange(176, 192).cuda()
+    slots = cache.tables[0, 11].long() * 16 + slots % 16
+    args = (q, *cache.parts(), cache.tables, cu, cache.seq_lens, D ** -0.5, [n], [n])
+    k, v = (torch.randn(16, H * D, generator=gen).to(K.F16).cuda() for _ in range(2))
+    C.block_scaled_cache(k, v, *cache.parts(), slots)
+    want = C.block_scaled_prefill(*args)
+    v[at - 176, ::5] = late
+    C.block_scaled_cache(k, v, *cache.parts(), slots)
+    got = C.block_scaled_prefill(*args)
+    assert torch.isfinite(got).all() and torch.equal(got[:176], want[:176])
+    if math.isinf(late):
+        return
+    out, size, reach, top = K.attention(q, cache, [n], D ** -0.5)
+    may = K.allowed(out, size, reach, top, K.F16, K.F16, n, D) + size * 2.0 ** -11
+    keep = out.abs() < 65000
+    assert ((got.double().cpu() - out).abs()[keep] <= may[keep]).all()

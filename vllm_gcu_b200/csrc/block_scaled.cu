@@ -238,6 +238,8 @@ struct ExpandArgs {
 
 constexpr int kTileKeys = 128;
 
+// (fp16: what lies beyond 65504 is held there, also the largest number of the type, whose code stands for 65536, and
+// what lies below 2^-25 is lost; every code times its scale is a bf16 number.)
 // 16 keys of a tile and their values by a CTA: a thread 8 codes at a time (one store of 16 bytes beside its neighbours'),
 // four of the keys and four of the values under way.  Bound by memory: one byte read and two written, and most of what is
 // written stays in L2 for the attention behind it (12.3 us for 7048 keys of 8 heads of 128, 43 MB: 53 per cent of
@@ -341,6 +343,11 @@ __global__ void __launch_bounds__(256) expand_kernel(const ExpandArgs a) {
           const float2 x = half_pair(lo), y = half_pair(hi);
           f[4 * j] = x.x * scale[kv][u]; f[4 * j + 1] = x.y * scale[kv][u];
           f[4 * j + 2] = y.x * scale[kv][u]; f[4 * j + 3] = y.y * scale[kv][u];
+        }
+        if constexpr (std::is_same<T, __half>::value) {
+          // (an infinity times a probability of 0 would reach the rows that do not see the key)
+#pragma unroll
+          for (int j = 0; j < 8; ++j) f[j] = fminf(fmaxf(f[j], -65504.0f), 65504.0f);
         }
         vec8_store<T>(out[kv] + static_cast<long long>(i) * 8, f);
       }

@@ -2128,7 +2128,8 @@ def block_scaled_prefill(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
     """The same for portions: ``q [T, Hq, D]``, the rows of request b from ``cu_q[b]`` on (``[B + 1]`` int32), its last token
     at position ``seq_lens[b] - 1``.  ``q_lens`` and ``kv_lens`` hold the same numbers on the host.  Rows of no request are
     left as they are.  Requests of few tokens read the codes as they are; for longer ones the keys and values that their
-    tokens can see are expanded to 16 bits, at most ``SCALED_EXPANDED_KEYS`` keys (or one request's) at a time."""
+    tokens can see are expanded to q's type, at most ``SCALED_EXPANDED_KEYS`` keys (or one request's) at a time.  In fp16
+    they are held between -65504 and 65504, and end at 2^-24, as in a cache of that type."""
     shape = nb, bs, H, D, row, int8, dev, *caches = _scaled_cache(k_cache, v_cache, k_scale, v_scale)
     T, Hq, q, pq, ldq, out, po, ldo = _scaled_query(q, out, shape)
     B = len(q_lens)
