@@ -58,6 +58,11 @@ def _check(got, q, cache, q_lens, scale, window, first, rel, step):
     assert torch.isfinite(got).all() and (worst <= 1).all(), worst.tolist()
 
 
+def _step(codes, D):
+    """fp16 of 2^11 times a probability ends at 2^-24: half a step is 2^-36.  int8 digits of multiples of 2^-26."""
+    return 2.0 ** -27 if codes == K.INT8 and D == 128 else 2.0 ** -36
+
+
 EXPANDED = [(K.FP8, 64), (K.INT8, 128), (K.FP8, 128)]
 
 
@@ -73,3 +78,29 @@ def test_expanded_portions(codes, D, window, first, dtype, monkeypatch):
     got = C.block_scaled_prefill(q, *cache.parts(), cache.tables, cu, cache.seq_lens, scale, q_lens, lens, window=window,
                                  first=first)
     _check(got, q, cache, q_lens, scale, window, first, torch.finfo(dtype).eps / 2, 2.0 ** -36 if dtype == K.F16 else 0.0)
+
+
+FEW = [(K.FP8, 64), (K.INT8, 64), (K.FP8, 256), (K.INT8, 256), (K.INT8, 128)]
+
+
+@pytest.mark.parametrize("dtype", [K.F16, K.BF16])
+@pytest.mark.parametrize("window,first", [(0, 0), (300, 3)])
+@pytest.mark.parametrize("codes,D", FEW)
+def test_single_tokens(codes, D, window, first, dtype):
+    lens = [600, 40, 0, 1, 17, 5000]
+    cache, scale = _cache(codes, D, lens), D ** -0.5
+    q = _queries(len(lens), D, scale, dtype)
+    for splits in (0, 1, 3, 12):
+        got = C.block_scaled_decode(q, *cache.parts(), cache.tables, cache.seq_lens, scale, num_splits=splits,
+                                    window=window, first=first)
+        _check(got, q, cache, [1] * len(lens), scale, window, first, torch.finfo(K.F16).eps / 2, _step(codes, D))
+
+
+@pytest.mark.parametrize("codes,D", FEW)
+def test_portions_of_few_tokens(codes, D):
+    q_lens, lens = [4, 1, 3, 10], [600, 40, 3, 2500]
+    cache, scale = _cache(codes, D, lens), D ** -0.5
+    q = _queries(sum(q_lens), D, scale, K.F16)
+    cu = torch.tensor([0] + q_lens).cumsum(0).int().cuda()
+    got = C.block_scaled_prefill(q, *cache.parts(), cache.tables, cu, cache.seq_lens, scale, q_lens, lens)
+    _check(got, q, cache, q_lens, scale, 0, 0, torch.finfo(K.F16).eps / 2, _step(codes, D))

@@ -19,8 +19,9 @@
 // Queries are scaled to a largest number in [1, 2) by a power of two, so that fp16 holds bf16 ones; what falls below its
 // range is 2^-24 of the row's largest.  The scale of a block's keys is a factor of its scores.  That of its values
 // joins the exponent: p'_j = p_j * scale, so that codes are all that the second product sees; the running maximum is that
-// of the exponents with it, and the sum of p takes p' / scale.  fp16 then holds p' to 2^-12 of itself down to 2^-14 of
-// the largest contribution.  The maximum is raised only when it is exceeded by 8 (log2), to which p' reaches 2^8.
+// of the exponents with it, and the sum of p takes p' / scale.  The maximum is raised only when it is exceeded by 4 (log2), to
+// which p' reaches 2^4, and fp16 holds 2^11 p': to 2^-11 of itself down to 2^-25 of the largest contribution and in steps
+// of 2^-35 of it below, so that the many keys behind one that takes nearly all of a row (18 nats are 2^-26) keep their sum.
 #include "block_scaled.cuh"
 
 namespace b200 {
@@ -32,6 +33,8 @@ constexpr unsigned int kKernelId = 77;
 constexpr int kChunk = 16;         // tokens of a TMA box, and of a warp at a time
 constexpr int kTile = 64;          // tokens of a stage
 constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kRaise = 4.0f;     // log2, by which a score may exceed the running maximum
+constexpr float kUp = 11.0f;       // log2 of what a probability is held with
 
 struct Args {
   const void* q;               // [T, Hq * D], row pitch ldq
@@ -328,6 +331,7 @@ __global__ void __launch_bounds__(kGroups * 128 + 32)
 #pragma unroll
     for (int i = 0; i < kNT; ++i) o_acc[i][0] = o_acc[i][1] = o_acc[i][2] = o_acc[i][3] = 0.0f;
     float m_run[2] = {-INFINITY, -INFINITY}, l_run[2] = {0.0f, 0.0f};
+    const float kDown = power_of_two(-static_cast<int>(kUp));
     const uint32_t smem_base = smem_u32(smem);
 
     int stage = 0;
@@ -391,7 +395,7 @@ __global__ void __launch_bounds__(kGroups * 128 + 32)
             }
           }
         }
-        if (__any_sync(0xffffffffu, top[0] > m_run[0] + 8.0f || top[1] > m_run[1] + 8.0f)) {
+        if (__any_sync(0xffffffffu, top[0] > m_run[0] + kRaise || top[1] > m_run[1] + kRaise)) {
 #pragma unroll
           for (int r = 0; r < 2; ++r) {
             top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 1));
@@ -410,7 +414,7 @@ __global__ void __launch_bounds__(kGroups * 128 + 32)
         const float unit = __fdividef(1.0f, vs);
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
-          const float m = m_run[r] == -INFINITY ? 0.0f : m_run[r];
+          const float m = m_run[r] == -INFINITY ? 0.0f : m_run[r] - kUp;
           float sum = 0.0f;
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
@@ -421,7 +425,7 @@ __global__ void __launch_bounds__(kGroups * 128 + 32)
               sum += v;
             }
           }
-          l_run[r] = fmaf(sum, unit, l_run[r]);
+          l_run[r] = fmaf(sum * kDown, unit, l_run[r]);
         }
         uint32_t pf[4];
         pf[0] = pack_half(s[0][0], s[0][1]);
@@ -493,7 +497,8 @@ __global__ void __launch_bounds__(kGroups * 128 + 32)
     for (int nt = 0; nt < kNT; ++nt) {
 #pragma unroll
       for (int e = 0; e < 4; ++e)
-        sm_o[(part * kRows + group * 16 + g + (e >> 1) * 8) * HD + column_of<HD>(nt, 2 * tig + (e & 1))] = o_acc[nt][e];
+        sm_o[(part * kRows + group * 16 + g + (e >> 1) * 8) * HD + column_of<HD>(nt, 2 * tig + (e & 1))] =
+            o_acc[nt][e] * kDown;
     }
     asm volatile("bar.sync 1, %0;" ::"n"(kConsumers) : "memory");
     for (int idx = threadIdx.x; idx < live * HD; idx += kConsumers) {

@@ -42,7 +42,6 @@ constexpr int kTcTile = 128;                 // tokens of a tile
 constexpr int kTcBytes = kTcTile * 128;      // of its keys, or values
 constexpr int kGroup = 4;                    // tiles whose block-table entries and scales a lane each of the TMA warp reads
 constexpr int kGroups = 4;                   // places for their scales
-constexpr float kRaise = 4.0f;               // log2, by which a score may exceed the running maximum
 constexpr int kMostTiles = 512;              // int8: whose sums of whole numbers one accumulator takes, 2^16 * 128 * 128 < 2^31
 
 template <bool kInt8, int kR>
