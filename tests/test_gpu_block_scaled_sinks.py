@@ -80,7 +80,7 @@ def test_expanded_portions(codes, D, window, first, dtype, monkeypatch):
     _check(got, q, cache, q_lens, scale, window, first, torch.finfo(dtype).eps / 2, 2.0 ** -36 if dtype == K.F16 else 0.0)
 
 
-FEW = [(K.FP8, 64), (K.INT8, 64), (K.FP8, 256), (K.INT8, 256), (K.INT8, 128)]
+FEW = [(K.FP8, 64), (K.INT8, 64), (K.FP8, 256), (K.INT8, 256), (K.FP8, 128), (K.INT8, 128)]
 
 
 @pytest.mark.parametrize("dtype", [K.F16, K.BF16])

@@ -5,9 +5,12 @@
 // without loss instead: a query and a probability are sums of 8-bit numbers ("parts") of falling weight, which are as
 // many columns of the small operand.
 //   S^T = K Q^T    M = 128 tokens (K-major rows of 128 bytes), N = 3 kR columns: part x query row
-//   O^T = V^T P^T  M = 128 columns of the values (MN-major, as they lie), N = 3 or 4 kR columns, K = 128 tokens
-// e4m3: parts of 4 bits each, every one 16 times the rest of the one before, 12 bits together (probabilities are rounded
-// to fp16 before); int8: digits to the base 128 of a number of 21 bits, of a probability to the base 256 of one of 30,
+//   O^T = V^T P^T  M = 128 columns of the values (MN-major, as they lie), N = 4 kR columns, K = 128 tokens
+// e4m3: parts of 4 bits each of a query, every one 16 times the rest of the one before, 12 bits together.  Probabilities are
+// floating-point numbers there as well, since many keys may lie far below one that takes nearly all of a row: 2^11 times
+// the probability as fp16, which is the sum of four e5m2 numbers (its upper byte, and 8 times the rest, three times) without
+// rounding, so 11 bits down to 2^-25 of the largest and steps of 2^-35 of it below (parts in e4m3, which has one exponent bit
+// less, would end at 2^-21, four of them at 2^-25; 16 nats are 2^-23).  int8: digits to the base 128 of a number of 21 bits, of a probability to the base 256 of one of 30,
 // since those of many keys may be small beside the largest; the products' sums are exact.  A lane of the softmax warps owns
 // a token: block scales are factors of its scores and of its probabilities, and there is no conversion of codes at all,
 // which is what bounds a kernel that feeds 16-bit matrix instructions from 8-bit codes (attention_block_scaled.cu, head
@@ -46,7 +49,7 @@ constexpr int kMostTiles = 512;              // int8: whose sums of whole number
 
 template <bool kInt8, int kR>
 struct Tc {
-  static constexpr int kParts = kInt8 ? 4 : 3;                 // of a probability
+  static constexpr int kParts = 4;                             // of a probability
   static constexpr int kNS = (3 * kR + 15) / 16 * 16;          // columns of scores
   static constexpr int kN = (kParts * kR + 15) / 16 * 16;      // and of outputs
   static constexpr int kRW = kR < 8 ? kR : 8;                  // rows of a softmax warp
@@ -69,18 +72,16 @@ struct Tc {
   static constexpr int kBytes = kOffMax + 6 * kR * 4 + 1024;
 };
 
-// A pair of fp16 numbers as three pairs of e4m3 parts: x = p0 + p1 / 16 + p2 / 256, each pair in 16 bits.
-__device__ __forceinline__ void parts_e4m3(uint32_t x, uint32_t (&p)[3]) {
+// A pair of fp16 numbers as four pairs of e5m2 parts, each in the upper bytes of the pair's halves: x = p0 + p1 / 8 + p2 / 64 +
+// p3 / 512.  e5m2 is the upper byte of fp16: a part takes the three leading bits of what is left (or what reaches 2^-16).
+// The rest of a number below 2^16 is below 2^13, so that 8 times it is one as well.
+__device__ __forceinline__ void parts_e5m2(uint32_t x, uint32_t (&p)[4]) {
 #pragma unroll
-  for (int i = 0; i < 3; ++i) {
-    uint16_t c;
-    asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;" : "=h"(c) : "r"(x));
-    p[i] = c;
-    if (i < 2) {
-      uint32_t back;
-      asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(back) : "h"(c));
-      const __half2 rest = __hmul2(__hsub2(*reinterpret_cast<__half2*>(&x), *reinterpret_cast<__half2*>(&back)),
-                                   __floats2half2_rn(16.0f, 16.0f));
+  for (int i = 0; i < 4; ++i) {
+    p[i] = x & 0xff00ff00u;
+    if (i < 3) {
+      const __half2 rest = __hmul2(__hsub2(*reinterpret_cast<__half2*>(&x), *reinterpret_cast<__half2*>(&p[i])),
+                                   __floats2half2_rn(8.0f, 8.0f));
       x = *reinterpret_cast<const uint32_t*>(&rest);
     }
   }
@@ -102,9 +103,9 @@ __device__ __forceinline__ void tmem_ld_32x8(uint32_t taddr, uint32_t (&r)[8]) {
 // Numbers of a lane's columns, parts put together: column part * kStride + row -> [row].
 template <bool kInt8, int kRW, int kStride, int kParts, int kBits>
 __device__ __forceinline__ void sum_parts(uint32_t tmem, float (&s)[kRW]) {
-  // weights of the parts: of digits to the base 2^kBits (the last one's is 1), or 16^-p
+  // weights of the parts: of digits to the base 2^kBits (the last one's is 1), or 2^(-kBits p)
   auto weight = [](int p) {
-    return kInt8 ? static_cast<float>(1 << kBits * (kParts - 1 - p)) : 1.0f / static_cast<float>(1 << 4 * p);
+    return kInt8 ? static_cast<float>(1 << kBits * (kParts - 1 - p)) : 1.0f / static_cast<float>(1 << kBits * p);
   };
   const float last = weight(kParts - 1);
   auto number = [](uint32_t u) { return kInt8 ? static_cast<float>(static_cast<int>(u)) : __uint_as_float(u); };
@@ -546,7 +547,7 @@ __global__ void __launch_bounds__(Tc<kInt8, kR>::kThreads, Tc<kInt8, kR>::kCtas)
     if (elect_one()) {
       constexpr uint32_t kA = kInt8 ? 1 : 0, kC = kInt8 ? 2 : 1;          // s8 or e4m3, s32 or f32
       constexpr uint32_t kIdescS = make_idesc(kTcTile, kNS, kA, kA, kC);
-      constexpr uint32_t kIdescO = make_idesc(128, kN, kA, kA, kC) | 1u << 15;      // A is MN-major
+      constexpr uint32_t kIdescO = make_idesc(128, kN, kA, 1, kC) | 1u << 15;       // B s8 or e5m2; A is MN-major
       const uint64_t q_desc = make_desc_k_sw128(smem_u32(smem + S::kOffQ));
       const uint64_t p_desc = make_desc_k_sw128(smem_u32(smem + S::kOffP));
       const uint64_t k_desc = make_desc_k_sw128(smem_u32(smem));
@@ -691,7 +692,7 @@ __global__ void __launch_bounds__(Tc<kInt8, kR>::kThreads, Tc<kInt8, kR>::kCtas)
     clear(kParts * kR, kN, S::kOffP + kN * 128);
 
     // ---------------- softmax: lane = token of the tile ----------------
-    constexpr float kUnit = kInt8 ? 67108864.0f : 16.0f;       // of a probability: 16 of them (nearly) fill the parts
+    constexpr float kUnit = kInt8 ? 67108864.0f : 2048.0f;     // of a probability: 16 of them (nearly) fill the parts
     int t = 0, groups = 0;
     Work k = {};
     float m[kRW], l[kRW], o[kRW];
@@ -700,7 +701,7 @@ __global__ void __launch_bounds__(Tc<kInt8, kR>::kThreads, Tc<kInt8, kR>::kCtas)
     // what P V of earlier tiles left in tensor memory
     auto drain = [&]() {
       float v[kRW];
-      sum_parts<kInt8, kRW, kR, kParts, 8>(lane_addr + kScores * kNS, v);
+      sum_parts<kInt8, kRW, kR, kParts, kInt8 ? 8 : 3>(lane_addr + kScores * kNS, v);
 #pragma unroll
       for (int r = 0; r < kRW; ++r) o[r] = fmaf(v[r], 1.0f / kUnit, o[r]);
     };
@@ -768,7 +769,7 @@ __global__ void __launch_bounds__(Tc<kInt8, kR>::kThreads, Tc<kInt8, kR>::kCtas)
         pass_warp(&s_full[t % kScores], (t / kScores) & 1, a.status, 0x350u, abort_flag);
         tc_fence_after();
         float x[kRW];
-        sum_parts<kInt8, kRW, kR, 3, 7>(lane_addr + t % kScores * kNS, x);
+        sum_parts<kInt8, kRW, kR, 3, kInt8 ? 7 : 4>(lane_addr + t % kScores * kNS, x);
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&s_free[t % kScores]);
@@ -861,12 +862,12 @@ __global__ void __launch_bounds__(Tc<kInt8, kR>::kThreads, Tc<kInt8, kR>::kCtas)
               for (int j = 0; j < kParts; ++j) put(j * kR + r + e, f >> 8 * (kParts - 1 - j));
             }
           } else {
-            uint32_t q[3];
-            parts_e4m3(pack_half(v[0] * kUnit, v[1] * kUnit), q);
+            uint32_t q[4];
+            parts_e5m2(pack_half(v[0] * kUnit, v[1] * kUnit), q);
 #pragma unroll
-            for (int j = 0; j < 3; ++j) {
-              put(j * kR + r, q[j]);
-              put(j * kR + r + 1, q[j] >> 8);
+            for (int j = 0; j < 4; ++j) {
+              put(j * kR + r, q[j] >> 8);
+              put(j * kR + r + 1, q[j] >> 24);
             }
           }
         }
