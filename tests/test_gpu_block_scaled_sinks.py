@@ -59,8 +59,8 @@ def _check(got, q, cache, q_lens, scale, window, first, rel, step):
 
 
 def _step(codes, D):
-    """fp16 of 2^11 times a probability ends at 2^-24: half a step is 2^-36.  int8 digits of multiples of 2^-26."""
-    return 2.0 ** -27 if codes == K.INT8 and D == 128 else 2.0 ** -36
+    """fp16 of 2^11 times a probability ends at 2^-24: half a step is 2^-36.  int8 digits of multiples of 2^-31."""
+    return 2.0 ** -32 if codes == K.INT8 and D == 128 else 2.0 ** -36
 
 
 EXPANDED = [(K.FP8, 64), (K.INT8, 128), (K.FP8, 128)]

@@ -9,12 +9,13 @@
 // e4m3: parts of 4 bits each of a query, every one 16 times the rest of the one before, 12 bits together.  Probabilities are
 // floating-point numbers there as well, since many keys may lie far below one that takes nearly all of a row: 2^11 times
 // the probability as fp16, which is the sum of four e5m2 numbers (its upper byte, and 8 times the rest, three times) without
-// rounding, so 11 bits down to 2^-25 of the largest and steps of 2^-35 of it below (parts in e4m3, which has one exponent bit
-// less, would end at 2^-21, four of them at 2^-25; 16 nats are 2^-23).  int8: digits to the base 128 of a number of 21 bits, of a probability to the base 256 of one of 30,
-// since those of many keys may be small beside the largest; the products' sums are exact.  A lane of the softmax warps owns
-// a token: block scales are factors of its scores and of its probabilities, and there is no conversion of codes at all,
-// which is what bounds a kernel that feeds 16-bit matrix instructions from 8-bit codes (attention_block_scaled.cu, head
-// dimensions 64 and 256).
+// rounding, so 11 bits down to 2^-25 of the largest and steps of 2^-35 of it below (parts in e4m3, which has one exponent
+// bit less, would end at 2^-21, four of them at 2^-25; 16 nats are 2^-23).  int8: a query of 21 bits as digits to the base
+// 128, a probability as a multiple of 2^-31, whose four bytes are unsigned digits to the base 256; the products' sums are
+// exact.  What lies 16 nats below the largest is off by up to 2^-9 of itself there, 18 nats 2^-6: whole numbers have no
+// exponent, and a fifth digit would leave room for two CTAs an SM in place of three.  A lane of the softmax warps owns a token: block scales
+// are factors of its scores and of its probabilities, and there is no conversion of codes at all, which is what bounds a
+// kernel that feeds 16-bit matrix instructions from 8-bit codes (attention_block_scaled.cu, head dimensions 64 and 256).
 //
 // Bound by memory: 256 requests of 1024 to 1279 keys, 8 key heads, 4 query rows each: 109 us and 613 MB, 86 per cent of the
 // measured copy rate, tensor pipe 4.5 per cent, issue slots 33 per cent; 4 requests of 31007 to 120001 keys, 4 key heads, 7
@@ -33,7 +34,8 @@
 // Warps: four for every eight rows queries and softmax, lane = token of a tile and at the end column of the output; then one
 // for TMA, block tables and scales and one for tcgen05.mma and tensor memory.  K Q^T of a tile runs while the one before is
 // at its softmax; keys and values have places of their own, given back when their product is done.
-// The running maximum is raised when a score exceeds it by 4 (log2), which all softmax warps vote on; then the sums in
+// The running maximum is raised when a score exceeds it by 4 (log2; int8, whose numbers end where they start higher, by 1: 32 x
+// 4 tokens of 28 rows 50.5 us, with 4 48.5, single tokens the same), which all softmax warps vote on; then the sums in
 // tensor memory are taken to registers, rescaled, and start anew (rare behind the first tiles, and the only form for sums
 // of whole numbers).
 #pragma once
@@ -45,7 +47,7 @@ constexpr int kTcTile = 128;                 // tokens of a tile
 constexpr int kTcBytes = kTcTile * 128;      // of its keys, or values
 constexpr int kGroup = 4;                    // tiles whose block-table entries and scales a lane each of the TMA warp reads
 constexpr int kGroups = 4;                   // places for their scales
-constexpr int kMostTiles = 512;              // int8: whose sums of whole numbers one accumulator takes, 2^16 * 128 * 128 < 2^31
+constexpr int kMostTiles = 512;              // int8: whose sums of whole numbers one accumulator takes, 2^16 * 128 * 255 < 2^31
 
 template <bool kInt8, int kR>
 struct Tc {
@@ -547,7 +549,7 @@ __global__ void __launch_bounds__(Tc<kInt8, kR>::kThreads, Tc<kInt8, kR>::kCtas)
     if (elect_one()) {
       constexpr uint32_t kA = kInt8 ? 1 : 0, kC = kInt8 ? 2 : 1;          // s8 or e4m3, s32 or f32
       constexpr uint32_t kIdescS = make_idesc(kTcTile, kNS, kA, kA, kC);
-      constexpr uint32_t kIdescO = make_idesc(128, kN, kA, 1, kC) | 1u << 15;       // B s8 or e5m2; A is MN-major
+      constexpr uint32_t kIdescO = make_idesc(128, kN, kA, kInt8 ? 0 : 1, kC) | 1u << 15;    // B u8 or e5m2; A is MN-major
       const uint64_t q_desc = make_desc_k_sw128(smem_u32(smem + S::kOffQ));
       const uint64_t p_desc = make_desc_k_sw128(smem_u32(smem + S::kOffP));
       const uint64_t k_desc = make_desc_k_sw128(smem_u32(smem));
@@ -692,7 +694,8 @@ __global__ void __launch_bounds__(Tc<kInt8, kR>::kThreads, Tc<kInt8, kR>::kCtas)
     clear(kParts * kR, kN, S::kOffP + kN * 128);
 
     // ---------------- softmax: lane = token of the tile ----------------
-    constexpr float kUnit = kInt8 ? 67108864.0f : 2048.0f;     // of a probability: 16 of them (nearly) fill the parts
+    // (2 or 16 of them fill the parts)
+    constexpr float kUnit = kInt8 ? 2147483648.0f : 2048.0f, kMost = kInt8 ? 1.0f : kRaise;
     int t = 0, groups = 0;
     Work k = {};
     float m[kRW], l[kRW], o[kRW];
@@ -802,7 +805,7 @@ __global__ void __launch_bounds__(Tc<kInt8, kR>::kThreads, Tc<kInt8, kR>::kCtas)
           for (int r = 0; r < kRW; ++r)
             if ((unseen >> r & 1u) != 0u && x[r] > -INFINITY) top = INFINITY;
         }
-        if (any_of<kSoft>(top > kRaise || (kInt8 && it % kMostTiles == kMostTiles - 1))) {
+        if (any_of<kSoft>(top > kMost || (kInt8 && it % kMostTiles == kMostTiles - 1))) {
           // new maxima of all rows; the sums in tensor memory belong to the old ones
           float tops[kRW];
 #pragma unroll
@@ -850,14 +853,13 @@ __global__ void __launch_bounds__(Tc<kInt8, kR>::kThreads, Tc<kInt8, kR>::kCtas)
           float v[2];
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            v[e] = ex2(x[r + e]);           // up to 16
+            v[e] = ex2(x[r + e]);           // up to 16 (int8: 2)
             l[r + e] = fmaf(v[e], scale.z, l[r + e]);
           }
           if constexpr (kInt8) {
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-              // digits -128 .. 127: with 128 added to each but the first one they are the number's bytes
-              const uint32_t f = (__float2uint_rn(v[e] * kUnit) + 0x00808080u) ^ 0x00808080u;
+              const uint32_t f = __float2uint_rn(v[e] * kUnit);       // (2 of them: the largest number)
 #pragma unroll
               for (int j = 0; j < kParts; ++j) put(j * kR + r + e, f >> 8 * (kParts - 1 - j));
             }
