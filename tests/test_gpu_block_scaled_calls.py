@@ -124,3 +124,22 @@ def test_the_largest_numbers_of_fp16_in_expanded_values(codes, D, late, monkeypa
     may = K.allowed(out, size, reach, top, K.F16, K.F16, n, D) + size * 2.0 ** -11
     keep = out.abs() < 65000
     assert ((got.double().cpu() - out).abs()[keep] <= may[keep]).all()
+
+
+@pytest.mark.parametrize("codes", CODES)
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("log2", [30, 60])
+def test_zeros_beside_the_largest_values(codes, D, log2):
+    """Blocks of zeros have the least scale: their keys count beside values of 2^30 or 2^60 times a code."""
+    lens = [200, 64, 33]
+    cache = K.Cache(codes, 2, D, 16, lens, seed=D, spread=0.0)
+    cache.scales[1] = 2.0 ** log2
+    for r, n in enumerate(lens):
+        for b in range(0, -(-n // 16), 2):
+            cache.scales[1, cache.tables[r, b].long()] = 2.0 ** -100
+            cache.codes[1, cache.tables[r, b].long()] = 0
+    cache.to("cuda")
+    q = torch.randn(3, 8, D, device="cuda", dtype=K.BF16)
+    for splits in (0, 1, 5, 12):
+        got = C.block_scaled_decode(q, *cache.parts(), cache.tables, cache.seq_lens, D ** -0.5, num_splits=splits)
+        K.check(got, q, cache, [1] * 3, D ** -0.5, 0, 0, K.F16)

@@ -35,6 +35,9 @@ constexpr int kTile = 64;          // tokens of a stage
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kRaise = 4.0f;     // log2, by which a score may exceed the running maximum
 constexpr float kUp = 11.0f;       // log2 of what a probability is held with
+// Scales of values (log2) below which a key's p' may vanish beside those of blocks of larger values while its p counts in the
+// sum (a block of zeros has the least scale of all): there the sum takes p by itself.
+constexpr float kSmallScale = -40.0f;
 
 struct Args {
   const void* q;               // [T, Hq * D], row pitch ldq
@@ -401,9 +404,10 @@ __global__ void __launch_bounds__(kGroups * 128 + 32)
             top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 1));
             top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 2));
             const float m_new = fmaxf(m_run[r], top[r]);
-            const float corr = m_run[r] == -INFINITY ? 0.0f : ex2(m_run[r] - m_new);
+            // (the sum, which may be as large as the inverse of a small scale, in two steps)
+            const float root = m_run[r] == -INFINITY ? 0.0f : ex2(0.5f * (m_run[r] - m_new)), corr = root * root;
             m_run[r] = m_new;
-            l_run[r] *= corr;
+            l_run[r] = l_run[r] * root * root;
 #pragma unroll
             for (int nt = 0; nt < kNT; ++nt) {
               o_acc[nt][2 * r] *= corr;
@@ -412,6 +416,14 @@ __global__ void __launch_bounds__(kGroups * 128 + 32)
           }
         }
         const float unit = __fdividef(1.0f, vs);
+        const bool small = l2vs < kSmallScale;       // (the same for the warp)
+        if (small) {
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            const float m = m_run[r] == -INFINITY ? 0.0f : m_run[r] + l2vs;
+            l_run[r] += (ex2(s[0][2 * r] - m) + ex2(s[0][2 * r + 1] - m)) + (ex2(s[1][2 * r] - m) + ex2(s[1][2 * r + 1] - m));
+          }
+        }
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
           const float m = m_run[r] == -INFINITY ? 0.0f : m_run[r] - kUp;
@@ -425,7 +437,7 @@ __global__ void __launch_bounds__(kGroups * 128 + 32)
               sum += v;
             }
           }
-          l_run[r] = fmaf(sum * kDown, unit, l_run[r]);
+          if (!small) l_run[r] = fmaf(sum * kDown, unit, l_run[r]);
         }
         uint32_t pf[4];
         pf[0] = pack_half(s[0][0], s[0][1]);
@@ -511,10 +523,10 @@ __global__ void __launch_bounds__(kGroups * 128 + 32)
       for (int w = 0; w < 4; ++w) {
         const float mw = sm_m[w * kRows + r];
         // (a warp without keys has no sum; one whose scores are all NaN has no maximum)
-        const float f = mw == -INFINITY ? (sm_l[w * kRows + r] == 0.0f ? 0.0f : 1.0f) : exp2f(mw - M);
-        if (f == 0.0f) continue;
-        L = fmaf(sm_l[w * kRows + r], f, L);
-        o = fmaf(sm_o[(w * kRows + r) * HD + d], f, o);
+        const float root = mw == -INFINITY ? (sm_l[w * kRows + r] == 0.0f ? 0.0f : 1.0f) : exp2f(0.5f * (mw - M));
+        if (root == 0.0f) continue;
+        L = fmaf(sm_l[w * kRows + r] * root, root, L);
+        o = fmaf(sm_o[(w * kRows + r) * HD + d], root * root, o);
       }
       const float val = L == 0.0f ? 0.0f : o / L;
       const float lse = L == 0.0f ? -INFINITY : M + log2f(L);

@@ -66,7 +66,8 @@ struct Tc {
   static_assert(kAlloc * kCtas <= 512, "tensor memory of an SM");
   static constexpr int kOffQ = 2 * kStages * kTcBytes;         // (keys, then values in front)
   static constexpr int kOffP = kOffQ + kNS * 128;
-  static constexpr int kOffScale = kOffP + 2 * kN * 128;       // [kGroups][32] scales of keys, log2 and inverse of values', flag
+  // [kGroups][32] scales of keys, log2 and inverse of values' (below 0: a small one), flag
+  static constexpr int kOffScale = kOffP + 2 * kN * 128;
   static constexpr int kOffBar = kOffScale + kGroups * 32 * 16;
   static constexpr int kOffWork = kOffBar + 384;               // [2]
   static constexpr int kOffRow = kOffWork + 128;               // (16-byte places) factor and position of every row; [2] token and head
@@ -457,7 +458,7 @@ __global__ void __launch_bounds__(Tc<kInt8, kR>::kThreads, Tc<kInt8, kR>::kCtas)
       };
       auto row_of = [&](int g, int block) { return block * a.block_size + first_token(chunk_of(g)) % a.block_size; };
       auto scales_of = [&](int g, int block) {
-        float4 s = make_float4(0.0f, power_of_two(kLowExponent), 0.0f, 0.0f);
+        float4 s = make_float4(0.0f, 1.0f, 0.0f, 0.0f);
         if (chunk_of(g) >= k.c1) return s;
         if (block >= 0 && block < a.num_blocks) {
           const long long i = static_cast<long long>(block) * a.Hkv + kvh;
@@ -474,6 +475,7 @@ __global__ void __launch_bounds__(Tc<kInt8, kR>::kThreads, Tc<kInt8, kR>::kCtas)
         const float vs = fmaxf(s.y, power_of_two(kLowExponent));
         s.y = __log2f(vs);
         s.z = __fdividef(1.0f, vs);
+        if (s.y < kSmallScale) s.z = -s.z;
         // whether all rows see all of the chunk
         s.w = c < k.c1 && tok + kChunk - 1 <= p.lo_pos &&
                       (a.window <= 0 || tok > p.hi_pos - a.window || tok + kChunk <= a.first) ? 1.0f : 0.0f;
@@ -826,19 +828,26 @@ __global__ void __launch_bounds__(Tc<kInt8, kR>::kThreads, Tc<kInt8, kR>::kCtas)
           const bool seen = (unseen >> lane % kRW & 1u) == 0u;
           const bool moves = seen ? up > 0.0f : up > -INFINITY;
           if (!moves) up = 0.0f;
-          const float corr = moves ? (seen ? ex2(-up) : 0.0f) : 1.0f;
+          // (the sum, which may be as large as the inverse of a small scale, in two steps)
+          const float root = moves ? (seen ? ex2(-0.5f * up) : 0.0f) : 1.0f;
           unseen &= ~__ballot_sync(0xffffffffu, moves && lane < kRW);
 #pragma unroll
           for (int r = 0; r < kRW; ++r) {
-            const float d = __shfl_sync(0xffffffffu, up, r), c = __shfl_sync(0xffffffffu, corr, r);
+            const float d = __shfl_sync(0xffffffffu, up, r), c = __shfl_sync(0xffffffffu, root, r);
             m[r] += d;
-            l[r] *= c;
-            o[r] *= c;
+            l[r] = l[r] * c * c;
+            o[r] *= c * c;
             x[r] -= d;
           }
           sync_softmax<kSoft>();            // (warp_top is free again)
           drained = true;
         }
+        if (__any_sync(0xffffffffu, scale.z < 0.0f)) {
+          const float up = scale.z < 0.0f ? __log2f(-scale.z) : -INFINITY;
+#pragma unroll
+          for (int r = 0; r < kRW; ++r) l[r] += ex2(x[r] + up);
+        }
+        const float unit = fmaxf(scale.z, 0.0f);            // of a probability in the sum
         if (threadIdx.x == 0) adds[t & 1] = drained ? 0u : 1u;
         drained = false;
         // (rows of a warp start at a multiple of 8 columns: their places in a group of eight are constants; bits 4 .. 6 of an
@@ -854,7 +863,7 @@ __global__ void __launch_bounds__(Tc<kInt8, kR>::kThreads, Tc<kInt8, kR>::kCtas)
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
             v[e] = ex2(x[r + e]);           // up to 16 (int8: 2)
-            l[r + e] = fmaf(v[e], scale.z, l[r + e]);
+            l[r + e] = fmaf(v[e], unit, l[r + e]);
           }
           if constexpr (kInt8) {
 #pragma unroll
