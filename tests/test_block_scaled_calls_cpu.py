@@ -122,3 +122,16 @@ def test_tables_of_more_tokens_than_32_bits_hold_are_refused():
         C.block_scaled_decode(q, *cache.parts(), tables, cache.seq_lens, 0.1)
     with pytest.raises(ValueError, match="2.31 tokens"):
         C.block_scaled_prefill(q, *cache.parts(), tables, cu, cache.seq_lens, 0.1, [1], [40])
+
+
+@pytest.mark.parametrize("model,kw,match", [
+    ("tiny-fizunex", dict(sliding_window=8, sliding_window_first=4), "alike"),
+    ("tiny-deepseek", dict(sliding_window=8, sliding_window_first=4), "alike"),
+    ("llama-3-8b", dict(num_hidden_layers=1, hidden_size=64, intermediate_size=64, num_attention_heads=1, head_dim=64,
+                        num_key_value_heads=1, vocab_size=64, sliding_window=8, sliding_window_first=-1), "first tokens"),
+])
+def test_first_tokens_of_models_without_them(model, kw, match):
+    """Models whose attention takes no first tokens refuse them in place of leaving them out."""
+    from vllm_gcu_b200 import LLM
+    with pytest.raises(ValueError, match=match):
+        LLM(model, device="cpu", dtype="float32", num_gpu_blocks=16, max_model_len=64, max_num_seqs=2, **kw)

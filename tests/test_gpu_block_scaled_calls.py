@@ -143,3 +143,20 @@ def test_zeros_beside_the_largest_values(codes, D, log2):
     for splits in (0, 1, 5, 12):
         got = C.block_scaled_decode(q, *cache.parts(), cache.tables, cache.seq_lens, D ** -0.5, num_splits=splits)
         K.check(got, q, cache, [1] * 3, D ** -0.5, 0, 0, K.F16)
+
+
+def test_types_and_drafters_that_are_refused():
+    """Before the first step: activations in fp32, and a drafter whose heads have another size."""
+    from vllm_gcu_b200 import LLM
+    kw = dict(num_hidden_layers=1, max_num_seqs=2, max_num_batched_tokens=64, max_model_len=64, num_gpu_blocks=16,
+              device="cuda", enforce_eager=True, kv_cache_dtype="fp8_block")
+    with pytest.raises(ValueError, match="bf16 or fp16"):
+        LLM("llama-3-8b", dtype="float32", **kw)
+    llm = LLM("llama-3-8b", **kw)
+
+    class Drafter:
+        def kv_cache_spec(self):
+            return {"type": "gqa", "layers": 1, "kv_heads": 2, "head_dim": 96}
+    llm.engine.runner.drafter = Drafter()
+    with pytest.raises(ValueError, match="not 96"):
+        llm.engine.runner.init_kv_cache(16)

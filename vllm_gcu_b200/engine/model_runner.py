@@ -293,9 +293,14 @@ class ModelRunner:
                 dt = torch.float8_e4m3fn
             elif kvd.startswith("int8"):
                 dt = torch.int8
+        if mc.sliding_window_first < 0:
+            raise ValueError(f"{mc.sliding_window_first} first tokens beside a sliding window")
         if mc.sliding_window_first and self.is_cuda and not self._block_scaled(spec):
             raise ValueError("first tokens that stay visible beside a sliding window need "
                              "kv_cache_dtype fp8_block or int8_block")
+        if mc.sliding_window_first and (spec["type"] != "gqa" or "layer_shapes" in spec):
+            raise ValueError(f"{mc.architecture}: first tokens stay visible beside a sliding window in models whose layers "
+                             f"all cache keys and values alike")
         scaled = self.is_cuda and self._block_scaled(spec)
         if kvd.endswith("_block") and self.is_cuda and not scaled:
             raise ValueError(f"kv_cache_dtype {mc.kv_cache_dtype!r}: fp8_block or int8_block, of models whose layers all "
@@ -306,7 +311,12 @@ class ModelRunner:
             raise ValueError(f"kv_cache_dtype {mc.kv_cache_dtype!r}: heads of 64, 128 or 256 and blocks of a multiple of 16 "
                              f"tokens, not {spec['head_dim']} and {self.block_size}")
 
+        if scaled and mc.dtype not in (torch.bfloat16, torch.float16):
+            raise ValueError(f"kv_cache_dtype {mc.kv_cache_dtype!r}: models in bf16 or fp16, not {mc.dtype}")
+
         def kv(blocks: int, heads: int, dim: int):
+            if scaled and dim not in (64, 128, 256):
+                raise ValueError(f"kv_cache_dtype {mc.kv_cache_dtype!r}: heads of 64, 128 or 256, not {dim}")
             if scaled:
                 return BlockScaledCache.zeros(blocks, self.block_size, heads, dim, dt, self.device)
             return torch.zeros(2, blocks, self.block_size, heads, dim, dtype=dt, device=self.device)
