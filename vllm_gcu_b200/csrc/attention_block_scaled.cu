@@ -35,6 +35,7 @@ constexpr int kTile = 64;          // tokens of a stage
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kRaise = 4.0f;     // log2, by which a score may exceed the running maximum
 constexpr float kUp = 11.0f;       // log2 of what a probability is held with
+constexpr float kDown = 1.0f / 2048.0f;
 // Scales of values (log2) below which a key's p' may vanish beside those of blocks of larger values while its p counts in the
 // sum (a block of zeros has the least scale of all): there the sum takes p by itself.
 constexpr float kSmallScale = -40.0f;
@@ -334,7 +335,6 @@ __global__ void __launch_bounds__(kGroups * 128 + 32)
 #pragma unroll
     for (int i = 0; i < kNT; ++i) o_acc[i][0] = o_acc[i][1] = o_acc[i][2] = o_acc[i][3] = 0.0f;
     float m_run[2] = {-INFINITY, -INFINITY}, l_run[2] = {0.0f, 0.0f};
-    const float kDown = power_of_two(-static_cast<int>(kUp));
     const uint32_t smem_base = smem_u32(smem);
 
     int stage = 0;

@@ -17,10 +17,10 @@
 // are factors of its scores and of its probabilities, and there is no conversion of codes at all, which is what bounds a
 // kernel that feeds 16-bit matrix instructions from 8-bit codes (attention_block_scaled.cu, head dimensions 64 and 256).
 //
-// Bound by memory: 256 requests of 1024 to 1279 keys, 8 key heads, 4 query rows each: 109 us and 613 MB, 86 per cent of the
-// measured copy rate, tensor pipe 4.5 per cent, issue slots 33 per cent; 4 requests of 31007 to 120001 keys, 4 key heads, 7
-// query rows: 62 us and 324 MB, 80 per cent.  What the rate does not explain is some 5 us of start (lengths, block table,
-// first tile).  16 rows a CTA: by the softmax, 32 x 4 tokens of 7 query heads behind 1500 to 3391 keys 44 us, issue slots 52
+// Bound by memory: 256 requests of 1024 to 1279 keys, 8 key heads, 4 query rows each: 110 us and 613 MB, 85 per cent of the
+// measured copy rate, tensor pipe 4.6 per cent, issue slots 35 per cent; 4 requests of 31007 to 120001 keys, 4 key heads, 7
+// query rows: 63 us and 324 MB, 78 per cent.  What the rate does not explain is some 5 us of start (lengths, block table,
+// first tile).  16 rows a CTA: by the softmax, 32 x 4 tokens of 7 query heads behind 1500 to 3391 keys 46 us, issue slots 53
 // per cent, their warps most often waiting for scores from tensor memory.
 //
 // A CTA stays on its SM and takes an even share of the tiles of all requests for one key head, one behind the other (as
@@ -904,7 +904,7 @@ __global__ void __launch_bounds__(Tc<kInt8, kR>::kThreads, Tc<kInt8, kR>::kCtas)
 // Parts of a request's rows that several CTAs computed: by the CTAs whose numbers are those of all parts but the first, a
 // row at a time for each warp, or, of many parts, for each CTA, whose warps take every fourth part.  Bound by latency (unit,
 // sums, outputs one behind the other): with all rows merged by the second part's CTA one request of 32000 keys, a key head and 8
-// query rows, 250 parts, took 91 us in all, now 23; 256 requests of two or three parts each 128 and 121 (the merge itself 6 us with a cold L2).
+// query rows, 250 parts, took 91 us in all, now 24; 256 requests of two or three parts each 128 and 121 (the merge itself 6 us with a cold L2).
 constexpr int kFewParts = 8;                 // that a warp takes by itself
 template <typename T>
 __global__ void __launch_bounds__(128) merge_units_kernel(const Args a, int kR) {

@@ -63,8 +63,8 @@ struct Eight {
   }
 };
 
-// Bound by issue slots (56 per cent) and the chain slot - row - maximum - code: 8192 rows of 8 heads of 128, 50 MB, 14.5 us,
-// 53 per cent of the measured copy rate.
+// Bound by the chain slot - scale - row - maximum - code: 8192 rows of 8 heads of 128, 50 MB, 14.4 us, 53 per cent of the
+// measured copy rate and 56 per cent of the issue slots.
 // A warp takes one head of the keys or the values for every run of rows that starts in its window of `window` rows: a run
 // is the rows of one block, which follow each other in rising order of slots, and lies in no other warp.  The rows of a run
 // stay in registers (the first kHold pieces of a lane; blocks of 32 tokens and more are read again from L1) between their

@@ -1939,7 +1939,9 @@ def block_scaled_cache(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, 
 
     A scale is a power of two.  A block whose first place is written starts anew, with the least scale (2^-100 .. 2^121)
     that holds the rows' numbers; else the scale stays, or grows where a number does not fit, and the codes in front of the
-    new rows are rounded to it.  Infinities become the largest code and NaN the code 0; neither counts for the scale."""
+    new rows are rounded to it.  Infinities become the largest code and NaN the code 0; neither counts for the scale.  A
+    scale that grew stays until the block starts anew, also when the row that it grew for is written over, as that of a
+    rejected draft."""
     nb, bs, H, D, row, int8, dev, pkc, pvc, pks, pvs = _scaled_cache(k_cache, v_cache, k_scale, v_scale)
     dtype = k.dtype
     if dtype not in DTYPE_CODE or k.dim() != 2:
@@ -1959,8 +1961,8 @@ def block_scaled_cache(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, 
 
 def block_scaled_splits(requests: int, heads: int, max_seq_len: int, width: int = 64) -> int:
     """Splits of the keys that ``block_scaled_decode`` takes for so many requests and key heads of 64 or 256.  Up to 8 are a
-    cluster; more are merged by a second launch, which pays for long keys: a request of 8 key heads, 16384 keys of 64, 26 us
-    in 8 splits and 16 in 32 (4096 keys: 10 and 11), four such requests 34 and, in 10, 31."""
+    cluster; more are merged by a second launch, which pays for long keys: a request of 8 key heads, 16384 keys of 64, 27 us
+    in 8 splits and 17 in 32 (4096 keys: 12 in both), four such requests 34 and, in 10, 32."""
     ctas, sms = requests * heads, _sms()
     if ctas <= 0 or max_seq_len <= 256:
         return 1
@@ -2109,8 +2111,8 @@ def _expanded_tiles(q_len: int, kv_len: int, window: int, first: int) -> int:
 def _rows_pay(q_lens, tiles, heads: int, G: int) -> bool:
     """Whether portions (head dimension 128) over so many tiles of 128 keys each take less time in the kernel for few rows,
     16 of a key head at a time, than with keys expanded and two heads of 128 rows at a time.  us of both, 4 key heads: 64
-    requests of 1000 keys and 16 tokens of 4 query heads 74 : 118, 32 tokens 131 : 118; 32 of 2000 and 16 tokens of 8 heads
-    118 : 182, 32 tokens 218 : 183; one of 32000 and 64 tokens of 8 heads, whose expanded form leaves most SMs idle, 201 : 422."""
+    requests of 1000 keys and 16 tokens of 4 query heads 73 : 115, 32 tokens 129 : 116; 32 of 2000 and 16 tokens of 8 heads
+    118 : 176, 32 tokens 217 : 176; one of 32000 and 64 tokens of 8 heads, whose expanded form leaves most SMs idle, 205 : 422."""
     rows, pieces = 0, 0
     for n, t in zip(q_lens, tiles):
         rows += -(-n * G // 16) * t
