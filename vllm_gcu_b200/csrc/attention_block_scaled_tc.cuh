@@ -13,9 +13,10 @@
 // bit less, would end at 2^-21, four of them at 2^-25; 16 nats are 2^-23).  int8: a query of 21 bits as digits to the base
 // 128, a probability as a multiple of 2^-31, whose four bytes are unsigned digits to the base 256; the products' sums are
 // exact.  What lies 16 nats below the largest is off by up to 2^-9 of itself there, 18 nats 2^-6: whole numbers have no
-// exponent, and a fifth digit would leave room for two CTAs an SM in place of three.  A lane of the softmax warps owns a token: block scales
-// are factors of its scores and of its probabilities, and there is no conversion of codes at all, which is what bounds a
-// kernel that feeds 16-bit matrix instructions from 8-bit codes (attention_block_scaled.cu, head dimensions 64 and 256).
+// exponent, and a fifth digit would leave room for two CTAs an SM in place of three.  A lane of the softmax warps owns a
+// token: block scales are factors of its scores and of its probabilities, and there is no conversion of codes at all, which
+// is what bounds a kernel that feeds 16-bit matrix instructions from 8-bit codes (attention_block_scaled.cu, head dimensions
+// 64 and 256).
 //
 // Bound by memory: 256 requests of 1024 to 1279 keys, 8 key heads, 4 query rows each: 110 us and 613 MB, 85 per cent of the
 // measured copy rate, tensor pipe 4.6 per cent, issue slots 35 per cent; 4 requests of 31007 to 120001 keys, 4 key heads, 7
